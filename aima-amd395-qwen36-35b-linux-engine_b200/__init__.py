@@ -7,13 +7,17 @@ parent on ``sys.path`` and import it through ``importlib.import_module``.
 """
 from .provider import (  # noqa: F401
     AimaMoeError,
+    KvBatch,
+    KvCache,
     MoeLibrary,
     LmHead,
     MoeProvider,
     StripedImage,
     library_path,
     load_library,
+    verify_drafts,
 )
 from . import synth  # noqa: F401
 
-__all__ = ["AimaMoeError", "LmHead", "MoeLibrary", "MoeProvider", "StripedImage", "library_path", "load_library", "synth"]
+__all__ = ["AimaMoeError", "KvBatch", "KvCache", "LmHead", "MoeLibrary", "MoeProvider", "StripedImage", "library_path", "load_library", "synth",
+           "verify_drafts"]

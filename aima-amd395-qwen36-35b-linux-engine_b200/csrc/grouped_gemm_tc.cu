@@ -28,6 +28,7 @@
 // Every mbarrier wait is bounded; on expiry the block sets the status word,
 // stops issuing, waits for its copies in flight, frees tensor memory and returns.
 #include "grouped_gemm.cuh"
+#include "tcgen05.cuh"
 
 #include <cuda.h>
 #include <mutex>
@@ -74,13 +75,6 @@ struct TcProblem {
 };
 
 // ---- PTX wrappers ---------------------------------------------------------
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y,
-                                            uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3}], [%4];"
-      :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
 // The producer and MMA loops below are run by their WHOLE warp and only the issuing instructions are guarded by
 // elect_one().  With a branch on lane == 0 around the loops a stage cost its TMA thread 680 cycles (two loads) and its MMA
 // thread 320 (four MMAs) of issue time -- more than the 512 cycles the tensor cores need for it.
@@ -94,21 +88,6 @@ __device__ __forceinline__ void cp_async_arrive_noinc(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(bar) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t columns) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-               :: "r"(smem_dst), "r"(columns) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t columns) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(taddr), "r"(columns) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
 __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
                                           uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -116,36 +95,7 @@ __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t adesc, uint6
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-               :: "r"(bar) : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
 
-// Shared-memory matrix descriptor for a K-major tile whose rows are 128 bytes
-// (64 BF16) with the 128-byte swizzle TMA applies: 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t smem_desc_k_major_sw128(uint32_t smem_addr) {
-  uint64_t desc = 0;
-  desc |= static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4);          // start address
-  desc |= static_cast<uint64_t>(1) << 16;                               // leading byte offset (unused)
-  desc |= static_cast<uint64_t>(1024 >> 4) << 32;                       // stride byte offset
-  desc |= static_cast<uint64_t>(1) << 46;                               // descriptor version (sm_100)
-  desc |= static_cast<uint64_t>(2) << 61;                               // SWIZZLE_128B
-  return desc;
-}
 
 // Instruction descriptor: D = F32, A = B = BF16, both K-major, M = 128, N = 256.
 constexpr uint32_t kInstrDesc =

@@ -281,7 +281,7 @@ extern "C" {
 
 #define AIMA_EXPORT __attribute__((visibility("default")))
 
-AIMA_EXPORT uint32_t aima_moe_abi_version(void) { return (1u << 16) | 0u; }
+AIMA_EXPORT uint32_t aima_moe_abi_version(void) { return (1u << 16) | 1u; }
 
 AIMA_EXPORT const char* aima_moe_last_error_string(void) { return g_last_error; }
 

@@ -103,6 +103,43 @@ class LmHeadResult(ctypes.Structure):
     ]
 
 
+class KvConfig(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", c_uint32), ("q_heads", c_uint32), ("kv_heads", c_uint32), ("head_dim", c_uint32), ("rotary_dim", c_uint32),
+        ("page_tokens", c_uint32), ("pages", c_uint32), ("layers", c_uint32), ("max_sequences", c_uint32), ("softmax_scale", c_float),
+    ]
+
+
+class KvLayer(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", c_uint32), ("reserved", c_uint32),
+        ("keys", c_void_p), ("keys_bytes", c_uint64), ("values", c_void_p), ("values_bytes", c_uint64),
+        ("key_scales", c_void_p), ("key_scales_bytes", c_uint64), ("value_scales", c_void_p), ("value_scales_bytes", c_uint64),
+    ]
+
+
+class KvBatchStruct(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", c_uint32), ("sequences", c_uint32), ("tokens", c_uint32), ("max_new_tokens", c_uint32),
+        ("table_columns", c_uint32), ("reserved", c_uint32),
+        ("page_table", c_void_p), ("row_offsets", c_void_p), ("lengths", c_void_p),
+    ]
+
+
+class KvRows(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("row_stride", c_uint64), ("head_stride", c_uint64)]
+
+
+class VerifyDrafts(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", c_uint32), ("sequences", c_uint32), ("max_drafts", c_uint32), ("vocabulary", c_uint32),
+        ("target", c_void_p), ("target_sequence_stride", c_uint64), ("target_row_stride", c_uint64),
+        ("draft", c_void_p), ("draft_sequence_stride", c_uint64), ("draft_row_stride", c_uint64),
+        ("draft_tokens", c_void_p), ("draft_counts", c_void_p), ("uniforms", c_void_p), ("cache_lengths", c_void_p),
+        ("accepted", c_void_p), ("tokens", c_void_p), ("new_lengths", c_void_p),
+    ]
+
+
 # every symbol include/aima_moe.h declares: (name, restype, argtypes)
 EXPORTS = [
     ("aima_moe_abi_version", c_uint32, []),
@@ -162,6 +199,17 @@ EXPORTS = [
     ("aima_moe_image_scatter_ingest", c_int,
      [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(c_uint64), ctypes.POINTER(c_uint64), ctypes.POINTER(c_uint64),
       c_uint64, c_uint64, c_uint64, c_uint64, c_int, c_uint64, c_uint64, ctypes.POINTER(ImageIngestResult)]),
+    ("aima_moe_kv_prepare", c_int, [ctypes.POINTER(KvConfig), ctypes.POINTER(c_void_p)]),
+    ("aima_moe_kv_bind_layer", c_int, [c_void_p, c_uint32, ctypes.POINTER(KvLayer)]),
+    ("aima_moe_kv_set_rotation", c_int, [c_void_p, c_void_p, c_uint32]),
+    ("aima_moe_kv_append_launch", c_int,
+     [c_void_p, c_uint32, ctypes.POINTER(KvBatchStruct), ctypes.POINTER(KvRows), ctypes.POINTER(KvRows), ctypes.POINTER(KvRows),
+      c_void_p, c_void_p]),
+    ("aima_moe_kv_attention_launch", c_int,
+     [c_void_p, c_uint32, ctypes.POINTER(KvBatchStruct), ctypes.POINTER(KvRows), c_void_p, c_void_p]),
+    ("aima_moe_kv_sync", c_int, [c_void_p]),
+    ("aima_moe_kv_release", c_int, [c_void_p]),
+    ("aima_moe_verify_drafts_launch", c_int, [ctypes.POINTER(VerifyDrafts), c_void_p]),
     ("aima_moe_sync_metrics", c_int, [c_void_p, ctypes.POINTER(Metrics)]),
     ("aima_moe_release", c_int, [c_void_p]),
 ]
@@ -662,3 +710,168 @@ class StripedImage:
             count, lane_bytes[0], lane_bytes[1], chunk_bytes, 0 if expected is None else 1,
             0 if expected is None else expected[0], 0 if expected is None else expected[1], ctypes.byref(result)))
         return result
+
+
+class KvBatch:
+    """One step's sequences for KvCache: their pages, their lengths and their rows of q, k and v.  Keeps its tensors alive; the
+    contents may change between launches (they are read on the device)."""
+
+    def __init__(self, page_table: Any, lengths: Any, row_offsets: Any, tokens: int, max_new_tokens: int) -> None:
+        import torch
+
+        for name, tensor, shape in (("page_table", page_table, None), ("lengths", lengths, (page_table.shape[0],)),
+                                    ("row_offsets", row_offsets, (page_table.shape[0] + 1,))):
+            if tensor is not None and (tensor.dtype != torch.int32 or (tensor.dim() != 2 if shape is None else tuple(tensor.shape) != shape)):
+                raise ValueError(f"{name} must be int32 {'[sequences, columns]' if shape is None else list(shape)}, got "
+                                 f"{tensor.dtype} {list(tensor.shape)}")
+        self.page_table, self.lengths, self.row_offsets = page_table, lengths, row_offsets
+        self.tokens = tokens
+        self.struct = KvBatchStruct(ctypes.sizeof(KvBatchStruct), int(page_table.shape[0]), tokens, max_new_tokens, int(page_table.shape[1]), 0,
+                                    _ptr(page_table), _ptr(row_offsets), _ptr(lengths))
+        self.ref = ctypes.byref(self.struct)
+
+
+class KvCache:
+    """Paged 8-bit key/value cache of the full-attention layers: the binding of aima_moe_kv_*.  The cache tensors are the
+    caller's, one set per layer: keys and values [pages, kv_heads, page_tokens, head_dim] (float8_e4m3fn or uint8) and their
+    FP32 scales [pages, kv_heads]."""
+
+    def __init__(self, *, q_heads: int = 16, kv_heads: int = 2, head_dim: int = 256, rotary_dim: int = 64, page_tokens: int = 64,
+                 pages: int, layers: int = 1, max_sequences: int = 256, softmax_scale: float = 0.0,
+                 library: MoeLibrary | None = None) -> None:
+        import torch
+
+        if not torch.cuda.is_available():
+            raise RuntimeError("aima_moe needs a CUDA device (sm_100a); there is no CPU fallback")
+        self._torch = torch
+        self.lib = library or load_library()
+        self.config = KvConfig(ctypes.sizeof(KvConfig), q_heads, kv_heads, head_dim, rotary_dim, page_tokens, pages, layers, max_sequences,
+                               softmax_scale)
+        handle = c_void_p()
+        self.lib.check(self.lib.aima_moe_kv_prepare(ctypes.byref(self.config), ctypes.byref(handle)))
+        self.handle = handle
+        self._q_shape, self._kv_shape = (q_heads, head_dim), (kv_heads, head_dim)
+        self._keepalive: dict[Any, Any] = {}
+
+    # -- setup ---------------------------------------------------------------
+    def allocate_layer(self) -> tuple[Any, Any, Any, Any]:
+        """Zeroed cache tensors of one layer, in the order bind_layer takes them."""
+        torch, c = self._torch, self.config
+        codes = [torch.zeros(c.pages, c.kv_heads, c.page_tokens, c.head_dim, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+                 for _ in range(2)]
+        return (*codes, *(torch.ones(c.pages, c.kv_heads, dtype=torch.float32, device="cuda") for _ in range(2)))
+
+    def bind_layer(self, layer: int, keys: Any, values: Any, key_scales: Any, value_scales: Any) -> None:
+        torch = self._torch
+        for name, tensor in (("keys", keys), ("values", values)):
+            if tensor.dtype not in (torch.float8_e4m3fn, torch.uint8):
+                raise ValueError(f"{name} must be float8_e4m3fn or uint8, got {tensor.dtype}")
+        for name, tensor in (("key_scales", key_scales), ("value_scales", value_scales)):
+            if tensor.dtype != torch.float32:
+                raise ValueError(f"{name} must be float32, got {tensor.dtype}")
+        tensors = KvLayer(ctypes.sizeof(KvLayer), 0, _ptr(keys), _nbytes(keys), _ptr(values), _nbytes(values),
+                          _ptr(key_scales), _nbytes(key_scales), _ptr(value_scales), _nbytes(value_scales))
+        self.lib.check(self.lib.aima_moe_kv_bind_layer(self.handle, layer, ctypes.byref(tensors)))
+        self._keepalive[layer] = (keys, values, key_scales, value_scales)
+
+    def set_rotation(self, table: Any) -> None:
+        """FP32 [positions, rotary_dim]: the cosines of a position's angles, then their sines."""
+        if table.dtype != self._torch.float32 or table.dim() != 2 or table.shape[1] != self.config.rotary_dim:
+            raise ValueError(f"the rotation table must be float32 [positions, {self.config.rotary_dim}]")
+        self.lib.check(self.lib.aima_moe_kv_set_rotation(self.handle, _ptr(table), int(table.shape[0])))
+        self._keepalive["rotation"] = table
+
+    @staticmethod
+    def batch(page_table: Any, lengths: Any, *, tokens: int, row_offsets: Any = None, max_new_tokens: int | None = None) -> KvBatch:
+        """page_table int32 [sequences, columns]; lengths int32 [sequences], the new tokens included; row_offsets int32
+        [sequences + 1] into the `tokens` rows of q, k and v, or None for the same number of rows each."""
+        if max_new_tokens is None:
+            max_new_tokens = tokens if row_offsets is not None else tokens // int(page_table.shape[0])
+        return KvBatch(page_table, lengths, row_offsets, tokens, max_new_tokens)
+
+    # -- launches ------------------------------------------------------------
+    def _rows(self, tensor: Any, name: str, tokens: int, shape: tuple[int, int]) -> KvRows:
+        if tensor.dtype is not self._torch.bfloat16 or not tensor.is_cuda or tuple(tensor.shape) != (tokens, *shape) or tensor.stride(2) != 1:
+            raise ValueError(f"{name} must be a CUDA bfloat16 tensor [{tokens}, {shape[0]}, {shape[1]}] with contiguous heads, got "
+                             f"{tensor.dtype} {list(tensor.shape)} with strides {list(tensor.stride())}")
+        row_stride, head_stride, _ = tensor.stride()
+        return KvRows(tensor.data_ptr(), row_stride, head_stride)
+
+    def append(self, layer: int, batch: KvBatch, k: Any, v: Any, q: Any = None, q_out: Any = None) -> Any:
+        """Rotates k and stores it and v; with q returns the rotated queries [tokens, q_heads, head_dim].  k, v and q may be views
+        into one row of a fused projection."""
+        torch, tokens = self._torch, batch.tokens
+        k_rows, v_rows = self._rows(k, "k", tokens, self._kv_shape), self._rows(v, "v", tokens, self._kv_shape)
+        q_rows = None
+        if q is not None:
+            q_rows = self._rows(q, "q", tokens, self._q_shape)
+            if q_out is None:
+                q_out = torch.empty((tokens, *self._q_shape), dtype=torch.bfloat16, device=q.device)
+        self.lib.check(self.lib.aima_moe_kv_append_launch(
+            self.handle, layer, batch.ref, k_rows, v_rows, q_rows, None if q_out is None else _ptr(q_out), _stream(torch)))
+        return q_out
+
+    def attention(self, layer: int, batch: KvBatch, q: Any, out: Any = None) -> Any:
+        """Causal attention of the batch's rows over the cache (after append): [tokens, q_heads, head_dim]."""
+        torch = self._torch
+        q_rows = self._rows(q, "q", batch.tokens, self._q_shape)
+        if out is None:
+            out = torch.empty((batch.tokens, *self._q_shape), dtype=torch.bfloat16, device=q.device)
+        elif out.dtype is not torch.bfloat16 or tuple(out.shape) != (batch.tokens, *self._q_shape):
+            raise ValueError(f"out must be bfloat16 [{batch.tokens}, {self._q_shape[0]}, {self._q_shape[1]}]")
+        self.lib.check(self.lib.aima_moe_kv_attention_launch(self.handle, layer, batch.ref, q_rows, _ptr(out), _stream(torch)))
+        return out
+
+    def sync(self) -> None:
+        """Waits for the last launch and raises AimaMoeError if device-side data of a batch was out of range."""
+        self.lib.check(self.lib.aima_moe_kv_sync(self.handle))
+
+    def release(self) -> None:
+        if getattr(self, "handle", None):
+            self.lib.aima_moe_kv_release(self.handle)
+            self.handle = None
+            self._keepalive.clear()
+
+    def __del__(self) -> None:  # best effort
+        try:
+            self.release()
+        except Exception:
+            pass
+
+
+def verify_drafts(target: Any, draft_tokens: Any, uniforms: Any, draft_probabilities: Any = None, draft_counts: Any = None,
+                  cache_lengths: Any = None, library: MoeLibrary | None = None) -> tuple:
+    """Accepts drafted tokens against the target's probabilities and draws the token that follows (aima_moe_verify_drafts_launch).
+
+    target FP32 [sequences, drafts + 1, vocabulary]; draft_tokens int32 [sequences, drafts]; uniforms FP32 [sequences, drafts + 1];
+    draft_probabilities FP32 [sequences, drafts, vocabulary] or None for drafts that were not drawn at random; draft_counts int32
+    [sequences] for fewer drafts.  Returns (accepted int32 [sequences], tokens int32 [sequences, drafts + 1]) and, with
+    cache_lengths int32 [sequences], the lengths without the rejected drafts."""
+    import torch
+
+    lib = library or load_library()
+    if target.dim() != 3:
+        raise ValueError("target must be [sequences, drafts + 1, vocabulary]")
+    sequences, rows, vocabulary = target.shape
+    for name, tensor, dtype, shape in (
+            ("target", target, torch.float32, (sequences, rows, vocabulary)), ("draft_tokens", draft_tokens, torch.int32, (sequences, rows - 1)),
+            ("uniforms", uniforms, torch.float32, (sequences, rows)),
+            ("draft_probabilities", draft_probabilities, torch.float32, (sequences, rows - 1, vocabulary)),
+            ("draft_counts", draft_counts, torch.int32, (sequences,)), ("cache_lengths", cache_lengths, torch.int32, (sequences,))):
+        if tensor is not None and (tensor.dtype is not dtype or tuple(tensor.shape) != shape or not tensor.is_cuda):
+            raise ValueError(f"{name} must be a CUDA {dtype} tensor {list(shape)}, got {tensor.dtype} {list(tensor.shape)}")
+    for name, tensor in (("target", target), ("draft_probabilities", draft_probabilities)):
+        if tensor is not None and vocabulary > 1 and tensor.stride(2) != 1:
+            raise ValueError(f"rows of {name} must be contiguous")
+    out = torch.empty((sequences, rows + 1 if cache_lengths is None else rows + 2), dtype=torch.int32, device=target.device)
+    flat = out.view(-1)
+    accepted, tokens = flat[:sequences], flat[sequences:sequences * (rows + 1)].view(sequences, rows)
+    new_lengths = None if cache_lengths is None else flat[sequences * (rows + 1):]
+    has_draft = draft_probabilities is not None
+    call = VerifyDrafts(
+        ctypes.sizeof(VerifyDrafts), sequences, rows - 1, vocabulary, target.data_ptr(), target.stride(0), target.stride(1),
+        draft_probabilities.data_ptr() if has_draft else None, draft_probabilities.stride(0) if has_draft else 0,
+        draft_probabilities.stride(1) if has_draft else 0, _ptr(draft_tokens), _ptr(draft_counts), _ptr(uniforms), _ptr(cache_lengths),
+        accepted.data_ptr(), tokens.data_ptr(), None if new_lengths is None else new_lengths.data_ptr())
+    lib.check(lib.aima_moe_verify_drafts_launch(call, _stream(torch)))
+    return (accepted, tokens) if new_lengths is None else (accepted, tokens, new_lengths)

@@ -486,6 +486,134 @@ int aima_moe_image_scatter_ingest(const char* lane0_path, const char* lane1_path
                                   int check_expected, uint64_t expected_xor, uint64_t expected_sum,
                                   aima_moe_image_ingest_result* result);
 
+/* ---------------------------------------------------------------------------
+ * Full-attention cache.  What a host needs on the attention side of a full-attention layer (10 of the 40 layers: 16 query
+ * heads, 2 key/value heads of 256, 64 of them rotated) between its fused input projection and its output projection: the
+ * counterpart of the reference's head rotation, KV append and grouped decode attention
+ * (native/src/native_full_attention.hip.cpp) and of the causal prefill provider
+ * (benchmarks/shape-lab/native/src/qrt_ck_fmha_q8192_provider.cpp), over a cache that is paged and held in 8 bits.
+ *
+ * Layout, caller-owned, per layer: keys and values [pages, kv_heads, page_tokens, head_dim] in e4m3 (one byte each), and for
+ * each an FP32 scale [pages, kv_heads]: the element stands for its code times the scale of its page and head.
+ * aima_moe_kv_append_launch writes powers of two as scales; the attention takes any positive finite scale.
+ *
+ * A batch names, for every sequence, its pages (page_table, page i holds positions [i * page_tokens, ...)), the number of
+ * tokens in the cache once the new ones are in it (lengths), and the rows of q, k and v that are its new tokens
+ * (row_offsets): its last row is position lengths - 1, the one before it lengths - 2, and so on.  A row whose position is
+ * negative is inactive: it is not stored and its attention is zero (a sequence of length 0 in a padded batch).  All of it is
+ * read on the device, so a captured graph can be replayed for other lengths. */
+#define AIMA_MOE_KV_MAX_LAYERS 64
+#define AIMA_MOE_KV_MAX_SEQUENCES 1024
+typedef struct aima_moe_kv aima_moe_kv;
+
+typedef struct aima_moe_kv_config {
+  uint32_t struct_bytes;   /* sizeof(aima_moe_kv_config), ABI check                               */
+  uint32_t q_heads;        /* a multiple of kv_heads, at most 128 per kv head                     */
+  uint32_t kv_heads;       /* 1 .. 128                                                            */
+  uint32_t head_dim;       /* 64, 128 or 256                                                      */
+  uint32_t rotary_dim;     /* 0 .. head_dim, a multiple of 16: the first elements of a head; element j turns with
+                              element j + rotary_dim / 2                                          */
+  uint32_t page_tokens;    /* 16, 32, 64 or 128                                                   */
+  uint32_t pages;          /* pages of every layer's tensors; pages * kv_heads * page_tokens < 2^31 */
+  uint32_t layers;         /* 1 .. AIMA_MOE_KV_MAX_LAYERS                                         */
+  uint32_t max_sequences;  /* 1 .. AIMA_MOE_KV_MAX_SEQUENCES sequences in a batch                 */
+  float softmax_scale;     /* of the scores; 0 = 1 / sqrt(head_dim)                               */
+} aima_moe_kv_config;
+
+typedef struct aima_moe_kv_layer {
+  uint32_t struct_bytes;
+  uint32_t reserved;
+  void* keys;          uint64_t keys_bytes;           /* pages * kv_heads * page_tokens * head_dim */
+  void* values;        uint64_t values_bytes;
+  void* key_scales;    uint64_t key_scales_bytes;     /* pages * kv_heads * 4                      */
+  void* value_scales;  uint64_t value_scales_bytes;
+} aima_moe_kv_layer;
+
+typedef struct aima_moe_kv_batch {
+  uint32_t struct_bytes;
+  uint32_t sequences;          /* 1 .. max_sequences                                            */
+  uint32_t tokens;             /* rows of q, k and v                                            */
+  uint32_t max_new_tokens;     /* no sequence has more rows than this; 1 .. tokens              */
+  uint32_t table_columns;      /* pages a sequence can have                                     */
+  uint32_t reserved;
+  const int32_t* page_table;   /* [sequences, table_columns]                                    */
+  const int32_t* row_offsets;  /* [sequences + 1], from 0 to at most tokens, not falling; NULL: max_new_tokens rows each
+                                  (tokens = sequences * max_new_tokens)                         */
+  const int32_t* lengths;      /* [sequences]                                                   */
+} aima_moe_kv_batch;
+
+/* Rows of heads: element (row, head, i) is at row * row_stride + head * head_stride + i, in elements (BF16).  16-byte
+ * aligned, strides multiples of 8. */
+typedef struct aima_moe_kv_rows {
+  const void* data;
+  uint64_t row_stride;
+  uint64_t head_stride;
+} aima_moe_kv_rows;
+
+/* Checks the configuration and allocates the workspace on the current device (the only allocation). */
+int aima_moe_kv_prepare(const aima_moe_kv_config* config, aima_moe_kv** handle);
+/* Records one layer's cache tensors.  16-byte aligned, of the handle's device. */
+int aima_moe_kv_bind_layer(aima_moe_kv* handle, uint32_t layer, const aima_moe_kv_layer* tensors);
+/* The rotation by position: FP32 [positions, rotary_dim], a row holds the cosines of its rotary_dim / 2 angles, then the
+ * sines.  The table stays the caller's.  Needed before an append if rotary_dim > 0. */
+int aima_moe_kv_set_rotation(aima_moe_kv* handle, const void* table_f32, uint32_t positions);
+
+/* Rotates k by the rows' positions and stores it and v in the cache, one launch; with q (data not NULL) also writes the
+ * rotated queries to q_out (BF16 [tokens, q_heads, head_dim], contiguous, may not overlap q).
+ * Per page and head the scale is the least power of two, from 2^-64 on, that keeps every element within e4m3's 448.  A page
+ * that held tokens before keeps its scale unless a new token needs a larger one; then the older codes are rounded to it.
+ * A token that brings a NaN or an infinity to a head (in its rotated key or in its value) is stored there with NaN keys and
+ * zero values: every query that sees it gets NaN, and no other does.
+ * The pages that the new tokens go to belong to one sequence each. */
+int aima_moe_kv_append_launch(aima_moe_kv* handle, uint32_t layer, const aima_moe_kv_batch* batch,
+                              const aima_moe_kv_rows* k, const aima_moe_kv_rows* v, const aima_moe_kv_rows* q,
+                              void* q_out, void* stream);
+
+/* Attention of the batch's rows over the cache, causal: the row at position p sees positions 0 .. p.
+ * out (BF16 [tokens, q_heads, head_dim], contiguous) = softmax(softmax_scale q k^T) v; query head h reads key/value head
+ * h / (q_heads / kv_heads).  Rows that see nothing are zero; rows of no sequence (behind the last offset) are not written.
+ * Bytes of a page behind a sequence's length can hold anything.  out may not overlap q.  Calls of one handle share its
+ * workspace: issue them on one stream or order them with events. */
+int aima_moe_kv_attention_launch(aima_moe_kv* handle, uint32_t layer, const aima_moe_kv_batch* batch,
+                                 const aima_moe_kv_rows* q, void* out, void* stream);
+
+/* Synchronises the last stream and reports what launches since the last call found wrong in device-side data:
+ * AIMA_MOE_ERR_INVALID_ARGUMENT for a length, row offset or position outside its range (such a sequence was treated as one
+ * without tokens) or a page number outside its range (its positions were left out), AIMA_MOE_ERR_TIMEOUT for a bounded wait that ran out. */
+int aima_moe_kv_sync(aima_moe_kv* handle);
+int aima_moe_kv_release(aima_moe_kv* handle);
+
+/* Verification of drafted tokens against the target's probabilities, from given random numbers; no handle, no workspace.
+ * Per sequence with n drafts x_0 .. x_{n-1}, target probabilities p_0 .. p_n and draft probabilities q_0 .. q_{n-1}: draft i is
+ * accepted while u_i q_i(x_i) < p_i(x_i); without draft probabilities q is 1 at the draft and 0 elsewhere (drafts that were
+ * not drawn at random).  With a drafts accepted the token that follows is drawn with weights p_n if a = n, else
+ * max(p_a - q_a, 0), by u_n: weights are taken as whole multiples of 2^-40 and summed as integers, and the token is the lowest
+ * whose running sum exceeds floor(total * floor(2^24 u_n) / 2^24), so the result does not depend on any order of summation.
+ * If nothing of the weights is left, p_a itself is used; if that is zero too, the token is -1.  A draft outside the
+ * vocabulary is rejected.  NaN and negative probabilities count as 0, u is clamped to [0, 1).
+ * accepted [sequences]; tokens [sequences, max_drafts + 1]: the accepted drafts, the token drawn, then -1; new_lengths
+ * [sequences] = cache_lengths - (n - a), the cache's lengths without the rejected drafts (both NULL or neither; in place is fine). */
+typedef struct aima_moe_verify_drafts {
+  uint32_t struct_bytes;
+  uint32_t sequences;
+  uint32_t max_drafts;                /* 0 .. 64                                                        */
+  uint32_t vocabulary;                /* 1 .. 2^22                                                      */
+  const void* target;                 /* FP32 (sequence, 0 .. max_drafts, token)                        */
+  uint64_t target_sequence_stride;    /* in elements                                                    */
+  uint64_t target_row_stride;
+  const void* draft;                  /* FP32 (sequence, 0 .. max_drafts - 1, token) or NULL            */
+  uint64_t draft_sequence_stride;
+  uint64_t draft_row_stride;
+  const int32_t* draft_tokens;        /* [sequences, max_drafts]                                        */
+  const int32_t* draft_counts;        /* [sequences], clamped to 0 .. max_drafts; NULL: max_drafts each */
+  const float* uniforms;              /* [sequences, max_drafts + 1]; u_n is at column max_drafts       */
+  const int32_t* cache_lengths;
+  int32_t* accepted;
+  int32_t* tokens;
+  int32_t* new_lengths;
+} aima_moe_verify_drafts;
+int aima_moe_verify_drafts_launch(const aima_moe_verify_drafts* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
