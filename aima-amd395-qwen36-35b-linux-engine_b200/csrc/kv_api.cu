@@ -1,5 +1,5 @@
 // C ABI of the full-attention cache and of the verification of drafted tokens (contract in include/aima_moe.h).
-#include "kv_cache.cuh"
+#include "kv_attention.cuh"
 
 #include <cmath>
 #include <cstdarg>
@@ -15,10 +15,11 @@ struct aima_moe_kv {
   aima::KvShape shape{};
   float scale_log2 = 0.0f;
   aima::KvLayer layers[AIMA_MOE_KV_MAX_LAYERS]{};
+  aima::KvMaps maps[AIMA_MOE_KV_MAX_LAYERS]{};
   bool bound[AIMA_MOE_KV_MAX_LAYERS]{};
   const float* rotation = nullptr;     // the caller's
   int positions = 0;
-  int* status = nullptr;
+  int* status = nullptr;               // the allocation: 256 bytes, then the attention's workspace
   cudaStream_t last_stream = nullptr;
 };
 
@@ -163,7 +164,7 @@ AIMA_EXPORT int aima_moe_kv_prepare(const aima_moe_kv_config* config, aima_moe_k
                            static_cast<int>(config->pages)};
   const double scale = config->softmax_scale != 0.0f ? config->softmax_scale : 1.0 / std::sqrt(static_cast<double>(config->head_dim));
   h->scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-  error = cudaMalloc(&h->status, 256);
+  error = cudaMalloc(&h->status, 256 + aima::kv_workspace_bytes(h->shape, static_cast<int>(config->max_sequences)));
   if (error == cudaSuccess) error = cudaMemset(h->status, 0, 256);
   if (error != cudaSuccess) {
     cudaFree(h->status);
@@ -195,6 +196,7 @@ AIMA_EXPORT int aima_moe_kv_bind_layer(aima_moe_kv* h, uint32_t layer, const aim
   }
   const aima::KvLayer bound{static_cast<uint8_t*>(t->keys), static_cast<uint8_t*>(t->values), static_cast<float*>(t->key_scales),
                                    static_cast<float*>(t->value_scales)};
+  if (!aima::kv_make_maps(h->shape, bound, &h->maps[layer])) return kv_fail(AIMA_MOE_ERR_INTERNAL, "kv: tensor maps of the cache could not be made");
   h->layers[layer] = bound;
   h->bound[layer] = true;
   return AIMA_MOE_OK;
@@ -251,7 +253,7 @@ AIMA_EXPORT int aima_moe_kv_attention_launch(aima_moe_kv* h, uint32_t layer, con
   a.out = static_cast<__nv_bfloat16*>(out);
   a.scale_log2 = h->scale_log2;
   a.status = h->status;
-  const cudaError_t error = aima::kv_attention(a, static_cast<cudaStream_t>(stream));
+  const cudaError_t error = aima::kv_attention(a, h->maps[layer], reinterpret_cast<uint8_t*>(h->status) + 256, h->sm_count, static_cast<cudaStream_t>(stream));
   if (error != cudaSuccess) return kv_fail_cuda(error, "kv attention launch");
   h->last_stream = static_cast<cudaStream_t>(stream);
   return AIMA_MOE_OK;

@@ -91,7 +91,10 @@ struct KvAttention {
   float scale_log2;        // softmax scale * log2(e)
   int* status;
 };
-cudaError_t kv_attention(const KvAttention& args, cudaStream_t stream);
+struct KvMaps;             // tensor maps of a layer's cache
+size_t kv_workspace_bytes(const KvShape& shape, int max_sequences);
+bool kv_make_maps(const KvShape& shape, const KvLayer& layer, KvMaps* maps);
+cudaError_t kv_attention(const KvAttention& args, const KvMaps& maps, void* workspace, int sm_count, cudaStream_t stream);
 
 cudaError_t verify_drafts(const aima_moe_verify_drafts& call, cudaStream_t stream);
 
