@@ -16,7 +16,8 @@ CSRC = HERE / "csrc"
 LIB = HERE / "libaima_moe_b200.so"
 SOURCES = ["moe_api.cu", "decode_kernel.cu", "decode_noalloc.cu", "pointwise.cu", "prefill.cu",
            "grouped_gemm_simt.cu", "grouped_gemm_tc.cu", "lm_head.cu", "lm_head_api.cu",
-           "image_loader.cu", "kv_api.cu", "kv_append.cu", "kv_attention.cu", "kv_decode.cu", "verify_drafts.cu"]
+           "image_loader.cu", "kv_api.cu", "kv_append.cu", "kv_attention.cu", "kv_decode.cu", "kv_prompt.cu",
+           "verify_drafts.cu"]
 
 
 def nvcc_path() -> str:

@@ -253,7 +253,7 @@ AIMA_EXPORT int aima_moe_kv_attention_launch(aima_moe_kv* h, uint32_t layer, con
   a.out = static_cast<__nv_bfloat16*>(out);
   a.scale_log2 = h->scale_log2;
   a.status = h->status;
-  const cudaError_t error = aima::kv_attention(a, h->maps[layer], reinterpret_cast<uint8_t*>(h->status) + 256, h->sm_count, static_cast<cudaStream_t>(stream));
+  const cudaError_t error = aima::kv_attention(a, h->maps[layer], reinterpret_cast<uint8_t*>(h->status) + 256, static_cast<int>(h->config.max_sequences), h->sm_count, static_cast<cudaStream_t>(stream));
   if (error != cudaSuccess) return kv_fail_cuda(error, "kv attention launch");
   h->last_stream = static_cast<cudaStream_t>(stream);
   return AIMA_MOE_OK;

@@ -94,7 +94,7 @@ struct KvAttention {
 struct KvMaps;             // tensor maps of a layer's cache
 size_t kv_workspace_bytes(const KvShape& shape, int max_sequences);
 bool kv_make_maps(const KvShape& shape, const KvLayer& layer, KvMaps* maps);
-cudaError_t kv_attention(const KvAttention& args, const KvMaps& maps, void* workspace, int sm_count, cudaStream_t stream);
+cudaError_t kv_attention(const KvAttention& args, const KvMaps& maps, void* workspace, int max_sequences, int sm_count, cudaStream_t stream);
 
 cudaError_t verify_drafts(const aima_moe_verify_drafts& call, cudaStream_t stream);
 

@@ -1,0 +1,774 @@
+// Attention of many rows per sequence (chunks of prompts) over the paged 8-bit cache.
+//
+//   t_ij = scale q_i . k_j (log2 units) + log2(value scale of j's page),   w_ij = 2^(t_ij - m_i)
+//   o_i  = sum_j w_ij code(v_j) / sum_j w_ij / (value scale of j's page)
+// as in kv_decode.cu, here with the rows as the M side.  A row tile is up to 128 rows: whole new tokens x the query heads that
+// share a key/value head, so that K and V are loaded once for all of them.
+//
+// Bound: the products, 4 x rows x positions x head_dim flops at the rate of 16-bit ones.  Queries and weights are BF16-like, the
+// cache is e4m3, and no operand of mixed width exists; unpacking K and V would cost conversions and shared memory per tile,
+// so Q and the weights are split into two 8-bit terms instead and the products run twice at twice the rate:
+//   q 2^-e  = hi (e4m3) + lo (e5m2)          exact down to 2^-16 (largest 448)
+//   w 2^7   = hi (e4m3) + lo (e5m2)          to 2^-8 of itself, down to 2^-16
+// both terms into the same accumulator.  S[128 rows, 128 positions] = Q K^T with both operands in shared memory;
+// O[128, head_dim] += W V with W in tensor memory, where it takes the place of the scores it was made from, and V MN-major.
+//
+// One block per SM.  Warp 0 loads tiles by page, warp 1 issues the products, warp 3 fetches the scales; warps 4-7 and 8-11 (thread =
+// row) take turns with the tiles: while one group turns the scores of a tile into weights the other waits for the next
+// tile's scores or has just stored its weights.  What passes between them is the reference maximum of each row, warp by warp.
+#include "kv_attention.cuh"
+
+#include <cuda_fp16.h>
+
+namespace aima {
+namespace {
+
+constexpr int kThreads = 384;
+// The reference of a row's weights moves up when a tile's maximum exceeds it by more than kGrow, and down when a tile's maximum
+// falls short of it by more than kFall: small weights have few bits, and where one position outweighs all others by 2^14
+// and brings nothing (a sink), they are the result.  It stays within kDepth of the row's maximum so that nothing overflows.
+constexpr float kGrow = 1.75f;            // 2^7 * 2^1.75 = 430 <= 448
+constexpr float kFall = 8.0f;
+constexpr float kDepth = 30.0f;
+constexpr float kWeightExponent = 7.0f;
+constexpr int kScaleSlots = 4;
+
+template <int kDim>
+struct Prompt {
+  static constexpr int kRowBytes = kDim >= 128 ? 128 : 64;
+  static constexpr int kPanels = kDim / kRowBytes;
+  static constexpr int kPanelBytes = kKvTile * kRowBytes;
+  static constexpr int kSlotBytes = kKvTile * kDim;
+  static constexpr int kSlots = kDim == 256 ? 4 : 8;
+  static constexpr int kQueryAt = kSlots * kSlotBytes;                  // hi, then lo
+  static constexpr int kSmallAt = kQueryAt + 2 * kSlotBytes;
+  static constexpr int kScoreColumn = 256;                              // tensor memory: O | S0 | S1
+};
+
+struct Small {
+  float4 scales[kScaleSlots][8];           // per 16 positions: key scale x softmax scale, log2 and inverse of the value scale
+  unsigned long long full[8], empty[8], scales_full[kScaleSlots], scales_empty[kScaleSlots];
+  unsigned long long s_full[2], p_full[2], o_done[2], top_done[2][4], q_full, drain;
+  float row_scale[128];
+  float2 top[128];                         // per row: the reference, and the maximum so far
+  float sum[2][128], group_top[2][128];
+  uint32_t tmem;
+  int abort_flag;
+};
+
+// A block's share of the list, unit by unit.
+struct Walk {
+  const KvAttentionPlan* plan;
+  int sequence, row_tile, head, tile0, tiles;
+  long long left;
+  KvSequence seq;
+  KvUnit unit;
+  int row_tiles;
+  __device__ __forceinline__ void load() {
+    seq = kv_sequence(plan->a.batch, plan->a.shape, sequence);
+    row_tiles = (seq.rows + plan->tile_tokens - 1) / plan->tile_tokens;
+  }
+  __device__ __forceinline__ void begin(const KvAttentionPlan& p, const KvStart& start, long long end) {
+    plan = &p;
+    left = end - start.at;
+    sequence = start.sequence;
+    row_tile = start.row_tile;
+    head = start.head;
+    tile0 = start.tile;
+    if (left > 0) load();
+  }
+  __device__ __forceinline__ bool next() {
+    if (left <= 0) return false;
+    for (;;) {
+      if (row_tile < row_tiles) {
+        unit = kv_unit(seq, row_tile, plan->tile_tokens);
+        if (tile0 < unit.tiles) break;
+        tile0 = 0;
+        if (unit.tiles > 0 && ++head < plan->a.shape.kv_heads) continue;
+        head = 0;
+        ++row_tile;
+      } else {
+        row_tile = 0;
+        ++sequence;
+        load();
+      }
+    }
+    tiles = static_cast<int>(min(static_cast<long long>(unit.tiles - tile0), left));
+    return true;
+  }
+  __device__ __forceinline__ void advance() {
+    left -= tiles;
+    tile0 += tiles;
+  }
+};
+
+__device__ __forceinline__ void group_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// Cuts the list into `blocks` shares.  The list runs over sequences, their row tiles, the key/value heads and the tiles of the
+// cache.  A cut that falls near the end of a unit moves there: a divided unit costs its two blocks a write of 128 x head_dim
+// sums each and the join a read of them, about as much as kSnap tiles.  One block; items are row tiles.
+constexpr int kPlanThreads = 1024;
+constexpr int kSnap = 6;
+__global__ void __launch_bounds__(kPlanThreads)
+kv_plan_kernel(const KvAttentionPlan plan) {
+  __shared__ int first_item[AIMA_MOE_KV_MAX_SEQUENCES + 1];
+  __shared__ long long warp_sum[kPlanThreads / 32];
+  __shared__ long long carry, total_s;
+  pdl_enter();
+  const KvAttention& a = plan.a;
+  const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
+  const int heads = a.shape.kv_heads, dim = a.shape.head_dim;
+  auto scan = [&](long long x) {               // inclusive, over the block
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long other = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += other;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+      long long w = warp_sum[lane];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long other = __shfl_up_sync(0xffffffffu, w, d);
+        if (lane >= d) w += other;
+      }
+      warp_sum[lane] = w;
+    }
+    __syncthreads();
+    const long long before = warp > 0 ? warp_sum[warp - 1] : 0;
+    return before + x;
+  };
+  int items_here = 0;
+  if (thread < a.batch.sequences) {
+    const KvSequence seq = kv_sequence(a.batch, a.shape, thread);
+    if (seq.bad) atomicOr(a.status, kKvBadBatch);
+    items_here = (seq.rows + plan.tile_tokens - 1) / plan.tile_tokens;
+  }
+  const int upto = static_cast<int>(scan(items_here));
+  if (thread < a.batch.sequences) first_item[thread + 1] = upto;
+  if (thread == 0) first_item[0] = 0;
+  __syncthreads();
+  const int items = first_item[a.batch.sequences];
+  for (int pass = 0; pass < 2; ++pass) {
+    if (thread == 0) carry = 0;
+    __syncthreads();
+    for (int item0 = 0; item0 < items; item0 += kPlanThreads) {
+      const int item = item0 + thread;
+      int s = 0, row_tile = 0;
+      KvUnit unit{0, 0, 0};
+      KvSequence seq{};
+      if (item < items) {
+        int low = 0, high = a.batch.sequences;
+        while (high - low > 1) {
+          const int mid = (low + high) >> 1;
+          if (first_item[mid] <= item) low = mid; else high = mid;
+        }
+        s = low;
+        row_tile = item - first_item[s];
+        seq = kv_sequence(a.batch, a.shape, s);
+        unit = kv_unit(seq, row_tile, plan.tile_tokens);
+      }
+      const long long end = scan(static_cast<long long>(unit.tiles) * heads) + carry;
+      const long long begin = end - static_cast<long long>(unit.tiles) * heads;
+      if (pass == 1 && unit.tiles > 0) {
+        // the cuts c with begin < total c / blocks <= end, and the list's own begin
+        const long long total = total_s;
+        for (long long c = begin == 0 ? 0 : begin * plan.blocks / total + 1; c <= plan.blocks; ++c) {
+          const long long cut = total * c / plan.blocks;
+          if (cut > end) break;
+          if (cut <= begin && begin != 0) continue;
+          int head = static_cast<int>(min((cut - begin) / unit.tiles, static_cast<long long>(heads - 1)));
+          int tile = static_cast<int>(cut - begin - static_cast<long long>(head) * unit.tiles);
+          if (tile <= kSnap && tile <= unit.tiles - tile) tile = 0;
+          else if (unit.tiles - tile <= kSnap) tile = unit.tiles;
+          plan.work.starts[c] = KvStart{begin + static_cast<long long>(head) * unit.tiles + tile, s, row_tile, head, tile};
+        }
+      }
+      if (pass == 1 && item < items && unit.tiles == 0) {
+        // rows that see nothing
+        for (int i = 0; i < unit.tokens; ++i) {
+          uint4* out = reinterpret_cast<uint4*>(a.out + (seq.row0 + row_tile * plan.tile_tokens + i) * static_cast<long long>(a.shape.q_heads) * dim);
+          for (int j = 0; j < a.shape.q_heads * dim / 8; ++j) out[j] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      __syncthreads();
+      if (thread == kPlanThreads - 1) carry = end;
+      __syncthreads();
+    }
+    if (pass == 0) {
+      if (thread == 0) total_s = carry;
+      __syncthreads();
+      if (total_s == 0) {
+        for (int c = thread; c <= plan.blocks; c += kPlanThreads) plan.work.starts[c] = KvStart{0, 0, 0, 0, 0};
+      }
+    }
+  }
+}
+
+template <int kDim>
+__global__ void __launch_bounds__(kThreads, 1)
+kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ KvAttentionPlan plan) {
+  using L = Prompt<kDim>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* generic = smem_raw + (base - smem_u32(smem_raw));
+  Small& sm = *reinterpret_cast<Small*>(generic + L::kSmallAt);
+  volatile int* abort_flag = &sm.abort_flag;
+  const KvAttention& a = plan.a;
+  const KvShape& shape = a.shape;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L::kSlots; ++s) {
+      mbar_init(smem_u32(&sm.full[s]), 1);
+      mbar_init(smem_u32(&sm.empty[s]), 1);
+    }
+    for (int s = 0; s < kScaleSlots; ++s) {
+      mbar_init(smem_u32(&sm.scales_full[s]), 1);
+      mbar_init(smem_u32(&sm.scales_empty[s]), 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sm.s_full[i]), 1);
+      mbar_init(smem_u32(&sm.p_full[i]), 4);
+      mbar_init(smem_u32(&sm.o_done[i]), 1);
+      for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&sm.top_done[i][q]), 1);
+    }
+    mbar_init(smem_u32(&sm.q_full), 8);
+    mbar_init(smem_u32(&sm.drain), 1);
+    sm.abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 2) tmem_alloc(smem_u32(&sm.tmem), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  pdl_enter();
+
+  const KvStart start = plan.work.starts[blockIdx.x];
+  Walk walk;
+  walk.begin(plan, start, plan.work.starts[blockIdx.x + 1].at);
+  auto wait = [&](unsigned long long* bar, uint32_t parity) {
+    if (mbar_wait_bounded_warp(smem_u32(bar), parity, abort_flag, plan.wait_limit_ns)) return true;
+    if (lane == 0) atomicOr(a.status, kKvTimeout);
+    return false;
+  };
+  // Ring of K and V tiles, in the order in which the products take them: K0 K1 V0 K2 V1 .. V(n-2) V(n-1) of a segment.
+  auto ring_k = [](int first, int j) { return first + (j == 0 ? 0 : 2 * j - 1); };
+  auto ring_v = [](int first, int j, int n) { return first + (j + 1 < n ? 2 * j + 2 : 2 * n - 1); };
+
+  if (warp < 4) {
+    if (warp == 0) {
+      // ------------------------------ loads ------------------------------
+      const int boxes = (kKvTile >> shape.page_shift) * L::kPanels;     // of a tile; a lane each
+      const int my_page = lane / L::kPanels, my_panel = lane % L::kPanels;
+      int ring = 0;
+      bool alive = true;
+      while (alive && walk.next()) {
+        const int* table = a.batch.table + static_cast<size_t>(walk.sequence) * a.batch.columns;
+        const int pages = (walk.seq.length + shape.page_tokens - 1) >> shape.page_shift;
+        auto page_of = [&](int j) {          // of this lane's box; -1: behind the sequence's last
+          const int column = ((walk.tile0 + j) << (7 - shape.page_shift)) + my_page;
+          if (j >= walk.tiles || lane >= boxes || column >= pages) return -1;
+          int page = table[column];
+          if (page < 0 || page >= shape.pages) {
+            atomicOr(a.status, kKvBadBatch);
+            page = 0;                        // its positions are masked
+          }
+          return page;
+        };
+        auto issue = [&](bool is_k, int page) {
+          const int slot = ring % L::kSlots;
+          if (!wait(&sm.empty[slot], ((ring / L::kSlots) & 1) ^ 1)) return false;
+          const int loads = __popc(__ballot_sync(0xffffffffu, page >= 0));
+          if (lane == 0) mbar_arrive_expect_tx(smem_u32(&sm.full[slot]), loads * shape.page_tokens * L::kRowBytes);
+          __syncwarp();
+          if (page >= 0)
+            tma_load_2d(base + slot * L::kSlotBytes + my_panel * L::kPanelBytes + (my_page << shape.page_shift) * L::kRowBytes,
+                        is_k ? &maps.keys : &maps.values, my_panel * L::kRowBytes,
+                        static_cast<int>((static_cast<long long>(page) * shape.kv_heads + walk.head) << shape.page_shift),
+                        smem_u32(&sm.full[slot]));
+          __syncwarp();
+          ++ring;
+          return true;
+        };
+        int page = page_of(0), next = page_of(1);
+        alive = issue(true, page);
+        for (int j = 0; j < walk.tiles && alive; ++j) {
+          if (j + 1 < walk.tiles) alive = issue(true, next);
+          alive = alive && issue(false, page);
+          page = next;
+          next = page_of(j + 2);
+        }
+        walk.advance();
+      }
+      if (*abort_flag != 0) {              // what is in flight lands before the block leaves
+        volatile int ignore = 0;
+        for (int i = max(0, ring - L::kSlots); i < ring; ++i) mbar_wait_bounded(smem_u32(&sm.full[i % L::kSlots]), (i / L::kSlots) & 1, &ignore);
+      }
+    } else if (warp == 1) {
+      // ------------------------------ products ------------------------------
+      constexpr uint32_t kScoresHigh = instr_desc_f8(kE4m3, kE4m3, 0, 0, 128, kKvTile);
+      constexpr uint32_t kScoresLow = instr_desc_f8(kE5m2, kE4m3, 0, 0, 128, kKvTile);
+      constexpr uint32_t kSumsHigh = instr_desc_f8(kE4m3, kE4m3, 0, 1, 128, kDim);
+      constexpr uint32_t kSumsLow = instr_desc_f8(kE5m2, kE4m3, 0, 1, 128, kDim);
+      int ring = 0, tile = 0, segment = 0;
+      bool alive = true;
+      while (alive && walk.next()) {
+        const int n = walk.tiles;
+        auto scores = [&](int j) {
+          // the scores' buffer is free: the product that read the weights in it was issued before
+          const int r = ring_k(ring, j), slot = r % L::kSlots, buffer = (tile + j) & 1;
+          if (!wait(&sm.full[slot], (r / L::kSlots) & 1)) return false;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t k0 = base + slot * L::kSlotBytes, q0 = base + L::kQueryAt;
+#pragma unroll
+            for (int term = 0; term < 2; ++term) {
+#pragma unroll
+              for (int k = 0; k < kDim / 32; ++k) {
+                const int panel = k * 32 / L::kRowBytes, inside = k * 32 % L::kRowBytes;
+                umma_f8(tmem + L::kScoreColumn + buffer * 128,
+                        smem_desc_rows<L::kRowBytes>(q0 + term * L::kSlotBytes + panel * L::kPanelBytes) + (inside >> 4),
+                        smem_desc_rows<L::kRowBytes>(k0 + panel * L::kPanelBytes) + (inside >> 4), term == 0 ? kScoresHigh : kScoresLow,
+                        (term | k) != 0);
+              }
+            }
+            umma_commit(smem_u32(&sm.empty[slot]));
+            umma_commit(smem_u32(&sm.s_full[buffer]));
+          }
+          __syncwarp();
+          return true;
+        };
+        alive = wait(&sm.q_full, segment & 1) && scores(0);
+        for (int j = 0; j < n && alive; ++j) {
+          if (j + 1 < n && !scores(j + 1)) { alive = false; break; }
+          const int r = ring_v(ring, j, n), slot = r % L::kSlots, buffer = (tile + j) & 1;
+          if (!wait(&sm.p_full[buffer], ((tile + j) >> 1) & 1) || !wait(&sm.full[slot], (r / L::kSlots) & 1)) { alive = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t v0 = base + slot * L::kSlotBytes, w0 = tmem + L::kScoreColumn + buffer * 128;
+#pragma unroll
+            for (int term = 0; term < 2; ++term) {
+#pragma unroll
+              for (int k = 0; k < kKvTile / 32; ++k)
+                umma_f8_ts(tmem, w0 + k * 32 + term * 8, smem_desc_rows<L::kRowBytes>(v0 + k * 32 * L::kRowBytes, L::kPanelBytes),
+                           term == 0 ? kSumsHigh : kSumsLow, (j | term | k) != 0);
+            }
+            umma_commit(smem_u32(&sm.empty[slot]));
+            umma_commit(smem_u32(&sm.o_done[buffer]));
+          }
+          __syncwarp();
+        }
+        ring += 2 * n;
+        tile += n;
+        ++segment;
+        walk.advance();
+      }
+    } else if (warp == 3) {
+      // ------------------------------ scales ------------------------------
+      int tile = 0;
+      bool alive = true;
+      while (alive && walk.next()) {
+        const int* table = a.batch.table + static_cast<size_t>(walk.sequence) * a.batch.columns;
+        auto fetch = [&](int j) {            // lane g < 8: positions 16 g .. 16 g + 15 of the tile
+          const int position = (walk.tile0 + j) * kKvTile + 16 * lane;
+          float2 s = make_float2(0.0f, 1.0f);
+          if (j < walk.tiles && lane < 8 && position < walk.seq.length) {
+            const int page = table[position >> shape.page_shift];
+            if (page >= 0 && page < shape.pages) {
+              const size_t at = static_cast<size_t>(page) * shape.kv_heads + walk.head;
+              s = make_float2(a.layer.key_scales[at], a.layer.value_scales[at]);
+            }
+          }
+          return s;
+        };
+        float2 s = fetch(0);
+        for (int j = 0; j < walk.tiles; ++j, ++tile) {
+          const float2 after = fetch(j + 1);
+          const int slot = tile % kScaleSlots;
+          if (!wait(&sm.scales_empty[slot], ((tile / kScaleSlots) & 1) ^ 1)) { alive = false; break; }
+          // positions without a page are marked; their factor only has to be positive
+          if (lane < 8) sm.scales[slot][lane] = make_float4(s.x > 0.0f ? s.x * a.scale_log2 : 1.0f, log2f(s.y), __frcp_rn(s.y), s.x);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sm.scales_full[slot]));
+          s = after;
+        }
+        walk.advance();
+      }
+    }
+  } else {
+    // ------------------------------ softmax and results ------------------------------
+    const int group = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    int ring = 0, tile = 0, segment = 0;
+    // No wait that runs out leaves this loop: the warps meet at barriers, and every wait after the first that ran out ends at once.
+    while (walk.next()) {
+      const int n = walk.tiles;
+      const int rows = walk.unit.tokens * shape.group;
+      const int token0 = walk.seq.row0 + walk.row_tile * plan.tile_tokens;
+      // Queries: a warp takes every eighth row, eight at a time.
+      {
+        constexpr int kPer = kDim / 32;
+        const int w8 = warp - 4;
+#pragma unroll 1
+        for (int r0 = 0; r0 < 128; r0 += 64) {
+          uint32_t raw[8][kPer / 2];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = r0 + 8 * i + w8;
+            const int token = r / shape.group, g = r - token * shape.group;
+            const __nv_bfloat16* at = a.q.data + static_cast<long long>(token0 + token) * a.q.row_stride +
+                                      (walk.head * shape.group + g) * a.q.head_stride + lane * kPer;
+#pragma unroll
+            for (int e = 0; e < kPer / 2; ++e) raw[i][e] = 0;
+            if (r < rows) {
+              if constexpr (kPer == 8) {
+                const uint4 v = *reinterpret_cast<const uint4*>(at);
+                raw[i][0] = v.x; raw[i][1] = v.y; raw[i][2] = v.z; raw[i][3] = v.w;
+              } else if constexpr (kPer == 4) {
+                const uint2 v = *reinterpret_cast<const uint2*>(at);
+                raw[i][0] = v.x; raw[i][1] = v.y;
+              } else {
+                raw[i][0] = *reinterpret_cast<const uint32_t*>(at);
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = r0 + 8 * i + w8;
+            float top = 0.0f;
+            bool finite = true;
+#pragma unroll
+            for (int e = 0; e < kPer / 2; ++e) {
+              const float u = fabsf(bf16_lo(raw[i][e])), v = fabsf(bf16_hi(raw[i][e]));
+              finite = finite && u <= 3.402823466e38f && v <= 3.402823466e38f;
+              top = fmaxf(top, fmaxf(u, v));
+            }
+#pragma unroll
+            for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            finite = __all_sync(0xffffffffu, finite);
+            const int exponent = kv_scale_exponent(top);
+            const float inverse = kv_exp2(-exponent);
+            uint32_t hi[kPer / 2], lo[kPer / 2];
+#pragma unroll
+            for (int e = 0; e < kPer / 2; ++e) {
+              const float u = bf16_lo(raw[i][e]) * inverse, v = bf16_hi(raw[i][e]) * inverse;
+              hi[e] = cvt_e4m3x2(u, v);
+              const float2 back = e4m3x2_values(hi[e]);
+              lo[e] = cvt_e5m2x2(u - back.x, v - back.y);
+              if (!finite) {
+                hi[e] = kKvNan * 0x0101u;
+                lo[e] = 0;
+              }
+            }
+#pragma unroll
+            for (int term = 0; term < 2; ++term) {
+              const uint32_t* c = term == 0 ? hi : lo;
+              const int byte = lane * kPer, panel = byte / L::kRowBytes, inside = byte % L::kRowBytes;
+              const int piece = (inside >> 4) ^ (L::kRowBytes == 128 ? r & 7 : (r >> 1) & 3);
+              uint8_t* to = generic + L::kQueryAt + term * L::kSlotBytes + panel * L::kPanelBytes + r * L::kRowBytes + piece * 16 + (inside & 15);
+              if constexpr (kPer == 8) *reinterpret_cast<uint2*>(to) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+              else if constexpr (kPer == 4) *reinterpret_cast<uint32_t*>(to) = c[0] | (c[1] << 16);
+              else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(c[0]);
+            }
+            if (lane == 0) sm.row_scale[r] = kv_exp2(exponent);
+          }
+        }
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.q_full));
+        group_barrier();                   // row_scale
+      }
+      const float row_scale = sm.row_scale[row];
+      const int limit = row < rows ? walk.unit.first + row / shape.group : -1;     // last position the row sees
+      float top = -INFINITY, sum = 0.0f;                                           // this group's reference and sum
+      const int tile_first = tile;
+      for (int j = 0; j < n; ++j, ++tile) {
+        if ((tile & 1) != group) continue;
+        const int position0 = (walk.tile0 + j) * kKvTile;
+        const uint32_t scores = tmem + lanes + L::kScoreColumn + group * 128;
+        wait(&sm.scales_full[tile % kScaleSlots], (tile / kScaleSlots) & 1);
+        wait(&sm.s_full[group], (tile >> 1) & 1);
+        tc_fence_after();
+        const float4* scales = sm.scales[tile % kScaleSlots];
+        // the diagonal, the sequence's end, or a page that is not there: a bit for every position that counts
+        const bool masked = position0 + kKvTile - 1 > walk.unit.first || scales[0].w == 0.0f || scales[1].w == 0.0f || scales[2].w == 0.0f ||
+                            scales[3].w == 0.0f || scales[4].w == 0.0f || scales[5].w == 0.0f || scales[6].w == 0.0f || scales[7].w == 0.0f;
+        auto visible = [&](int chunk) {
+          uint32_t bits = 0xffffffffu;
+          const int seen = limit - position0 - 32 * chunk;               // last position of the chunk that the row sees
+          if (seen < 31) bits = seen < 0 ? 0u : (2u << seen) - 1u;
+          if (scales[2 * chunk].w == 0.0f) bits &= 0xffff0000u;
+          if (scales[2 * chunk + 1].w == 0.0f) bits &= 0x0000ffffu;
+          return bits;
+        };
+        auto mask = [&](int chunk, uint32_t* s) {
+          if (masked) {
+            const uint32_t bits = visible(chunk);
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (((bits >> c) & 1u) == 0u) s[c] = 0xff800000u;
+          }
+        };
+        // positive, so that a masked score stays -inf
+        auto factor_of = [&](float key) { return fmaxf(key * row_scale, 1.17549435e-38f); };
+        // The scores are read twice, for the maximum and for the weights, 32 at a time and the next 32 ahead: held between the
+        // two they would fill the registers.
+        float m = -INFINITY;
+        {
+          uint32_t s[2][32];
+          tmem_ld32(scores, s[0]);
+#pragma unroll
+          for (int chunk = 0; chunk < 4; ++chunk) {
+            uint32_t* now = s[chunk & 1];
+            tmem_ld_wait();
+            if (chunk < 3) tmem_ld32(scores + 32 * (chunk + 1), s[(chunk + 1) & 1]);
+            mask(chunk, now);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              float x = __uint_as_float(now[16 * g]);
+#pragma unroll
+              for (int c = 1; c < 16; ++c) x = fmaxf(x, __uint_as_float(now[16 * g + c]));
+              m = fmaxf(m, fmaf(x, factor_of(scales[2 * chunk + g].x), scales[2 * chunk + g].y));
+            }
+          }
+        }
+        float before = -INFINITY, peak = m;
+        if (tile != tile_first) {
+          wait(&sm.top_done[group ^ 1][quarter], ((tile - 1) >> 1) & 1);
+          const float2 x = sm.top[row];
+          before = x.x;
+          peak = fmaxf(peak, x.y);
+        }
+        float now = before;
+        if (m > before + kGrow || (before == -INFINITY && m > before)) now = m;
+        else if (m > -INFINITY && fmaxf(m, peak - kDepth) < before - kFall) now = fmaxf(m, peak - kDepth);
+        sm.top[row] = make_float2(now, peak);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.top_done[group][quarter]));
+        if (tile != tile_first && __any_sync(0xffffffffu, now != before)) {
+          wait(&sm.o_done[group ^ 1], ((tile - 1) >> 1) & 1);
+          tc_fence_after();
+          const float f = now != before ? fast_exp2(before - now) : 1.0f;
+#pragma unroll 1
+          for (int c = 0; c < kDim; c += 8) {
+            uint32_t o[8];
+            tmem_ld8(tmem + lanes + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st8(tmem + lanes + c, o);
+          }
+          tmem_st_wait();
+        }
+        if (top != now) {
+          sum *= fast_exp2(top - now);     // top is -inf at first: 0
+          top = now;
+        }
+        const float shift = kWeightExponent - (now == -INFINITY ? 0.0f : now);
+        {
+          uint32_t s[2][32];
+          tmem_ld32(scores, s[0]);
+#pragma unroll
+          for (int chunk = 0; chunk < 4; ++chunk) {
+            uint32_t* at = s[chunk & 1];
+            tmem_ld_wait();
+            if (chunk < 3) tmem_ld32(scores + 32 * (chunk + 1), s[(chunk + 1) & 1]);
+            mask(chunk, at);
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const float4 scale = scales[2 * chunk + g];
+              const float factor = factor_of(scale.x), offset = scale.y + shift;
+              float part = 0.0f;
+#pragma unroll
+              for (int c = 0; c < 16; c += 4) {
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  w[i] = fast_exp2(fmaf(__uint_as_float(at[16 * g + c + i]), factor, offset));
+                  part += w[i];
+                }
+                const uint32_t h0 = cvt_f16x2(w[0], w[1]), h1 = cvt_f16x2(w[2], w[3]);
+                const uint32_t c0 = cvt_e4m3x2_f16x2(h0), c1 = cvt_e4m3x2_f16x2(h1);
+                const uint32_t l0 = cvt_e5m2x2_f16x2(sub_f16x2(h0, e4m3x2_f16x2(c0))), l1 = cvt_e5m2x2_f16x2(sub_f16x2(h1, e4m3x2_f16x2(c1)));
+                hi[4 * g + c / 4] = c0 | (c1 << 16);
+                lo[4 * g + c / 4] = l0 | (l1 << 16);
+              }
+              sum = fmaf(part, scale.z, sum);
+            }
+            // where the scores of these 32 positions lay
+            tmem_st8(scores + 32 * chunk, hi);
+            tmem_st8(scores + 32 * chunk + 8, lo);
+          }
+        }
+        tmem_st_wait();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.scales_empty[tile % kScaleSlots]));
+        if (position0 + kKvTile > walk.seq.length) {
+          // behind the sequence's end a page can hold anything, and zero weights do not stop a NaN
+          const int r = ring_v(ring, j, n), slot = r % L::kSlots;
+          wait(&sm.full[slot], (r / L::kSlots) & 1);
+          if (position0 + row >= walk.seq.length) {
+#pragma unroll
+            for (int c = 0; c < kDim / 16; ++c)
+              *reinterpret_cast<uint4*>(generic + slot * L::kSlotBytes + (c * 16 / L::kRowBytes) * L::kPanelBytes + row * L::kRowBytes +
+                                        c * 16 % L::kRowBytes) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async_proxy();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[group]));
+      }
+      // the unit's sums, or this block's part of them; each group has half of the columns
+      sm.sum[group][row] = sum;
+      sm.group_top[group][row] = top;
+      group_barrier();
+      wait(&sm.o_done[(tile - 1) & 1], ((tile - 1) >> 1) & 1);
+      tc_fence_after();
+      const float last = sm.top[row].x;
+      float total = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float t = sm.group_top[i][row], x = sm.sum[i][row];
+        total += t == last ? x : x * fast_exp2(t - last);
+      }
+      const bool whole = n == walk.unit.tiles;
+      const int part = 2 * blockIdx.x + (walk.tile0 == 0 ? 1 : 0);
+      if (!whole && group == 0) plan.work.weights[static_cast<size_t>(part) * plan.work.rows_per_part + row] = make_float2(last, total);
+      const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+      const int token = row / shape.group, g = row - token * shape.group;
+      __nv_bfloat16* out = a.out + (static_cast<long long>(token0 + token) * shape.q_heads + walk.head * shape.group + g) * kDim;
+      float* sums = plan.work.sums + static_cast<size_t>(part) * plan.work.rows_per_part * kDim;
+#pragma unroll 1
+      for (int c = group * (kDim / 2); c < (group + 1) * (kDim / 2); c += 8) {
+        uint32_t o[8];
+        tmem_ld8(tmem + lanes + c, o);
+        tmem_ld_wait();
+        if (whole) {
+          uint32_t packed[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            packed[i] = static_cast<uint32_t>(float_to_bf16_bits(__uint_as_float(o[2 * i]) * inverse)) |
+                        (static_cast<uint32_t>(float_to_bf16_bits(__uint_as_float(o[2 * i + 1]) * inverse)) << 16);
+          if (row < rows) *reinterpret_cast<uint4*>(out + c) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+        } else {
+          // [head_dim / 4][rows][4]: a warp writes whole lines
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint4*>(sums + (static_cast<size_t>(c / 4 + i) * plan.work.rows_per_part + row) * 4) =
+                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      tc_fence_before();
+      group_barrier();                     // what the groups share of this segment has been read
+      ring += 2 * n;
+      ++segment;
+      walk.advance();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) {
+    // a wait ran out: the copies have been waited for above, and so are the products under way, by a last commit
+    volatile int ignore = 0;
+    if (warp == 1 && elect_one()) umma_commit(smem_u32(&sm.drain));
+    if (threadIdx.x == 0) mbar_wait_bounded(smem_u32(&sm.drain), 0, &ignore);
+    __syncthreads();
+  }
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of the units that a cut divides.  Block (c, slice): the unit that cut c divides, if no earlier cut does;
+// eight rows of it.
+template <int kDim>
+__global__ void __launch_bounds__(256)
+kv_prompt_join_kernel(const KvAttentionPlan plan) {
+  __shared__ float weight[kKvMaxBlocks][8];
+  __shared__ float total_s[8];
+  pdl_enter();
+  const KvAttention& a = plan.a;
+  const int cut = blockIdx.x + 1, row0 = blockIdx.y * 8;
+  const KvStart start = plan.work.starts[cut];
+  const KvSequence seq = kv_sequence(a.batch, a.shape, start.sequence);
+  const KvUnit unit = kv_unit(seq, start.row_tile, plan.tile_tokens);
+  const int rows = unit.tokens * a.shape.group;
+  if (start.tile == 0 || start.tile >= unit.tiles || row0 >= rows) return;
+  const long long first = start.at - start.tile, end = first + unit.tiles;
+  if (plan.work.starts[cut - 1].at > first) return;            // an earlier cut's
+  // Parts: block cut - 1 begins the unit; then every block that begins inside it.  Empty shares left none.
+  int last = cut;
+  while (last < plan.blocks && plan.work.starts[last + 1].at < end) ++last;
+  const int parts = last - cut + 2;
+  auto part_of = [&](int p) { return 2 * (cut - 1 + p) + (p == 0 ? 1 : 0); };
+  auto empty = [&](int p) { return p > 0 && plan.work.starts[cut - 1 + p].at == plan.work.starts[cut + p].at; };
+  const int thread = threadIdx.x;
+  if (thread < 8) {
+    float top = -INFINITY, total = 0.0f;
+    for (int p = 0; p < parts; ++p)
+      if (!empty(p)) top = fmaxf(top, plan.work.weights[static_cast<size_t>(part_of(p)) * plan.work.rows_per_part + row0 + thread].x);
+    for (int p = 0; p < parts; ++p) {
+      float w = 0.0f;
+      if (!empty(p)) {
+        const float2 x = plan.work.weights[static_cast<size_t>(part_of(p)) * plan.work.rows_per_part + row0 + thread];
+        // a part without a maximum has seen nothing, or nothing but NaN
+        w = exp2f(x.x - (top == -INFINITY ? 0.0f : top));
+        total += x.x == -INFINITY ? x.y : x.y * w;
+      }
+      weight[p][thread] = w;
+    }
+    total_s[thread] = total;
+  }
+  __syncthreads();
+  const int r = thread & 7, row = row0 + r;
+  if (row >= rows) return;
+  const float inverse = total_s[r] == 0.0f ? 0.0f : 1.0f / total_s[r];
+  const int token = row / a.shape.group, g = row - token * a.shape.group;
+  __nv_bfloat16* out = a.out + (static_cast<long long>(seq.row0 + start.row_tile * plan.tile_tokens + token) * a.shape.q_heads +
+                                start.head * a.shape.group + g) * kDim;
+  for (int d = thread >> 3; d < kDim / 4; d += 32) {
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = 0; p < parts; ++p) {
+      if (empty(p)) continue;
+      const float4 x = *reinterpret_cast<const float4*>(plan.work.sums + static_cast<size_t>(part_of(p)) * plan.work.rows_per_part * kDim +
+                                                        (static_cast<size_t>(d) * plan.work.rows_per_part + row) * 4);
+      const float w = weight[p][r];
+      acc.x = fmaf(x.x, w, acc.x);
+      acc.y = fmaf(x.y, w, acc.y);
+      acc.z = fmaf(x.z, w, acc.z);
+      acc.w = fmaf(x.w, w, acc.w);
+    }
+    uint2 w;
+    w.x = static_cast<uint32_t>(float_to_bf16_bits(acc.x * inverse)) | (static_cast<uint32_t>(float_to_bf16_bits(acc.y * inverse)) << 16);
+    w.y = static_cast<uint32_t>(float_to_bf16_bits(acc.z * inverse)) | (static_cast<uint32_t>(float_to_bf16_bits(acc.w * inverse)) << 16);
+    *reinterpret_cast<uint2*>(out + 4 * d) = w;
+  }
+}
+
+template <int kDim>
+cudaError_t launch(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
+  constexpr int bytes = Prompt<kDim>::kSmallAt + static_cast<int>(sizeof(Small)) + 1024;
+  static_assert(bytes <= 227 * 1024, "more shared memory than a block can have");
+  cudaError_t error = opt_in_dynamic_smem<kv_prompt_kernel<kDim>>(bytes);
+  if (error == cudaSuccess) error = launch_pdl(kv_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, plan);
+  if (error == cudaSuccess) error = launch_pdl(kv_prompt_kernel<kDim>, dim3(plan.blocks), dim3(kThreads), bytes, stream, maps, plan);
+  if (error == cudaSuccess && plan.blocks > 1)
+    error = launch_pdl(kv_prompt_join_kernel<kDim>, dim3(plan.blocks - 1, kKvTile / 8), dim3(256), 0, stream, plan);
+  return error;
+}
+
+}  // namespace
+
+cudaError_t kv_prompt(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
+  switch (plan.a.shape.head_dim) {
+    case 64: return launch<64>(plan, maps, stream);
+    case 128: return launch<128>(plan, maps, stream);
+    default: return launch<256>(plan, maps, stream);
+  }
+}
+
+}  // namespace aima
