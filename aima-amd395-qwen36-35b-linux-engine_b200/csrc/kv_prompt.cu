@@ -9,26 +9,29 @@
 // cache is e4m3, and no operand of mixed width exists; unpacking K and V would cost conversions and shared memory per tile,
 // so Q and the weights are split into two 8-bit terms instead and the products run twice at twice the rate:
 //   q 2^-e  = hi (e4m3) + lo (e5m2)          exact down to 2^-16 (largest 448)
-//   w 2^7   = hi (e4m3) + lo (e5m2)          to 2^-8 of itself, down to 2^-16
+//   w 2^7   = hi (e4m3) + lo (e5m2)          to 2^-8 of itself where it exceeds 2^-6, to 2^-13 below
+//           = three terms (e5m2)             to 2^-9 of itself where it exceeds 2^-8, to 2^-17 below
 // both terms into the same accumulator.  S[128 rows, 128 positions] = Q K^T with both operands in shared memory;
 // O[128, head_dim] += W V with W in tensor memory, where it takes the place of the scores it was made from, and V MN-major.
 //
 // One block per SM.  Warp 0 loads tiles by page, warp 1 issues the products, warp 3 fetches the scales; warps 4-7 and 8-11 (thread =
-// row) take turns with the tiles: while one group turns the scores of a tile into weights the other waits for the next
-// tile's scores or has just stored its weights.  What passes between them is the reference maximum of each row, warp by warp.
+// row) each turn half of a tile's scores into weights and agree on the maximum in between.  The scores are double-buffered: the
+// products of one tile run under the softmax of another.
 #include "kv_attention.cuh"
 
-#include <cuda_fp16.h>
+#include <type_traits>
 
 namespace aima {
 namespace {
 
 constexpr int kThreads = 384;
 // The reference of a row's weights moves up when a tile's maximum exceeds it by more than kGrow, and down when a tile's maximum
-// falls short of it by more than kFall: small weights have few bits, and where one position outweighs all others by 2^14
-// and brings nothing (a sink), they are the result.  It stays within kDepth of the row's maximum so that nothing overflows.
+// falls short of it by more than kFall: small weights have few bits, and where one position outweighs all others and brings
+// nothing (a sink), they are the result.  It stays within kDepth of the row's maximum so that nothing overflows.  A tile in
+// which some row's maximum is more than kLow below its reference is a low one: its weights are held by three e5m2 terms.
 constexpr float kGrow = 1.75f;            // 2^7 * 2^1.75 = 430 <= 448
-constexpr float kFall = 8.0f;
+constexpr float kLow = 8.0f;
+constexpr float kFall = 16.0f;
 constexpr float kDepth = 30.0f;
 constexpr float kWeightExponent = 7.0f;
 constexpr int kScaleSlots = 4;
@@ -46,12 +49,14 @@ struct Prompt {
 };
 
 struct Small {
-  float4 scales[kScaleSlots][8];           // per 16 positions: key scale x softmax scale, log2 and inverse of the value scale
+  float4 scales[kScaleSlots][8];           // per 16 positions: key scale x softmax scale, log2 and inverse of the value scale, 0: no page
+  int holes[kScaleSlots];                  // whether a page of the tile is missing
+  int low[2];                              // whether the tile's weights are three e5m2 terms
   unsigned long long full[8], empty[8], scales_full[kScaleSlots], scales_empty[kScaleSlots];
-  unsigned long long s_full[2], p_full[2], o_done[2], top_done[2][4], q_full, drain;
+  unsigned long long s_full[2], p_full[2], o_done[2], q_full, drain;
   float row_scale[128];
-  float2 top[128];                         // per row: the reference, and the maximum so far
-  float sum[2][128], group_top[2][128];
+  float half_top[2][2][128];               // per tile parity, half and row
+  float sum[2][128];
   uint32_t tmem;
   int abort_flag;
 };
@@ -103,6 +108,32 @@ struct Walk {
 };
 
 __device__ __forceinline__ void group_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ bool group_any(bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any) : "r"(static_cast<uint32_t>(mine)) : "memory");
+  return any != 0;
+}
+// Four weights as f16 pairs -> four codes of each term; e5m2 is the upper byte of an f16.
+template <bool kLowTile>
+__device__ __forceinline__ void split_weights(uint32_t h0, uint32_t h1, uint32_t* terms, int stride) {
+  constexpr uint32_t kHalf = 0x00800080u;
+  if (kLowTile) {
+#pragma unroll
+    for (int term = 0; term < 3; ++term) {
+      const uint32_t u0 = h0 + kHalf, u1 = h1 + kHalf;
+      terms[term * stride] = __byte_perm(u0, u1, 0x7531);
+      h0 = sub_f16x2(h0, u0 & 0xff00ff00u);
+      h1 = sub_f16x2(h1, u1 & 0xff00ff00u);
+    }
+  } else {
+    const uint32_t c0 = cvt_e4m3x2_f16x2(h0), c1 = cvt_e4m3x2_f16x2(h1);
+    terms[0] = __byte_perm(c0, c1, 0x5410);
+    terms[stride] = __byte_perm(sub_f16x2(h0, e4m3x2_f16x2(c0)) + kHalf, sub_f16x2(h1, e4m3x2_f16x2(c1)) + kHalf, 0x7531);
+  }
+}
 
 // Cuts the list into `blocks` shares.  The list runs over sequences, their row tiles, the key/value heads and the tiles of the
 // cache.  A cut that falls near the end of a unit moves there: a divided unit costs its two blocks a write of 128 x head_dim
@@ -227,13 +258,12 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
     }
     for (int s = 0; s < kScaleSlots; ++s) {
       mbar_init(smem_u32(&sm.scales_full[s]), 1);
-      mbar_init(smem_u32(&sm.scales_empty[s]), 4);
+      mbar_init(smem_u32(&sm.scales_empty[s]), 8);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&sm.s_full[i]), 1);
-      mbar_init(smem_u32(&sm.p_full[i]), 4);
+      mbar_init(smem_u32(&sm.p_full[i]), 8);
       mbar_init(smem_u32(&sm.o_done[i]), 1);
-      for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&sm.top_done[i][q]), 1);
     }
     mbar_init(smem_u32(&sm.q_full), 8);
     mbar_init(smem_u32(&sm.drain), 1);
@@ -312,8 +342,8 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
       // ------------------------------ products ------------------------------
       constexpr uint32_t kScoresHigh = instr_desc_f8(kE4m3, kE4m3, 0, 0, 128, kKvTile);
       constexpr uint32_t kScoresLow = instr_desc_f8(kE5m2, kE4m3, 0, 0, 128, kKvTile);
-      constexpr uint32_t kSumsHigh = instr_desc_f8(kE4m3, kE4m3, 0, 1, 128, kDim);
-      constexpr uint32_t kSumsLow = instr_desc_f8(kE5m2, kE4m3, 0, 1, 128, kDim);
+      constexpr uint32_t kSumsE4m3 = instr_desc_f8(kE4m3, kE4m3, 0, 1, 128, kDim);
+      constexpr uint32_t kSumsE5m2 = instr_desc_f8(kE5m2, kE4m3, 0, 1, 128, kDim);
       int ring = 0, tile = 0, segment = 0;
       bool alive = true;
       while (alive && walk.next()) {
@@ -348,14 +378,16 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
           const int r = ring_v(ring, j, n), slot = r % L::kSlots, buffer = (tile + j) & 1;
           if (!wait(&sm.p_full[buffer], ((tile + j) >> 1) & 1) || !wait(&sm.full[slot], (r / L::kSlots) & 1)) { alive = false; break; }
           tc_fence_after();
+          const bool low = *reinterpret_cast<volatile int*>(&sm.low[buffer]) != 0;
           if (elect_one()) {
             const uint32_t v0 = base + slot * L::kSlotBytes, w0 = tmem + L::kScoreColumn + buffer * 128;
 #pragma unroll
-            for (int term = 0; term < 2; ++term) {
+            for (int term = 0; term < 3; ++term) {
+              if (term == 2 && !low) break;
 #pragma unroll
               for (int k = 0; k < kKvTile / 32; ++k)
                 umma_f8_ts(tmem, w0 + k * 32 + term * 8, smem_desc_rows<L::kRowBytes>(v0 + k * 32 * L::kRowBytes, L::kPanelBytes),
-                           term == 0 ? kSumsHigh : kSumsLow, (j | term | k) != 0);
+                           term == 0 && !low ? kSumsE4m3 : kSumsE5m2, (j | term | k) != 0);
             }
             umma_commit(smem_u32(&sm.empty[slot]));
             umma_commit(smem_u32(&sm.o_done[buffer]));
@@ -391,6 +423,9 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
           const int slot = tile % kScaleSlots;
           if (!wait(&sm.scales_empty[slot], ((tile / kScaleSlots) & 1) ^ 1)) { alive = false; break; }
           // positions without a page are marked; their factor only has to be positive
+          const bool hole = lane < 8 && s.x == 0.0f;
+          const uint32_t holes = __ballot_sync(0xffffffffu, hole);
+          if (lane == 0) sm.holes[slot] = static_cast<int>(holes);
           if (lane < 8) sm.scales[slot][lane] = make_float4(s.x > 0.0f ? s.x * a.scale_log2 : 1.0f, log2f(s.y), __frcp_rn(s.y), s.x);
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&sm.scales_full[slot]));
@@ -484,162 +519,130 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
       }
       const float row_scale = sm.row_scale[row];
       const int limit = row < rows ? walk.unit.first + row / shape.group : -1;     // last position the row sees
-      float top = -INFINITY, sum = 0.0f;                                           // this group's reference and sum
-      const int tile_first = tile;
+      float top = -INFINITY, peak = -INFINITY, sum = 0.0f;       // reference and maximum so far; this half's sum of weights
       for (int j = 0; j < n; ++j, ++tile) {
-        if ((tile & 1) != group) continue;
+        const int buffer = tile & 1, slot = tile % kScaleSlots;
         const int position0 = (walk.tile0 + j) * kKvTile;
-        const uint32_t scores = tmem + lanes + L::kScoreColumn + group * 128;
-        wait(&sm.scales_full[tile % kScaleSlots], (tile / kScaleSlots) & 1);
-        wait(&sm.s_full[group], (tile >> 1) & 1);
+        const uint32_t scores = tmem + lanes + L::kScoreColumn + buffer * 128 + group * 64;
+        wait(&sm.scales_full[slot], (tile / kScaleSlots) & 1);
+        wait(&sm.s_full[buffer], (tile >> 1) & 1);
         tc_fence_after();
-        const float4* scales = sm.scales[tile % kScaleSlots];
-        // the diagonal, the sequence's end, or a page that is not there: a bit for every position that counts
-        const bool masked = position0 + kKvTile - 1 > walk.unit.first || scales[0].w == 0.0f || scales[1].w == 0.0f || scales[2].w == 0.0f ||
-                            scales[3].w == 0.0f || scales[4].w == 0.0f || scales[5].w == 0.0f || scales[6].w == 0.0f || scales[7].w == 0.0f;
-        auto visible = [&](int chunk) {
-          uint32_t bits = 0xffffffffu;
-          const int seen = limit - position0 - 32 * chunk;               // last position of the chunk that the row sees
-          if (seen < 31) bits = seen < 0 ? 0u : (2u << seen) - 1u;
-          if (scales[2 * chunk].w == 0.0f) bits &= 0xffff0000u;
-          if (scales[2 * chunk + 1].w == 0.0f) bits &= 0x0000ffffu;
-          return bits;
-        };
-        auto mask = [&](int chunk, uint32_t* s) {
-          if (masked) {
-            const uint32_t bits = visible(chunk);
+        uint32_t s[64];
+        tmem_ld32(scores, s);
+        tmem_ld32(scores + 32, s + 32);
+        const float4* scales = sm.scales[slot] + 4 * group;
+        const bool masked = position0 + kKvTile - 1 > walk.unit.first || sm.holes[slot] != 0;
+        float factor[4], offset[4];
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (((bits >> c) & 1u) == 0u) s[c] = 0xff800000u;
-          }
-        };
-        // positive, so that a masked score stays -inf
-        auto factor_of = [&](float key) { return fmaxf(key * row_scale, 1.17549435e-38f); };
-        // The scores are read twice, for the maximum and for the weights, 32 at a time and the next 32 ahead: held between the
-        // two they would fill the registers.
+        for (int g = 0; g < 4; ++g) {
+          factor[g] = fmaxf(scales[g].x * row_scale, 1.17549435e-38f);         // positive, so that a masked score stays -inf
+          offset[g] = scales[g].y;
+        }
+        tmem_ld_wait();
+        if (masked) {
+          // the diagonal, the sequence's end, or a page that is not there
+          const int seen = limit - position0 - 64 * group;                     // last of these positions that the row sees
+          const int holes = sm.holes[slot] >> (4 * group);
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c > seen || ((holes >> (c / 16)) & 1) != 0) s[c] = 0xff800000u;
+        }
         float m = -INFINITY;
-        {
-          uint32_t s[2][32];
-          tmem_ld32(scores, s[0]);
 #pragma unroll
-          for (int chunk = 0; chunk < 4; ++chunk) {
-            uint32_t* now = s[chunk & 1];
-            tmem_ld_wait();
-            if (chunk < 3) tmem_ld32(scores + 32 * (chunk + 1), s[(chunk + 1) & 1]);
-            mask(chunk, now);
+        for (int g = 0; g < 4; ++g) {
+          float x = __uint_as_float(s[16 * g]), y = __uint_as_float(s[16 * g + 1]);
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              float x = __uint_as_float(now[16 * g]);
-#pragma unroll
-              for (int c = 1; c < 16; ++c) x = fmaxf(x, __uint_as_float(now[16 * g + c]));
-              m = fmaxf(m, fmaf(x, factor_of(scales[2 * chunk + g].x), scales[2 * chunk + g].y));
-            }
+          for (int c = 2; c < 16; c += 4) {
+            x = fmaxf(fmaxf(x, __uint_as_float(s[16 * g + c])), __uint_as_float(s[16 * g + c + 1]));
+            if (c + 2 < 16) y = fmaxf(fmaxf(y, __uint_as_float(s[16 * g + c + 2])), __uint_as_float(s[16 * g + c + 3]));
           }
+          m = fmaxf(m, fmaf(fmaxf(x, y), factor[g], offset[g]));
         }
-        float before = -INFINITY, peak = m;
-        if (tile != tile_first) {
-          wait(&sm.top_done[group ^ 1][quarter], ((tile - 1) >> 1) & 1);
-          const float2 x = sm.top[row];
-          before = x.x;
-          peak = fmaxf(peak, x.y);
-        }
-        float now = before;
-        if (m > before + kGrow || (before == -INFINITY && m > before)) now = m;
-        else if (m > -INFINITY && fmaxf(m, peak - kDepth) < before - kFall) now = fmaxf(m, peak - kDepth);
-        sm.top[row] = make_float2(now, peak);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.top_done[group][quarter]));
-        if (tile != tile_first && __any_sync(0xffffffffu, now != before)) {
-          wait(&sm.o_done[group ^ 1], ((tile - 1) >> 1) & 1);
+        sm.half_top[buffer][group][row] = m;
+        group_barrier();
+        m = fmaxf(m, sm.half_top[buffer][group ^ 1][row]);
+        peak = fmaxf(peak, m);
+        float now = top;
+        if (m > top + kGrow || (top == -INFINITY && m > top)) now = m;
+        else if (m > -INFINITY && fmaxf(m, peak - kDepth) < top - kFall) now = fmaxf(m, peak - kDepth);
+        const bool low = group_any(m > -INFINITY && m < now - kLow);
+        if (threadIdx.x == 128) sm.low[buffer] = low ? 1 : 0;
+        if (j > 0 && __any_sync(0xffffffffu, now != top)) {
+          wait(&sm.o_done[buffer ^ 1], ((tile - 1) >> 1) & 1);
           tc_fence_after();
-          const float f = now != before ? fast_exp2(before - now) : 1.0f;
+          const float f = now != top ? fast_exp2(top - now) : 1.0f;
 #pragma unroll 1
-          for (int c = 0; c < kDim; c += 8) {
-            uint32_t o[8];
-            tmem_ld8(tmem + lanes + c, o);
+          for (int c = group * (kDim / 2); c < (group + 1) * (kDim / 2); c += 32) {
+            uint32_t o[32];
+            tmem_ld32(tmem + lanes + c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st8(tmem + lanes + c, o);
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st32(tmem + lanes + c, o);
           }
-          tmem_st_wait();
         }
-        if (top != now) {
+        if (now != top) {
           sum *= fast_exp2(top - now);     // top is -inf at first: 0
           top = now;
         }
         const float shift = kWeightExponent - (now == -INFINITY ? 0.0f : now);
-        {
-          uint32_t s[2][32];
-          tmem_ld32(scores, s[0]);
+        auto weights = [&](auto low_tile) {
 #pragma unroll
-          for (int chunk = 0; chunk < 4; ++chunk) {
-            uint32_t* at = s[chunk & 1];
-            tmem_ld_wait();
-            if (chunk < 3) tmem_ld32(scores + 32 * (chunk + 1), s[(chunk + 1) & 1]);
-            mask(chunk, at);
-            uint32_t hi[8], lo[8];
+          for (int chunk = 0; chunk < 2; ++chunk) {
+            uint32_t terms[24];
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-              const float4 scale = scales[2 * chunk + g];
-              const float factor = factor_of(scale.x), offset = scale.y + shift;
+              const float at = offset[2 * chunk + g] + shift;
               float part = 0.0f;
 #pragma unroll
               for (int c = 0; c < 16; c += 4) {
                 float w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  w[i] = fast_exp2(fmaf(__uint_as_float(at[16 * g + c + i]), factor, offset));
+                  w[i] = fast_exp2(fmaf(__uint_as_float(s[32 * chunk + 16 * g + c + i]), factor[2 * chunk + g], at));
                   part += w[i];
                 }
-                const uint32_t h0 = cvt_f16x2(w[0], w[1]), h1 = cvt_f16x2(w[2], w[3]);
-                const uint32_t c0 = cvt_e4m3x2_f16x2(h0), c1 = cvt_e4m3x2_f16x2(h1);
-                const uint32_t l0 = cvt_e5m2x2_f16x2(sub_f16x2(h0, e4m3x2_f16x2(c0))), l1 = cvt_e5m2x2_f16x2(sub_f16x2(h1, e4m3x2_f16x2(c1)));
-                hi[4 * g + c / 4] = c0 | (c1 << 16);
-                lo[4 * g + c / 4] = l0 | (l1 << 16);
+                split_weights<decltype(low_tile)::value>(cvt_f16x2(w[0], w[1]), cvt_f16x2(w[2], w[3]), terms + 4 * g + c / 4, 8);
               }
-              sum = fmaf(part, scale.z, sum);
+              sum = fmaf(part, scales[2 * chunk + g].z, sum);
             }
             // where the scores of these 32 positions lay
-            tmem_st8(scores + 32 * chunk, hi);
-            tmem_st8(scores + 32 * chunk + 8, lo);
+            tmem_st8(scores + 32 * chunk, terms);
+            tmem_st8(scores + 32 * chunk + 8, terms + 8);
+            if (decltype(low_tile)::value) tmem_st8(scores + 32 * chunk + 16, terms + 16);
           }
-        }
+        };
+        if (low) weights(std::true_type{}); else weights(std::false_type{});
         tmem_st_wait();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.scales_empty[tile % kScaleSlots]));
+        if (lane == 0) mbar_arrive(smem_u32(&sm.scales_empty[slot]));
         if (position0 + kKvTile > walk.seq.length) {
           // behind the sequence's end a page can hold anything, and zero weights do not stop a NaN
-          const int r = ring_v(ring, j, n), slot = r % L::kSlots;
-          wait(&sm.full[slot], (r / L::kSlots) & 1);
+          const int r = ring_v(ring, j, n), ring_slot = r % L::kSlots;
+          wait(&sm.full[ring_slot], (r / L::kSlots) & 1);
           if (position0 + row >= walk.seq.length) {
 #pragma unroll
-            for (int c = 0; c < kDim / 16; ++c)
-              *reinterpret_cast<uint4*>(generic + slot * L::kSlotBytes + (c * 16 / L::kRowBytes) * L::kPanelBytes + row * L::kRowBytes +
+            for (int i = 0; i < kDim / 32; ++i) {
+              const int c = group * (kDim / 32) + i;
+              *reinterpret_cast<uint4*>(generic + ring_slot * L::kSlotBytes + (c * 16 / L::kRowBytes) * L::kPanelBytes + row * L::kRowBytes +
                                         c * 16 % L::kRowBytes) = make_uint4(0, 0, 0, 0);
+            }
           }
           fence_async_proxy();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[group]));
+        if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[buffer]));
       }
       // the unit's sums, or this block's part of them; each group has half of the columns
       sm.sum[group][row] = sum;
-      sm.group_top[group][row] = top;
       group_barrier();
       wait(&sm.o_done[(tile - 1) & 1], ((tile - 1) >> 1) & 1);
       tc_fence_after();
-      const float last = sm.top[row].x;
-      float total = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float t = sm.group_top[i][row], x = sm.sum[i][row];
-        total += t == last ? x : x * fast_exp2(t - last);
-      }
+      const float total = sm.sum[0][row] + sm.sum[1][row];
       const bool whole = n == walk.unit.tiles;
       const int part = 2 * blockIdx.x + (walk.tile0 == 0 ? 1 : 0);
-      if (!whole && group == 0) plan.work.weights[static_cast<size_t>(part) * plan.work.rows_per_part + row] = make_float2(last, total);
+      if (!whole && group == 0) plan.work.weights[static_cast<size_t>(part) * plan.work.rows_per_part + row] = make_float2(top, total);
       const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
       const int token = row / shape.group, g = row - token * shape.group;
       __nv_bfloat16* out = a.out + (static_cast<long long>(token0 + token) * shape.q_heads + walk.head * shape.group + g) * kDim;
