@@ -9,31 +9,29 @@
 // cache is e4m3, and no operand of mixed width exists; unpacking K and V would cost conversions and shared memory per tile,
 // so Q and the weights are split into two 8-bit terms instead and the products run twice at twice the rate:
 //   q 2^-e  = hi (e4m3) + lo (e5m2)          exact down to 2^-16 (largest 448)
-//   w 2^7   = hi (e4m3) + lo (e5m2)          to 2^-8 of itself where it exceeds 2^-6, to 2^-13 below
-//           = three terms (e5m2)             to 2^-9 of itself where it exceeds 2^-8, to 2^-17 below
-// both terms into the same accumulator.  S[128 rows, 128 positions] = Q K^T with both operands in shared memory;
+//   w 2^9   = three terms (e5m2)             to 2^-8 of itself where it exceeds 2^-9 (2^-18 of the largest), to 2^-17 below
+// An e5m2 number is the upper byte of an f16, so the weights' terms take no conversions; two terms with an e4m3 first one would
+// take a fifth less of the tensor cores but hold weights below 2^-13 of the largest to a few bits only, which is not enough where
+// one position outweighs all others and brings nothing.
+// All terms of an operand go into one accumulator.  S[128 rows, 128 positions] = Q K^T with both operands in shared memory;
 // O[128, head_dim] += W V with W in tensor memory, where it takes the place of the scores it was made from, and V MN-major.
 //
 // One block per SM.  Warp 0 loads tiles by page, warp 1 issues the products, warp 3 fetches the scales; warps 4-7 and 8-11 (thread =
-// row) each turn half of a tile's scores into weights and agree on the maximum in between.  The scores are double-buffered: the
-// products of one tile run under the softmax of another.
+// row) each turn half of a tile's scores into weights; two warps with the same rows exchange their maxima in between.
+// The scores are double-buffered: the products of one tile run under the softmax of another.
 #include "kv_attention.cuh"
-
-#include <type_traits>
 
 namespace aima {
 namespace {
 
 constexpr int kThreads = 384;
 // The reference of a row's weights moves up when a tile's maximum exceeds it by more than kGrow, and down when a tile's maximum
-// falls short of it by more than kFall: small weights have few bits, and where one position outweighs all others and brings
-// nothing (a sink), they are the result.  It stays within kDepth of the row's maximum so that nothing overflows.  A tile in
-// which some row's maximum is more than kLow below its reference is a low one: its weights are held by three e5m2 terms.
-constexpr float kGrow = 1.75f;            // 2^7 * 2^1.75 = 430 <= 448
-constexpr float kLow = 8.0f;
+// falls short of it by more than kFall, where the weights get few bits.  It stays within kDepth of the row's maximum so that
+// nothing overflows.
+constexpr float kGrow = 6.75f;            // 2^9 * 2^6.75 = 55109 <= 57344
 constexpr float kFall = 16.0f;
 constexpr float kDepth = 30.0f;
-constexpr float kWeightExponent = 7.0f;
+constexpr float kWeightExponent = 9.0f;
 constexpr int kScaleSlots = 4;
 
 template <int kDim>
@@ -51,7 +49,6 @@ struct Prompt {
 struct Small {
   float4 scales[kScaleSlots][8];           // per 16 positions: key scale x softmax scale, log2 and inverse of the value scale, 0: no page
   int holes[kScaleSlots];                  // whether a page of the tile is missing
-  int low[2];                              // whether the tile's weights are three e5m2 terms
   unsigned long long full[8], empty[8], scales_full[kScaleSlots], scales_empty[kScaleSlots];
   unsigned long long s_full[2], p_full[2], o_done[2], q_full, drain;
   float row_scale[128];
@@ -108,31 +105,15 @@ struct Walk {
 };
 
 __device__ __forceinline__ void group_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-__device__ __forceinline__ bool group_any(bool mine) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(any) : "r"(static_cast<uint32_t>(mine)) : "memory");
-  return any != 0;
-}
-// Four weights as f16 pairs -> four codes of each term; e5m2 is the upper byte of an f16.
-template <bool kLowTile>
+// Four weights as f16 pairs -> four e5m2 codes of each of three terms: two cut off, the last rounded.
 __device__ __forceinline__ void split_weights(uint32_t h0, uint32_t h1, uint32_t* terms, int stride) {
-  constexpr uint32_t kHalf = 0x00800080u;
-  if (kLowTile) {
 #pragma unroll
-    for (int term = 0; term < 3; ++term) {
-      const uint32_t u0 = h0 + kHalf, u1 = h1 + kHalf;
-      terms[term * stride] = __byte_perm(u0, u1, 0x7531);
-      h0 = sub_f16x2(h0, u0 & 0xff00ff00u);
-      h1 = sub_f16x2(h1, u1 & 0xff00ff00u);
-    }
-  } else {
-    const uint32_t c0 = cvt_e4m3x2_f16x2(h0), c1 = cvt_e4m3x2_f16x2(h1);
-    terms[0] = __byte_perm(c0, c1, 0x5410);
-    terms[stride] = __byte_perm(sub_f16x2(h0, e4m3x2_f16x2(c0)) + kHalf, sub_f16x2(h1, e4m3x2_f16x2(c1)) + kHalf, 0x7531);
+  for (int term = 0; term < 2; ++term) {
+    terms[term * stride] = __byte_perm(h0, h1, 0x7531);
+    h0 = sub_f16x2(h0, h0 & 0xff00ff00u);
+    h1 = sub_f16x2(h1, h1 & 0xff00ff00u);
   }
+  terms[2 * stride] = __byte_perm(h0 + 0x00800080u, h1 + 0x00800080u, 0x7531);
 }
 
 // Cuts the list into `blocks` shares.  The list runs over sequences, their row tiles, the key/value heads and the tiles of the
@@ -342,8 +323,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
       // ------------------------------ products ------------------------------
       constexpr uint32_t kScoresHigh = instr_desc_f8(kE4m3, kE4m3, 0, 0, 128, kKvTile);
       constexpr uint32_t kScoresLow = instr_desc_f8(kE5m2, kE4m3, 0, 0, 128, kKvTile);
-      constexpr uint32_t kSumsE4m3 = instr_desc_f8(kE4m3, kE4m3, 0, 1, 128, kDim);
-      constexpr uint32_t kSumsE5m2 = instr_desc_f8(kE5m2, kE4m3, 0, 1, 128, kDim);
+      constexpr uint32_t kSums = instr_desc_f8(kE5m2, kE4m3, 0, 1, 128, kDim);
       int ring = 0, tile = 0, segment = 0;
       bool alive = true;
       while (alive && walk.next()) {
@@ -378,16 +358,14 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
           const int r = ring_v(ring, j, n), slot = r % L::kSlots, buffer = (tile + j) & 1;
           if (!wait(&sm.p_full[buffer], ((tile + j) >> 1) & 1) || !wait(&sm.full[slot], (r / L::kSlots) & 1)) { alive = false; break; }
           tc_fence_after();
-          const bool low = *reinterpret_cast<volatile int*>(&sm.low[buffer]) != 0;
           if (elect_one()) {
             const uint32_t v0 = base + slot * L::kSlotBytes, w0 = tmem + L::kScoreColumn + buffer * 128;
 #pragma unroll
             for (int term = 0; term < 3; ++term) {
-              if (term == 2 && !low) break;
 #pragma unroll
               for (int k = 0; k < kKvTile / 32; ++k)
                 umma_f8_ts(tmem, w0 + k * 32 + term * 8, smem_desc_rows<L::kRowBytes>(v0 + k * 32 * L::kRowBytes, L::kPanelBytes),
-                           term == 0 && !low ? kSumsE4m3 : kSumsE5m2, (j | term | k) != 0);
+                           kSums, (j | term | k) != 0);
             }
             umma_commit(smem_u32(&sm.empty[slot]));
             umma_commit(smem_u32(&sm.o_done[buffer]));
@@ -523,50 +501,53 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
       for (int j = 0; j < n; ++j, ++tile) {
         const int buffer = tile & 1, slot = tile % kScaleSlots;
         const int position0 = (walk.tile0 + j) * kKvTile;
-        const uint32_t scores = tmem + lanes + L::kScoreColumn + buffer * 128 + group * 64;
+        const uint32_t scores = tmem + lanes + L::kScoreColumn + buffer * 128;
         wait(&sm.scales_full[slot], (tile / kScaleSlots) & 1);
         wait(&sm.s_full[buffer], (tile >> 1) & 1);
         tc_fence_after();
+        const uint32_t half = 64 * group;
         uint32_t s[64];
-        tmem_ld32(scores, s);
-        tmem_ld32(scores + 32, s + 32);
-        const float4* scales = sm.scales[slot] + 4 * group;
-        const bool masked = position0 + kKvTile - 1 > walk.unit.first || sm.holes[slot] != 0;
-        float factor[4], offset[4];
+        tmem_ld32(scores + half, s);
+        tmem_ld32(scores + half + 32, s + 32);
+        const float4* scales = sm.scales[slot];
+        const int holes = sm.holes[slot];
+        const bool masked = position0 + kKvTile - 1 > walk.unit.first || holes != 0;
+        // positive, so that a masked score stays -inf
+        auto factor_of = [&](int g) { return fmaxf(scales[g].x * row_scale, 1.17549435e-38f); };
+        auto mask = [&](uint32_t* x, int first) {          // 32 scores from position `first` of the tile on
+          // the diagonal, the sequence's end, or a page that is not there
+          const int seen = limit - position0 - first;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          factor[g] = fmaxf(scales[g].x * row_scale, 1.17549435e-38f);         // positive, so that a masked score stays -inf
-          offset[g] = scales[g].y;
-        }
+          for (int c = 0; c < 32; ++c)
+            if (c > seen || ((holes >> ((first + c) / 16)) & 1) != 0) x[c] = 0xff800000u;
+        };
+        auto top_of = [&](const uint32_t* x, int first) {
+          float m = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            float a0 = __uint_as_float(x[16 * g]), a1 = __uint_as_float(x[16 * g + 1]);
+#pragma unroll
+            for (int c = 2; c < 16; c += 4) {
+              a0 = fmaxf(fmaxf(a0, __uint_as_float(x[16 * g + c])), __uint_as_float(x[16 * g + c + 1]));
+              if (c + 2 < 16) a1 = fmaxf(fmaxf(a1, __uint_as_float(x[16 * g + c + 2])), __uint_as_float(x[16 * g + c + 3]));
+            }
+            m = fmaxf(m, fmaf(fmaxf(a0, a1), factor_of(first / 16 + g), scales[first / 16 + g].y));
+          }
+          return m;
+        };
         tmem_ld_wait();
         if (masked) {
-          // the diagonal, the sequence's end, or a page that is not there
-          const int seen = limit - position0 - 64 * group;                     // last of these positions that the row sees
-          const int holes = sm.holes[slot] >> (4 * group);
-#pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (c > seen || ((holes >> (c / 16)) & 1) != 0) s[c] = 0xff800000u;
+          mask(s, half);
+          mask(s + 32, half + 32);
         }
-        float m = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float x = __uint_as_float(s[16 * g]), y = __uint_as_float(s[16 * g + 1]);
-#pragma unroll
-          for (int c = 2; c < 16; c += 4) {
-            x = fmaxf(fmaxf(x, __uint_as_float(s[16 * g + c])), __uint_as_float(s[16 * g + c + 1]));
-            if (c + 2 < 16) y = fmaxf(fmaxf(y, __uint_as_float(s[16 * g + c + 2])), __uint_as_float(s[16 * g + c + 3]));
-          }
-          m = fmaxf(m, fmaf(fmaxf(x, y), factor[g], offset[g]));
-        }
+        float m = fmaxf(top_of(s, half), top_of(s + 32, half + 32));
         sm.half_top[buffer][group][row] = m;
-        group_barrier();
+        asm volatile("bar.sync %0, 64;" :: "r"(2 + quarter) : "memory");
         m = fmaxf(m, sm.half_top[buffer][group ^ 1][row]);
         peak = fmaxf(peak, m);
         float now = top;
         if (m > top + kGrow || (top == -INFINITY && m > top)) now = m;
         else if (m > -INFINITY && fmaxf(m, peak - kDepth) < top - kFall) now = fmaxf(m, peak - kDepth);
-        const bool low = group_any(m > -INFINITY && m < now - kLow);
-        if (threadIdx.x == 128) sm.low[buffer] = low ? 1 : 0;
         if (j > 0 && __any_sync(0xffffffffu, now != top)) {
           wait(&sm.o_done[buffer ^ 1], ((tile - 1) >> 1) & 1);
           tc_fence_after();
@@ -586,33 +567,30 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
           top = now;
         }
         const float shift = kWeightExponent - (now == -INFINITY ? 0.0f : now);
-        auto weights = [&](auto low_tile) {
 #pragma unroll
-          for (int chunk = 0; chunk < 2; ++chunk) {
-            uint32_t terms[24];
+        for (int chunk = 0; chunk < 2; ++chunk) {
+          uint32_t terms[24];
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              const float at = offset[2 * chunk + g] + shift;
-              float part = 0.0f;
+          for (int g = 0; g < 2; ++g) {
+            const int at = half / 16 + 2 * chunk + g;
+            const float factor = factor_of(at), offset = scales[at].y + shift;
+            float part = 0.0f;
 #pragma unroll
-              for (int c = 0; c < 16; c += 4) {
-                float w[4];
+            for (int c = 0; c < 16; c += 4) {
+              float w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  w[i] = fast_exp2(fmaf(__uint_as_float(s[32 * chunk + 16 * g + c + i]), factor[2 * chunk + g], at));
-                  part += w[i];
-                }
-                split_weights<decltype(low_tile)::value>(cvt_f16x2(w[0], w[1]), cvt_f16x2(w[2], w[3]), terms + 4 * g + c / 4, 8);
+              for (int i = 0; i < 4; ++i) {
+                w[i] = fast_exp2(fmaf(__uint_as_float(s[32 * chunk + 16 * g + c + i]), factor, offset));
+                part += w[i];
               }
-              sum = fmaf(part, scales[2 * chunk + g].z, sum);
+              split_weights(cvt_f16x2(w[0], w[1]), cvt_f16x2(w[2], w[3]), terms + 4 * g + c / 4, 8);
             }
-            // where the scores of these 32 positions lay
-            tmem_st8(scores + 32 * chunk, terms);
-            tmem_st8(scores + 32 * chunk + 8, terms + 8);
-            if (decltype(low_tile)::value) tmem_st8(scores + 32 * chunk + 16, terms + 16);
+            sum = fmaf(part, scales[at].z, sum);
           }
-        };
-        if (low) weights(std::true_type{}); else weights(std::false_type{});
+          // where the scores of these 32 positions lay
+#pragma unroll
+          for (int term = 0; term < 3; ++term) tmem_st8(scores + half + 32 * chunk + 8 * term, terms + 8 * term);
+        }
         tmem_st_wait();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sm.scales_empty[slot]));
