@@ -89,7 +89,7 @@ kv_join_kernel(const KvAttentionPlan plan) {
   }
 }
 
-constexpr int kDecodeRows = 64;
+constexpr int kDecodeRows = 16;
 constexpr int kPartRows = 128;
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

@@ -23,10 +23,11 @@ __host__ __device__ inline int kv_block_of(long long total, long long tile, int 
   return static_cast<int>(((tile + 1) * blocks - 1) / total);
 }
 
-// Where a block of the prompt kernel begins in the list: the tile's number there, the unit and the tile inside the unit.
-struct KvStart {
+// Where a block of the prompt kernel begins: the unit and the tile inside it, and the place in the list in units of its cost.
+struct alignas(16) KvStart {
   long long at;
   int sequence, row_tile, head, tile;
+  int row0, rows, length, unused;       // of the sequence
 };
 
 // One part: rows x head_dim sums in FP32, and per row the reference maximum (log2) and the sum of the weights.

@@ -58,33 +58,38 @@ struct Small {
   int abort_flag;
 };
 
-// A block's share of the list, unit by unit.
+// A block's share of the list, unit by unit: from one cut to the next.
 struct Walk {
   const KvAttentionPlan* plan;
   int sequence, row_tile, head, tile0, tiles;
-  long long left;
+  int end_sequence, end_row_tile, end_head, end_tile;
   KvSequence seq;
   KvUnit unit;
   int row_tiles;
-  __device__ __forceinline__ void load() {
-    seq = kv_sequence(plan->a.batch, plan->a.shape, sequence);
-    row_tiles = (seq.rows + plan->tile_tokens - 1) / plan->tile_tokens;
-  }
-  __device__ __forceinline__ void begin(const KvAttentionPlan& p, const KvStart& start, long long end) {
+  __device__ __forceinline__ void begin(const KvAttentionPlan& p, const KvStart& start, const KvStart& end) {
     plan = &p;
-    left = end - start.at;
     sequence = start.sequence;
     row_tile = start.row_tile;
     head = start.head;
     tile0 = start.tile;
-    if (left > 0) load();
+    end_sequence = end.sequence;
+    end_row_tile = end.row_tile;
+    end_head = end.head;
+    end_tile = end.tile;
+    seq = KvSequence{start.row0, start.rows, start.length, false};
+    row_tiles = (seq.rows + plan->tile_tokens - 1) / plan->tile_tokens;
   }
   __device__ __forceinline__ bool next() {
-    if (left <= 0) return false;
     for (;;) {
+      int most = 0x7fffffff;
+      if (sequence == end_sequence && row_tile == end_row_tile && head == end_head) {
+        most = end_tile - tile0;
+        if (most <= 0) return false;
+      }
       if (row_tile < row_tiles) {
         unit = kv_unit(seq, row_tile, plan->tile_tokens);
-        if (tile0 < unit.tiles) break;
+        tiles = min(unit.tiles - tile0, most);
+        if (tiles > 0) return true;
         tile0 = 0;
         if (unit.tiles > 0 && ++head < plan->a.shape.kv_heads) continue;
         head = 0;
@@ -92,18 +97,21 @@ struct Walk {
       } else {
         row_tile = 0;
         ++sequence;
-        load();
+        seq = kv_sequence(plan->a.batch, plan->a.shape, sequence);
+        row_tiles = (seq.rows + plan->tile_tokens - 1) / plan->tile_tokens;
       }
     }
-    tiles = static_cast<int>(min(static_cast<long long>(unit.tiles - tile0), left));
-    return true;
   }
-  __device__ __forceinline__ void advance() {
-    left -= tiles;
-    tile0 += tiles;
-  }
+  __device__ __forceinline__ void advance() { tile0 += tiles; }
 };
 
+// 16 bytes to shared memory, or zeros
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool exists) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(exists ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// row / group for rows below 128, with inverse = ceil(2^16 / group)
+__device__ __forceinline__ int row_token(int row, int inverse) { return (row * inverse) >> 16; }
 __device__ __forceinline__ void group_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 // Four weights as f16 pairs -> four e5m2 codes of each of three terms: two cut off, the last rounded.
 __device__ __forceinline__ void split_weights(uint32_t h0, uint32_t h1, uint32_t* terms, int stride) {
@@ -116,16 +124,18 @@ __device__ __forceinline__ void split_weights(uint32_t h0, uint32_t h1, uint32_t
   terms[2 * stride] = __byte_perm(h0 + 0x00800080u, h1 + 0x00800080u, 0x7531);
 }
 
-// Cuts the list into `blocks` shares.  The list runs over sequences, their row tiles, the key/value heads and the tiles of the
-// cache.  A cut that falls near the end of a unit moves there: a divided unit costs its two blocks a write of 128 x head_dim
-// sums each and the join a read of them, about as much as kSnap tiles.  One block; items are row tiles.
+// Cuts the list into `blocks` shares of equal cost.  The list runs over sequences, their row tiles, the key/value heads and the
+// tiles of the cache; a unit costs its tiles and kUnitCost more, for its queries, the first scores that nothing overlaps and
+// its results.  A cut within kSnap tiles of a unit's end moves there: a divided unit costs all that twice, and the join.  One
+// block; items are row tiles.
 constexpr int kPlanThreads = 1024;
-constexpr int kSnap = 6;
+constexpr int kUnitCost = 3;
+constexpr int kSnap = 2;
 __global__ void __launch_bounds__(kPlanThreads)
 kv_plan_kernel(const KvAttentionPlan plan) {
   __shared__ int first_item[AIMA_MOE_KV_MAX_SEQUENCES + 1];
   __shared__ long long warp_sum[kPlanThreads / 32];
-  __shared__ long long carry, total_s;
+  long long total = 0;
   pdl_enter();
   const KvAttention& a = plan.a;
   const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
@@ -162,10 +172,10 @@ kv_plan_kernel(const KvAttentionPlan plan) {
   if (thread == 0) first_item[0] = 0;
   __syncthreads();
   const int items = first_item[a.batch.sequences];
-  for (int pass = 0; pass < 2; ++pass) {
-    if (thread == 0) carry = 0;
-    __syncthreads();
-    for (int item0 = 0; item0 < items; item0 += kPlanThreads) {
+  // Up to kPlanThreads items need one scan; more are gone through twice, for the total and for the cuts.
+  for (int pass = items > kPlanThreads ? 0 : 1; pass < 2; ++pass) {
+    long long carry = 0;                       // the same in all threads
+    for (int item0 = 0; item0 < items || item0 == 0; item0 += kPlanThreads) {
       const int item = item0 + thread;
       int s = 0, row_tile = 0;
       KvUnit unit{0, 0, 0};
@@ -181,20 +191,22 @@ kv_plan_kernel(const KvAttentionPlan plan) {
         seq = kv_sequence(a.batch, a.shape, s);
         unit = kv_unit(seq, row_tile, plan.tile_tokens);
       }
-      const long long end = scan(static_cast<long long>(unit.tiles) * heads) + carry;
-      const long long begin = end - static_cast<long long>(unit.tiles) * heads;
+      const long long unit_cost = unit.tiles > 0 ? unit.tiles + kUnitCost : 0, cost = unit_cost * heads;
+      const long long end = scan(cost) + carry, begin = end - cost;
+      carry += warp_sum[kPlanThreads / 32 - 1];
+      if (items <= kPlanThreads) total = carry;
       if (pass == 1 && unit.tiles > 0) {
         // the cuts c with begin < total c / blocks <= end, and the list's own begin
-        const long long total = total_s;
         for (long long c = begin == 0 ? 0 : begin * plan.blocks / total + 1; c <= plan.blocks; ++c) {
           const long long cut = total * c / plan.blocks;
           if (cut > end) break;
           if (cut <= begin && begin != 0) continue;
-          int head = static_cast<int>(min((cut - begin) / unit.tiles, static_cast<long long>(heads - 1)));
-          int tile = static_cast<int>(cut - begin - static_cast<long long>(head) * unit.tiles);
+          const int head = static_cast<int>(min((cut - begin) / unit_cost, static_cast<long long>(heads - 1)));
+          const long long unit_begin = begin + head * unit_cost;
+          int tile = max(0, static_cast<int>(cut - unit_begin) - kUnitCost);
           if (tile <= kSnap && tile <= unit.tiles - tile) tile = 0;
           else if (unit.tiles - tile <= kSnap) tile = unit.tiles;
-          plan.work.starts[c] = KvStart{begin + static_cast<long long>(head) * unit.tiles + tile, s, row_tile, head, tile};
+          plan.work.starts[c] = KvStart{unit_begin + (tile > 0 ? kUnitCost + tile : 0), s, row_tile, head, tile, seq.row0, seq.rows, seq.length, 0};
         }
       }
       if (pass == 1 && item < items && unit.tiles == 0) {
@@ -204,17 +216,12 @@ kv_plan_kernel(const KvAttentionPlan plan) {
           for (int j = 0; j < a.shape.q_heads * dim / 8; ++j) out[j] = make_uint4(0, 0, 0, 0);
         }
       }
-      __syncthreads();
-      if (thread == kPlanThreads - 1) carry = end;
-      __syncthreads();
+      __syncthreads();                         // warp_sum has been read
     }
-    if (pass == 0) {
-      if (thread == 0) total_s = carry;
-      __syncthreads();
-      if (total_s == 0) {
-        for (int c = thread; c <= plan.blocks; c += kPlanThreads) plan.work.starts[c] = KvStart{0, 0, 0, 0, 0};
-      }
-    }
+    total = carry;
+  }
+  if (total == 0) {
+    for (int c = thread; c <= plan.blocks; c += kPlanThreads) plan.work.starts[c] = KvStart{0, 0, 0, 0, 0, 0, 0, 0, 0};
   }
 }
 
@@ -258,9 +265,8 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
   const uint32_t tmem = sm.tmem;
   pdl_enter();
 
-  const KvStart start = plan.work.starts[blockIdx.x];
   Walk walk;
-  walk.begin(plan, start, plan.work.starts[blockIdx.x + 1].at);
+  walk.begin(plan, plan.work.starts[blockIdx.x], plan.work.starts[blockIdx.x + 1]);
   auto wait = [&](unsigned long long* bar, uint32_t parity) {
     if (mbar_wait_bounded_warp(smem_u32(bar), parity, abort_flag, plan.wait_limit_ns)) return true;
     if (lane == 0) atomicOr(a.status, kKvTimeout);
@@ -416,70 +422,74 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
     // ------------------------------ softmax and results ------------------------------
     const int group = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const int group_inverse = (65536 + shape.group - 1) / shape.group;
     int ring = 0, tile = 0, segment = 0;
     // No wait that runs out leaves this loop: the warps meet at barriers, and every wait after the first that ran out ends at once.
     while (walk.next()) {
       const int n = walk.tiles;
       const int rows = walk.unit.tokens * shape.group;
       const int token0 = walk.seq.row0 + walk.row_tile * plan.tile_tokens;
-      // Queries: a warp takes every eighth row, eight at a time.
+      // Queries: a warp takes every eighth row.  The raw BF16 row goes where its two terms will lie, all rows at once, and is
+      // converted in place: with the loads in registers either the loop is unrolled, and its code does not stay in the instruction
+      // cache between units, or every pass waits for its loads (8000 cycles either way).  BF16 numbers are f16 numbers
+      // down to 2^-14 of the row's scale.
       {
-        constexpr int kPer = kDim / 32;
+        constexpr int kPer = kDim / 32, kPieces = kDim / 8, kAtOnce = 32 / kPieces;
         const int w8 = warp - 4;
+        auto at_byte = [&](int r, int byte) {            // of a row of 2 kDim bytes: the first term's kDim, then the second's
+          const int term = byte / kDim, inside = byte % kDim;
+          return generic + L::kQueryAt + term * L::kSlotBytes + (inside / L::kRowBytes) * L::kPanelBytes + r * L::kRowBytes + inside % L::kRowBytes;
+        };
+#pragma unroll 4
+        for (int i = 0; i < 16; i += kAtOnce) {
+          const int r = 8 * (i + lane / kPieces) + w8;
+          const int token = row_token(r, group_inverse), g = r - token * shape.group;
+          const bool exists = r < rows;
+          cp_async_16_or_zero(smem_u32(at_byte(r, 16 * (lane % kPieces))),
+                              a.q.data + (exists ? static_cast<long long>(token0 + token) * a.q.row_stride + (walk.head * shape.group + g) * a.q.head_stride + 8 * (lane % kPieces) : 0),
+                              exists);
+        }
+        cp_async_wait_all();
+        __syncwarp();
 #pragma unroll 1
-        for (int r0 = 0; r0 < 128; r0 += 64) {
-          uint32_t raw[8][kPer / 2];
+        for (int i = 0; i < 16; i += 4) {                  // four rows side by side: one alone is a chain of 340 cycles
+          uint32_t raw[4][kPer / 2], codes[4][2][kPer / 2];
+          int exponent[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = r0 + 8 * i + w8;
-            const int token = r / shape.group, g = r - token * shape.group;
-            const __nv_bfloat16* at = a.q.data + static_cast<long long>(token0 + token) * a.q.row_stride +
-                                      (walk.head * shape.group + g) * a.q.head_stride + lane * kPer;
-#pragma unroll
-            for (int e = 0; e < kPer / 2; ++e) raw[i][e] = 0;
-            if (r < rows) {
-              if constexpr (kPer == 8) {
-                const uint4 v = *reinterpret_cast<const uint4*>(at);
-                raw[i][0] = v.x; raw[i][1] = v.y; raw[i][2] = v.z; raw[i][3] = v.w;
-              } else if constexpr (kPer == 4) {
-                const uint2 v = *reinterpret_cast<const uint2*>(at);
-                raw[i][0] = v.x; raw[i][1] = v.y;
-              } else {
-                raw[i][0] = *reinterpret_cast<const uint32_t*>(at);
-              }
+          for (int b = 0; b < 4; ++b) {
+            const uint8_t* from = at_byte(8 * (i + b) + w8, 2 * kPer * lane);
+            if constexpr (kPer == 8) {
+              const uint4 v = *reinterpret_cast<const uint4*>(from);
+              raw[b][0] = v.x; raw[b][1] = v.y; raw[b][2] = v.z; raw[b][3] = v.w;
+            } else if constexpr (kPer == 4) {
+              const uint2 v = *reinterpret_cast<const uint2*>(from);
+              raw[b][0] = v.x; raw[b][1] = v.y;
+            } else {
+              raw[b][0] = *reinterpret_cast<const uint32_t*>(from);
             }
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = r0 + 8 * i + w8;
-            float top = 0.0f;
-            bool finite = true;
+          for (int b = 0; b < 4; ++b) {
+            uint32_t largest = 0;          // magnitudes as integers: infinities and NaN come last
+#pragma unroll
+            for (int e = 0; e < kPer / 2; ++e) largest = max(largest, max(raw[b][e] & 0x7fffu, (raw[b][e] >> 16) & 0x7fffu));
+            largest = __reduce_max_sync(0xffffffffu, largest);           // all lanes have read the row
+            const bool finite = largest < 0x7f80u;
+            exponent[b] = kv_scale_exponent(__uint_as_float(largest << 16));
+            const float inverse = kv_exp2(-exponent[b]);
 #pragma unroll
             for (int e = 0; e < kPer / 2; ++e) {
-              const float u = fabsf(bf16_lo(raw[i][e])), v = fabsf(bf16_hi(raw[i][e]));
-              finite = finite && u <= 3.402823466e38f && v <= 3.402823466e38f;
-              top = fmaxf(top, fmaxf(u, v));
+              const uint32_t h = cvt_f16x2(bf16_lo(raw[b][e]) * inverse, bf16_hi(raw[b][e]) * inverse);
+              codes[b][0][e] = finite ? cvt_e4m3x2_f16x2(h) : kKvNan * 0x0101u;
+              codes[b][1][e] = finite ? cvt_e5m2x2_f16x2(sub_f16x2(h, e4m3x2_f16x2(codes[b][0][e]))) : 0u;
             }
+          }
 #pragma unroll
-            for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            finite = __all_sync(0xffffffffu, finite);
-            const int exponent = kv_scale_exponent(top);
-            const float inverse = kv_exp2(-exponent);
-            uint32_t hi[kPer / 2], lo[kPer / 2];
-#pragma unroll
-            for (int e = 0; e < kPer / 2; ++e) {
-              const float u = bf16_lo(raw[i][e]) * inverse, v = bf16_hi(raw[i][e]) * inverse;
-              hi[e] = cvt_e4m3x2(u, v);
-              const float2 back = e4m3x2_values(hi[e]);
-              lo[e] = cvt_e5m2x2(u - back.x, v - back.y);
-              if (!finite) {
-                hi[e] = kKvNan * 0x0101u;
-                lo[e] = 0;
-              }
-            }
+          for (int b = 0; b < 4; ++b) {
+            const int r = 8 * (i + b) + w8;
 #pragma unroll
             for (int term = 0; term < 2; ++term) {
-              const uint32_t* c = term == 0 ? hi : lo;
+              const uint32_t* c = codes[b][term];
               const int byte = lane * kPer, panel = byte / L::kRowBytes, inside = byte % L::kRowBytes;
               const int piece = (inside >> 4) ^ (L::kRowBytes == 128 ? r & 7 : (r >> 1) & 3);
               uint8_t* to = generic + L::kQueryAt + term * L::kSlotBytes + panel * L::kPanelBytes + r * L::kRowBytes + piece * 16 + (inside & 15);
@@ -487,7 +497,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
               else if constexpr (kPer == 4) *reinterpret_cast<uint32_t*>(to) = c[0] | (c[1] << 16);
               else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(c[0]);
             }
-            if (lane == 0) sm.row_scale[r] = kv_exp2(exponent);
+            if (lane == 0) sm.row_scale[r] = kv_exp2(exponent[b]);
           }
         }
         fence_async_proxy();
@@ -496,7 +506,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
         group_barrier();                   // row_scale
       }
       const float row_scale = sm.row_scale[row];
-      const int limit = row < rows ? walk.unit.first + row / shape.group : -1;     // last position the row sees
+      const int limit = row < rows ? walk.unit.first + row_token(row, group_inverse) : -1;     // last position the row sees
       float top = -INFINITY, peak = -INFINITY, sum = 0.0f;       // reference and maximum so far; this half's sum of weights
       for (int j = 0; j < n; ++j, ++tile) {
         const int buffer = tile & 1, slot = tile % kScaleSlots;
@@ -515,11 +525,14 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
         // positive, so that a masked score stays -inf
         auto factor_of = [&](int g) { return fmaxf(scales[g].x * row_scale, 1.17549435e-38f); };
         auto mask = [&](uint32_t* x, int first) {          // 32 scores from position `first` of the tile on
-          // the diagonal, the sequence's end, or a page that is not there
+          // the diagonal, the sequence's end, or a page that is not there: a bit for each that counts
           const int seen = limit - position0 - first;
+          uint32_t bits = seen >= 31 ? 0xffffffffu : seen < 0 ? 0u : (2u << seen) - 1u;
+          if ((holes >> (first / 16)) & 1) bits &= 0xffff0000u;
+          if ((holes >> (first / 16)) & 2) bits &= 0x0000ffffu;
 #pragma unroll
           for (int c = 0; c < 32; ++c)
-            if (c > seen || ((holes >> ((first + c) / 16)) & 1) != 0) x[c] = 0xff800000u;
+            if ((bits & (1u << c)) == 0u) x[c] = 0xff800000u;
         };
         auto top_of = [&](const uint32_t* x, int first) {
           float m = -INFINITY;
@@ -552,14 +565,15 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
           wait(&sm.o_done[buffer ^ 1], ((tile - 1) >> 1) & 1);
           tc_fence_after();
           const float f = now != top ? fast_exp2(top - now) : 1.0f;
+          const uint32_t sums = tmem + lanes + group * (kDim / 2);
 #pragma unroll 1
-          for (int c = group * (kDim / 2); c < (group + 1) * (kDim / 2); c += 32) {
+          for (int c = 0; c < kDim / 2; c += 32) {
             uint32_t o[32];
-            tmem_ld32(tmem + lanes + c, o);
+            tmem_ld32(sums + c, o);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st32(tmem + lanes + c, o);
+            tmem_st32(sums + c, o);
           }
         }
         if (now != top) {
@@ -622,27 +636,47 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
       const int part = 2 * blockIdx.x + (walk.tile0 == 0 ? 1 : 0);
       if (!whole && group == 0) plan.work.weights[static_cast<size_t>(part) * plan.work.rows_per_part + row] = make_float2(top, total);
       const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-      const int token = row / shape.group, g = row - token * shape.group;
-      __nv_bfloat16* out = a.out + (static_cast<long long>(token0 + token) * shape.q_heads + walk.head * shape.group + g) * kDim;
       float* sums = plan.work.sums + static_cast<size_t>(part) * plan.work.rows_per_part * kDim;
+      // The queries are no longer needed: their place takes the results, 16-byte pieces XORed with the row, so that they leave in
+      // whole rows.  (Each thread storing its own row took 5 us per unit.)
+      uint8_t* stage = generic + L::kQueryAt;
+      const uint32_t from = tmem + lanes + group * (kDim / 2);
 #pragma unroll 1
-      for (int c = group * (kDim / 2); c < (group + 1) * (kDim / 2); c += 8) {
-        uint32_t o[8];
-        tmem_ld8(tmem + lanes + c, o);
+      for (int c = 0; c < kDim / 64; ++c) {
+        uint32_t x[32];
+        tmem_ld32(from + 32 * c, x);
         tmem_ld_wait();
+        const int column = group * (kDim / 2) + 32 * c;
         if (whole) {
-          uint32_t packed[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            packed[i] = static_cast<uint32_t>(float_to_bf16_bits(__uint_as_float(o[2 * i]) * inverse)) |
-                        (static_cast<uint32_t>(float_to_bf16_bits(__uint_as_float(o[2 * i + 1]) * inverse)) << 16);
-          if (row < rows) *reinterpret_cast<uint4*>(out + c) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-        } else {
+          for (int k = 0; k < 4; ++k) {
+            uint32_t packed[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(x[8 * k + 2 * i]) * inverse, __uint_as_float(x[8 * k + 2 * i + 1]) * inverse);
+              packed[i] = *reinterpret_cast<const uint32_t*>(&two);
+            }
+            *reinterpret_cast<uint4*>(stage + row * 2 * kDim + (((column / 8 + k) ^ (row & 7)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+          }
+        } else if (row < rows) {
           // [head_dim / 4][rows][4]: a warp writes whole lines
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            *reinterpret_cast<uint4*>(sums + (static_cast<size_t>(c / 4 + i) * plan.work.rows_per_part + row) * 4) =
-                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int k = 0; k < 8; ++k)
+            *reinterpret_cast<uint4*>(sums + (static_cast<size_t>(column / 4 + k) * plan.work.rows_per_part + row) * 4) =
+                make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+        }
+      }
+      if (whole) {
+        constexpr int kPieces = kDim / 8, kRowsAtOnce = 32 / kPieces;
+        group_barrier();
+#pragma unroll 2
+        for (int r0 = (warp - 4) * kRowsAtOnce; r0 < rows; r0 += 8 * kRowsAtOnce) {
+          const int r = r0 + lane / kPieces, piece = lane % kPieces;
+          if (r < rows) {
+            const int token = row_token(r, group_inverse), g = r - token * shape.group;
+            *reinterpret_cast<uint4*>(a.out + (static_cast<long long>(token0 + token) * shape.q_heads + walk.head * shape.group + g) * kDim + 8 * piece) =
+                *reinterpret_cast<const uint4*>(stage + r * 2 * kDim + ((piece ^ (r & 7)) << 4));
+          }
         }
       }
       tc_fence_before();
@@ -669,37 +703,43 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
 template <int kDim>
 __global__ void __launch_bounds__(256)
 kv_prompt_join_kernel(const KvAttentionPlan plan) {
+  __shared__ long long at_s[kKvMaxBlocks + 1];
+  __shared__ float2 part_weight[kKvMaxBlocks][8];
   __shared__ float weight[kKvMaxBlocks][8];
   __shared__ float total_s[8];
   pdl_enter();
   const KvAttention& a = plan.a;
   const int cut = blockIdx.x + 1, row0 = blockIdx.y * 8;
+  const int thread = threadIdx.x;
+  for (int c = thread; c <= plan.blocks; c += 256) at_s[c] = plan.work.starts[c].at;
   const KvStart start = plan.work.starts[cut];
-  const KvSequence seq = kv_sequence(a.batch, a.shape, start.sequence);
-  const KvUnit unit = kv_unit(seq, start.row_tile, plan.tile_tokens);
+  const KvUnit unit = kv_unit(KvSequence{start.row0, start.rows, start.length, false}, start.row_tile, plan.tile_tokens);
   const int rows = unit.tokens * a.shape.group;
-  if (start.tile == 0 || start.tile >= unit.tiles || row0 >= rows) return;
-  const long long first = start.at - start.tile, end = first + unit.tiles;
-  if (plan.work.starts[cut - 1].at > first) return;            // an earlier cut's
+  if (start.tile == 0 || start.tile >= unit.tiles || row0 >= rows) return;     // the same in the whole block
+  const long long first = start.at - start.tile - kUnitCost, end = start.at - start.tile + unit.tiles;
+  __syncthreads();
+  if (at_s[cut - 1] > first) return;                           // an earlier cut's
   // Parts: block cut - 1 begins the unit; then every block that begins inside it.  Empty shares left none.
   int last = cut;
-  while (last < plan.blocks && plan.work.starts[last + 1].at < end) ++last;
+  while (last < plan.blocks && at_s[last + 1] < end) ++last;
   const int parts = last - cut + 2;
   auto part_of = [&](int p) { return 2 * (cut - 1 + p) + (p == 0 ? 1 : 0); };
-  auto empty = [&](int p) { return p > 0 && plan.work.starts[cut - 1 + p].at == plan.work.starts[cut + p].at; };
-  const int thread = threadIdx.x;
+  auto empty = [&](int p) { return p > 0 && at_s[cut - 1 + p] == at_s[cut + p]; };
+  for (int i = thread; i < 8 * parts; i += 256) {
+    const int p = i >> 3, r = i & 7;
+    // rows that the unit does not have were never written
+    part_weight[p][r] = empty(p) || row0 + r >= rows ? make_float2(-INFINITY, 0.0f)
+                                                     : plan.work.weights[static_cast<size_t>(part_of(p)) * plan.work.rows_per_part + row0 + r];
+  }
+  __syncthreads();
   if (thread < 8) {
     float top = -INFINITY, total = 0.0f;
-    for (int p = 0; p < parts; ++p)
-      if (!empty(p)) top = fmaxf(top, plan.work.weights[static_cast<size_t>(part_of(p)) * plan.work.rows_per_part + row0 + thread].x);
+    for (int p = 0; p < parts; ++p) top = fmaxf(top, part_weight[p][thread].x);
     for (int p = 0; p < parts; ++p) {
-      float w = 0.0f;
-      if (!empty(p)) {
-        const float2 x = plan.work.weights[static_cast<size_t>(part_of(p)) * plan.work.rows_per_part + row0 + thread];
-        // a part without a maximum has seen nothing, or nothing but NaN
-        w = exp2f(x.x - (top == -INFINITY ? 0.0f : top));
-        total += x.x == -INFINITY ? x.y : x.y * w;
-      }
+      const float2 x = part_weight[p][thread];
+      // a part without a maximum has seen nothing, or nothing but NaN
+      const float w = exp2f(x.x - (top == -INFINITY ? 0.0f : top));
+      total += x.x == -INFINITY ? x.y : x.y * w;
       weight[p][thread] = w;
     }
     total_s[thread] = total;
@@ -709,7 +749,7 @@ kv_prompt_join_kernel(const KvAttentionPlan plan) {
   if (row >= rows) return;
   const float inverse = total_s[r] == 0.0f ? 0.0f : 1.0f / total_s[r];
   const int token = row / a.shape.group, g = row - token * a.shape.group;
-  __nv_bfloat16* out = a.out + (static_cast<long long>(seq.row0 + start.row_tile * plan.tile_tokens + token) * a.shape.q_heads +
+  __nv_bfloat16* out = a.out + (static_cast<long long>(start.row0 + start.row_tile * plan.tile_tokens + token) * a.shape.q_heads +
                                 start.head * a.shape.group + g) * kDim;
   for (int d = thread >> 3; d < kDim / 4; d += 32) {
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
