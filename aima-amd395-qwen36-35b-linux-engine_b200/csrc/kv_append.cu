@@ -16,7 +16,10 @@
 namespace aima {
 namespace {
 
-constexpr int kAppendThreads = 256;
+// A thread keeps up to eight vectors of keys and eight of values.
+template <int kDim, int kPage>
+constexpr int append_threads = kPage * kDim > 64 * 256 ? 512 : 256;
+constexpr int kHeadsPerThread = 4;
 
 __device__ __forceinline__ bool finite8(const float* x) {
   bool ok = true;
@@ -47,28 +50,36 @@ __device__ __forceinline__ int exponent_of(float scale) {
   return min(max(((bits >> 23) & 255) - 127 + ((bits & 0x7fffff) != 0 ? 1 : 0), kKvMinExponent), kKvMaxExponent);
 }
 
+// The eight angles of a vector of the rotated part: cosines and sines of one position.
+struct Angles {
+  float4 c0, c1, s0, s1;
+};
+__device__ __forceinline__ Angles load_angles(const float* row, int piece, int half) {
+  const float4* c = reinterpret_cast<const float4*>(row) + 2 * (piece < half ? piece : piece - half);
+  const float4* s = c + 2 * half;
+  return Angles{__ldg(c), __ldg(c + 1), __ldg(s), __ldg(s + 1)};
+}
 // Vector `piece` (elements 8 piece .. 8 piece + 7) of a head, rotated.  Called by whole groups of kDim / 8 lanes that hold
-// one head; the partner's vector comes by shuffle.
+// one head; the partner's vector comes by shuffle.  half: vectors of one half of the rotated part.
 template <int kDim>
-__device__ __forceinline__ void rotate8(const uint4& raw, int piece, int rotary, const float* angle, bool active, float* x) {
-  const int half = rotary >> 4;              // vectors of one half
+__device__ __forceinline__ void rotate8(const uint4& raw, int piece, int half, const Angles& angles, bool active, float* x) {
   const int group0 = (threadIdx.x & 31) & ~(kDim / 8 - 1);
-  const int partner = group0 + (piece < half ? piece + half : piece - half);
   const bool turns = piece < 2 * half;
+  const int partner = turns ? group0 + (piece < half ? piece + half : piece - half) : 0;
   uint4 other;
-  other.x = __shfl_sync(0xffffffffu, raw.x, turns ? partner : 0);
-  other.y = __shfl_sync(0xffffffffu, raw.y, turns ? partner : 0);
-  other.z = __shfl_sync(0xffffffffu, raw.z, turns ? partner : 0);
-  other.w = __shfl_sync(0xffffffffu, raw.w, turns ? partner : 0);
+  other.x = __shfl_sync(0xffffffffu, raw.x, partner);
+  other.y = __shfl_sync(0xffffffffu, raw.y, partner);
+  other.z = __shfl_sync(0xffffffffu, raw.z, partner);
+  other.w = __shfl_sync(0xffffffffu, raw.w, partner);
   unpack8(raw, x);
   if (turns && active) {
+    const float c[8] = {angles.c0.x, angles.c0.y, angles.c0.z, angles.c0.w, angles.c1.x, angles.c1.y, angles.c1.z, angles.c1.w};
+    const float s[8] = {angles.s0.x, angles.s0.y, angles.s0.z, angles.s0.w, angles.s1.x, angles.s1.y, angles.s1.z, angles.s1.w};
     float y[8];
     unpack8(other, y);
-    const float* cosine = angle + 8 * (piece < half ? piece : piece - half);
-    const float* sine = cosine + 8 * half;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float a = __fmul_rn(x[i], __ldg(cosine + i)), b = __fmul_rn(y[i], __ldg(sine + i));
+      const float a = __fmul_rn(x[i], c[i]), b = __fmul_rn(y[i], s[i]);
       x[i] = piece < half ? __fsub_rn(a, b) : __fadd_rn(a, b);
     }
   }
@@ -87,8 +98,9 @@ __device__ __forceinline__ int sequence_of_row(const KvBatch& b, int row) {
 // One block per (sequence, touched page, head), then blocks for the queries.  A page and head belongs to one block, which
 // holds all of its new rows in registers between finding the scale and writing the codes: every byte is read once.
 template <int kDim, int kPage>
-__global__ void __launch_bounds__(kAppendThreads)
+__global__ void __launch_bounds__(append_threads<kDim, kPage>)
 kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
+  constexpr int kAppendThreads = append_threads<kDim, kPage>;
   constexpr int kPieces = kDim / 8;                                   // 16-byte vectors of a head
   constexpr int kRowsPerPass = kAppendThreads / kPieces;
   constexpr int kPasses = (kPage + kRowsPerPass - 1) / kRowsPerPass;
@@ -96,6 +108,7 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
   const int piece = threadIdx.x % kPieces;
   const int slot0 = threadIdx.x / kPieces;
   const KvShape& shape = a.shape;
+  const int half = shape.rotary >> 4;
 
   if (static_cast<int>(blockIdx.x) < page_blocks) {
     const int head = blockIdx.x % shape.kv_heads;
@@ -132,7 +145,9 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
       const int position = page_start + slot0 + p * kRowsPerPass;
       const bool active = position >= low && position < high;
       float k[8], v[8];
-      rotate8<kDim>(kraw[p], piece, shape.rotary, a.rotation + static_cast<size_t>(position) * shape.rotary, active, k);
+      Angles angles{};
+      if (active && piece < 2 * half) angles = load_angles(a.rotation + static_cast<size_t>(position) * shape.rotary, piece, half);
+      rotate8<kDim>(kraw[p], piece, half, angles, active, k);
       unpack8(vraw[p], v);
       int bad = (finite8(k) && finite8(v)) ? 0 : 1;
 #pragma unroll
@@ -181,7 +196,9 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
       const int slot = slot0 + p * kRowsPerPass, position = page_start + slot;
       const bool active = position >= low && position < high;
       float k[8], v[8];
-      rotate8<kDim>(kraw[p], piece, shape.rotary, a.rotation + static_cast<size_t>(position) * shape.rotary, active, k);
+      Angles angles{};
+      if (active && piece < 2 * half) angles = load_angles(a.rotation + static_cast<size_t>(position) * shape.rotary, piece, half);
+      rotate8<kDim>(kraw[p], piece, half, angles, active, k);
       unpack8(vraw[p], v);
       if (active) {
         uint2 kc = codes8(k, kinv), vc = codes8(v, vinv);
@@ -210,37 +227,50 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
     return;
   }
 
-  // queries: kPieces lanes hold one head of one row, which stays with its thread for all heads of the row
-  if (a.q.data == nullptr) return;
-  const int row = (blockIdx.x - page_blocks) * kRowsPerPass + slot0;
+  // queries: kPieces lanes hold one head of one row, kHeadsPerThread heads at once, which share the row's angles
+  const int head_groups = (shape.q_heads + kHeadsPerThread - 1) / kHeadsPerThread;
+  const long long work = static_cast<long long>(blockIdx.x - page_blocks) * kRowsPerPass + slot0;
+  const int row = static_cast<int>(min(work / head_groups, static_cast<long long>(a.batch.tokens)));
+  const int head0 = static_cast<int>(work % head_groups) * kHeadsPerThread;
   const bool exists = row < a.batch.tokens;
+  uint4 raw[kHeadsPerThread];
+#pragma unroll
+  for (int h = 0; h < kHeadsPerThread; ++h) {
+    raw[h] = make_uint4(0, 0, 0, 0);
+    if (exists && head0 + h < shape.q_heads)
+      raw[h] = *reinterpret_cast<const uint4*>(a.q.data + row * a.q.row_stride + (head0 + h) * a.q.head_stride + 8 * piece);
+  }
   int position = -1;
   if (exists) {
     const int s = sequence_of_row(a.batch, row);
     const KvSequence seq = kv_sequence(a.batch, shape, s);
     if (!seq.bad && row >= seq.row0 && row < seq.row0 + seq.rows) position = seq.length - seq.rows + row - seq.row0;
   }
-  const bool turns = position >= 0 && position < a.positions;
-  for (int head = 0; head < shape.q_heads; ++head) {
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (exists) raw = *reinterpret_cast<const uint4*>(a.q.data + row * a.q.row_stride + head * a.q.head_stride + 8 * piece);
+  const bool active = position >= 0 && position < a.positions;
+  Angles angles{};
+  if (active && piece < 2 * half) angles = load_angles(a.rotation + static_cast<size_t>(position) * shape.rotary, piece, half);
+#pragma unroll
+  for (int h = 0; h < kHeadsPerThread; ++h) {
     float x[8];
-    rotate8<kDim>(raw, piece, shape.rotary, a.rotation + static_cast<size_t>(max(position, 0)) * shape.rotary, turns, x);
+    rotate8<kDim>(raw[h], piece, half, angles, active, x);
     uint4 w;
     w.x = static_cast<uint32_t>(float_to_bf16_bits(x[0])) | (static_cast<uint32_t>(float_to_bf16_bits(x[1])) << 16);
     w.y = static_cast<uint32_t>(float_to_bf16_bits(x[2])) | (static_cast<uint32_t>(float_to_bf16_bits(x[3])) << 16);
     w.z = static_cast<uint32_t>(float_to_bf16_bits(x[4])) | (static_cast<uint32_t>(float_to_bf16_bits(x[5])) << 16);
     w.w = static_cast<uint32_t>(float_to_bf16_bits(x[6])) | (static_cast<uint32_t>(float_to_bf16_bits(x[7])) << 16);
-    if (exists) *reinterpret_cast<uint4*>(a.q_out + (static_cast<long long>(row) * shape.q_heads + head) * kDim + 8 * piece) = w;
+    if (exists && head0 + h < shape.q_heads)
+      *reinterpret_cast<uint4*>(a.q_out + (static_cast<long long>(row) * shape.q_heads + head0 + h) * kDim + 8 * piece) = w;
   }
 }
 
 template <int kDim, int kPage>
 cudaError_t launch(const KvAppend& a, cudaStream_t stream) {
+  constexpr int kAppendThreads = append_threads<kDim, kPage>;
   const int columns = (a.batch.max_new + kPage - 2) / kPage + 1;      // pages that max_new consecutive tokens can touch
   const long long page_blocks = static_cast<long long>(columns) * a.shape.kv_heads * a.batch.sequences;
-  const int rows_per_block = kAppendThreads / (kDim / 8);
-  const long long query_blocks = a.q.data != nullptr ? (a.batch.tokens + rows_per_block - 1) / rows_per_block : 0;
+  const long long query_work = static_cast<long long>(a.batch.tokens) * ((a.shape.q_heads + kHeadsPerThread - 1) / kHeadsPerThread);
+  const int work_per_block = kAppendThreads / (kDim / 8);
+  const long long query_blocks = a.q.data != nullptr ? (query_work + work_per_block - 1) / work_per_block : 0;
   if (page_blocks + query_blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   kv_append_kernel<kDim, kPage><<<static_cast<unsigned>(page_blocks + query_blocks), kAppendThreads, 0, stream>>>(a, static_cast<int>(page_blocks), columns);
   return cudaGetLastError();
