@@ -16,22 +16,32 @@
 namespace aima {
 namespace {
 
-// A thread keeps up to eight vectors of keys and eight of values.
+constexpr int kHeadsPerThread = 8;
+constexpr long long kApartElements = 1 << 20;
+constexpr int kRotateThreads = 256;
+// A thread of the page blocks keeps up to four vectors of keys and four of values.
 template <int kDim, int kPage>
-constexpr int append_threads = kPage * kDim > 64 * 256 ? 512 : 256;
-constexpr int kHeadsPerThread = 4;
+constexpr int append_threads = kPage * kDim < 256 * 32 ? 256 : kPage * kDim / 32;
 
-__device__ __forceinline__ bool finite8(const float* x) {
-  bool ok = true;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ok = ok && fabsf(x[i]) <= 3.402823466e38f;
-  return ok;
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// The largest magnitude; NaN if one of the values is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 __device__ __forceinline__ float amax8(const float* x) {
-  float m = 0.0f;
+  float m = fabsf(x[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
+  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(x[i]));
   return m;
+}
+// of eight BF16 values, whose magnitudes are ordered as integers, NaN last
+__device__ __forceinline__ float amax8(const uint4& raw) {
+  const uint32_t m = __vmaxu2(__vmaxu2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu), __vmaxu2(raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu));
+  return __uint_as_float(max(m & 0xffffu, m >> 16) << 16);
 }
 // eight values times a power of two -> eight e4m3 codes
 __device__ __forceinline__ uint2 codes8(const float* x, float inverse) {
@@ -95,10 +105,52 @@ __device__ __forceinline__ int sequence_of_row(const KvBatch& b, int row) {
   return low;
 }
 
+// Queries: kDim / 8 lanes hold one head of one row, kHeadsPerThread heads at once, which share the row's angles.
+template <int kDim, int kThreads>
+__device__ __forceinline__ void rotate_queries(const KvAppend& a, long long block) {
+  constexpr int kPieces = kDim / 8, kRowsPerPass = kThreads / kPieces;
+  const int piece = threadIdx.x % kPieces, slot0 = threadIdx.x / kPieces;
+  const KvShape& shape = a.shape;
+  const int half = shape.rotary >> 4;
+  const int head_groups = (shape.q_heads + kHeadsPerThread - 1) / kHeadsPerThread;
+  const long long work = block * kRowsPerPass + slot0;
+  const int row = static_cast<int>(min(work / head_groups, static_cast<long long>(a.batch.tokens)));
+  const int head0 = static_cast<int>(work % head_groups) * kHeadsPerThread;
+  const bool exists = row < a.batch.tokens;
+  uint4 raw[kHeadsPerThread];
+#pragma unroll
+  for (int h = 0; h < kHeadsPerThread; ++h) {
+    raw[h] = make_uint4(0, 0, 0, 0);
+    if (exists && head0 + h < shape.q_heads)
+      raw[h] = *reinterpret_cast<const uint4*>(a.q.data + row * a.q.row_stride + (head0 + h) * a.q.head_stride + 8 * piece);
+  }
+  int position = -1;
+  if (exists) {
+    const int s = sequence_of_row(a.batch, row);
+    const KvSequence seq = kv_sequence(a.batch, shape, s);
+    if (!seq.bad && row >= seq.row0 && row < seq.row0 + seq.rows) position = seq.length - seq.rows + row - seq.row0;
+  }
+  const bool active = position >= 0 && position < a.positions;
+  Angles angles{};
+  if (active && piece < 2 * half) angles = load_angles(a.rotation + static_cast<size_t>(position) * shape.rotary, piece, half);
+#pragma unroll
+  for (int h = 0; h < kHeadsPerThread; ++h) {
+    float x[8];
+    rotate8<kDim>(raw[h], piece, half, angles, active, x);
+    uint4 w;
+    w.x = static_cast<uint32_t>(float_to_bf16_bits(x[0])) | (static_cast<uint32_t>(float_to_bf16_bits(x[1])) << 16);
+    w.y = static_cast<uint32_t>(float_to_bf16_bits(x[2])) | (static_cast<uint32_t>(float_to_bf16_bits(x[3])) << 16);
+    w.z = static_cast<uint32_t>(float_to_bf16_bits(x[4])) | (static_cast<uint32_t>(float_to_bf16_bits(x[5])) << 16);
+    w.w = static_cast<uint32_t>(float_to_bf16_bits(x[6])) | (static_cast<uint32_t>(float_to_bf16_bits(x[7])) << 16);
+    if (exists && head0 + h < shape.q_heads)
+      *reinterpret_cast<uint4*>(a.q_out + (static_cast<long long>(row) * shape.q_heads + head0 + h) * kDim + 8 * piece) = w;
+  }
+}
+
 // One block per (sequence, touched page, head), then blocks for the queries.  A page and head belongs to one block, which
 // holds all of its new rows in registers between finding the scale and writing the codes: every byte is read once.
 template <int kDim, int kPage>
-__global__ void __launch_bounds__(append_threads<kDim, kPage>)
+__global__ void __launch_bounds__(append_threads<kDim, kPage>, 1024 / append_threads<kDim, kPage>)
 kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
   constexpr int kAppendThreads = append_threads<kDim, kPage>;
   constexpr int kPieces = kDim / 8;                                   // 16-byte vectors of a head
@@ -109,6 +161,7 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
   const int slot0 = threadIdx.x / kPieces;
   const KvShape& shape = a.shape;
   const int half = shape.rotary >> 4;
+  pdl_launch_dependents();       // after what came before this kernel has ended: it is launched without the attribute
 
   if (static_cast<int>(blockIdx.x) < page_blocks) {
     const int head = blockIdx.x % shape.kv_heads;
@@ -140,23 +193,22 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
     }
     float kmax = 0.0f, vmax = 0.0f;
     uint32_t poisoned = 0;
+    const uint32_t head_lanes = kPieces == 32 ? 0xffffffffu : ((1u << (kPieces & 31)) - 1u) << ((threadIdx.x & 31) & ~(kPieces - 1));
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int position = page_start + slot0 + p * kRowsPerPass;
       const bool active = position >= low && position < high;
-      float k[8], v[8];
+      float k[8];
       Angles angles{};
       if (active && piece < 2 * half) angles = load_angles(a.rotation + static_cast<size_t>(position) * shape.rotary, piece, half);
       rotate8<kDim>(kraw[p], piece, half, angles, active, k);
-      unpack8(vraw[p], v);
-      int bad = (finite8(k) && finite8(v)) ? 0 : 1;
-#pragma unroll
-      for (int d = kPieces / 2; d >= 1; d >>= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, d);
-      if (bad) {
+      const float k8 = amax8(k), v8 = amax8(vraw[p]);
+      const uint32_t bad = __ballot_sync(0xffffffffu, !(k8 <= 3.402823466e38f && v8 <= 3.402823466e38f));
+      if ((bad & head_lanes) != 0) {
         poisoned |= 1u << p;
       } else {
-        kmax = fmaxf(kmax, amax8(k));
-        vmax = fmaxf(vmax, amax8(v));
+        kmax = fmaxf(kmax, k8);
+        vmax = fmaxf(vmax, v8);
       }
     }
 #pragma unroll
@@ -227,40 +279,14 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
     return;
   }
 
-  // queries: kPieces lanes hold one head of one row, kHeadsPerThread heads at once, which share the row's angles
-  const int head_groups = (shape.q_heads + kHeadsPerThread - 1) / kHeadsPerThread;
-  const long long work = static_cast<long long>(blockIdx.x - page_blocks) * kRowsPerPass + slot0;
-  const int row = static_cast<int>(min(work / head_groups, static_cast<long long>(a.batch.tokens)));
-  const int head0 = static_cast<int>(work % head_groups) * kHeadsPerThread;
-  const bool exists = row < a.batch.tokens;
-  uint4 raw[kHeadsPerThread];
-#pragma unroll
-  for (int h = 0; h < kHeadsPerThread; ++h) {
-    raw[h] = make_uint4(0, 0, 0, 0);
-    if (exists && head0 + h < shape.q_heads)
-      raw[h] = *reinterpret_cast<const uint4*>(a.q.data + row * a.q.row_stride + (head0 + h) * a.q.head_stride + 8 * piece);
-  }
-  int position = -1;
-  if (exists) {
-    const int s = sequence_of_row(a.batch, row);
-    const KvSequence seq = kv_sequence(a.batch, shape, s);
-    if (!seq.bad && row >= seq.row0 && row < seq.row0 + seq.rows) position = seq.length - seq.rows + row - seq.row0;
-  }
-  const bool active = position >= 0 && position < a.positions;
-  Angles angles{};
-  if (active && piece < 2 * half) angles = load_angles(a.rotation + static_cast<size_t>(position) * shape.rotary, piece, half);
-#pragma unroll
-  for (int h = 0; h < kHeadsPerThread; ++h) {
-    float x[8];
-    rotate8<kDim>(raw[h], piece, half, angles, active, x);
-    uint4 w;
-    w.x = static_cast<uint32_t>(float_to_bf16_bits(x[0])) | (static_cast<uint32_t>(float_to_bf16_bits(x[1])) << 16);
-    w.y = static_cast<uint32_t>(float_to_bf16_bits(x[2])) | (static_cast<uint32_t>(float_to_bf16_bits(x[3])) << 16);
-    w.z = static_cast<uint32_t>(float_to_bf16_bits(x[4])) | (static_cast<uint32_t>(float_to_bf16_bits(x[5])) << 16);
-    w.w = static_cast<uint32_t>(float_to_bf16_bits(x[6])) | (static_cast<uint32_t>(float_to_bf16_bits(x[7])) << 16);
-    if (exists && head0 + h < shape.q_heads)
-      *reinterpret_cast<uint4*>(a.q_out + (static_cast<long long>(row) * shape.q_heads + head0 + h) * kDim + 8 * piece) = w;
-  }
+  if (a.q.data != nullptr) rotate_queries<kDim, kAppendThreads>(a, static_cast<long long>(blockIdx.x) - page_blocks);
+}
+
+template <int kDim>
+__global__ void __launch_bounds__(kRotateThreads)
+kv_rotate_kernel(const KvAppend a) {
+  rotate_queries<kDim, kRotateThreads>(a, blockIdx.x);
+  pdl_wait();          // the page kernel has ended when this one does: whoever waits for this one waits for both
 }
 
 template <int kDim, int kPage>
@@ -268,12 +294,19 @@ cudaError_t launch(const KvAppend& a, cudaStream_t stream) {
   constexpr int kAppendThreads = append_threads<kDim, kPage>;
   const int columns = (a.batch.max_new + kPage - 2) / kPage + 1;      // pages that max_new consecutive tokens can touch
   const long long page_blocks = static_cast<long long>(columns) * a.shape.kv_heads * a.batch.sequences;
-  const long long query_work = static_cast<long long>(a.batch.tokens) * ((a.shape.q_heads + kHeadsPerThread - 1) / kHeadsPerThread);
-  const int work_per_block = kAppendThreads / (kDim / 8);
-  const long long query_blocks = a.q.data != nullptr ? (query_work + work_per_block - 1) / work_per_block : 0;
-  if (page_blocks + query_blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  kv_append_kernel<kDim, kPage><<<static_cast<unsigned>(page_blocks + query_blocks), kAppendThreads, 0, stream>>>(a, static_cast<int>(page_blocks), columns);
-  return cudaGetLastError();
+  const long long query_work = a.q.data != nullptr ? static_cast<long long>(a.batch.tokens) * ((a.shape.q_heads + kHeadsPerThread - 1) / kHeadsPerThread) : 0;
+  // Few queries are rotated by blocks of the same launch.  Many are a stream of their own beside the page blocks, whose registers
+  // would leave too few of the stream's bytes in flight.
+  const bool apart = query_work * kHeadsPerThread * kDim > kApartElements;
+  const long long query_blocks = apart ? 0 : (query_work + kAppendThreads / (kDim / 8) - 1) / (kAppendThreads / (kDim / 8));
+  const long long rotate_blocks = (query_work + kRotateThreads / (kDim / 8) - 1) / (kRotateThreads / (kDim / 8));
+  if (page_blocks + query_blocks > 0x7fffffffll || rotate_blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  KvAppend pages = a;
+  if (apart) pages.q.data = nullptr;
+  kv_append_kernel<kDim, kPage><<<static_cast<unsigned>(page_blocks + query_blocks), kAppendThreads, 0, stream>>>(pages, static_cast<int>(page_blocks), columns);
+  const cudaError_t error = cudaGetLastError();
+  if (error != cudaSuccess || !apart) return error;
+  return launch_pdl(kv_rotate_kernel<kDim>, dim3(static_cast<unsigned>(rotate_blocks)), dim3(kRotateThreads), 0, stream, a);
 }
 
 template <int kDim>
