@@ -268,6 +268,11 @@ def _stream(torch: Any) -> c_void_p:
     return c_void_p(int(torch.cuda.current_stream().cuda_stream))
 
 
+def _raw_stream(torch: Any) -> int:
+    """The current stream's handle without a Stream object, which takes 3 us to build: as long as the launch itself."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
 # reference weight-dict keys (four_layer_mini_engine.py: weights["router"],
 # ["expert_gate_up"], ["expert_down"], ["shared_gate"], ["shared_gate_proj"],
 # ["shared_up_proj"], ["shared_down_proj"], ["post_attention_layernorm"])
@@ -790,36 +795,38 @@ class KvCache:
         return KvBatch(page_table, lengths, row_offsets, tokens, max_new_tokens)
 
     # -- launches ------------------------------------------------------------
-    def _rows(self, tensor: Any, name: str, tokens: int, shape: tuple[int, int]) -> KvRows:
-        if tensor.dtype is not self._torch.bfloat16 or not tensor.is_cuda or tuple(tensor.shape) != (tokens, *shape) or tensor.stride(2) != 1:
-            raise ValueError(f"{name} must be a CUDA bfloat16 tensor [{tokens}, {shape[0]}, {shape[1]}] with contiguous heads, got "
+    def _rows(self, tensor: Any, name: str, shape: tuple[int, int, int]) -> KvRows:
+        row_stride, head_stride, stride = tensor.stride() if tensor.dim() == 3 else (0, 0, 0)
+        if tensor.dtype is not self._torch.bfloat16 or not tensor.is_cuda or tensor.shape != shape or stride != 1:
+            raise ValueError(f"{name} must be a CUDA bfloat16 tensor {list(shape)} with contiguous heads, got "
                              f"{tensor.dtype} {list(tensor.shape)} with strides {list(tensor.stride())}")
-        row_stride, head_stride, _ = tensor.stride()
         return KvRows(tensor.data_ptr(), row_stride, head_stride)
+
+    def _out(self, out: Any, q: Any, name: str) -> Any:
+        if out is None:
+            return self._torch.empty_like(q, memory_format=self._torch.contiguous_format)
+        if out.dtype is not self._torch.bfloat16 or not out.is_cuda or out.shape != q.shape or not out.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous CUDA bfloat16 tensor {list(q.shape)}")
+        return out
 
     def append(self, layer: int, batch: KvBatch, k: Any, v: Any, q: Any = None, q_out: Any = None) -> Any:
         """Rotates k and stores it and v; with q returns the rotated queries [tokens, q_heads, head_dim].  k, v and q may be views
         into one row of a fused projection."""
-        torch, tokens = self._torch, batch.tokens
-        k_rows, v_rows = self._rows(k, "k", tokens, self._kv_shape), self._rows(v, "v", tokens, self._kv_shape)
+        kv_shape = (batch.tokens, *self._kv_shape)
+        k_rows, v_rows = self._rows(k, "k", kv_shape), self._rows(v, "v", kv_shape)
         q_rows = None
         if q is not None:
-            q_rows = self._rows(q, "q", tokens, self._q_shape)
-            if q_out is None:
-                q_out = torch.empty((tokens, *self._q_shape), dtype=torch.bfloat16, device=q.device)
+            q_rows = self._rows(q, "q", (batch.tokens, *self._q_shape))
+            q_out = self._out(q_out, q, "q_out")
         self.lib.check(self.lib.aima_moe_kv_append_launch(
-            self.handle, layer, batch.ref, k_rows, v_rows, q_rows, None if q_out is None else _ptr(q_out), _stream(torch)))
+            self.handle, layer, batch.ref, k_rows, v_rows, q_rows, None if q is None else q_out.data_ptr(), _raw_stream(self._torch)))
         return q_out
 
     def attention(self, layer: int, batch: KvBatch, q: Any, out: Any = None) -> Any:
         """Causal attention of the batch's rows over the cache (after append): [tokens, q_heads, head_dim]."""
-        torch = self._torch
-        q_rows = self._rows(q, "q", batch.tokens, self._q_shape)
-        if out is None:
-            out = torch.empty((batch.tokens, *self._q_shape), dtype=torch.bfloat16, device=q.device)
-        elif out.dtype is not torch.bfloat16 or tuple(out.shape) != (batch.tokens, *self._q_shape):
-            raise ValueError(f"out must be bfloat16 [{batch.tokens}, {self._q_shape[0]}, {self._q_shape[1]}]")
-        self.lib.check(self.lib.aima_moe_kv_attention_launch(self.handle, layer, batch.ref, q_rows, _ptr(out), _stream(torch)))
+        q_rows = self._rows(q, "q", (batch.tokens, *self._q_shape))
+        out = self._out(out, q, "out")
+        self.lib.check(self.lib.aima_moe_kv_attention_launch(self.handle, layer, batch.ref, q_rows, out.data_ptr(), _raw_stream(self._torch)))
         return out
 
     def sync(self) -> None:
@@ -853,25 +860,33 @@ def verify_drafts(target: Any, draft_tokens: Any, uniforms: Any, draft_probabili
     if target.dim() != 3:
         raise ValueError("target must be [sequences, drafts + 1, vocabulary]")
     sequences, rows, vocabulary = target.shape
-    for name, tensor, dtype, shape in (
-            ("target", target, torch.float32, (sequences, rows, vocabulary)), ("draft_tokens", draft_tokens, torch.int32, (sequences, rows - 1)),
-            ("uniforms", uniforms, torch.float32, (sequences, rows)),
-            ("draft_probabilities", draft_probabilities, torch.float32, (sequences, rows - 1, vocabulary)),
-            ("draft_counts", draft_counts, torch.int32, (sequences,)), ("cache_lengths", cache_lengths, torch.int32, (sequences,))):
-        if tensor is not None and (tensor.dtype is not dtype or tuple(tensor.shape) != shape or not tensor.is_cuda):
+    drafts = (sequences, rows - 1)
+
+    def check(name: str, tensor: Any, dtype: Any, shape: tuple) -> None:
+        if tensor.dtype is not dtype or tensor.shape != shape or not tensor.is_cuda:
             raise ValueError(f"{name} must be a CUDA {dtype} tensor {list(shape)}, got {tensor.dtype} {list(tensor.shape)}")
+
+    check("target", target, torch.float32, target.shape)
+    check("draft_tokens", draft_tokens, torch.int32, drafts)
+    check("uniforms", uniforms, torch.float32, (sequences, rows))
+    if draft_probabilities is not None:
+        check("draft_probabilities", draft_probabilities, torch.float32, (*drafts, vocabulary))
+    for name, tensor in (("draft_counts", draft_counts), ("cache_lengths", cache_lengths)):
+        if tensor is not None:
+            check(name, tensor, torch.int32, (sequences,))
     for name, tensor in (("target", target), ("draft_probabilities", draft_probabilities)):
         if tensor is not None and vocabulary > 1 and tensor.stride(2) != 1:
             raise ValueError(f"rows of {name} must be contiguous")
-    out = torch.empty((sequences, rows + 1 if cache_lengths is None else rows + 2), dtype=torch.int32, device=target.device)
-    flat = out.view(-1)
-    accepted, tokens = flat[:sequences], flat[sequences:sequences * (rows + 1)].view(sequences, rows)
-    new_lengths = None if cache_lengths is None else flat[sequences * (rows + 1):]
+    # accepted, tokens and lengths in one allocation
+    out = torch.empty_strided((sequences * (rows + 2),), (1,), dtype=torch.int32, device=target.device)
+    accepted = out.as_strided((sequences,), (1,), 0)
+    tokens = out.as_strided((sequences, rows), (rows, 1), sequences)
+    new_lengths = None if cache_lengths is None else out.as_strided((sequences,), (1,), sequences * (rows + 1))
     has_draft = draft_probabilities is not None
     call = VerifyDrafts(
         ctypes.sizeof(VerifyDrafts), sequences, rows - 1, vocabulary, target.data_ptr(), target.stride(0), target.stride(1),
         draft_probabilities.data_ptr() if has_draft else None, draft_probabilities.stride(0) if has_draft else 0,
         draft_probabilities.stride(1) if has_draft else 0, _ptr(draft_tokens), _ptr(draft_counts), _ptr(uniforms), _ptr(cache_lengths),
         accepted.data_ptr(), tokens.data_ptr(), None if new_lengths is None else new_lengths.data_ptr())
-    lib.check(lib.aima_moe_verify_drafts_launch(call, _stream(torch)))
+    lib.check(lib.aima_moe_verify_drafts_launch(call, _raw_stream(torch)))
     return (accepted, tokens) if new_lengths is None else (accepted, tokens, new_lengths)
