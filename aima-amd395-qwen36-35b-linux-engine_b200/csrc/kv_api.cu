@@ -164,8 +164,8 @@ AIMA_EXPORT int aima_moe_kv_prepare(const aima_moe_kv_config* config, aima_moe_k
                            static_cast<int>(config->pages)};
   const double scale = config->softmax_scale != 0.0f ? config->softmax_scale : 1.0 / std::sqrt(static_cast<double>(config->head_dim));
   h->scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-  error = cudaMalloc(&h->status, 256 + aima::kv_workspace_bytes(h->shape, static_cast<int>(config->max_sequences)));
-  if (error == cudaSuccess) error = cudaMemset(h->status, 0, 256);
+  error = cudaMalloc(&h->status, 256 + aima::kv_workspace_bytes(h->shape));
+  if (error == cudaSuccess) error = cudaMemset(h->status, 0, 256 + aima::kv_counter_bytes());
   if (error != cudaSuccess) {
     cudaFree(h->status);
     delete h;
@@ -253,7 +253,7 @@ AIMA_EXPORT int aima_moe_kv_attention_launch(aima_moe_kv* h, uint32_t layer, con
   a.out = static_cast<__nv_bfloat16*>(out);
   a.scale_log2 = h->scale_log2;
   a.status = h->status;
-  const cudaError_t error = aima::kv_attention(a, h->maps[layer], reinterpret_cast<uint8_t*>(h->status) + 256, static_cast<int>(h->config.max_sequences), h->sm_count, static_cast<cudaStream_t>(stream));
+  const cudaError_t error = aima::kv_attention(a, h->maps[layer], reinterpret_cast<uint8_t*>(h->status) + 256, h->sm_count, static_cast<cudaStream_t>(stream));
   if (error != cudaSuccess) return kv_fail_cuda(error, "kv attention launch");
   h->last_stream = static_cast<cudaStream_t>(stream);
   return AIMA_MOE_OK;
@@ -266,7 +266,8 @@ AIMA_EXPORT int aima_moe_kv_sync(aima_moe_kv* h) {
   cudaError_t error = cudaMemcpyAsync(&status, h->status, sizeof status, cudaMemcpyDeviceToHost, h->last_stream);
   if (error == cudaSuccess) error = cudaStreamSynchronize(h->last_stream);
   if (error == cudaSuccess && status != 0) {
-    error = cudaMemsetAsync(h->status, 0, sizeof status, h->last_stream);
+    // after a wait that ran out the counters of the joins may be anything
+    error = cudaMemsetAsync(h->status, 0, 256 + aima::kv_counter_bytes(), h->last_stream);
     if (error == cudaSuccess) error = cudaStreamSynchronize(h->last_stream);
   }
   if (error != cudaSuccess) return kv_fail_cuda(error, "kv sync");

@@ -1,5 +1,5 @@
-// What the attention kernels over the paged 8-bit cache share: tensor maps, the division of the work and the join of what
-// was divided.
+// What the attention kernels over the paged 8-bit cache share: tensor maps, the workspace of units that several blocks work on,
+// and the join of their parts.
 #pragma once
 
 #include "kv_cache.cuh"
@@ -9,61 +9,170 @@ namespace aima {
 
 constexpr int kKvTile = 128;            // positions of the cache per step
 constexpr int kKvMaxBlocks = 160;       // blocks of an attention kernel at most (one per SM)
+constexpr int kKvPartRows = 128;
 
 struct KvMaps {
   CUtensorMap keys, values;             // [pages * kv_heads * page_tokens, head_dim] bytes, boxes of one page x up to 128 bytes
 };
 
-// The list of work: for every sequence, head by head and row tile by row tile, the tiles of the cache that its rows see.
-// Block c of G takes the tiles [total c / G, total (c + 1) / G) of it, so that all stream the same amount; a unit (the tiles
-// of one sequence, head and row tile) that ends up in several blocks leaves its part in the workspace of each, and
-// kv_join_kernel puts the parts together.
-__host__ __device__ inline long long kv_block_begin(long long total, int block, int blocks) { return total * block / blocks; }
-__host__ __device__ inline int kv_block_of(long long total, long long tile, int blocks) {
-  return static_cast<int>(((tile + 1) * blocks - 1) / total);
-}
-
 // Where a block of the prompt kernel begins: the unit and the tile inside it, and the place in the list in units of its cost.
 struct alignas(16) KvStart {
-  long long at;
+  long long at, total;
   int sequence, row_tile, head, tile;
-  int row0, rows, length, unused;       // of the sequence
+  int row0, rows, length;               // of the sequence
+  int blocks;                           // the shares of the list
 };
 
-// One part: rows x head_dim sums in FP32, and per row the reference maximum (log2) and the sum of the weights.
-// A block has two: of the unit it begins in the middle (or that covers its whole share), and of the one it does not finish.
+// A unit is the tiles of the cache that a row tile (up to 128 rows: query heads of one key/value head x new tokens) sees.
+// The kernels go through the list of all units' tiles, every block through an equal share; a unit that ends up in several
+// blocks leaves its part in the workspace of each, and those blocks put the parts together, each a share of the results
+// (kv_join).  A block has two parts: of the unit that it begins in the middle, and of the one that it does not finish.
 struct KvWorkspace {
-  float* sums;            // [2 * kKvMaxBlocks][rows_per_part][head_dim]
-  float2* weights;        // [2 * kKvMaxBlocks][rows_per_part]: maximum, sum
-  long long* prefix;      // few rows: [sequences + 1] tiles before each sequence, left by block 0 for kv_join_kernel
-  KvStart* starts;        // prompts: [blocks + 1]
-  int rows_per_part;
+  unsigned* arrived;      // [2 * kKvMaxBlocks], by the block that begins the unit: parts written, parts joined; zero between launches
+  float2* weights;        // [2 * kKvMaxBlocks][kKvPartRows]: reference maximum (log2), sum of the weights
+  float* sums;            // [2 * kKvMaxBlocks][head_dim / 4][kKvPartRows][4]
+  KvStart* starts;        // [kKvMaxBlocks + 1], for prompts of many row tiles
 };
-// part of a unit that begins at tile `first` of the list, in block `block`
-__host__ __device__ inline int kv_part(long long first, long long block_begin, int block) { return 2 * block + (first >= block_begin ? 1 : 0); }
 
 struct KvAttentionPlan {
   KvAttention a;
   KvWorkspace work;
   int blocks;
-  int tile_rows;          // rows (query heads of one key/value head x new tokens) of a row tile
+  int tile_rows;          // rows that a sequence has at most for one key/value head
   int tile_tokens;        // prompts: new tokens of a row tile
   unsigned long long wait_limit_ns;
 };
 
-// A unit of the prompt kernel: the rows of `tokens` new tokens of a sequence, for the query heads of one key/value head.
-struct KvUnit {
-  int tokens;             // new tokens of the row tile
-  int first;              // position of the first one (negative: it sees nothing)
-  int tiles;              // tiles of the cache that the last one sees
+// What a block keeps of a unit that it shares with others until it has written its last part; parts = 0: none.
+struct KvShared {
+  int first_block, parts;       // blocks first_block .. first_block + parts - 1
+  int mine;                     // which of the parts this block wrote
+  int rows;
+  int row0, head;               // of q: the unit's first row and query head
 };
-__device__ __forceinline__ KvUnit kv_unit(const KvSequence& seq, int row_tile, int tile_tokens) {
-  KvUnit u;
-  const int before = row_tile * tile_tokens;
-  u.tokens = min(tile_tokens, seq.rows - before);
-  u.first = seq.length - seq.rows + before;
-  u.tiles = max(0, u.first + u.tokens + kKvTile - 1) / kKvTile;
-  return u;
+
+__device__ __forceinline__ size_t kv_part_index(int block, bool begins) { return 2 * block + (begins ? 1 : 0); }
+__device__ __forceinline__ float2* kv_part_weight(const KvWorkspace& work, size_t part, int row) { return work.weights + part * kKvPartRows + row; }
+template <int kDim>
+__device__ __forceinline__ float* kv_part_sum(const KvWorkspace& work, size_t part, int row, int d) {       // d: a multiple of 4
+  return work.sums + part * kKvPartRows * kDim + (static_cast<size_t>(d >> 2) * kKvPartRows + row) * 4;
+}
+
+// The block's part has been written, before a barrier of the block that this thread has passed.
+__device__ __forceinline__ void kv_arrive(const KvWorkspace& work, const KvShared& unit) {
+  __threadfence();
+  atomicAdd(work.arrived + 2 * unit.first_block, 1u);
+}
+
+// Joins a unit's parts: waits until all have been written, then takes the `mine`-th share of its results.  Called by all
+// threads of a block.  The blocks of the launch are all resident (it is a cooperative one), and none waits before its own parts
+// are written; the wait has its limit all the same.  A result is four neighbouring elements of a row; 1 .. 32 lanes share the
+// parts of one, so that they are read by a few instructions, in the same order in every launch.
+template <int kDim, int kThreads>
+__device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace& work, const KvShared& unit, unsigned long long limit_ns, int* verdict) {
+  unsigned* arrived = work.arrived + 2 * unit.first_block;
+  if (threadIdx.x == 0) {
+    const unsigned long long start = global_timer_ns();
+    int ok = 1;
+    for (;;) {
+      unsigned seen;
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(arrived) : "memory");
+      if (seen >= static_cast<unsigned>(unit.parts)) break;
+      if (global_timer_ns() - start > limit_ns) {
+        atomicOr(a.status, kKvTimeout);
+        ok = 0;
+        break;
+      }
+    }
+    *verdict = ok;
+  }
+  __syncthreads();
+  const bool ok = *verdict != 0;
+  if (ok) {
+    int lanes = 1;
+    while (lanes < 32 && 4 * lanes < unit.parts) lanes *= 2;
+    const int results = unit.rows * (kDim / 4);
+    const int begin = results * unit.mine / unit.parts, end = results * (unit.mine + 1) / unit.parts;
+    const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes;
+    for (int i0 = begin; i0 < end; i0 += kThreads / lanes) {
+      const int i = min(i0 + slot, end - 1);                      // whole warps stay together
+      const int row = i % unit.rows, d = 4 * (i / unit.rows);
+      float4 x[5];
+      float2 w[5];
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 5; ++k) {
+        const int p = lane + k * lanes;
+        w[k] = make_float2(-INFINITY, 0.0f);
+        x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (p < unit.parts) {
+          const size_t part = kv_part_index(unit.first_block + p, p == 0);
+          w[k] = __ldcg(kv_part_weight(work, part, row));
+          x[k] = __ldcg(reinterpret_cast<const float4*>(kv_part_sum<kDim>(work, part, row, d)));
+        }
+        top = fmaxf(top, w[k].x);
+      }
+      for (int step = lanes >> 1; step >= 1; step >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+      if (top == -INFINITY) top = 0.0f;                           // nothing seen, or nothing but NaN
+      float sum = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < 5; ++k) {
+        const float f = fast_exp2(w[k].x - top);
+        sum += w[k].x == -INFINITY ? w[k].y : w[k].y * f;
+        acc.x = fmaf(x[k].x, f, acc.x);
+        acc.y = fmaf(x[k].y, f, acc.y);
+        acc.z = fmaf(x[k].z, f, acc.z);
+        acc.w = fmaf(x[k].w, f, acc.w);
+      }
+      for (int step = lanes >> 1; step >= 1; step >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, step);
+        acc.x += __shfl_xor_sync(0xffffffffu, acc.x, step);
+        acc.y += __shfl_xor_sync(0xffffffffu, acc.y, step);
+        acc.z += __shfl_xor_sync(0xffffffffu, acc.z, step);
+        acc.w += __shfl_xor_sync(0xffffffffu, acc.w, step);
+      }
+      if (lane == 0 && i0 + slot < end) {
+        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int token = row / a.shape.group, g = row - token * a.shape.group;
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inverse, acc.y * inverse), hi = __floats2bfloat162_rn(acc.z * inverse, acc.w * inverse);
+        *reinterpret_cast<uint2*>(a.out + (static_cast<long long>(unit.row0 + token) * a.shape.q_heads + unit.head + g) * kDim + d) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      }
+    }
+    // the last to leave puts the counters back
+    if (threadIdx.x == 0 && atomicAdd(arrived + 1, 1u) == static_cast<unsigned>(unit.parts) - 1u) {
+      arrived[0] = 0;
+      arrived[1] = 0;
+    }
+  }
+  __syncthreads();
+}
+
+// Rows [row0, row0 + rows) of the output are zero: they see nothing.  Called by all threads of a block.
+template <int kDim, int kThreads>
+__device__ __forceinline__ void kv_zero_rows(const KvAttention& a, int row0, int rows) {
+  uint4* out = reinterpret_cast<uint4*>(a.out + static_cast<long long>(row0) * a.shape.q_heads * kDim);
+  const long long pieces = static_cast<long long>(rows) * a.shape.q_heads * (kDim / 8);
+  for (long long i = threadIdx.x; i < pieces; i += kThreads) out[i] = make_uint4(0, 0, 0, 0);
+}
+
+// Launches a kernel whose blocks are all resident, with programmatic serialisation like launch_pdl.
+template <typename... KernelArgs, typename... Args>
+inline cudaError_t launch_resident(void (*kernel)(KernelArgs...), dim3 grid, dim3 block, size_t smem_bytes, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = smem_bytes;
+  config.stream = stream;
+  cudaLaunchAttribute attribute[2];
+  attribute[0].id = cudaLaunchAttributeCooperative;
+  attribute[0].val.cooperative = 1;
+  attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute;
+  config.numAttrs = 2;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<KernelArgs>(args)...);
 }
 
 cudaError_t kv_decode(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream);

@@ -92,9 +92,10 @@ struct KvAttention {
   int* status;
 };
 struct KvMaps;             // tensor maps of a layer's cache
-size_t kv_workspace_bytes(const KvShape& shape, int max_sequences);
+size_t kv_workspace_bytes(const KvShape& shape);
+size_t kv_counter_bytes();  // at its begin, zero between launches
 bool kv_make_maps(const KvShape& shape, const KvLayer& layer, KvMaps* maps);
-cudaError_t kv_attention(const KvAttention& args, const KvMaps& maps, void* workspace, int max_sequences, int sm_count, cudaStream_t stream);
+cudaError_t kv_attention(const KvAttention& args, const KvMaps& maps, void* workspace, int sm_count, cudaStream_t stream);
 
 cudaError_t verify_drafts(const aima_moe_verify_drafts& call, cudaStream_t stream);
 

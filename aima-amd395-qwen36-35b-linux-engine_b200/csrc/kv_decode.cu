@@ -5,7 +5,7 @@
 // A page's scale of V is carried by the weight, so that V enters the product as the codes that lie in memory; its share of
 // the sum of the weights is divided out again in FP32.
 //
-// Bound: the cache is read once, 2 head_dim bytes per position and key/value head, and the products with the 1 .. 64 rows
+// Bound: the cache is read once, 2 head_dim bytes per position and key/value head, and the products with the 1 .. 16 rows
 // that share them are small.  So the CACHE is the M side of both products, as it comes by TMA, and the rows are the N side:
 //   S^T[128 positions, rows]   = K[128, head_dim] . Q^T            K-major A
 //   O^T[head_dim, rows]       += V^T[head_dim, 128] . P^T           MN-major A: V's rows are the K dimension
@@ -36,7 +36,7 @@ struct Decode {
   static constexpr int kPanels = kDim / kRowBytes;
   static constexpr int kPanelBytes = kKvTile * kRowBytes;
   static constexpr int kSlotBytes = kKvTile * kDim;
-  static constexpr int kSlots = kDim == 256 ? (kRows <= 16 ? 6 : kRows == 32 ? 5 : 4) : 8;
+  static constexpr int kSlots = kDim == 256 ? 6 : 8;
   static constexpr int kWeightRows = kRows < 16 ? 16 : kRows;           // N of the second product
   static constexpr int kQueryBytes = 2 * kRows * kDim;
   static constexpr int kWeightBytes = kWeightRows * kKvTile;            // one term of one buffer
@@ -51,6 +51,7 @@ struct Decode {
 struct SegmentInfo {
   int length;               // positions of the sequence
   int rows;                 // rows of the unit
+  int row0;                 // of q, the first one's
 };
 
 template <int kRows>
@@ -63,6 +64,8 @@ struct Small {              // shared memory that is not an operand
   long long out_at[2][kRows];
   SegmentInfo info[2];
   long long scan[kThreads / 32];
+  KvShared shared[2];       // the units divided at the share's begin and at its end
+  int verdict;
   uint32_t tmem;
   int abort_flag;
 };
@@ -136,6 +139,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
     mbar_init(smem_u32(&sm.q_empty), 1);
     mbar_init(smem_u32(&sm.drain), 1);
     sm.abort_flag = 0;
+    sm.shared[0].parts = sm.shared[1].parts = 0;
     mbar_fence_init();
   }
   if (warp == 2) tmem_alloc(smem_u32(&sm.tmem), 512);
@@ -183,16 +187,16 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
   const long long total = prefix[a.batch.sequences];
-  if (blockIdx.x == 0) {
-    for (int s = threadIdx.x; s <= a.batch.sequences; s += kThreads) plan.work.prefix[s] = prefix[s];
-  }
+  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), total));        // with a share; none is empty
   Walk walk;
   walk.prefix = prefix;
   walk.heads = shape.kv_heads;
-  walk.at = kv_block_begin(total, blockIdx.x, gridDim.x);
-  walk.end = kv_block_begin(total, blockIdx.x + 1, gridDim.x);
+  walk.at = walk.end = 0;
+  if (static_cast<int>(blockIdx.x) < blocks) {
+    walk.at = total * blockIdx.x / blocks;
+    walk.end = total * (blockIdx.x + 1) / blocks;
+  }
   walk.sequence = 0;
-  const long long block_begin = walk.at;
   auto wait = [&](unsigned long long* bar, uint32_t parity) {
     if (mbar_wait_bounded_warp(smem_u32(bar), parity, abort_flag, plan.wait_limit_ns)) return true;
     if (lane == 0) atomicOr(a.status, kKvTimeout);
@@ -317,7 +321,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
       const KvSequence seq = kv_sequence(a.batch, shape, walk.sequence);
       const int rows = seq.rows * shape.group, which = segment & 1;
       if (!wait(&sm.info_empty[which], ((segment >> 1) & 1) ^ 1) || !wait(&sm.q_empty, (segment & 1) ^ 1)) break;
-      if (warp == 2 && lane == 0) sm.info[which] = SegmentInfo{seq.length, rows};
+      if (warp == 2 && lane == 0) sm.info[which] = SegmentInfo{seq.length, rows, seq.row0};
 #pragma unroll 4
       for (int r = warp - 2; r < kRows; r += 2) {
         const int i = r / shape.group, g = r - i * shape.group;
@@ -538,15 +542,21 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
       softmax_barrier();
       wait(&sm.o_done[last], ((tile - 1) >> 1) & 1);
       tc_fence_after();
-      const bool whole = walk.whole();
-      const int part = kv_part(walk.at - walk.tile0, block_begin, blockIdx.x);
+      const bool whole = walk.whole(), begins = walk.tile0 == 0;
+      const size_t part = kv_part_index(blockIdx.x, begins);
       const int rows = sm.info[which].rows;
       if (!whole && token == 0) {
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
           const float4 s4 = *reinterpret_cast<const float4*>(sm.part[last ^ 1][r]);
-          if (r < rows) plan.work.weights[static_cast<size_t>(part) * plan.work.rows_per_part + r] = make_float2(top[r], (s4.x + s4.y) + (s4.z + s4.w));
+          if (r < rows) *kv_part_weight(plan.work, part, r) = make_float2(top[r], (s4.x + s4.y) + (s4.z + s4.w));
         }
+        // the block of tile t is the last c with total c / blocks <= t
+        const long long first = walk.at - walk.tile0;
+        const int block0 = begins ? static_cast<int>(blockIdx.x) : static_cast<int>(((first + 1) * blocks - 1) / total);
+        const int block1 = static_cast<int>(((first + walk.unit_tiles) * blocks - 1) / total);
+        sm.shared[begins ? 1 : 0] = KvShared{block0, block1 - block0 + 1, static_cast<int>(blockIdx.x) - block0, rows, sm.info[which].row0,
+                                             walk.head * shape.group};
       }
 #pragma unroll
       for (int panel = 0; panel < L::kOutPanels; ++panel) {
@@ -568,7 +578,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
               const float sum = (s4.x + s4.y) + (s4.z + s4.w);
               a.out[sm.out_at[which][r] + d] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : o / sum);
             } else {
-              plan.work.sums[(static_cast<size_t>(part) * plan.work.rows_per_part + r) * kDim + d] = o;
+              kv_part_sum<kDim>(plan.work, part, r, d & ~3)[d & 3] = o;
             }
           }
         }
@@ -591,6 +601,20 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
     __syncthreads();
   }
   if (warp == 2) tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i)
+      if (sm.shared[i].parts > 0) kv_arrive(plan.work, sm.shared[i]);
+  }
+  // sequences without anything in the cache
+  for (int s = blockIdx.x; s < a.batch.sequences; s += gridDim.x) {
+    if (prefix[s + 1] != prefix[s]) continue;
+    const KvSequence seq = kv_sequence(a.batch, shape, s);
+    kv_zero_rows<kDim, kThreads>(a, seq.row0, seq.rows);
+  }
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    if (sm.shared[i].parts > 0) kv_join<kDim, kThreads>(a, plan.work, sm.shared[i], plan.wait_limit_ns, &sm.verdict);
+  }
 }
 
 template <int kDim, int kRows>
@@ -599,15 +623,12 @@ cudaError_t launch(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t
   static_assert(bytes <= 227 * 1024, "more shared memory than a block can have");
   const cudaError_t error = opt_in_dynamic_smem<kv_decode_kernel<kDim, kRows>>(bytes);
   if (error != cudaSuccess) return error;
-  return launch_pdl(kv_decode_kernel<kDim, kRows>, dim3(plan.blocks), dim3(kThreads), bytes, stream, maps, plan);
+  return launch_resident(kv_decode_kernel<kDim, kRows>, dim3(plan.blocks), dim3(kThreads), bytes, stream, maps, plan);
 }
 
 template <int kDim>
 cudaError_t launch_rows(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
-  if (plan.tile_rows <= 8) return launch<kDim, 8>(plan, maps, stream);
-  if (plan.tile_rows <= 16) return launch<kDim, 16>(plan, maps, stream);
-  if (plan.tile_rows <= 32) return launch<kDim, 32>(plan, maps, stream);
-  return launch<kDim, 64>(plan, maps, stream);
+  return plan.tile_rows <= 8 ? launch<kDim, 8>(plan, maps, stream) : launch<kDim, 16>(plan, maps, stream);
 }
 
 }  // namespace

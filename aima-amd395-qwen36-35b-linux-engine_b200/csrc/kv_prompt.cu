@@ -54,9 +54,27 @@ struct Small {
   float row_scale[128];
   float half_top[2][2][128];               // per tile parity, half and row
   float sum[2][128];
+  KvStart cut[2];
+  KvShared shared[2];                      // the units divided at the share's begin and at its end
+  int verdict;
   uint32_t tmem;
   int abort_flag;
 };
+
+// A unit of the list: the rows of `tokens` new tokens of a sequence, for the query heads of one key/value head.
+struct KvUnit {
+  int tokens;             // new tokens of the row tile
+  int first;              // position of the first one (negative: it sees nothing)
+  int tiles;              // tiles of the cache that the last one sees
+};
+__device__ __forceinline__ KvUnit kv_unit(const KvSequence& seq, int row_tile, int tile_tokens) {
+  KvUnit u;
+  const int before = row_tile * tile_tokens;
+  u.tokens = min(tile_tokens, seq.rows - before);
+  u.first = seq.length - seq.rows + before;
+  u.tiles = max(0, u.first + u.tokens + kKvTile - 1) / kKvTile;
+  return u;
+}
 
 // A block's share of the list, unit by unit: from one cut to the next.
 struct Walk {
@@ -124,58 +142,61 @@ __device__ __forceinline__ void split_weights(uint32_t h0, uint32_t h1, uint32_t
   terms[2 * stride] = __byte_perm(h0 + 0x00800080u, h1 + 0x00800080u, 0x7531);
 }
 
-// Cuts the list into `blocks` shares of equal cost.  The list runs over sequences, their row tiles, the key/value heads and the
+// Cuts the list into shares of equal cost.  The list runs over sequences, their row tiles, the key/value heads and the
 // tiles of the cache; a unit costs its tiles and kUnitCost more, for its queries, the first scores that nothing overlaps and
 // its results.  A cut within kSnap tiles of a unit's end moves there: a divided unit costs all that twice, and the join.  One
-// block; items are row tiles.
-constexpr int kPlanThreads = 1024;
+// block; items are row tiles, one for a thread at a time.  emit(c, start) is called for the cuts c in [cut0, cut1], by some
+// thread; nothing(row0, rows) for an item whose rows see nothing.
 constexpr int kUnitCost = 3;
 constexpr int kSnap = 2;
-__global__ void __launch_bounds__(kPlanThreads)
-kv_plan_kernel(const KvAttentionPlan plan) {
-  __shared__ int first_item[AIMA_MOE_KV_MAX_SEQUENCES + 1];
-  __shared__ long long warp_sum[kPlanThreads / 32];
-  long long total = 0;
-  pdl_enter();
+template <int kThreadCount>
+struct PlanMemory {
+  int first_item[AIMA_MOE_KV_MAX_SEQUENCES + 1];
+  long long warp_sum[kThreadCount / 32];
+};
+template <int kThreadCount, typename Emit, typename Nothing>
+__device__ __forceinline__ void plan_list(const KvAttentionPlan& plan, PlanMemory<kThreadCount>& memory, int cut0, int cut1, Emit emit, Nothing nothing) {
   const KvAttention& a = plan.a;
   const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
-  const int heads = a.shape.kv_heads, dim = a.shape.head_dim;
-  auto scan = [&](long long x) {               // inclusive, over the block
+  const int heads = a.shape.kv_heads;
+  auto scan = [&](long long x, long long* all) {         // inclusive, over the block
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const long long other = __shfl_up_sync(0xffffffffu, x, d);
       if (lane >= d) x += other;
     }
-    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();                                     // the scan before has been read
+    if (lane == 31) memory.warp_sum[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-      long long w = warp_sum[lane];
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffu, w, d);
-        if (lane >= d) w += other;
-      }
-      warp_sum[lane] = w;
+    *all = 0;
+    for (int w = 0; w < kThreadCount / 32; ++w) {
+      const long long s = memory.warp_sum[w];
+      if (w < warp) x += s;
+      *all += s;
     }
-    __syncthreads();
-    const long long before = warp > 0 ? warp_sum[warp - 1] : 0;
-    return before + x;
+    return x;
   };
-  int items_here = 0;
-  if (thread < a.batch.sequences) {
-    const KvSequence seq = kv_sequence(a.batch, a.shape, thread);
-    if (seq.bad) atomicOr(a.status, kKvBadBatch);
-    items_here = (seq.rows + plan.tile_tokens - 1) / plan.tile_tokens;
+  long long items_so_far = 0;
+  for (int s0 = 0; s0 < a.batch.sequences; s0 += kThreadCount) {
+    int mine = 0;
+    if (s0 + thread < a.batch.sequences) {
+      const KvSequence seq = kv_sequence(a.batch, a.shape, s0 + thread);
+      if (seq.bad) atomicOr(a.status, kKvBadBatch);
+      mine = (seq.rows + plan.tile_tokens - 1) / plan.tile_tokens;
+    }
+    long long all;
+    const long long upto = scan(mine, &all) + items_so_far;
+    if (s0 + thread < a.batch.sequences) memory.first_item[s0 + thread + 1] = static_cast<int>(upto);
+    items_so_far += all;
   }
-  const int upto = static_cast<int>(scan(items_here));
-  if (thread < a.batch.sequences) first_item[thread + 1] = upto;
-  if (thread == 0) first_item[0] = 0;
+  if (thread == 0) memory.first_item[0] = 0;
   __syncthreads();
-  const int items = first_item[a.batch.sequences];
-  // Up to kPlanThreads items need one scan; more are gone through twice, for the total and for the cuts.
-  for (int pass = items > kPlanThreads ? 0 : 1; pass < 2; ++pass) {
-    long long carry = 0;                       // the same in all threads
-    for (int item0 = 0; item0 < items || item0 == 0; item0 += kPlanThreads) {
+  const int items = static_cast<int>(items_so_far);
+  long long total = 0;
+  // Items for which the threads suffice need one scan; more are gone through twice, for the total and for the cuts.
+  for (int pass = items > kThreadCount ? 0 : 1; pass < 2; ++pass) {
+    long long before = 0;
+    for (int item0 = 0; item0 < items; item0 += kThreadCount) {
       const int item = item0 + thread;
       int s = 0, row_tile = 0;
       KvUnit unit{0, 0, 0};
@@ -184,48 +205,66 @@ kv_plan_kernel(const KvAttentionPlan plan) {
         int low = 0, high = a.batch.sequences;
         while (high - low > 1) {
           const int mid = (low + high) >> 1;
-          if (first_item[mid] <= item) low = mid; else high = mid;
+          if (memory.first_item[mid] <= item) low = mid; else high = mid;
         }
         s = low;
-        row_tile = item - first_item[s];
+        row_tile = item - memory.first_item[s];
         seq = kv_sequence(a.batch, a.shape, s);
         unit = kv_unit(seq, row_tile, plan.tile_tokens);
       }
-      const long long unit_cost = unit.tiles > 0 ? unit.tiles + kUnitCost : 0, cost = unit_cost * heads;
-      const long long end = scan(cost) + carry, begin = end - cost;
-      carry += warp_sum[kPlanThreads / 32 - 1];
-      if (items <= kPlanThreads) total = carry;
-      if (pass == 1 && unit.tiles > 0) {
-        // the cuts c with begin < total c / blocks <= end, and the list's own begin
-        for (long long c = begin == 0 ? 0 : begin * plan.blocks / total + 1; c <= plan.blocks; ++c) {
-          const long long cut = total * c / plan.blocks;
-          if (cut > end) break;
-          if (cut <= begin && begin != 0) continue;
+      const int unit_cost = unit.tiles > 0 ? unit.tiles + kUnitCost : 0;
+      long long all;
+      const long long end = scan(static_cast<long long>(unit_cost) * heads, &all) + before, begin = end - static_cast<long long>(unit_cost) * heads;
+      before += all;
+      if (items <= kThreadCount) total = before;
+      if (pass == 1) {
+        const int blocks = static_cast<int>(min(static_cast<long long>(plan.blocks), total));
+        for (int c = cut0; c <= cut1; ++c) {
+          const long long cut = total * min(c, blocks) / max(blocks, 1);
+          if (unit_cost == 0 || cut > end || (cut <= begin && (cut != 0 || begin != 0))) continue;
           const int head = static_cast<int>(min((cut - begin) / unit_cost, static_cast<long long>(heads - 1)));
-          const long long unit_begin = begin + head * unit_cost;
+          const long long unit_begin = begin + static_cast<long long>(head) * unit_cost;
           int tile = max(0, static_cast<int>(cut - unit_begin) - kUnitCost);
           if (tile <= kSnap && tile <= unit.tiles - tile) tile = 0;
           else if (unit.tiles - tile <= kSnap) tile = unit.tiles;
-          plan.work.starts[c] = KvStart{unit_begin + (tile > 0 ? kUnitCost + tile : 0), s, row_tile, head, tile, seq.row0, seq.rows, seq.length, 0};
+          emit(c, KvStart{unit_begin + (tile > 0 ? kUnitCost + tile : 0), total, s, row_tile, head, tile, seq.row0, seq.rows, seq.length, blocks});
         }
+        if (item < items && unit_cost == 0) nothing(item, seq.row0 + row_tile * plan.tile_tokens, unit.tokens);
       }
-      if (pass == 1 && item < items && unit.tiles == 0) {
-        // rows that see nothing
-        for (int i = 0; i < unit.tokens; ++i) {
-          uint4* out = reinterpret_cast<uint4*>(a.out + (seq.row0 + row_tile * plan.tile_tokens + i) * static_cast<long long>(a.shape.q_heads) * dim);
-          for (int j = 0; j < a.shape.q_heads * dim / 8; ++j) out[j] = make_uint4(0, 0, 0, 0);
-        }
-      }
-      __syncthreads();                         // warp_sum has been read
     }
-    total = carry;
+    total = before;
   }
   if (total == 0) {
-    for (int c = thread; c <= plan.blocks; c += kPlanThreads) plan.work.starts[c] = KvStart{0, 0, 0, 0, 0, 0, 0, 0, 0};
+    for (int c = cut0 + thread; c <= cut1; c += kThreadCount) emit(c, KvStart{0, 0, 0, 0, 0, 0, 0, 0, 0, 0});
   }
 }
 
-template <int kDim>
+// For lists of many row tiles: one block writes all cuts.
+constexpr int kPlanThreads = 1024;
+__global__ void __launch_bounds__(kPlanThreads)
+kv_plan_kernel(const KvAttentionPlan plan) {
+  __shared__ PlanMemory<kPlanThreads> memory;
+  pdl_enter();
+  plan_list<kPlanThreads>(
+      plan, memory, 0, plan.blocks, [&](int c, const KvStart& start) { plan.work.starts[c] = start; },
+      [&](int, int row0, int rows) {
+        uint4* out = reinterpret_cast<uint4*>(plan.a.out + static_cast<long long>(row0) * plan.a.shape.q_heads * plan.a.shape.head_dim);
+        for (int i = 0; i < rows * plan.a.shape.q_heads * plan.a.shape.head_dim / 8; ++i) out[i] = make_uint4(0, 0, 0, 0);
+      });
+}
+
+// The unit that cut `cut` divides: its blocks.  Cut c lies at total c / blocks, and divides a unit if it leaves more than kSnap
+// tiles of it on either side.
+__device__ __forceinline__ void divided_unit(const KvStart& cut, int tiles, int* first_block, int* parts) {
+  const long long unit_begin = cut.at - cut.tile - kUnitCost, low = unit_begin + kUnitCost + kSnap + 1, high = unit_begin + kUnitCost + tiles - kSnap;
+  const int first = static_cast<int>((low * cut.blocks + cut.total - 1) / cut.total);      // least c with total c / blocks >= low
+  const int last = static_cast<int>((high * cut.blocks + cut.total - 1) / cut.total) - 1;  // largest c with total c / blocks < high
+  *first_block = first - 1;
+  *parts = last - first + 2;
+}
+
+// kPlanned: kv_plan_kernel has left the cuts; else every block finds its own two.
+template <int kDim, bool kPlanned>
 __global__ void __launch_bounds__(kThreads, 1)
 kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ KvAttentionPlan plan) {
   using L = Prompt<kDim>;
@@ -256,6 +295,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
     mbar_init(smem_u32(&sm.q_full), 8);
     mbar_init(smem_u32(&sm.drain), 1);
     sm.abort_flag = 0;
+    sm.shared[0].parts = sm.shared[1].parts = 0;
     mbar_fence_init();
   }
   if (warp == 2) tmem_alloc(smem_u32(&sm.tmem), 512);
@@ -266,7 +306,30 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
   pdl_enter();
 
   Walk walk;
-  walk.begin(plan, plan.work.starts[blockIdx.x], plan.work.starts[blockIdx.x + 1]);
+  if (kPlanned) {
+    if (threadIdx.x < 2) sm.cut[threadIdx.x] = plan.work.starts[blockIdx.x + threadIdx.x];
+  } else {
+    // in the place of the first tiles
+    PlanMemory<kThreads>& memory = *reinterpret_cast<PlanMemory<kThreads>*>(generic);
+    int* empty = reinterpret_cast<int*>(generic + sizeof(PlanMemory<kThreads>));         // row, rows of items that see nothing
+    empty[2 * threadIdx.x + 1] = 0;
+    bool mine = false;
+    plan_list<kThreads>(plan, memory, blockIdx.x, blockIdx.x + 1, [&](int c, const KvStart& start) { sm.cut[c - blockIdx.x] = start; },
+                        [&](int item, int row0, int rows) {
+                          if (item % gridDim.x != blockIdx.x) return;
+                          empty[2 * threadIdx.x] = row0;
+                          empty[2 * threadIdx.x + 1] = rows;
+                          mine = true;
+                        });
+    if (__syncthreads_or(mine)) {
+      for (int i = 0; i < kThreads; ++i) {
+        if (empty[2 * i + 1] > 0) kv_zero_rows<kDim, kThreads>(a, empty[2 * i], empty[2 * i + 1]);
+      }
+    }
+    fence_async_proxy();                   // tiles will be written where the plan lay
+  }
+  __syncthreads();
+  walk.begin(plan, sm.cut[0], sm.cut[1]);
   auto wait = [&](unsigned long long* bar, uint32_t parity) {
     if (mbar_wait_bounded_warp(smem_u32(bar), parity, abort_flag, plan.wait_limit_ns)) return true;
     if (lane == 0) atomicOr(a.status, kKvTimeout);
@@ -632,11 +695,18 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
       wait(&sm.o_done[(tile - 1) & 1], ((tile - 1) >> 1) & 1);
       tc_fence_after();
       const float total = sm.sum[0][row] + sm.sum[1][row];
-      const bool whole = n == walk.unit.tiles;
-      const int part = 2 * blockIdx.x + (walk.tile0 == 0 ? 1 : 0);
-      if (!whole && group == 0) plan.work.weights[static_cast<size_t>(part) * plan.work.rows_per_part + row] = make_float2(top, total);
+      const bool whole = n == walk.unit.tiles, begins = walk.tile0 == 0;
+      const size_t part = kv_part_index(blockIdx.x, begins);
+      if (!whole) {
+        if (group == 0 && row < rows) *kv_part_weight(plan.work, part, row) = make_float2(top, total);
+        if (threadIdx.x == 128) {
+          KvShared shared{0, 0, 0, rows, token0, walk.head * shape.group};
+          divided_unit(sm.cut[begins ? 1 : 0], walk.unit.tiles, &shared.first_block, &shared.parts);
+          shared.mine = static_cast<int>(blockIdx.x) - shared.first_block;
+          sm.shared[begins ? 1 : 0] = shared;
+        }
+      }
       const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-      float* sums = plan.work.sums + static_cast<size_t>(part) * plan.work.rows_per_part * kDim;
       // The queries are no longer needed: their place takes the results, 16-byte pieces XORed with the row, so that they leave in
       // whole rows.  (Each thread storing its own row took 5 us per unit.)
       uint8_t* stage = generic + L::kQueryAt;
@@ -659,11 +729,9 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
             *reinterpret_cast<uint4*>(stage + row * 2 * kDim + (((column / 8 + k) ^ (row & 7)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
           }
         } else if (row < rows) {
-          // [head_dim / 4][rows][4]: a warp writes whole lines
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            *reinterpret_cast<uint4*>(sums + (static_cast<size_t>(column / 4 + k) * plan.work.rows_per_part + row) * 4) =
-                make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+            *reinterpret_cast<uint4*>(kv_part_sum<kDim>(plan.work, part, row, column + 4 * k)) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
         }
       }
       if (whole) {
@@ -696,90 +764,33 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
     __syncthreads();
   }
   if (warp == 2) tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i)
+      if (sm.shared[i].parts > 0) kv_arrive(plan.work, sm.shared[i]);
+  }
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    if (sm.shared[i].parts > 0) kv_join<kDim, kThreads>(a, plan.work, sm.shared[i], plan.wait_limit_ns, &sm.verdict);
+  }
 }
 
-// Joins the parts of the units that a cut divides.  Block (c, slice): the unit that cut c divides, if no earlier cut does;
-// eight rows of it.
-template <int kDim>
-__global__ void __launch_bounds__(256)
-kv_prompt_join_kernel(const KvAttentionPlan plan) {
-  __shared__ long long at_s[kKvMaxBlocks + 1];
-  __shared__ float2 part_weight[kKvMaxBlocks][8];
-  __shared__ float weight[kKvMaxBlocks][8];
-  __shared__ float total_s[8];
-  pdl_enter();
-  const KvAttention& a = plan.a;
-  const int cut = blockIdx.x + 1, row0 = blockIdx.y * 8;
-  const int thread = threadIdx.x;
-  for (int c = thread; c <= plan.blocks; c += 256) at_s[c] = plan.work.starts[c].at;
-  const KvStart start = plan.work.starts[cut];
-  const KvUnit unit = kv_unit(KvSequence{start.row0, start.rows, start.length, false}, start.row_tile, plan.tile_tokens);
-  const int rows = unit.tokens * a.shape.group;
-  if (start.tile == 0 || start.tile >= unit.tiles || row0 >= rows) return;     // the same in the whole block
-  const long long first = start.at - start.tile - kUnitCost, end = start.at - start.tile + unit.tiles;
-  __syncthreads();
-  if (at_s[cut - 1] > first) return;                           // an earlier cut's
-  // Parts: block cut - 1 begins the unit; then every block that begins inside it.  Empty shares left none.
-  int last = cut;
-  while (last < plan.blocks && at_s[last + 1] < end) ++last;
-  const int parts = last - cut + 2;
-  auto part_of = [&](int p) { return 2 * (cut - 1 + p) + (p == 0 ? 1 : 0); };
-  auto empty = [&](int p) { return p > 0 && at_s[cut - 1 + p] == at_s[cut + p]; };
-  for (int i = thread; i < 8 * parts; i += 256) {
-    const int p = i >> 3, r = i & 7;
-    // rows that the unit does not have were never written
-    part_weight[p][r] = empty(p) || row0 + r >= rows ? make_float2(-INFINITY, 0.0f)
-                                                     : plan.work.weights[static_cast<size_t>(part_of(p)) * plan.work.rows_per_part + row0 + r];
-  }
-  __syncthreads();
-  if (thread < 8) {
-    float top = -INFINITY, total = 0.0f;
-    for (int p = 0; p < parts; ++p) top = fmaxf(top, part_weight[p][thread].x);
-    for (int p = 0; p < parts; ++p) {
-      const float2 x = part_weight[p][thread];
-      // a part without a maximum has seen nothing, or nothing but NaN
-      const float w = exp2f(x.x - (top == -INFINITY ? 0.0f : top));
-      total += x.x == -INFINITY ? x.y : x.y * w;
-      weight[p][thread] = w;
-    }
-    total_s[thread] = total;
-  }
-  __syncthreads();
-  const int r = thread & 7, row = row0 + r;
-  if (row >= rows) return;
-  const float inverse = total_s[r] == 0.0f ? 0.0f : 1.0f / total_s[r];
-  const int token = row / a.shape.group, g = row - token * a.shape.group;
-  __nv_bfloat16* out = a.out + (static_cast<long long>(start.row0 + start.row_tile * plan.tile_tokens + token) * a.shape.q_heads +
-                                start.head * a.shape.group + g) * kDim;
-  for (int d = thread >> 3; d < kDim / 4; d += 32) {
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int p = 0; p < parts; ++p) {
-      if (empty(p)) continue;
-      const float4 x = *reinterpret_cast<const float4*>(plan.work.sums + static_cast<size_t>(part_of(p)) * plan.work.rows_per_part * kDim +
-                                                        (static_cast<size_t>(d) * plan.work.rows_per_part + row) * 4);
-      const float w = weight[p][r];
-      acc.x = fmaf(x.x, w, acc.x);
-      acc.y = fmaf(x.y, w, acc.y);
-      acc.z = fmaf(x.z, w, acc.z);
-      acc.w = fmaf(x.w, w, acc.w);
-    }
-    uint2 w;
-    w.x = static_cast<uint32_t>(float_to_bf16_bits(acc.x * inverse)) | (static_cast<uint32_t>(float_to_bf16_bits(acc.y * inverse)) << 16);
-    w.y = static_cast<uint32_t>(float_to_bf16_bits(acc.z * inverse)) | (static_cast<uint32_t>(float_to_bf16_bits(acc.w * inverse)) << 16);
-    *reinterpret_cast<uint2*>(out + 4 * d) = w;
-  }
+template <int kDim, bool kPlanned>
+cudaError_t launch_planned(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
+  constexpr int bytes = Prompt<kDim>::kSmallAt + static_cast<int>(sizeof(Small)) + 1024;
+  static_assert(bytes <= 227 * 1024, "more shared memory than a block can have");
+  static_assert(sizeof(PlanMemory<kThreads>) + 8 * kThreads <= Prompt<kDim>::kQueryAt, "the plan lies in the ring");
+  const cudaError_t error = opt_in_dynamic_smem<kv_prompt_kernel<kDim, kPlanned>>(bytes);
+  if (error != cudaSuccess) return error;
+  return launch_resident(kv_prompt_kernel<kDim, kPlanned>, dim3(plan.blocks), dim3(kThreads), bytes, stream, maps, plan);
 }
 
 template <int kDim>
 cudaError_t launch(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
-  constexpr int bytes = Prompt<kDim>::kSmallAt + static_cast<int>(sizeof(Small)) + 1024;
-  static_assert(bytes <= 227 * 1024, "more shared memory than a block can have");
-  cudaError_t error = opt_in_dynamic_smem<kv_prompt_kernel<kDim>>(bytes);
-  if (error == cudaSuccess) error = launch_pdl(kv_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, plan);
-  if (error == cudaSuccess) error = launch_pdl(kv_prompt_kernel<kDim>, dim3(plan.blocks), dim3(kThreads), bytes, stream, maps, plan);
-  if (error == cudaSuccess && plan.blocks > 1)
-    error = launch_pdl(kv_prompt_join_kernel<kDim>, dim3(plan.blocks - 1, kKvTile / 8), dim3(256), 0, stream, plan);
-  return error;
+  // row tiles at most; with one for each thread of a block every block can find its share by itself
+  const long long items = plan.a.batch.tokens / plan.tile_tokens + plan.a.batch.sequences;
+  if (items <= kThreads) return launch_planned<kDim, false>(plan, maps, stream);
+  const cudaError_t error = launch_pdl(kv_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, plan);
+  return error != cudaSuccess ? error : launch_planned<kDim, true>(plan, maps, stream);
 }
 
 }  // namespace
