@@ -10,6 +10,7 @@ namespace aima {
 constexpr int kKvTile = 128;            // positions of the cache per step
 constexpr int kKvMaxBlocks = 160;       // blocks of an attention kernel at most (one per SM)
 constexpr int kKvPartRows = 128;
+constexpr int kKvMaxList = 1 << 24;     // tiles (with the units' own cost) of a launch: shares are computed in 32 bits
 
 struct KvMaps {
   CUtensorMap keys, values;             // [pages * kv_heads * page_tokens, head_dim] bytes, boxes of one page x up to 128 bytes
@@ -17,10 +18,11 @@ struct KvMaps {
 
 // Where a block of the prompt kernel begins: the unit and the tile inside it, and the place in the list in units of its cost.
 struct alignas(16) KvStart {
-  long long at, total;
+  int at, total;
+  int blocks;                           // the shares of the list
   int sequence, row_tile, head, tile;
   int row0, rows, length;               // of the sequence
-  int blocks;                           // the shares of the list
+  int unused[2];
 };
 
 // A unit is the tiles of the cache that a row tile (up to 128 rows: query heads of one key/value head x new tokens) sees.
@@ -50,6 +52,12 @@ struct KvShared {
   int rows;
   int row0, head;               // of q: the unit's first row and query head
 };
+
+// floor(total c / blocks) and ceil(x blocks / total), x <= total <= kKvMaxList
+__device__ __forceinline__ int kv_cut(int total, int c, int blocks) { return static_cast<int>(static_cast<uint32_t>(total) * static_cast<uint32_t>(c) / static_cast<uint32_t>(blocks)); }
+__device__ __forceinline__ int kv_first_cut(int x, int total, int blocks) {
+  return static_cast<int>((static_cast<uint32_t>(x) * static_cast<uint32_t>(blocks) + static_cast<uint32_t>(total) - 1u) / static_cast<uint32_t>(total));
+}
 
 __device__ __forceinline__ size_t kv_part_index(int block, bool begins) { return 2 * block + (begins ? 1 : 0); }
 __device__ __forceinline__ float2* kv_part_weight(const KvWorkspace& work, size_t part, int row) { return work.weights + part * kKvPartRows + row; }
@@ -151,7 +159,7 @@ __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace&
 
 // Rows [row0, row0 + rows) of the output are zero: they see nothing.  Called by all threads of a block.
 template <int kDim, int kThreads>
-__device__ __forceinline__ void kv_zero_rows(const KvAttention& a, int row0, int rows) {
+__device__ __noinline__ void kv_zero_rows(const KvAttention& a, int row0, int rows) {
   uint4* out = reinterpret_cast<uint4*>(a.out + static_cast<long long>(row0) * a.shape.q_heads * kDim);
   const long long pieces = static_cast<long long>(rows) * a.shape.q_heads * (kDim / 8);
   for (long long i = threadIdx.x; i < pieces; i += kThreads) out[i] = make_uint4(0, 0, 0, 0);

@@ -27,7 +27,7 @@ constexpr int kThreads = 256;
 constexpr float kGrow = 0.75f;            // 2^8 * 2^0.75 = 430 <= 448
 constexpr float kWeightScale = 256.0f;
 constexpr float kLowScale = 2048.0f;      // a remainder is at most 16: 32768 <= 57344
-constexpr float kQueryLow = 16.0f;        // a remainder is at most 16: 256 <= 448
+constexpr float kQueryLow = 16.0f;        // a remainder is at most 16: 256 <= 448 (0x4c00 as f16)
 constexpr int kMaxPrefix = AIMA_MOE_KV_MAX_SEQUENCES + 1;
 
 template <int kDim, int kRows>
@@ -45,7 +45,7 @@ struct Decode {
   static constexpr int kQueryAt = kSlots * kSlotBytes;
   static constexpr int kWeightAt = kQueryAt + kQueryBytes;
   static constexpr int kPrefixAt = kWeightAt + 4 * kWeightBytes;
-  static constexpr int kSmallAt = kPrefixAt + kMaxPrefix * 8 + 8;
+  static constexpr int kSmallAt = (kPrefixAt + kMaxPrefix * 4 + 15) / 16 * 16;
 };
 
 struct SegmentInfo {
@@ -63,7 +63,7 @@ struct Small {              // shared memory that is not an operand
   int limit[2][kRows];      // last position a row sees; -1: none
   long long out_at[2][kRows];
   SegmentInfo info[2];
-  long long scan[kThreads / 32];
+  int scan[kThreads / 32];
   KvShared shared[2];       // the units divided at the share's begin and at its end
   int verdict;
   uint32_t tmem;
@@ -72,20 +72,20 @@ struct Small {              // shared memory that is not an operand
 
 // A block's share of the list, unit by unit.
 struct Walk {
-  const long long* prefix;
+  const int* prefix;
   int heads;
-  long long at, end;
+  int at, end;
   int sequence;
   // the current segment
   int head, tile0, tiles, unit_tiles;
   __device__ __forceinline__ bool next() {
     if (at >= end) return false;
     while (prefix[sequence + 1] <= at) ++sequence;
-    unit_tiles = static_cast<int>((prefix[sequence + 1] - prefix[sequence]) / heads);
-    const long long within = at - prefix[sequence];
-    head = static_cast<int>(within / unit_tiles);
-    tile0 = static_cast<int>(within - static_cast<long long>(head) * unit_tiles);
-    tiles = static_cast<int>(min(static_cast<long long>(unit_tiles - tile0), end - at));
+    unit_tiles = static_cast<int>(static_cast<uint32_t>(prefix[sequence + 1] - prefix[sequence]) / static_cast<uint32_t>(heads));
+    const int within = at - prefix[sequence];
+    head = static_cast<int>(static_cast<uint32_t>(within) / static_cast<uint32_t>(unit_tiles));
+    tile0 = within - head * unit_tiles;
+    tiles = min(unit_tiles - tile0, end - at);
     return true;
   }
   __device__ __forceinline__ void advance() { at += tiles; }
@@ -115,7 +115,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* generic = smem_raw + (base - smem_u32(smem_raw));
-  long long* prefix = reinterpret_cast<long long*>(generic + L::kPrefixAt);
+  int* prefix = reinterpret_cast<int*>(generic + L::kPrefixAt);
   Small<kRows>& sm = *reinterpret_cast<Small<kRows>*>(generic + L::kSmallAt);
   volatile int* abort_flag = &sm.abort_flag;
   const KvAttention& a = plan.a;
@@ -152,28 +152,26 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
 
   // tiles before each sequence; four sequences per thread
   {
-    long long mine[4], sum = 0;
+    int mine[4], sum = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int s = threadIdx.x * 4 + i;
-      long long tiles = 0;
+      mine[i] = sum;
       if (s < a.batch.sequences) {
         const KvSequence seq = kv_sequence(a.batch, shape, s);
         if (seq.bad && blockIdx.x == 0) atomicOr(a.status, kKvBadBatch);
-        if (seq.rows > 0) tiles = static_cast<long long>((seq.length + kKvTile - 1) / kKvTile) * shape.kv_heads;
+        if (seq.rows > 0) sum = min(kKvMaxList + 1, sum + (seq.length + kKvTile - 1) / kKvTile * shape.kv_heads);
       }
-      mine[i] = sum;
-      sum += tiles;
     }
-    long long run = sum;
+    int run = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const long long other = __shfl_up_sync(0xffffffffu, run, d);
-      if (lane >= d) run += other;
+      const int other = __shfl_up_sync(0xffffffffu, run, d);
+      if (lane >= d) run = min(kKvMaxList + 1, run + other);
     }
     if (lane == 31) sm.scan[warp] = run;
     __syncthreads();
-    long long before = run - sum;
+    int before = run - sum;
     for (int w = 0; w < warp; ++w) before += sm.scan[w];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -186,22 +184,22 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
-  const long long total = prefix[a.batch.sequences];
-  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), total));        // with a share; none is empty
+  int total = prefix[a.batch.sequences];
+  if (total > kKvMaxList) {
+    if (threadIdx.x == 0) atomicOr(a.status, kKvBadBatch);
+    total = 0;
+  }
+  const int blocks = min(static_cast<int>(gridDim.x), total);        // with a share; none is empty
   Walk walk;
   walk.prefix = prefix;
   walk.heads = shape.kv_heads;
   walk.at = walk.end = 0;
   if (static_cast<int>(blockIdx.x) < blocks) {
-    walk.at = total * blockIdx.x / blocks;
-    walk.end = total * (blockIdx.x + 1) / blocks;
+    walk.at = kv_cut(total, blockIdx.x, blocks);
+    walk.end = kv_cut(total, blockIdx.x + 1, blocks);
   }
   walk.sequence = 0;
-  auto wait = [&](unsigned long long* bar, uint32_t parity) {
-    if (mbar_wait_bounded_warp(smem_u32(bar), parity, abort_flag, plan.wait_limit_ns)) return true;
-    if (lane == 0) atomicOr(a.status, kKvTimeout);
-    return false;
-  };
+  auto wait = [&](unsigned long long* bar, uint32_t parity) { return mbar_wait_bounded_warp(smem_u32(bar), parity, abort_flag, plan.wait_limit_ns); };
   // Ring of K and V tiles, in the order in which the products take them: K0 K1 V0 K2 V1 .. V(n-2) V(n-1) of a segment.
   auto ring_k = [](int start, int j) { return start + (j == 0 ? 0 : 2 * j - 1); };
   auto ring_v = [](int start, int j, int n) { return start + (j + 1 < n ? 2 * j + 2 : 2 * n - 1); };
@@ -322,65 +320,61 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
       const int rows = seq.rows * shape.group, which = segment & 1;
       if (!wait(&sm.info_empty[which], ((segment >> 1) & 1) ^ 1) || !wait(&sm.q_empty, (segment & 1) ^ 1)) break;
       if (warp == 2 && lane == 0) sm.info[which] = SegmentInfo{seq.length, rows, seq.row0};
-#pragma unroll 4
-      for (int r = warp - 2; r < kRows; r += 2) {
-        const int i = r / shape.group, g = r - i * shape.group;
-        const int head = walk.head * shape.group + g;
-        float x[kPer];
+#pragma unroll 1
+      for (int r0 = 4 * (warp - 2); r0 < kRows; r0 += 8) {       // four rows side by side: one alone is a chain of 340 cycles
+        uint32_t raw[4][kPer / 2];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) x[e] = 0.0f;
-        if (r < rows) {
+        for (int b = 0; b < 4; ++b) {
+          const int r = r0 + b, i = r / shape.group, g = r - i * shape.group;
+          const int head = walk.head * shape.group + g;
           const __nv_bfloat16* at = a.q.data + (seq.row0 + i) * a.q.row_stride + head * a.q.head_stride + lane * kPer;
-          if constexpr (kPer == 8) {
-            unpack8(*reinterpret_cast<const uint4*>(at), x);
-          } else if constexpr (kPer == 4) {
-            const uint2 w = *reinterpret_cast<const uint2*>(at);
-            x[0] = bf16_lo(w.x); x[1] = bf16_hi(w.x); x[2] = bf16_lo(w.y); x[3] = bf16_hi(w.y);
-          } else {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(at);
-            x[0] = bf16_lo(w); x[1] = bf16_hi(w);
+#pragma unroll
+          for (int e = 0; e < kPer / 2; ++e) raw[b][e] = 0;
+          if (r < rows) {
+            if constexpr (kPer == 8) {
+              const uint4 v = *reinterpret_cast<const uint4*>(at);
+              raw[b][0] = v.x; raw[b][1] = v.y; raw[b][2] = v.z; raw[b][3] = v.w;
+            } else if constexpr (kPer == 4) {
+              const uint2 v = *reinterpret_cast<const uint2*>(at);
+              raw[b][0] = v.x; raw[b][1] = v.y;
+            } else {
+              raw[b][0] = *reinterpret_cast<const uint32_t*>(at);
+            }
           }
-        }
-        float top = 0.0f;
-        bool finite = true;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const float m = fabsf(x[e]);
-          finite = finite && m <= 3.402823466e38f;
-          top = fmaxf(top, m);
-        }
-#pragma unroll
-        for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        finite = __all_sync(0xffffffffu, finite);
-        const int exponent = kv_scale_exponent(top);
-        const float inverse = kv_exp2(-exponent);
-        uint32_t hi[kPer / 2], lo[kPer / 2];
-#pragma unroll
-        for (int e = 0; e < kPer / 2; ++e) {
-          const float u = x[2 * e] * inverse, v = x[2 * e + 1] * inverse;
-          hi[e] = cvt_e4m3x2(u, v);
-          const float2 back = e4m3x2_values(hi[e]);
-          lo[e] = cvt_e4m3x2((u - back.x) * kQueryLow, (v - back.y) * kQueryLow);
-          if (!finite) {
-            hi[e] = kKvNan * 0x0101u;
-            lo[e] = 0;
+          if (lane == 0) {
+            sm.limit[which][r] = r < rows ? seq.length - seq.rows + i : -1;
+            sm.out_at[which][r] = ((seq.row0 + i) * static_cast<long long>(shape.q_heads) + head) * kDim;
           }
         }
 #pragma unroll
-        for (int term = 0; term < 2; ++term) {
-          const uint32_t* c = term == 0 ? hi : lo;
-          const int row = r + term * kRows, byte = lane * kPer;
-          const int panel = byte / L::kRowBytes, inside = byte % L::kRowBytes;
-          const int piece = (inside >> 4) ^ (L::kRowBytes == 128 ? row & 7 : (row >> 1) & 3);
-          uint8_t* to = generic + L::kQueryAt + (panel * 2 * kRows + row) * L::kRowBytes + piece * 16 + (inside & 15);
-          if constexpr (kPer == 8) *reinterpret_cast<uint2*>(to) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
-          else if constexpr (kPer == 4) *reinterpret_cast<uint32_t*>(to) = c[0] | (c[1] << 16);
-          else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(c[0]);
-        }
-        if (lane == 0) {
-          sm.row_scale[which][r] = kv_exp2(exponent) * a.scale_log2;
-          sm.limit[which][r] = r < rows ? seq.length - seq.rows + i : -1;
-          sm.out_at[which][r] = ((seq.row0 + i) * static_cast<long long>(shape.q_heads) + head) * kDim;
+        for (int b = 0; b < 4; ++b) {
+          const int r = r0 + b;
+          uint32_t largest = 0;            // magnitudes as integers: infinities and NaN come last
+#pragma unroll
+          for (int e = 0; e < kPer / 2; ++e) largest = max(largest, max(raw[b][e] & 0x7fffu, (raw[b][e] >> 16) & 0x7fffu));
+          largest = __reduce_max_sync(0xffffffffu, largest);
+          const bool finite = largest < 0x7f80u;
+          const int exponent = kv_scale_exponent(__uint_as_float(largest << 16));
+          const float inverse = kv_exp2(-exponent);
+          uint32_t codes[2][kPer / 2];
+#pragma unroll
+          for (int e = 0; e < kPer / 2; ++e) {
+            const uint32_t h = cvt_f16x2(bf16_lo(raw[b][e]) * inverse, bf16_hi(raw[b][e]) * inverse);
+            codes[0][e] = finite ? cvt_e4m3x2_f16x2(h) : kKvNan * 0x0101u;
+            codes[1][e] = finite ? cvt_e4m3x2_f16x2(mul_f16x2(sub_f16x2(h, e4m3x2_f16x2(codes[0][e])), 0x4c004c00u)) : 0u;       // times 16
+          }
+#pragma unroll
+          for (int term = 0; term < 2; ++term) {
+            const uint32_t* c = codes[term];
+            const int row = r + term * kRows, byte = lane * kPer;
+            const int panel = byte / L::kRowBytes, inside = byte % L::kRowBytes;
+            const int piece = (inside >> 4) ^ (L::kRowBytes == 128 ? row & 7 : (row >> 1) & 3);
+            uint8_t* to = generic + L::kQueryAt + (panel * 2 * kRows + row) * L::kRowBytes + piece * 16 + (inside & 15);
+            if constexpr (kPer == 8) *reinterpret_cast<uint2*>(to) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+            else if constexpr (kPer == 4) *reinterpret_cast<uint32_t*>(to) = c[0] | (c[1] << 16);
+            else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(c[0]);
+          }
+          if (lane == 0) sm.row_scale[which][r] = kv_exp2(exponent) * a.scale_log2;
         }
       }
       fence_async_proxy();
@@ -477,7 +471,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
               top[r0 + i] = to;
             }
             if (j > 0) {
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < 2 * L::kOutPanels; ++c) {
                 const uint32_t at = tmem + lanes + L::kOutColumn + c * L::kWeightRows + r0;
                 uint32_t o[8];
@@ -551,14 +545,14 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
           const float4 s4 = *reinterpret_cast<const float4*>(sm.part[last ^ 1][r]);
           if (r < rows) *kv_part_weight(plan.work, part, r) = make_float2(top[r], (s4.x + s4.y) + (s4.z + s4.w));
         }
-        // the block of tile t is the last c with total c / blocks <= t
-        const long long first = walk.at - walk.tile0;
-        const int block0 = begins ? static_cast<int>(blockIdx.x) : static_cast<int>(((first + 1) * blocks - 1) / total);
-        const int block1 = static_cast<int>(((first + walk.unit_tiles) * blocks - 1) / total);
+        // the block of tile t is the last whose cut is not behind it: the one before the first cut at t + 1 or later
+        const int first = walk.at - walk.tile0;
+        const int block0 = begins ? static_cast<int>(blockIdx.x) : kv_first_cut(first + 1, total, blocks) - 1;
+        const int block1 = kv_first_cut(first + walk.unit_tiles, total, blocks) - 1;
         sm.shared[begins ? 1 : 0] = KvShared{block0, block1 - block0 + 1, static_cast<int>(blockIdx.x) - block0, rows, sm.info[which].row0,
                                              walk.head * shape.group};
       }
-#pragma unroll
+#pragma unroll 1
       for (int panel = 0; panel < L::kOutPanels; ++panel) {
         const int d = panel * 128 + token;
 #pragma unroll
@@ -596,6 +590,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
   if (*abort_flag != 0) {
     // a wait ran out: the copies have been waited for above, and so are the products under way, by a last commit
     volatile int ignore = 0;
+    if (threadIdx.x == 0) atomicOr(a.status, kKvTimeout);
     if (warp == 1 && elect_one()) umma_commit(smem_u32(&sm.drain));
     if (threadIdx.x == 0) mbar_wait_bounded(smem_u32(&sm.drain), 0, &ignore);
     __syncthreads();

@@ -152,31 +152,31 @@ constexpr int kSnap = 2;
 template <int kThreadCount>
 struct PlanMemory {
   int first_item[AIMA_MOE_KV_MAX_SEQUENCES + 1];
-  long long warp_sum[kThreadCount / 32];
+  int warp_sum[kThreadCount / 32];
 };
 template <int kThreadCount, typename Emit, typename Nothing>
 __device__ __forceinline__ void plan_list(const KvAttentionPlan& plan, PlanMemory<kThreadCount>& memory, int cut0, int cut1, Emit emit, Nothing nothing) {
   const KvAttention& a = plan.a;
   const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
   const int heads = a.shape.kv_heads;
-  auto scan = [&](long long x, long long* all) {         // inclusive, over the block
+  auto scan = [&](int x, int* all) {                     // inclusive, over the block
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const long long other = __shfl_up_sync(0xffffffffu, x, d);
-      if (lane >= d) x += other;
+      const int other = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x = min(kKvMaxList + 1, x + other);
     }
     __syncthreads();                                     // the scan before has been read
     if (lane == 31) memory.warp_sum[warp] = x;
     __syncthreads();
     *all = 0;
     for (int w = 0; w < kThreadCount / 32; ++w) {
-      const long long s = memory.warp_sum[w];
-      if (w < warp) x += s;
-      *all += s;
+      const int s = memory.warp_sum[w];
+      if (w < warp) x = min(kKvMaxList + 1, x + s);
+      *all = min(kKvMaxList + 1, *all + s);
     }
     return x;
   };
-  long long items_so_far = 0;
+  int items_so_far = 0;
   for (int s0 = 0; s0 < a.batch.sequences; s0 += kThreadCount) {
     int mine = 0;
     if (s0 + thread < a.batch.sequences) {
@@ -184,18 +184,18 @@ __device__ __forceinline__ void plan_list(const KvAttentionPlan& plan, PlanMemor
       if (seq.bad) atomicOr(a.status, kKvBadBatch);
       mine = (seq.rows + plan.tile_tokens - 1) / plan.tile_tokens;
     }
-    long long all;
-    const long long upto = scan(mine, &all) + items_so_far;
-    if (s0 + thread < a.batch.sequences) memory.first_item[s0 + thread + 1] = static_cast<int>(upto);
+    int all;
+    const int upto = scan(mine, &all) + items_so_far;
+    if (s0 + thread < a.batch.sequences) memory.first_item[s0 + thread + 1] = upto;
     items_so_far += all;
   }
   if (thread == 0) memory.first_item[0] = 0;
   __syncthreads();
-  const int items = static_cast<int>(items_so_far);
-  long long total = 0;
+  const int items = items_so_far;
+  int total = 0;
   // Items for which the threads suffice need one scan; more are gone through twice, for the total and for the cuts.
   for (int pass = items > kThreadCount ? 0 : 1; pass < 2; ++pass) {
-    long long before = 0;
+    int before = 0;
     for (int item0 = 0; item0 < items; item0 += kThreadCount) {
       const int item = item0 + thread;
       int s = 0, row_tile = 0;
@@ -213,29 +213,34 @@ __device__ __forceinline__ void plan_list(const KvAttentionPlan& plan, PlanMemor
         unit = kv_unit(seq, row_tile, plan.tile_tokens);
       }
       const int unit_cost = unit.tiles > 0 ? unit.tiles + kUnitCost : 0;
-      long long all;
-      const long long end = scan(static_cast<long long>(unit_cost) * heads, &all) + before, begin = end - static_cast<long long>(unit_cost) * heads;
-      before += all;
+      const int cost = min(kKvMaxList + 1, unit_cost * heads);
+      int all;
+      const int end = min(kKvMaxList + 1, scan(cost, &all) + before), begin = end - cost;
+      before = min(kKvMaxList + 1, before + all);
       if (items <= kThreadCount) total = before;
       if (pass == 1) {
-        const int blocks = static_cast<int>(min(static_cast<long long>(plan.blocks), total));
-        for (int c = cut0; c <= cut1; ++c) {
-          const long long cut = total * min(c, blocks) / max(blocks, 1);
-          if (unit_cost == 0 || cut > end || (cut <= begin && (cut != 0 || begin != 0))) continue;
-          const int head = static_cast<int>(min((cut - begin) / unit_cost, static_cast<long long>(heads - 1)));
-          const long long unit_begin = begin + static_cast<long long>(head) * unit_cost;
-          int tile = max(0, static_cast<int>(cut - unit_begin) - kUnitCost);
+        if (total > kKvMaxList) {
+          atomicOr(a.status, kKvBadBatch);
+          continue;
+        }
+        const int blocks = min(plan.blocks, total);
+        for (int c = cut0; c <= cut1 && unit_cost > 0; ++c) {
+          const int cut = kv_cut(total, min(c, blocks), blocks);
+          if (cut > end || (cut <= begin && (cut != 0 || begin != 0))) continue;
+          const int head = min(static_cast<int>(static_cast<uint32_t>(cut - begin) / static_cast<uint32_t>(unit_cost)), heads - 1);
+          const int unit_begin = begin + head * unit_cost;
+          int tile = max(0, cut - unit_begin - kUnitCost);
           if (tile <= kSnap && tile <= unit.tiles - tile) tile = 0;
           else if (unit.tiles - tile <= kSnap) tile = unit.tiles;
-          emit(c, KvStart{unit_begin + (tile > 0 ? kUnitCost + tile : 0), total, s, row_tile, head, tile, seq.row0, seq.rows, seq.length, blocks});
+          emit(c, KvStart{unit_begin + (tile > 0 ? kUnitCost + tile : 0), total, blocks, s, row_tile, head, tile, seq.row0, seq.rows, seq.length, {0, 0}});
         }
         if (item < items && unit_cost == 0) nothing(item, seq.row0 + row_tile * plan.tile_tokens, unit.tokens);
       }
     }
     total = before;
   }
-  if (total == 0) {
-    for (int c = cut0 + thread; c <= cut1; c += kThreadCount) emit(c, KvStart{0, 0, 0, 0, 0, 0, 0, 0, 0, 0});
+  if (total == 0 || total > kKvMaxList) {
+    for (int c = cut0 + thread; c <= cut1; c += kThreadCount) emit(c, KvStart{});
   }
 }
 
@@ -256,9 +261,8 @@ kv_plan_kernel(const KvAttentionPlan plan) {
 // The unit that cut `cut` divides: its blocks.  Cut c lies at total c / blocks, and divides a unit if it leaves more than kSnap
 // tiles of it on either side.
 __device__ __forceinline__ void divided_unit(const KvStart& cut, int tiles, int* first_block, int* parts) {
-  const long long unit_begin = cut.at - cut.tile - kUnitCost, low = unit_begin + kUnitCost + kSnap + 1, high = unit_begin + kUnitCost + tiles - kSnap;
-  const int first = static_cast<int>((low * cut.blocks + cut.total - 1) / cut.total);      // least c with total c / blocks >= low
-  const int last = static_cast<int>((high * cut.blocks + cut.total - 1) / cut.total) - 1;  // largest c with total c / blocks < high
+  const int tiles_begin = cut.at - cut.tile;
+  const int first = kv_first_cut(tiles_begin + kSnap + 1, cut.total, cut.blocks), last = kv_first_cut(tiles_begin + tiles - kSnap, cut.total, cut.blocks) - 1;
   *first_block = first - 1;
   *parts = last - first + 2;
 }
@@ -330,11 +334,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
   }
   __syncthreads();
   walk.begin(plan, sm.cut[0], sm.cut[1]);
-  auto wait = [&](unsigned long long* bar, uint32_t parity) {
-    if (mbar_wait_bounded_warp(smem_u32(bar), parity, abort_flag, plan.wait_limit_ns)) return true;
-    if (lane == 0) atomicOr(a.status, kKvTimeout);
-    return false;
-  };
+  auto wait = [&](unsigned long long* bar, uint32_t parity) { return mbar_wait_bounded_warp(smem_u32(bar), parity, abort_flag, plan.wait_limit_ns); };
   // Ring of K and V tiles, in the order in which the products take them: K0 K1 V0 K2 V1 .. V(n-2) V(n-1) of a segment.
   auto ring_k = [](int first, int j) { return first + (j == 0 ? 0 : 2 * j - 1); };
   auto ring_v = [](int first, int j, int n) { return first + (j + 1 < n ? 2 * j + 2 : 2 * n - 1); };
@@ -759,6 +759,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
   if (*abort_flag != 0) {
     // a wait ran out: the copies have been waited for above, and so are the products under way, by a last commit
     volatile int ignore = 0;
+    if (threadIdx.x == 0) atomicOr(a.status, kKvTimeout);
     if (warp == 1 && elect_one()) umma_commit(smem_u32(&sm.drain));
     if (threadIdx.x == 0) mbar_wait_bounded(smem_u32(&sm.drain), 0, &ignore);
     __syncthreads();
