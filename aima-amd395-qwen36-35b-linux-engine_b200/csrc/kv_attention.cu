@@ -52,6 +52,19 @@ bool kv_make_maps(const KvShape& shape, const KvLayer& layer, KvMaps* maps) {
   return true;
 }
 
+bool kv_make_query_map(const KvAttention& a, int tile_tokens, CUtensorMap* map) {
+  const PFN_cuTensorMapEncodeTiled_v12000 encode = encode_fn();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.shape.head_dim), static_cast<cuuint64_t>(a.shape.q_heads), static_cast<cuuint64_t>(a.batch.tokens)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.q.head_stride) * 2, static_cast<cuuint64_t>(a.q.row_stride) * 2};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(a.shape.head_dim >= 128 ? 64 : 32), static_cast<cuuint32_t>(a.shape.group),
+                             static_cast<cuuint32_t>(tile_tokens)};
+  const cuuint32_t step[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16*>(a.q.data), dims, strides, box, step,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 cudaError_t kv_attention(const KvAttention& a, const KvMaps& maps, void* workspace, int sm_count, cudaStream_t stream) {
   KvAttentionPlan plan{};
   plan.a = a;

@@ -183,6 +183,8 @@ inline cudaError_t launch_resident(void (*kernel)(KernelArgs...), dim3 grid, dim
   return cudaLaunchKernelEx(&config, kernel, static_cast<KernelArgs>(args)...);
 }
 
+// Map of a call's queries: boxes of kRowBytes x the heads of a key/value head x tile_tokens.
+bool kv_make_query_map(const KvAttention& a, int tile_tokens, CUtensorMap* map);
 cudaError_t kv_decode(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream);
 cudaError_t kv_prompt(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream);
 

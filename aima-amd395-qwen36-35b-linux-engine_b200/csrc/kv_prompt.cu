@@ -33,6 +33,7 @@ constexpr float kFall = 16.0f;
 constexpr float kDepth = 30.0f;
 constexpr float kWeightExponent = 9.0f;
 constexpr int kScaleSlots = 4;
+constexpr int kStageBytes = 32 * 64;      // of a warp: 32 rows x 32 results
 
 template <int kDim>
 struct Prompt {
@@ -42,7 +43,8 @@ struct Prompt {
   static constexpr int kSlotBytes = kKvTile * kDim;
   static constexpr int kSlots = kDim == 256 ? 4 : 8;
   static constexpr int kQueryAt = kSlots * kSlotBytes;                  // hi, then lo
-  static constexpr int kSmallAt = kQueryAt + 2 * kSlotBytes;
+  static constexpr int kStageAt = kQueryAt + 2 * kSlotBytes;
+  static constexpr int kSmallAt = kStageAt + 8 * kStageBytes;
   static constexpr int kScoreColumn = 256;                              // tensor memory: O | S0 | S1
 };
 
@@ -50,10 +52,10 @@ struct Small {
   float4 scales[kScaleSlots][8];           // per 16 positions: key scale x softmax scale, log2 and inverse of the value scale, 0: no page
   int holes[kScaleSlots];                  // whether a page of the tile is missing
   unsigned long long full[8], empty[8], scales_full[kScaleSlots], scales_empty[kScaleSlots];
-  unsigned long long s_full[2], p_full[2], o_done[2], q_full, drain;
+  unsigned long long s_full[2], p_full[2], o_done[2], q_raw, q_full, q_empty, drain;
   float row_scale[128];
   float half_top[2][2][128];               // per tile parity, half and row
-  float sum[2][128];
+  float sum[2][2][128];                    // per parity of the unit, half and row
   KvStart cut[2];
   KvShared shared[2];                      // the units divided at the share's begin and at its end
   int verdict;
@@ -123,11 +125,16 @@ struct Walk {
   __device__ __forceinline__ void advance() { tile0 += tiles; }
 };
 
-// 16 bytes to shared memory, or zeros
-__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool exists) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(exists ? 16 : 0) : "memory");
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 // row / group for rows below 128, with inverse = ceil(2^16 / group)
 __device__ __forceinline__ int row_token(int row, int inverse) { return (row * inverse) >> 16; }
 __device__ __forceinline__ void group_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -270,7 +277,7 @@ __device__ __forceinline__ void divided_unit(const KvStart& cut, int tiles, int*
 // kPlanned: kv_plan_kernel has left the cuts; else every block finds its own two.
 template <int kDim, bool kPlanned>
 __global__ void __launch_bounds__(kThreads, 1)
-kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ KvAttentionPlan plan) {
+kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CUtensorMap queries, const __grid_constant__ KvAttentionPlan plan) {
   using L = Prompt<kDim>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -296,7 +303,9 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
       mbar_init(smem_u32(&sm.p_full[i]), 8);
       mbar_init(smem_u32(&sm.o_done[i]), 1);
     }
+    mbar_init(smem_u32(&sm.q_raw), 1);
     mbar_init(smem_u32(&sm.q_full), 8);
+    mbar_init(smem_u32(&sm.q_empty), 1);
     mbar_init(smem_u32(&sm.drain), 1);
     sm.abort_flag = 0;
     sm.shared[0].parts = sm.shared[1].parts = 0;
@@ -417,6 +426,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
             }
             umma_commit(smem_u32(&sm.empty[slot]));
             umma_commit(smem_u32(&sm.s_full[buffer]));
+            if (j + 1 == n) umma_commit(smem_u32(&sm.q_empty));
           }
           __syncwarp();
           return true;
@@ -445,6 +455,26 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
         tile += n;
         ++segment;
         walk.advance();
+      }
+    } else if (warp == 2) {
+      // ------------------------------ queries, as they are ------------------------------
+      // A BF16 row of a head is as long as its two terms together and goes where they will lie, kRowBytes at a time, so that it
+      // can be converted in place.  Rows behind the unit's last are another unit's or zeros; their results go nowhere.
+      int segment = 0;
+      for (; walk.next(); ++segment, walk.advance()) {
+        if (!wait(&sm.q_empty, (segment & 1) ^ 1)) break;
+        if (elect_one()) {
+          constexpr int kBoxes = 2 * kDim / L::kRowBytes;
+          mbar_arrive_expect_tx(smem_u32(&sm.q_raw), kBoxes * plan.tile_tokens * shape.group * L::kRowBytes);
+          for (int i = 0; i < kBoxes; ++i)
+            tma_load_3d(base + L::kQueryAt + (i / L::kPanels) * L::kSlotBytes + (i % L::kPanels) * L::kPanelBytes, &queries, i * L::kRowBytes / 2,
+                        walk.head * shape.group, walk.seq.row0 + walk.row_tile * plan.tile_tokens, smem_u32(&sm.q_raw));
+        }
+        __syncwarp();
+      }
+      if (*abort_flag != 0 && segment > 0) {
+        volatile int ignore = 0;
+        mbar_wait_bounded(smem_u32(&sm.q_raw), (segment - 1) & 1, &ignore);
       }
     } else if (warp == 3) {
       // ------------------------------ scales ------------------------------
@@ -492,35 +522,25 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
       const int n = walk.tiles;
       const int rows = walk.unit.tokens * shape.group;
       const int token0 = walk.seq.row0 + walk.row_tile * plan.tile_tokens;
-      // Queries: a warp takes every eighth row.  The raw BF16 row goes where its two terms will lie, all rows at once, and is
-      // converted in place: with the loads in registers either the loop is unrolled, and its code does not stay in the instruction
-      // cache between units, or every pass waits for its loads (8000 cycles either way).  BF16 numbers are f16 numbers
-      // down to 2^-14 of the row's scale.
+      // Queries: a warp takes every eighth row, four side by side (one alone is a chain of 340 cycles).  BF16 numbers are f16 numbers
+      // down to 2^-14 of the row's scale; a row that is not finite becomes NaN.
+      wait(&sm.q_raw, segment & 1);
       {
-        constexpr int kPer = kDim / 32, kPieces = kDim / 8, kAtOnce = 32 / kPieces;
+        constexpr int kPer = kDim / 32;
         const int w8 = warp - 4;
-        auto at_byte = [&](int r, int byte) {            // of a row of 2 kDim bytes: the first term's kDim, then the second's
-          const int term = byte / kDim, inside = byte % kDim;
-          return generic + L::kQueryAt + term * L::kSlotBytes + (inside / L::kRowBytes) * L::kPanelBytes + r * L::kRowBytes + inside % L::kRowBytes;
-        };
-#pragma unroll 4
-        for (int i = 0; i < 16; i += kAtOnce) {
-          const int r = 8 * (i + lane / kPieces) + w8;
-          const int token = row_token(r, group_inverse), g = r - token * shape.group;
-          const bool exists = r < rows;
-          cp_async_16_or_zero(smem_u32(at_byte(r, 16 * (lane % kPieces))),
-                              a.q.data + (exists ? static_cast<long long>(token0 + token) * a.q.row_stride + (walk.head * shape.group + g) * a.q.head_stride + 8 * (lane % kPieces) : 0),
-                              exists);
-        }
-        cp_async_wait_all();
-        __syncwarp();
+        uint8_t* queries_at = generic + L::kQueryAt;
+        const int raw_byte = 2 * kPer * lane, byte = kPer * lane;
+        const int raw_at = (raw_byte / kDim) * L::kSlotBytes + (raw_byte % kDim / L::kRowBytes) * L::kPanelBytes + raw_byte % L::kRowBytes + w8 * L::kRowBytes;
+        // the swizzle takes the row modulo 8, which is the warp
+        const int piece = (byte % L::kRowBytes >> 4) ^ (L::kRowBytes == 128 ? w8 : w8 >> 1);
+        const int code_at = (byte / L::kRowBytes) * L::kPanelBytes + piece * 16 + (byte & 15) + w8 * L::kRowBytes;
 #pragma unroll 1
-        for (int i = 0; i < 16; i += 4) {                  // four rows side by side: one alone is a chain of 340 cycles
+        for (int i = 0; i < 16 && 8 * i < rows; i += 4) {
           uint32_t raw[4][kPer / 2], codes[4][2][kPer / 2];
           int exponent[4];
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            const uint8_t* from = at_byte(8 * (i + b) + w8, 2 * kPer * lane);
+            const uint8_t* from = queries_at + raw_at + 8 * (i + b) * L::kRowBytes;
             if constexpr (kPer == 8) {
               const uint4 v = *reinterpret_cast<const uint4*>(from);
               raw[b][0] = v.x; raw[b][1] = v.y; raw[b][2] = v.z; raw[b][3] = v.w;
@@ -535,32 +555,35 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
           for (int b = 0; b < 4; ++b) {
             uint32_t largest = 0;          // magnitudes as integers: infinities and NaN come last
 #pragma unroll
-            for (int e = 0; e < kPer / 2; ++e) largest = max(largest, max(raw[b][e] & 0x7fffu, (raw[b][e] >> 16) & 0x7fffu));
-            largest = __reduce_max_sync(0xffffffffu, largest);           // all lanes have read the row
-            const bool finite = largest < 0x7f80u;
+            for (int e = 0; e < kPer / 2; ++e) largest = __vmaxu2(largest, raw[b][e] & 0x7fff7fffu);
+            largest = __reduce_max_sync(0xffffffffu, max(largest & 0xffffu, largest >> 16));           // all lanes have read the row
             exponent[b] = kv_scale_exponent(__uint_as_float(largest << 16));
-            const float inverse = kv_exp2(-exponent[b]);
+            const uint32_t inverse = largest < 0x7f80u ? static_cast<uint32_t>(127 - exponent[b]) * 0x00800080u : 0x7fff7fffu;      // two BF16 numbers
+            uint32_t h[kPer / 2];
 #pragma unroll
             for (int e = 0; e < kPer / 2; ++e) {
-              const uint32_t h = cvt_f16x2(bf16_lo(raw[b][e]) * inverse, bf16_hi(raw[b][e]) * inverse);
-              codes[b][0][e] = finite ? cvt_e4m3x2_f16x2(h) : kKvNan * 0x0101u;
-              codes[b][1][e] = finite ? cvt_e5m2x2_f16x2(sub_f16x2(h, e4m3x2_f16x2(codes[b][0][e]))) : 0u;
+              const uint32_t scaled = mul_bf16x2(raw[b][e], inverse);
+              h[e] = cvt_f16x2(bf16_lo(scaled), bf16_hi(scaled));
+              codes[b][0][e] = cvt_e4m3x2_f16x2(h[e]);
+              h[e] = sub_f16x2(h[e], e4m3x2_f16x2(codes[b][0][e])) + 0x00800080u;           // rounded to e5m2, its upper byte
+            }
+#pragma unroll
+            for (int e = 0; e < kPer / 2; e += 2) {
+              codes[b][0][e / 2] = __byte_perm(codes[b][0][e], kPer > 2 ? codes[b][0][e + 1 < kPer / 2 ? e + 1 : e] : 0u, 0x5410);
+              codes[b][1][e / 2] = __byte_perm(h[e], h[e + 1 < kPer / 2 ? e + 1 : e], 0x7531);
             }
           }
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            const int r = 8 * (i + b) + w8;
 #pragma unroll
             for (int term = 0; term < 2; ++term) {
               const uint32_t* c = codes[b][term];
-              const int byte = lane * kPer, panel = byte / L::kRowBytes, inside = byte % L::kRowBytes;
-              const int piece = (inside >> 4) ^ (L::kRowBytes == 128 ? r & 7 : (r >> 1) & 3);
-              uint8_t* to = generic + L::kQueryAt + term * L::kSlotBytes + panel * L::kPanelBytes + r * L::kRowBytes + piece * 16 + (inside & 15);
-              if constexpr (kPer == 8) *reinterpret_cast<uint2*>(to) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
-              else if constexpr (kPer == 4) *reinterpret_cast<uint32_t*>(to) = c[0] | (c[1] << 16);
+              uint8_t* to = queries_at + term * L::kSlotBytes + code_at + 8 * (i + b) * L::kRowBytes;
+              if constexpr (kPer == 8) *reinterpret_cast<uint2*>(to) = make_uint2(c[0], c[1]);
+              else if constexpr (kPer == 4) *reinterpret_cast<uint32_t*>(to) = c[0];
               else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(c[0]);
             }
-            if (lane == 0) sm.row_scale[r] = kv_exp2(exponent[b]);
+            if (lane == 0) sm.row_scale[8 * (i + b) + w8] = kv_exp2(exponent[b]);
           }
         }
         fence_async_proxy();
@@ -568,7 +591,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
         if (lane == 0) mbar_arrive(smem_u32(&sm.q_full));
         group_barrier();                   // row_scale
       }
-      const float row_scale = sm.row_scale[row];
+      const float row_scale = row < rows ? sm.row_scale[row] : 0.0f;
       const int limit = row < rows ? walk.unit.first + row_token(row, group_inverse) : -1;     // last position the row sees
       float top = -INFINITY, peak = -INFINITY, sum = 0.0f;       // reference and maximum so far; this half's sum of weights
       for (int j = 0; j < n; ++j, ++tile) {
@@ -690,11 +713,11 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
         if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[buffer]));
       }
       // the unit's sums, or this block's part of them; each group has half of the columns
-      sm.sum[group][row] = sum;
-      group_barrier();
+      sm.sum[segment & 1][group][row] = sum;
+      asm volatile("bar.sync %0, 64;" :: "r"(2 + quarter) : "memory");
+      const float total = sm.sum[segment & 1][0][row] + sm.sum[segment & 1][1][row];
       wait(&sm.o_done[(tile - 1) & 1], ((tile - 1) >> 1) & 1);
       tc_fence_after();
-      const float total = sm.sum[0][row] + sm.sum[1][row];
       const bool whole = n == walk.unit.tiles, begins = walk.tile0 == 0;
       const size_t part = kv_part_index(blockIdx.x, begins);
       if (!whole) {
@@ -707,9 +730,9 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
         }
       }
       const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-      // The queries are no longer needed: their place takes the results, 16-byte pieces XORed with the row, so that they leave in
-      // whole rows.  (Each thread storing its own row took 5 us per unit.)
-      uint8_t* stage = generic + L::kQueryAt;
+      // 32 columns at a time through shared memory, 16-byte pieces XORed with the row, so that every store writes 64 bytes of
+      // eight rows.  (Each thread storing its own row took 5 us per unit.)
+      uint8_t* stage = generic + L::kStageAt + (warp - 4) * kStageBytes;
       const uint32_t from = tmem + lanes + group * (kDim / 2);
 #pragma unroll 1
       for (int c = 0; c < kDim / 64; ++c) {
@@ -726,29 +749,27 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
               const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(x[8 * k + 2 * i]) * inverse, __uint_as_float(x[8 * k + 2 * i + 1]) * inverse);
               packed[i] = *reinterpret_cast<const uint32_t*>(&two);
             }
-            *reinterpret_cast<uint4*>(stage + row * 2 * kDim + (((column / 8 + k) ^ (row & 7)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
           }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = 8 * i + (lane >> 2), r = quarter * 32 + at;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + at * 64 + (((lane & 3) ^ ((at >> 1) & 3)) << 4));
+            if (r < rows) {
+              const int token = row_token(r, group_inverse), g = r - token * shape.group;
+              *reinterpret_cast<uint4*>(a.out + (static_cast<long long>(token0 + token) * shape.q_heads + walk.head * shape.group + g) * kDim +
+                                        column + 8 * (lane & 3)) = v;
+            }
+          }
+          __syncwarp();
         } else if (row < rows) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
             *reinterpret_cast<uint4*>(kv_part_sum<kDim>(plan.work, part, row, column + 4 * k)) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
         }
       }
-      if (whole) {
-        constexpr int kPieces = kDim / 8, kRowsAtOnce = 32 / kPieces;
-        group_barrier();
-#pragma unroll 2
-        for (int r0 = (warp - 4) * kRowsAtOnce; r0 < rows; r0 += 8 * kRowsAtOnce) {
-          const int r = r0 + lane / kPieces, piece = lane % kPieces;
-          if (r < rows) {
-            const int token = row_token(r, group_inverse), g = r - token * shape.group;
-            *reinterpret_cast<uint4*>(a.out + (static_cast<long long>(token0 + token) * shape.q_heads + walk.head * shape.group + g) * kDim + 8 * piece) =
-                *reinterpret_cast<const uint4*>(stage + r * 2 * kDim + ((piece ^ (r & 7)) << 4));
-          }
-        }
-      }
       tc_fence_before();
-      group_barrier();                     // what the groups share of this segment has been read
       ring += 2 * n;
       ++segment;
       walk.advance();
@@ -776,22 +797,24 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ Kv
 }
 
 template <int kDim, bool kPlanned>
-cudaError_t launch_planned(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
+cudaError_t launch_planned(const KvAttentionPlan& plan, const KvMaps& maps, const CUtensorMap& queries, cudaStream_t stream) {
   constexpr int bytes = Prompt<kDim>::kSmallAt + static_cast<int>(sizeof(Small)) + 1024;
   static_assert(bytes <= 227 * 1024, "more shared memory than a block can have");
   static_assert(sizeof(PlanMemory<kThreads>) + 8 * kThreads <= Prompt<kDim>::kQueryAt, "the plan lies in the ring");
   const cudaError_t error = opt_in_dynamic_smem<kv_prompt_kernel<kDim, kPlanned>>(bytes);
   if (error != cudaSuccess) return error;
-  return launch_resident(kv_prompt_kernel<kDim, kPlanned>, dim3(plan.blocks), dim3(kThreads), bytes, stream, maps, plan);
+  return launch_resident(kv_prompt_kernel<kDim, kPlanned>, dim3(plan.blocks), dim3(kThreads), bytes, stream, maps, queries, plan);
 }
 
 template <int kDim>
 cudaError_t launch(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
   // row tiles at most; with one for each thread of a block every block can find its share by itself
   const long long items = plan.a.batch.tokens / plan.tile_tokens + plan.a.batch.sequences;
-  if (items <= kThreads) return launch_planned<kDim, false>(plan, maps, stream);
+  CUtensorMap queries;
+  if (!kv_make_query_map(plan.a, plan.tile_tokens, &queries)) return cudaErrorInvalidValue;
+  if (items <= kThreads) return launch_planned<kDim, false>(plan, maps, queries, stream);
   const cudaError_t error = launch_pdl(kv_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, plan);
-  return error != cudaSuccess ? error : launch_planned<kDim, true>(plan, maps, stream);
+  return error != cudaSuccess ? error : launch_planned<kDim, true>(plan, maps, queries, stream);
 }
 
 }  // namespace
