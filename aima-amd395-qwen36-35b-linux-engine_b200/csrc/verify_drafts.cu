@@ -10,7 +10,8 @@
 namespace aima {
 namespace {
 
-constexpr int kVerifyThreads = 1024;
+constexpr int kVerifyThreads = 512;
+constexpr int kAhead = 4;                      // steps whose loads are under way together
 constexpr uint32_t kSplitVocabulary = 16384;   // more than four steps per warp of one block: a cluster of eight
 
 // floor(2^40 w) of w clamped to [0, 1]; NaN counts as 0
@@ -49,6 +50,23 @@ struct Weights {
     out[1] = of(x.y, y.y, t + 1);
     out[2] = of(x.z, y.z, t + 2);
     out[3] = of(x.w, y.w, t + 3);
+  }
+  // the sum over tokens t .. t + 3 of kAhead steps, all loads first
+  __device__ __forceinline__ unsigned long long ahead(int t) const {
+    float4 x[kAhead], y[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) x[i] = __ldcs(reinterpret_cast<const float4*>(p + t + 128 * i));
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) y[i] = q != nullptr ? __ldcs(reinterpret_cast<const float4*>(q + t + 128 * i)) : make_float4(0, 0, 0, 0);
+    unsigned long long sum = 0;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      sum += of(x[i].x, y[i].x, t + 128 * i);
+      sum += of(x[i].y, y[i].y, t + 128 * i + 1);
+      sum += of(x[i].z, y[i].z, t + 128 * i + 2);
+      sum += of(x[i].w, y[i].w, t + 128 * i + 3);
+    }
+    return sum;
   }
 };
 
@@ -110,10 +128,13 @@ verify_drafts_kernel(const aima_moe_verify_drafts c) {
 #pragma unroll 1
   for (int attempt = 0; attempt < 2 && !found; ++attempt) {
     unsigned long long sum = 0;
-#pragma unroll 4
-    for (int t = first + 4 * lane; t < last; t += 128) {
+    int t0 = first;
+    if (kAligned) {
+      for (; t0 + 128 * kAhead <= last; t0 += 128 * kAhead) sum += w.ahead(t0 + 4 * lane);
+    }
+    for (; t0 < last; t0 += 128) {
       unsigned long long v[4];
-      w.four<kAligned>(t, last, v);
+      w.four<kAligned>(t0 + 4 * lane, last, v);
       sum += (v[0] + v[1]) + (v[2] + v[3]);
     }
 #pragma unroll
@@ -123,7 +144,7 @@ verify_drafts_kernel(const aima_moe_verify_drafts c) {
     if (kBlocks > 1 && attempt == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     __syncthreads();
     if (warp == 0) {
-      unsigned long long mine = warp_sum[lane];
+      unsigned long long mine = lane < kWarps ? warp_sum[lane] : 0ull;
 #pragma unroll
       for (int d = 16; d >= 1; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
       if (kBlocks > 1) {
@@ -152,7 +173,7 @@ verify_drafts_kernel(const aima_moe_verify_drafts c) {
       if (before <= below && below - before < block_sum[attempt][rank]) {
         for (int i = 0; i < warp; ++i) before += warp_sum[i];
         if (before <= below && below - before < sum) {                  // one warp of all: its run holds the token
-          for (int t0 = first; t0 < last; t0 += 128) {
+          for (t0 = first; t0 < last; t0 += 128) {
             unsigned long long v[4];
             w.four<kAligned>(t0 + 4 * lane, last, v);
             const unsigned long long mine = (v[0] + v[1]) + (v[2] + v[3]);
