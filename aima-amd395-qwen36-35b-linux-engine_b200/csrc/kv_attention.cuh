@@ -74,8 +74,10 @@ __device__ __forceinline__ void kv_arrive(const KvWorkspace& work, const KvShare
 
 // Joins a unit's parts: waits until all have been written, then takes the `mine`-th share of its results.  Called by all
 // threads of a block.  The blocks of the launch are all resident (it is a cooperative one), and none waits before its own parts
-// are written; the wait has its limit all the same.  A result is four neighbouring elements of a row; 1 .. 32 lanes share the
-// parts of one, so that they are read by a few instructions, in the same order in every launch.
+// are written; the wait has its limit all the same.  A result is four neighbouring elements of a row.  Few parts (a row tile of a
+// prompt in two or three blocks): a thread keeps to one row, so that the parts' factors are found once, and all blocks share the
+// columns.  Many parts (one token's few rows in 74 blocks): 4 .. 32 lanes share the parts of a result.  Either way in the same
+// order in every launch.
 template <int kDim, int kThreads>
 __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace& work, const KvShared& unit, unsigned long long limit_ns, int* verdict) {
   unsigned* arrived = work.arrived + 2 * unit.first_block;
@@ -96,8 +98,60 @@ __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace&
   }
   __syncthreads();
   const bool ok = *verdict != 0;
-  if (ok) {
-    int lanes = 1;
+  auto store = [&](int row, int d, const float4& x, float inverse) {
+    const int token = row / a.shape.group, g = row - token * a.shape.group;
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inverse, x.y * inverse), hi = __floats2bfloat162_rn(x.z * inverse, x.w * inverse);
+    *reinterpret_cast<uint2*>(a.out + (static_cast<long long>(unit.row0 + token) * a.shape.q_heads + unit.head + g) * kDim + d) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  };
+  constexpr int kFew = 8;
+  if (ok && unit.parts <= kFew) {
+    const int at_once = kThreads / unit.rows, row = threadIdx.x % unit.rows;       // kThreads is at least a row tile's rows
+    const int end = 4 * (kDim / 4 * (unit.mine + 1) / unit.parts);
+    int d = 4 * (kDim / 4 * unit.mine / unit.parts + static_cast<int>(threadIdx.x) / unit.rows);
+    if (static_cast<int>(threadIdx.x) < at_once * unit.rows && d < end) {
+      float2 w[kFew];
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int p = 0; p < kFew; ++p) {
+        w[p] = make_float2(-INFINITY, 0.0f);
+        if (p < unit.parts) w[p] = __ldcg(kv_part_weight(work, kv_part_index(unit.first_block + p, p == 0), row));
+        top = fmaxf(top, w[p].x);
+      }
+      if (top == -INFINITY) top = 0.0f;                           // nothing seen, or nothing but NaN
+#pragma unroll
+      for (int p = 0; p < kFew; ++p) {
+        const float f = fast_exp2(w[p].x - top);
+        sum += w[p].x == -INFINITY ? w[p].y : w[p].y * f;
+        w[p].x = f;
+      }
+      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+      for (; d < end; d += 8 * at_once) {
+        const bool second = d + 4 * at_once < end;
+        float4 x[2][kFew];
+#pragma unroll
+        for (int p = 0; p < kFew; ++p) {
+          const size_t part = kv_part_index(unit.first_block + p, p == 0);
+          x[0][p] = x[1][p] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (p < unit.parts) x[0][p] = __ldcg(reinterpret_cast<const float4*>(kv_part_sum<kDim>(work, part, row, d)));
+          if (p < unit.parts && second) x[1][p] = __ldcg(reinterpret_cast<const float4*>(kv_part_sum<kDim>(work, part, row, d + 4 * at_once)));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+          for (int p = 0; p < kFew; ++p) {
+            acc.x = fmaf(x[i][p].x, w[p].x, acc.x);
+            acc.y = fmaf(x[i][p].y, w[p].x, acc.y);
+            acc.z = fmaf(x[i][p].z, w[p].x, acc.z);
+            acc.w = fmaf(x[i][p].w, w[p].x, acc.w);
+          }
+          if (i == 0 || second) store(row, d + 4 * at_once * i, acc, inverse);
+        }
+      }
+    }
+  } else if (ok) {
+    int lanes = 4;
     while (lanes < 32 && 4 * lanes < unit.parts) lanes *= 2;
     const int results = unit.rows * (kDim / 4);
     const int begin = results * unit.mine / unit.parts, end = results * (unit.mine + 1) / unit.parts;
@@ -140,14 +194,10 @@ __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace&
         acc.z += __shfl_xor_sync(0xffffffffu, acc.z, step);
         acc.w += __shfl_xor_sync(0xffffffffu, acc.w, step);
       }
-      if (lane == 0 && i0 + slot < end) {
-        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int token = row / a.shape.group, g = row - token * a.shape.group;
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inverse, acc.y * inverse), hi = __floats2bfloat162_rn(acc.z * inverse, acc.w * inverse);
-        *reinterpret_cast<uint2*>(a.out + (static_cast<long long>(unit.row0 + token) * a.shape.q_heads + unit.head + g) * kDim + d) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-      }
+      if (lane == 0 && i0 + slot < end) store(row, d, acc, sum == 0.0f ? 0.0f : 1.0f / sum);
     }
+  }
+  if (ok) {
     // the last to leave puts the counters back
     if (threadIdx.x == 0 && atomicAdd(arrived + 1, 1u) == static_cast<unsigned>(unit.parts) - 1u) {
       arrived[0] = 0;
@@ -164,6 +214,10 @@ __device__ __noinline__ void kv_zero_rows(const KvAttention& a, int row0, int ro
   const long long pieces = static_cast<long long>(rows) * a.shape.q_heads * (kDim / 8);
   for (long long i = threadIdx.x; i < pieces; i += kThreads) out[i] = make_uint4(0, 0, 0, 0);
 }
+
+// Shared memory of a block, so much at least that a SM holds one: a second block would wait for the first one's tensor memory, while
+// the first may wait for the second one's part of a unit.
+constexpr int kv_smem_bytes(int needed) { return needed > 120 * 1024 ? needed : 120 * 1024; }
 
 // Launches a kernel whose blocks are all resident, with programmatic serialisation like launch_pdl.
 template <typename... KernelArgs, typename... Args>

@@ -43,7 +43,7 @@ struct Decode {
   static constexpr int kOutPanels = kDim >= 128 ? kDim / 128 : 1;
   static constexpr int kOutColumn = 4 * kRows;                          // tensor memory: S0 | S1 | per panel hi | lo
   static constexpr int kQueryAt = kSlots * kSlotBytes;
-  static constexpr int kWeightAt = kQueryAt + kQueryBytes;
+  static constexpr int kWeightAt = kQueryAt + 2 * kQueryBytes;          // two segments' queries
   static constexpr int kPrefixAt = kWeightAt + 4 * kWeightBytes;
   static constexpr int kSmallAt = (kPrefixAt + kMaxPrefix * 4 + 15) / 16 * 16;
 };
@@ -57,8 +57,8 @@ struct SegmentInfo {
 template <int kRows>
 struct Small {              // shared memory that is not an operand
   unsigned long long full[8], empty[8];
-  unsigned long long s_full[2], s_empty[2], p_full[2], o_done[2], q_full[2], info_empty[2], q_empty, drain;
-  float part[2][kRows][4];  // per row and warp: maxima of a tile (two buffers), sums at the end of a segment
+  unsigned long long s_full[2], s_empty[2], p_full[2], o_done[2], q_full[2], info_empty[2], drain;
+  alignas(16) float part[2][kRows][4];  // per row and warp: maxima of a tile (two buffers), sums at the end of a segment
   float row_scale[2][kRows];
   int limit[2][kRows];      // last position a row sees; -1: none
   long long out_at[2][kRows];
@@ -136,7 +136,6 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
       mbar_init(smem_u32(&sm.q_full[i]), 2);
       mbar_init(smem_u32(&sm.info_empty[i]), 4);
     }
-    mbar_init(smem_u32(&sm.q_empty), 1);
     mbar_init(smem_u32(&sm.drain), 1);
     sm.abort_flag = 0;
     sm.shared[0].parts = sm.shared[1].parts = 0;
@@ -267,7 +266,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
         if (!wait(&sm.full[slot], (r / L::kSlots) & 1) || !wait(&sm.s_empty[buffer], (((tile + j) >> 1) & 1) ^ 1)) return false;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t k0 = base + slot * L::kSlotBytes, q0 = base + L::kQueryAt;
+          const uint32_t k0 = base + slot * L::kSlotBytes, q0 = base + L::kQueryAt + (segment & 1) * L::kQueryBytes;
 #pragma unroll
           for (int k = 0; k < kDim / 32; ++k) {
             const int panel = k * 32 / L::kRowBytes, inside = k * 32 % L::kRowBytes;
@@ -276,7 +275,6 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
           }
           umma_commit(smem_u32(&sm.empty[slot]));
           umma_commit(smem_u32(&sm.s_full[buffer]));
-          if (j + 1 == n) umma_commit(smem_u32(&sm.q_empty));
         }
         __syncwarp();
         return true;
@@ -318,7 +316,8 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
     while (alive && walk.next()) {
       const KvSequence seq = kv_sequence(a.batch, shape, walk.sequence);
       const int rows = seq.rows * shape.group, which = segment & 1;
-      if (!wait(&sm.info_empty[which], ((segment >> 1) & 1) ^ 1) || !wait(&sm.q_empty, (segment & 1) ^ 1)) break;
+      // empty once the segment before the last has been finished: its products too
+      if (!wait(&sm.info_empty[which], ((segment >> 1) & 1) ^ 1)) break;
       if (warp == 2 && lane == 0) sm.info[which] = SegmentInfo{seq.length, rows, seq.row0};
 #pragma unroll 1
       for (int r0 = 4 * (warp - 2); r0 < kRows; r0 += 8) {       // four rows side by side: one alone is a chain of 340 cycles
@@ -369,7 +368,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
             const int row = r + term * kRows, byte = lane * kPer;
             const int panel = byte / L::kRowBytes, inside = byte % L::kRowBytes;
             const int piece = (inside >> 4) ^ (L::kRowBytes == 128 ? row & 7 : (row >> 1) & 3);
-            uint8_t* to = generic + L::kQueryAt + (panel * 2 * kRows + row) * L::kRowBytes + piece * 16 + (inside & 15);
+            uint8_t* to = generic + L::kQueryAt + which * L::kQueryBytes + (panel * 2 * kRows + row) * L::kRowBytes + piece * 16 + (inside & 15);
             if constexpr (kPer == 8) *reinterpret_cast<uint2*>(to) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
             else if constexpr (kPer == 4) *reinterpret_cast<uint32_t*>(to) = c[0] | (c[1] << 16);
             else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(c[0]);
@@ -614,7 +613,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
 
 template <int kDim, int kRows>
 cudaError_t launch(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
-  constexpr int bytes = Decode<kDim, kRows>::kSmallAt + static_cast<int>(sizeof(Small<kRows>)) + 1024;
+  constexpr int bytes = kv_smem_bytes(Decode<kDim, kRows>::kSmallAt + static_cast<int>(sizeof(Small<kRows>)) + 1024);
   static_assert(bytes <= 227 * 1024, "more shared memory than a block can have");
   const cudaError_t error = opt_in_dynamic_smem<kv_decode_kernel<kDim, kRows>>(bytes);
   if (error != cudaSuccess) return error;

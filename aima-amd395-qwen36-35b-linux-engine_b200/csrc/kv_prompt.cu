@@ -798,7 +798,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
 
 template <int kDim, bool kPlanned>
 cudaError_t launch_planned(const KvAttentionPlan& plan, const KvMaps& maps, const CUtensorMap& queries, cudaStream_t stream) {
-  constexpr int bytes = Prompt<kDim>::kSmallAt + static_cast<int>(sizeof(Small)) + 1024;
+  constexpr int bytes = kv_smem_bytes(Prompt<kDim>::kSmallAt + static_cast<int>(sizeof(Small)) + 1024);
   static_assert(bytes <= 227 * 1024, "more shared memory than a block can have");
   static_assert(sizeof(PlanMemory<kThreads>) + 8 * kThreads <= Prompt<kDim>::kQueryAt, "the plan lies in the ring");
   const cudaError_t error = opt_in_dynamic_smem<kv_prompt_kernel<kDim, kPlanned>>(bytes);
