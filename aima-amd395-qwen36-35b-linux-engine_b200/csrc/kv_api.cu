@@ -19,7 +19,8 @@ struct aima_moe_kv {
   bool bound[AIMA_MOE_KV_MAX_LAYERS]{};
   const float* rotation = nullptr;     // the caller's
   int positions = 0;
-  int* status = nullptr;               // the allocation: 256 bytes, then the attention's workspace
+  int* status = nullptr;               // the workspace: 256 bytes, then the attention's
+  bool owns = false;                   // whether prepare allocated it
   cudaStream_t last_stream = nullptr;
 };
 
@@ -71,6 +72,15 @@ int check_config(const aima_moe_kv_config* c) {
     return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: softmax_scale must be finite and not negative");
   return AIMA_MOE_OK;
 }
+
+aima::KvShape shape_of(const aima_moe_kv_config& c) {
+  int shift = 4;
+  while ((1u << shift) < c.page_tokens) ++shift;
+  return aima::KvShape{static_cast<int>(c.q_heads), static_cast<int>(c.kv_heads), static_cast<int>(c.q_heads / c.kv_heads),
+                       static_cast<int>(c.head_dim), static_cast<int>(c.rotary_dim), static_cast<int>(c.page_tokens), shift,
+                       static_cast<int>(c.pages)};
+}
+uint64_t workspace_bytes(const aima::KvShape& shape) { return 256 + aima::kv_workspace_bytes(shape); }
 
 int check_device_pointer(const void* pointer, int device, const char* name) {
   cudaPointerAttributes attributes{};
@@ -137,6 +147,13 @@ extern "C" {
 
 #define AIMA_EXPORT __attribute__((visibility("default")))
 
+AIMA_EXPORT int aima_moe_kv_query_workspace(const aima_moe_kv_config* config, uint64_t* bytes) {
+  if (bytes == nullptr) return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: bytes is null");
+  if (const int status = check_config(config); status != AIMA_MOE_OK) return status;
+  *bytes = workspace_bytes(shape_of(*config));
+  return AIMA_MOE_OK;
+}
+
 AIMA_EXPORT int aima_moe_kv_prepare(const aima_moe_kv_config* config, aima_moe_kv** out) {
   if (out == nullptr) return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: handle is null");
   *out = nullptr;
@@ -157,17 +174,29 @@ AIMA_EXPORT int aima_moe_kv_prepare(const aima_moe_kv_config* config, aima_moe_k
   h->device = device;
   h->sm_count = sm_count;
   h->config = *config;
-  int shift = 4;
-  while ((1u << shift) < config->page_tokens) ++shift;
-  h->shape = aima::KvShape{static_cast<int>(config->q_heads), static_cast<int>(config->kv_heads), static_cast<int>(config->q_heads / config->kv_heads),
-                           static_cast<int>(config->head_dim), static_cast<int>(config->rotary_dim), static_cast<int>(config->page_tokens), shift,
-                           static_cast<int>(config->pages)};
+  h->shape = shape_of(*config);
   const double scale = config->softmax_scale != 0.0f ? config->softmax_scale : 1.0 / std::sqrt(static_cast<double>(config->head_dim));
   h->scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-  error = cudaMalloc(&h->status, 256 + aima::kv_workspace_bytes(h->shape));
+  const uint64_t bytes = workspace_bytes(h->shape);
+  if (config->workspace != nullptr) {
+    int status = AIMA_MOE_OK;
+    if (reinterpret_cast<uintptr_t>(config->workspace) % 256 != 0 || config->workspace_bytes < bytes)
+      status = kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: the workspace is not 256-byte aligned or has less than %llu bytes",
+                       static_cast<unsigned long long>(bytes));
+    else
+      status = check_device_pointer(config->workspace, device, "the workspace");
+    if (status != AIMA_MOE_OK) {
+      delete h;
+      return status;
+    }
+    h->status = static_cast<int*>(config->workspace);
+  } else {
+    error = cudaMalloc(&h->status, bytes);
+    h->owns = true;
+  }
   if (error == cudaSuccess) error = cudaMemset(h->status, 0, 256 + aima::kv_counter_bytes());
   if (error != cudaSuccess) {
-    cudaFree(h->status);
+    if (h->owns) cudaFree(h->status);
     delete h;
     return kv_fail_cuda(error, "allocation of the kv workspace");
   }
@@ -279,7 +308,7 @@ AIMA_EXPORT int aima_moe_kv_sync(aima_moe_kv* h) {
 
 AIMA_EXPORT int aima_moe_kv_release(aima_moe_kv* h) {
   if (h == nullptr) return AIMA_MOE_OK;
-  cudaFree(h->status);
+  if (h->owns) cudaFree(h->status);
   delete h;
   return AIMA_MOE_OK;
 }

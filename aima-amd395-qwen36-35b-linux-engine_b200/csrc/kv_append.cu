@@ -122,7 +122,7 @@ __device__ __forceinline__ void rotate_queries(const KvAppend& a, long long bloc
   for (int h = 0; h < kHeadsPerThread; ++h) {
     raw[h] = make_uint4(0, 0, 0, 0);
     if (exists && head0 + h < shape.q_heads)
-      raw[h] = *reinterpret_cast<const uint4*>(a.q.data + row * a.q.row_stride + (head0 + h) * a.q.head_stride + 8 * piece);
+      raw[h] = __ldcs(reinterpret_cast<const uint4*>(a.q.data + row * a.q.row_stride + (head0 + h) * a.q.head_stride + 8 * piece));
   }
   int position = -1;
   if (exists) {
@@ -150,7 +150,7 @@ __device__ __forceinline__ void rotate_queries(const KvAppend& a, long long bloc
 // One block per (sequence, touched page, head), then blocks for the queries.  A page and head belongs to one block, which
 // holds all of its new rows in registers between finding the scale and writing the codes: every byte is read once.
 template <int kDim, int kPage>
-__global__ void __launch_bounds__(append_threads<kDim, kPage>, 1024 / append_threads<kDim, kPage>)
+__global__ void __launch_bounds__(append_threads<kDim, kPage>, append_threads<kDim, kPage> > 512 ? 1 : 512 / append_threads<kDim, kPage>)
 kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
   constexpr int kAppendThreads = append_threads<kDim, kPage>;
   constexpr int kPieces = kDim / 8;                                   // 16-byte vectors of a head
@@ -283,7 +283,7 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
 }
 
 template <int kDim>
-__global__ void __launch_bounds__(kRotateThreads)
+__global__ void __launch_bounds__(kRotateThreads, 4)
 kv_rotate_kernel(const KvAppend a) {
   rotate_queries<kDim, kRotateThreads>(a, blockIdx.x);
   pdl_wait();          // the page kernel has ended when this one does: whoever waits for this one waits for both

@@ -107,6 +107,7 @@ class KvConfig(ctypes.Structure):
     _fields_ = [
         ("struct_bytes", c_uint32), ("q_heads", c_uint32), ("kv_heads", c_uint32), ("head_dim", c_uint32), ("rotary_dim", c_uint32),
         ("page_tokens", c_uint32), ("pages", c_uint32), ("layers", c_uint32), ("max_sequences", c_uint32), ("softmax_scale", c_float),
+        ("workspace", c_void_p), ("workspace_bytes", c_uint64),
     ]
 
 
@@ -199,6 +200,7 @@ EXPORTS = [
     ("aima_moe_image_scatter_ingest", c_int,
      [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(c_uint64), ctypes.POINTER(c_uint64), ctypes.POINTER(c_uint64),
       c_uint64, c_uint64, c_uint64, c_uint64, c_int, c_uint64, c_uint64, ctypes.POINTER(ImageIngestResult)]),
+    ("aima_moe_kv_query_workspace", c_int, [ctypes.POINTER(KvConfig), ctypes.POINTER(c_uint64)]),
     ("aima_moe_kv_prepare", c_int, [ctypes.POINTER(KvConfig), ctypes.POINTER(c_void_p)]),
     ("aima_moe_kv_bind_layer", c_int, [c_void_p, c_uint32, ctypes.POINTER(KvLayer)]),
     ("aima_moe_kv_set_rotation", c_int, [c_void_p, c_void_p, c_uint32]),
@@ -751,12 +753,17 @@ class KvCache:
         self._torch = torch
         self.lib = library or load_library()
         self.config = KvConfig(ctypes.sizeof(KvConfig), q_heads, kv_heads, head_dim, rotary_dim, page_tokens, pages, layers, max_sequences,
-                               softmax_scale)
-        handle = c_void_p()
+                               softmax_scale, None, 0)
+        size, handle = c_uint64(), c_void_p()
+        self.lib.check(self.lib.aima_moe_kv_query_workspace(ctypes.byref(self.config), ctypes.byref(size)))
+        # from torch's allocator, which has it at hand where the driver takes milliseconds
+        self._workspace = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+        self.config.workspace, self.config.workspace_bytes = self._workspace.data_ptr(), size.value
         self.lib.check(self.lib.aima_moe_kv_prepare(ctypes.byref(self.config), ctypes.byref(handle)))
         self.handle = handle
         self._q_shape, self._kv_shape = (q_heads, head_dim), (kv_heads, head_dim)
         self._keepalive: dict[Any, Any] = {}
+        self._streams: set[int] = set()
 
     # -- setup ---------------------------------------------------------------
     def allocate_layer(self) -> tuple[Any, Any, Any, Any]:
@@ -819,15 +826,20 @@ class KvCache:
             q_rows = self._rows(q, "q", (batch.tokens, *self._q_shape))
             q_out = self._out(q_out, q, "q_out")
         self.lib.check(self.lib.aima_moe_kv_append_launch(
-            self.handle, layer, batch.ref, k_rows, v_rows, q_rows, None if q is None else q_out.data_ptr(), _raw_stream(self._torch)))
+            self.handle, layer, batch.ref, k_rows, v_rows, q_rows, None if q is None else q_out.data_ptr(), self._stream()))
         return q_out
 
     def attention(self, layer: int, batch: KvBatch, q: Any, out: Any = None) -> Any:
         """Causal attention of the batch's rows over the cache (after append): [tokens, q_heads, head_dim]."""
         q_rows = self._rows(q, "q", (batch.tokens, *self._q_shape))
         out = self._out(out, q, "out")
-        self.lib.check(self.lib.aima_moe_kv_attention_launch(self.handle, layer, batch.ref, q_rows, out.data_ptr(), _raw_stream(self._torch)))
+        self.lib.check(self.lib.aima_moe_kv_attention_launch(self.handle, layer, batch.ref, q_rows, out.data_ptr(), self._stream()))
         return out
+
+    def _stream(self) -> int:
+        stream = _raw_stream(self._torch)
+        self._streams.add(stream)
+        return stream
 
     def sync(self) -> None:
         """Waits for the last launch and raises AimaMoeError if device-side data of a batch was out of range."""
@@ -837,6 +849,9 @@ class KvCache:
         if getattr(self, "handle", None):
             self.lib.aima_moe_kv_release(self.handle)
             self.handle = None
+            for stream in self._streams:        # what is under way there still uses the workspace
+                self._workspace.record_stream(self._torch.cuda.ExternalStream(stream))
+            self._workspace = None
             self._keepalive.clear()
 
     def __del__(self) -> None:  # best effort

@@ -516,8 +516,11 @@ typedef struct aima_moe_kv_config {
   uint32_t page_tokens;    /* 16, 32, 64 or 128                                                   */
   uint32_t pages;          /* pages of every layer's tensors; pages * kv_heads * page_tokens < 2^31 */
   uint32_t layers;         /* 1 .. AIMA_MOE_KV_MAX_LAYERS                                         */
-  uint32_t max_sequences;  /* 1 .. AIMA_MOE_KV_MAX_SEQUENCES sequences in a batch                 */
+  uint32_t max_sequences;  /* 1 .. AIMA_MOE_KV_MAX_SEQUENCES sequences in a batch; over a batch kv_heads * tiles of 128 tokens
+                              (for prompts times the row tiles) stay within 2^24                  */
   float softmax_scale;     /* of the scores; 0 = 1 / sqrt(head_dim)                               */
+  void* workspace;         /* device memory of the caller's, 256-byte aligned, for the handle's lifetime; NULL: prepare allocates */
+  uint64_t workspace_bytes; /* of it, at least what aima_moe_kv_query_workspace says               */
 } aima_moe_kv_config;
 
 typedef struct aima_moe_kv_layer {
@@ -550,7 +553,10 @@ typedef struct aima_moe_kv_rows {
   uint64_t head_stride;
 } aima_moe_kv_rows;
 
-/* Checks the configuration and allocates the workspace on the current device (the only allocation). */
+/* Device bytes of a handle's workspace (about 40 MB at head_dim 256), which depend on head_dim alone. */
+int aima_moe_kv_query_workspace(const aima_moe_kv_config* config, uint64_t* bytes);
+/* Checks the configuration and, unless the caller brings the workspace, allocates it on the current device (the only
+ * allocation; it takes the driver milliseconds). */
 int aima_moe_kv_prepare(const aima_moe_kv_config* config, aima_moe_kv** handle);
 /* Records one layer's cache tensors.  16-byte aligned, of the handle's device. */
 int aima_moe_kv_bind_layer(aima_moe_kv* handle, uint32_t layer, const aima_moe_kv_layer* tensors);
