@@ -110,13 +110,16 @@ int check_batch(const aima_moe_kv* h, const aima_moe_kv_batch* b, aima::KvBatch*
   return AIMA_MOE_OK;
 }
 
-int check_rows(const aima_moe_kv_rows* rows, const char* name, aima::KvRows* out) {
+int check_rows(const aima_moe_kv_rows* rows, const char* name, int tokens, int heads, int head_dim, aima::KvRows* out) {
   if (rows == nullptr || rows->data == nullptr) return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: %s is null", name);
-  if (misaligned(rows->data) || rows->row_stride % 8 != 0 || rows->head_stride % 8 != 0)
+  // what a single head or row has as its stride means nothing
+  const uint64_t head_stride = heads > 1 ? rows->head_stride : tokens > 1 ? rows->row_stride : head_dim;
+  const uint64_t row_stride = tokens > 1 ? rows->row_stride : head_stride * heads;
+  if (misaligned(rows->data) || row_stride % 8 != 0 || head_stride % 8 != 0)
     return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: %s must be 16-byte aligned with strides that are multiples of 8 elements", name);
-  if (rows->row_stride >= (1ull << 36) || rows->head_stride >= (1ull << 36))
+  if (row_stride >= (1ull << 36) || head_stride >= (1ull << 36))
     return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: a stride of %s is too large", name);
-  *out = aima::KvRows{static_cast<const __nv_bfloat16*>(rows->data), static_cast<long long>(rows->row_stride), static_cast<long long>(rows->head_stride)};
+  *out = aima::KvRows{static_cast<const __nv_bfloat16*>(rows->data), static_cast<long long>(row_stride), static_cast<long long>(head_stride)};
   return AIMA_MOE_OK;
 }
 
@@ -194,7 +197,9 @@ AIMA_EXPORT int aima_moe_kv_prepare(const aima_moe_kv_config* config, aima_moe_k
     error = cudaMalloc(&h->status, bytes);
     h->owns = true;
   }
-  if (error == cudaSuccess) error = cudaMemset(h->status, 0, 256 + aima::kv_counter_bytes());
+  // here and now: the launches may come on streams that do not wait for the default one
+  if (error == cudaSuccess) error = cudaMemsetAsync(h->status, 0, 256 + aima::kv_counter_bytes(), cudaStreamPerThread);
+  if (error == cudaSuccess) error = cudaStreamSynchronize(cudaStreamPerThread);
   if (error != cudaSuccess) {
     if (h->owns) cudaFree(h->status);
     delete h;
@@ -250,10 +255,10 @@ AIMA_EXPORT int aima_moe_kv_append_launch(aima_moe_kv* h, uint32_t layer, const 
   a.shape = h->shape;
   a.layer = h->layers[layer];
   if (const int status = check_batch(h, batch, &a.batch); status != AIMA_MOE_OK) return status;
-  if (const int status = check_rows(k, "k", &a.k); status != AIMA_MOE_OK) return status;
-  if (const int status = check_rows(v, "v", &a.v); status != AIMA_MOE_OK) return status;
+  if (const int status = check_rows(k, "k", a.batch.tokens, h->shape.kv_heads, h->shape.head_dim, &a.k); status != AIMA_MOE_OK) return status;
+  if (const int status = check_rows(v, "v", a.batch.tokens, h->shape.kv_heads, h->shape.head_dim, &a.v); status != AIMA_MOE_OK) return status;
   if (q != nullptr && q->data != nullptr) {
-    if (const int status = check_rows(q, "q", &a.q); status != AIMA_MOE_OK) return status;
+    if (const int status = check_rows(q, "q", a.batch.tokens, h->shape.q_heads, h->shape.head_dim, &a.q); status != AIMA_MOE_OK) return status;
     if (q_out == nullptr || misaligned(q_out)) return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: q_out is null or not 16-byte aligned");
     if (overlaps(a.q, q_out, h->shape, a.batch.tokens)) return kv_fail(AIMA_MOE_ERR_ALIAS, "kv: q_out overlaps q");
     a.q_out = static_cast<__nv_bfloat16*>(q_out);
@@ -276,7 +281,7 @@ AIMA_EXPORT int aima_moe_kv_attention_launch(aima_moe_kv* h, uint32_t layer, con
   a.shape = h->shape;
   a.layer = h->layers[layer];
   if (const int status = check_batch(h, batch, &a.batch); status != AIMA_MOE_OK) return status;
-  if (const int status = check_rows(q, "q", &a.q); status != AIMA_MOE_OK) return status;
+  if (const int status = check_rows(q, "q", a.batch.tokens, h->shape.q_heads, h->shape.head_dim, &a.q); status != AIMA_MOE_OK) return status;
   if (out == nullptr || misaligned(out)) return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: out is null or not 16-byte aligned");
   if (overlaps(a.q, out, h->shape, a.batch.tokens)) return kv_fail(AIMA_MOE_ERR_ALIAS, "kv: out overlaps q");
   a.out = static_cast<__nv_bfloat16*>(out);

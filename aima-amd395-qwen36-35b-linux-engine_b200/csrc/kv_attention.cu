@@ -76,6 +76,7 @@ cudaError_t kv_attention(const KvAttention& a, const KvMaps& maps, void* workspa
   plan.blocks = sm_count < kKvMaxBlocks ? sm_count : kKvMaxBlocks;
   plan.tile_rows = static_cast<int>(std::min(static_cast<long long>(a.batch.max_new) * a.shape.group, 1ll << 30));
   plan.tile_tokens = kKvTile / a.shape.group;
+  plan.query_map = kv_query_map_fits(a.q);
   plan.wait_limit_ns = kWaitBudgetNs;
   return plan.tile_rows <= kDecodeRows ? kv_decode(plan, maps, stream) : kv_prompt(plan, maps, stream);
 }

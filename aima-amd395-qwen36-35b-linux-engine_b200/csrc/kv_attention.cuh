@@ -42,6 +42,7 @@ struct KvAttentionPlan {
   int blocks;
   int tile_rows;          // rows that a sequence has at most for one key/value head
   int tile_tokens;        // prompts: new tokens of a row tile
+  bool query_map;         // prompts: queries come through a tensor map
   unsigned long long wait_limit_ns;
 };
 
@@ -237,6 +238,8 @@ inline cudaError_t launch_resident(void (*kernel)(KernelArgs...), dim3 grid, dim
   return cudaLaunchKernelEx(&config, kernel, static_cast<KernelArgs>(args)...);
 }
 
+// Whether queries of these strides can have a tensor map: each stride is a whole multiple of the one before it, and none is zero.
+inline bool kv_query_map_fits(const KvRows& q) { return q.head_stride > 0 && q.row_stride > 0 && q.row_stride % q.head_stride == 0; }
 // Map of a call's queries: boxes of kRowBytes x the heads of a key/value head x tile_tokens.
 bool kv_make_query_map(const KvAttention& a, int tile_tokens, CUtensorMap* map);
 cudaError_t kv_decode(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream);

@@ -13,7 +13,7 @@ constexpr int kKvBadBatch = 1;       // a page number, length, row offset or pos
 constexpr int kKvTimeout = 2;        // a bounded wait ran out
 
 constexpr int kKvMinExponent = -64;  // of a scale: values below 2^-73 of a page that has nothing larger become zero
-constexpr int kKvMaxExponent = 119;  // 448 * 2^119 exceeds the largest BF16 value
+constexpr int kKvMaxExponent = 120;  // 448 * 2^119 is below the largest BF16 values
 constexpr uint8_t kKvNan = 0x7f;     // e4m3 NaN
 
 // 2^e, e in -126 .. 127

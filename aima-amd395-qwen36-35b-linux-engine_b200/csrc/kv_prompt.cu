@@ -459,16 +459,30 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
     } else if (warp == 2) {
       // ------------------------------ queries, as they are ------------------------------
       // A BF16 row of a head is as long as its two terms together and goes where they will lie, kRowBytes at a time, so that it
-      // can be converted in place.  Rows behind the unit's last are another unit's or zeros; their results go nowhere.
+      // can be converted in place.  Rows behind the unit's last are another unit's, zeros or what lay there; their results go
+      // nowhere.  Strides that a tensor map cannot have (see kv_query_map_fits) are loaded row by row: 4 .. 8 copies per row
+      // instead of as many per unit.
       int segment = 0;
       for (; walk.next(); ++segment, walk.advance()) {
         if (!wait(&sm.q_empty, (segment & 1) ^ 1)) break;
-        if (elect_one()) {
-          constexpr int kBoxes = 2 * kDim / L::kRowBytes;
-          mbar_arrive_expect_tx(smem_u32(&sm.q_raw), kBoxes * plan.tile_tokens * shape.group * L::kRowBytes);
-          for (int i = 0; i < kBoxes; ++i)
-            tma_load_3d(base + L::kQueryAt + (i / L::kPanels) * L::kSlotBytes + (i % L::kPanels) * L::kPanelBytes, &queries, i * L::kRowBytes / 2,
-                        walk.head * shape.group, walk.seq.row0 + walk.row_tile * plan.tile_tokens, smem_u32(&sm.q_raw));
+        constexpr int kBoxes = 2 * kDim / L::kRowBytes;
+        auto box_at = [&](int i) { return base + L::kQueryAt + (i / L::kPanels) * L::kSlotBytes + (i % L::kPanels) * L::kPanelBytes; };
+        const int row0 = walk.seq.row0 + walk.row_tile * plan.tile_tokens, head0 = walk.head * shape.group;
+        if (plan.query_map) {
+          if (elect_one()) {
+            mbar_arrive_expect_tx(smem_u32(&sm.q_raw), kBoxes * plan.tile_tokens * shape.group * L::kRowBytes);
+            for (int i = 0; i < kBoxes; ++i) tma_load_3d(box_at(i), &queries, i * L::kRowBytes / 2, head0, row0, smem_u32(&sm.q_raw));
+          }
+        } else {
+          const int rows = walk.unit.tokens * shape.group;
+          if (lane == 0) mbar_arrive_expect_tx(smem_u32(&sm.q_raw), rows * 2 * kDim);
+          __syncwarp();
+          for (int r = lane; r < rows; r += 32) {
+            const int token = r / shape.group;
+            const __nv_bfloat16* from = a.q.data + (row0 + token) * a.q.row_stride + (head0 + r - token * shape.group) * a.q.head_stride;
+#pragma unroll 1
+            for (int i = 0; i < kBoxes; ++i) bulk_g2s(box_at(i) + r * L::kRowBytes, from + i * L::kRowBytes / 2, L::kRowBytes, smem_u32(&sm.q_raw));
+          }
         }
         __syncwarp();
       }
@@ -810,8 +824,8 @@ template <int kDim>
 cudaError_t launch(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
   // row tiles at most; with one for each thread of a block every block can find its share by itself
   const long long items = plan.a.batch.tokens / plan.tile_tokens + plan.a.batch.sequences;
-  CUtensorMap queries;
-  if (!kv_make_query_map(plan.a, plan.tile_tokens, &queries)) return cudaErrorInvalidValue;
+  CUtensorMap queries{};
+  if (plan.query_map && !kv_make_query_map(plan.a, plan.tile_tokens, &queries)) return cudaErrorInvalidValue;
   if (items <= kThreads) return launch_planned<kDim, false>(plan, maps, queries, stream);
   const cudaError_t error = launch_pdl(kv_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, plan);
   return error != cudaSuccess ? error : launch_planned<kDim, true>(plan, maps, queries, stream);

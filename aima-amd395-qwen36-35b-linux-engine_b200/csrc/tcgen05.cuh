@@ -140,11 +140,6 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2_f16x2(uint32_t h) {
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(h));
   return r;
 }
-__device__ __forceinline__ uint32_t cvt_e5m2x2_f16x2(uint32_t h) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(r) : "r"(h));
-  return r;
-}
 __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t codes) {
   uint32_t h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(codes)));

@@ -759,6 +759,7 @@ class KvCache:
         # from torch's allocator, which has it at hand where the driver takes milliseconds
         self._workspace = torch.empty(size.value, dtype=torch.uint8, device="cuda")
         self.config.workspace, self.config.workspace_bytes = self._workspace.data_ptr(), size.value
+        torch.cuda.current_stream().synchronize()      # what had this memory before is done with it
         self.lib.check(self.lib.aima_moe_kv_prepare(ctypes.byref(self.config), ctypes.byref(handle)))
         self.handle = handle
         self._q_shape, self._kv_shape = (q_heads, head_dim), (kv_heads, head_dim)

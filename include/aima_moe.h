@@ -519,7 +519,8 @@ typedef struct aima_moe_kv_config {
   uint32_t max_sequences;  /* 1 .. AIMA_MOE_KV_MAX_SEQUENCES sequences in a batch; over a batch kv_heads * tiles of 128 tokens
                               (for prompts times the row tiles) stay within 2^24                  */
   float softmax_scale;     /* of the scores; 0 = 1 / sqrt(head_dim)                               */
-  void* workspace;         /* device memory of the caller's, 256-byte aligned, for the handle's lifetime; NULL: prepare allocates */
+  void* workspace;         /* device memory of the caller's, 256-byte aligned, from prepare (nothing under way may use it)
+                              for the handle's lifetime; NULL: prepare allocates                  */
   uint64_t workspace_bytes; /* of it, at least what aima_moe_kv_query_workspace says               */
 } aima_moe_kv_config;
 
@@ -546,7 +547,7 @@ typedef struct aima_moe_kv_batch {
 } aima_moe_kv_batch;
 
 /* Rows of heads: element (row, head, i) is at row * row_stride + head * head_stride + i, in elements (BF16).  16-byte
- * aligned, strides multiples of 8. */
+ * aligned, strides multiples of 8 (zero too: a broadcast); the stride of a single row or head is not looked at. */
 typedef struct aima_moe_kv_rows {
   const void* data;
   uint64_t row_stride;

@@ -6,7 +6,7 @@ import math
 
 import torch
 
-LARGEST, MIN_EXPONENT, MAX_EXPONENT = 448.0, -64, 119
+LARGEST, MIN_EXPONENT, MAX_EXPONENT = 448.0, -64, 120
 
 
 def e4m3(x: torch.Tensor) -> torch.Tensor:

@@ -164,6 +164,15 @@ def test_append_exact_edges_of_a_scale(package):
         assert setup.gpu[3].cpu()[int(setup.table[0, 0]), 0] == 2.0 ** exponent
 
 
+def test_append_of_the_largest_values(package):
+    """Above 448 * 2^119 (2.98e38) a page needs the scale 2^120; BF16 ends at 3.39e38."""
+    setup = Setup(package, [40, 70], [5, 70], rotary=0, seed=8)
+    k, v = (setup.randn(setup.tokens, 2, 256) for _ in range(2))
+    largest = torch.finfo(torch.bfloat16).max
+    k[3], v[3, 1], k[40, 0, 7], v[60, 0, 0] = largest, -largest, -3.0e38, 2.97e38
+    _check_append(setup, k, v, gpu_rows=(k.cuda(), v.cuda(), None))
+
+
 def test_append_token_by_token_stores_what_one_call_stores(package):
     """Powers of two: a page filled one token at a time ends with the scale, and up to codes below the normal range the codes, of
     a page filled at once."""
@@ -247,6 +256,32 @@ def test_attention_of_strided_queries(package, new):
     setup = Setup(package, [300, 77], [new, new], seed=21)
     wide = setup.randn(setup.tokens, 16, 512)
     _check_attention(setup, wide[:, :, :256], wide.cuda()[:, :, :256])
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("heads", [(16, 2, 256), (6, 2, 128), (8, 8, 64)])
+@pytest.mark.parametrize("layout", ["heads first", "one row for all", "one head for all", "rows that are no multiple of heads"])
+def test_queries_of_any_strides(package, new, heads, layout):
+    setup = Setup(package, [300, 77], [new, new], heads, seed=22)
+    n, (h, _, dim) = setup.tokens, heads
+    if layout == "heads first":
+        gpu = setup.randn(h, n, dim).cuda().transpose(0, 1)
+    elif layout == "one row for all":
+        gpu = setup.randn(1, h, dim).cuda().expand(n, h, dim)
+    elif layout == "one head for all":
+        gpu = setup.randn(n, 1, dim).cuda().expand(n, h, dim)
+    else:
+        gpu = setup.randn(n, h * dim + 8).cuda()[:, :h * dim].unflatten(1, (h, dim))
+    _check_attention(setup, gpu.cpu(), gpu)
+
+
+def test_strides_of_a_single_row_or_head_are_not_looked_at(package):
+    setup = Setup(package, [300], [1], seed=23)
+    q = setup.randn(1, 16, 256)
+    _check_attention(setup, q, torch.as_strided(q.cuda(), (1, 16, 256), (3, 256, 1)))
+    setup = Setup(package, [300], [200], (1, 1, 128), seed=24)
+    q = setup.randn(200, 1, 128)
+    _check_attention(setup, q, torch.as_strided(q.cuda(), (200, 1, 128), (128, 3, 1)))
 
 
 @pytest.mark.parametrize("new", [1, 40])
@@ -384,6 +419,57 @@ def test_another_stream_and_a_captured_graph(package):
         codes = [t.cpu().float() for t in setup.gpu]
         want, spread = kv_oracle.attention(*codes, setup.table.tolist(), setup.offsets, lengths, q.cpu(), 1 / 16, 64)
         assert ((out.cpu().double() - want).abs() <= want.abs() * 2.0 ** -8 + spread * (2.0 ** -8 + 2.0 ** -9)).all()
+
+
+def test_a_handle_of_a_side_stream_and_its_release_with_work_under_way(package):
+    """The workspace comes from the stream that is current at creation and goes back without a wait: what is still under way on
+    another stream keeps it."""
+    setup = Setup(package, [3000, 2000], [40, 40], seed=92)
+    q = setup.randn(80, 16, 256).cuda()
+    want = setup.cache.attention(1, setup.batch, q)
+    torch.cuda.synchronize()
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(first):
+        scratch = [torch.full((1 << 24,), 0x7f7f7f7f, dtype=torch.int32, device="cuda") for _ in range(4)]
+        del scratch                                              # memory that is written when the handle is made from it
+        cache = package.KvCache(rotary_dim=0, pages=setup.cache.config.pages, layers=2, max_sequences=2)
+        cache.bind_layer(1, *setup.gpu)
+    with torch.cuda.stream(second):
+        outs = [cache.attention(1, setup.batch, q) for _ in range(50)]
+        cache.release()
+    with torch.cuda.stream(first):
+        scratch = [torch.full((1 << 24,), 0x7f7f7f7f, dtype=torch.int32, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for out in outs)
+
+
+def test_workspace_of_the_callers(package):
+    import ctypes
+
+    setup = Setup(package, [300, 77], [1, 1], seed=93)
+    q = setup.randn(2, 16, 256).cuda()
+    want = setup.cache.attention(1, setup.batch, q)
+    lib, provider = setup.cache.lib, package.provider
+    size, handle = ctypes.c_uint64(), ctypes.c_void_p()
+    config = provider.KvConfig.from_buffer_copy(setup.cache.config)
+    assert lib.aima_moe_kv_query_workspace(ctypes.byref(config), ctypes.byref(size)) == 0 and size.value == config.workspace_bytes
+    memory = torch.full((size.value + 256,), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    for pointer, given in ((memory.data_ptr(), size.value - 1), (memory.data_ptr() + 16, size.value),
+                           (torch.empty(64, dtype=torch.uint8).data_ptr() // 256 * 256, size.value)):
+        config.workspace, config.workspace_bytes = pointer, given
+        assert lib.aima_moe_kv_prepare(ctypes.byref(config), ctypes.byref(handle)) == -1 and not handle.value
+    for pointer, given in ((memory.data_ptr(), size.value), (None, 0)):          # the caller's, and one that prepare allocates
+        config.workspace, config.workspace_bytes = pointer, given
+        lib.check(lib.aima_moe_kv_prepare(ctypes.byref(config), ctypes.byref(handle)))
+        kept, setup.cache.handle = setup.cache.handle, handle
+        setup.cache.bind_layer(1, *setup.gpu)
+        out = setup.cache.attention(1, setup.batch, q)
+        setup.cache.sync()
+        setup.cache.handle = kept
+        assert torch.equal(out, want)
+        assert lib.aima_moe_kv_release(handle) == 0
+    assert (memory[size.value:] == 255).all()
 
 
 @pytest.mark.parametrize("new", [1, 40])
