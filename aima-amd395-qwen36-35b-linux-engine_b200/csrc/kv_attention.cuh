@@ -5,6 +5,8 @@
 #include "kv_cache.cuh"
 #include "tcgen05.cuh"
 
+#include <type_traits>
+
 namespace aima {
 
 constexpr int kKvTile = 128;            // positions of the cache per step
@@ -105,52 +107,67 @@ __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace&
     *reinterpret_cast<uint2*>(a.out + (static_cast<long long>(unit.row0 + token) * a.shape.q_heads + unit.head + g) * kDim + d) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
   };
-  constexpr int kFew = 8;
-  if (ok && unit.parts <= kFew) {
+  // kFew parts at most, kColumns results of a row under way together
+  auto by_rows = [&](auto few, auto columns) {
+    constexpr int kFew = decltype(few)::value, kColumns = decltype(columns)::value;
     const int at_once = kThreads / unit.rows, row = threadIdx.x % unit.rows;       // kThreads is at least a row tile's rows
     const int end = 4 * (kDim / 4 * (unit.mine + 1) / unit.parts);
     int d = 4 * (kDim / 4 * unit.mine / unit.parts + static_cast<int>(threadIdx.x) / unit.rows);
-    if (static_cast<int>(threadIdx.x) < at_once * unit.rows && d < end) {
-      float2 w[kFew];
-      float top = -INFINITY, sum = 0.0f;
+    if (static_cast<int>(threadIdx.x) >= at_once * unit.rows || d >= end) return;
+    float4 x[kColumns][kFew];
+    auto load = [&] {
 #pragma unroll
-      for (int p = 0; p < kFew; ++p) {
-        w[p] = make_float2(-INFINITY, 0.0f);
-        if (p < unit.parts) w[p] = __ldcg(kv_part_weight(work, kv_part_index(unit.first_block + p, p == 0), row));
-        top = fmaxf(top, w[p].x);
-      }
-      if (top == -INFINITY) top = 0.0f;                           // nothing seen, or nothing but NaN
-#pragma unroll
-      for (int p = 0; p < kFew; ++p) {
-        const float f = fast_exp2(w[p].x - top);
-        sum += w[p].x == -INFINITY ? w[p].y : w[p].y * f;
-        w[p].x = f;
-      }
-      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-      for (; d < end; d += 8 * at_once) {
-        const bool second = d + 4 * at_once < end;
-        float4 x[2][kFew];
+      for (int i = 0; i < kColumns; ++i) {
 #pragma unroll
         for (int p = 0; p < kFew; ++p) {
-          const size_t part = kv_part_index(unit.first_block + p, p == 0);
-          x[0][p] = x[1][p] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (p < unit.parts) x[0][p] = __ldcg(reinterpret_cast<const float4*>(kv_part_sum<kDim>(work, part, row, d)));
-          if (p < unit.parts && second) x[1][p] = __ldcg(reinterpret_cast<const float4*>(kv_part_sum<kDim>(work, part, row, d + 4 * at_once)));
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-          for (int p = 0; p < kFew; ++p) {
-            acc.x = fmaf(x[i][p].x, w[p].x, acc.x);
-            acc.y = fmaf(x[i][p].y, w[p].x, acc.y);
-            acc.z = fmaf(x[i][p].z, w[p].x, acc.z);
-            acc.w = fmaf(x[i][p].w, w[p].x, acc.w);
-          }
-          if (i == 0 || second) store(row, d + 4 * at_once * i, acc, inverse);
+          x[i][p] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (p < unit.parts && d + 4 * at_once * i < end)
+            x[i][p] = __ldcg(reinterpret_cast<const float4*>(kv_part_sum<kDim>(work, kv_part_index(unit.first_block + p, p == 0), row, d + 4 * at_once * i)));
         }
       }
+    };
+    float2 w[kFew];
+#pragma unroll
+    for (int p = 0; p < kFew; ++p) {
+      w[p] = make_float2(-INFINITY, 0.0f);
+      if (p < unit.parts) w[p] = __ldcg(kv_part_weight(work, kv_part_index(unit.first_block + p, p == 0), row));
     }
+    load();
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kFew; ++p) top = fmaxf(top, w[p].x);
+    if (top == -INFINITY) top = 0.0f;                             // nothing seen, or nothing but NaN
+#pragma unroll
+    for (int p = 0; p < kFew; ++p) {
+      const float f = fast_exp2(w[p].x - top);
+      sum += w[p].x == -INFINITY ? w[p].y : w[p].y * f;
+      w[p].x = f;
+    }
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll 1
+    for (;;) {
+#pragma unroll
+      for (int i = 0; i < kColumns; ++i) {
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int p = 0; p < kFew; ++p) {
+          acc.x = fmaf(x[i][p].x, w[p].x, acc.x);
+          acc.y = fmaf(x[i][p].y, w[p].x, acc.y);
+          acc.z = fmaf(x[i][p].z, w[p].x, acc.z);
+          acc.w = fmaf(x[i][p].w, w[p].x, acc.w);
+        }
+        if (d + 4 * at_once * i < end) store(row, d + 4 * at_once * i, acc, inverse);
+      }
+      d += 4 * kColumns * at_once;
+      if (d >= end) break;
+      load();
+    }
+  };
+  constexpr int kMost = 8;
+  if (ok && unit.parts <= 4) {
+    by_rows(std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
+  } else if (ok && unit.parts <= kMost) {
+    by_rows(std::integral_constant<int, kMost>(), std::integral_constant<int, 2>());
   } else if (ok) {
     int lanes = 4;
     while (lanes < 32 && 4 * lanes < unit.parts) lanes *= 2;
