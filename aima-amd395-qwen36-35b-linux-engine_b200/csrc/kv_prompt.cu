@@ -135,6 +135,19 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// two FP32 operations per instruction
+__device__ __forceinline__ unsigned long long both(float2 x) { return __float_as_uint(x.x) | (static_cast<unsigned long long>(__float_as_uint(x.y)) << 32); }
+__device__ __forceinline__ float2 both(unsigned long long x) { return make_float2(__uint_as_float(static_cast<uint32_t>(x)), __uint_as_float(static_cast<uint32_t>(x >> 32))); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(both(a)), "l"(both(b)), "l"(both(c)));
+  return both(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(both(a)), "l"(both(b)));
+  return both(r);
+}
 // row / group for rows below 128, with inverse = ceil(2^16 / group)
 __device__ __forceinline__ int row_token(int row, int inverse) { return (row * inverse) >> 16; }
 __device__ __forceinline__ void group_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -610,12 +623,16 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
       const float row_scale = row < rows ? sm.row_scale[row] : 0.0f;
       const int limit = row < rows ? walk.unit.first + row_token(row, group_inverse) : -1;     // last position the row sees
       float top = -INFINITY, peak = -INFINITY, sum = 0.0f;       // reference and maximum so far; this half's sum of weights
+      float shift = kWeightExponent;                             // less the reference
       for (int j = 0; j < n; ++j, ++tile) {
         const int buffer = tile & 1, slot = tile % kScaleSlots;
         const int position0 = (walk.tile0 + j) * kKvTile;
         const uint32_t scores = tmem + lanes + L::kScoreColumn + buffer * 128;
-        wait(&sm.scales_full[slot], (tile / kScaleSlots) & 1);
-        wait(&sm.s_full[buffer], (tile >> 1) & 1);
+        // both at once: even a wait that has ended takes 85 cycles to say so
+        const bool scales_there = mbar_test(smem_u32(&sm.scales_full[slot]), (tile / kScaleSlots) & 1);
+        const bool scores_there = mbar_test(smem_u32(&sm.s_full[buffer]), (tile >> 1) & 1);
+        if (!__all_sync(0xffffffffu, scores_there)) wait(&sm.s_full[buffer], (tile >> 1) & 1);
+        if (!__all_sync(0xffffffffu, scales_there)) wait(&sm.scales_full[slot], (tile / kScaleSlots) & 1);
         tc_fence_after();
         const uint32_t half = 64 * group;
         uint32_t s[64];
@@ -660,29 +677,29 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
         asm volatile("bar.sync %0, 64;" :: "r"(2 + quarter) : "memory");
         m = fmaxf(m, sm.half_top[buffer][group ^ 1][row]);
         peak = fmaxf(peak, m);
-        float now = top;
-        if (m > top + kGrow || (top == -INFINITY && m > top)) now = m;
-        else if (m > -INFINITY && fmaxf(m, peak - kDepth) < top - kFall) now = fmaxf(m, peak - kDepth);
-        if (j > 0 && __any_sync(0xffffffffu, now != top)) {
-          wait(&sm.o_done[buffer ^ 1], ((tile - 1) >> 1) & 1);
-          tc_fence_after();
-          const float f = now != top ? fast_exp2(top - now) : 1.0f;
-          const uint32_t sums = tmem + lanes + group * (kDim / 2);
+        const bool falls = m > -INFINITY && fmaxf(m, peak - kDepth) < top - kFall;
+        const bool moves = m > top + kGrow || falls;               // the first that is seen is above -inf
+        if (__any_sync(0xffffffffu, moves)) {
+          const float now = falls ? fmaxf(m, peak - kDepth) : moves ? m : top;
+          const float f = moves ? fast_exp2(top - now) : 1.0f;     // top is -inf at first: 0
+          if (j > 0) {
+            wait(&sm.o_done[buffer ^ 1], ((tile - 1) >> 1) & 1);
+            tc_fence_after();
+            const uint32_t sums = tmem + lanes + group * (kDim / 2);
 #pragma unroll 1
-          for (int c = 0; c < kDim / 2; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(sums + c, o);
-            tmem_ld_wait();
+            for (int c = 0; c < kDim / 2; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(sums + c, o);
+              tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st32(sums + c, o);
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st32(sums + c, o);
+            }
           }
-        }
-        if (now != top) {
-          sum *= fast_exp2(top - now);     // top is -inf at first: 0
+          sum *= f;
           top = now;
+          shift = kWeightExponent - (top == -INFINITY ? 0.0f : top);
         }
-        const float shift = kWeightExponent - (now == -INFINITY ? 0.0f : now);
 #pragma unroll
         for (int chunk = 0; chunk < 2; ++chunk) {
           uint32_t terms[24];
@@ -690,18 +707,21 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
           for (int g = 0; g < 2; ++g) {
             const int at = half / 16 + 2 * chunk + g;
             const float factor = factor_of(at), offset = scales[at].y + shift;
-            float part = 0.0f;
+            float2 part = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int c = 0; c < 16; c += 4) {
               float w[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                w[i] = fast_exp2(fmaf(__uint_as_float(s[32 * chunk + 16 * g + c + i]), factor, offset));
-                part += w[i];
+              for (int i = 0; i < 4; i += 2) {
+                const uint32_t* x = s + 32 * chunk + 16 * g + c + i;
+                const float2 t = fma2(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), make_float2(factor, factor), make_float2(offset, offset));
+                w[i] = fast_exp2(t.x);
+                w[i + 1] = fast_exp2(t.y);
+                part = add2(part, make_float2(w[i], w[i + 1]));
               }
               split_weights(cvt_f16x2(w[0], w[1]), cvt_f16x2(w[2], w[3]), terms + 4 * g + c / 4, 8);
             }
-            sum = fmaf(part, scales[at].z, sum);
+            sum = fmaf(part.x + part.y, scales[at].z, sum);
           }
           // where the scores of these 32 positions lay
 #pragma unroll
