@@ -11,8 +11,10 @@ namespace aima {
 namespace {
 
 constexpr int kVerifyThreads = 512;
-constexpr int kAhead = 4;                      // steps whose loads are under way together
-constexpr uint32_t kSplitVocabulary = 16384;   // more than four steps per warp of one block: a cluster of eight
+constexpr int kAhead = 4;                      // steps of a warp whose loads are under way together
+constexpr uint32_t kWholeVocabulary = 4096;    // up to here one block per sequence
+constexpr uint32_t kResident = 256;            // blocks of the launch that run at once
+constexpr uint32_t kLongRun = 32768;           // tokens of a block that are worth a cluster whatever runs beside it
 
 // floor(2^40 w) of w clamped to [0, 1]; NaN counts as 0
 __device__ __forceinline__ unsigned long long whole(float w) {
@@ -76,6 +78,10 @@ __device__ __forceinline__ void store_u64_in_block(unsigned long long* local, ui
   asm volatile("st.shared::cluster.u64 [%0], %1;" :: "r"(remote), "l"(value) : "memory");
 }
 
+// Bound: reading one row (or a row of each) once, 8 bytes per token of the vocabulary with draft probabilities, and for few
+// sequences the chain of dependent loads: draft, its probabilities, the row, the found run again.  32 sequences of 248320 (64 MB):
+// 16.0 us with the rows in L2, 20.6 us from memory (3.1 TB/s); 148 sequences (294 MB) 63 us (4.7 TB/s); 1 sequence 8.3 us.  The
+// loads of four steps are issued together: with one step at a time 17.8 and 10.1 us.
 // A cluster of kBlocks per sequence.  The vocabulary is cut into one run of whole 128-token steps per warp; each warp sums its
 // run (a float4 per lane and step), the blocks exchange their sums through each other's shared memory, and the warp whose run
 // holds the token goes through it a second time.
@@ -234,9 +240,17 @@ cudaError_t launch(const aima_moe_verify_drafts& call, cudaStream_t stream) {
 cudaError_t verify_drafts(const aima_moe_verify_drafts& call, cudaStream_t stream) {
   const bool aligned = reinterpret_cast<uintptr_t>(call.target) % 16 == 0 && call.target_sequence_stride % 4 == 0 && call.target_row_stride % 4 == 0 &&
                        reinterpret_cast<uintptr_t>(call.draft) % 16 == 0 && call.draft_sequence_stride % 4 == 0 && call.draft_row_stride % 4 == 0;
-  const bool split = call.vocabulary > kSplitVocabulary;
-  if (split) return aligned ? launch<8, true>(call, stream) : launch<8, false>(call, stream);
-  return aligned ? launch<1, true>(call, stream) : launch<1, false>(call, stream);
+  // As many blocks per sequence as run at once.  us with 1 / 2 / 4 / 8 blocks, vocabulary 4096: 1 sequence 3.5 / 3.9 / 3.7 / 3.8;
+  // 32768: 8 sequences 10.1 / 7.9 / 5.7 / 4.9, 64 10.6 / 8.6 / 6.9 / 10.3, 300 18.2 / 19.7 / 24.7 / 44.3; 131072: 8 sequences
+  // 33 / 18 / 12 / 8.0, 148 58 / 37 / 35 / 38.
+  uint32_t blocks = call.vocabulary <= kWholeVocabulary ? 1 : 8;
+  while (blocks > 1 && call.sequences * blocks > kResident && call.vocabulary / blocks < kLongRun) blocks /= 2;
+  switch (blocks) {
+    case 8: return aligned ? launch<8, true>(call, stream) : launch<8, false>(call, stream);
+    case 4: return aligned ? launch<4, true>(call, stream) : launch<4, false>(call, stream);
+    case 2: return aligned ? launch<2, true>(call, stream) : launch<2, false>(call, stream);
+    default: return aligned ? launch<1, true>(call, stream) : launch<1, false>(call, stream);
+  }
 }
 
 }  // namespace aima

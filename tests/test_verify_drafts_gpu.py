@@ -45,6 +45,13 @@ def test_verify(package, sequences, drafts, vocabulary, probabilities):
         assert len(set(want)) > 1                                 # some accepted, some rejected
 
 
+@pytest.mark.parametrize("sequences,drafts,vocabulary", [(33, 2, 8191), (64, 2, 20000), (100, 2, 33001), (150, 2, 5000), (70, 1, 140000)])
+def test_verify_of_many_sequences(package, sequences, drafts, vocabulary):
+    """Eight, four, two and one block per sequence."""
+    target, draft, tokens, uniforms, _ = _case(sequences, drafts, vocabulary, seed=sequences, sharp=4.0)
+    _check(package, target, tokens, uniforms, draft)
+
+
 def test_every_draft_accepted_and_none(package):
     target, draft, tokens, uniforms, _ = _case(4, 3, 501, seed=2)
     uniforms[:, :3] = 0.0
