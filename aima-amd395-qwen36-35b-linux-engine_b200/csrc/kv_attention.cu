@@ -7,9 +7,9 @@
 namespace aima {
 namespace {
 
-// Up to here the few-row kernel: 16 sequences x 24 rows of 8000 positions 78 us with it and 64 us with the prompt kernel, 64 x 32
-// rows of 4000 142 and 87, 16 x 40 rows of 4111 138 and 62; at 8 and 16 rows it streams the cache and the prompt kernel would wait
-// for its products.
+// Up to here the few-row kernel.  us with it and with the prompt kernel: 8 rows, one sequence of 32768 positions 15.1 and 22.6, 64
+// of up to 8192 78 and 107; 16 rows, 64 of up to 8192 96 and 123, with heads of 128 278 and 274.  In a form that took 40 rows it
+// needed 138 for 16 sequences of 4111, where the prompt kernel needs 27.
 constexpr int kDecodeRows = 16;
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

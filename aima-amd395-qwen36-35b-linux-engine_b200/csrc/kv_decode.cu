@@ -18,6 +18,9 @@
 // issues the products, warps 2 and 3 prepare the queries of the next unit, warps 4-7 (thread = position) do the softmax and
 // write the results.  S is double-buffered: the product of the next tile runs under the softmax of this one.  The running
 // maximum moves only when a tile's exceeds it by more than kGrow, so the accumulators are rarely rescaled.
+//
+// Measured: 64 sequences of up to 8192 positions, one token, 16/2 heads of 256 (406 MB) 77.7 us = 5.2 TB/s, 80 % of a copy; one sequence
+// of 32768 14.9 us, of which the tiles are 3 and the rest is a chain: cuts, queries, first scores, results, join.
 #include "kv_attention.cuh"
 
 namespace aima {
@@ -622,6 +625,7 @@ cudaError_t launch(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t
 
 template <int kDim>
 cudaError_t launch_rows(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
+  // N of the products: 8 rows in the kernel for 16 take 18.6 us instead of 15.0 (one sequence of 32768), 90 instead of 78 (64 of 8192)
   return plan.tile_rows <= 8 ? launch<kDim, 8>(plan, maps, stream) : launch<kDim, 16>(plan, maps, stream);
 }
 

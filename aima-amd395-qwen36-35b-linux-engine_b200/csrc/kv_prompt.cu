@@ -7,7 +7,7 @@
 //
 // Bound: the products, 4 x rows x positions x head_dim flops at the rate of 16-bit ones.  Queries and weights are BF16-like, the
 // cache is e4m3, and no operand of mixed width exists; unpacking K and V would cost conversions and shared memory per tile,
-// so Q and the weights are split into two 8-bit terms instead and the products run twice at twice the rate:
+// so Q is split into two 8-bit terms and the weights into three, and the products run twice and three times at twice the rate:
 //   q 2^-e  = hi (e4m3) + lo (e5m2)          exact down to 2^-16 (largest 448)
 //   w 2^9   = three terms (e5m2)             to 2^-8 of itself where it exceeds 2^-9 (2^-18 of the largest), to 2^-17 below
 // An e5m2 number is the upper byte of an f16, so the weights' terms take no conversions; two terms with an e4m3 first one would
@@ -19,6 +19,12 @@
 // One block per SM.  Warp 0 loads tiles by page, warp 1 issues the products, warp 3 fetches the scales; warps 4-7 and 8-11 (thread =
 // row) each turn half of a tile's scores into weights; two warps with the same rows exchange their maxima in between.
 // The scores are double-buffered: the products of one tile run under the softmax of another.
+//
+// Measured: 8192 tokens of 32768 with 16/2 heads of 256 3.68 ms = 1.04 PFLOP/s at the 1.5 GHz that the power cap leaves, 2560 cycles
+// of products in the 3250 of a tile: both operands of Q K^T come from shared memory at its full rate while the next tiles are
+// written there.  With heads of 128 a tile takes 2440 cycles, which its softmax needs (27 instructions per four weights on two
+// warps per scheduler), the products 1400: 7 prompts of 1531 .. 2999 with 32/8 heads 390 us.  1024 tokens alone 27 us, most of it
+// before the first tile and after the last.
 #include "kv_attention.cuh"
 
 namespace aima {
