@@ -141,6 +141,9 @@ class VerifyDrafts(ctypes.Structure):
     ]
 
 
+_VERIFY_BYTES = ctypes.sizeof(VerifyDrafts)
+
+
 # every symbol include/aima_moe.h declares: (name, restype, argtypes)
 EXPORTS = [
     ("aima_moe_abi_version", c_uint32, []),
@@ -268,11 +271,6 @@ def _nbytes(tensor: Any) -> int:
 
 def _stream(torch: Any) -> c_void_p:
     return c_void_p(int(torch.cuda.current_stream().cuda_stream))
-
-
-def _raw_stream(torch: Any) -> int:
-    """The current stream's handle without a Stream object, which takes 3 us to build: as long as the launch itself."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 # reference weight-dict keys (four_layer_mini_engine.py: weights["router"],
@@ -731,7 +729,10 @@ class KvBatch:
             if tensor is not None and (tensor.dtype != torch.int32 or (tensor.dim() != 2 if shape is None else tuple(tensor.shape) != shape)):
                 raise ValueError(f"{name} must be int32 {'[sequences, columns]' if shape is None else list(shape)}, got "
                                  f"{tensor.dtype} {list(tensor.shape)}")
+            if tensor is not None and tensor.get_device() != page_table.get_device():
+                raise ValueError(f"{name} and page_table are on different devices")
         self.page_table, self.lengths, self.row_offsets = page_table, lengths, row_offsets
+        self.device = page_table.get_device()
         self.tokens = tokens
         self.struct = KvBatchStruct(ctypes.sizeof(KvBatchStruct), int(page_table.shape[0]), tokens, max_new_tokens, int(page_table.shape[1]), 0,
                                     _ptr(page_table), _ptr(row_offsets), _ptr(lengths))
@@ -751,6 +752,7 @@ class KvCache:
         if not torch.cuda.is_available():
             raise RuntimeError("aima_moe needs a CUDA device (sm_100a); there is no CPU fallback")
         self._torch = torch
+        self._device = torch.cuda.current_device()
         self.lib = library or load_library()
         self.config = KvConfig(ctypes.sizeof(KvConfig), q_heads, kv_heads, head_dim, rotary_dim, page_tokens, pages, layers, max_sequences,
                                softmax_scale, None, 0)
@@ -805,21 +807,23 @@ class KvCache:
     # -- launches ------------------------------------------------------------
     def _rows(self, tensor: Any, name: str, shape: tuple[int, int, int]) -> KvRows:
         row_stride, head_stride, stride = tensor.stride() if tensor.dim() == 3 else (0, 0, 0)
-        if tensor.dtype is not self._torch.bfloat16 or not tensor.is_cuda or tensor.shape != shape or stride != 1:
-            raise ValueError(f"{name} must be a CUDA bfloat16 tensor {list(shape)} with contiguous heads, got "
-                             f"{tensor.dtype} {list(tensor.shape)} with strides {list(tensor.stride())}")
+        if tensor.dtype is not self._torch.bfloat16 or tensor.get_device() != self._device or tensor.shape != shape or stride != 1:
+            raise ValueError(f"{name} must be a bfloat16 tensor {list(shape)} with contiguous heads of the handle's device, got "
+                             f"{tensor.dtype} {list(tensor.shape)} with strides {list(tensor.stride())} on {tensor.device}")
         return KvRows(tensor.data_ptr(), row_stride, head_stride)
 
     def _out(self, out: Any, q: Any, name: str) -> Any:
         if out is None:
             return self._torch.empty_like(q, memory_format=self._torch.contiguous_format)
-        if out.dtype is not self._torch.bfloat16 or not out.is_cuda or out.shape != q.shape or not out.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous CUDA bfloat16 tensor {list(q.shape)}")
+        if out.dtype is not self._torch.bfloat16 or out.get_device() != self._device or out.shape != q.shape or not out.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous bfloat16 tensor {list(q.shape)} of the handle's device")
         return out
 
     def append(self, layer: int, batch: KvBatch, k: Any, v: Any, q: Any = None, q_out: Any = None) -> Any:
         """Rotates k and stores it and v; with q returns the rotated queries [tokens, q_heads, head_dim].  k, v and q may be views
         into one row of a fused projection."""
+        if batch.device != self._device:
+            self._refuse_device(batch)
         kv_shape = (batch.tokens, *self._kv_shape)
         k_rows, v_rows = self._rows(k, "k", kv_shape), self._rows(v, "v", kv_shape)
         q_rows = None
@@ -832,13 +836,18 @@ class KvCache:
 
     def attention(self, layer: int, batch: KvBatch, q: Any, out: Any = None) -> Any:
         """Causal attention of the batch's rows over the cache (after append): [tokens, q_heads, head_dim]."""
+        if batch.device != self._device:
+            self._refuse_device(batch)
         q_rows = self._rows(q, "q", (batch.tokens, *self._q_shape))
         out = self._out(out, q, "out")
         self.lib.check(self.lib.aima_moe_kv_attention_launch(self.handle, layer, batch.ref, q_rows, out.data_ptr(), self._stream()))
         return out
 
+    def _refuse_device(self, batch: KvBatch) -> None:
+        raise ValueError(f"the batch's tensors are of device {batch.device}, the handle is of {self._device}")
+
     def _stream(self) -> int:
-        stream = _raw_stream(self._torch)
+        stream = self._torch._C._cuda_getCurrentRawStream(self._device)
         self._streams.add(stream)
         return stream
 
@@ -876,33 +885,53 @@ def verify_drafts(target: Any, draft_tokens: Any, uniforms: Any, draft_probabili
     if target.dim() != 3:
         raise ValueError("target must be [sequences, drafts + 1, vocabulary]")
     sequences, rows, vocabulary = target.shape
-    drafts = (sequences, rows - 1)
-
-    def check(name: str, tensor: Any, dtype: Any, shape: tuple) -> None:
-        if tensor.dtype is not dtype or tensor.shape != shape or not tensor.is_cuda:
-            raise ValueError(f"{name} must be a CUDA {dtype} tensor {list(shape)}, got {tensor.dtype} {list(tensor.shape)}")
-
-    check("target", target, torch.float32, target.shape)
-    check("draft_tokens", draft_tokens, torch.int32, drafts)
-    check("uniforms", uniforms, torch.float32, (sequences, rows))
-    if draft_probabilities is not None:
-        check("draft_probabilities", draft_probabilities, torch.float32, (*drafts, vocabulary))
-    for name, tensor in (("draft_counts", draft_counts), ("cache_lengths", cache_lengths)):
-        if tensor is not None:
-            check(name, tensor, torch.int32, (sequences,))
-    for name, tensor in (("target", target), ("draft_probabilities", draft_probabilities)):
-        if tensor is not None and vocabulary > 1 and tensor.stride(2) != 1:
-            raise ValueError(f"rows of {name} must be contiguous")
-    # accepted, tokens and lengths in one allocation
-    out = torch.empty_strided((sequences * (rows + 2),), (1,), dtype=torch.int32, device=target.device)
-    accepted = out.as_strided((sequences,), (1,), 0)
-    tokens = out.as_strided((sequences, rows), (rows, 1), sequences)
-    new_lengths = None if cache_lengths is None else out.as_strided((sequences,), (1,), sequences * (rows + 1))
-    has_draft = draft_probabilities is not None
+    int32, device, drafts = torch.int32, target.get_device(), draft_probabilities
+    has_draft, has_counts, has_lengths = drafts is not None, draft_counts is not None, cache_lengths is not None
+    # in one expression: the call on the host takes longer than the kernel
+    if not (device == torch._C._cuda_getDevice() and target.dtype is torch.float32
+            and draft_tokens.dtype is int32 and draft_tokens.shape == (sequences, rows - 1) and draft_tokens.get_device() == device
+            and draft_tokens.is_contiguous()
+            and uniforms.dtype is torch.float32 and uniforms.shape == (sequences, rows) and uniforms.get_device() == device
+            and uniforms.is_contiguous()
+            and (not has_draft or (drafts.dtype is torch.float32 and drafts.shape == (sequences, rows - 1, vocabulary)
+                                   and drafts.get_device() == device))
+            and (not has_counts or (draft_counts.dtype is int32 and draft_counts.shape == (sequences,) and draft_counts.get_device() == device
+                                    and draft_counts.is_contiguous()))
+            and (not has_lengths or (cache_lengths.dtype is int32 and cache_lengths.shape == (sequences,)
+                                     and cache_lengths.get_device() == device and cache_lengths.is_contiguous()))):
+        _refuse_verification(target, draft_tokens, uniforms, drafts, draft_counts, cache_lengths)
+    target_strides = target.stride()
+    draft_strides = drafts.stride() if has_draft else (0, 0, 1)
+    if vocabulary > 1 and (target_strides[2] != 1 or draft_strides[2] != 1):
+        raise ValueError("rows of target and draft_probabilities must be contiguous")
+    accepted = torch.empty_like(cache_lengths) if has_lengths else draft_tokens.new_empty((sequences,))
+    new_lengths = torch.empty_like(cache_lengths) if has_lengths else None
+    tokens = torch.empty_like(uniforms, dtype=int32)
     call = VerifyDrafts(
-        ctypes.sizeof(VerifyDrafts), sequences, rows - 1, vocabulary, target.data_ptr(), target.stride(0), target.stride(1),
-        draft_probabilities.data_ptr() if has_draft else None, draft_probabilities.stride(0) if has_draft else 0,
-        draft_probabilities.stride(1) if has_draft else 0, _ptr(draft_tokens), _ptr(draft_counts), _ptr(uniforms), _ptr(cache_lengths),
-        accepted.data_ptr(), tokens.data_ptr(), None if new_lengths is None else new_lengths.data_ptr())
-    lib.check(lib.aima_moe_verify_drafts_launch(call, _raw_stream(torch)))
-    return (accepted, tokens) if new_lengths is None else (accepted, tokens, new_lengths)
+        _VERIFY_BYTES, sequences, rows - 1, vocabulary, target.data_ptr(), target_strides[0], target_strides[1],
+        drafts.data_ptr() if has_draft else None, draft_strides[0], draft_strides[1], draft_tokens.data_ptr(),
+        draft_counts.data_ptr() if has_counts else None, uniforms.data_ptr(), cache_lengths.data_ptr() if has_lengths else None,
+        accepted.data_ptr(), tokens.data_ptr(), new_lengths.data_ptr() if has_lengths else None)
+    lib.check(lib.aima_moe_verify_drafts_launch(call, torch._C._cuda_getCurrentRawStream(device)))
+    return (accepted, tokens, new_lengths) if has_lengths else (accepted, tokens)
+
+
+def _refuse_verification(target: Any, draft_tokens: Any, uniforms: Any, draft_probabilities: Any, draft_counts: Any, cache_lengths: Any) -> None:
+    """Says which of verify_drafts' tensors is not what it has to be."""
+    import torch
+
+    sequences, rows, vocabulary = target.shape
+    device = torch.cuda.current_device()
+    for name, tensor, dtype, shape in (
+            ("target", target, torch.float32, target.shape), ("draft_tokens", draft_tokens, torch.int32, (sequences, rows - 1)),
+            ("uniforms", uniforms, torch.float32, (sequences, rows)),
+            ("draft_probabilities", draft_probabilities, torch.float32, (sequences, rows - 1, vocabulary)),
+            ("draft_counts", draft_counts, torch.int32, (sequences,)), ("cache_lengths", cache_lengths, torch.int32, (sequences,))):
+        if tensor is None:
+            continue
+        if tensor.dtype is not dtype or tensor.shape != shape or tensor.get_device() != device:
+            raise ValueError(f"{name} must be a {dtype} tensor {list(shape)} of the current CUDA device, got {tensor.dtype} {list(tensor.shape)} "
+                             f"on {tensor.device}")
+        if name not in ("target", "draft_probabilities") and not tensor.is_contiguous():
+            raise RuntimeError("aima_moe tensors must be contiguous CUDA tensors")
+    raise ValueError("verify_drafts: arguments are not what they have to be")
