@@ -16,11 +16,10 @@
 namespace aima {
 namespace {
 
-constexpr int kHeadsPerThread = 8;                  // query heads of a row that share its angles: 8192 tokens 35.8 us, with four 37.6
+constexpr int kHeadsPerThread = 8;                  // query heads of a row that share its angles; with four 8192 tokens took 1.8 us more
 constexpr long long kApartElements = 1 << 21;       // of queries: more are rotated by a kernel of their own
 constexpr int kRotateThreads = 256;
-// A thread of the page blocks keeps up to four vectors of keys and four of values.  (Eight: one token 5.8 us instead of 3.9, 8192
-// tokens 37.3 instead of 35.8.)
+// A thread of the page blocks has up to four vectors of keys and four of values under way.  (Eight: one token 5.8 us instead of 3.9.)
 template <int kDim, int kPage>
 constexpr int append_threads = kPage * kDim < 256 * 32 ? 256 : kPage * kDim / 32;
 
@@ -59,6 +58,13 @@ __device__ __forceinline__ uint2 codes8(const float* x, float inverse) {
 __device__ __forceinline__ int exponent_of(float scale) {
   const int bits = __float_as_int(scale);
   return min(max(((bits >> 23) & 255) - 127 + ((bits & 0x7fffff) != 0 ? 1 : 0), kKvMinExponent), kKvMaxExponent);
+}
+
+// A vector that this thread has read before; the compiler would keep the first one in registers.
+__device__ __forceinline__ uint4 load_again(const void* from) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(from));
+  return v;
 }
 
 // The eight angles of a vector of the rotated part: cosines and sines of one position.
@@ -148,13 +154,15 @@ __device__ __forceinline__ void rotate_queries(const KvAppend& a, long long bloc
   }
 }
 
-// One block per (sequence, touched page, head), then blocks for the queries.  A page and head belongs to one block, which
-// holds all of its new rows in registers between finding the scale and writing the codes: every byte is read once.
+// One block per (sequence, touched page, head), then blocks for the queries.  A page and head belongs to one block, which goes
+// through its new rows twice: for the largest magnitudes, and, with the scale, for the codes.  The second time they come from
+// the caches: held in registers they would leave room for one block per SM (8192 tokens 35.8 us instead of 33.4, with 32/8 heads of
+// 128 50.7 instead of 45.7; one token 3.9 instead of 4.2).
 //
-// Bound: bytes.  8192 tokens with 16/2 heads of 256 read 84 MB and write 75 MB; 36 us are 4.4 TB/s (the queries' stream, 134 MB, alone
-// 27 us).  One token is bound by its launch and three dependent loads (length, page, rows): 3.8 us.
+// Bound: bytes.  8192 tokens with 16/2 heads of 256 read 84 MB and write 75 MB; 33.4 us are 4.8 TB/s (the queries' stream, 134 MB, alone
+// 27 us).  One token is bound by its launch and three dependent loads (length, page, rows).
 template <int kDim, int kPage>
-__global__ void __launch_bounds__(append_threads<kDim, kPage>, append_threads<kDim, kPage> > 512 ? 1 : 512 / append_threads<kDim, kPage>)
+__global__ void __launch_bounds__(append_threads<kDim, kPage>, append_threads<kDim, kPage> > 512 ? 1 : 1024 / append_threads<kDim, kPage>)
 kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
   constexpr int kAppendThreads = append_threads<kDim, kPage>;
   constexpr int kPieces = kDim / 8;                                   // 16-byte vectors of a head
@@ -252,10 +260,16 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
       const int slot = slot0 + p * kRowsPerPass, position = page_start + slot;
       const bool active = position >= low && position < high;
       float k[8], v[8];
+      uint4 kagain = make_uint4(0, 0, 0, 0), vagain = kagain;
+      if (active) {
+        const long long row = first_row + position;
+        kagain = load_again(a.k.data + row * a.k.row_stride + head * a.k.head_stride + 8 * piece);
+        vagain = load_again(a.v.data + row * a.v.row_stride + head * a.v.head_stride + 8 * piece);
+      }
       Angles angles{};
       if (active && piece < 2 * half) angles = load_angles(a.rotation + static_cast<size_t>(position) * shape.rotary, piece, half);
-      rotate8<kDim>(kraw[p], piece, half, angles, active, k);
-      unpack8(vraw[p], v);
+      rotate8<kDim>(kagain, piece, half, angles, active, k);
+      unpack8(vagain, v);
       if (active) {
         uint2 kc = codes8(k, kinv), vc = codes8(v, vinv);
         if ((poisoned >> p) & 1u) {
@@ -301,7 +315,7 @@ cudaError_t launch(const KvAppend& a, cudaStream_t stream) {
   const long long query_work = a.q.data != nullptr ? static_cast<long long>(a.batch.tokens) * ((a.shape.q_heads + kHeadsPerThread - 1) / kHeadsPerThread) : 0;
   // Few queries are rotated by blocks of the same launch.  Many are a stream of their own beside the page blocks, whose registers
   // would leave too few of the stream's bytes in flight.  us together / apart, 16 heads of 256: 256 tokens 5.7 / 6.3, 512 6.0 / 6.4,
-  // 1024 8.0 / 6.5, 8192 43 / 36.
+  // 1024 8.0 / 6.5, 8192 43 / 33.
   const bool apart = query_work * kHeadsPerThread * kDim > kApartElements;
   const long long query_blocks = apart ? 0 : (query_work + kAppendThreads / (kDim / 8) - 1) / (kAppendThreads / (kDim / 8));
   const long long rotate_blocks = (query_work + kRotateThreads / (kDim / 8) - 1) / (kRotateThreads / (kDim / 8));
