@@ -6,13 +6,17 @@
 // share a key/value head, so that K and V are loaded once for all of them.
 //
 // Bound: the products, 4 x rows x positions x head_dim flops at the rate of 16-bit ones.  Queries and weights are BF16-like, the
-// cache is e4m3, and no operand of mixed width exists; unpacking K and V would cost conversions and shared memory per tile,
-// so Q is split into two 8-bit terms and the weights into three, and the products run twice and three times at twice the rate:
+// cache is e4m3, and no operand of mixed width exists.  So Q is split into two 8-bit terms and its product runs twice at twice the rate:
 //   q 2^-e  = hi (e4m3) + lo (e5m2)          exact down to 2^-16 (largest 448)
+// Weights and values, heads of 256:
 //   w 2^9   = three terms (e5m2)             to 2^-8 of itself where it exceeds 2^-9 (2^-18 of the largest), to 2^-17 below
 // An e5m2 number is the upper byte of an f16, so the weights' terms take no conversions; two terms with an e4m3 first one would
 // take a fifth less of the tensor cores but hold weights below 2^-13 of the largest to a few bits only, which is not enough where
-// one position outweighs all others and brings nothing.
+// one position outweighs all others and brings nothing.  Heads of 64 and 128 (kWide), whose softmax takes longer than their products:
+//   w 2^9   = one f16                        to 2^-11 of itself down to 2^-23 of the largest
+// with V's codes as f16, which they are exactly, in a second pair of buffers (heads of 256 would need 128 KB for them).  That saves the
+// softmax 13 of 23 instructions per four weights and the tensor cores a third of the second product; the softmax warps widen V on
+// the way.  4096 tokens of 16384 with 32/8 heads of 128 1235 us in three terms and 1125 this way, with 8/8 of 64 275 and 247.
 // All terms of an operand go into one accumulator.  S[128 rows, 128 positions] = Q K^T with both operands in shared memory;
 // O[128, head_dim] += W V with W in tensor memory, where it takes the place of the scores it was made from, and V MN-major.
 //
@@ -22,9 +26,9 @@
 //
 // Measured: 8192 tokens of 32768 with 16/2 heads of 256 3.68 ms = 1.04 PFLOP/s at the 1.5 GHz that the power cap leaves, 2560 cycles
 // of products in the 3250 of a tile: both operands of Q K^T come from shared memory at its full rate while the next tiles are
-// written there.  With heads of 128 a tile takes 2440 cycles, which its softmax needs (27 instructions per four weights on two
-// warps per scheduler), the products 1400: 7 prompts of 1531 .. 2999 with 32/8 heads 390 us.  1024 tokens alone 27 us, most of it
-// before the first tile and after the last.
+// written there.  With heads of 128 a tile takes 2250 cycles, which its softmax needs (a chain of loads, maxima, an exchange and 64
+// weights per thread on two warps per scheduler), the products 1050: 7 prompts of 1531 .. 2999 with 32/8 heads 361 us.  1024
+// tokens of 16/2 heads of 256 alone 27 us, most of it before the first tile and after the last.
 #include "kv_attention.cuh"
 
 namespace aima {
@@ -47,9 +51,12 @@ struct Prompt {
   static constexpr int kPanels = kDim / kRowBytes;
   static constexpr int kPanelBytes = kKvTile * kRowBytes;
   static constexpr int kSlotBytes = kKvTile * kDim;
-  static constexpr int kSlots = kDim == 256 ? 4 : 8;
+  static constexpr bool kWide = kDim <= 128;                            // weights and values in 16 bits
+  static constexpr int kWideBytes = kWide ? kKvTile * kDim * 2 : 0;     // a tile of V, rows of 64 values per panel
+  static constexpr int kSlots = kDim == 256 ? 4 : kDim == 128 ? 6 : 8;
   static constexpr int kQueryAt = kSlots * kSlotBytes;                  // hi, then lo
-  static constexpr int kStageAt = kQueryAt + 2 * kSlotBytes;
+  static constexpr int kWideAt = kQueryAt + 2 * kSlotBytes;
+  static constexpr int kStageAt = kWideAt + 2 * kWideBytes;
   static constexpr int kSmallAt = kStageAt + 8 * kStageBytes;
   static constexpr int kScoreColumn = 256;                              // tensor memory: O | S0 | S1
 };
@@ -153,6 +160,31 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   unsigned long long r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(both(a)), "l"(both(b)));
   return both(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(both(a)), "l"(both(b)));
+  return both(r);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 2^t without the exponential unit: t = n + f with n whole and |f| <= 1/2, 2^f by the polynomial of degree 3 whose largest relative error
+// is the least (2^-13.7, found by exchange), 2^n put together from n + 127.  Below -127 it is 0, NaN stays NaN.  A quarter of the
+// exponentials of kWide go this way, whose unit would otherwise be busy for 1024 cycles of a tile: 4096 of 16384 with 32/8 heads
+// of 128 1192 -> 1150 us, with three eighths 1164, with half 1177; in the three-term form every one of them lost time.
+__device__ __forceinline__ float2 exp2_by_polynomial(float2 t) {
+  constexpr float kMagic = 12582912.0f + 127.0f;         // 1.5 * 2^23: the sum's low bits are n + 127
+  t.x = max_nan(t.x, -127.0f);
+  t.y = max_nan(t.y, -127.0f);
+  const float2 shifted = add2(t, make_float2(kMagic, kMagic));
+  const float2 f = add2(t, fma2(shifted, make_float2(-1.0f, -1.0f), make_float2(kMagic, kMagic)));
+  float2 p = fma2(f, make_float2(0.055171665f, 0.055171665f), make_float2(0.24261113f, 0.24261113f));
+  p = fma2(p, f, make_float2(0.69326097f, 0.69326097f));
+  p = fma2(p, f, make_float2(0.99992806f, 0.99992806f));
+  return mul2(p, make_float2(__uint_as_float(__float_as_uint(shifted.x) << 23), __uint_as_float(__float_as_uint(shifted.y) << 23)));
 }
 // row / group for rows below 128, with inverse = ceil(2^16 / group)
 __device__ __forceinline__ int row_token(int row, int inverse) { return (row * inverse) >> 16; }
@@ -371,6 +403,35 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
   auto ring_k = [](int first, int j) { return first + (j == 0 ? 0 : 2 * j - 1); };
   auto ring_v = [](int first, int j, int n) { return first + (j + 1 < n ? 2 * j + 2 : 2 * n - 1); };
 
+  // V of a tile from its codes to 16 bits, 16 rows by each of warps 4 .. 11.  Rows behind the sequence's end, where a page can hold
+  // anything, become zeros.
+  auto widen = [&](int slot, int buffer, int seen) {
+    constexpr int kPieces = kDim < 256 ? kDim / 16 : 8, kRowsAtOnce = 32 / kPieces, kSteps = 16 / kRowsAtOnce;    // of 16 codes; rows of a step
+    const uint8_t* from = generic + slot * L::kSlotBytes;
+    uint8_t* to = generic + L::kWideAt + buffer * L::kWideBytes;
+    const int piece = lane % kPieces, first = 16 * (warp - 4) + lane / kPieces;
+    const uint32_t order = piece >> 2, swap = 0u - order;                 // the upper half first, so that eight lanes write to all banks
+    uint4 codes[kSteps];
+#pragma unroll
+    for (int b = 0; b < kSteps; ++b) {
+      const int at = first + b * kRowsAtOnce;
+      codes[b] = *reinterpret_cast<const uint4*>(from + at * L::kRowBytes + ((piece ^ (L::kRowBytes == 128 ? at & 7 : (at >> 1) & 3)) << 4));
+    }
+#pragma unroll
+    for (int b = 0; b < kSteps; ++b) {
+      const int at = first + b * kRowsAtOnce;
+      const uint32_t there = at < seen ? 0xffffffffu : 0u;
+      uint4 c = make_uint4(codes[b].x & there, codes[b].y & there, codes[b].z & there, codes[b].w & there);
+      const uint32_t x = (c.x ^ c.z) & swap, y = (c.y ^ c.w) & swap;
+      c = make_uint4(c.x ^ x, c.y ^ y, c.z ^ x, c.w ^ y);
+      uint8_t* row_at = to + (piece >> 2) * (kKvTile * 128) + at * 128;
+      const uint32_t even = (((2 * (piece & 3)) ^ (at & 7)) ^ order) << 4;
+      *reinterpret_cast<uint4*>(row_at + even) = make_uint4(e4m3x2_f16x2(c.x), e4m3x2_f16x2(c.x >> 16), e4m3x2_f16x2(c.y), e4m3x2_f16x2(c.y >> 16));
+      *reinterpret_cast<uint4*>(row_at + (even ^ 16)) = make_uint4(e4m3x2_f16x2(c.z), e4m3x2_f16x2(c.z >> 16), e4m3x2_f16x2(c.w), e4m3x2_f16x2(c.w >> 16));
+    }
+    fence_async_proxy();
+  };
+
   if (warp < 4) {
     if (warp == 0) {
       // ------------------------------ loads ------------------------------
@@ -424,7 +485,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
       // ------------------------------ products ------------------------------
       constexpr uint32_t kScoresHigh = instr_desc_f8(kE4m3, kE4m3, 0, 0, 128, kKvTile);
       constexpr uint32_t kScoresLow = instr_desc_f8(kE5m2, kE4m3, 0, 0, 128, kKvTile);
-      constexpr uint32_t kSums = instr_desc_f8(kE5m2, kE4m3, 0, 1, 128, kDim);
+      constexpr uint32_t kSums = L::kWide ? instr_desc_f8(kF16, kF16, 0, 1, 128, kDim) : instr_desc_f8(kE5m2, kE4m3, 0, 1, 128, kDim);
       int ring = 0, tile = 0, segment = 0;
       bool alive = true;
       while (alive && walk.next()) {
@@ -458,9 +519,19 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
         for (int j = 0; j < n && alive; ++j) {
           if (j + 1 < n && !scores(j + 1)) { alive = false; break; }
           const int r = ring_v(ring, j, n), slot = r % L::kSlots, buffer = (tile + j) & 1;
-          if (!wait(&sm.p_full[buffer], ((tile + j) >> 1) & 1) || !wait(&sm.full[slot], (r / L::kSlots) & 1)) { alive = false; break; }
+          if (!wait(&sm.p_full[buffer], ((tile + j) >> 1) & 1) || (!L::kWide && !wait(&sm.full[slot], (r / L::kSlots) & 1))) { alive = false; break; }
           tc_fence_after();
-          if (elect_one()) {
+          if (L::kWide) {
+            if (lane == 0) mbar_arrive(smem_u32(&sm.empty[slot]));         // its codes have been read
+            __syncwarp();
+            if (elect_one()) {
+              const uint32_t v0 = base + L::kWideAt + buffer * L::kWideBytes, w0 = tmem + L::kScoreColumn + buffer * 128;
+#pragma unroll
+              for (int k = 0; k < kKvTile / 16; ++k)
+                umma_f16_ts(tmem, w0 + (k / 4) * 64 + (k % 4) * 8, smem_desc_rows<128>(v0 + k * 16 * 128, kKvTile * 128), kSums, (j | k) != 0);
+              umma_commit(smem_u32(&sm.o_done[buffer]));
+            }
+          } else if (elect_one()) {
             const uint32_t v0 = base + slot * L::kSlotBytes, w0 = tmem + L::kScoreColumn + buffer * 128;
 #pragma unroll
             for (int term = 0; term < 3; ++term) {
@@ -633,9 +704,17 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
         const int buffer = tile & 1, slot = tile % kScaleSlots;
         const int position0 = (walk.tile0 + j) * kKvTile;
         const uint32_t scores = tmem + lanes + L::kScoreColumn + buffer * 128;
-        // both at once: even a wait that has ended takes 85 cycles to say so
+        // all at once: even a wait that has ended takes 85 cycles to say so
         const bool scales_there = mbar_test(smem_u32(&sm.scales_full[slot]), (tile / kScaleSlots) & 1);
         const bool scores_there = mbar_test(smem_u32(&sm.s_full[buffer]), (tile >> 1) & 1);
+        if (L::kWide) {
+          const int r = ring_v(ring, j, n), ring_slot = r % L::kSlots;
+          const bool codes_there = mbar_test(smem_u32(&sm.full[ring_slot]), (r / L::kSlots) & 1);
+          const bool room = mbar_test(smem_u32(&sm.o_done[buffer]), ((tile >> 1) & 1) ^ 1);
+          if (!__all_sync(0xffffffffu, codes_there)) wait(&sm.full[ring_slot], (r / L::kSlots) & 1);
+          if (!__all_sync(0xffffffffu, room)) wait(&sm.o_done[buffer], ((tile >> 1) & 1) ^ 1);
+          widen(ring_slot, buffer, walk.seq.length - position0);
+        }
         if (!__all_sync(0xffffffffu, scores_there)) wait(&sm.s_full[buffer], (tile >> 1) & 1);
         if (!__all_sync(0xffffffffu, scales_there)) wait(&sm.scales_full[slot], (tile / kScaleSlots) & 1);
         tc_fence_after();
@@ -707,7 +786,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
         }
 #pragma unroll
         for (int chunk = 0; chunk < 2; ++chunk) {
-          uint32_t terms[24];
+          uint32_t terms[24];                 // kWide: 16 pairs of weights
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const int at = half / 16 + 2 * chunk + g;
@@ -720,22 +799,33 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
               for (int i = 0; i < 4; i += 2) {
                 const uint32_t* x = s + 32 * chunk + 16 * g + c + i;
                 const float2 t = fma2(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), make_float2(factor, factor), make_float2(offset, offset));
-                w[i] = fast_exp2(t.x);
-                w[i + 1] = fast_exp2(t.y);
+                if (L::kWide && i == 2 && c >= 8) {
+                  const float2 e = exp2_by_polynomial(t);
+                  w[i] = e.x;
+                  w[i + 1] = e.y;
+                } else {
+                  w[i] = fast_exp2(t.x);
+                  w[i + 1] = fast_exp2(t.y);
+                }
                 part = add2(part, make_float2(w[i], w[i + 1]));
               }
-              split_weights(cvt_f16x2(w[0], w[1]), cvt_f16x2(w[2], w[3]), terms + 4 * g + c / 4, 8);
+              if (L::kWide) {
+                terms[8 * g + c / 2] = cvt_f16x2(w[0], w[1]);
+                terms[8 * g + c / 2 + 1] = cvt_f16x2(w[2], w[3]);
+              } else {
+                split_weights(cvt_f16x2(w[0], w[1]), cvt_f16x2(w[2], w[3]), terms + 4 * g + c / 4, 8);
+              }
             }
             sum = fmaf(part.x + part.y, scales[at].z, sum);
           }
-          // where the scores of these 32 positions lay
+          // where the scores of these 32 positions lay (kWide: those of the half's first 32)
 #pragma unroll
-          for (int term = 0; term < 3; ++term) tmem_st8(scores + half + 32 * chunk + 8 * term, terms + 8 * term);
+          for (int term = 0; term < (L::kWide ? 2 : 3); ++term) tmem_st8(scores + half + (L::kWide ? 16 : 32) * chunk + 8 * term, terms + 8 * term);
         }
         tmem_st_wait();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sm.scales_empty[slot]));
-        if (position0 + kKvTile > walk.seq.length) {
+        if (!L::kWide && position0 + kKvTile > walk.seq.length) {
           // behind the sequence's end a page can hold anything, and zero weights do not stop a NaN
           const int r = ring_v(ring, j, n), ring_slot = r % L::kSlots;
           wait(&sm.full[ring_slot], (r / L::kSlots) & 1);

@@ -73,7 +73,7 @@ __device__ __forceinline__ uint64_t smem_desc_rows(uint32_t smem_addr, uint32_t 
   desc |= static_cast<uint64_t>(kRowBytes == 128 ? 2 : 4) << 61;
   return desc;
 }
-constexpr int kE4m3 = 0, kE5m2 = 1;
+constexpr int kE4m3 = 0, kE5m2 = 1, kF16 = 0;
 // D = F32, A and B 8-bit floating point of the given formats, each K-major or (1) MN-major
 __host__ __device__ constexpr uint32_t instr_desc_f8(int a_format, int b_format, int a_mn, int b_mn, int m, int n) {
   return (1u << 4) | (static_cast<uint32_t>(a_format) << 7) | (static_cast<uint32_t>(b_format) << 10) |
@@ -91,6 +91,14 @@ __device__ __forceinline__ void umma_f8_ts(uint32_t tmem_d, uint32_t tmem_a, uin
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}"
+      :: "r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// 16-bit operands, F32 = F16 . F16 with A in tensor memory: two elements of K in a column.  The instruction descriptor has the fields
+// of the 8-bit one, F16 is format 0.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       :: "r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
