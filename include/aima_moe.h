@@ -579,7 +579,8 @@ int aima_moe_kv_append_launch(aima_moe_kv* handle, uint32_t layer, const aima_mo
 /* Attention of the batch's rows over the cache, causal: the row at position p sees positions 0 .. p.
  * out (BF16 [tokens, q_heads, head_dim], contiguous) = softmax(softmax_scale q k^T) v; query head h reads key/value head
  * h / (q_heads / kv_heads).  Rows that see nothing are zero; rows of no sequence (behind the last offset) are not written.
- * Bytes of a page behind a sequence's length can hold anything.  out may not overlap q.  Calls of one handle share its
+ * Bytes of a page behind a sequence's length can hold anything; a value code before it is a number (append writes no NaN there).
+ * out may not overlap q.  Calls of one handle share its
  * workspace: issue them on one stream or order them with events. */
 int aima_moe_kv_attention_launch(aima_moe_kv* handle, uint32_t layer, const aima_moe_kv_batch* batch,
                                  const aima_moe_kv_rows* q, void* out, void* stream);

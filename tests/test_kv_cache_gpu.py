@@ -258,6 +258,62 @@ def test_attention_of_strided_queries(package, new):
     _check_attention(setup, wide[:, :, :256], wide.cuda()[:, :, :256])
 
 
+OTHER_HEADS = [(16, 2, 128), (24, 8, 128), (16, 2, 64), (8, 8, 64)]
+
+
+@pytest.mark.parametrize("new", [1, 40, 150])
+@pytest.mark.parametrize("heads", OTHER_HEADS)
+def test_scores_and_values_of_other_head_sizes(package, heads, new):
+    """Sharp scores, rising ones, a sink whose value is zero, NaN behind the sequences, and rows of every size."""
+    setup = Setup(package, [400, 129, 200], [new, min(new, 100), new], heads, 64, 0, seed=new + heads[2])
+    h, kv_heads, dim = heads
+    q = setup.randn(setup.tokens, h, dim, std=8.0)
+    for which in (0, 1):
+        raw = setup.gpu[which].view(torch.uint8)
+        for s, n in enumerate(setup.lengths):
+            raw[int(setup.table[s, (n - 1) // 64]), :, n % 64 or 64:] = 0x7F
+        raw[setup.unused.cuda()] = 0xFF
+    _check_attention(setup, q)
+    q[0, 0] *= 2.0 ** -100
+    q[0, 1, 7] = 900.0
+    q[0, 2] = 0.0
+    _check_attention(setup, q)
+    setup = Setup(package, [1024], [new], heads, 64, 0, seed=42)
+    q = torch.zeros(new, h, dim).bfloat16()
+    q[..., 0] = 4.0 * dim ** 0.5 / 16
+    codes = setup.gpu[0].cpu().float()
+    setup.gpu[2].fill_(2.0 ** -4)
+    for i, page in enumerate(setup.table[0].tolist()):
+        codes[page, :, :, 0] = torch.arange(64) * 0.5 + 32.0 * i - 256
+    setup.gpu[0].copy_(codes.to(torch.float8_e4m3fn).cuda())
+    _check_attention(setup, q)
+    codes[..., :] = 0.0
+    codes[int(setup.table[0, 0]), :, 3, 0] = 448.0
+    setup.gpu[0].copy_(codes.to(torch.float8_e4m3fn).cuda())
+    setup.gpu[1].view(torch.uint8)[int(setup.table[0, 0]), :, 3] = 0
+    q[..., 0] = 8.0 * dim ** 0.5 / 16
+    _check_attention(setup, q)
+
+
+@pytest.mark.parametrize("heads", OTHER_HEADS)
+@pytest.mark.parametrize("new", [3, 30])
+def test_not_finite_tokens_and_queries_of_other_head_sizes(package, heads, new):
+    h, kv_heads, dim = heads
+    setup = Setup(package, [150], [new], heads, 64, 64, seed=12)
+    k, v, q = setup.randn(new, kv_heads, dim), setup.randn(new, kv_heads, dim), setup.randn(new, h, dim)
+    k[new - 2, 1, dim - 1] = math.nan
+    v[new - 1, 0, 3] = math.inf
+    q[0, h - 1, 5] = math.nan
+    _check_append(setup, k, v)
+    out = setup.cache.attention(1, setup.batch, q.cuda()).cpu()
+    setup.cache.sync()
+    lost = torch.zeros(new, h, dtype=torch.bool)
+    lost[new - 2:, h // kv_heads:2 * h // kv_heads] = True
+    lost[new - 1, :h // kv_heads] = True
+    lost[0, h - 1] = True
+    assert torch.equal(torch.isnan(out).all(-1), lost) and torch.equal(torch.isnan(out).any(-1), lost)
+
+
 @pytest.mark.parametrize("new", [1, 40])
 @pytest.mark.parametrize("heads", [(16, 2, 256), (6, 2, 128), (8, 8, 64)])
 @pytest.mark.parametrize("layout", ["heads first", "one row for all", "one head for all", "rows that are no multiple of heads"])
