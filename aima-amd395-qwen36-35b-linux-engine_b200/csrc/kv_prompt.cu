@@ -16,7 +16,7 @@
 //   w 2^9   = one f16                        to 2^-11 of itself down to 2^-23 of the largest
 // with V's codes as f16, which they are exactly, in a second pair of buffers (heads of 256 would need 128 KB for them).  That saves the
 // softmax 13 of 23 instructions per four weights and the tensor cores a third of the second product; the softmax warps widen V on
-// the way.  4096 tokens of 16384 with 32/8 heads of 128 1235 us in three terms and 1125 this way, with 8/8 of 64 275 and 247.
+// the way.  4096 tokens of 16384 with 32/8 heads of 128 1235 us in three terms and 1090 this way, with 8/8 of 64 275 and 242.
 // All terms of an operand go into one accumulator.  S[128 rows, 128 positions] = Q K^T with both operands in shared memory;
 // O[128, head_dim] += W V with W in tensor memory, where it takes the place of the scores it was made from, and V MN-major.
 //
@@ -26,8 +26,8 @@
 //
 // Measured: 8192 tokens of 32768 with 16/2 heads of 256 3.68 ms = 1.04 PFLOP/s at the 1.5 GHz that the power cap leaves, 2560 cycles
 // of products in the 3250 of a tile: both operands of Q K^T come from shared memory at its full rate while the next tiles are
-// written there.  With heads of 128 a tile takes 2250 cycles, which its softmax needs (a chain of loads, maxima, an exchange and 64
-// weights per thread on two warps per scheduler), the products 1050: 7 prompts of 1531 .. 2999 with 32/8 heads 361 us.  1024
+// written there.  With heads of 128 a tile takes 2200 cycles, which its softmax needs (a chain of V's widening, maxima, an exchange and 64
+// weights per thread on two warps per scheduler), the products 1050: 7 prompts of 1531 .. 2999 with 32/8 heads 352 us.  1024
 // tokens of 16/2 heads of 256 alone 27 us, most of it before the first tile and after the last.
 #include "kv_attention.cuh"
 
@@ -404,28 +404,32 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
   auto ring_v = [](int first, int j, int n) { return first + (j + 1 < n ? 2 * j + 2 : 2 * n - 1); };
 
   // V of a tile from its codes to 16 bits, 16 rows by each of warps 4 .. 11.  Rows behind the sequence's end, where a page can hold
-  // anything, become zeros.
+  // anything, become zeros.  Which rows eight lanes have together lets them read and write all banks: with heads of 128 four pieces of
+  // rows r and r ^ 5, whose swizzles differ in the bit that tells even pieces from odd ones and in the one that tells halves.
   auto widen = [&](int slot, int buffer, int seen) {
-    constexpr int kPieces = kDim < 256 ? kDim / 16 : 8, kRowsAtOnce = 32 / kPieces, kSteps = 16 / kRowsAtOnce;    // of 16 codes; rows of a step
+    constexpr bool kLong = kDim == 128;
+    constexpr int kSteps = kLong ? 4 : 2;
+    const int piece = kLong ? (lane & 3) | ((lane >> 2) & 4) : lane & 3;          // of 16 codes
+    const int low = kLong ? (5 * ((lane >> 2) & 1)) ^ ((lane >> 3) & 1) : lane >> 2;
+    auto row_of = [&](int b) { return 16 * (warp - 4) + low + (kLong ? 2 * (b & 1) + 8 * (b >> 1) : 8 * b); };
     const uint8_t* from = generic + slot * L::kSlotBytes;
-    uint8_t* to = generic + L::kWideAt + buffer * L::kWideBytes;
-    const int piece = lane % kPieces, first = 16 * (warp - 4) + lane / kPieces;
-    const uint32_t order = piece >> 2, swap = 0u - order;                 // the upper half first, so that eight lanes write to all banks
+    uint8_t* to = generic + L::kWideAt + buffer * L::kWideBytes + (piece >> 2) * (kKvTile * 128);
     uint4 codes[kSteps];
 #pragma unroll
     for (int b = 0; b < kSteps; ++b) {
-      const int at = first + b * kRowsAtOnce;
-      codes[b] = *reinterpret_cast<const uint4*>(from + at * L::kRowBytes + ((piece ^ (L::kRowBytes == 128 ? at & 7 : (at >> 1) & 3)) << 4));
+      const int swizzle = kLong ? low ^ (2 * (b & 1)) : (low >> 1) & 3;
+      codes[b] = *reinterpret_cast<const uint4*>(from + row_of(b) * L::kRowBytes + ((piece ^ swizzle) << 4));
+    }
+    if (seen < kKvTile) {
+#pragma unroll
+      for (int b = 0; b < kSteps; ++b)
+        if (row_of(b) >= seen) codes[b] = make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int b = 0; b < kSteps; ++b) {
-      const int at = first + b * kRowsAtOnce;
-      const uint32_t there = at < seen ? 0xffffffffu : 0u;
-      uint4 c = make_uint4(codes[b].x & there, codes[b].y & there, codes[b].z & there, codes[b].w & there);
-      const uint32_t x = (c.x ^ c.z) & swap, y = (c.y ^ c.w) & swap;
-      c = make_uint4(c.x ^ x, c.y ^ y, c.z ^ x, c.w ^ y);
-      uint8_t* row_at = to + (piece >> 2) * (kKvTile * 128) + at * 128;
-      const uint32_t even = (((2 * (piece & 3)) ^ (at & 7)) ^ order) << 4;
+      const uint4& c = codes[b];
+      const uint32_t even = ((2 * (piece & 3)) ^ (kLong ? low ^ (2 * (b & 1)) : low)) << 4;
+      uint8_t* row_at = to + row_of(b) * 128;
       *reinterpret_cast<uint4*>(row_at + even) = make_uint4(e4m3x2_f16x2(c.x), e4m3x2_f16x2(c.x >> 16), e4m3x2_f16x2(c.y), e4m3x2_f16x2(c.y >> 16));
       *reinterpret_cast<uint4*>(row_at + (even ^ 16)) = make_uint4(e4m3x2_f16x2(c.z), e4m3x2_f16x2(c.z >> 16), e4m3x2_f16x2(c.w), e4m3x2_f16x2(c.w >> 16));
     }
