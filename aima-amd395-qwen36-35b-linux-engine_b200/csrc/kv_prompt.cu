@@ -24,8 +24,8 @@
 // row) each turn half of a tile's scores into weights; two warps with the same rows exchange their maxima in between.
 // The scores are double-buffered: the products of one tile run under the softmax of another.
 //
-// Measured: 8192 tokens of 32768 with 16/2 heads of 256 3.68 ms = 1.04 PFLOP/s at the 1.5 GHz that the power cap leaves, 2560 cycles
-// of products in the 3250 of a tile: both operands of Q K^T come from shared memory at its full rate while the next tiles are
+// Measured: 8192 tokens of 32768 with 16/2 heads of 256 3.74 ms = 1.03 PFLOP/s at the 1.5 GHz that the power cap leaves, 2560 cycles
+// of products in the 3300 of a tile: both operands of Q K^T come from shared memory at its full rate while the next tiles are
 // written there.  With heads of 128 a tile takes 2200 cycles, which its softmax needs (a chain of V's widening, maxima, an exchange and 64
 // weights per thread on two warps per scheduler), the products 1050: 7 prompts of 1531 .. 2999 with 32/8 heads 352 us.  1024
 // tokens of 16/2 heads of 256 alone 27 us, most of it before the first tile and after the last.
@@ -495,9 +495,10 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
       while (alive && walk.next()) {
         const int n = walk.tiles;
         auto scores = [&](int j) {
-          // the scores' buffer is free: the product that read the weights in it was issued before
+          // the scores' buffer is free once the product that reads the weights in it has ended: products of different shapes
+          // need not run in the order of issue (the wait costs heads of 256 two percent, smaller ones nothing)
           const int r = ring_k(ring, j), slot = r % L::kSlots, buffer = (tile + j) & 1;
-          if (!wait(&sm.full[slot], (r / L::kSlots) & 1)) return false;
+          if (!wait(&sm.full[slot], (r / L::kSlots) & 1) || !wait(&sm.o_done[buffer], (((tile + j) >> 1) & 1) ^ 1)) return false;
           tc_fence_after();
           if (elect_one()) {
             const uint32_t k0 = base + slot * L::kSlotBytes, q0 = base + L::kQueryAt;
