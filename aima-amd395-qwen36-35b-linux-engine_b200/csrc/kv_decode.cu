@@ -10,9 +10,12 @@
 //   S^T[128 positions, rows]   = K[128, head_dim] . Q^T            K-major A
 //   O^T[head_dim, rows]       += V^T[head_dim, 128] . P^T           MN-major A: V's rows are the K dimension
 // Nothing is unpacked to 16 bits.  A BF16 query is split into two e4m3 terms, q 2^-e = hi + lo / 16 -- exact but for elements
-// below 2^-15 of the row's largest -- that are 2 x rows columns of one product.  A weight is split into an e4m3 term and an
-// e5m2 term scaled by 2^11, w 2^8 = hi + lo 2^-11, which holds it to 2^-8 of itself down to 2^-29 of the largest and to
-// 2^-36 below that; the two have accumulators of their own.  All sums are FP32 in tensor memory.
+// below 2^-15 of the row's largest -- that are 2 x rows columns of one product.  A weight becomes an f16, w 2^14, and that three
+// e5m2 terms, the upper bytes of it and of what is left of it, times 8 each time: w 2^14 = t0 + t1 / 8 + t2 / 64 to 2^-8.7 of
+// itself where it exceeds 2^-28 of the largest and to 2^-36 of the largest below that.  (Without the factors of 8 the last terms of a
+// small weight are subnormal; an e4m3 first term with an e5m2 remainder leaves 3 bits below 2^-18, which shows where one position outweighs
+// all others and brings nothing.)  The terms are 3 x rows columns of one product, each with its accumulators.  All sums are FP32 in
+// tensor memory.
 //
 // One block per SM; the list of all tiles is cut into equal shares (kv_attention.cuh).  Warp 0 loads tiles by page, warp 1
 // issues the products, warps 2 and 3 prepare the queries of the next unit, warps 4-7 (thread = position) do the softmax and
@@ -27,9 +30,8 @@ namespace aima {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kGrow = 0.75f;            // 2^8 * 2^0.75 = 430 <= 448
-constexpr float kWeightScale = 256.0f;
-constexpr float kLowScale = 2048.0f;      // a remainder is at most 16: 32768 <= 57344
+constexpr float kGrow = 0.75f;            // 2^14 * 2^0.75 = 27554: a remainder times 8 rounds to at most 32768
+constexpr float kWeightExponent = 14.0f;  // of the weights and of their sum alike
 constexpr float kQueryLow = 16.0f;        // a remainder is at most 16: 256 <= 448 (0x4c00 as f16)
 constexpr int kMaxPrefix = AIMA_MOE_KV_MAX_SEQUENCES + 1;
 
@@ -40,14 +42,14 @@ struct Decode {
   static constexpr int kPanelBytes = kKvTile * kRowBytes;
   static constexpr int kSlotBytes = kKvTile * kDim;
   static constexpr int kSlots = kDim == 256 ? 6 : 8;
-  static constexpr int kWeightRows = kRows < 16 ? 16 : kRows;           // N of the second product
+  static constexpr int kWeightRows = (3 * kRows + 15) / 16 * 16;        // N of the second product: three terms, and zeros
   static constexpr int kQueryBytes = 2 * kRows * kDim;
-  static constexpr int kWeightBytes = kWeightRows * kKvTile;            // one term of one buffer
+  static constexpr int kWeightBytes = kWeightRows * kKvTile;            // one buffer
   static constexpr int kOutPanels = kDim >= 128 ? kDim / 128 : 1;
-  static constexpr int kOutColumn = 4 * kRows;                          // tensor memory: S0 | S1 | per panel hi | lo
+  static constexpr int kOutColumn = 4 * kRows;                          // tensor memory: S0 | S1 | per panel the terms
   static constexpr int kQueryAt = kSlots * kSlotBytes;
   static constexpr int kWeightAt = kQueryAt + 2 * kQueryBytes;          // two segments' queries
-  static constexpr int kPrefixAt = kWeightAt + 4 * kWeightBytes;
+  static constexpr int kPrefixAt = kWeightAt + 2 * kWeightBytes;
   static constexpr int kSmallAt = (kPrefixAt + kMaxPrefix * 4 + 15) / 16 * 16;
 };
 
@@ -145,8 +147,8 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
     mbar_fence_init();
   }
   if (warp == 2) tmem_alloc(smem_u32(&sm.tmem), 512);
-  if (kRows < 16) {           // rows of the weights that no query has
-    for (int i = threadIdx.x; i < 4 * L::kWeightBytes / 16; i += kThreads)
+  if (L::kWeightRows > 3 * kRows) {           // rows of the weights that are no term
+    for (int i = threadIdx.x; i < 2 * L::kWeightBytes / 16; i += kThreads)
       *reinterpret_cast<uint4*>(generic + L::kWeightAt + 16 * i) = make_uint4(0, 0, 0, 0);
     fence_async_proxy();
   }
@@ -258,8 +260,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
   } else if (warp == 1) {
     // ------------------------------ products ------------------------------
     constexpr uint32_t kScores = instr_desc_f8(kE4m3, kE4m3, 0, 0, 128, 2 * kRows);
-    constexpr uint32_t kSumsHigh = instr_desc_f8(kE4m3, kE4m3, 1, 0, 128, L::kWeightRows);
-    constexpr uint32_t kSumsLow = instr_desc_f8(kE4m3, kE5m2, 1, 0, 128, L::kWeightRows);
+    constexpr uint32_t kSums = instr_desc_f8(kE4m3, kE5m2, 1, 0, 128, L::kWeightRows);
     int ring = 0, tile = 0, segment = 0;
     bool alive = true;
     while (alive && walk.next()) {
@@ -289,16 +290,15 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
         if (!wait(&sm.p_full[buffer], ((tile + j) >> 1) & 1) || !wait(&sm.full[slot], (r / L::kSlots) & 1)) { alive = false; break; }
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t v0 = base + slot * L::kSlotBytes, p0 = base + L::kWeightAt + buffer * 2 * L::kWeightBytes;
+          const uint32_t v0 = base + slot * L::kSlotBytes, p0 = base + L::kWeightAt + buffer * L::kWeightBytes;
 #pragma unroll
           for (int panel = 0; panel < L::kOutPanels; ++panel) {
-            const uint32_t d = tmem + L::kOutColumn + panel * 2 * L::kWeightRows;
+            const uint32_t d = tmem + L::kOutColumn + panel * L::kWeightRows;
 #pragma unroll
             for (int k = 0; k < kKvTile / 32; ++k) {
               // head_dim 64: the instruction's upper 64 rows read the next slot (or the queries); nothing reads them
               const uint64_t v = smem_desc_rows<L::kRowBytes>(v0 + panel * L::kPanelBytes + k * 32 * L::kRowBytes, L::kPanelBytes);
-              umma_f8(d, v, smem_desc_rows<128>(p0) + k * 2, kSumsHigh, (j | k) != 0);
-              umma_f8(d + L::kWeightRows, v, smem_desc_rows<128>(p0 + L::kWeightBytes) + k * 2, kSumsLow, (j | k) != 0);
+              umma_f8(d, v, smem_desc_rows<128>(p0) + k * 2, kSums, (j | k) != 0);
             }
           }
           umma_commit(smem_u32(&sm.empty[slot]));
@@ -474,8 +474,8 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
             }
             if (j > 0) {
 #pragma unroll 1
-              for (int c = 0; c < 2 * L::kOutPanels; ++c) {
-                const uint32_t at = tmem + lanes + L::kOutColumn + c * L::kWeightRows + r0;
+              for (int c = 0; c < 3 * L::kOutPanels; ++c) {
+                const uint32_t at = tmem + lanes + L::kOutColumn + c / 3 * L::kWeightRows + c % 3 * kRows + r0;
                 uint32_t o[8];
                 tmem_ld8(at, o);
                 tmem_ld_wait();
@@ -489,24 +489,23 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
         }
         // the buffer of the weights is free once the product of two tiles ago has read it
         wait(&sm.o_done[buffer], ((tile >> 1) & 1) ^ 1);
-        uint8_t* high = generic + L::kWeightAt + buffer * 2 * L::kWeightBytes;
+        uint8_t* terms = generic + L::kWeightAt + buffer * L::kWeightBytes;
 #pragma unroll
         for (int r = 0; r < kRows; r += 2) {
           float w[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            w[i] = fast_exp2(t[r + i] - (top[r + i] == -INFINITY ? 0.0f : top[r + i]));
+            w[i] = fast_exp2(t[r + i] + (kWeightExponent - (top[r + i] == -INFINITY ? 0.0f : top[r + i])));
             weights[r + i] = fmaf(w[i], value_inverse, weights[r + i]);
-            w[i] *= kWeightScale;
           }
-          const uint32_t hi = cvt_e4m3x2(w[0], w[1]);
-          const float2 back = e4m3x2_values(hi);
-          const uint32_t lo = cvt_e5m2x2((w[0] - back.x) * kLowScale, (w[1] - back.y) * kLowScale);
+          uint32_t h = cvt_f16x2(w[0], w[1]);
+          const int at = r * 128 + (token & 15), piece = token >> 4;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int at = (r + i) * 128 + (((token >> 4) ^ ((r + i) & 7)) << 4) + (token & 15);
-            high[at] = static_cast<uint8_t>(hi >> (8 * i));
-            high[L::kWeightBytes + at] = static_cast<uint8_t>(lo >> (8 * i));
+          for (int term = 0; term < 3; ++term) {
+            const uint32_t codes = term < 2 ? h : h + 0x00800080u;        // two cut off, the last rounded
+            terms[term * kRows * 128 + at + ((piece ^ (r & 7)) << 4)] = static_cast<uint8_t>(codes >> 8);
+            terms[term * kRows * 128 + at + 128 + ((piece ^ ((r + 1) & 7)) << 4)] = static_cast<uint8_t>(codes >> 24);
+            if (term < 2) h = mul_f16x2(sub_f16x2(h, h & 0xff00ff00u), 0x48004800u);        // times 8
           }
         }
         if (j + 1 == n && (walk.tile0 + n) * kKvTile > length) {
@@ -559,22 +558,21 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
         const int d = panel * 128 + token;
 #pragma unroll
         for (int r0 = 0; r0 < kRows; r0 += 8) {
-          uint32_t hi[8], lo[8];
-          const uint32_t at = tmem + lanes + L::kOutColumn + panel * 2 * L::kWeightRows + r0;
-          tmem_ld8(at, hi);
-          tmem_ld8(at + L::kWeightRows, lo);
+          uint32_t o[3][8];
+#pragma unroll
+          for (int term = 0; term < 3; ++term) tmem_ld8(tmem + lanes + L::kOutColumn + panel * L::kWeightRows + term * kRows + r0, o[term]);
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int r = r0 + i;
             if (r >= rows || d >= kDim) continue;
-            const float o = fmaf(__uint_as_float(lo[i]), 1.0f / kLowScale, __uint_as_float(hi[i])) * (1.0f / kWeightScale);
+            const float x = fmaf(__uint_as_float(o[2][i]), 1.0f / 64.0f, fmaf(__uint_as_float(o[1][i]), 1.0f / 8.0f, __uint_as_float(o[0][i])));
             if (whole) {
               const float4 s4 = *reinterpret_cast<const float4*>(sm.part[last ^ 1][r]);
               const float sum = (s4.x + s4.y) + (s4.z + s4.w);
-              a.out[sm.out_at[which][r] + d] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : o / sum);
+              a.out[sm.out_at[which][r] + d] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : x / sum);
             } else {
-              kv_part_sum<kDim>(plan.work, part, r, d & ~3)[d & 3] = o;
+              kv_part_sum<kDim>(plan.work, part, r, d & ~3)[d & 3] = x;
             }
           }
         }
