@@ -9,7 +9,7 @@
 // cache is e4m3, and no operand of mixed width exists.  So Q is split into two 8-bit terms and its product runs twice at twice the rate:
 //   q 2^-e  = hi (e4m3) + lo (e5m2)          exact down to 2^-16 (largest 448)
 // Weights and values, heads of 256:
-//   w 2^9   = three terms (e5m2)             to 2^-8 of itself where it exceeds 2^-9 (2^-18 of the largest), to 2^-17 below
+//   w 2^9   = three terms (e5m2)             to 2^-8 of itself where it exceeds 2^-9, to 2^-17 below
 // An e5m2 number is the upper byte of an f16, so the weights' terms take no conversions; two terms with an e4m3 first one would
 // take a fifth less of the tensor cores but hold weights below 2^-13 of the largest to a few bits only, which is not enough where
 // one position outweighs all others and brings nothing.  Heads of 64 and 128 (kWide), whose softmax takes longer than their products:
@@ -39,6 +39,13 @@ constexpr int kThreads = 384;
 // falls short of it by more than kFall, where the weights get few bits.  It stays within kDepth of the row's maximum so that
 // nothing overflows.
 constexpr float kGrow = 6.75f;            // 2^9 * 2^6.75 = 55109 <= 57344
+// Of three terms the last is subnormal where a weight is small, so a row's first maximum, and one that exceeds all before it by more than
+// kJump, is placed kLift above the reference: the other weights of its tile keep 2^-8 of themselves down to 2^-22.75 of it instead of
+// 2^-18, which shows where one position outweighs all others and brings nothing.  The next time that a row of the warp moves, the
+// others give the lift back, so that ordinary scores, whose maximum grows slowly, rescale once or twice more per unit.  (Always so
+// little room above the maximum: 4096 tokens of 16384 955 -> 1006 us.)
+constexpr float kLift = 4.75f;
+constexpr float kJump = 8.0f;
 constexpr float kFall = 16.0f;
 constexpr float kDepth = 30.0f;
 constexpr float kWeightExponent = 9.0f;
@@ -769,8 +776,11 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
         const bool falls = m > -INFINITY && fmaxf(m, peak - kDepth) < top - kFall;
         const bool moves = m > top + kGrow || falls;               // the first that is seen is above -inf
         if (__any_sync(0xffffffffu, moves)) {
-          const float now = falls ? fmaxf(m, peak - kDepth) : moves ? m : top;
-          const float f = moves ? fast_exp2(top - now) : 1.0f;     // top is -inf at first: 0
+          float now = top;
+          if (falls) now = fmaxf(m, peak - kDepth);
+          else if (moves) now = !L::kWide && m > top + kJump ? m - kLift : m;
+          else if (!L::kWide && peak - top <= kLift) now = fmaxf(top, peak);       // a lift that is given back; a fallen reference stays
+          const float f = now != top ? fast_exp2(top - now) : 1.0f;                // top is -inf at first: 0
           if (j > 0) {
             wait(&sm.o_done[buffer ^ 1], ((tile - 1) >> 1) & 1);
             tc_fence_after();

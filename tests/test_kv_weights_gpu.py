@@ -39,3 +39,11 @@ def test_small_weights_of_few_rows_keep_their_bits(package, heads, new, length):
     """One position outweighs all others by 2^12 .. 2^27 and brings nothing."""
     for low, high in ((12.0, 16.0), (16.0, 20.0), (20.0, 24.0), (24.0, 27.0)):
         _check_attention(*_sink(package, length, new if new * heads[0] // heads[1] <= 16 else 1, heads, (low, high)))
+
+
+@pytest.mark.parametrize("length", [60, 300, 1024])
+@pytest.mark.parametrize("heads", [(16, 2, 256), (16, 2, 128), (8, 1, 64), (8, 8, 64)])
+def test_small_weights_of_prompts_keep_their_bits(package, heads, length):
+    """The same for many rows, up to where heads of 256 hold the weights beside the largest to 2^-8: 2^-22 of it."""
+    for low, high in ((12.0, 16.0), (16.0, 19.0), (19.0, 22.0)) + (((22.0, 26.0),) if heads[2] < 256 else ()):
+        _check_attention(*_sink(package, length, 40, heads, (low, high)))
