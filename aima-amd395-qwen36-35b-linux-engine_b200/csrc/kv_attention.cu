@@ -25,7 +25,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 size_t round256(size_t bytes) { return (bytes + 255) / 256 * 256; }
 size_t sums_bytes(const KvShape& shape) { return round256(2ull * kKvMaxBlocks * kKvPartRows * shape.head_dim * sizeof(float)); }
-size_t weights_bytes() { return round256(2ull * kKvMaxBlocks * kKvPartRows * sizeof(float2)); }
+size_t weights_bytes() { return round256(2ull * kKvMaxBlocks * kKvPartRows * sizeof(float4)); }
 
 }  // namespace
 
@@ -70,7 +70,7 @@ cudaError_t kv_attention(const KvAttention& a, const KvMaps& maps, void* workspa
   plan.a = a;
   uint8_t* cursor = static_cast<uint8_t*>(workspace);
   plan.work.arrived = reinterpret_cast<unsigned*>(cursor); cursor += kv_counter_bytes();
-  plan.work.weights = reinterpret_cast<float2*>(cursor); cursor += weights_bytes();
+  plan.work.weights = reinterpret_cast<float4*>(cursor); cursor += weights_bytes();
   plan.work.sums = reinterpret_cast<float*>(cursor); cursor += sums_bytes(a.shape);
   plan.work.starts = reinterpret_cast<KvStart*>(cursor);
   plan.blocks = sm_count < kKvMaxBlocks ? sm_count : kKvMaxBlocks;

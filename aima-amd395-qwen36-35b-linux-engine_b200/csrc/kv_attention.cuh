@@ -14,6 +14,13 @@ constexpr int kKvMaxBlocks = 160;       // blocks of an attention kernel at most
 constexpr int kKvPartRows = 128;
 constexpr int kKvMaxList = 1 << 24;     // tiles (with the units' own cost) of a launch: shares are computed in 32 bits
 
+// A value's scale vs rides on its weight, w = 2^(s + log2 vs - m), which is relative to the largest of them.  The softmax's denominator
+// wants them without it.  While the scales stay within 2^kKvApart of 2^e, the exponent of the first page's, it is the sum of w 2^e / vs,
+// relative to 2^l with l = m - e: no weight that counts there is lost in w.  From the first page beyond that on its terms are
+// exponentials of their own, 2^(s - l) with a running l: a page of zeros, whose scale is the least, may lie beside one of the
+// largest values.  Either way o = 2^(m - l) * (sum of w code) / denominator.
+constexpr float kKvApart = 32.0f;
+
 struct KvMaps {
   CUtensorMap keys, values;             // [pages * kv_heads * page_tokens, head_dim] bytes, boxes of one page x up to 128 bytes
 };
@@ -33,7 +40,7 @@ struct alignas(16) KvStart {
 // (kv_join).  A block has two parts: of the unit that it begins in the middle, and of the one that it does not finish.
 struct KvWorkspace {
   unsigned* arrived;      // [2 * kKvMaxBlocks], by the block that begins the unit: parts written, parts joined; zero between launches
-  float2* weights;        // [2 * kKvMaxBlocks][kKvPartRows]: reference maximum (log2), sum of the weights
+  float4* weights;        // [2 * kKvMaxBlocks][kKvPartRows]: m, denominator, l
   float* sums;            // [2 * kKvMaxBlocks][head_dim / 4][kKvPartRows][4]
   KvStart* starts;        // [kKvMaxBlocks + 1], for prompts of many row tiles
 };
@@ -63,7 +70,12 @@ __device__ __forceinline__ int kv_first_cut(int x, int total, int blocks) {
 }
 
 __device__ __forceinline__ size_t kv_part_index(int block, bool begins) { return 2 * block + (begins ? 1 : 0); }
-__device__ __forceinline__ float2* kv_part_weight(const KvWorkspace& work, size_t part, int row) { return work.weights + part * kKvPartRows + row; }
+// Two factors whose product is 2^d, each within FP32's range.
+__device__ __forceinline__ float2 kv_exp2_factors(float d) {
+  const float near = fminf(fmaxf(d, -60.0f), 60.0f);
+  return make_float2(fast_exp2(near), fast_exp2(d - near));
+}
+__device__ __forceinline__ float4* kv_part_weight(const KvWorkspace& work, size_t part, int row) { return work.weights + part * kKvPartRows + row; }
 template <int kDim>
 __device__ __forceinline__ float* kv_part_sum(const KvWorkspace& work, size_t part, int row, int d) {       // d: a multiple of 4
   return work.sums + part * kKvPartRows * kDim + (static_cast<size_t>(d >> 2) * kKvPartRows + row) * 4;
@@ -102,9 +114,10 @@ __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace&
   }
   __syncthreads();
   const bool ok = *verdict != 0;
-  auto store = [&](int row, int d, const float4& x, float inverse) {
+  auto store = [&](int row, int d, const float4& sums, float inverse, float rest) {
+    const float4 x = make_float4(sums.x * inverse, sums.y * inverse, sums.z * inverse, sums.w * inverse);
     const int token = row / a.shape.group, g = row - token * a.shape.group;
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inverse, x.y * inverse), hi = __floats2bfloat162_rn(x.z * inverse, x.w * inverse);
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * rest, x.y * rest), hi = __floats2bfloat162_rn(x.z * rest, x.w * rest);
     *reinterpret_cast<uint2*>(a.out + (static_cast<long long>(unit.row0 + token) * a.shape.q_heads + unit.head + g) * kDim + d) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
   };
@@ -127,24 +140,27 @@ __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace&
         }
       }
     };
-    float2 w[kFew];
+    float4 w[kFew];
 #pragma unroll
     for (int p = 0; p < kFew; ++p) {
-      w[p] = make_float2(-INFINITY, 0.0f);
+      w[p] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
       if (p < unit.parts) w[p] = __ldcg(kv_part_weight(work, kv_part_index(unit.first_block + p, p == 0), row));
     }
     load();
-    float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int p = 0; p < kFew; ++p) top = fmaxf(top, w[p].x);
-    if (top == -INFINITY) top = 0.0f;                             // nothing seen, or nothing but NaN
+    float top = -INFINITY, low = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int p = 0; p < kFew; ++p) {
-      const float f = fast_exp2(w[p].x - top);
-      sum += w[p].x == -INFINITY ? w[p].y : w[p].y * f;
-      w[p].x = f;
+      top = fmaxf(top, w[p].x);
+      low = fmaxf(low, w[p].z);
     }
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (top == -INFINITY) top = low = 0.0f;                       // nothing seen, or nothing but NaN
+#pragma unroll
+    for (int p = 0; p < kFew; ++p) {
+      sum += w[p].z == -INFINITY ? w[p].y : w[p].y * fast_exp2(w[p].z - low);
+      w[p].x = fast_exp2(w[p].x - top);
+    }
+    const float2 back = kv_exp2_factors(top - low);
+    const float inverse = sum == 0.0f ? 0.0f : back.x / sum;
 #pragma unroll 1
     for (;;) {
 #pragma unroll
@@ -157,7 +173,7 @@ __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace&
           acc.z = fmaf(x[i][p].z, w[p].x, acc.z);
           acc.w = fmaf(x[i][p].w, w[p].x, acc.w);
         }
-        if (d + 4 * at_once * i < end) store(row, d + 4 * at_once * i, acc, inverse);
+        if (d + 4 * at_once * i < end) store(row, d + 4 * at_once * i, acc, inverse, back.y);
       }
       d += 4 * kColumns * at_once;
       if (d >= end) break;
@@ -179,12 +195,12 @@ __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace&
       const int i = min(i0 + slot, end - 1);                      // whole warps stay together
       const int row = i % unit.rows, d = 4 * (i / unit.rows);
       float4 x[5];
-      float2 w[5];
-      float top = -INFINITY;
+      float4 w[5];
+      float top = -INFINITY, low = -INFINITY;
 #pragma unroll
       for (int k = 0; k < 5; ++k) {
         const int p = lane + k * lanes;
-        w[k] = make_float2(-INFINITY, 0.0f);
+        w[k] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
         x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (p < unit.parts) {
           const size_t part = kv_part_index(unit.first_block + p, p == 0);
@@ -192,15 +208,19 @@ __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace&
           x[k] = __ldcg(reinterpret_cast<const float4*>(kv_part_sum<kDim>(work, part, row, d)));
         }
         top = fmaxf(top, w[k].x);
+        low = fmaxf(low, w[k].z);
       }
-      for (int step = lanes >> 1; step >= 1; step >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
-      if (top == -INFINITY) top = 0.0f;                           // nothing seen, or nothing but NaN
+      for (int step = lanes >> 1; step >= 1; step >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+        low = fmaxf(low, __shfl_xor_sync(0xffffffffu, low, step));
+      }
+      if (top == -INFINITY) top = low = 0.0f;                     // nothing seen, or nothing but NaN
       float sum = 0.0f;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int k = 0; k < 5; ++k) {
         const float f = fast_exp2(w[k].x - top);
-        sum += w[k].x == -INFINITY ? w[k].y : w[k].y * f;
+        sum += w[k].z == -INFINITY ? w[k].y : w[k].y * fast_exp2(w[k].z - low);
         acc.x = fmaf(x[k].x, f, acc.x);
         acc.y = fmaf(x[k].y, f, acc.y);
         acc.z = fmaf(x[k].z, f, acc.z);
@@ -213,7 +233,8 @@ __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace&
         acc.z += __shfl_xor_sync(0xffffffffu, acc.z, step);
         acc.w += __shfl_xor_sync(0xffffffffu, acc.w, step);
       }
-      if (lane == 0 && i0 + slot < end) store(row, d, acc, sum == 0.0f ? 0.0f : 1.0f / sum);
+      const float2 back = kv_exp2_factors(top - low);
+      if (lane == 0 && i0 + slot < end) store(row, d, acc, sum == 0.0f ? 0.0f : back.x / sum, back.y);
     }
   }
   if (ok) {

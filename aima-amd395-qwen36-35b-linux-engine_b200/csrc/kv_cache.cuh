@@ -25,6 +25,9 @@ __device__ __forceinline__ int kv_scale_exponent(float amax) {
   return amax == 0.0f ? kKvMinExponent : min(max(e, kKvMinExponent), kKvMaxExponent);
 }
 
+// floor(log2 x) of a normal number
+__device__ __forceinline__ int kv_float_exponent(float x) { return ((__float_as_int(x) >> 23) & 255) - 127; }
+
 struct KvLayer {
   uint8_t* keys;           // [pages, kv_heads, page_tokens, head_dim] e4m3
   uint8_t* values;

@@ -2,8 +2,8 @@
 //
 //   t_j = scale q . k_j  (log2 units) + log2(value scale of j's page),   w_j = 2^(t_j - m)
 //   o   = sum_j w_j code(v_j) / sum_j w_j / (value scale of j's page)
-// A page's scale of V is carried by the weight, so that V enters the product as the codes that lie in memory; its share of
-// the sum of the weights is divided out again in FP32.
+// A page's scale of V is carried by the weight, so that V enters the product as the codes that lie in memory; the denominator is
+// taken without it (kv_attention.cuh).
 //
 // Bound: the cache is read once, 2 head_dim bytes per position and key/value head, and the products with the 1 .. 16 rows
 // that share them are small.  So the CACHE is the M side of both products, as it comes by TMA, and the rows are the N side:
@@ -64,6 +64,7 @@ struct Small {              // shared memory that is not an operand
   unsigned long long full[8], empty[8];
   unsigned long long s_full[2], s_empty[2], p_full[2], o_done[2], q_full[2], info_empty[2], drain;
   alignas(16) float part[2][kRows][4];  // per row and warp: maxima of a tile (two buffers), sums at the end of a segment
+  alignas(16) float low[kRows][4];      // scales far apart: maxima of a tile without them
   float row_scale[2][kRows];
   int limit[2][kRows];      // last position a row sees; -1: none
   long long out_at[2][kRows];
@@ -112,6 +113,17 @@ __device__ __forceinline__ float reduce8(const float* v, int lane) {
   return join(c, __shfl_xor_sync(0xffffffffu, c, 1));
 }
 __device__ __forceinline__ void softmax_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// ... and whether x holds in any of its threads
+__device__ __forceinline__ bool softmax_barrier_or(bool x) {
+  uint32_t any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(any) : "r"(static_cast<uint32_t>(x)) : "memory");
+  return any != 0;
+}
+__device__ __forceinline__ float max4(const float* at) {
+  const float4 m = *reinterpret_cast<const float4*>(at);
+  return fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
+}
 
 template <int kDim, int kRows>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -408,20 +420,24 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
         const size_t at = static_cast<size_t>(page) * shape.kv_heads + walk.head;
         return make_float2(a.layer.key_scales[at], a.layer.value_scales[at]);
       };
-      float top[kRows], weights[kRows];
+      float top[kRows], weights[kRows], low[kRows];      // low: once scales are apart
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        top[r] = -INFINITY;
+        top[r] = low[r] = -INFINITY;
         weights[r] = 0.0f;
       }
+      bool apart = false;                  // the same in all threads
       int page = page_of(0), page_next = page_of(1);
       float2 scales = scales_of(page);
+      const int page_first = table[(walk.tile0 * kKvTile) >> shape.page_shift];
+      const float first = page_first < 0 || page_first >= shape.pages
+                              ? 0.0f : static_cast<float>(kv_float_exponent(a.layer.value_scales[static_cast<size_t>(page_first) * shape.kv_heads + walk.head]));
       for (int j = 0; j < n; ++j, ++tile) {
         const int buffer = tile & 1;
         const float2 scales_next = scales_of(page_next);
         const int page_after = page_of(j + 2);
         const int position = page >= 0 ? (walk.tile0 + j) * kKvTile + token : 0x7fffffff;
-        const float value_log2 = log2f(scales.y), value_inverse = __frcp_rn(scales.y);
+        const float value_log2 = log2f(scales.y);
         wait(&sm.s_full[buffer], (tile >> 1) & 1);
         tc_fence_after();
         float t[kRows];
@@ -445,13 +461,29 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
           const float m = reduce8<true>(t + r0, lane);
           if ((lane & 3) == 0) sm.part[buffer][r0 + reduce8_slot(lane)][quarter] = m;
         }
-        softmax_barrier();
-        auto tile_top = [&](int r) {
-          const float4 m = *reinterpret_cast<const float4*>(sm.part[buffer][r]);
-          return fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
-        };
+        const bool was_apart = apart;
+        apart = softmax_barrier_or(apart || (page >= 0 && fabsf(value_log2 - first) > kKvApart));
+        if (__builtin_expect(apart, 0)) {
+#pragma unroll
+          for (int r0 = 0; r0 < kRows; r0 += 8) {
+            float s[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = t[r0 + i] - value_log2;
+            const float m = reduce8<true>(s, lane);
+            if ((lane & 3) == 0) sm.low[r0 + reduce8_slot(lane)][quarter] = m;
+          }
+          softmax_barrier();
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            const float from = was_apart ? low[r] : top[r] - first;
+            low[r] = fmaxf(from, max4(sm.low[r]));
+            if (from != low[r]) weights[r] *= fast_exp2(from - low[r]);
+            weights[r] += fast_exp2(t[r] - value_log2 + (kWeightExponent - (low[r] == -INFINITY ? 0.0f : low[r])));
+          }
+        }
+        const float value_inverse = apart ? 0.0f : fast_exp2(first - value_log2);
         auto grown = [&](int r) {          // the reference maximum after this tile
-          const float m = tile_top(r);
+          const float m = max4(sm.part[buffer][r]);
           return m > top[r] + kGrow || (top[r] == -INFINITY && m > top[r]) ? m : top[r];
         };
         bool grows = false;                // the same in all threads
@@ -469,7 +501,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
             for (int i = 0; i < 8; ++i) {
               const float to = grown(r0 + i);
               f[i] = top[r0 + i] == to ? 1.0f : fast_exp2(top[r0 + i] - to);
-              weights[r0 + i] *= f[i];
+              if (!apart) weights[r0 + i] *= f[i];
               top[r0 + i] = to;
             }
             if (j > 0) {
@@ -544,7 +576,7 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
           const float4 s4 = *reinterpret_cast<const float4*>(sm.part[last ^ 1][r]);
-          if (r < rows) *kv_part_weight(plan.work, part, r) = make_float2(top[r], (s4.x + s4.y) + (s4.z + s4.w));
+          if (r < rows) *kv_part_weight(plan.work, part, r) = make_float4(top[r], (s4.x + s4.y) + (s4.z + s4.w), apart ? low[r] : top[r] - first, 0.0f);
         }
         // the block of tile t is the last whose cut is not behind it: the one before the first cut at t + 1 or later
         const int first = walk.at - walk.tile0;
@@ -570,7 +602,8 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
             if (whole) {
               const float4 s4 = *reinterpret_cast<const float4*>(sm.part[last ^ 1][r]);
               const float sum = (s4.x + s4.y) + (s4.z + s4.w);
-              a.out[sm.out_at[which][r] + d] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : x / sum);
+              const float2 back = kv_exp2_factors(!apart ? first : top[r] == -INFINITY ? 0.0f : top[r] - low[r]);
+              a.out[sm.out_at[which][r] + d] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : x / sum * back.x * back.y);
             } else {
               kv_part_sum<kDim>(plan.work, part, r, d & ~3)[d & 3] = x;
             }

@@ -2,8 +2,8 @@
 //
 //   t_ij = scale q_i . k_j (log2 units) + log2(value scale of j's page),   w_ij = 2^(t_ij - m_i)
 //   o_i  = sum_j w_ij code(v_j) / sum_j w_ij / (value scale of j's page)
-// as in kv_decode.cu, here with the rows as the M side.  A row tile is up to 128 rows: whole new tokens x the query heads that
-// share a key/value head, so that K and V are loaded once for all of them.
+// as in kv_decode.cu (and the denominator as in kv_attention.cuh), here with the rows as the M side.  A row tile is up to 128 rows:
+// whole new tokens x the query heads that share a key/value head, so that K and V are loaded once for all of them.
 //
 // Bound: the products, 4 x rows x positions x head_dim flops at the rate of 16-bit ones.  Queries and weights are BF16-like, the
 // cache is e4m3, and no operand of mixed width exists.  So Q is split into two 8-bit terms and its product runs twice at twice the rate:
@@ -50,6 +50,7 @@ constexpr float kFall = 16.0f;
 constexpr float kDepth = 30.0f;
 constexpr float kWeightExponent = 9.0f;
 constexpr int kScaleSlots = 4;
+constexpr int kApart = 256;               // of a tile's marks: value scales of the segment so far are far apart
 constexpr int kStageBytes = 32 * 64;      // of a warp: 32 rows x 32 results
 
 template <int kDim>
@@ -69,12 +70,13 @@ struct Prompt {
 };
 
 struct Small {
-  float4 scales[kScaleSlots][8];           // per 16 positions: key scale x softmax scale, log2 and inverse of the value scale, 0: no page
-  int holes[kScaleSlots];                  // whether a page of the tile is missing
+  float4 scales[kScaleSlots][8];           // per 16 positions: key scale x softmax scale, log2 of the value scale, 2^e / value scale (0: far apart)
+  int2 marks[kScaleSlots];                 // a bit for each 16 positions without a page, and kApart; e
   unsigned long long full[8], empty[8], scales_full[kScaleSlots], scales_empty[kScaleSlots];
   unsigned long long s_full[2], p_full[2], o_done[2], q_raw, q_full, q_empty, drain;
   float row_scale[128];
   float half_top[2][2][128];               // per tile parity, half and row
+  float half_low[2][128];                  // scales far apart: the same without them
   float sum[2][2][128];                    // per parity of the unit, half and row
   KvStart cut[2];
   KvShared shared[2];                      // the units divided at the share's begin and at its end
@@ -607,6 +609,8 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
           return s;
         };
         float2 s = fetch(0);
+        int first = 0;                       // exponent of the first value scale
+        bool known = false, apart = false;
         for (int j = 0; j < walk.tiles; ++j, ++tile) {
           const float2 after = fetch(j + 1);
           const int slot = tile % kScaleSlots;
@@ -614,8 +618,14 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
           // positions without a page are marked; their factor only has to be positive
           const bool hole = lane < 8 && s.x == 0.0f;
           const uint32_t holes = __ballot_sync(0xffffffffu, hole);
-          if (lane == 0) sm.holes[slot] = static_cast<int>(holes);
-          if (lane < 8) sm.scales[slot][lane] = make_float4(s.x > 0.0f ? s.x * a.scale_log2 : 1.0f, log2f(s.y), __frcp_rn(s.y), s.x);
+          if (!known && holes != 0xffu) {
+            first = __shfl_sync(0xffffffffu, kv_float_exponent(s.y), __ffs(static_cast<int>(~holes)) - 1);
+            known = true;
+          }
+          const float value_log2 = log2f(s.y), relative = static_cast<float>(first) - value_log2;
+          apart = apart || __any_sync(0xffffffffu, lane < 8 && !hole && fabsf(relative) > kKvApart);
+          if (lane == 0) sm.marks[slot] = make_int2(static_cast<int>(holes) | (apart ? kApart : 0), first);
+          if (lane < 8) sm.scales[slot][lane] = make_float4(s.x > 0.0f ? s.x * a.scale_log2 : 1.0f, value_log2, apart ? 0.0f : fast_exp2(relative), 0.0f);
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&sm.scales_full[slot]));
           s = after;
@@ -710,7 +720,10 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
       }
       const float row_scale = row < rows ? sm.row_scale[row] : 0.0f;
       const int limit = row < rows ? walk.unit.first + row_token(row, group_inverse) : -1;     // last position the row sees
-      float top = -INFINITY, peak = -INFINITY, sum = 0.0f;       // reference and maximum so far; this half's sum of weights
+      float top = -INFINITY, peak = -INFINITY, sum = 0.0f;       // reference and maximum so far; this half's denominator
+      float low = -INFINITY;                                     // the denominator's reference once scales are apart
+      bool apart = false;
+      int first = 0;                                             // e
       float shift = kWeightExponent;                             // less the reference
       for (int j = 0; j < n; ++j, ++tile) {
         const int buffer = tile & 1, slot = tile % kScaleSlots;
@@ -735,8 +748,10 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
         tmem_ld32(scores + half, s);
         tmem_ld32(scores + half + 32, s + 32);
         const float4* scales = sm.scales[slot];
-        const int holes = sm.holes[slot];
-        const bool masked = position0 + kKvTile - 1 > walk.unit.first || holes != 0;
+        const int2 marks = sm.marks[slot];
+        const int holes = marks.x & (kApart - 1);
+        first = marks.y;
+        const bool masked = position0 + kKvTile - 1 > walk.unit.first || marks.x != 0;        // or scales apart
         // positive, so that a masked score stays -inf
         auto factor_of = [&](int g) { return fmaxf(scales[g].x * row_scale, 1.17549435e-38f); };
         auto mask = [&](uint32_t* x, int first) {          // 32 scores from position `first` of the tile on
@@ -767,6 +782,28 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
         if (masked) {
           mask(s, half);
           mask(s + 32, half + 32);
+          if ((marks.x & kApart) != 0) {
+            float s_top = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              float x = __uint_as_float(s[16 * g]);
+#pragma unroll
+              for (int c = 1; c < 16; ++c) x = fmaxf(x, __uint_as_float(s[16 * g + c]));
+              s_top = fmaxf(s_top, x * factor_of(half / 16 + g));
+            }
+            sm.half_low[group][row] = s_top;
+            asm volatile("bar.sync %0, 64;" :: "r"(2 + quarter) : "memory");
+            const float from = apart ? low : top - static_cast<float>(first);
+            low = fmaxf(from, fmaxf(s_top, sm.half_low[group ^ 1][row]));
+            if (from != low) sum *= fast_exp2(from - low);
+            const float low_shift = kWeightExponent - (low == -INFINITY ? 0.0f : low);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+#pragma unroll
+              for (int c = 0; c < 16; ++c) sum += fast_exp2(fmaf(__uint_as_float(s[16 * g + c]), factor_of(half / 16 + g), low_shift));
+            }
+            apart = true;
+          }
         }
         float m = fmaxf(top_of(s, half), top_of(s + 32, half + 32));
         sm.half_top[buffer][group][row] = m;
@@ -795,7 +832,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
               tmem_st32(sums + c, o);
             }
           }
-          sum *= f;
+          if (!apart) sum *= f;
           top = now;
           shift = kWeightExponent - (top == -INFINITY ? 0.0f : top);
         }
@@ -867,7 +904,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
       const bool whole = n == walk.unit.tiles, begins = walk.tile0 == 0;
       const size_t part = kv_part_index(blockIdx.x, begins);
       if (!whole) {
-        if (group == 0 && row < rows) *kv_part_weight(plan.work, part, row) = make_float2(top, total);
+        if (group == 0 && row < rows) *kv_part_weight(plan.work, part, row) = make_float4(top, total, apart ? low : top - static_cast<float>(first), 0.0f);
         if (threadIdx.x == 128) {
           KvShared shared{0, 0, 0, rows, token0, walk.head * shape.group};
           divided_unit(sm.cut[begins ? 1 : 0], walk.unit.tiles, &shared.first_block, &shared.parts);
@@ -875,7 +912,8 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
           sm.shared[begins ? 1 : 0] = shared;
         }
       }
-      const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+      const float2 back = kv_exp2_factors(!apart ? static_cast<float>(first) : top == -INFINITY ? 0.0f : top - low);
+      const float inverse = total == 0.0f ? 0.0f : back.x / total;
       // 32 columns at a time through shared memory, 16-byte pieces XORed with the row, so that every store writes 64 bytes of
       // eight rows.  (Each thread storing its own row took 5 us per unit.)
       uint8_t* stage = generic + L::kStageAt + (warp - 4) * kStageBytes;
@@ -892,7 +930,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
             uint32_t packed[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(x[8 * k + 2 * i]) * inverse, __uint_as_float(x[8 * k + 2 * i + 1]) * inverse);
+              const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(x[8 * k + 2 * i]) * inverse * back.y, __uint_as_float(x[8 * k + 2 * i + 1]) * inverse * back.y);
               packed[i] = *reinterpret_cast<const uint32_t*>(&two);
             }
             *reinterpret_cast<uint4*>(stage + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);

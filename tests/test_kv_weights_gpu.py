@@ -47,3 +47,67 @@ def test_small_weights_of_prompts_keep_their_bits(package, heads, length):
     """The same for many rows, up to where heads of 256 hold the weights beside the largest to 2^-8: 2^-22 of it."""
     for low, high in ((12.0, 16.0), (16.0, 19.0), (19.0, 22.0)) + (((22.0, 26.0),) if heads[2] < 256 else ()):
         _check_attention(*_sink(package, length, 40, heads, (low, high)))
+
+
+def _scaled(package, lengths, new, heads, scales, scores=None, std=1.0, seed=7):
+    """Pages whose value scales are `scales` in turn and whose keys lead to the scores `scores` (log2 units, by scale) above random
+    ones; values between 1/2 and 1 times their scale."""
+    q_heads, kv_heads, dim = heads
+    setup = Setup(package, lengths, [min(new, n) for n in lengths], heads, 64, 0, seed=seed)
+    codes = torch.randn(setup.gpu[0].shape, generator=setup.g) * 16
+    codes[..., 0] = 0.0
+    setup.gpu[2].fill_(2.0 ** -4)
+    for row, length in zip(setup.table.tolist(), lengths):
+        for column in range((length + 63) // 64):
+            at = column % len(scales)
+            setup.gpu[3][row[column]] = scales[at]
+            if scores is not None:
+                codes[row[column], :, :, 0] = scores[at]
+    setup.gpu[0].copy_(codes.to(torch.float8_e4m3fn).cuda())
+    setup.gpu[1].copy_((torch.rand(setup.gpu[1].shape, generator=setup.g) / 2 + 0.5).to(torch.float8_e4m3fn).cuda())
+    q = setup.randn(setup.tokens, q_heads, dim, std=std).float()
+    q[..., 0] = math.log(2.0) * dim ** 0.5 * 16                      # a code of 1 is a score of 1 in log2 units
+    return setup, q.bfloat16()
+
+
+FAR_APART = [
+    [2.0 ** -64, 2.0 ** 63],                                         # a page of zeros beside one of values above 2e21
+    [2.0 ** 63, 2.0 ** -64, 1.0],
+    [2.0 ** 120, 2.0 ** -64],
+    [2.0 ** -64, 2.0 ** -64, 2.0 ** -64, 2.0 ** 120, 1.0],
+    [1.0] * 9 + [2.0 ** 100, 2.0 ** -60],
+    [2.0 ** -33, 1.0, 2.0 ** 33],
+    [2.0 ** -105], [2.0 ** -115], [3.0e-35], [2.0 ** 120], [3.0e35],
+]
+BATCHES = [([1000], 1), ([1000] * 40, 1), ([300] * 90, 2), ([700, 5, 64, 129], 5), ([1000], 40), ([1000] * 12, 40), ([200, 130, 64] * 6, 150)]
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 256), (16, 2, 128), (8, 8, 64)])
+@pytest.mark.parametrize("lengths,new", BATCHES)
+def test_value_scales_far_apart_and_far_from_one(package, lengths, new, heads):
+    """The weights' sum counts every position alike, whatever its value's scale: in one block, and where several join their parts."""
+    for scales in FAR_APART:
+        _check_attention(*_scaled(package, lengths, new, heads, scales))
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 256), (8, 8, 64)])
+@pytest.mark.parametrize("lengths,new", [([1000], 1), ([1000] * 40, 2), ([1000], 40), ([1000] * 12, 40)])
+def test_small_values_that_the_scores_prefer_to_large_ones(package, lengths, new, heads):
+    """The large values' scores are so low that the small ones decide the output, and the other way round."""
+    for scales, scores in (([2.0 ** -64, 2.0 ** 60], [0.0, -208.0]), ([2.0 ** 60, 2.0 ** -64, 2.0 ** -50], [-208.0, 8.0, 0.0]),
+                           ([2.0 ** -64, 2.0 ** 60], [104.0, 0.0]), ([2.0 ** 100, 2.0 ** -20], [-120.0, 0.0]), ([2.0 ** -64, 2.0 ** 100], [160.0, 0.0])):
+        _check_attention(*_scaled(package, lengths, new, heads, scales, scores))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_page_of_zeros_beside_one_of_large_values(package, new):
+    """As append leaves them: the least scale, and one above 2^100."""
+    setup = Setup(package, [256], [256], seed=17, rotary=0)
+    k, v = setup.randn(256, 2, 256, std=0.1), setup.randn(256, 2, 256)
+    v[:64] = 0.0                                                     # scale 2^-64
+    v[128:192] = (v[128:192].float().abs() * 2.0 ** 110).bfloat16()
+    setup.cache.append(1, setup.batch, k.cuda(), v.cuda())
+    q = setup.randn(256, 16, 256)[:new]
+    setup.new, setup.offsets, setup.tokens = [new], [0, new], new
+    setup.batch = setup.make_batch()
+    _check_attention(setup, q)
