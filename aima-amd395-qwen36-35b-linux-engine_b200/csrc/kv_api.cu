@@ -123,13 +123,13 @@ int check_rows(const aima_moe_kv_rows* rows, const char* name, int tokens, int h
   return AIMA_MOE_OK;
 }
 
-// Whether rows of q and the contiguous output share bytes.
-bool overlaps(const aima::KvRows& q, const void* out, const aima::KvShape& shape, int tokens) {
-  const char* q0 = reinterpret_cast<const char*>(q.data);
-  const char* q1 = reinterpret_cast<const char*>(q.data + (tokens - 1) * q.row_stride + (shape.q_heads - 1) * q.head_stride + shape.head_dim);
+// Whether the span of an input's rows and the contiguous output share bytes.
+bool overlaps(const aima::KvRows& x, int heads, const void* out, const aima::KvShape& shape, int tokens) {
+  const char* x0 = reinterpret_cast<const char*>(x.data);
+  const char* x1 = reinterpret_cast<const char*>(x.data + (tokens - 1) * x.row_stride + (heads - 1) * x.head_stride + shape.head_dim);
   const char* o0 = static_cast<const char*>(out);
   const char* o1 = o0 + 2ull * tokens * shape.q_heads * shape.head_dim;
-  return q0 < o1 && o0 < q1;
+  return x0 < o1 && o0 < x1;
 }
 
 int check_launch(aima_moe_kv* h, uint32_t layer) {
@@ -260,7 +260,10 @@ AIMA_EXPORT int aima_moe_kv_append_launch(aima_moe_kv* h, uint32_t layer, const 
   if (q != nullptr && q->data != nullptr) {
     if (const int status = check_rows(q, "q", a.batch.tokens, h->shape.q_heads, h->shape.head_dim, &a.q); status != AIMA_MOE_OK) return status;
     if (q_out == nullptr || misaligned(q_out)) return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: q_out is null or not 16-byte aligned");
-    if (overlaps(a.q, q_out, h->shape, a.batch.tokens)) return kv_fail(AIMA_MOE_ERR_ALIAS, "kv: q_out overlaps q");
+    if (overlaps(a.q, h->shape.q_heads, q_out, h->shape, a.batch.tokens)) return kv_fail(AIMA_MOE_ERR_ALIAS, "kv: q_out overlaps q");
+    // the blocks that write it run beside those that read k and v, twice
+    if (overlaps(a.k, h->shape.kv_heads, q_out, h->shape, a.batch.tokens) || overlaps(a.v, h->shape.kv_heads, q_out, h->shape, a.batch.tokens))
+      return kv_fail(AIMA_MOE_ERR_ALIAS, "kv: q_out overlaps k or v");
     a.q_out = static_cast<__nv_bfloat16*>(q_out);
   }
   if (h->shape.rotary > 0 && h->rotation == nullptr) return kv_fail(AIMA_MOE_ERR_NOT_BOUND, "kv: no rotation table was set");
@@ -283,7 +286,7 @@ AIMA_EXPORT int aima_moe_kv_attention_launch(aima_moe_kv* h, uint32_t layer, con
   if (const int status = check_batch(h, batch, &a.batch); status != AIMA_MOE_OK) return status;
   if (const int status = check_rows(q, "q", a.batch.tokens, h->shape.q_heads, h->shape.head_dim, &a.q); status != AIMA_MOE_OK) return status;
   if (out == nullptr || misaligned(out)) return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: out is null or not 16-byte aligned");
-  if (overlaps(a.q, out, h->shape, a.batch.tokens)) return kv_fail(AIMA_MOE_ERR_ALIAS, "kv: out overlaps q");
+  if (overlaps(a.q, h->shape.q_heads, out, h->shape, a.batch.tokens)) return kv_fail(AIMA_MOE_ERR_ALIAS, "kv: out overlaps q");
   a.out = static_cast<__nv_bfloat16*>(out);
   a.scale_log2 = h->scale_log2;
   a.status = h->status;

@@ -566,7 +566,7 @@ int aima_moe_kv_bind_layer(aima_moe_kv* handle, uint32_t layer, const aima_moe_k
 int aima_moe_kv_set_rotation(aima_moe_kv* handle, const void* table_f32, uint32_t positions);
 
 /* Rotates k by the rows' positions and stores it and v in the cache, one launch; with q (data not NULL) also writes the
- * rotated queries to q_out (BF16 [tokens, q_heads, head_dim], contiguous, may not overlap q).
+ * rotated queries to q_out (BF16 [tokens, q_heads, head_dim], contiguous; it may not overlap the span of q, k or v).
  * Per page and head the scale is the least power of two, from 2^-64 on, that keeps every element within e4m3's 448.  A page
  * that held tokens before keeps its scale unless a new token needs a larger one; then the older codes are rounded to it.
  * A token that brings a NaN or an infinity to a head (in its rotated key or in its value) is stored there with NaN keys and
