@@ -50,6 +50,22 @@ int kv_fail_cuda(cudaError_t error, const char* what) {
 
 bool misaligned(const void* pointer) { return reinterpret_cast<uintptr_t>(pointer) % 16 != 0; }
 
+// A device that is the current one for the span of a call: the default stream belongs to whichever that is.
+struct OnDevice {
+  int before = -1;
+  cudaError_t error;
+  explicit OnDevice(int device) {
+    error = cudaGetDevice(&before);
+    if (error == cudaSuccess && before == device) before = -1;
+    else if (error == cudaSuccess) error = cudaSetDevice(device);
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)cudaSetDevice(before);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+};
+
 int check_config(const aima_moe_kv_config* c) {
   if (c == nullptr) return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: config is null");
   if (c->struct_bytes != sizeof(aima_moe_kv_config))
@@ -299,6 +315,8 @@ AIMA_EXPORT int aima_moe_kv_attention_launch(aima_moe_kv* h, uint32_t layer, con
 AIMA_EXPORT int aima_moe_kv_sync(aima_moe_kv* h) {
   if (h == nullptr) return kv_fail(AIMA_MOE_ERR_INVALID_ARGUMENT, "kv: handle is null");
   std::lock_guard<std::mutex> lock(h->mutex);
+  const OnDevice scope(h->device);
+  if (scope.error != cudaSuccess) return kv_fail_cuda(scope.error, "cudaSetDevice");
   int status = 0;
   cudaError_t error = cudaMemcpyAsync(&status, h->status, sizeof status, cudaMemcpyDeviceToHost, h->last_stream);
   if (error == cudaSuccess) error = cudaStreamSynchronize(h->last_stream);

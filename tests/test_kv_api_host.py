@@ -87,3 +87,21 @@ def test_rotated_queries_may_not_lie_over_any_input(package, lib, tokens):
     assert h.append(tokens, *rows, end) == 0
     assert h.append(tokens, *rows, end - 16) == -4
     assert lib.fake_appends() == before + 3
+
+
+@pytest.mark.parametrize("stream", [None, 4096])
+@pytest.mark.parametrize("bits,status", [(1, -1), (2, -5), (3, -5), (0, 0)])
+def test_sync_reports_a_handle_of_another_device(package, lib, stream, bits, status):
+    """The default stream is that of the current device: what the handle's device has under way there is waited for all the same,
+    and the caller's device stays current."""
+    h = Handle(package, lib, device=1)
+    rows = (4 * ROW, 128, 64), (6 * ROW, 128, 64), (0, 256, 64)
+    assert h.append(1, *rows, 8 * ROW, stream) == 0
+    lib.fake_leave(1, stream, ctypes.addressof(h.status.contents), bits)
+    lib.fake_device(0)
+    assert h.append(1, *rows, 8 * ROW, stream) == -1                          # launches want the handle's device
+    assert lib.aima_moe_kv_sync(h.handle) == status
+    assert lib.fake_current() == 0 and h.status[0] == 0
+    assert lib.aima_moe_kv_sync(h.handle) == 0
+    lib.fake_device(1)
+    assert lib.aima_moe_kv_sync(h.handle) == 0 and lib.fake_current() == 1
