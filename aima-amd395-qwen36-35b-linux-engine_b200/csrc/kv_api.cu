@@ -321,8 +321,9 @@ AIMA_EXPORT int aima_moe_kv_sync(aima_moe_kv* h) {
   cudaError_t error = cudaMemcpyAsync(&status, h->status, sizeof status, cudaMemcpyDeviceToHost, h->last_stream);
   if (error == cudaSuccess) error = cudaStreamSynchronize(h->last_stream);
   if (error == cudaSuccess && status != 0) {
-    // after a wait that ran out the counters of the joins may be anything
-    error = cudaMemsetAsync(h->status, 0, 256 + aima::kv_counter_bytes(), h->last_stream);
+    // after a wait that ran out the counters of the joins may be anything; else they are left to what may be under way elsewhere
+    const size_t bytes = (status & aima::kKvTimeout) != 0 ? 256 + aima::kv_counter_bytes() : sizeof status;
+    error = cudaMemsetAsync(h->status, 0, bytes, h->last_stream);
     if (error == cudaSuccess) error = cudaStreamSynchronize(h->last_stream);
   }
   if (error != cudaSuccess) return kv_fail_cuda(error, "kv sync");

@@ -587,7 +587,8 @@ int aima_moe_kv_attention_launch(aima_moe_kv* handle, uint32_t layer, const aima
 
 /* Synchronises the last stream and reports what launches since the last call found wrong in device-side data:
  * AIMA_MOE_ERR_INVALID_ARGUMENT for a length, row offset or position outside its range (such a sequence was treated as one
- * without tokens) or a page number outside its range (its positions were left out), AIMA_MOE_ERR_TIMEOUT for a bounded wait that ran out. */
+ * without tokens) or a page number outside its range (its positions were left out), AIMA_MOE_ERR_TIMEOUT for a bounded wait that ran out.
+ * Launches on other streams, appends too, are covered if the last one was ordered behind them. */
 int aima_moe_kv_sync(aima_moe_kv* handle);
 int aima_moe_kv_release(aima_moe_kv* handle);
 

@@ -105,3 +105,12 @@ def test_sync_reports_a_handle_of_another_device(package, lib, stream, bits, sta
     assert lib.aima_moe_kv_sync(h.handle) == 0
     lib.fake_device(1)
     assert lib.aima_moe_kv_sync(h.handle) == 0 and lib.fake_current() == 1
+
+
+@pytest.mark.parametrize("bits,left", [(1, 7), (2, 0), (3, 0)])
+def test_sync_puts_the_joins_counters_back_only_after_a_wait_that_ran_out(package, lib, bits, left):
+    """A launch under way on another stream counts on them; a length out of range does not touch them."""
+    h = Handle(package, lib)
+    h.status[0], h.status[64], h.status[64 + 511] = bits, 7, 7
+    assert lib.aima_moe_kv_sync(h.handle) == (-1 if bits == 1 else -5)
+    assert (h.status[0], h.status[64], h.status[64 + 511]) == (0, left, left)
