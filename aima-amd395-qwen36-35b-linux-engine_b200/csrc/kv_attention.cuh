@@ -10,6 +10,9 @@
 namespace aima {
 
 constexpr int kKvTile = 128;            // positions of the cache per step
+// In place of a page number out of range: a box in front of the tensor, which TMA fills with zeros.  The positions are masked, but what
+// lies in V is multiplied by their zero weights, and any page that exists may hold NaN there.
+constexpr int kNoPage = -2;
 constexpr int kKvMaxBlocks = 160;       // blocks of an attention kernel at most (one per SM)
 constexpr int kKvPartRows = 128;
 constexpr int kKvMaxList = 1 << 24;     // tiles (with the units' own cost) of a launch: shares are computed in 32 bits

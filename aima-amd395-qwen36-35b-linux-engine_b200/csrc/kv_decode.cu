@@ -230,26 +230,26 @@ kv_decode_kernel(const __grid_constant__ KvMaps maps, const KvAttentionPlan plan
       const KvSequence seq = kv_sequence(a.batch, shape, walk.sequence);
       const int* table = a.batch.table + static_cast<size_t>(walk.sequence) * a.batch.columns;
       const int pages = (seq.length + shape.page_tokens - 1) >> shape.page_shift;
-      auto page_of = [&](int j) {          // of this lane's box; -1: behind the sequence's last
+      auto page_of = [&](int j) {          // of this lane's box; -1: behind the sequence's last, kNoPage: its table has none
         const int column = ((walk.tile0 + j) << (7 - shape.page_shift)) + my_page;
         if (j >= walk.tiles || lane >= boxes || column >= pages) return -1;
         int page = table[column];
         if (page < 0 || page >= shape.pages) {
           atomicOr(a.status, kKvBadBatch);
-          page = 0;                        // its positions are masked
+          page = kNoPage;
         }
         return page;
       };
       auto issue = [&](bool is_k, int page) {
         const int slot = ring % L::kSlots;
         if (!wait(&sm.empty[slot], ((ring / L::kSlots) & 1) ^ 1)) return false;
-        const int loads = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        const int loads = __popc(__ballot_sync(0xffffffffu, page != -1));
         if (lane == 0) mbar_arrive_expect_tx(smem_u32(&sm.full[slot]), loads * shape.page_tokens * L::kRowBytes);
         __syncwarp();
-        if (page >= 0)
+        if (page != -1)
           tma_load_2d(base + slot * L::kSlotBytes + my_panel * L::kPanelBytes + (my_page << shape.page_shift) * L::kRowBytes,
                       is_k ? &maps.keys : &maps.values, my_panel * L::kRowBytes,
-                      static_cast<int>((static_cast<long long>(page) * shape.kv_heads + walk.head) << shape.page_shift),
+                      page == kNoPage ? -shape.page_tokens : static_cast<int>((static_cast<long long>(page) * shape.kv_heads + walk.head) << shape.page_shift),
                       smem_u32(&sm.full[slot]));
         __syncwarp();
         ++ring;

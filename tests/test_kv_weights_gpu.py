@@ -111,3 +111,38 @@ def test_a_page_of_zeros_beside_one_of_large_values(package, new):
     setup.new, setup.offsets, setup.tokens = [new], [0, new], new
     setup.batch = setup.make_batch()
     _check_attention(setup, q)
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 256), (16, 2, 128), (8, 8, 64)])
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("bad", ["too large", "negative"])
+def test_positions_of_a_page_out_of_range_are_left_out(package, heads, new, bad):
+    """Whatever the pages that exist hold: all that is of no sequence is NaN here, the first page among it."""
+    setup = Setup(package, [150, 90], [new, new], heads, 64, 0, seed=33)
+    spare = int(setup.unused[0])
+    used = torch.arange(setup.columns)[None, :] < torch.tensor([[3], [2]])
+    setup.table[used & (setup.table == 0)] = spare                    # the first page is nobody's
+    nobody = torch.ones(len(setup.gpu[0]), dtype=torch.bool)
+    nobody[setup.table[used].long()] = False
+    for which in (0, 1):
+        setup.gpu[which].view(torch.uint8)[nobody.cuda()] = 0x7F
+    q = setup.randn(setup.tokens, heads[0], heads[2])
+    table = setup.table.clone()
+    table[0, 1] = len(setup.gpu[0]) if bad == "too large" else -1
+    setup.table, whole = table, setup.table
+    setup.batch = setup.make_batch()
+    out = setup.cache.attention(1, setup.batch, q.cuda())
+    with pytest.raises(package.AimaMoeError) as error:
+        setup.cache.sync()
+    assert error.value.status == -1
+    # the same sequence without the page: its new rows lie behind it
+    setup.table = whole.clone()
+    setup.table[0, 1] = whole[0, 2]
+    setup.lengths[0] -= 64
+    setup.batch = setup.make_batch()
+    _check_attention(setup, q)
+    codes = [t.cpu().float() for t in setup.gpu]
+    import kv_oracle
+
+    want, spread = kv_oracle.attention(*codes, setup.table.tolist(), setup.offsets, setup.lengths, q, heads[2] ** -0.5, 64)
+    assert ((out.cpu().double() - want).abs() <= want.abs() * 2.0 ** -8 + spread * (2.0 ** -8 + 2.0 ** -9)).all()
