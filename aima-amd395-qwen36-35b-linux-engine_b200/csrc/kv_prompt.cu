@@ -315,18 +315,39 @@ __device__ __forceinline__ void plan_list(const KvAttentionPlan& plan, PlanMemor
   }
 }
 
-// For lists of many row tiles: one block writes all cuts.
+// For lists of many row tiles: one block writes all cuts.  (Rows that see nothing are left to the blocks of the next launch, which divide
+// them: here each row tile would be zeroed by the one thread that has it.)
 constexpr int kPlanThreads = 1024;
 __global__ void __launch_bounds__(kPlanThreads)
 kv_plan_kernel(const KvAttentionPlan plan) {
   __shared__ PlanMemory<kPlanThreads> memory;
   pdl_enter();
-  plan_list<kPlanThreads>(
-      plan, memory, 0, plan.blocks, [&](int c, const KvStart& start) { plan.work.starts[c] = start; },
-      [&](int, int row0, int rows) {
-        uint4* out = reinterpret_cast<uint4*>(plan.a.out + static_cast<long long>(row0) * plan.a.shape.q_heads * plan.a.shape.head_dim);
-        for (int i = 0; i < rows * plan.a.shape.q_heads * plan.a.shape.head_dim / 8; ++i) out[i] = make_uint4(0, 0, 0, 0);
-      });
+  plan_list<kPlanThreads>(plan, memory, 0, plan.blocks, [&](int c, const KvStart& start) { plan.work.starts[c] = start; }, [](int, int, int) {});
+}
+
+// Zeroes the row tiles that see nothing, this block's share of each sequence's: the first rows of one that has more rows than positions.
+// Called by all threads; `memory` holds 2 * AIMA_MOE_KV_MAX_SEQUENCES + 1 numbers.
+template <int kDim, int kThreadCount>
+__device__ __forceinline__ void zero_unseen(const KvAttentionPlan& plan, int* memory) {
+  if (threadIdx.x == 0) memory[0] = 0;
+  __syncthreads();
+  for (int s = threadIdx.x; s < plan.a.batch.sequences; s += kThreadCount) {
+    const KvSequence seq = kv_sequence(plan.a.batch, plan.a.shape, s);
+    const int rows = seq.length <= 0 ? seq.rows : max(0, seq.rows - seq.length) / plan.tile_tokens * plan.tile_tokens;
+    if (rows > 0) {
+      const int at = atomicAdd(memory, 1);
+      memory[1 + 2 * at] = seq.row0;
+      memory[2 + 2 * at] = rows;
+    }
+  }
+  __syncthreads();
+  const int count = memory[0], blocks = gridDim.x;
+  for (int i = 0; i < count; ++i) {
+    const int row0 = memory[1 + 2 * i], rows = memory[2 + 2 * i];
+    const int block = static_cast<int>((blockIdx.x + static_cast<uint32_t>(row0)) % gridDim.x);       // not the same few for every short one
+    const int begin = static_cast<int>(static_cast<long long>(rows) * block / blocks), end = static_cast<int>(static_cast<long long>(rows) * (block + 1) / blocks);
+    if (begin < end) kv_zero_rows<kDim, kThreadCount>(plan.a, row0 + begin, end - begin);
+  }
 }
 
 // The unit that cut `cut` divides: its blocks.  Cut c lies at total c / blocks, and divides a unit if it leaves more than
@@ -385,6 +406,8 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
   Walk walk;
   if (kPlanned) {
     if (threadIdx.x < 2) sm.cut[threadIdx.x] = plan.work.starts[blockIdx.x + threadIdx.x];
+    zero_unseen<kDim, kThreads>(plan, reinterpret_cast<int*>(generic));        // in the place of the first tiles
+    fence_async_proxy();
   } else {
     // in the place of the first tiles
     PlanMemory<kThreads>& memory = *reinterpret_cast<PlanMemory<kThreads>*>(generic);
@@ -985,6 +1008,7 @@ cudaError_t launch_planned(const KvAttentionPlan& plan, const KvMaps& maps, cons
   constexpr int bytes = kv_smem_bytes(Prompt<kDim>::kSmallAt + static_cast<int>(sizeof(Small)) + 1024);
   static_assert(bytes <= 227 * 1024, "more shared memory than a block can have");
   static_assert(sizeof(PlanMemory<kThreads>) + 8 * kThreads <= Prompt<kDim>::kQueryAt, "the plan lies in the ring");
+  static_assert(4 * (2 * AIMA_MOE_KV_MAX_SEQUENCES + 1) <= Prompt<kDim>::kQueryAt, "so do the sequences with rows that see nothing");
   const cudaError_t error = opt_in_dynamic_smem<kv_prompt_kernel<kDim, kPlanned>>(bytes);
   if (error != cudaSuccess) return error;
   return launch_resident(kv_prompt_kernel<kDim, kPlanned>, dim3(plan.blocks), dim3(kThreads), bytes, stream, maps, queries, plan);
