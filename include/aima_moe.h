@@ -599,7 +599,8 @@ int aima_moe_kv_release(aima_moe_kv* handle);
  * max(p_a - q_a, 0), by u_n: weights are taken as whole multiples of 2^-40 and summed as integers, and the token is the lowest
  * whose running sum exceeds floor(total * floor(2^24 u_n) / 2^24), so the result does not depend on any order of summation.
  * If nothing of the weights is left, p_a itself is used; if that is zero too, the token is -1.  A draft outside the
- * vocabulary is rejected.  NaN and negative probabilities count as 0, u is clamped to [0, 1).
+ * vocabulary is rejected.  NaN and negative probabilities count as 0, and so do such u_i; a u_i of 1 or more is compared as it is.
+ * u_n is clamped to [0, 1).
  * accepted [sequences]; tokens [sequences, max_drafts + 1]: the accepted drafts, the token drawn, then -1; new_lengths
  * [sequences] = cache_lengths - (n - a), the cache's lengths without the rejected drafts (both NULL or neither; in place is fine). */
 typedef struct aima_moe_verify_drafts {
