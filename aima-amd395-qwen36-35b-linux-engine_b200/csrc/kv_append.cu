@@ -2,7 +2,8 @@
 //
 //   rot(x)[j]     = x[j] cos_j - x[j + h] sin_j
 //   rot(x)[j + h] = x[j + h] cos_j + x[j] sin_j        j < h = rotary / 2, the rest of a head passes through
-//   scale         = 2^e, e the least integer with max|x| <= 448 * 2^e over the page's rows of a head
+//   scale         = 2^e, e the least integer with max|x| <= 448 * 2^e over the page's new rows of a head; a page that holds older
+//                   rows keeps the scale it has while the new ones fit
 //   code          = e4m3(x / scale)
 // in FP32, every product, difference and sum rounded on its own.  One rounding leads from the rotated key to its code.
 //
@@ -54,10 +55,11 @@ __device__ __forceinline__ uint2 codes8(const float* x, float inverse) {
   }
   return make_uint2(w[0], w[1]);
 }
-// exponent of the power of two that is not below a scale
-__device__ __forceinline__ int exponent_of(float scale) {
+
+// 1 / scale; powers of two, which is what an append writes, by their exponent
+__device__ __forceinline__ float inverse_of(float scale) {
   const int bits = __float_as_int(scale);
-  return min(max(((bits >> 23) & 255) - 127 + ((bits & 0x7fffff) != 0 ? 1 : 0), kKvMinExponent), kKvMaxExponent);
+  return (bits & 0x7fffff) == 0 && bits > 0 && bits < (254 << 23) ? __int_as_float((254 << 23) - bits) : __frcp_rn(scale);
 }
 
 // A vector that this thread has read before; the compiler would keep the first one in registers.
@@ -240,21 +242,21 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
       old_scale[1] = a.layer.value_scales[scale_at];
     }
     __syncthreads();
-    int exponent[2];
+    float scale[2], inverse[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       float m = warp_amax[t][0];
 #pragma unroll
       for (int w = 1; w < kAppendThreads / 32; ++w) m = fmaxf(m, warp_amax[t][w]);
-      exponent[t] = kv_scale_exponent(m);
-      if (held) exponent[t] = max(exponent[t], exponent_of(old_scale[t]));
+      // a scale that the page came with stays as it is while the new rows fit, whether it is a power of two or not
+      scale[t] = held && m <= 448.0f * old_scale[t] ? old_scale[t] : kv_exp2(kv_scale_exponent(m));
+      inverse[t] = inverse_of(scale[t]);
     }
     if (threadIdx.x == 0) {
-      a.layer.key_scales[scale_at] = kv_exp2(exponent[0]);
-      a.layer.value_scales[scale_at] = kv_exp2(exponent[1]);
+      a.layer.key_scales[scale_at] = scale[0];
+      a.layer.value_scales[scale_at] = scale[1];
     }
     const size_t base = scale_at * kPage * kDim;
-    const float kinv = kv_exp2(-exponent[0]), vinv = kv_exp2(-exponent[1]);
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int slot = slot0 + p * kRowsPerPass, position = page_start + slot;
@@ -271,7 +273,7 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
       rotate8<kDim>(kagain, piece, half, angles, active, k);
       unpack8(vagain, v);
       if (active) {
-        uint2 kc = codes8(k, kinv), vc = codes8(v, vinv);
+        uint2 kc = codes8(k, inverse[0]), vc = codes8(v, inverse[1]);
         if ((poisoned >> p) & 1u) {
           kc = make_uint2(kKvNan * 0x01010101u, kKvNan * 0x01010101u);
           vc = make_uint2(0, 0);
@@ -282,8 +284,8 @@ kv_append_kernel(const KvAppend a, int page_blocks, int columns_per_sequence) {
         // an older token: to the larger scale, where there is one
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float ratio = old_scale[t] * kv_exp2(-exponent[t]);
-          if (ratio == 1.0f) continue;
+          if (scale[t] == old_scale[t]) continue;
+          const float ratio = old_scale[t] * inverse[t];
           uint2* at = reinterpret_cast<uint2*>((t == 0 ? a.layer.keys : a.layer.values) + base + slot * kDim + 8 * piece);
           const uint2 codes = *at;
           float x[8];

@@ -63,15 +63,15 @@ def append(keys, values, key_scales, value_scales, table, offsets, lengths, k, v
         sound = [(slot, a, b) for slot, a, b in entry["rows"] if bool(torch.isfinite(a).all() and torch.isfinite(b).all())]
         for which, codes, scales in ((1, keys, key_scales), (2, values, value_scales)):
             amax = max((float(r[which].abs().max()) for r in sound), default=0.0)
-            e = exponent_for(amax)
-            old = float(scales[page, h])
-            if held > 0:
-                e = max(e, math.frexp(old)[1] - 1)
-                codes[page, h, :held] = e4m3(codes[page, h, :held] * (old * 2.0 ** -e))
+            scale, old = 2.0 ** exponent_for(amax), float(scales[page, h])
+            if held > 0 and amax <= LARGEST * old:
+                scale = old                                       # the page keeps the one it has
+            elif held > 0:
+                codes[page, h, :held] = e4m3(codes[page, h, :held] * (old / scale))
             entry["amax%d" % which] = amax
-            scales[page, h] = 2.0 ** e
+            scales[page, h] = scale
             for r in entry["rows"]:
-                codes[page, h, r[0]] = e4m3(r[which] * 2.0 ** -e)
+                codes[page, h, r[0]] = e4m3(r[which] / scale)
         for slot, a, b in entry["rows"]:
             if not bool(torch.isfinite(a).all() and torch.isfinite(b).all()):
                 keys[page, h, slot] = math.nan
