@@ -7,10 +7,12 @@
 namespace aima {
 namespace {
 
-// Up to here the few-row kernel.  us with it and with the prompt kernel: 8 rows, one sequence of 32768 positions 15.1 and 22.6, 64
-// of up to 8192 78 and 107; 16 rows, 64 of up to 8192 96 and 123, with heads of 128 278 and 274.  In a form that took 40 rows it
-// needed 138 for 16 sequences of 4111, where the prompt kernel needs 27.
-constexpr int kDecodeRows = 16;
+// Up to so many rows the few-row kernel.  us with it and with the prompt kernel, heads of 256: 8 rows, one sequence of 32768 positions 15.8
+// and 22.8, 64 of up to 8192 78 and 110; 16 rows 23.4 and 31, 103 and 110 .. 122, but 16 of 4111 31 and 26.  Heads of 128, 64 of up
+// to 8192: 8 rows 195 and 231 .. 264, 16 rows 285 and 234 .. 261, 16 rows and 16 of 4111 54 and 46.  Heads of 64, 64 of up to 8192: 8 rows
+// 193 and 207, 16 rows 309 and 207, one of 32768 36 and 30.  In a form that took 40 rows it needed 138 for 16 sequences of 4111, where
+// the prompt kernel needs 29.
+constexpr int decode_rows(int head_dim) { return head_dim == 256 ? 16 : 8; }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
@@ -78,7 +80,7 @@ cudaError_t kv_attention(const KvAttention& a, const KvMaps& maps, void* workspa
   plan.tile_tokens = kKvTile / a.shape.group;
   plan.query_map = kv_query_map_fits(a.q);
   plan.wait_limit_ns = kWaitBudgetNs;
-  return plan.tile_rows <= kDecodeRows ? kv_decode(plan, maps, stream) : kv_prompt(plan, maps, stream);
+  return plan.tile_rows <= decode_rows(a.shape.head_dim) ? kv_decode(plan, maps, stream) : kv_prompt(plan, maps, stream);
 }
 
 }  // namespace aima

@@ -656,8 +656,12 @@ cudaError_t launch(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t
 
 template <int kDim>
 cudaError_t launch_rows(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
-  // N of the products: 8 rows in the kernel for 16 take 18.6 us instead of 15.0 (one sequence of 32768), 90 instead of 78 (64 of 8192)
-  return plan.tile_rows <= 8 ? launch<kDim, 8>(plan, maps, stream) : launch<kDim, 16>(plan, maps, stream);
+  // N of the products: 8 rows in the kernel for 16 take 18.6 us instead of 15.0 (one sequence of 32768), 90 instead of 78 (64 of 8192).
+  // Heads of 64 and 128 come with 8 rows at most.
+  if constexpr (kDim == 256) {
+    if (plan.tile_rows > 8) return launch<kDim, 16>(plan, maps, stream);
+  }
+  return launch<kDim, 8>(plan, maps, stream);
 }
 
 }  // namespace
