@@ -146,3 +146,31 @@ def test_positions_of_a_page_out_of_range_are_left_out(package, heads, new, bad)
 
     want, spread = kv_oracle.attention(*codes, setup.table.tolist(), setup.offsets, setup.lengths, q, heads[2] ** -0.5, 64)
     assert ((out.cpu().double() - want).abs() <= want.abs() * 2.0 ** -8 + spread * (2.0 ** -8 + 2.0 ** -9)).all()
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 256), (16, 2, 128), (8, 8, 64)])
+@pytest.mark.parametrize("length,new", [(300, 1), (257, 2), (300, 30), (385, 140), (1030, 20)])
+def test_no_position_is_dropped_or_added(package, heads, length, new):
+    """Equal scores, and one position that has a value: a row that sees it returns its share of that value, the others return zero."""
+    setup = Setup(package, [length, 130], [new, min(new, 20)], heads, 64, 0, seed=length)
+    q = torch.zeros(setup.tokens, heads[0], heads[2]).bfloat16()
+    last = length - 1
+    for position in sorted({0, 1, 63, 64, 127, 128, 255, 256, last - new, last - new + 1, last - new // 2, last - 1, last} & set(range(length))):
+        setup.gpu[1].zero_()
+        setup.gpu[1][int(setup.table[0, position // 64]), :, position % 64] = 96.0
+        _check_attention(setup, q)
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 256), (32, 8, 128), (8, 8, 64)])
+@pytest.mark.parametrize("lengths,new", [([4000, 700, 33], 1), ([4000, 700, 33], 2), ([2500, 700], 40), ([900], 600)])
+def test_distance_from_64_bits(package, heads, lengths, new):
+    """Off by the output's rounding to BF16, 2^-9.2 of the norm, and by the weights', of at most 2^-8.7 / sqrt(3) each: by 0.0022 of the
+    norm together where a row sees few positions, less where it sees many."""
+    import kv_oracle
+
+    setup = Setup(package, lengths, [min(new, n) for n in lengths], heads, 64, 0, seed=sum(lengths))
+    q = setup.randn(setup.tokens, heads[0], heads[2], std=1.5).cuda()
+    want, _ = kv_oracle.attention(*(t.float() for t in setup.gpu), setup.table.tolist(), setup.offsets, setup.lengths, q, heads[2] ** -0.5, 64)
+    got = setup.cache.attention(1, setup.batch, q).double()
+    setup.cache.sync()
+    assert float((got - want).norm() / want.norm()) <= 0.0022
