@@ -95,8 +95,8 @@ __device__ __forceinline__ void kv_arrive(const KvWorkspace& work, const KvShare
 // are written; the wait has its limit all the same.  A result is four neighbouring elements of a row.  Few parts (a row tile of a
 // prompt in two or three blocks): a thread keeps to one row, so that the parts' factors are found once, and all blocks share the
 // columns.  Many parts (one token's few rows in 74 blocks): 4 .. 32 lanes share the parts of a result.  Either way in the same
-// order in every launch.  512 tokens of 4096 (2 or 3 parts of 128 rows) 51 us by rows and 94 by lanes, 16 x 40 rows of 4111 (4 .. 6
-// parts) 26.7 and 32.5, 10 sequences of 4000 19.7 and 20.5; with 74 parts a row's factors alone would be 74 loads per thread.
+// order in every launch.  512 tokens of 4096 (2 or 3 parts of 128 rows) 51 us by rows and 100 by lanes, 16 x 40 rows of 4111 (4 .. 6
+// parts) 28.7 and 35.4, 10 x 40 rows of 4000 22.6 and 25.7; with 74 parts a row's factors alone would be 74 loads per thread.
 template <int kDim, int kThreads>
 __device__ __forceinline__ void kv_join(const KvAttention& a, const KvWorkspace& work, const KvShared& unit, unsigned long long limit_ns, int* verdict) {
   unsigned* arrived = work.arrived + 2 * unit.first_block;

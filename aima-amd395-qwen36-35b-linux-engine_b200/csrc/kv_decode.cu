@@ -22,8 +22,9 @@
 // write the results.  S is double-buffered: the product of the next tile runs under the softmax of this one.  The running
 // maximum moves only when a tile's exceeds it by more than kGrow, so the accumulators are rarely rescaled.
 //
-// Measured: 64 sequences of up to 8192 positions, one token, 16/2 heads of 256 (406 MB) 77.7 us = 5.2 TB/s, 80 % of a copy; one sequence
-// of 32768 14.9 us, of which the tiles are 3 and the rest is a chain: cuts, queries, first scores, results, join.
+// Measured: 64 sequences of up to 8192 positions, one token, 16/2 heads of 256 (406 MB) 78 us = 5.2 TB/s, 80 % of a copy; two tokens 103:
+// the softmax threads, which also bound heads of 128 (32/8, one token 190 us) and 64 (8/8, 188 us); one sequence of 32768 15.9 us, of which the
+// tiles are 3 and the rest is a chain: cuts, queries, first scores, results, join.
 #include "kv_attention.cuh"
 
 namespace aima {
@@ -656,7 +657,7 @@ cudaError_t launch(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t
 
 template <int kDim>
 cudaError_t launch_rows(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
-  // N of the products: 8 rows in the kernel for 16 take 18.6 us instead of 15.0 (one sequence of 32768), 90 instead of 78 (64 of 8192).
+  // N of the products: 8 rows in the kernel for 16 take 20.6 us instead of 16.0 (one sequence of 32768), 96 instead of 79 (64 of 8192).
   // Heads of 64 and 128 come with 8 rows at most.
   if constexpr (kDim == 256) {
     if (plan.tile_rows > 8) return launch<kDim, 16>(plan, maps, stream);

@@ -16,7 +16,8 @@
 //   w 2^9   = one f16                        to 2^-11 of itself down to 2^-23 of the largest
 // with V's codes as f16, which they are exactly, in a second pair of buffers (heads of 256 would need 128 KB for them).  That saves the
 // softmax 13 of 23 instructions per four weights and the tensor cores a third of the second product; the softmax warps widen V on
-// the way.  4096 tokens of 16384 with 32/8 heads of 128 1235 us in three terms and 1090 this way, with 8/8 of 64 275 and 242.
+// the way.  4096 tokens of 16384 with 32/8 heads of 128 1235 us in three terms and 1090 this way, with 8/8 of 64 275 and 242 (both before
+// the denominator had a reference of its own: now 1090 .. 1113 and 239 .. 249).
 // All terms of an operand go into one accumulator.  S[128 rows, 128 positions] = Q K^T with both operands in shared memory;
 // O[128, head_dim] += W V with W in tensor memory, where it takes the place of the scores it was made from, and V MN-major.
 //
@@ -24,11 +25,11 @@
 // row) each turn half of a tile's scores into weights; two warps with the same rows exchange their maxima in between.
 // The scores are double-buffered: the products of one tile run under the softmax of another.
 //
-// Measured: 8192 tokens of 32768 with 16/2 heads of 256 3.74 ms = 1.03 PFLOP/s at the 1.5 GHz that the power cap leaves, 2560 cycles
+// Measured: 8192 tokens of 32768 with 16/2 heads of 256 3.75 ms = 1.03 PFLOP/s at the 1.5 GHz that the power cap leaves, 2560 cycles
 // of products in the 3300 of a tile: both operands of Q K^T come from shared memory at its full rate while the next tiles are
 // written there.  With heads of 128 a tile takes 2200 cycles, which its softmax needs (a chain of V's widening, maxima, an exchange and 64
-// weights per thread on two warps per scheduler), the products 1050: 7 prompts of 1531 .. 2999 with 32/8 heads 352 us.  1024
-// tokens of 16/2 heads of 256 alone 27 us, most of it before the first tile and after the last.
+// weights per thread on two warps per scheduler), the products 1050: 7 prompts of 1531 .. 2999 with 32/8 heads 354 us.  1024
+// tokens of 16/2 heads of 256 alone 28 us, most of it before the first tile and after the last.
 #include "kv_attention.cuh"
 
 namespace aima {
@@ -212,9 +213,10 @@ __device__ __forceinline__ void split_weights(uint32_t h0, uint32_t h1, uint32_t
 // Cuts the list into shares of equal cost.  The list runs over sequences, their row tiles, the key/value heads and the
 // tiles of the cache; a unit costs its tiles and kUnitCost more, for its queries, the first scores that nothing overlaps and
 // its results.  A cut within kv_snap tiles of a unit's end moves there: a divided unit costs all that twice, and the join.  Units
-// that several cuts divide anyway are left closer to equal shares (of no more than one tile: 16 sequences x 40 rows of 4111 27.4 us
-// and 30.8 with two; 1024 tokens, whose units of 1 .. 8 tiles two tiles keep whole, 27.3 and 38.1 with one).  One block; items are row tiles, one for a thread at a time.  emit(c, start) is called for the cuts c in
-// [cut0, cut1], by some thread; nothing(row0, rows) for an item whose rows see nothing.
+// that several cuts divide anyway are left closer to equal shares (of no more than one tile: 16 sequences x 40 rows of 4111 28.7 us
+// and 31.0 with two; 1024 tokens, whose units of 1 .. 8 tiles two tiles keep whole, 27.9 and 36.9 with one).  One block; items are row
+// tiles, one for a thread at a time.  emit(c, start) is called for the cuts c in [cut0, cut1], by some thread; nothing(item, row0, rows)
+// for an item whose rows see nothing.
 constexpr int kUnitCost = 3;
 __device__ __forceinline__ int kv_snap(int tiles, int total, int blocks) { return static_cast<long long>(tiles) * blocks <= 2ll * total ? 2 : 1; }
 template <int kThreadCount>
@@ -592,7 +594,7 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
       // A BF16 row of a head is as long as its two terms together and goes where they will lie, kRowBytes at a time, so that it
       // can be converted in place.  Rows behind the unit's last are another unit's or zeros; their results go nowhere.  Queries
       // whose strides a tensor map cannot have are read from where they are by the warps that convert them, which waits for
-      // memory four times per unit: 1024 tokens 28.5 us instead of 27.0, no difference from some thousands of positions on.
+      // memory four times per unit: 1024 tokens 29.5 us instead of 27.9, no difference from some thousands of positions on.
       int segment = 0;
       for (; walk.next(); ++segment, walk.advance()) {
         if (!wait(&sm.q_empty, (segment & 1) ^ 1)) break;
@@ -1017,7 +1019,7 @@ cudaError_t launch_planned(const KvAttentionPlan& plan, const KvMaps& maps, cons
 template <int kDim>
 cudaError_t launch(const KvAttentionPlan& plan, const KvMaps& maps, cudaStream_t stream) {
   // Row tiles at most.  With one for each thread of a block every block can find its share by itself, which saves a launch: 1024
-  // tokens 27.0 us and 30.0 with the plan kernel, 4096 tokens 165 with either.
+  // tokens 27.9 us and 31.7 with the plan kernel, 4096 tokens 160 .. 164 with either.
   const long long items = plan.a.batch.tokens / plan.tile_tokens + plan.a.batch.sequences;
   CUtensorMap queries{};
   if (plan.query_map && !kv_make_query_map(plan.a, plan.tile_tokens, &queries)) return cudaErrorInvalidValue;

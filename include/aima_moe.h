@@ -487,15 +487,17 @@ int aima_moe_image_scatter_ingest(const char* lane0_path, const char* lane1_path
                                   aima_moe_image_ingest_result* result);
 
 /* ---------------------------------------------------------------------------
- * Full-attention cache.  What a host needs on the attention side of a full-attention layer (10 of the 40 layers: 16 query
- * heads, 2 key/value heads of 256, 64 of them rotated) between its fused input projection and its output projection: the
- * counterpart of the reference's head rotation, KV append and grouped decode attention
- * (native/src/native_full_attention.hip.cpp) and of the causal prefill provider
- * (benchmarks/shape-lab/native/src/qrt_ck_fmha_q8192_provider.cpp), over a cache that is paged and held in 8 bits.
+ * Full-attention cache.  The attention side of a full-attention layer (10 of the 40 layers: 16 query heads, 2 key/value heads
+ * of 256, 64 of them rotated) from the rotation to the attention's output: the counterpart of the reference's head rotation,
+ * KV append and grouped decode attention (native/src/native_full_attention.hip.cpp) and of the causal prefill provider
+ * (benchmarks/shape-lab/native/src/qrt_ck_fmha_q8192_provider.cpp), over a cache that is paged and held in 8 bits.  The model's
+ * norm of each query's and key's head, between the input projection and the rotation, is the caller's, as are the output gate
+ * and the projections.
  *
  * Layout, caller-owned, per layer: keys and values [pages, kv_heads, page_tokens, head_dim] in e4m3 (one byte each), and for
  * each an FP32 scale [pages, kv_heads]: the element stands for its code times the scale of its page and head.
- * aima_moe_kv_append_launch writes powers of two as scales; the attention takes any positive finite scale.
+ * aima_moe_kv_append_launch writes powers of two as scales; the attention takes any positive finite scale, and scales of any
+ * distance from each other in one sequence.
  *
  * A batch names, for every sequence, its pages (page_table, page i holds positions [i * page_tokens, ...)), the number of
  * tokens in the cache once the new ones are in it (lengths), and the rows of q, k and v that are its new tokens
@@ -568,7 +570,8 @@ int aima_moe_kv_set_rotation(aima_moe_kv* handle, const void* table_f32, uint32_
 /* Rotates k by the rows' positions and stores it and v in the cache, one launch; with q (data not NULL) also writes the
  * rotated queries to q_out (BF16 [tokens, q_heads, head_dim], contiguous; it may not overlap the span of q, k or v).
  * Per page and head the scale is the least power of two, from 2^-64 on, that keeps every element within e4m3's 448.  A page
- * that held tokens before keeps its scale unless a new token needs a larger one; then the older codes are rounded to it.
+ * that held tokens before keeps its scale, whatever it is, unless a new token needs a larger one; then the older codes are
+ * rounded to it.
  * A token that brings a NaN or an infinity to a head (in its rotated key or in its value) is stored there with NaN keys and
  * zero values: every query that sees it gets NaN, and no other does.
  * The pages that the new tokens go to belong to one sequence each. */
