@@ -3,8 +3,9 @@ the verification of drafted tokens in the loop they are made for.
 
     python examples/speculative_decode.py [--sequences 4] [--layers 2] [--prompt 1000] [--drafts 4] [--steps 16]
 
-Each layer is the model's full-attention layer (16 query heads, 2 key/value heads of 256, 64 of them rotated, an output gate)
-with random weights; the draft model is a table of next-token probabilities.  A step feeds every sequence its last token and its
+Each layer is the model's full-attention layer (16 query heads, 2 key/value heads of 256, 64 of them rotated, a norm of each query's
+and key's head before that, an output gate) with random weights; the draft model is a table of next-token probabilities.  The head norm
+and the gate are plain torch: the library has neither.  A step feeds every sequence its last token and its
 drafts in one call, verifies the drafts against the step's probabilities, and takes the rejected ones back by setting the lengths
 to what the verification returns: their keys and values stay in the pages until the next append writes over them.  Nothing in the
 loop waits for the GPU."""
@@ -22,6 +23,12 @@ from __graft_entry__ import load_package  # noqa: E402
 HIDDEN, Q_HEADS, KV_HEADS, HEAD_DIM, ROTARY, PAGE = 2048, 16, 2, 256, 64, 64
 THETA = 1.0e7
 QUERY_COLUMNS, KV_COLUMNS = Q_HEADS * 2 * HEAD_DIM, KV_HEADS * HEAD_DIM      # a head's query, then its gate
+
+
+def head_norm(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """Root mean square norm of each head, in FP32."""
+    x = x.float()
+    return (x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1.0e-6) * (1.0 + weight.float())).bfloat16()
 
 
 class Model:
@@ -43,6 +50,7 @@ class Model:
         self.norms = [torch.zeros(HIDDEN, dtype=torch.bfloat16, device=device) for _ in range(layers + 1)]      # stored less one
         self.qkv = [normal(QUERY_COLUMNS + 2 * KV_COLUMNS, HIDDEN) for _ in range(layers)]
         self.out = [normal(HIDDEN, Q_HEADS * HEAD_DIM) for _ in range(layers)]
+        self.head_norms = [(normal(HEAD_DIM, std=0.1), normal(HEAD_DIM, std=0.1)) for _ in range(layers)]      # of q and k, stored less one
         self.draft_table = torch.softmax(normal(vocabulary, vocabulary, std=1.0, dtype=torch.float32), dim=-1)
 
         columns = (tokens + PAGE - 1) // PAGE
@@ -59,11 +67,12 @@ class Model:
         self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
 
     def projection(self, layer: int, normed: torch.Tensor) -> tuple[torch.Tensor, ...]:
-        """q and its gate [tokens, 16, 256], k and v [tokens, 2, 256]: views of one product's rows."""
+        """q and its gate [tokens, 16, 256], k and v [tokens, 2, 256]; gate and v are views of one product's rows."""
         row = self.moe.gemm(normed, self.qkv[layer])
         q = row[:, :QUERY_COLUMNS].unflatten(1, (Q_HEADS, 2, HEAD_DIM))
         k, v = row[:, QUERY_COLUMNS:].unflatten(1, (2, KV_HEADS, HEAD_DIM)).unbind(1)
-        return q[:, :, 0], q[:, :, 1], k, v
+        q_norm, k_norm = self.head_norms[layer]
+        return head_norm(q[:, :, 0], q_norm), q[:, :, 1], head_norm(k, k_norm), v
 
     def probabilities(self, tokens: torch.Tensor, all_rows: bool) -> torch.Tensor:
         """Next-token probabilities after the tokens [sequences, new], which go into the cache: FP32 [sequences, rows, vocabulary]."""
