@@ -41,11 +41,12 @@ constexpr int kThreads = 384;
 // nothing overflows.
 constexpr float kGrow = 6.75f;            // 2^9 * 2^6.75 = 55109 <= 57344
 // Of three terms the last is subnormal where a weight is small, so a row's first maximum, and one that exceeds all before it by more than
-// kJump, is placed kLift above the reference: the other weights of its tile keep 2^-8 of themselves down to 2^-22.75 of it instead of
+// kJump, is placed kLift above the reference: the other weights of its tile keep 2^-8 of themselves down to 2^-22 of it instead of
 // 2^-18, which shows where one position outweighs all others and brings nothing.  The next time that a row of the warp moves, the
 // others give the lift back, so that ordinary scores, whose maximum grows slowly, rescale once or twice more per unit.  (Always so
-// little room above the maximum: 4096 tokens of 16384 955 -> 1006 us.)
-constexpr float kLift = 4.75f;
+// little room above the maximum: 4096 tokens of 16384 955 -> 1006 us.)  A whole number: the largest weight, which often is a third of
+// the row's, then is a power of two and exact; at 2^13.75 it is rounded up by 2^-9.8, in every row.
+constexpr float kLift = 4.0f;
 constexpr float kJump = 8.0f;
 constexpr float kFall = 16.0f;
 constexpr float kDepth = 30.0f;
@@ -834,13 +835,14 @@ kv_prompt_kernel(const __grid_constant__ KvMaps maps, const __grid_constant__ CU
         sm.half_top[buffer][group][row] = m;
         asm volatile("bar.sync %0, 64;" :: "r"(2 + quarter) : "memory");
         m = fmaxf(m, sm.half_top[buffer][group ^ 1][row]);
+        const bool jumps = m > peak + kJump;
         peak = fmaxf(peak, m);
         const bool falls = m > -INFINITY && fmaxf(m, peak - kDepth) < top - kFall;
         const bool moves = m > top + kGrow || falls;               // the first that is seen is above -inf
         if (__any_sync(0xffffffffu, moves)) {
           float now = top;
           if (falls) now = fmaxf(m, peak - kDepth);
-          else if (moves) now = !L::kWide && m > top + kJump ? m - kLift : m;
+          else if (moves) now = !L::kWide && jumps ? m - kLift : m;
           else if (!L::kWide && peak - top <= kLift) now = fmaxf(top, peak);       // a lift that is given back; a fallen reference stays
           const float f = now != top ? fast_exp2(top - now) : 1.0f;                // top is -inf at first: 0
           if (j > 0) {

@@ -174,3 +174,5 @@ def test_distance_from_64_bits(package, heads, lengths, new):
     got = setup.cache.attention(1, setup.batch, q).double()
     setup.cache.sync()
     assert float((got - want).norm() / want.norm()) <= 0.0022
+    # and not the same way everywhere: ties of the weights' last term go up, 2^-12.5 of a weight on the average
+    assert abs(float((got * want).sum() / want.square().sum()) - 1.0) <= 2.0 ** -11.5
