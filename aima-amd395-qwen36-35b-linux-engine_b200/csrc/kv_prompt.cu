@@ -27,7 +27,7 @@
 //
 // Measured: 8192 tokens of 32768 with 16/2 heads of 256 3.75 ms = 1.03 PFLOP/s at the 1.5 GHz that the power cap leaves, 2560 cycles
 // of products in the 3300 of a tile: both operands of Q K^T come from shared memory at its full rate while the next tiles are
-// written there.  With heads of 128 a tile takes 2200 cycles, which its softmax needs (a chain of V's widening, maxima, an exchange and 64
+// written there.  With heads of 128 a tile takes 2250 cycles, which its softmax needs (a chain of V's widening, maxima, an exchange and 64
 // weights per thread on two warps per scheduler), the products 1050: 7 prompts of 1531 .. 2999 with 32/8 heads 354 us.  1024
 // tokens of 16/2 heads of 256 alone 28 us, most of it before the first tile and after the last.
 #include "kv_attention.cuh"
