@@ -120,3 +120,16 @@ def test_many_row_tiles_in_a_captured_graph(package):
         graph.replay()
         setup.cache.sync()
         _check(setup, q, out, lengths)
+
+
+@pytest.mark.parametrize("heads,new", [((16, 2, 256), 1), ((16, 2, 256), 3), ((8, 8, 64), 5), ((16, 2, 128), 4)])
+def test_as_many_sequences_as_a_batch_can_have(package, heads, new):
+    """1024 sequences, some of them empty, some with fewer positions than rows: few rows, and many with shares from a launch of their own."""
+    g = torch.Generator().manual_seed(new)
+    lengths = torch.randint(0, 260, (1024,), generator=g).tolist()
+    lengths[0], lengths[500], lengths[1023] = 0, 1500, 2
+    setup = Setup(package, lengths, [new] * 1024, heads, 64, 0, seed=new, gap=1)
+    q = setup.randn(setup.tokens, heads[0], heads[2], std=1.5).cuda()
+    out = _run(setup, q)
+    setup.cache.sync()
+    _check(setup, q, out)
