@@ -9,15 +9,18 @@ from .provider import (  # noqa: F401
     AimaMoeError,
     KvBatch,
     KvCache,
+    LinearAttention,
+    LinearBatch,
     MoeLibrary,
     LmHead,
     MoeProvider,
     StripedImage,
+    head_norm,
     library_path,
     load_library,
     verify_drafts,
 )
 from . import synth  # noqa: F401
 
-__all__ = ["AimaMoeError", "KvBatch", "KvCache", "LmHead", "MoeLibrary", "MoeProvider", "StripedImage", "library_path", "load_library", "synth",
+__all__ = ["AimaMoeError", "KvBatch", "KvCache", "LinearAttention", "LinearBatch", "LmHead", "MoeLibrary", "MoeProvider", "StripedImage", "head_norm", "library_path", "load_library", "synth",
            "verify_drafts"]

@@ -1,0 +1,157 @@
+// Linear-attention layers: what their kernels and their C ABI (linear_api.cu) share.
+#pragma once
+
+#include "../../include/aima_moe.h"
+#include "common.cuh"
+#include "kv_cache.cuh"
+
+namespace aima {
+
+constexpr int kLinearDim = AIMA_MOE_LINEAR_HEAD_DIM;
+constexpr int kLinearBadBatch = 1;   // bits of a handle's status word
+constexpr int kLinearTimeout = 2;
+
+struct LinearBatch {
+  const int* slots;        // [sequences]
+  const int* offsets;      // [sequences + 1] or nullptr: max_new rows each
+  const int* lengths;      // [sequences] or nullptr
+  const int* keep;         // [sequences] or nullptr
+  int sequences, tokens, max_new;
+  int slot_count;          // of the handle
+};
+
+// One sequence of a batch as every kernel reads it.  Its numbers come from the device, so they are held to their ranges here: a
+// sequence that breaks them has no rows, and `bad` is set.
+struct LinearSequence {
+  int row0, rows;
+  int slot;                // -1: not there
+  int first;               // its first row that is active: rows before position 0, or of a sequence that is not there, are not
+  int kept;                // rows that enter the state; nothing does unless this is above `first`
+  bool fresh;              // begins with zeros, not with what its slot holds
+  bool bad;
+};
+__device__ __forceinline__ LinearSequence linear_sequence(const LinearBatch& b, int s) {
+  LinearSequence out;
+  out.row0 = b.offsets != nullptr ? b.offsets[s] : s * b.max_new;
+  const int end = b.offsets != nullptr ? b.offsets[s + 1] : out.row0 + b.max_new;
+  out.slot = b.slots[s];
+  const int length = b.lengths != nullptr ? b.lengths[s] : -1;
+  const int kept = b.keep != nullptr ? b.keep[s] : b.max_new;
+  out.rows = end - out.row0;
+  out.bad = out.row0 < 0 || end > b.tokens || out.rows < 0 || out.rows > b.max_new || out.slot < -1 || out.slot >= b.slot_count ||
+            (b.lengths != nullptr && length < 0);
+  if (out.bad) out.row0 = out.rows = 0;
+  out.fresh = b.lengths != nullptr && length <= out.rows;
+  out.first = out.slot < 0 || out.bad ? out.rows : out.fresh ? out.rows - length : 0;
+  out.kept = min(max(kept, 0), out.rows);
+  return out;
+}
+
+// Runs of `per` rows of the sequences, one after the other: how many there can be.
+inline long long linear_runs(const LinearBatch& b, int per) {
+  const long long each = (b.max_new + per - 1) / per;
+  const long long most = each * b.sequences;
+  const long long ragged = (b.tokens + per - 1) / per + static_cast<long long>(b.sequences);
+  return b.offsets != nullptr && each > 1 && ragged < most ? ragged : most;
+}
+// The sequence and the run in it that is number `index` of them, found by a whole block of kThreads threads; false: there is none.
+// Where linear_runs counts each sequence's most, a division says it; else the block adds up the runs of all sequences.
+template <int kThreads>
+__device__ __forceinline__ bool linear_find_run(const LinearBatch& b, int per, int index, int* sequence, int* run) {
+  const int each = (b.max_new + per - 1) / per;
+  if (b.offsets == nullptr || each == 1 || (b.tokens + per - 1) / per + b.sequences >= each * static_cast<long long>(b.sequences)) {
+    *sequence = index / each;
+    *run = index - *sequence * each;
+    return true;
+  }
+  __shared__ int sums[kThreads / 32];
+  __shared__ int found[2];
+  const int t = static_cast<int>(threadIdx.x), lane = t & 31;
+  const int share = (b.sequences + kThreads - 1) / kThreads;
+  const int first = t * share, last = min(first + share, b.sequences);
+  int mine = 0;
+  for (int s = first; s < last; ++s) mine += (linear_sequence(b, s).rows + per - 1) / per;
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += x;
+  }
+  if (lane == 31) sums[t >> 5] = upto;
+  if (t == 0) found[0] = -1;
+  __syncthreads();
+  for (int w = 0; w < (t >> 5); ++w) upto += sums[w];
+  if (upto - mine <= index && index < upto) {
+    int at = upto - mine;
+    for (int s = first; s < last; ++s) {
+      const int runs = (linear_sequence(b, s).rows + per - 1) / per;
+      if (index < at + runs) {
+        found[0] = s;
+        found[1] = index - at;
+        break;
+      }
+      at += runs;
+    }
+  }
+  __syncthreads();
+  *sequence = found[0];
+  *run = found[1];
+  return found[0] >= 0;
+}
+// One block looks all sequences over.
+__device__ __forceinline__ void linear_report(const LinearBatch& b, int* status, int thread, int threads) {
+  for (int s = thread; s < b.sequences; s += threads)
+    if (linear_sequence(b, s).bad) atomicOr(status, kLinearBadBatch);
+}
+
+__device__ __forceinline__ float linear_reciprocal(float x) {
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / (1 + e^-x), to a few units of the last place
+__device__ __forceinline__ float linear_sigmoid(float x) { return linear_reciprocal(1.0f + __expf(-x)); }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+struct LinearConv {
+  LinearBatch batch;
+  int channels, width;
+  const __nv_bfloat16* x;
+  long long x_stride;
+  const __nv_bfloat16* weight;
+  __nv_bfloat16* states;
+  __nv_bfloat16* out;
+  int* status;
+};
+cudaError_t linear_conv(const LinearConv& args, cudaStream_t stream);
+
+struct LinearDelta {
+  LinearBatch batch;
+  int k_heads, v_heads, group;
+  KvRows q, k, v, gate;               // gate.data may be nullptr
+  const __nv_bfloat16* a;
+  const __nv_bfloat16* b;
+  long long a_stride, b_stride;
+  const float* a_log;
+  const float* dt_bias;
+  const __nv_bfloat16* norm_weight;
+  float eps;
+  float* states;
+  __nv_bfloat16* out;                 // may be nullptr
+  int* status;
+};
+cudaError_t linear_step(const LinearDelta& args, cudaStream_t stream);
+
+struct HeadNorm {
+  int tokens, heads, dim, activation;
+  float offset, eps;
+  KvRows x, gate;
+  const __nv_bfloat16* weight;
+  __nv_bfloat16* out;
+};
+cudaError_t head_norm(const HeadNorm& args, cudaStream_t stream);
+
+}  // namespace aima

@@ -144,6 +144,50 @@ class VerifyDrafts(ctypes.Structure):
 _VERIFY_BYTES = ctypes.sizeof(VerifyDrafts)
 
 
+class LinearConfig(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", c_uint32), ("k_heads", c_uint32), ("v_heads", c_uint32), ("head_dim", c_uint32), ("conv_width", c_uint32),
+        ("slots", c_uint32), ("layers", c_uint32), ("max_sequences", c_uint32), ("max_tokens", c_uint32), ("eps", c_float),
+        ("workspace", c_void_p), ("workspace_bytes", c_uint64),
+    ]
+
+
+class LinearLayer(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", c_uint32), ("reserved", c_uint32),
+        ("conv_weight", c_void_p), ("conv_weight_bytes", c_uint64), ("conv_states", c_void_p), ("conv_states_bytes", c_uint64),
+        ("states", c_void_p), ("states_bytes", c_uint64), ("a_log", c_void_p), ("a_log_bytes", c_uint64),
+        ("dt_bias", c_void_p), ("dt_bias_bytes", c_uint64), ("norm_weight", c_void_p), ("norm_weight_bytes", c_uint64),
+    ]
+
+
+class LinearBatchStruct(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", c_uint32), ("sequences", c_uint32), ("tokens", c_uint32), ("max_new_tokens", c_uint32),
+        ("slots", c_void_p), ("row_offsets", c_void_p), ("lengths", c_void_p), ("keep", c_void_p),
+    ]
+
+
+class LinearDelta(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", c_uint32), ("reserved", c_uint32), ("q", KvRows), ("k", KvRows), ("v", KvRows), ("gate", KvRows),
+        ("a", c_void_p), ("b", c_void_p), ("a_row_stride", c_uint64), ("b_row_stride", c_uint64), ("out", c_void_p),
+    ]
+
+
+class HeadNorm(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", c_uint32), ("tokens", c_uint32), ("heads", c_uint32), ("head_dim", c_uint32), ("activation", c_uint32),
+        ("weight_offset", c_float), ("eps", c_float), ("reserved", c_uint32), ("x", KvRows), ("gate", KvRows),
+        ("weight", c_void_p), ("out", c_void_p),
+    ]
+
+
+_LINEAR_DELTA_BYTES, _HEAD_NORM_BYTES = ctypes.sizeof(LinearDelta), ctypes.sizeof(HeadNorm)
+LINEAR_HEAD_DIM = 128
+GATE_ACTIVATIONS = {"none": 0, "silu": 1, "sigmoid": 2}
+
+
 # every symbol include/aima_moe.h declares: (name, restype, argtypes)
 EXPORTS = [
     ("aima_moe_abi_version", c_uint32, []),
@@ -215,6 +259,16 @@ EXPORTS = [
     ("aima_moe_kv_sync", c_int, [c_void_p]),
     ("aima_moe_kv_release", c_int, [c_void_p]),
     ("aima_moe_verify_drafts_launch", c_int, [ctypes.POINTER(VerifyDrafts), c_void_p]),
+    ("aima_moe_linear_query_workspace", c_int, [ctypes.POINTER(LinearConfig), ctypes.POINTER(c_uint64)]),
+    ("aima_moe_linear_prepare", c_int, [ctypes.POINTER(LinearConfig), ctypes.POINTER(c_void_p)]),
+    ("aima_moe_linear_bind_layer", c_int, [c_void_p, c_uint32, ctypes.POINTER(LinearLayer)]),
+    ("aima_moe_linear_conv_launch", c_int,
+     [c_void_p, c_uint32, ctypes.POINTER(LinearBatchStruct), c_void_p, c_uint64, c_void_p, c_void_p]),
+    ("aima_moe_linear_delta_launch", c_int,
+     [c_void_p, c_uint32, ctypes.POINTER(LinearBatchStruct), ctypes.POINTER(LinearDelta), c_void_p]),
+    ("aima_moe_linear_sync", c_int, [c_void_p]),
+    ("aima_moe_linear_release", c_int, [c_void_p]),
+    ("aima_moe_head_norm_launch", c_int, [ctypes.POINTER(HeadNorm), c_void_p]),
     ("aima_moe_sync_metrics", c_int, [c_void_p, ctypes.POINTER(Metrics)]),
     ("aima_moe_release", c_int, [c_void_p]),
 ]
@@ -935,3 +989,213 @@ def _refuse_verification(target: Any, draft_tokens: Any, uniforms: Any, draft_pr
         if name not in ("target", "draft_probabilities") and not tensor.is_contiguous():
             raise RuntimeError("aima_moe tensors must be contiguous CUDA tensors")
     raise ValueError("verify_drafts: arguments are not what they have to be")
+
+
+class LinearBatch:
+    """One step's sequences for LinearAttention: their slots, their rows, and optionally their lengths and how many rows enter the
+    state.  Keeps its tensors alive; the contents may change between launches (they are read on the device)."""
+
+    def __init__(self, slots: Any, lengths: Any, row_offsets: Any, keep: Any, tokens: int, max_new_tokens: int) -> None:
+        import torch
+
+        sequences = int(slots.shape[0]) if slots.dim() == 1 else -1
+        for name, tensor, size in (("slots", slots, sequences), ("lengths", lengths, sequences), ("row_offsets", row_offsets, sequences + 1),
+                                   ("keep", keep, sequences)):
+            if tensor is not None and (tensor.dtype != torch.int32 or tuple(tensor.shape) != (size,)):
+                raise ValueError(f"{name} must be int32 [{'sequences' if size < 0 else size}], got {tensor.dtype} {list(tensor.shape)}")
+            if tensor is not None and tensor.get_device() != slots.get_device():
+                raise ValueError(f"{name} and slots are on different devices")
+        self.slots, self.lengths, self.row_offsets, self.keep = slots, lengths, row_offsets, keep
+        self.device = slots.get_device()
+        self.tokens = tokens
+        self.struct = LinearBatchStruct(ctypes.sizeof(LinearBatchStruct), sequences, tokens, max_new_tokens, _ptr(slots), _ptr(row_offsets),
+                                        _ptr(lengths), _ptr(keep))
+        self.ref = ctypes.byref(self.struct)
+
+
+class LinearAttention:
+    """The linear-attention layers' convolution and gated delta rule over caller-owned states: the binding of aima_moe_linear_*."""
+
+    def __init__(self, *, k_heads: int = 16, v_heads: int = 32, conv_width: int = 4, slots: int, layers: int = 1, max_sequences: int = 256,
+                 max_tokens: int = 8192, eps: float = 0.0, library: MoeLibrary | None = None) -> None:
+        import torch
+
+        if not torch.cuda.is_available():
+            raise RuntimeError("aima_moe needs a CUDA device (sm_100a); there is no CPU fallback")
+        self._torch = torch
+        self._device = torch.cuda.current_device()
+        self.lib = library or load_library()
+        self.config = LinearConfig(ctypes.sizeof(LinearConfig), k_heads, v_heads, LINEAR_HEAD_DIM, conv_width, slots, layers, max_sequences,
+                                   max_tokens, eps, None, 0)
+        size, handle = c_uint64(), c_void_p()
+        self.lib.check(self.lib.aima_moe_linear_query_workspace(ctypes.byref(self.config), ctypes.byref(size)))
+        # from torch's allocator, which has it at hand where the driver takes milliseconds
+        self._workspace = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+        self.config.workspace, self.config.workspace_bytes = self._workspace.data_ptr(), size.value
+        torch.cuda.current_stream().synchronize()      # what had this memory before is done with it
+        self.lib.check(self.lib.aima_moe_linear_prepare(ctypes.byref(self.config), ctypes.byref(handle)))
+        self.handle = handle
+        self.channels = (2 * k_heads + v_heads) * LINEAR_HEAD_DIM
+        self._k_shape, self._v_shape = (k_heads, LINEAR_HEAD_DIM), (v_heads, LINEAR_HEAD_DIM)
+        self._keepalive: dict[int, Any] = {}
+        self._streams: set[int] = set()
+
+    # -- setup ---------------------------------------------------------------
+    def allocate_layer(self) -> tuple[Any, Any]:
+        """Zeroed conv_states and states of one layer."""
+        torch, c = self._torch, self.config
+        return (torch.zeros(c.slots, c.conv_width - 1, self.channels, dtype=torch.bfloat16, device="cuda"),
+                torch.zeros(c.slots, c.v_heads, LINEAR_HEAD_DIM, LINEAR_HEAD_DIM, dtype=torch.float32, device="cuda"))
+
+    def bind_layer(self, layer: int, *, conv_weight: Any = None, conv_states: Any = None, states: Any = None, a_log: Any = None,
+                   dt_bias: Any = None, norm_weight: Any = None) -> None:
+        """conv_weight BF16 [channels, conv_width] and conv_states BF16 [slots, conv_width - 1, channels] for conv; states FP32
+        [slots, v_heads, 128, 128], a_log and dt_bias FP32 [v_heads] for delta; norm_weight BF16 [128] for its gate."""
+        torch = self._torch
+        tensors = LinearLayer(ctypes.sizeof(LinearLayer), 0)
+        for name, tensor, dtype in (("conv_weight", conv_weight, torch.bfloat16), ("conv_states", conv_states, torch.bfloat16),
+                                    ("states", states, torch.float32), ("a_log", a_log, torch.float32), ("dt_bias", dt_bias, torch.float32),
+                                    ("norm_weight", norm_weight, torch.bfloat16)):
+            if tensor is not None and tensor.dtype != dtype:
+                raise ValueError(f"{name} must be {dtype}, got {tensor.dtype}")
+            setattr(tensors, name, _ptr(tensor))
+            setattr(tensors, name + "_bytes", _nbytes(tensor))
+        self.lib.check(self.lib.aima_moe_linear_bind_layer(self.handle, layer, ctypes.byref(tensors)))
+        self._keepalive[layer] = (conv_weight, conv_states, states, a_log, dt_bias, norm_weight)
+
+    @staticmethod
+    def batch(slots: Any, *, tokens: int, lengths: Any = None, row_offsets: Any = None, max_new_tokens: int | None = None, keep: Any = None) -> LinearBatch:
+        """slots int32 [sequences], -1 for a sequence that is not there; lengths int32 [sequences], the new tokens included: a sequence
+        that is no longer than its rows starts with them; row_offsets int32 [sequences + 1] into the `tokens` rows, or None for the
+        same number of rows each; keep int32 [sequences]: rows that enter the state."""
+        if max_new_tokens is None:
+            max_new_tokens = tokens if row_offsets is not None else tokens // int(slots.shape[0])
+        return LinearBatch(slots, lengths, row_offsets, keep, tokens, max_new_tokens)
+
+    # -- launches ------------------------------------------------------------
+    def conv(self, layer: int, batch: LinearBatch, x: Any, out: Any = None) -> Any:
+        """Short causal convolution with SiLU over the rows of x, BF16 [tokens, channels] (a view of wider rows is fine)."""
+        if batch.device != self._device:
+            self._refuse_device(batch)
+        torch, shape = self._torch, (batch.tokens, self.channels)
+        if x.dtype is not torch.bfloat16 or x.get_device() != self._device or x.shape != shape or x.stride(1) != 1:
+            raise ValueError(f"x must be a bfloat16 tensor {list(shape)} with contiguous rows of the handle's device, got {x.dtype} {list(x.shape)} "
+                             f"with strides {list(x.stride())} on {x.device}")
+        out = self._out(out, x, shape)
+        self.lib.check(self.lib.aima_moe_linear_conv_launch(self.handle, layer, batch.ref, x.data_ptr(), x.stride(0), out.data_ptr(), self._stream()))
+        return out
+
+    def delta(self, layer: int, batch: LinearBatch, q: Any, k: Any, v: Any, a: Any, b: Any, gate: Any = None, out: Any = None,
+              outputs: bool = True) -> Any:
+        """The gated delta rule: q and k BF16 [tokens, k_heads, 128], v and the gate [tokens, v_heads, 128], a and b [tokens, v_heads];
+        all of them may be views.  Returns BF16 [tokens, v_heads, 128], normed and gated if there is a gate; with outputs=False it
+        only brings the states to the rows that `keep` says and returns None."""
+        if batch.device != self._device:
+            self._refuse_device(batch)
+        tokens = batch.tokens
+        k_shape, v_shape = (tokens, *self._k_shape), (tokens, *self._v_shape)
+        call = LinearDelta(_LINEAR_DELTA_BYTES, 0, self._rows(q, "q", k_shape), self._rows(k, "k", k_shape), self._rows(v, "v", v_shape),
+                           KvRows() if gate is None else self._rows(gate, "gate", v_shape), a.data_ptr(), b.data_ptr(), self._numbers(a, "a", v_shape),
+                           self._numbers(b, "b", v_shape))
+        if outputs:
+            out = self._out(out, v, v_shape)
+            call.out = out.data_ptr()
+        else:
+            out = None
+        self.lib.check(self.lib.aima_moe_linear_delta_launch(self.handle, layer, batch.ref, call, self._stream()))
+        return out
+
+    def _rows(self, tensor: Any, name: str, shape: tuple[int, int, int]) -> KvRows:
+        row_stride, head_stride, stride = tensor.stride() if tensor.dim() == 3 else (0, 0, 0)
+        if tensor.dtype is not self._torch.bfloat16 or tensor.get_device() != self._device or tensor.shape != shape or stride != 1:
+            raise ValueError(f"{name} must be a bfloat16 tensor {list(shape)} with contiguous heads of the handle's device, got "
+                             f"{tensor.dtype} {list(tensor.shape)} with strides {list(tensor.stride())} on {tensor.device}")
+        return KvRows(tensor.data_ptr(), row_stride, head_stride)
+
+    def _numbers(self, tensor: Any, name: str, shape: tuple[int, int, int]) -> int:
+        if (tensor.dtype is not self._torch.bfloat16 or tensor.get_device() != self._device or tensor.shape != shape[:2]
+                or (tensor.stride(1) != 1 and shape[1] > 1)):
+            raise ValueError(f"{name} must be a bfloat16 tensor {list(shape[:2])} with contiguous rows of the handle's device, got "
+                             f"{tensor.dtype} {list(tensor.shape)} with strides {list(tensor.stride())} on {tensor.device}")
+        return tensor.stride(0)
+
+    def _out(self, out: Any, like: Any, shape: tuple) -> Any:
+        if out is None:
+            return self._torch.empty(shape, dtype=self._torch.bfloat16, device=like.device)
+        if out.dtype is not self._torch.bfloat16 or out.get_device() != self._device or out.shape != shape or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous bfloat16 tensor {list(shape)} of the handle's device")
+        return out
+
+    def _refuse_device(self, batch: LinearBatch) -> None:
+        raise ValueError(f"the batch's tensors are of device {batch.device}, the handle is of {self._device}")
+
+    def _stream(self) -> int:
+        stream = self._torch._C._cuda_getCurrentRawStream(self._device)
+        self._streams.add(stream)
+        return stream
+
+    def sync(self) -> None:
+        """Waits for the last launch and raises AimaMoeError if device-side data of a batch was out of range."""
+        self.lib.check(self.lib.aima_moe_linear_sync(self.handle))
+
+    def release(self) -> None:
+        if getattr(self, "handle", None):
+            self.lib.aima_moe_linear_release(self.handle)
+            self.handle = None
+            for stream in self._streams:        # what is under way there still uses the workspace
+                self._workspace.record_stream(self._torch.cuda.ExternalStream(stream))
+            self._workspace = None
+            self._keepalive.clear()
+
+    def __del__(self) -> None:  # best effort
+        try:
+            self.release()
+        except Exception:
+            pass
+
+
+def head_norm(x: Any, weight: Any = None, *, offset: float = 0.0, gate: Any = None, activation: str = "none", eps: float = 1.0e-6,
+              out: Any = None, library: MoeLibrary | None = None) -> Any:
+    """x / sqrt(mean(x^2) + eps) * (weight + offset) * act(gate) over each head (aima_moe_head_norm_launch): x and gate BF16
+    [tokens, heads, 64, 128 or 256], views of wider rows or not; weight BF16 [head_dim], or None for x * act(gate) without a norm;
+    activation "silu" or "sigmoid" with a gate.  Returns BF16 [tokens, heads, head_dim]; out may be x itself."""
+    import torch
+
+    lib = library or load_library()
+    device, shape = x.get_device(), x.shape
+    # in one expression: the call on the host takes longer than the kernel
+    if not (device == torch._C._cuda_getDevice() and x.dtype is torch.bfloat16 and len(shape) == 3 and x.stride(2) == 1
+            and activation in GATE_ACTIVATIONS
+            and (gate is None or (gate.dtype is torch.bfloat16 and gate.shape == shape and gate.get_device() == device and gate.stride(2) == 1))
+            and (weight is None or (weight.dtype is torch.bfloat16 and weight.shape == shape[2:] and weight.get_device() == device
+                                    and weight.is_contiguous()))
+            and (out is None or (out.dtype is torch.bfloat16 and out.shape == shape and out.get_device() == device and out.is_contiguous()))):
+        _refuse_head_norm(x, weight, gate, activation, out)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
+    call = HeadNorm(_HEAD_NORM_BYTES, shape[0], shape[1], shape[2], GATE_ACTIVATIONS[activation], offset, eps, 0,
+                    KvRows(x.data_ptr(), x.stride(0), x.stride(1)),
+                    KvRows() if gate is None else KvRows(gate.data_ptr(), gate.stride(0), gate.stride(1)),
+                    None if weight is None else weight.data_ptr(), out.data_ptr())
+    lib.check(lib.aima_moe_head_norm_launch(call, torch._C._cuda_getCurrentRawStream(device)))
+    return out
+
+
+def _refuse_head_norm(x: Any, weight: Any, gate: Any, activation: str, out: Any) -> None:
+    """Says which of head_norm's arguments is not what it has to be."""
+    import torch
+
+    device = torch.cuda.current_device()
+    if activation not in GATE_ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(GATE_ACTIVATIONS)}, got {activation!r}")
+    if x.dim() != 3:
+        raise ValueError(f"x must be [tokens, heads, head_dim], got {list(x.shape)}")
+    for name, tensor, shape in (("x", x, x.shape), ("gate", gate, x.shape), ("weight", weight, x.shape[2:]), ("out", out, x.shape)):
+        if tensor is None:
+            continue
+        if tensor.dtype is not torch.bfloat16 or tensor.shape != shape or tensor.get_device() != device:
+            raise ValueError(f"{name} must be a bfloat16 tensor {list(shape)} of the current CUDA device, got {tensor.dtype} {list(tensor.shape)} "
+                             f"on {tensor.device}")
+        if tensor.stride(-1) != 1 or (name in ("weight", "out") and not tensor.is_contiguous()):
+            raise ValueError(f"{name} must have contiguous {'heads' if name in ('x', 'gate') else 'elements'}, got strides {list(tensor.stride())}")
+    raise ValueError("head_norm: arguments are not what they have to be")

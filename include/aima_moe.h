@@ -627,6 +627,132 @@ typedef struct aima_moe_verify_drafts {
 } aima_moe_verify_drafts;
 int aima_moe_verify_drafts_launch(const aima_moe_verify_drafts* call, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Linear-attention layers (30 of the 40 layers): from the rows of the input projection to the rows that the output projection
+ * takes.  The counterpart of the reference's convolution, gated delta rule and gated norm (native/src/native_linear_layer.hip.cpp,
+ * native/src/native_linear_prefill.hip.cpp); the projections are the caller's (aima_moe_gemm_bf16_launch).
+ *
+ * Per layer and value head a state S of 128 x 128 (FP32, [key element, value element]) and, for the convolution, the last
+ * conv_width - 1 inputs of every channel.  Both are caller-owned and lie in slots; a sequence keeps its slot over its life.
+ *
+ * A batch names for every sequence its slot, the rows that are its new tokens (row_offsets), and optionally its length with
+ * them and how many of them enter the state:
+ *   slots    -1: the sequence is not there (a padded batch): its rows give zeros and no state is touched.  The slots of a batch
+ *            differ from one another.
+ *   lengths  tokens of the sequence, the new ones included, as aima_moe_kv_batch has them.  A sequence whose length is not above
+ *            its rows starts here: it begins with zeros whatever its slot holds, and rows before its position 0 are inactive (they
+ *            give zeros and enter nothing).  NULL: every sequence goes on from its slot.
+ *   keep     rows of the sequence, from its first on, that enter the state (clamped to 0 .. its rows); the others are computed all
+ *            the same.  NULL: all.  With drafted tokens: a call with keep 0 gives their outputs, and once it is known how many stand a
+ *            second call on the same rows, without outputs, brings the state there.
+ * All of it is read on the device, so a captured graph can be replayed for other contents. */
+#define AIMA_MOE_LINEAR_HEAD_DIM 128
+typedef struct aima_moe_linear aima_moe_linear;
+
+typedef struct aima_moe_linear_config {
+  uint32_t struct_bytes;   /* sizeof(aima_moe_linear_config), ABI check                            */
+  uint32_t k_heads;        /* heads of q and k, 1 .. 128                                          */
+  uint32_t v_heads;        /* heads of v: a multiple of k_heads, at most 256; value head h goes with key head h / (v_heads / k_heads) */
+  uint32_t head_dim;       /* must be 128                                                         */
+  uint32_t conv_width;     /* 2 .. 4                                                              */
+  uint32_t slots;          /* states of every layer, 1 .. 2^20                                    */
+  uint32_t layers;         /* 1 .. AIMA_MOE_MAX_LAYERS                                            */
+  uint32_t max_sequences;  /* of a batch, 1 .. 1024                                               */
+  uint32_t max_tokens;     /* rows of a batch, 1 .. 2^20; the workspace grows with it             */
+  float eps;               /* of the norms; 0 = 1e-6                                              */
+  void* workspace;         /* device memory of the caller's, 256-byte aligned, from prepare (nothing under way may use it)
+                              for the handle's lifetime; NULL: prepare allocates                  */
+  uint64_t workspace_bytes; /* of it, at least what aima_moe_linear_query_workspace says          */
+} aima_moe_linear_config;
+
+/* channels = (2 k_heads + v_heads) * 128: the heads of q, then of k, then of v.  The convolution needs the first two, the delta
+ * rule the next three, its gate the last; the others may be NULL. */
+typedef struct aima_moe_linear_layer {
+  uint32_t struct_bytes;
+  uint32_t reserved;
+  const void* conv_weight; uint64_t conv_weight_bytes; /* bf16 [channels, conv_width], the last one is the token's own */
+  void* conv_states;       uint64_t conv_states_bytes; /* bf16 [slots, conv_width - 1, channels], oldest first         */
+  void* states;            uint64_t states_bytes;      /* f32  [slots, v_heads, 128, 128]                              */
+  const void* a_log;       uint64_t a_log_bytes;       /* f32  [v_heads]                                               */
+  const void* dt_bias;     uint64_t dt_bias_bytes;     /* f32  [v_heads]                                               */
+  const void* norm_weight; uint64_t norm_weight_bytes; /* bf16 [128]                                                   */
+} aima_moe_linear_layer;
+
+typedef struct aima_moe_linear_batch {
+  uint32_t struct_bytes;
+  uint32_t sequences;          /* 1 .. max_sequences                                            */
+  uint32_t tokens;             /* rows, 1 .. max_tokens                                         */
+  uint32_t max_new_tokens;     /* no sequence has more rows than this; 1 .. tokens              */
+  const int32_t* slots;        /* [sequences]                                                   */
+  const int32_t* row_offsets;  /* [sequences + 1], from 0 to at most tokens, not falling; NULL: max_new_tokens rows each
+                                  (tokens = sequences * max_new_tokens)                         */
+  const int32_t* lengths;      /* [sequences] or NULL                                           */
+  const int32_t* keep;         /* [sequences] or NULL                                           */
+} aima_moe_linear_batch;
+
+/* Device bytes of a handle's workspace. */
+int aima_moe_linear_query_workspace(const aima_moe_linear_config* config, uint64_t* bytes);
+int aima_moe_linear_prepare(const aima_moe_linear_config* config, aima_moe_linear** handle);
+/* Records one layer's tensors.  16-byte aligned, of the handle's device. */
+int aima_moe_linear_bind_layer(aima_moe_linear* handle, uint32_t layer, const aima_moe_linear_layer* tensors);
+
+/* out[t, c] = silu(sum_j weight[c, j] x[t - (conv_width - 1) + j, c]), one launch; what lies before a sequence's first row comes from
+ * its slot, which then holds its last conv_width - 1 inputs that were kept.  x: bf16 [tokens, channels], 16-byte aligned, rows
+ * x_row_stride elements apart (a multiple of 8).  out: bf16 [tokens, channels], contiguous; it may not overlap x. */
+int aima_moe_linear_conv_launch(aima_moe_linear* handle, uint32_t layer, const aima_moe_linear_batch* batch, const void* x,
+                                uint64_t x_row_stride, void* out, void* stream);
+
+/* The gated delta rule.  Per value head, with q and k scaled to length 1 (x / sqrt(|x|^2 + eps)):
+ *   S <- exp(g) S,  S <- S + k (beta (v - S^T k))^T,  o = S^T q / sqrt(128),
+ *   g = -exp(a_log) softplus(a + dt_bias),  beta = sigmoid(b).
+ * With a gate z: out = o / sqrt(mean(o^2) + eps) * norm_weight * silu(z), else out = o.
+ * FP32 state, sums and norms.  A NaN or infinity that a token brings reaches what depends on it and nothing else: no token before it,
+ * and no other sequence. */
+typedef struct aima_moe_linear_delta {
+  uint32_t struct_bytes;
+  uint32_t reserved;
+  aima_moe_kv_rows q;       /* bf16 [tokens, k_heads, 128]                                          */
+  aima_moe_kv_rows k;
+  aima_moe_kv_rows v;       /* bf16 [tokens, v_heads, 128]                                          */
+  aima_moe_kv_rows gate;    /* bf16 [tokens, v_heads, 128]; data NULL: none                         */
+  const void* a;            /* bf16 [tokens, v_heads], rows a_row_stride elements apart             */
+  const void* b;
+  uint64_t a_row_stride;
+  uint64_t b_row_stride;
+  void* out;                /* bf16 [tokens, v_heads, 128], contiguous, 16-byte aligned; may not overlap the span of an
+                               input; NULL: the states alone                                      */
+} aima_moe_linear_delta;
+int aima_moe_linear_delta_launch(aima_moe_linear* handle, uint32_t layer, const aima_moe_linear_batch* batch,
+                                 const aima_moe_linear_delta* call, void* stream);
+
+/* Synchronises the last stream and reports what launches since the last call found wrong in device-side data:
+ * AIMA_MOE_ERR_INVALID_ARGUMENT for a slot, row offset or length outside its range (such a sequence was treated as one without tokens),
+ * AIMA_MOE_ERR_TIMEOUT for a bounded wait that ran out.  Calls of one handle share its workspace: issue them on one stream or order
+ * them with events. */
+int aima_moe_linear_sync(aima_moe_linear* handle);
+int aima_moe_linear_release(aima_moe_linear* handle);
+
+/* Norm of each head with an optional gate: out = x / sqrt(mean(x^2) + eps) * (weight + weight_offset) * act(gate), in FP32, rounded
+ * once.  The norm of a full-attention layer's queries and keys before their rotation, its output gate (no weight: no norm), the
+ * gated norm of a linear-attention layer's output.  No handle, no workspace; one launch on the current device. */
+enum { AIMA_MOE_GATE_NONE = 0, AIMA_MOE_GATE_SILU = 1, AIMA_MOE_GATE_SIGMOID = 2 };
+typedef struct aima_moe_head_norm {
+  uint32_t struct_bytes;
+  uint32_t tokens;          /* 1 .. 2^24                                                           */
+  uint32_t heads;           /* 1 .. 1024                                                           */
+  uint32_t head_dim;        /* 64, 128 or 256                                                      */
+  uint32_t activation;      /* AIMA_MOE_GATE_*; NONE exactly if gate.data is NULL                  */
+  float weight_offset;      /* 1 for weights that are stored less one                              */
+  float eps;
+  uint32_t reserved;
+  aima_moe_kv_rows x;       /* bf16 [tokens, heads, head_dim]                                      */
+  aima_moe_kv_rows gate;
+  const void* weight;       /* bf16 [head_dim], 16-byte aligned; NULL: no norm, out = x * act(gate) */
+  void* out;                /* bf16 [tokens, heads, head_dim], contiguous, 16-byte aligned; x itself if x is contiguous, else it may
+                               not overlap x, gate or weight                                      */
+} aima_moe_head_norm;
+int aima_moe_head_norm_launch(const aima_moe_head_norm* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
