@@ -17,7 +17,8 @@ LIB = HERE / "libaima_moe_b200.so"
 SOURCES = ["moe_api.cu", "decode_kernel.cu", "decode_noalloc.cu", "pointwise.cu", "prefill.cu",
            "grouped_gemm_simt.cu", "grouped_gemm_tc.cu", "lm_head.cu", "lm_head_api.cu",
            "image_loader.cu", "kv_api.cu", "kv_append.cu", "kv_attention.cu", "kv_decode.cu", "kv_prompt.cu",
-           "verify_drafts.cu", "linear_api.cu", "linear_conv.cu", "linear_step.cu", "head_norm.cu"]
+           "verify_drafts.cu", "linear_api.cu", "linear_conv.cu", "linear_step.cu", "linear_prepare.cu",
+           "linear_chunk.cu", "head_norm.cu"]
 
 
 def nvcc_path() -> str:

@@ -45,7 +45,9 @@ int check_config(const aima_moe_linear_config* c) {
 }
 
 uint64_t channels_of(const aima_moe_linear_config& c) { return (2ull * c.k_heads + c.v_heads) * kDim; }
-uint64_t workspace_bytes(const aima_moe_linear_config&) { return 256; }
+uint64_t workspace_bytes(const aima_moe_linear_config& c) {
+  return 256 + (c.max_tokens > aima::kLinearStepRows ? aima::linear_chunk_workspace(c.k_heads, c.v_heads, c.max_tokens, c.max_sequences) : 0);
+}
 
 int check_device_pointer(const void* pointer, int device, const char* name) {
   cudaPointerAttributes attributes{};
@@ -276,7 +278,12 @@ AIMA_EXPORT int aima_moe_linear_delta_launch(aima_moe_linear* h, uint32_t layer,
   a.states = static_cast<float*>(t.states);
   a.out = static_cast<__nv_bfloat16*>(call->out);
   a.status = h->status;
-  const cudaError_t error = aima::linear_step(a, static_cast<cudaStream_t>(stream));
+  // Sequences of few rows go token by token, longer ones in chunks; a batch that may have both takes both launches.
+  cudaError_t error = cudaSuccess;
+  const bool chunks = a.batch.max_new > aima::kLinearStepRows, steps = !chunks || (a.batch.sequences > 1 && a.batch.offsets != nullptr);
+  if (steps) error = aima::linear_step(a, chunks ? aima::kLinearStepRows : a.batch.max_new, static_cast<cudaStream_t>(stream));
+  if (error == cudaSuccess && chunks)
+    error = aima::linear_chunks(a, steps ? aima::kLinearStepRows : 0, reinterpret_cast<uint8_t*>(h->status) + 256, static_cast<cudaStream_t>(stream));
   if (error != cudaSuccess) return fail_cuda(error, "linear delta launch");
   h->last_stream = static_cast<cudaStream_t>(stream);
   return AIMA_MOE_OK;

@@ -35,12 +35,13 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const float4& v) {
 __device__ __forceinline__ float dot4(const float4& a, const float4& b) { return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, a.x * b.x))); }
 __device__ __forceinline__ float4 scaled(const float4& a, float s) { return make_float4(a.x * s, a.y * s, a.z * s, a.w * s); }
 
-__global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const LinearDelta a) {
+__global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const LinearDelta a, int max_rows) {
   __shared__ StepRow rows[kStepRows];
   __shared__ float decay[kStepRows], rate[kStepRows], overlap[kStepRows];
   const int head = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const LinearSequence seq = linear_sequence(a.batch, blockIdx.y);
   if (seq.bad && head == 0 && threadIdx.x == 0) atomicOr(a.status, kLinearBadBatch);
+  if (seq.rows > max_rows) return;
   // rows that have to be gone through: the active ones, without outputs only those that stay
   const int end = a.out != nullptr ? seq.rows : min(seq.rows, seq.kept);
   if (a.out != nullptr)
@@ -164,8 +165,8 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
 
 }  // namespace
 
-cudaError_t linear_step(const LinearDelta& a, cudaStream_t stream) {
-  linear_step_kernel<<<dim3(a.v_heads, a.batch.sequences), kStepThreads, 0, stream>>>(a);
+cudaError_t linear_step(const LinearDelta& a, int max_rows, cudaStream_t stream) {
+  linear_step_kernel<<<dim3(a.v_heads, a.batch.sequences), kStepThreads, 0, stream>>>(a, max_rows);
   return cudaGetLastError();
 }
 

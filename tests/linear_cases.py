@@ -90,11 +90,11 @@ class Problem:
 
     def delta_wanted(self, states=None, batch=None):
         return linear_oracle.delta(self.q, self.k, self.v, self.a, self.b, self.a_log, self.dt_bias, self.states if states is None else states,
-                                   batch or self.batch, gate=self.gate, norm_weight=self.norm_weight)
+                                   batch or self.batch, gate=self.gate, norm_weight=self.norm_weight, floor=constants(max(self.rows))[1])
 
 
 def constants(rows):
-    """(c of the bound, relative error of what an output adds up) by the form that a batch of at most so many rows a sequence takes.
+    """c of the bound by the form that a batch of at most so many rows a sequence takes, and its floor in units of c.
 
     Token by token: a dot of 128 products is a chain of 16 and three sums by pairs (19 roundings), normalised keys are off by 12 (128
     squares in a chain of 4 and 5 pairs, a root, a product), decay and rate by 8, the update by 3: below 64 in all.
@@ -102,24 +102,31 @@ def constants(rows):
     Chunks of 64 tokens: a dot with the state is a sum of 128 products in FP32 and, its operand being held in two 11-bit terms, off by
     another 2^-22 of each: 128 + 4; the corrections of a chunk come from a sum over up to 64 tokens, each with an operand pair good to
     2^-21 (64 + 8 each, on numbers no larger than those of the bound): 64 * 72 if all of them count, whose sizes add up to the column's
-    length with the chunk's; so 8192 covers both forms of the sum.  An output's operands are rounded to 11 bits: 2^-11 of what is added."""
-    return (64.0, 0.0) if rows <= STEP_ROWS else (8192.0, 2.0 ** -11)
+    length with the chunk's; so 8192 covers both forms of the sum.  Floor: the second term has steps of 2^-24 where the column's largest
+    number is 1/2 or more, so an operand is off by 2^-24 of that; 12 of them in a dot with a key of length 1 (the sum of its elements' sizes
+    is at most sqrt(128)) and 64 corrections: 768 roundings."""
+    return (64.0, 0.0) if rows <= STEP_ROWS else (8192.0, 768.0 / 8192.0)
 
 
-STEP_ROWS = 1 << 30
+STEP_ROWS = 32
 
 
-def check_delta(got, states, wanted, most, touched=None):
+def check_delta(got, states, wanted, most, typical=True):
     """got against the oracle's out (None: not looked at), states against its; `most`: the largest number of rows of a sequence."""
-    c, rough = constants(most)
+    c, _ = constants(most)
     if got is not None:
         out = wanted["out"]
         fine = torch.isfinite(out)
-        bound = out.abs() * (HALF_STEP + 2.0 ** -18) + c * UNIT * wanted["out_error"] + rough * 16 * wanted["reach"] + 2.0 ** -133
+        bound = out.abs() * (HALF_STEP + 2.0 ** -18) + c * UNIT * wanted["out_error"] + 2.0 ** -133
         off = (got.double() - out).abs()
         worst = (off / bound)[fine]
         assert worst.numel() == 0 or float(worst.max()) <= 1.0, float(worst.max())
     error = (states.double() - wanted["states"]).abs()
+    # the bound is of the worst case; roundings of either sign add up to a few of 2^-22 over a whole state
+    size = torch.where(torch.isfinite(wanted["states"]), wanted["states"], 0.0)
+    if typical:
+        norm = float(torch.where(torch.isfinite(error), error, 0.0).norm() / size.norm())
+        assert norm <= 2.0 ** -19, norm
     # of a column of the state: its length errs by so much, so does each element
     bound = c * UNIT * wanted["state_error"][:, :, None, :] + UNIT * wanted["states"].abs()
     fine = torch.isfinite(wanted["states"])

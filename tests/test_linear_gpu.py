@@ -7,7 +7,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 import linear_oracle  # noqa: E402
-from linear_cases import DIM, HALF_STEP, Problem, check_delta, offsets_of  # noqa: E402
+from linear_cases import DIM, HALF_STEP, Problem, check_delta, constants  # noqa: E402
 
 # rows of each sequence, tokens before them
 BATCHES = {
@@ -208,7 +208,7 @@ def test_delta_rule_of_extreme_gates(package, rows):
     wanted = p.delta_wanted()
     got = p.delta()
     p.layer.sync()
-    check_delta(got, p.states, wanted, most(rows))
+    check_delta(got, p.states, wanted, most(rows), typical=False)
 
 
 @pytest.mark.parametrize("rows", [[30, 30], [150, 130]])
@@ -334,7 +334,8 @@ def test_captured_calls_follow_their_inputs(package, rows):
         torch.cuda.synchronize()
         p.check_conv(y.view(p.tokens, -1), p.conv_states, conv_wanted)
         parts = y.split([q, k, v], dim=1)
-        wanted = linear_oracle.delta(*parts, p.a, p.b, p.a_log, p.dt_bias, states, p.batch, gate=p.gate, norm_weight=p.norm_weight)
+        wanted = linear_oracle.delta(*parts, p.a, p.b, p.a_log, p.dt_bias, states, p.batch, gate=p.gate, norm_weight=p.norm_weight,
+                                     floor=constants(most(rows))[1])
         check_delta(out, p.states, wanted, most(rows))
     p.layer.sync()
 
