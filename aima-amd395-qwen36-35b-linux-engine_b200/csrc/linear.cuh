@@ -104,13 +104,12 @@ __device__ __forceinline__ void linear_report(const LinearBatch& b, int* status,
     if (linear_sequence(b, s).bad) atomicOr(status, kLinearBadBatch);
 }
 
-__device__ __forceinline__ float linear_reciprocal(float x) {
+// 1 / (1 + e^-x), to a few units of the last place; a quarter of the denominator, so that the reciprocal is a normal number
+__device__ __forceinline__ float linear_sigmoid(float x) {
   float y;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(__expf(-x), 0.25f, 0.25f)));
+  return 0.25f * y;
 }
-// 1 / (1 + e^-x), to a few units of the last place
-__device__ __forceinline__ float linear_sigmoid(float x) { return linear_reciprocal(1.0f + __expf(-x)); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);

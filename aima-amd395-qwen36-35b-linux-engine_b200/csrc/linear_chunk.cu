@@ -7,46 +7,50 @@
 // them.  Per chunk:
 //   R = S^T k, Q = S^T q    ->  right side beta v - enter R  ->  D = (right side) T^T
 //   S <- decay S + (stay D) k,  O = D scores^T               ->  o = (read Q + O) / sqrt(128)
-// Two warp groups have 32 tokens or 64 key elements each of that chain, a third the output, one warp issues products, one loads.
+// Four warp groups have 16 tokens or 32 key elements each of that chain, two the output, one warp issues products, three load.
 #include "linear_chunk.cuh"
 
 #include <algorithm>
+#include <cuda_fp16.h>
 
 namespace aima {
 namespace {
 
-constexpr int kChainWarps = 8, kOutWarps = 4;
-constexpr int kChunkThreads = 32 * (kChainWarps + kOutWarps + 4);          // four warp groups; the last one issues products and loads
-// registers of a thread: 128 at launch, in all as many as there are
-constexpr int kChainRegisters = 168, kOutRegisters = 136, kIssueRegisters = 40;
-static_assert(2 * kChainRegisters + kOutRegisters + kIssueRegisters <= 4 * 128, "the warp groups share what the block was launched with");
+constexpr int kChainGroups = 2, kOutGroups = 2;        // of four warps, one for each 32 lanes of tensor memory
+constexpr int kChainWarps = 4 * kChainGroups, kOutWarps = 4 * kOutGroups;
+constexpr int kChunkThreads = 32 * (kChainWarps + kOutWarps + 4);          // the last group issues products and loads
+constexpr int kTokens = kChunk / kChainGroups, kKeys = kLinearDim / kChainGroups;      // of a group of the chain
+// registers of a thread: as many at launch for all, in all as many as there are
+constexpr int kLaunchRegisters = 96, kChainRegisters = 152, kOutRegisters = 64, kIssueRegisters = 48;
+static_assert(kChainGroups * kChainRegisters + kOutGroups * kOutRegisters + kIssueRegisters <= (kChainGroups + kOutGroups + 1) * kLaunchRegisters,
+              "the warp groups share what the block was launched with");
 constexpr int kStages = 2;
-constexpr int kStageValues = kChunkPairBytes + kChunkHeadBytes;           // v: 64 rows of 256 bytes
+constexpr int kStageValues = kChunkPairBytes + kChunkHeadBytes;           // v: 64 rows of 256 bytes, zeros behind the last
 constexpr int kStageBytes = (kStageValues + kChunk * kLinearDim * 2 + 1023) / 1024 * 1024;
 constexpr int kOutRow = kLinearDim + 4;
 
-// columns of tensor memory
-constexpr uint32_t kStateAt = 0, kHighAt = 128, kLowAt = 192, kDotsAt = 256, kReadAt = 320, kEnterAt = 384, kFreshAt = 448;
+// Columns of tensor memory.  Operands lie as eight columns of first and eight of second terms for every 16 elements of K: what a warp
+// splits at a time and a step of a product takes.
+constexpr uint32_t kStateAt = 0, kTermsAt = 128, kFreshAt = 256, kDotsAt = 320, kReadAt = 384, kEnterAt = 448;
+__device__ __forceinline__ constexpr uint32_t operand(int k, int term) { return 16 * k + 8 * term; }
 
 struct __align__(1024) ChunkMemory {
   uint8_t stages[kStages][kStageBytes];
   float out[kChunk * kOutRow];
-  float largest[2][kLinearDim];           // of a column of the state or of what comes, by warp group
+  __nv_bfloat16 gate[kChunk * kLinearDim];
+  float largest[kChainGroups][kLinearDim];      // of a column of the state, by warp group
+  float largest_value[kStages][2][kLinearDim];   // of a column of v, by the warp that brought the rows; not of numbers that are not finite
   float scale[2][kLinearDim];             // the power of two of a column, by parity of the chunk
   int broken[2][kLinearDim];              // the first token of the chunk whose right side is not finite
   int sums[kChunkThreads / 32];
   unsigned long long full[kStages], empty[kStages];
-  unsigned long long state_ready, dots_full, enter_ready, fresh_full, stay_ready, state_full, out_full, dots_empty;
+  unsigned long long values_full[kStages], state_ready[2], dots_full, enter_ready[2], fresh_full, stay_ready[2], state_full, fresh_ready, out_full, dots_empty;
   uint32_t tmem;
   int abort_flag;
 };
 
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* r) {
-  tmem_ld32(taddr, reinterpret_cast<uint32_t*>(r));
-  tmem_ld32(taddr + 32, reinterpret_cast<uint32_t*>(r) + 32);
-}
-__device__ __forceinline__ void chain_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-__device__ __forceinline__ void out_barrier() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
+__device__ __forceinline__ void chain_barrier() { asm volatile("bar.sync 1, %0;" :: "n"(32 * kChainWarps) : "memory"); }
+__device__ __forceinline__ void out_barrier() { asm volatile("bar.sync 2, %0;" :: "n"(32 * kOutWarps) : "memory"); }
 // mbar_wait_bounded_warp without a call: the numbers that are alive across one would go to memory.
 __device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit_ns) {
   if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
@@ -95,13 +99,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&m.full[i]), 1);
       mbar_init(smem_u32(&m.empty[i]), 1 + kChainWarps + kOutWarps);
+      mbar_init(smem_u32(&m.values_full[i]), 2);
     }
-    mbar_init(smem_u32(&m.state_ready), kChainWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&m.state_ready[i]), kChainWarps);
     mbar_init(smem_u32(&m.dots_full), 1);
-    mbar_init(smem_u32(&m.enter_ready), kChainWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&m.enter_ready[i]), kChainWarps);
     mbar_init(smem_u32(&m.fresh_full), 1);
-    mbar_init(smem_u32(&m.stay_ready), kChainWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&m.stay_ready[i]), kChainWarps);
     mbar_init(smem_u32(&m.state_full), 1);
+    mbar_init(smem_u32(&m.fresh_ready), kChainWarps);
     mbar_init(smem_u32(&m.out_full), 1);
     mbar_init(smem_u32(&m.dots_empty), kOutWarps);
     m.abort_flag = 0;
@@ -112,7 +118,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   __syncthreads();
   tc_fence_after();
   for (int w = 0; w < kChunkThreads / 32; ++w) tile0 += m.sums[w];
-  const uint32_t tmem = m.tmem;
+  constexpr uint32_t tmem = 0;               // all 512 columns begin at 0
   const bool fits = tile0 + chunks_of(seq, plan.min_rows) <= plan.tiles;       // not if sequences overlap, which the first kernel reports
   const int n = fits ? chunks : 0;
   if (!fits && threadIdx.x == 0) atomicOr(a.status, kLinearBadBatch);
@@ -128,165 +134,209 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
     // No wait that runs out leaves this loop: the warps meet at barriers, and every wait after the first that ran out ends at once.
     const int group = warp >> 2, column = (warp & 3) * 32 + lane;              // a value element
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    float s[64];                                                               // key elements 64 group ..
+    Pair s[kKeys / 2];                                                         // key elements kKeys group ..
     float scale = 1.0f;
-    if (seq.fresh || n == 0) {
+    {
+      float largest = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 64; ++i) s[i] = 0.0f;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 64; ++i) s[i] = state[(64 * group + i) * kLinearDim + column];
+      for (int i = 0; i < kKeys; i += 2) {
+        float x = 0.0f, y = 0.0f;
+        if (!seq.fresh && n > 0) {
+          x = state[(kKeys * group + i) * kLinearDim + column];
+          y = state[(kKeys * group + i + 1) * kLinearDim + column];
+        }
+        s[i / 2] = Pair(x, y);
+        largest = max3_abs(largest, x, y);
+      }
+      m.largest[group][column] = largest;
+      chain_barrier();
     }
-    uint32_t v[16];                                                            // tokens 32 group .., two in a word
-    for (int c = 0; c <= n; ++c) {
+    float value_before = 0.0f;
+    for (int c = 0; c < n; ++c) {
       const uint8_t* stage = m.stages[c % kStages];
       const ChunkNumbers& numbers = *reinterpret_cast<const ChunkNumbers*>(stage + kChunkPairBytes + kChunkNumbersAt);
-      if (c < n) {
-        wait(&m.full[c % kStages], c / kStages);
-        const uint16_t* values = reinterpret_cast<const uint16_t*>(stage + kStageValues) + 32 * group * kLinearDim + column;
-        const int there = rows - c * kChunk - 32 * group;
-        if (there >= 32) {
+      const int there = rows - c * kChunk;                                     // tokens
+      wait(&m.values_full[c % kStages], c / kStages);
+      // The column's power of two, from the largest of the state one chunk ago and of the values since: the state is at most
+      // sqrt(128) of it longer with 64 of them added, so that 140 times the largest bounds all that is held in 16 bits here.
+      bool rescale;
+      float up = 1.0f;
+      {
+        const float value = fmaxf(m.largest_value[c % kStages][0][column], m.largest_value[c % kStages][1][column]);
+        float largest = fmaxf(value, value_before);
 #pragma unroll
-          for (int t = 0; t < 32; t += 2) v[t / 2] = values[t * kLinearDim] | static_cast<uint32_t>(values[(t + 1) * kLinearDim]) << 16;
-        } else {
-#pragma unroll
-          for (int t = 0; t < 32; t += 2) {
-            const uint32_t v0 = t < there ? values[t * kLinearDim] : 0, v1 = t + 1 < there ? values[(t + 1) * kLinearDim] : 0;
-            v[t / 2] = v0 | v1 << 16;
-          }
+        for (int i = 0; i < kChainGroups; ++i) largest = fmaxf(largest, m.largest[i][column]);
+        const float held = largest * scale;
+        value_before = value;
+        rescale = !(held <= 256.0f && held >= 0.5f) && largest > 0.0f && largest < INFINITY;
+        if (rescale) {
+          const int now = kv_float_exponent(scale), next = min(max(3 - kv_float_exponent(largest), -120), 100);
+          up = kv_exp2(max(min(next - now, 126), -126));
+          scale = kv_exp2(next);
+        }
+        if (group == 0) {
+          m.scale[c & 1][column] = scale;
+          m.broken[c & 1][column] = kChunk;
         }
       }
       if (c > 0) {
         wait(&m.state_full, c - 1);
         tc_fence_after();
-        tmem_ld64(lanes + kStateAt + 64 * group, s);
+#pragma unroll
+        for (int b = 0; b < kKeys / 16; ++b) tmem_ld16(lanes + kStateAt + kKeys * group + 16 * b, reinterpret_cast<uint32_t*>(s + 8 * b));
         tmem_ld_wait();
         if (m.broken[(c - 1) & 1][column] < kChunk) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) s[i] = NAN;
+          for (int i = 0; i < kKeys / 2; ++i) s[i] = Pair(NAN, NAN);
         }
       }
-      if (c == n) break;
-      // the column's power of two
+      if (rescale) {
+#pragma unroll
+        for (int i = 0; i < kKeys / 2; ++i) s[i] = s[i] * Pair(up, up);
+      }
+      // the state in two terms, and decayed for the sum that follows; products begin with the first half of each group's elements
+#pragma unroll
+      for (int b = 0; b < kKeys / 16; ++b) {
+        uint32_t terms[16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) split_f16(s[8 * b + i], &terms[i], &terms[8 + i]);
+        tmem_st16(lanes + kTermsAt + kKeys * group + 16 * b, terms);
+        if (b % (kKeys / 32) == kKeys / 32 - 1) {
+          tmem_st_wait();
+          warp_arrive(&m.state_ready[b / (kKeys / 32)], lane);
+        }
+      }
+      float largest_here;
       {
-        uint32_t most = 0;
+        const float decay = plan.kept_only ? numbers.decay_kept : numbers.decay, back = kv_exp2(-kv_float_exponent(scale));
+        float largest = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 16; ++t) most = __vmaxu2(most, v[t] & 0x7fff7fffu);
-        most = max(most & 0xffffu, most >> 16);
-        if (most >= 0x7f80u) {                                                 // not of numbers that are not finite
-          most = 0;
+        for (int b = 0; b < kKeys / 16; ++b) {
 #pragma unroll
-          for (int t = 0; t < 16; ++t) {
-            const uint32_t low = v[t] & 0x7fffu, high = (v[t] >> 16) & 0x7fffu;
-            if (low < 0x7f80u) most = max(most, low);
-            if (high < 0x7f80u) most = max(most, high);
+          for (int i = 0; i < 8; ++i) {
+            const float2 x = s[8 * b + i].values();
+            largest = max3_abs(largest, x.x, x.y);
+            s[8 * b + i] = s[8 * b + i] * Pair(decay, decay);
           }
+          tmem_st16(lanes + kStateAt + kKeys * group + 16 * b, reinterpret_cast<uint32_t*>(s + 8 * b));
         }
-        float largest = bf16_bits_to_float(static_cast<uint16_t>(most)) * scale;
-#pragma unroll
-        for (int i = 0; i < 64; i += 2) largest = max3_abs(largest, s[i], s[i + 1]);
-        m.largest[group][column] = largest;
-        if (group == 0) m.broken[c & 1][column] = kChunk;
-        chain_barrier();
-        largest = fmaxf(largest, m.largest[group ^ 1][column]);
-        if ((largest > 512.0f || largest < 0.5f) && largest > 0.0f && largest < INFINITY) {
-          const int now = kv_float_exponent(scale), next = min(max(now + 4 - kv_float_exponent(largest), -120), 100);
-          const float up = kv_exp2(max(min(next - now, 126), -126));
-          scale = kv_exp2(next);
-#pragma unroll
-          for (int i = 0; i < 64; ++i) s[i] *= up;
-        }
-        if (group == 0) m.scale[c & 1][column] = scale;
+        largest_here = largest * back;
       }
-      // the state in two terms, and decayed for the sum that follows
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        uint32_t high[16], low[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) split_f16(s[32 * b + 2 * i], s[32 * b + 2 * i + 1], &high[i], &low[i]);
-        tmem_st16(lanes + kHighAt + 32 * group + 16 * b, high);
-        tmem_st16(lanes + kLowAt + 32 * group + 16 * b, low);
-      }
-      tmem_st_wait();
-      warp_arrive(&m.state_ready, lane);
+      uint32_t v[kTokens / 2];                                                 // tokens kTokens group .., two in a word
       {
-        const float decay = plan.kept_only ? numbers.decay_kept : numbers.decay;
-        // for a chunk that ends before its last row the numbers of the kept ones are those of all
+        const uint16_t* values = reinterpret_cast<const uint16_t*>(stage + kStageValues) + kTokens * group * kLinearDim + column;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) s[i] *= decay;
-        tmem_st32(lanes + kStateAt + 64 * group, reinterpret_cast<uint32_t*>(s));
-        tmem_st32(lanes + kStateAt + 64 * group + 32, reinterpret_cast<uint32_t*>(s) + 32);
+        for (int t = 0; t < kTokens; t += 2) v[t / 2] = values[t * kLinearDim] | static_cast<uint32_t>(values[(t + 1) * kLinearDim]) << 16;
       }
+      wait(&m.dots_full, c);
+      tc_fence_after();
+      m.largest[group][column] = largest_here;                                 // all warps have read what the chunk before left here
       // the right side
       {
-        float r[32];
-        wait(&m.dots_full, c);
-        tc_fence_after();
-        tmem_ld32(lanes + kDotsAt + 32 * group, reinterpret_cast<uint32_t*>(r));
+        const Pair scales(scale, scale);
+        Pair all[kTokens / 2];             // read before the first products write there
+#pragma unroll
+        for (int b = 0; b < kTokens / 16; ++b) tmem_ld16(lanes + kDotsAt + kTokens * group + 16 * b, reinterpret_cast<uint32_t*>(all + 8 * b));
         tmem_ld_wait();
-        const int there = rows - c * kChunk - 32 * group;
-        float check = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 32; ++t) {
-          const float2 e = numbers.enter[32 * group + t];
-          const float value = (t & 1) != 0 ? bf16_hi(v[t / 2]) : bf16_lo(v[t / 2]);
-          r[t] = fmaf(-e.y, r[t], e.x * scale * value);
-          if (plan.kept_only && t >= there) r[t] = 0.0f;                       // not a row that is gone through
-          check = fmaf(r[t], 0.0f, check);
-        }
-        if (check != 0.0f) {
-          int first = kChunk;
+        for (int b = 0; b < kTokens / 16; ++b) {
+          const int token = kTokens * group + 16 * b;
+          Pair* const r = all + 8 * b;
+          uint32_t terms[16];
+          __half2 check = __half2half2(__ushort_as_half(0));
 #pragma unroll
-          for (int t = 31; t >= 0; --t) {
-            if (!(fabsf(r[t]) < INFINITY)) {
-              first = 32 * group + t;
-              r[t] = 0.0f;
+          for (int t = 0; t < 16; t += 4) {
+            const float4 rate = *reinterpret_cast<const float4*>(&numbers.rate[token + t]), enter = *reinterpret_cast<const float4*>(&numbers.enter[token + t]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int j = t / 2 + i;
+              const Pair value = Pair(bf16_lo(v[8 * b + j]), bf16_hi(v[8 * b + j])) * scales;
+              r[j] = fma2(i == 0 ? Pair(enter.x, enter.y) : Pair(enter.z, enter.w), r[j], (i == 0 ? Pair(rate.x, rate.y) : Pair(rate.z, rate.w)) * value);
+              split_f16(r[j], &terms[j], &terms[8 + j]);
+              check = __hfma2(*reinterpret_cast<const __half2*>(&terms[j]), __half2half2(__ushort_as_half(0)), check);
             }
           }
-          atomicMin(&m.broken[c & 1][column], first);
-        }
-        uint32_t high[16], low[16];
+          if ((*reinterpret_cast<const uint32_t*>(&check) & 0x7fff7fffu) != 0) {
+            int first = kChunk;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) split_f16(r[2 * i], r[2 * i + 1], &high[i], &low[i]);
-        tmem_st16(lanes + kEnterAt + 16 * group, high);
-        tmem_st16(lanes + kEnterAt + 32 + 16 * group, low);
-        tmem_st_wait();
-        warp_arrive(&m.enter_ready, lane);
+            for (int j = 7; j >= 0; --j) {
+              float2 x = r[j].values();
+              if (!(fabsf(x.y) < INFINITY)) {
+                if (token + 2 * j + 1 < there) first = token + 2 * j + 1;      // rows that are not gone through say nothing
+                x.y = 0.0f;
+              }
+              if (!(fabsf(x.x) < INFINITY)) {
+                if (token + 2 * j < there) first = token + 2 * j;
+                x.x = 0.0f;
+              }
+              split_f16(x.x, x.y, &terms[j], &terms[8 + j]);
+            }
+            atomicMin(&m.broken[c & 1][column], first);
+          }
+          tmem_st16(lanes + kEnterAt + token, terms);
+          tmem_st_wait();
+          warp_arrive(&m.enter_ready[b], lane);
+        }
       }
       // the corrections
       {
-        float d[32];
+        Pair d[kTokens / 2];
         wait(&m.fresh_full, c);
         tc_fence_after();
-        tmem_ld32(lanes + kDotsAt + 32 * group, reinterpret_cast<uint32_t*>(d));
+        const float* stay = (plan.kept_only ? numbers.stay_kept : numbers.stay) + kTokens * group;
+        uint32_t terms[16];
+#pragma unroll
+        for (int b = 0; b < kTokens / 16; ++b) tmem_ld16(lanes + kDotsAt + kTokens * group + 16 * b, reinterpret_cast<uint32_t*>(d + 8 * b));
         tmem_ld_wait();
-        uint32_t high[16], low[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) split_f16(d[2 * i], d[2 * i + 1], &high[i], &low[i]);
-        tmem_st16(lanes + kFreshAt + 16 * group, high);
-        tmem_st16(lanes + kFreshAt + 32 + 16 * group, low);
-        const float* stay = plan.kept_only ? numbers.stay_kept : numbers.stay;
+        for (int b = 0; b < kTokens / 16; ++b) {
 #pragma unroll
-        for (int t = 0; t < 32; ++t) d[t] *= stay[32 * group + t];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) split_f16(d[2 * i], d[2 * i + 1], &high[i], &low[i]);
-        tmem_st16(lanes + kEnterAt + 16 * group, high);
-        tmem_st16(lanes + kEnterAt + 32 + 16 * group, low);
-        tmem_st_wait();
-        warp_arrive(&m.stay_ready, lane);
+          for (int t = 0; t < 16; t += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(&stay[16 * b + t]);
+            const int j = t / 2;
+            split_f16(d[8 * b + j] * Pair(x.x, x.y), &terms[j], &terms[8 + j]);
+            split_f16(d[8 * b + j + 1] * Pair(x.z, x.w), &terms[j + 1], &terms[8 + j + 1]);
+          }
+          tmem_st16(lanes + kEnterAt + kTokens * group + 16 * b, terms);
+          tmem_st_wait();
+          warp_arrive(&m.stay_ready[b], lane);
+        }
         if (lane == 0) mbar_arrive(smem_u32(&m.empty[c % kStages]));
+#pragma unroll
+        for (int b = 0; b < kTokens / 16; ++b) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) split_f16(d[8 * b + i], &terms[i], &terms[8 + i]);
+          tmem_st16(lanes + kFreshAt + kTokens * group + 16 * b, terms);
+        }
+        tmem_st_wait();
+        warp_arrive(&m.fresh_ready, lane);
+      }
+    }
+    if (n > 0) {
+      wait(&m.state_full, n - 1);
+      tc_fence_after();
+#pragma unroll
+      for (int b = 0; b < kKeys / 16; ++b) tmem_ld16(lanes + kStateAt + kKeys * group + 16 * b, reinterpret_cast<uint32_t*>(s + 8 * b));
+      tmem_ld_wait();
+      if (m.broken[(n - 1) & 1][column] < kChunk) {
+#pragma unroll
+        for (int i = 0; i < kKeys / 2; ++i) s[i] = Pair(NAN, NAN);
       }
     }
     if (n > 0 && plan.store && seq.kept > seq.first) {
       const float back = kv_exp2(-kv_float_exponent(scale));
 #pragma unroll
-      for (int i = 0; i < 64; ++i) state[(64 * group + i) * kLinearDim + column] = s[i] * back;
+      for (int i = 0; i < kKeys / 2; ++i) {
+        const float2 x = s[i].values();
+        state[(kKeys * group + 2 * i) * kLinearDim + column] = x.x * back;
+        state[(kKeys * group + 2 * i + 1) * kLinearDim + column] = x.y * back;
+      }
     }
   } else if (warp < kChainWarps + kOutWarps) {
     // ------------------------------ outputs ------------------------------
-    more_registers<kOutRegisters>();
-    const int w = warp - kChainWarps, column = w * 32 + lane;
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    fewer_registers<kOutRegisters>();
+    const int w = warp - kChainWarps, group = w >> 2, column = (w & 3) * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((w & 3) * 32) << 16);
     const bool outputs = a.out != nullptr && !plan.kept_only, gated = outputs && a.gate.data != nullptr;
     const int half = lane >> 4, piece = lane & 15;
     uint4 weights = make_uint4(0, 0, 0, 0);
@@ -294,14 +344,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
     for (int c = 0; c < n; ++c) {
       const uint8_t* stage = m.stages[c % kStages];
       const ChunkNumbers& numbers = *reinterpret_cast<const ChunkNumbers*>(stage + kChunkPairBytes + kChunkNumbersAt);
-      // the gate's rows come while the chunk is under way: 16 lanes a row, eight rows a thread
+      // the gate's rows come while the chunk is under way: 16 lanes a row, four rows a thread, which reads no others
       const int there = min(kChunk, rows - c * kChunk);
-      uint4 gate[8];
       if (gated) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int t = 8 * i + 2 * w + half;
-          if (t < there) gate[i] = *reinterpret_cast<const uint4*>(a.gate.data + (row0 + c * kChunk + t) * a.gate.row_stride + head * a.gate.head_stride + 8 * piece);
+        for (int i = 0; i < kChunk / 2 / kOutWarps; ++i) {
+          const int t = 2 * kOutWarps * i + 2 * w + half;
+          if (t < there)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                         :: "r"(smem_u32(&m.gate[t * kLinearDim + 8 * piece])),
+                            "l"(a.gate.data + (row0 + c * kChunk + t) * a.gate.row_stride + head * a.gate.head_stride + 8 * piece) : "memory");
         }
       }
       wait(&m.out_full, c);
@@ -311,42 +363,67 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
         const int broken = m.broken[c & 1][column];
         out_barrier();                                                         // the rows of the chunk before have been read
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float o[32], q[32];
-          tmem_ld32(lanes + kDotsAt + 32 * h, reinterpret_cast<uint32_t*>(o));
-          tmem_ld32(lanes + kReadAt + 32 * h, reinterpret_cast<uint32_t*>(q));
+        for (int h = 0; h < 2; ++h) {                                          // 16 tokens
+          const int token = 32 * group + 16 * h;
+          Pair o[8], q[8];
+          tmem_ld16(lanes + kDotsAt + token, reinterpret_cast<uint32_t*>(o));
+          tmem_ld16(lanes + kReadAt + token, reinterpret_cast<uint32_t*>(q));
           tmem_ld_wait();
           if (h == 1) warp_arrive(&m.dots_empty, lane);
 #pragma unroll
-          for (int t = 0; t < 32; ++t) {
-            const float x = fmaf(numbers.read[32 * h + t], q[t], o[t]) * back;
-            m.out[(32 * h + t) * kOutRow + column] = 32 * h + t < broken ? x : NAN;
+          for (int t = 0; t < 16; t += 4) {
+            const float4 read = *reinterpret_cast<const float4*>(&numbers.read[token + t]);
+            const float2 x = (fma2(Pair(read.x, read.y), q[t / 2], o[t / 2]) * Pair(back, back)).values();
+            const float2 y = (fma2(Pair(read.z, read.w), q[t / 2 + 1], o[t / 2 + 1]) * Pair(back, back)).values();
+            float* to = &m.out[(token + t) * kOutRow + column];
+            to[0] = x.x;
+            to[kOutRow] = x.y;
+            to[2 * kOutRow] = y.x;
+            to[3 * kOutRow] = y.y;
           }
         }
+        for (int t = max(broken, kChunk / kOutGroups * group); t < kChunk / kOutGroups * (group + 1); ++t) m.out[t * kOutRow + column] = NAN;
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&m.empty[c % kStages]));
         out_barrier();
+        // two rows' loads, then the arithmetic, then the stores: rows need not wait for each other
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int t = 8 * i + 2 * w + half;
-          float o[8];
-          *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(&m.out[t * kOutRow + 8 * piece]);
-          *reinterpret_cast<float4*>(o + 4) = *reinterpret_cast<const float4*>(&m.out[t * kOutRow + 8 * piece + 4]);
+        for (int i0 = 0; i0 < kChunk / 2 / kOutWarps; i0 += 2) {
+          float o[2][8], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float* from = &m.out[(2 * kOutWarps * (i0 + i) + 2 * w + half) * kOutRow + 8 * piece];
+            *reinterpret_cast<float4*>(o[i]) = *reinterpret_cast<const float4*>(from);
+            *reinterpret_cast<float4*>(o[i] + 4) = *reinterpret_cast<const float4*>(from + 4);
+          }
           if (gated) {
-            float sum = 0.0f, z[8], weight[8];
+            if (i0 == 0) asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) sum[i] = fmaf(o[i][j], o[i][j], sum[i]);
+#pragma unroll
+            for (int d = 8; d >= 1; d /= 2)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
+            float weight[8];
             unpack8(weights, weight);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(o[j], o[j], sum);
+            for (int i = 0; i < 2; ++i) {
+              const float factor = rsqrtf(fmaf(sum[i], 1.0f / kLinearDim, a.eps));
+              float z[8];
+              unpack8(*reinterpret_cast<const uint4*>(&m.gate[(2 * kOutWarps * (i0 + i) + 2 * w + half) * kLinearDim + 8 * piece]), z);
 #pragma unroll
-            for (int d = 8; d >= 1; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            const float factor = __frsqrt_rn(fmaf(sum, 1.0f / kLinearDim, a.eps));
-            unpack8(gate[i], z);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] *= factor * weight[j] * (z[j] * linear_sigmoid(z[j]));
+              for (int j = 0; j < 8; ++j) o[i][j] *= factor * weight[j] * (z[j] * linear_sigmoid(z[j]));
+            }
           }
-          if (t < there)
-            *reinterpret_cast<uint4*>(a.out + ((row0 + c * kChunk + t) * a.v_heads + head) * kLinearDim + 8 * piece) =
-                make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int t = 2 * kOutWarps * (i0 + i) + 2 * w + half;
+            if (t < there)
+              *reinterpret_cast<uint4*>(a.out + ((row0 + c * kChunk + t) * a.v_heads + head) * kLinearDim + 8 * piece) =
+                  make_uint4(pack_bf16(o[i][0], o[i][1]), pack_bf16(o[i][2], o[i][3]), pack_bf16(o[i][4], o[i][5]), pack_bf16(o[i][6], o[i][7]));
+          }
         }
       } else {
         warp_arrive(&m.dots_empty, lane);
@@ -358,56 +435,77 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
     if (warp == kChainWarps + kOutWarps) {
       // ------------------------------ products ------------------------------
       // Products of different shapes need not run in the order of issue: one that reads or writes what another wrote waits for its commit.
-      constexpr uint32_t kNarrow = instr_desc_f8(kF16, kF16, 0, 0, 128, kChunk);
-      constexpr uint32_t kWide = instr_desc_f8(kF16, kF16, 0, 1, 128, kLinearDim);
+      // A step with N = 64 takes 32 cycles, one with 128 takes 64.  What the chain waits for goes first.
+      constexpr uint32_t kNarrow = instr_desc_f8(kF16, kF16, 0, 0, 128, kChunk), kUpdate = instr_desc_f8(kF16, kF16, 0, 1, 128, kLinearDim);
+      // descriptors: those of a stage's begin, to which constants are added (an address takes their low 14 bits)
       const uint32_t base = smem_u32(m.stages[0]);
       for (int c = 0; c < n; ++c) {
-        const uint32_t pair = base + (c % kStages) * kStageBytes, inverse = pair + kChunkPairBytes, scores = inverse + 2 * kChunkMatrixBytes;
-        if (!wait(&m.full[c % kStages], c / kStages) || !wait(&m.state_ready, c) || (c > 0 && !wait(&m.dots_empty, c - 1))) break;
+        const uint32_t at = base + (c % kStages) * kStageBytes;
+        const uint64_t rows_desc = smem_desc_rows<128>(at), update_desc = smem_desc_rows<128>(at, kChunkPanelBytes);
+        auto dots = [&](int half, uint32_t to, uint32_t rows_at) {                // of a half of each group's key elements
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int term = i & 1, g = (i >> 1) % kChainGroups, k = g * (kKeys / 16) + half * (kKeys / 32) + (i >> 1) / kChainGroups;
+            if ((i >> 1) / kChainGroups < kKeys / 32)
+              umma_f16_ts(to, kTermsAt + operand(k, term), rows_desc + ((rows_at + (k / 4) * kChunkPanelBytes + (k % 4) * 32) >> 4), kNarrow, (half | i) != 0);
+          }
+        };
+        if (!wait(&m.full[c % kStages], c / kStages) || (c > 0 && !wait(&m.dots_empty, c - 1)) || !wait(&m.state_ready[0], c)) break;
+        tc_fence_after();
+        if (elect_one()) dots(0, kDotsAt, 0);
+        __syncwarp();
+        if (!wait(&m.state_ready[1], c)) break;
         tc_fence_after();
         if (elect_one()) {
-#pragma unroll
-          for (int term = 0; term < 2; ++term)
-#pragma unroll
-            for (int k = 0; k < kLinearDim / 16; ++k)
-              umma_f16_ts(tmem + kDotsAt, tmem + (term == 0 ? kHighAt : kLowAt) + 8 * k,
-                          smem_desc_rows<128>(pair + (k / 4) * kChunkPanelBytes) + ((k % 4) * 32 >> 4), kNarrow, (term | k) != 0);
+          dots(1, kDotsAt, 0);
           umma_commit(smem_u32(&m.dots_full));
-#pragma unroll
-          for (int term = 0; term < 2; ++term)
-#pragma unroll
-            for (int k = 0; k < kLinearDim / 16; ++k)
-              umma_f16_ts(tmem + kReadAt, tmem + (term == 0 ? kHighAt : kLowAt) + 8 * k,
-                          smem_desc_rows<128>(pair + (k / 4) * kChunkPanelBytes + kChunk * 128) + ((k % 4) * 32 >> 4), kNarrow, (term | k) != 0);
+          dots(0, kReadAt, kChunk * 128);
+          dots(1, kReadAt, kChunk * 128);
         }
         __syncwarp();
-        if (!wait(&m.enter_ready, c)) break;
+        bool alive = true;
+#pragma unroll
+        for (int half = 0; half < 2 && alive; ++half) {                           // of each group's tokens
+          alive = wait(&m.enter_ready[half], c);
+          tc_fence_after();
+          if (alive && elect_one()) {
+#pragma unroll
+            for (int g = 0; g < kChainGroups; ++g)
+#pragma unroll
+              for (int term = 0; term < 3; ++term) {                              // both terms by T's first, the first by T's second
+                const int k = g * (kTokens / 16) + half;
+                umma_f16_ts(kDotsAt, kEnterAt + operand(k, term == 1), rows_desc + ((kChunkPairBytes + (term == 2 ? kChunkMatrixBytes : 0) + k * 32) >> 4), kNarrow,
+                            (half | g | term) != 0);
+              }
+            if (half == 1) umma_commit(smem_u32(&m.fresh_full));
+          }
+          __syncwarp();
+        }
+#pragma unroll
+        for (int half = 0; half < 2 && alive; ++half) {
+          alive = wait(&m.stay_ready[half], c);
+          tc_fence_after();
+          if (alive && elect_one()) {
+#pragma unroll
+            for (int g = 0; g < kChainGroups; ++g)
+#pragma unroll
+              for (int term = 0; term < 2; ++term) {
+                const int k = g * (kTokens / 16) + half;
+                umma_f16_ts(kStateAt, kEnterAt + operand(k, term), update_desc + ((k * 16 * 128) >> 4), kUpdate, 1);
+              }
+            if (half == 1) umma_commit(smem_u32(&m.state_full));
+          }
+          __syncwarp();
+        }
+        if (!alive || !wait(&m.fresh_ready, c)) break;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int term = 0; term < 3; ++term)                                   // both terms by T's first, the first by T's second
+          for (int term = 0; term < 3; ++term)                                    // both terms by the scores' first, the first by their second
 #pragma unroll
             for (int k = 0; k < kChunk / 16; ++k)
-              umma_f16_ts(tmem + kDotsAt, tmem + kEnterAt + (term == 1 ? 32 : 0) + 8 * k,
-                          smem_desc_rows<128>(inverse + (term == 2 ? kChunkMatrixBytes : 0)) + (k * 32 >> 4), kNarrow, (term | k) != 0);
-          umma_commit(smem_u32(&m.fresh_full));
-        }
-        __syncwarp();
-        if (!wait(&m.stay_ready, c)) break;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int term = 0; term < 2; ++term)
-#pragma unroll
-            for (int k = 0; k < kChunk / 16; ++k)
-              umma_f16_ts(tmem + kStateAt, tmem + kEnterAt + 32 * term + 8 * k, smem_desc_rows<128>(pair + k * 16 * 128, kChunkPanelBytes), kWide, 1);
-          umma_commit(smem_u32(&m.state_full));
-#pragma unroll
-          for (int term = 0; term < 3; ++term)
-#pragma unroll
-            for (int k = 0; k < kChunk / 16; ++k)
-              umma_f16_ts(tmem + kDotsAt, tmem + kFreshAt + (term == 1 ? 32 : 0) + 8 * k,
-                          smem_desc_rows<128>(scores + (term == 2 ? kChunkMatrixBytes : 0)) + (k * 32 >> 4), kNarrow, (term | k) != 0);
+              umma_f16_ts(kDotsAt, kFreshAt + operand(k, term == 1),
+                          rows_desc + ((kChunkPairBytes + (term == 2 ? 3 : 2) * kChunkMatrixBytes + k * 32) >> 4), kNarrow, (term | k) != 0);
           umma_commit(smem_u32(&m.out_full));
           umma_commit(smem_u32(&m.empty[c % kStages]));
         }
@@ -420,20 +518,56 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
         const int slot = c % kStages;
         if (!wait(&m.empty[slot], c / kStages + 1)) break;
         const uint32_t to = smem_u32(m.stages[slot]), bar = smem_u32(&m.full[slot]);
-        const int there = min(kChunk, rows - c * kChunk);
         if (lane == 0) {
-          mbar_arrive_expect_tx(bar, kStageValues + there * 2 * kLinearDim);
+          mbar_arrive_expect_tx(bar, kStageValues);
           const size_t tile = static_cast<size_t>(tile0 + c);
           bulk_g2s(to, plan.pairs + (tile * a.k_heads + head / a.group) * kChunkPairBytes, kChunkPairBytes, bar);
           bulk_g2s(to + kChunkPairBytes, plan.heads + (tile * a.v_heads + head) * kChunkHeadBytes, kChunkHeadBytes, bar);
         }
         __syncwarp();
-        for (int t = lane; t < there; t += 32)
-          bulk_g2s(to + kStageValues + t * 2 * kLinearDim, a.v.data + (row0 + c * kChunk + t) * a.v.row_stride + head * a.v.head_stride, 2 * kLinearDim, bar);
       }
       if (*abort_flag != 0) {                // what is in flight lands before the block leaves
         volatile int ignore = 0;
         for (int i = max(0, c - kStages); i < c; ++i) wait_inline(smem_u32(&m.full[i % kStages]), (i / kStages) & 1, &ignore, kWaitBudgetNs);
+      }
+    } else {
+      // ------------------------------ values, and the largest of each column ------------------------------
+      // 16 lanes a row, 16 rows a thread.  (A copy of 256 bytes for each row took 70 cycles to issue, 5000 for the chunk.)
+      const int which = warp & 1, piece = lane & 15, first = 2 * which + (lane >> 4);
+      for (int c = 0; c < n; ++c) {
+        const int slot = c % kStages, there = min(kChunk, rows - c * kChunk);
+        uint8_t* to = m.stages[slot] + kStageValues + first * 2 * kLinearDim + piece * 16;
+        const __nv_bfloat16* from = a.v.data + (row0 + c * kChunk + first) * a.v.row_stride + head * a.v.head_stride + 8 * piece;
+        wait(&m.empty[slot], c / kStages + 1);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool is = first + 4 * i < there;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                       :: "r"(smem_u32(to + i * 4 * 2 * kLinearDim)), "l"(is ? from + 4 * i * a.v.row_stride : a.v.data), "r"(is ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        uint32_t most[4] = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+          const uint4 x = *reinterpret_cast<const uint4*>(to + i * 4 * 2 * kLinearDim);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t y = (&x.x)[j] & 0x7fff7fffu;
+            if ((y & 0xffffu) >= 0x7f80u) y &= 0xffff0000u;
+            if (y >= 0x7f800000u) y &= 0xffffu;
+            most[j] = __vmaxu2(most[j], y);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most[j] = __vmaxu2(most[j], __shfl_xor_sync(0xffffffffu, most[j], 16));
+        if (lane < 16) {
+          float4* largest = reinterpret_cast<float4*>(&m.largest_value[slot][which][8 * piece]);
+          largest[0] = make_float4(bf16_lo(most[0]), bf16_hi(most[0]), bf16_lo(most[1]), bf16_hi(most[1]));
+          largest[1] = make_float4(bf16_lo(most[2]), bf16_hi(most[2]), bf16_lo(most[3]), bf16_hi(most[3]));
+        }
+        wait(&m.full[slot], c / kStages);                                         // for those that wait for this alone
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&m.values_full[slot]));
       }
     }
   }

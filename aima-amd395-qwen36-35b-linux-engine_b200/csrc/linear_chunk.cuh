@@ -27,7 +27,8 @@ constexpr int kChunkPanelBytes = kChunkPairBytes / 2;
 constexpr int kChunkMatrixBytes = kChunk * kChunk * 2;           // T's first terms, its second, the scores' first, their second: rows of 128 bytes, swizzled
 constexpr int kChunkNumbersAt = 4 * kChunkMatrixBytes;
 struct ChunkNumbers {                                            // of a chunk and value head
-  float2 enter[kChunk];        // beta; beta e^G / |k|
+  float rate[kChunk];          // beta
+  float enter[kChunk];         // -beta e^G / |k|
   float stay[kChunk];          // e^(G_last - G) / |k|
   float read[kChunk];          // e^G / |q|
   float stay_kept[kChunk];     // as `stay`, for the last token that enters the state; 0 behind it
@@ -60,6 +61,12 @@ __device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint64_t adesc, uin
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
@@ -74,6 +81,35 @@ __device__ __forceinline__ void split_f16(float x0, float x1, uint32_t* high, ui
       "fma.rn.f32.f16 %0, l, m, %3;\n\tfma.rn.f32.f16 %1, u, m, %4;\n\t}"
       : "=f"(l0), "=f"(l1) : "r"(*high), "f"(x0), "f"(x1));
   *low = cvt_f16x2(l0, l1);
+}
+struct Pair {                  // two FP32 numbers that one instruction takes
+  unsigned long long bits;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ float2 values() const {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(bits));
+    return v;
+  }
+};
+__device__ __forceinline__ Pair operator*(const Pair& a, const Pair& b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
+  return d;
+}
+__device__ __forceinline__ Pair operator+(const Pair& a, const Pair& b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
+  return d;
+}
+__device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return d;
+}
+__device__ __forceinline__ void split_f16(const Pair& x, uint32_t* high, uint32_t* low) {
+  const float2 v = x.values();
+  split_f16(v.x, v.y, high, low);
 }
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   float y;

@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(kPrepareThreads) linear_prepare_kernel(const C
         m.rate[warp][t] = beta[i];
         const float k_length = m.length[t], q_length = m.length[kChunk + t], reach = exp2f(high);
         const bool there = t < rows;
-        numbers->enter[t] = make_float2(beta[i], broken[i] ? NAN : there ? beta[i] * reach * k_length : 0.0f);
+        numbers->rate[t] = beta[i];
+        numbers->enter[t] = broken[i] ? NAN : there ? -(beta[i] * reach * k_length) : 0.0f;
         numbers->stay[t] = there ? exp2f(static_cast<float>(last - total[i])) * k_length : 0.0f;
         numbers->read[t] = !there ? 0.0f : m.broken[kChunk + t] != 0 ? NAN : reach * q_length;
         numbers->stay_kept[t] = t < kept ? exp2f(static_cast<float>(last_kept - total[i])) * k_length : 0.0f;

@@ -48,7 +48,7 @@ def conv(x, weight, states, batch):
 
 def delta(q, k, v, a, b, a_log, dt_bias, states, batch, eps=1.0e-6, gate=None, norm_weight=None, floor=0.0):
     """{"out", "states", "out_error", "state_error", "reach"}.  `floor` is for arithmetic in chunks of 64 tokens, which holds a column and its
-    values to so much of the largest that they come to within a chunk: that much is added to e with every chunk.  out_error [tokens, heads, 128] and state_error [slots, heads, 128] (of a
+    values to so much of the largest that they come to within a chunk and the one before: that much is added to e with every chunk.  out_error [tokens, heads, 128] and state_error [slots, heads, 128] (of a
     column) are the bound above for c = 1 and a rounding of 1; reach [tokens, heads, 128] is the length of the column that the query
     reads, and with it of what it has added up, over sqrt(128).  Rows of no sequence are NaN."""
     device = v.device
@@ -70,7 +70,7 @@ def delta(q, k, v, a, b, a_log, dt_bias, states, batch, eps=1.0e-6, gate=None, n
         s = torch.zeros_like(states[slot]) if fresh else states[slot].clone()
         e = torch.zeros(heads, DIM, dtype=torch.float64, device=device)
         n = s.square().sum(1).sqrt()
-        largest = torch.zeros_like(n)
+        largest, largest_before = torch.zeros_like(n), torch.zeros_like(n)
         for t in range(row0 + first, row0 + rows):
             largest = torch.maximum(largest, torch.maximum(n, v[t].abs()).nan_to_num(0.0, 0.0))
             al, be, kt = alpha[t, :, None], beta[t, :, None], k[t][..., None]
@@ -84,11 +84,12 @@ def delta(q, k, v, a, b, a_log, dt_bias, states, batch, eps=1.0e-6, gate=None, n
             out_error[t] = e / math.sqrt(DIM) + reach[t]
             here, last = t - row0 - first, t == row0 + rows - 1
             if t - row0 + 1 == kept:
-                states[slot], state_error[slot] = s, e + floor * largest
+                states[slot], state_error[slot] = s, e + floor * torch.maximum(largest, largest_before)
             if here % 64 == 63 or last:
-                out_error[t - here % 64:t + 1] += floor * largest / math.sqrt(DIM)
-                e = e + floor * largest
-                largest = torch.zeros_like(n)
+                held = torch.maximum(largest, largest_before)
+                out_error[t - here % 64:t + 1] += floor * held / math.sqrt(DIM)
+                e = e + floor * held
+                largest_before, largest = largest, torch.zeros_like(n)
     result = {"out": out, "states": states, "out_error": out_error, "state_error": state_error, "reach": reach}
     if gate is not None:
         z, w = gate.double(), norm_weight.double()
