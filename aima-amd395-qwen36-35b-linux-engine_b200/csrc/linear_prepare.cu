@@ -1,44 +1,109 @@
 // The gated delta rule in chunks, first kernel: what a chunk needs that does not depend on the state (formulas in linear_chunk.cuh).
 //
 // A block takes a chunk and a key head.  k and q are scaled by a power of two per row to f16; one product of [k; q] with k gives k.k
-// and q.k of all pairs of tokens, exactly but for the order of the sums.  Then, for every value head of that key head: sums of g
-// (64 bits, kept as two FP32 numbers, so that differences of large sums keep theirs), decays, the scores, and the inverse of the unit
-// lower triangle 1 + A by blocks of 16: the diagonal's by substitution, those below from T_ij = -T_ii sum_k A_ik T_kj.
+// and q.k of all pairs of tokens, exactly but for the order of the sums.  Then, for every value head of that key head:
+// sums of g (64 bits, kept as two FP32 numbers, so that differences of large sums keep theirs), decays, the scores, and the inverse of
+// the unit lower triangle 1 + A by blocks of 16.  Decays between tokens of different blocks are products of two, from a token to its
+// block's first and from that to the other token, which spares three quarters of the exponentials.  The diagonal's blocks are inverted
+// by substitution; those below follow, a warp per column of blocks, from
+//   X_i = T_ij = -T_ii (A_ij T_jj + sum_(j < k < i) A_ik X_k),
+// transposed: the accumulators of each product are the first operand of the next as they lie in the warp's registers.  All operands
+// have two f16 terms.
 #include "linear_chunk.cuh"
 
 namespace aima {
 namespace {
 
-constexpr int kPrepareThreads = 256;
-constexpr int kHeadsAtOnce = 8;                 // a warp each for their sums
-constexpr int kRow = kChunk + 4;                // of a matrix in shared memory
+constexpr int kRowWarps = 8, kGateWarps = 2;
+constexpr int kPrepareThreads = 32 * (kRowWarps + kGateWarps);
+constexpr int kHeadsAtOnce = kGateWarps;        // whose gates are taken together
+constexpr int kHalfRow = kChunk + 8;            // of a 16-bit matrix in shared memory
+constexpr int kBlockRow = 20;                   // of a block of the diagonal
 
+struct __align__(16) Terms {                    // a matrix in two terms, without swizzle
+  uint16_t of[2][kChunk * kHalfRow];
+};
 struct __align__(1024) PrepareMemory {
-  uint8_t pair[kChunkPairBytes];
-  float overlap[kChunk * kRow];                 // A
-  float inverse[kChunk * kRow];                 // T
-  float partial[3 * 16 * 20];                   // of three blocks
+  union {
+    uint8_t pair[kChunkPairBytes];              // until its products are there
+    struct {
+      Terms overlap, scores;                    // A, q.k
+    };
+  };
+  Terms inverse;                                // T
+  float diagonal[4][16 * kBlockRow];            // A's
   float length[2 * kChunk];                     // 1 / |k|, then 1 / |q|, of the scaled rows
   int broken[2 * kChunk];                       // rows that are not finite
   float sum_high[kHeadsAtOnce][kChunk], sum_low[kHeadsAtOnce][kChunk];         // log2(e) G
-  float rate[kHeadsAtOnce][kChunk];             // beta, 0 for a row that is not finite
+  float rate[kHeadsAtOnce][kChunk];             // beta, 0 for a token whose gates are not numbers
+  float down[kHeadsAtOnce][kChunk];             // from a block's first token to a token of it
+  float across[kHeadsAtOnce][4][kChunk];        // from a token to the first one of a later block
+  int found[2];
+  int sums[kPrepareThreads / 32];
   unsigned long long done;
   uint32_t tmem;
   int abort_flag;
 };
 
-__device__ __forceinline__ float quarter_max(float v) {          // over 16 lanes
-#pragma unroll
-  for (int d = 8; d >= 1; d /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-  return v;
+__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, const uint32_t* b) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-__device__ __forceinline__ float quarter_sum(float v) {
+// 16 x 16 of a matrix in two terms as a first operand, transposed
+__device__ __forceinline__ void load_transposed(const uint16_t* at, int lane, uint32_t* a) {
+  // tiles of 8: (rows 0, columns 0), (rows 0, columns 8), (rows 8, columns 0), (rows 8, columns 8) of the matrix
+  const uint32_t from = smem_u32(at + ((lane & 7) + (lane >> 4) * 8) * kHalfRow + ((lane >> 3) & 1) * 8);
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(from) : "memory");
+}
+// the other way
+__device__ __forceinline__ void store_transposed(uint16_t* at, int lane, const uint32_t* a) {
+  const uint32_t to = smem_u32(at + ((lane & 7) + (lane >> 4) * 8) * kHalfRow + ((lane >> 3) & 1) * 8);
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" :: "r"(to), "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]) : "memory");
+}
+// d[2][4] (16 x 16) += x y^T of x in two terms (first operand) and a 16 x 16 block y in two terms
+__device__ __forceinline__ void add_product(float (*d)[4], const uint32_t (*x)[4], const Terms& y, int row, int column, int lane) {
 #pragma unroll
-  for (int d = 8; d >= 1; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
-  return v;
+  for (int n = 0; n < 2; ++n) {
+    uint32_t b[2][2];
+#pragma unroll
+    for (int term = 0; term < 2; ++term) {
+      const uint16_t* from = &y.of[term][(row + 8 * n + (lane >> 2)) * kHalfRow + column + 2 * (lane & 3)];
+      b[term][0] = *reinterpret_cast<const uint32_t*>(from);
+      b[term][1] = *reinterpret_cast<const uint32_t*>(from + 8);
+    }
+    mma_f16(d[n], x[0], b[0]);
+    mma_f16(d[n], x[1], b[0]);
+    mma_f16(d[n], x[0], b[1]);
+  }
+}
+// accumulators times `sign` as a first operand in two terms
+__device__ __forceinline__ void as_operand(const float (*d)[4], float sign, uint32_t (*x)[4]) {
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    split_f16(sign * d[n][0], sign * d[n][1], &x[0][2 * n], &x[1][2 * n]);
+    split_f16(sign * d[n][2], sign * d[n][3], &x[0][2 * n + 1], &x[1][2 * n + 1]);
+  }
 }
 
-__global__ void __launch_bounds__(kPrepareThreads) linear_prepare_kernel(const ChunkPlan plan) {
+// A lower triangle in two terms to where the second kernel takes it from, by 256 threads; zeros in the blocks above it.
+template <int kTerms>
+__device__ __forceinline__ void write_terms(const Terms& from, uint8_t* to, int thread) {
+  const int piece = thread & 7, row = thread >> 3;
+#pragma unroll
+  for (int term = 0; term < kTerms; ++term) {
+#pragma unroll
+    for (int r = row; r < kChunk; r += 32)
+      *reinterpret_cast<uint4*>(to + term * kChunkMatrixBytes + swizzled(r, piece)) =
+          piece / 2 <= r / 16 ? *reinterpret_cast<const uint4*>(&from.of[term][r * kHalfRow + 8 * piece]) : make_uint4(0, 0, 0, 0);
+  }
+}
+__device__ __forceinline__ void row_barrier() {
+  tc_fence_before();
+  asm volatile("bar.sync 1, %0;" :: "n"(32 * kRowWarps) : "memory");
+  tc_fence_after();
+}
+
+__global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(const ChunkPlan plan) {
   extern __shared__ uint8_t raw[];
   PrepareMemory& m = *reinterpret_cast<PrepareMemory*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const LinearDelta& a = plan.a;
@@ -47,9 +112,14 @@ __global__ void __launch_bounds__(kPrepareThreads) linear_prepare_kernel(const C
   if (tile == 0 && k_head == 0) linear_report(a.batch, a.status, threadIdx.x, kPrepareThreads);
 
   // the sequence and chunk of this tile
-  __shared__ int found[2];
-  __shared__ int sums[kPrepareThreads / 32];
-  {
+  if (warp == 0) tmem_alloc(smem_u32(&m.tmem), 64);
+  if (threadIdx.x == 0) {
+    m.found[0] = -1;
+    m.abort_flag = 0;
+    mbar_init(smem_u32(&m.done), 1);
+    mbar_fence_init();
+  }
+  if (a.batch.sequences > 1) {
     const int share = (a.batch.sequences + kPrepareThreads - 1) / kPrepareThreads;
     const int first = threadIdx.x * share, last = min(first + share, a.batch.sequences);
     int mine = 0;
@@ -60,148 +130,179 @@ __global__ void __launch_bounds__(kPrepareThreads) linear_prepare_kernel(const C
       const int x = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += x;
     }
-    if (lane == 31) sums[warp] = upto;
-    if (threadIdx.x == 0) {
-      found[0] = -1;
-      m.abort_flag = 0;
-      mbar_init(smem_u32(&m.done), 1);
-      mbar_fence_init();
-    }
+    if (lane == 31) m.sums[warp] = upto;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) upto += sums[w];
+    for (int w = 0; w < warp; ++w) upto += m.sums[w];
     int at = upto - mine;
     if (at <= tile && tile < upto) {
       for (int s = first; s < last; ++s) {
         const int chunks = chunks_of(linear_sequence(a.batch, s), plan.min_rows);
         if (tile < at + chunks) {
-          found[0] = s;
-          found[1] = tile - at;
+          m.found[0] = s;
+          m.found[1] = tile - at;
           break;
         }
         at += chunks;
       }
     }
-    __syncthreads();
+  } else if (threadIdx.x == 0 && tile < chunks_of(linear_sequence(a.batch, 0), plan.min_rows)) {
+    m.found[0] = 0;
+    m.found[1] = tile;
   }
-  if (found[0] < 0) return;
-  const LinearSequence seq = linear_sequence(a.batch, found[0]);
-  const int begin = seq.first + found[1] * kChunk;
-  const int rows = min(kChunk, seq.rows - begin);
-  const int kept = min(max(seq.kept - begin, 0), rows);
-  const long long row0 = seq.row0 + begin;
-  if (warp == 0) tmem_alloc(smem_u32(&m.tmem), 64);
-
-  // k's rows, then q's: 16 lanes a row, eight rows a thread
-  uint8_t* pair = plan.pairs + (static_cast<size_t>(tile) * a.k_heads + k_head) * kChunkPairBytes;
-  {
-    const int piece = lane & 15, half = lane >> 4;
-    uint4 data[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 16 * i + 2 * warp + half, t = r & (kChunk - 1);
-      const KvRows& from = r < kChunk ? a.k : a.q;
-      data[i] = t < rows ? *reinterpret_cast<const uint4*>(from.data + (row0 + t) * from.row_stride + k_head * from.head_stride + 8 * piece) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 16 * i + 2 * warp + half;
-      float x[8];
-      unpack8(data[i], x);
-      float largest = 0.0f;
-      bool finite = true;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        largest = fmaxf(largest, fabsf(x[j]));
-        finite = finite && fabsf(x[j]) < INFINITY;
-      }
-      largest = quarter_max(finite ? largest : INFINITY);
-      const bool broken = !(largest < INFINITY);
-      // 2^-e with 2^e <= max < 2^(e + 1); a row of zeros, subnormal or broken: e as near as may be
-      const int e = broken ? 0 : min(max(kv_float_exponent(largest), -126), 126);
-      const float scale = kv_exp2(-e);
-      float sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = broken ? 0.0f : x[j] * scale;
-        sum = fmaf(x[j], x[j], sum);
-      }
-      sum = quarter_sum(sum);
-      if (piece == 0) {
-        // 2^e / sqrt(|x|^2 + eps) from |x 2^-e|^2; 2^-2e in two steps
-        m.length[r] = broken ? 0.0f : 1.0f / sqrtf(sum + a.eps * scale * scale);
-        m.broken[r] = broken;
-      }
-      const uint4 packed = make_uint4(cvt_f16x2(x[0], x[1]), cvt_f16x2(x[2], x[3]), cvt_f16x2(x[4], x[5]), cvt_f16x2(x[6], x[7]));
-      const uint32_t at = (piece >> 3) * kChunkPanelBytes + swizzled(r, piece & 7);
-      *reinterpret_cast<uint4*>(m.pair + at) = packed;
-      *reinterpret_cast<uint4*>(pair + at) = packed;
-    }
-  }
-  fence_async_proxy();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = m.tmem;
-  if (warp == 0) {
-    if (elect_one()) {
-      constexpr uint32_t kForm = instr_desc_f8(kF16, kF16, 0, 0, 128, kChunk);
-      const uint32_t base = smem_u32(m.pair);
-#pragma unroll
-      for (int k = 0; k < kLinearDim / 16; ++k) {
-        const uint64_t desc = smem_desc_rows<128>(base + (k / 4) * kChunkPanelBytes) + ((k % 4) * 32 >> 4);
-        umma_f16_ss(tmem, desc, desc, kForm, k != 0);
-      }
-      umma_commit(smem_u32(&m.done));
-    }
-    __syncwarp();
-  }
-
-  const int half = warp >> 2, row = (warp & 3) * 32 + lane;         // row of [k; q], columns 32 half ..
-  float dots[32];
+  const bool there_is = m.found[0] >= 0;
+  const LinearSequence seq = linear_sequence(a.batch, max(m.found[0], 0));
+  const int begin = seq.first + m.found[1] * kChunk;
+  const int rows = there_is ? min(kChunk, seq.rows - begin) : 0;
+  const int kept = min(max(seq.kept - begin, 0), rows);
+  const long long row0 = seq.row0 + begin;
   bool alive = true;
-  for (int base = 0; base < a.group; base += kHeadsAtOnce) {
+  const int half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane, token = row & (kChunk - 1), block = token >> 4;
+  for (int base = 0; there_is && base < a.group; base += kHeadsAtOnce) {
     const int heads = min(kHeadsAtOnce, a.group - base);
-    if (warp < heads) {
-      const int head = k_head * a.group + base + warp;
-      ChunkNumbers* numbers = reinterpret_cast<ChunkNumbers*>(plan.heads + (static_cast<size_t>(tile) * a.v_heads + head) * kChunkHeadBytes + kChunkNumbersAt);
-      float g[2], beta[2];
-      bool broken[2];
-      const float slope = expf(a.a_log[head]) * 1.44269504088896341f, bias = a.dt_bias[head];
+    double total[2] = {0.0, 0.0}, last = 0.0;
+    float beta[2] = {0.0f, 0.0f};
+    bool broken[2] = {false, false};
+    if (warp >= kRowWarps) {
+      // sums of g and decays: two tokens a lane, a head a warp
+      const int h = warp - kRowWarps, head = k_head * a.group + base + h;
+      if (h < heads) {
+        float g[2] = {0.0f, 0.0f}, x[2] = {0.0f, 0.0f}, y[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int t = 2 * lane + i;
-        g[i] = beta[i] = 0.0f;
-        broken[i] = false;
-        if (t < rows) {
-          const float x = __bfloat162float(a.a[(row0 + t) * a.a_stride + head]) + bias;
-          g[i] = -slope * (x > 20.0f ? x : log1pf(expf(x)));
-          beta[i] = 1.0f / (1.0f + expf(-__bfloat162float(a.b[(row0 + t) * a.b_stride + head])));
-          broken[i] = m.broken[t] != 0 || g[i] != g[i] || beta[i] != beta[i];
-          if (broken[i]) g[i] = beta[i] = 0.0f;
-          g[i] = fmaxf(g[i], -1.0e6f);                   // e^g is 0 long before
+        for (int i = 0; i < 2; ++i) {
+          if (2 * lane + i < rows) {
+            x[i] = __bfloat162float(a.a[(row0 + 2 * lane + i) * a.a_stride + head]);
+            y[i] = __bfloat162float(a.b[(row0 + 2 * lane + i) * a.b_stride + head]);
+          }
+        }
+        const float slope = expf(a.a_log[head]) * 1.44269504088896341f, bias = a.dt_bias[head];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (2 * lane + i < rows) {
+            const float z = x[i] + bias;
+            g[i] = -slope * (z > 20.0f ? z : log1pf(expf(z)));
+            beta[i] = 1.0f / (1.0f + expf(-y[i]));
+            broken[i] = g[i] != g[i] || beta[i] != beta[i];
+            if (broken[i]) g[i] = beta[i] = 0.0f;
+            g[i] = fmaxf(g[i], -1.0e6f);                             // e^g is 0 long before
+          }
+        }
+        double upto = static_cast<double>(g[0]) + g[1];
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+          const double z = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += z;
+        }
+        total[0] = upto - g[1];
+        total[1] = upto;
+        last = __shfl_sync(0xffffffffu, upto, 31);                   // rows behind the last have g = 0
+        double first[4];                                             // of each block
+#pragma unroll
+        for (int b = 0; b < 4; ++b) first[b] = __shfl_sync(0xffffffffu, total[0], 8 * b);
+        const double mine = lane < 8 ? first[0] : lane < 16 ? first[1] : lane < 24 ? first[2] : first[3];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int t = 2 * lane + i;
+          const float high = static_cast<float>(total[i]);
+          m.sum_high[h][t] = high;
+          m.sum_low[h][t] = static_cast<float>(total[i] - high);
+          m.rate[h][t] = beta[i];
+          m.down[h][t] = fast_exp2(static_cast<float>(total[i] - mine));
+#pragma unroll
+          for (int b = 1; b < 4; ++b) m.across[h][b][t] = t < 16 * b ? fast_exp2(static_cast<float>(first[b] - total[i])) : 0.0f;
         }
       }
-      double upto = static_cast<double>(g[0]) + g[1];
+    } else if (base == 0) {
+      // k's rows, then q's: four lanes a row, two rows a thread
+      uint8_t* const pair = plan.pairs + (static_cast<size_t>(tile) * a.k_heads + k_head) * kChunkPairBytes;
+      uint4 data[2][4];
 #pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const double x = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += x;
+      for (int i = 0; i < 2; ++i) {
+        const int t = 8 * warp + (lane >> 2);
+        const KvRows& from = i == 0 ? a.k : a.q;
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+          data[i][p] = t < rows ? *reinterpret_cast<const uint4*>(from.data + (row0 + t) * from.row_stride + k_head * from.head_stride + 8 * (4 * p + (lane & 3)))
+                                : make_uint4(0, 0, 0, 0);
       }
-      const double total[2] = {upto - g[1], upto};
-      const double last = __shfl_sync(0xffffffffu, upto, 31);          // rows behind the last have g = 0
-      const double last_kept_pair0 = __shfl_sync(0xffffffffu, total[0], max(kept - 1, 0) >> 1), last_kept_pair1 = __shfl_sync(0xffffffffu, total[1], max(kept - 1, 0) >> 1);
-      const double last_kept = kept == 0 ? 0.0 : ((kept - 1) & 1) != 0 ? last_kept_pair1 : last_kept_pair0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = i * kChunk + 8 * warp + (lane >> 2);
+        uint32_t most = 0;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          most = __vmaxu2(most, data[i][p].x & 0x7fff7fffu);
+          most = __vmaxu2(most, data[i][p].y & 0x7fff7fffu);
+          most = __vmaxu2(most, data[i][p].z & 0x7fff7fffu);
+          most = __vmaxu2(most, data[i][p].w & 0x7fff7fffu);
+        }
+        most = max(most & 0xffffu, most >> 16);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const bool bad = most >= 0x7f80u;
+        // 2^-e with 2^e <= max < 2^(e + 1); a row of zeros, subnormal or broken: e as near as may be
+        const int e = bad ? 0 : min(max(static_cast<int>(most >> 7) - 127, -126), 126);
+        const float scale = kv_exp2(-e);
+        float sum = 0.0f;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          float x[8];
+          unpack8(data[i][p], x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            x[j] *= scale;
+            sum = fmaf(x[j], x[j], sum);
+          }
+          uint4 packed = make_uint4(cvt_f16x2(x[0], x[1]), cvt_f16x2(x[2], x[3]), cvt_f16x2(x[4], x[5]), cvt_f16x2(x[6], x[7]));
+          if (bad) packed = make_uint4(0, 0, 0, 0);
+          const int piece = 4 * p + (lane & 3);
+          const uint32_t at = (piece >> 3) * kChunkPanelBytes + swizzled(r, piece & 7);
+          *reinterpret_cast<uint4*>(m.pair + at) = packed;
+          *reinterpret_cast<uint4*>(pair + at) = packed;
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if ((lane & 3) == 0) {
+          // 2^e / sqrt(|x|^2 + eps) from |x 2^-e|^2
+          m.length[r] = bad ? 0.0f : 1.0f / sqrtf(sum + a.eps * scale * scale);
+          m.broken[r] = bad;
+        }
+      }
+      fence_async_proxy();
+      row_barrier();
+      if (warp == 0) {
+        if (elect_one()) {
+          constexpr uint32_t kForm = instr_desc_f8(kF16, kF16, 0, 0, 128, kChunk);
+          const uint64_t desc = smem_desc_rows<128>(smem_u32(m.pair));
+#pragma unroll
+          for (int k = 0; k < kLinearDim / 16; ++k) {
+            const uint64_t at = desc + (((k / 4) * kChunkPanelBytes + (k % 4) * 32) >> 4);
+            umma_f16_ss(tmem, at, at, kForm, k != 0);
+          }
+          umma_commit(smem_u32(&m.done));
+        }
+        __syncwarp();
+      }
+      alive = mbar_wait_bounded_warp(smem_u32(&m.done), 0, &m.abort_flag, plan.wait_limit_ns);
+      tc_fence_after();
+    }
+    __syncthreads();                                                 // the gates are there; A and the scores take the rows' place
+    if (warp >= kRowWarps && warp - kRowWarps < heads) {
+      // what the second kernel multiplies by
+      const int head = k_head * a.group + base + warp - kRowWarps;
+      ChunkNumbers* numbers = reinterpret_cast<ChunkNumbers*>(plan.heads + (static_cast<size_t>(tile) * a.v_heads + head) * kChunkHeadBytes + kChunkNumbersAt);
+      const double pair0 = __shfl_sync(0xffffffffu, total[0], max(kept - 1, 0) >> 1), pair1 = __shfl_sync(0xffffffffu, total[1], max(kept - 1, 0) >> 1);
+      const double last_kept = kept == 0 ? 0.0 : ((kept - 1) & 1) != 0 ? pair1 : pair0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int t = 2 * lane + i;
-        const float high = static_cast<float>(total[i]);
-        m.sum_high[warp][t] = high;
-        m.sum_low[warp][t] = static_cast<float>(total[i] - high);
-        m.rate[warp][t] = beta[i];
-        const float k_length = m.length[t], q_length = m.length[kChunk + t], reach = exp2f(high);
         const bool there = t < rows;
+        const float k_length = m.length[t], q_length = m.length[kChunk + t], reach = exp2f(static_cast<float>(total[i]));
         numbers->rate[t] = beta[i];
-        numbers->enter[t] = broken[i] ? NAN : there ? -(beta[i] * reach * k_length) : 0.0f;
+        numbers->enter[t] = broken[i] || m.broken[t] != 0 ? NAN : there ? -(beta[i] * reach * k_length) : 0.0f;
         numbers->stay[t] = there ? exp2f(static_cast<float>(last - total[i])) * k_length : 0.0f;
         numbers->read[t] = !there ? 0.0f : m.broken[kChunk + t] != 0 ? NAN : reach * q_length;
         numbers->stay_kept[t] = t < kept ? exp2f(static_cast<float>(last_kept - total[i])) * k_length : 0.0f;
@@ -211,112 +312,108 @@ __global__ void __launch_bounds__(kPrepareThreads) linear_prepare_kernel(const C
         numbers->decay_kept = exp2f(static_cast<float>(last_kept));
       }
     }
-    if (base == 0) {
-      alive = mbar_wait_bounded_warp(smem_u32(&m.done), 0, &m.abort_flag, plan.wait_limit_ns);
-      tc_fence_after();
-      tmem_ld32(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 32 * half, reinterpret_cast<uint32_t*>(dots));
-      tmem_ld_wait();
-    }
-    __syncthreads();
+#pragma unroll 1
     for (int h = 0; h < heads; ++h) {
-      const int head = k_head * a.group + base + h;
-      uint8_t* out = plan.heads + (static_cast<size_t>(tile) * a.v_heads + head) * kChunkHeadBytes;
-      // A, and the scores
-      {
-        const int t = row & (kChunk - 1);
+      uint8_t* const out = plan.heads + (static_cast<size_t>(tile) * a.v_heads + k_head * a.group + base + h) * kChunkHeadBytes;
+      if (warp < kRowWarps) {
+        // A, and the scores: a row of [k; q] and 32 columns a thread
         const bool is_k = row < kChunk;
-        const float high = m.sum_high[h][t], low = m.sum_low[h][t];
-        const float factor = is_k ? m.rate[h][t] * m.length[t] : m.length[row];
-        float x[32];
+        Terms& to = is_k ? m.overlap : m.scores;
+        const float own = (is_k ? m.rate[h][token] : 1.0f) * m.length[row], down = own * m.down[h][token];
+        const float high = m.sum_high[h][token], low = m.sum_low[h][token];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const int c = 32 * half + j;
-          const float apart = fminf((high - m.sum_high[h][c]) + (low - m.sum_low[h][c]), 0.0f);          // above 0 only where nothing is taken
-          x[j] = (is_k ? c < t : c <= t) ? factor * m.length[c] * dots[j] * fast_exp2(apart) : 0.0f;
-        }
-        if (is_k) {
+        for (int q = 0; q < 2; ++q) {                                // 16 columns
+          const int column = 32 * half + 16 * q;
+          float x[16];
+          tmem_ld16(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + column, reinterpret_cast<uint32_t*>(x));
+          tmem_ld_wait();
+          if (column >> 4 < block) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(&m.overlap[t * kRow + 32 * half + j]) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-        } else {
+            for (int j = 0; j < 16; j += 4) {
+              const float4 y = *reinterpret_cast<const float4*>(&m.across[h][block][column + j]), z = *reinterpret_cast<const float4*>(&m.length[column + j]);
+              x[j] *= down * (y.x * z.x);
+              x[j + 1] *= down * (y.y * z.y);
+              x[j + 2] *= down * (y.z * z.z);
+              x[j + 3] *= down * (y.w * z.w);
+            }
+          } else if (column >> 4 == block) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            uint32_t hi[4], lo[4];
+            for (int j = 0; j < 16; ++j) {
+              const float apart = (high - m.sum_high[h][column + j]) + (low - m.sum_low[h][column + j]);
+              x[j] = (is_k ? column + j < token : column + j <= token) ? x[j] * (own * m.length[column + j] * fast_exp2(apart)) : 0.0f;
+            }
+            if (is_k) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) split_f16(x[j + 2 * i], x[j + 2 * i + 1], &hi[i], &lo[i]);
-            const uint32_t at = 2 * kChunkMatrixBytes + swizzled(t, (32 * half + j) / 8);
-            *reinterpret_cast<uint4*>(out + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(out + kChunkMatrixBytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(&m.diagonal[block][(token & 15) * kBlockRow + j]) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+            }
+          }
+          if (column >> 4 < block + !is_k) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 8) {
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) split_f16(x[j + 2 * i], x[j + 2 * i + 1], &hi[i], &lo[i]);
+              *reinterpret_cast<uint4*>(&to.of[0][token * kHalfRow + column + j]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              *reinterpret_cast<uint4*>(&to.of[1][token * kHalfRow + column + j]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
           }
         }
       }
       __syncthreads();
-      // the diagonal's blocks: a column a thread; zeros above them
-      if (threadIdx.x < 64) {
-        const int b = threadIdx.x >> 4, j = threadIdx.x & 15;
-        const float* at = &m.overlap[16 * b * kRow + 16 * b];
+      if (warp < 2) {
+        // the diagonal's blocks: a column a thread
+        const int b = 2 * warp + (lane >> 4), j = lane & 15;
+        const float* at = m.diagonal[b];
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float sum = i == j ? 1.0f : 0.0f;
+          float y[16], sum = i == j ? 1.0f : 0.0f;
 #pragma unroll
-          for (int k = 0; k < i; ++k) sum = fmaf(-at[i * kRow + k], x[k], sum);
+          for (int k = 0; k < i; k += 4) *reinterpret_cast<float4*>(y + k) = *reinterpret_cast<const float4*>(&at[i * kBlockRow + k]);
+#pragma unroll
+          for (int k = 0; k < i; ++k) sum = fmaf(-y[k], x[k], sum);
           x[i] = sum;
-          m.inverse[(16 * b + i) * kRow + 16 * b + j] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          uint32_t hi, lo;
+          split_f16(x[i], x[i + 1], &hi, &lo);
+          uint16_t* first = &m.inverse.of[0][(16 * b + i) * kHalfRow + 16 * b + j];
+          uint16_t* second = &m.inverse.of[1][(16 * b + i) * kHalfRow + 16 * b + j];
+          first[0] = static_cast<uint16_t>(hi);
+          first[kHalfRow] = static_cast<uint16_t>(hi >> 16);
+          second[0] = static_cast<uint16_t>(lo);
+          second[kHalfRow] = static_cast<uint16_t>(lo >> 16);
+        }
+      } else {
+        write_terms<2>(m.scores, out + 2 * kChunkMatrixBytes, threadIdx.x - 64);
+      }
+      __syncthreads();
+      // the blocks below the diagonal's, a column of them a warp
+      if (warp < 3) {
+        const int j = warp;
+        uint32_t x[4][2][4];                                         // x[k]: the block of row j + k, transposed
+#pragma unroll
+        for (int term = 0; term < 2; ++term) load_transposed(&m.inverse.of[term][16 * j * kHalfRow + 16 * j], lane, x[0][term]);
+#pragma unroll
+        for (int d = 1; d < 4; ++d) {
+          if (j + d < 4) {
+            const int i = j + d;
+            float sum[2][4] = {};
+#pragma unroll
+            for (int k = 0; k < d; ++k) add_product(sum, x[k], m.overlap, 16 * i, 16 * (j + k), lane);
+            uint32_t y[2][4];
+            as_operand(sum, -1.0f, y);
+            float z[2][4] = {};
+            add_product(z, y, m.inverse, 16 * i, 16 * i, lane);
+            as_operand(z, 1.0f, x[d]);
+#pragma unroll
+            for (int term = 0; term < 2; ++term) store_transposed(&m.inverse.of[term][16 * i * kHalfRow + 16 * j], lane, x[d][term]);
+          }
         }
       }
       __syncthreads();
-      // block diagonals below: thread = block, row, four columns
-      const int b = threadIdx.x >> 6, i = (threadIdx.x >> 2) & 15, q = 4 * (threadIdx.x & 3);
-#pragma unroll
-      for (int d = 1; d < 4; ++d) {
-        const bool mine = b < 4 - d;
-        const int bi = b + d, bj = b;
-        float4 sum = make_float4(0, 0, 0, 0);
-        if (mine) {
-          for (int k = 16 * bj; k < 16 * bi; ++k) {
-            const float w = m.overlap[(16 * bi + i) * kRow + k];
-            const float4 y = *reinterpret_cast<const float4*>(&m.inverse[k * kRow + 16 * bj + q]);
-            sum.x = fmaf(w, y.x, sum.x);
-            sum.y = fmaf(w, y.y, sum.y);
-            sum.z = fmaf(w, y.z, sum.z);
-            sum.w = fmaf(w, y.w, sum.w);
-          }
-          *reinterpret_cast<float4*>(&m.partial[(b * 16 + i) * 20 + q]) = sum;
-        }
-        __syncthreads();
-        if (mine) {
-          sum = make_float4(0, 0, 0, 0);
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float w = m.inverse[(16 * bi + i) * kRow + 16 * bi + k];
-            const float4 y = *reinterpret_cast<const float4*>(&m.partial[(b * 16 + k) * 20 + q]);
-            sum.x = fmaf(-w, y.x, sum.x);
-            sum.y = fmaf(-w, y.y, sum.y);
-            sum.z = fmaf(-w, y.z, sum.z);
-            sum.w = fmaf(-w, y.w, sum.w);
-          }
-          *reinterpret_cast<float4*>(&m.inverse[(16 * bi + i) * kRow + 16 * bj + q]) = sum;
-        }
-        __syncthreads();
-      }
-      // in two terms: row i, sixteen columns a thread
-      {
-        const int r = threadIdx.x >> 2, c = 16 * (threadIdx.x & 3);
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int column = c + 8 * p + 2 * j;
-            const float2 x = column / 16 <= r / 16 ? *reinterpret_cast<const float2*>(&m.inverse[r * kRow + column]) : make_float2(0.0f, 0.0f);
-            split_f16(x.x, x.y, &hi[j], &lo[j]);
-          }
-          const uint32_t at = swizzled(r, (c + 8 * p) / 8);
-          *reinterpret_cast<uint4*>(out + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(out + kChunkMatrixBytes + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-      }
-      __syncthreads();
+      if (warp >= 2) write_terms<2>(m.inverse, out, threadIdx.x - 64);
     }
     __syncthreads();
   }
