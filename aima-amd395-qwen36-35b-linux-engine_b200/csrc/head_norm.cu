@@ -1,7 +1,7 @@
 // Norm of each head with an optional gate: y = x / sqrt(mean(x^2) + eps) * (w + offset) * act(z), or x * act(z) alone.
 //
 // A head of 64, 128 or 256 lies in 8, 16 or 32 neighbouring lanes, eight elements each: one load per lane and tensor, the sum of
-// squares by shuffles inside them.  All of it is bytes.
+// squares by shuffles inside them.  All of it is bytes, so a thread of a large call has the loads of four heads under way.
 #include "linear.cuh"
 
 namespace aima {
@@ -9,60 +9,93 @@ namespace {
 
 constexpr int kNormThreads = 256;
 
-template <int kDim, bool kNorm, int kActivation>
-__global__ void __launch_bounds__(kNormThreads) head_norm_kernel(const HeadNorm a) {
-  constexpr int kLanes = kDim / 8;                       // of a head
+template <int kDim, bool kNorm, int kActivation, int kUnits>
+__global__ void __launch_bounds__(kNormThreads) head_norm_kernel(const HeadNorm a, const int units) {
+  constexpr int kLanes = kDim / 8, kPerBlock = kNormThreads / kLanes;          // lanes of a head, heads that a block takes at a time
   const int lane = threadIdx.x % kLanes;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kNormThreads / kLanes) + threadIdx.x / kLanes;
-  const bool live = unit < static_cast<long long>(a.tokens) * a.heads;
-  const int row = live ? static_cast<int>(unit / a.heads) : 0, head = live ? static_cast<int>(unit - static_cast<long long>(row) * a.heads) : 0;
-  const uint4 raw = *reinterpret_cast<const uint4*>(a.x.data + row * a.x.row_stride + head * a.x.head_stride + 8 * lane);
-  uint4 gate = make_uint4(0, 0, 0, 0);
-  if (kActivation != AIMA_MOE_GATE_NONE) gate = *reinterpret_cast<const uint4*>(a.gate.data + row * a.gate.row_stride + head * a.gate.head_stride + 8 * lane);
-  float x[8];
-  unpack8(raw, x);
+  uint4 raw[kUnits], gate[kUnits];
+  int unit[kUnits];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    unit[u] = (static_cast<int>(blockIdx.x) * kUnits + u) * kPerBlock + static_cast<int>(threadIdx.x) / kLanes;
+    const int at = min(unit[u], units - 1), row = at / a.heads, head = at - row * a.heads;
+    raw[u] = *reinterpret_cast<const uint4*>(a.x.data + row * a.x.row_stride + head * a.x.head_stride + 8 * lane);
+    if (kActivation != AIMA_MOE_GATE_NONE) gate[u] = *reinterpret_cast<const uint4*>(a.gate.data + row * a.gate.row_stride + head * a.gate.head_stride + 8 * lane);
+  }
+  float w[8];
   if (kNorm) {
-    float w[8], sum = 0.0f;
     unpack8(*reinterpret_cast<const uint4*>(a.weight + 8 * lane), w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
-#pragma unroll
-    for (int d = 1; d < kLanes; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    const float scale = __frsqrt_rn(fmaf(sum, 1.0f / kDim, a.eps));
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = x[j] * scale * (w[j] + a.offset);
+    for (int j = 0; j < 8; ++j) w[j] += a.offset;
   }
-  if (kActivation != AIMA_MOE_GATE_NONE) {
-    float z[8];
-    unpack8(gate, z);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] *= kActivation == AIMA_MOE_GATE_SILU ? z[j] * linear_sigmoid(z[j]) : linear_sigmoid(z[j]);
+  for (int u = 0; u < kUnits; ++u) {
+    float x[8];
+    unpack8(raw[u], x);
+    if (kNorm) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
+#pragma unroll
+      for (int d = 1; d < kLanes; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const float scale = __frsqrt_rn(fmaf(sum, 1.0f / kDim, a.eps));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = x[j] * scale * w[j];
+    }
+    if (kActivation != AIMA_MOE_GATE_NONE) {
+      float z[8];
+      unpack8(gate[u], z);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] *= kActivation == AIMA_MOE_GATE_SILU ? z[j] * linear_sigmoid(z[j]) : linear_sigmoid(z[j]);
+    }
+    if (unit[u] < units)
+      *reinterpret_cast<uint4*>(a.out + static_cast<long long>(unit[u]) * kDim + 8 * lane) =
+          make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
   }
-  if (live)
-    *reinterpret_cast<uint4*>(a.out + unit * kDim + 8 * lane) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+}
+
+template <int kDim, bool kNorm, int kActivation>
+void launch_units(const HeadNorm& a, cudaStream_t stream) {
+  constexpr int kPerBlock = kNormThreads / (kDim / 8);
+  const int units = a.tokens * a.heads;
+  if (units > 4 * 4 * 148 * kPerBlock)      // four rounds of four heads a thread on every multiprocessor
+    head_norm_kernel<kDim, kNorm, kActivation, 4><<<(units + 4 * kPerBlock - 1) / (4 * kPerBlock), kNormThreads, 0, stream>>>(a, units);
+  else
+    head_norm_kernel<kDim, kNorm, kActivation, 1><<<(units + kPerBlock - 1) / kPerBlock, kNormThreads, 0, stream>>>(a, units);
 }
 
 template <int kDim>
-cudaError_t launch(const HeadNorm& a, cudaStream_t stream) {
-  const long long units = static_cast<long long>(a.tokens) * a.heads;
-  const unsigned grid = static_cast<unsigned>((units * (kDim / 8) + kNormThreads - 1) / kNormThreads);
+void launch(const HeadNorm& a, cudaStream_t stream) {
   if (a.weight == nullptr) {
-    if (a.activation == AIMA_MOE_GATE_SILU) head_norm_kernel<kDim, false, AIMA_MOE_GATE_SILU><<<grid, kNormThreads, 0, stream>>>(a);
-    else head_norm_kernel<kDim, false, AIMA_MOE_GATE_SIGMOID><<<grid, kNormThreads, 0, stream>>>(a);
+    if (a.activation == AIMA_MOE_GATE_SILU) launch_units<kDim, false, AIMA_MOE_GATE_SILU>(a, stream);
+    else launch_units<kDim, false, AIMA_MOE_GATE_SIGMOID>(a, stream);
   } else if (a.activation == AIMA_MOE_GATE_NONE) {
-    head_norm_kernel<kDim, true, AIMA_MOE_GATE_NONE><<<grid, kNormThreads, 0, stream>>>(a);
+    launch_units<kDim, true, AIMA_MOE_GATE_NONE>(a, stream);
   } else if (a.activation == AIMA_MOE_GATE_SILU) {
-    head_norm_kernel<kDim, true, AIMA_MOE_GATE_SILU><<<grid, kNormThreads, 0, stream>>>(a);
+    launch_units<kDim, true, AIMA_MOE_GATE_SILU>(a, stream);
   } else {
-    head_norm_kernel<kDim, true, AIMA_MOE_GATE_SIGMOID><<<grid, kNormThreads, 0, stream>>>(a);
+    launch_units<kDim, true, AIMA_MOE_GATE_SIGMOID>(a, stream);
   }
-  return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t head_norm(const HeadNorm& a, cudaStream_t stream) {
-  return a.dim == 64 ? launch<64>(a, stream) : a.dim == 128 ? launch<128>(a, stream) : launch<256>(a, stream);
+cudaError_t head_norm(const HeadNorm& all, cudaStream_t stream) {
+  // launches of at most 2^30 heads, which 32 bits count
+  const int most = (1 << 30) / all.heads;
+  for (int begin = 0; begin < all.tokens; begin += most) {
+    HeadNorm a = all;
+    a.tokens = all.tokens - begin < most ? all.tokens - begin : most;
+    a.x.data += begin * a.x.row_stride;
+    if (a.gate.data != nullptr) a.gate.data += begin * a.gate.row_stride;
+    a.out += static_cast<long long>(begin) * a.heads * a.dim;
+    if (a.dim == 64) launch<64>(a, stream);
+    else if (a.dim == 128) launch<128>(a, stream);
+    else launch<256>(a, stream);
+    const cudaError_t error = cudaGetLastError();
+    if (error != cudaSuccess) return error;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace aima

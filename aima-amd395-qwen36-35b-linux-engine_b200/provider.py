@@ -17,6 +17,7 @@ is present, construction fails loudly.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import c_char_p, c_float, c_int, c_int32, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 from typing import Any, Mapping
@@ -183,7 +184,9 @@ class HeadNorm(ctypes.Structure):
     ]
 
 
-_LINEAR_DELTA_BYTES, _HEAD_NORM_BYTES = ctypes.sizeof(LinearDelta), ctypes.sizeof(HeadNorm)
+# the same two, filled in one go: a Structure of so many members takes longer to fill than the launch takes
+_LINEAR_DELTA, _HEAD_NORM = struct.Struct("<II17Q"), struct.Struct("<IIIIIffI8Q")
+assert _LINEAR_DELTA.size == ctypes.sizeof(LinearDelta) and _HEAD_NORM.size == ctypes.sizeof(HeadNorm)
 LINEAR_HEAD_DIM = 128
 GATE_ACTIVATIONS = {"none": 0, "silu": 1, "sigmoid": 2}
 
@@ -265,10 +268,10 @@ EXPORTS = [
     ("aima_moe_linear_conv_launch", c_int,
      [c_void_p, c_uint32, ctypes.POINTER(LinearBatchStruct), c_void_p, c_uint64, c_void_p, c_void_p]),
     ("aima_moe_linear_delta_launch", c_int,
-     [c_void_p, c_uint32, ctypes.POINTER(LinearBatchStruct), ctypes.POINTER(LinearDelta), c_void_p]),
+     [c_void_p, c_uint32, ctypes.POINTER(LinearBatchStruct), c_void_p, c_void_p]),
     ("aima_moe_linear_sync", c_int, [c_void_p]),
     ("aima_moe_linear_release", c_int, [c_void_p]),
-    ("aima_moe_head_norm_launch", c_int, [ctypes.POINTER(HeadNorm), c_void_p]),
+    ("aima_moe_head_norm_launch", c_int, [c_void_p, c_void_p]),
     ("aima_moe_sync_metrics", c_int, [c_void_p, ctypes.POINTER(Metrics)]),
     ("aima_moe_release", c_int, [c_void_p]),
 ]
@@ -1075,14 +1078,15 @@ class LinearAttention:
     # -- launches ------------------------------------------------------------
     def conv(self, layer: int, batch: LinearBatch, x: Any, out: Any = None) -> Any:
         """Short causal convolution with SiLU over the rows of x, BF16 [tokens, channels] (a view of wider rows is fine)."""
-        if batch.device != self._device:
-            self._refuse_device(batch)
-        torch, shape = self._torch, (batch.tokens, self.channels)
-        if x.dtype is not torch.bfloat16 or x.get_device() != self._device or x.shape != shape or x.stride(1) != 1:
-            raise ValueError(f"x must be a bfloat16 tensor {list(shape)} with contiguous rows of the handle's device, got {x.dtype} {list(x.shape)} "
-                             f"with strides {list(x.stride())} on {x.device}")
-        out = self._out(out, x, shape)
-        self.lib.check(self.lib.aima_moe_linear_conv_launch(self.handle, layer, batch.ref, x.data_ptr(), x.stride(0), out.data_ptr(), self._stream()))
+        device, tokens, bfloat16 = self._device, batch.tokens, self._torch.bfloat16
+        shape, stride = x.shape, x.stride()
+        # in one expression: the call on the host takes longer than the kernel
+        if not (batch.device == device and x.dtype is bfloat16 and x.get_device() == device and shape == (tokens, self.channels) and stride[1] == 1
+                and (out is None or (out.dtype is bfloat16 and out.get_device() == device and out.shape == shape and out.is_contiguous()))):
+            self._refuse(batch, (("x", x, (tokens, self.channels)),), out, (tokens, self.channels))
+        if out is None:
+            out = x.new_empty(shape)
+        self.lib.check(self.lib.aima_moe_linear_conv_launch(self.handle, layer, batch.ref, x.data_ptr(), stride[0], out.data_ptr(), self._stream()))
         return out
 
     def delta(self, layer: int, batch: LinearBatch, q: Any, k: Any, v: Any, a: Any, b: Any, gate: Any = None, out: Any = None,
@@ -1090,41 +1094,46 @@ class LinearAttention:
         """The gated delta rule: q and k BF16 [tokens, k_heads, 128], v and the gate [tokens, v_heads, 128], a and b [tokens, v_heads];
         all of them may be views.  Returns BF16 [tokens, v_heads, 128], normed and gated if there is a gate; with outputs=False it
         only brings the states to the rows that `keep` says and returns None."""
-        if batch.device != self._device:
-            self._refuse_device(batch)
-        tokens = batch.tokens
-        k_shape, v_shape = (tokens, *self._k_shape), (tokens, *self._v_shape)
-        call = LinearDelta(_LINEAR_DELTA_BYTES, 0, self._rows(q, "q", k_shape), self._rows(k, "k", k_shape), self._rows(v, "v", v_shape),
-                           KvRows() if gate is None else self._rows(gate, "gate", v_shape), a.data_ptr(), b.data_ptr(), self._numbers(a, "a", v_shape),
-                           self._numbers(b, "b", v_shape))
-        if outputs:
-            out = self._out(out, v, v_shape)
-            call.out = out.data_ptr()
-        else:
+        device, tokens, bfloat16 = self._device, batch.tokens, self._torch.bfloat16
+        k_shape, v_shape, numbers = (tokens, *self._k_shape), (tokens, *self._v_shape), (tokens, self._v_shape[0])
+        gated = gate is not None
+        if not (batch.device == device
+                and q.dtype is bfloat16 and q.shape == k_shape and q.get_device() == device and k.dtype is bfloat16 and k.shape == k_shape
+                and k.get_device() == device and v.dtype is bfloat16 and v.shape == v_shape and v.get_device() == device
+                and a.dtype is bfloat16 and a.shape == numbers and a.get_device() == device and b.dtype is bfloat16 and b.shape == numbers
+                and b.get_device() == device and (not gated or (gate.dtype is bfloat16 and gate.shape == v_shape and gate.get_device() == device))
+                and (out is None or (out.dtype is bfloat16 and out.get_device() == device and out.shape == v_shape and out.is_contiguous()))):
+            self._refuse(batch, (("q", q, k_shape), ("k", k, k_shape), ("v", v, v_shape), ("gate", gate, v_shape), ("a", a, numbers), ("b", b, numbers)),
+                         out, v_shape)
+        q_row, q_head, q_one = q.stride()
+        k_row, k_head, k_one = k.stride()
+        v_row, v_head, v_one = v.stride()
+        a_row, a_one = a.stride()
+        b_row, b_one = b.stride()
+        z_row, z_head, z_one = gate.stride() if gated else (0, 0, 1)
+        if not (q_one == k_one == v_one == z_one == 1 and (a_one == b_one == 1 or numbers[1] == 1)):
+            self._refuse(batch, (("q", q, k_shape), ("k", k, k_shape), ("v", v, v_shape), ("gate", gate, v_shape), ("a", a, numbers), ("b", b, numbers)),
+                         out, v_shape)
+        if not outputs:
             out = None
+        elif out is None:
+            out = v.new_empty(v_shape)
+        call = _LINEAR_DELTA.pack(_LINEAR_DELTA.size, 0, q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+                                  gate.data_ptr() if gated else 0, z_row, z_head, a.data_ptr(), b.data_ptr(), a_row, b_row,
+                                  0 if out is None else out.data_ptr())
         self.lib.check(self.lib.aima_moe_linear_delta_launch(self.handle, layer, batch.ref, call, self._stream()))
         return out
 
-    def _rows(self, tensor: Any, name: str, shape: tuple[int, int, int]) -> KvRows:
-        row_stride, head_stride, stride = tensor.stride() if tensor.dim() == 3 else (0, 0, 0)
-        if tensor.dtype is not self._torch.bfloat16 or tensor.get_device() != self._device or tensor.shape != shape or stride != 1:
-            raise ValueError(f"{name} must be a bfloat16 tensor {list(shape)} with contiguous heads of the handle's device, got "
-                             f"{tensor.dtype} {list(tensor.shape)} with strides {list(tensor.stride())} on {tensor.device}")
-        return KvRows(tensor.data_ptr(), row_stride, head_stride)
-
-    def _numbers(self, tensor: Any, name: str, shape: tuple[int, int, int]) -> int:
-        if (tensor.dtype is not self._torch.bfloat16 or tensor.get_device() != self._device or tensor.shape != shape[:2]
-                or (tensor.stride(1) != 1 and shape[1] > 1)):
-            raise ValueError(f"{name} must be a bfloat16 tensor {list(shape[:2])} with contiguous rows of the handle's device, got "
-                             f"{tensor.dtype} {list(tensor.shape)} with strides {list(tensor.stride())} on {tensor.device}")
-        return tensor.stride(0)
-
-    def _out(self, out: Any, like: Any, shape: tuple) -> Any:
-        if out is None:
-            return self._torch.empty(shape, dtype=self._torch.bfloat16, device=like.device)
-        if out.dtype is not self._torch.bfloat16 or out.get_device() != self._device or out.shape != shape or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous bfloat16 tensor {list(shape)} of the handle's device")
-        return out
+    def _refuse(self, batch: LinearBatch, tensors: tuple, out: Any, out_shape: tuple) -> None:
+        """Says which of a call's tensors is not what it has to be."""
+        if batch.device != self._device:
+            self._refuse_device(batch)
+        for name, tensor, shape in tensors:
+            if tensor is not None and (tensor.dtype is not self._torch.bfloat16 or tensor.get_device() != self._device or tensor.shape != shape
+                                       or (tensor.stride(-1) != 1 and shape[-1] > 1)):
+                raise ValueError(f"{name} must be a bfloat16 tensor {list(shape)} with contiguous {'heads' if len(shape) == 3 else 'rows'} of the handle's "
+                                 f"device, got {tensor.dtype} {list(tensor.shape)} with strides {list(tensor.stride())} on {tensor.device}")
+        raise ValueError(f"out must be a contiguous bfloat16 tensor {list(out_shape)} of the handle's device")
 
     def _refuse_device(self, batch: LinearBatch) -> None:
         raise ValueError(f"the batch's tensors are of device {batch.device}, the handle is of {self._device}")
@@ -1162,21 +1171,23 @@ def head_norm(x: Any, weight: Any = None, *, offset: float = 0.0, gate: Any = No
     import torch
 
     lib = library or load_library()
-    device, shape = x.get_device(), x.shape
+    device, shape, bfloat16, code = x.get_device(), x.shape, torch.bfloat16, GATE_ACTIVATIONS.get(activation)
+    gated = gate is not None
     # in one expression: the call on the host takes longer than the kernel
-    if not (device == torch._C._cuda_getDevice() and x.dtype is torch.bfloat16 and len(shape) == 3 and x.stride(2) == 1
-            and activation in GATE_ACTIVATIONS
-            and (gate is None or (gate.dtype is torch.bfloat16 and gate.shape == shape and gate.get_device() == device and gate.stride(2) == 1))
-            and (weight is None or (weight.dtype is torch.bfloat16 and weight.shape == shape[2:] and weight.get_device() == device
-                                    and weight.is_contiguous()))
-            and (out is None or (out.dtype is torch.bfloat16 and out.shape == shape and out.get_device() == device and out.is_contiguous()))):
+    if not (device == torch._C._cuda_getDevice() and x.dtype is bfloat16 and len(shape) == 3 and code is not None
+            and (not gated or (gate.dtype is bfloat16 and gate.shape == shape and gate.get_device() == device))
+            and (weight is None or (weight.dtype is bfloat16 and weight.shape == shape[2:] and weight.get_device() == device and weight.is_contiguous()))
+            and (out is None or (out.dtype is bfloat16 and out.shape == shape and out.get_device() == device and out.is_contiguous()))):
+        _refuse_head_norm(x, weight, gate, activation, out)
+    x_row, x_head, x_one = x.stride()
+    z_row, z_head, z_one = gate.stride() if gated else (0, 0, 1)
+    if not (x_one == z_one == 1):
         _refuse_head_norm(x, weight, gate, activation, out)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
-    call = HeadNorm(_HEAD_NORM_BYTES, shape[0], shape[1], shape[2], GATE_ACTIVATIONS[activation], offset, eps, 0,
-                    KvRows(x.data_ptr(), x.stride(0), x.stride(1)),
-                    KvRows() if gate is None else KvRows(gate.data_ptr(), gate.stride(0), gate.stride(1)),
-                    None if weight is None else weight.data_ptr(), out.data_ptr())
+        out = x.new_empty(shape)
+    tokens, heads, dim = shape
+    call = _HEAD_NORM.pack(_HEAD_NORM.size, tokens, heads, dim, code, offset, eps, 0, x.data_ptr(), x_row, x_head,
+                           gate.data_ptr() if gated else 0, z_row, z_head, 0 if weight is None else weight.data_ptr(), out.data_ptr())
     lib.check(lib.aima_moe_head_norm_launch(call, torch._C._cuda_getCurrentRawStream(device)))
     return out
 
