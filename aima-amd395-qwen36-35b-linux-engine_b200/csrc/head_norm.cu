@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kNormThreads) head_norm_kernel(const HeadNorm 
       float z[8];
       unpack8(gate[u], z);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= kActivation == AIMA_MOE_GATE_SILU ? z[j] * linear_sigmoid(z[j]) : linear_sigmoid(z[j]);
+      for (int j = 0; j < 8; ++j) x[j] *= kActivation == AIMA_MOE_GATE_SILU ? linear_silu(z[j]) : linear_sigmoid(z[j]);
     }
     if (unit[u] < units)
       *reinterpret_cast<uint4*>(a.out + static_cast<long long>(unit[u]) * kDim + 8 * lane) =

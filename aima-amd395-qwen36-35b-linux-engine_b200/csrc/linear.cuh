@@ -104,12 +104,15 @@ __device__ __forceinline__ void linear_report(const LinearBatch& b, int* status,
     if (linear_sequence(b, s).bad) atomicOr(status, kLinearBadBatch);
 }
 
-// 1 / (1 + e^-x), to a few units of the last place; a quarter of the denominator, so that the reciprocal is a normal number
-__device__ __forceinline__ float linear_sigmoid(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(__expf(-x), 0.25f, 0.25f)));
-  return 0.25f * y;
+// 4 / (1 + e^-x), to a few units of the last place: of a quarter of the denominator, so that the reciprocal is a normal number
+__device__ __forceinline__ float linear_four_sigmoid(float x) {
+  float quarter, y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(quarter) : "f"(fmaf(x, -1.4426950408889634f, -2.0f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(quarter + 0.25f));
+  return y;
 }
+__device__ __forceinline__ float linear_sigmoid(float x) { return 0.25f * linear_four_sigmoid(x); }
+__device__ __forceinline__ float linear_silu(float x) { return (0.25f * x) * linear_four_sigmoid(x); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);

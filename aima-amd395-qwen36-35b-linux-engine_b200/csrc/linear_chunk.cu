@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
               float z[8];
               unpack8(*reinterpret_cast<const uint4*>(&m.gate[(2 * kOutWarps * (i0 + i) + 2 * w + half) * kLinearDim + 8 * piece]), z);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) o[i][j] *= factor * weight[j] * (z[j] * linear_sigmoid(z[j]));
+              for (int j = 0; j < 8; ++j) o[i][j] *= factor * weight[j] * linear_silu(z[j]);
             }
           }
 #pragma unroll

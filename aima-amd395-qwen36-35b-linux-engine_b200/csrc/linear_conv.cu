@@ -1,9 +1,8 @@
 // Short causal convolution of a linear-attention layer: y[t, c] = silu(sum_j w[c, j] x[t - (W - 1) + j, c]) for W of 2 .. 4, and
 // the state, the last W - 1 inputs of a sequence.
 //
-// A thread takes eight channels of a run of eight rows: all rows that it needs, the W - 1 before its own too, are loaded before any
-// arithmetic, so that a multiprocessor has some 100 KB under way; the rows before come from L2.  Two channels at a time are then widened,
-// summed and put back in the rows' place.  Runs begin with a sequence, so only a sequence's first run reads its state; the same threads
+// A thread takes eight channels of a run of 16 rows, four at a time: the next four are under way while these are widened, two channels
+// at a time, summed and put back in their own place.  Runs begin with a sequence, so only a sequence's first run reads its state; the same threads
 // write it, after that, from the inputs themselves.
 #include "linear.cuh"
 
@@ -11,10 +10,11 @@ namespace aima {
 namespace {
 
 constexpr int kConvThreads = 128;
-constexpr int kConvRows = 8;         // of a run
+constexpr int kConvRows = 16;        // of a run
+constexpr int kConvStep = 4;         // of them at a time
 
 template <int kWidth>
-__global__ void __launch_bounds__(kConvThreads) linear_conv_kernel(const LinearConv a) {
+__global__ void __launch_bounds__(kConvThreads, 5) linear_conv_kernel(const LinearConv a) {
   const LinearBatch& b = a.batch;
   if (blockIdx.x == 0 && blockIdx.y == 0) linear_report(b, a.status, threadIdx.x, kConvThreads);
   int s, run;
@@ -34,9 +34,9 @@ __global__ void __launch_bounds__(kConvThreads) linear_conv_kernel(const LinearC
     if (seq.fresh || seq.slot < 0 || row < first - kBefore) return make_uint4(0, 0, 0, 0);
     return *reinterpret_cast<const uint4*>(a.states + slot_base + static_cast<long long>(row - first + kBefore) * a.channels);
   };
-  uint4 rows[kBefore + kConvRows], weights[kWidth];
+  uint4 rows[kBefore + kConvStep], next[kConvStep], weights[kWidth];
 #pragma unroll
-  for (int i = 0; i < kBefore + kConvRows; ++i) rows[i] = value(begin - kBefore + i);
+  for (int i = 0; i < kBefore + kConvStep; ++i) rows[i] = value(begin - kBefore + i);
 #pragma unroll
   for (int i = 0; i < kWidth; ++i) weights[i] = *reinterpret_cast<const uint4*>(a.weight + static_cast<long long>(channel) * kWidth + 8 * i);
   if (begin == 0 && seq.kept > first) {     // fresh sequences may have inactive rows in front: none of them enters the state
@@ -49,35 +49,53 @@ __global__ void __launch_bounds__(kConvThreads) linear_conv_kernel(const LinearC
 #pragma unroll
     for (int i = 0; i < kBefore; ++i) *reinterpret_cast<uint4*>(a.states + slot_base + static_cast<long long>(i) * a.channels) = last[i];
   }
+  __nv_bfloat16* out = a.out + static_cast<long long>(seq.row0 + begin) * a.channels + channel;
+  const __nv_bfloat16* from = x + (begin + kConvStep) * a.x_stride;
+#pragma unroll 1
+  for (int row = begin; row < end; row += kConvStep) {
+    // the next rows; after the first step they are all behind the first active one, unless that one comes late
+    if (row + kConvStep >= first && row + 2 * kConvStep <= end) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {             // channels 2 j, 2 j + 1
-    float w[2][kWidth], lo[kBefore + kConvRows], hi[kBefore + kConvRows];
+      for (int i = 0; i < kConvStep; ++i, from += a.x_stride) next[i] = *reinterpret_cast<const uint4*>(from);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2 * kWidth; ++i) {
-      const int at = 2 * j * kWidth + i;    // of the thread's weights, eight to a vector
-      const uint32_t word = (&weights[at / 8].x)[(at % 8) / 2];
-      w[i / kWidth][i % kWidth] = at % 2 == 0 ? bf16_lo(word) : bf16_hi(word);
+      for (int i = 0; i < kConvStep; ++i) next[i] = value(row + kConvStep + i);
+      from += kConvStep * a.x_stride;
     }
+    uint4 y[kConvStep];
 #pragma unroll
-    for (int i = 0; i < kBefore + kConvRows; ++i) {
-      lo[i] = bf16_lo((&rows[i].x)[j]);
-      hi[i] = bf16_hi((&rows[i].x)[j]);
-    }
+    for (int j = 0; j < 4; ++j) {             // channels 2 j, 2 j + 1
+      float w[2][kWidth], lo[kBefore + kConvStep], hi[kBefore + kConvStep];
 #pragma unroll
-    for (int r = 0; r < kConvRows; ++r) {
-      float y0 = lo[r] * w[0][0], y1 = hi[r] * w[1][0];
-#pragma unroll
-      for (int i = 1; i < kWidth; ++i) {
-        y0 = fmaf(lo[r + i], w[0][i], y0);
-        y1 = fmaf(hi[r + i], w[1][i], y1);
+      for (int i = 0; i < 2 * kWidth; ++i) {
+        const int at = 2 * j * kWidth + i;    // of the thread's weights, eight to a vector
+        const uint32_t word = (&weights[at / 8].x)[(at % 8) / 2];
+        w[i / kWidth][i % kWidth] = at % 2 == 0 ? bf16_lo(word) : bf16_hi(word);
       }
-      (&rows[r].x)[j] = pack_bf16(y0 * linear_sigmoid(y0), y1 * linear_sigmoid(y1));         // the row before is not needed again
-    }
-  }
-  __nv_bfloat16* out = a.out + static_cast<long long>(seq.row0) * a.channels + channel;
 #pragma unroll
-  for (int r = 0; r < kConvRows; ++r)
-    if (begin + r < end) *reinterpret_cast<uint4*>(out + static_cast<long long>(begin + r) * a.channels) = begin + r < first ? make_uint4(0, 0, 0, 0) : rows[r];
+      for (int i = 0; i < kBefore + kConvStep; ++i) {
+        lo[i] = bf16_lo((&rows[i].x)[j]);
+        hi[i] = bf16_hi((&rows[i].x)[j]);
+      }
+#pragma unroll
+      for (int r = 0; r < kConvStep; ++r) {
+        float y0 = lo[r] * w[0][0], y1 = hi[r] * w[1][0];
+#pragma unroll
+        for (int i = 1; i < kWidth; ++i) {
+          y0 = fmaf(lo[r + i], w[0][i], y0);
+          y1 = fmaf(hi[r + i], w[1][i], y1);
+        }
+        (&y[r].x)[j] = pack_bf16(linear_silu(y0), linear_silu(y1));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kConvStep; ++r, out += a.channels)
+      if (row + r < end) *reinterpret_cast<uint4*>(out) = row + r < first ? make_uint4(0, 0, 0, 0) : y[r];
+#pragma unroll
+    for (int i = 0; i < kBefore; ++i) rows[i] = rows[kConvStep + i];
+#pragma unroll
+    for (int i = 0; i < kConvStep; ++i) rows[kBefore + i] = next[i];
+  }
 }
 
 }  // namespace

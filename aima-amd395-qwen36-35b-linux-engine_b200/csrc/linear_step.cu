@@ -151,10 +151,10 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
           const float4 z = load4(a.gate.data + row * a.gate.row_stride + head * a.gate.head_stride + 4 * lane);
           const float4 w = load4(a.norm_weight + 4 * lane);
           const float scale = __frsqrt_rn(fmaf(warp_sum(dot4(o, o)), 1.0f / kLinearDim, a.eps));
-          o.x *= scale * w.x * (z.x * linear_sigmoid(z.x));
-          o.y *= scale * w.y * (z.y * linear_sigmoid(z.y));
-          o.z *= scale * w.z * (z.z * linear_sigmoid(z.z));
-          o.w *= scale * w.w * (z.w * linear_sigmoid(z.w));
+          o.x *= scale * w.x * linear_silu(z.x);
+          o.y *= scale * w.y * linear_silu(z.y);
+          o.z *= scale * w.z * linear_silu(z.z);
+          o.w *= scale * w.w * linear_silu(z.w);
         }
         store4(a.out + (row * a.v_heads + head) * kLinearDim + 4 * lane, o);
       }
