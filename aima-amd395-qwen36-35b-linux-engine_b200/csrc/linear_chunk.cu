@@ -7,7 +7,10 @@
 // them.  Per chunk:
 //   R = S^T k, Q = S^T q    ->  right side beta v - enter R  ->  D = (right side) T^T
 //   S <- decay S + (stay D) k,  O = D scores^T               ->  o = (read Q + O) / sqrt(128)
-// Four warp groups have 16 tokens or 32 key elements each of that chain, two the output, one warp issues products, three load.
+// Four warp groups have 16 tokens or 32 key elements each of that chain.  What does not depend on the chain is put where it waits for a
+// product: the outputs of the chunk before are taken from tensor memory and turned into rows while R runs, and normed and written while D
+// and S run; warps of their own for that slowed the chain by as much as they saved (9000 cycles a chunk; the floor of the products is
+// 2300).  One warp issues products, three load.
 #include "linear_chunk.cuh"
 
 #include <algorithm>
@@ -16,41 +19,37 @@
 namespace aima {
 namespace {
 
-constexpr int kChainGroups = 2, kOutGroups = 2;        // of four warps, one for each 32 lanes of tensor memory
-constexpr int kChainWarps = 4 * kChainGroups, kOutWarps = 4 * kOutGroups;
-constexpr int kChunkThreads = 32 * (kChainWarps + kOutWarps + 4);          // the last group issues products and loads
-constexpr int kTokens = kChunk / kChainGroups, kKeys = kLinearDim / kChainGroups;      // of a group of the chain
-// registers of a thread: as many at launch for all, in all as many as there are
-constexpr int kLaunchRegisters = 96, kChainRegisters = 152, kOutRegisters = 64, kIssueRegisters = 48;
-static_assert(kChainGroups * kChainRegisters + kOutGroups * kOutRegisters + kIssueRegisters <= (kChainGroups + kOutGroups + 1) * kLaunchRegisters,
-              "the warp groups share what the block was launched with");
+constexpr int kGroups = 4, kChainWarps = 4 * kGroups;                      // groups of four warps, one for each 32 lanes of tensor memory
+constexpr int kChunkThreads = 32 * (kChainWarps + 4);
+constexpr int kTokens = kChunk / kGroups, kKeys = kLinearDim / kGroups;    // of a group
+constexpr int kTokenSteps = kTokens / 16;                                  // of products over tokens, by when their operands come
 constexpr int kStages = 2;
 constexpr int kStageValues = kChunkPairBytes + kChunkHeadBytes;           // v: 64 rows of 256 bytes, zeros behind the last
 constexpr int kStageBytes = (kStageValues + kChunk * kLinearDim * 2 + 1023) / 1024 * 1024;
 constexpr int kOutRow = kLinearDim + 4;
+constexpr int kOutRows = 2 * kChainWarps, kOutPasses = kChunk / kOutRows;   // rows that the groups write at a time, 16 lanes a row
 
 // Columns of tensor memory.  Operands lie as eight columns of first and eight of second terms for every 16 elements of K: what a warp
-// splits at a time and a step of a product takes.
+// splits at a time and a step of a product takes.  O is left where the corrections of the state were.
 constexpr uint32_t kStateAt = 0, kTermsAt = 128, kFreshAt = 256, kDotsAt = 320, kReadAt = 384, kEnterAt = 448;
 __device__ __forceinline__ constexpr uint32_t operand(int k, int term) { return 16 * k + 8 * term; }
 
 struct __align__(1024) ChunkMemory {
   uint8_t stages[kStages][kStageBytes];
   float out[kChunk * kOutRow];
-  __nv_bfloat16 gate[kChunk * kLinearDim];
-  float largest[kChainGroups][kLinearDim];      // of a column of the state, by warp group
+  float largest[kGroups][kLinearDim];     // of a column of the state, by warp group
   float largest_value[kStages][2][kLinearDim];   // of a column of v, by the warp that brought the rows; not of numbers that are not finite
   float scale[2][kLinearDim];             // the power of two of a column, by parity of the chunk
   int broken[2][kLinearDim];              // the first token of the chunk whose right side is not finite
+  float read[2][kChunk];                  // of ChunkNumbers, for when its stage is gone
   int sums[kChunkThreads / 32];
-  unsigned long long full[kStages], empty[kStages];
-  unsigned long long values_full[kStages], state_ready[2], dots_full, enter_ready[2], fresh_full, stay_ready[2], state_full, fresh_ready, out_full, dots_empty;
+  unsigned long long full[kStages], empty[kStages], values_full[kStages];
+  unsigned long long state_ready[2], dots_full, enter_ready[kTokenSteps], fresh_full, stay_ready[kTokenSteps], state_full, fresh_ready, out_full, out_taken;
   uint32_t tmem;
   int abort_flag;
 };
 
 __device__ __forceinline__ void chain_barrier() { asm volatile("bar.sync 1, %0;" :: "n"(32 * kChainWarps) : "memory"); }
-__device__ __forceinline__ void out_barrier() { asm volatile("bar.sync 2, %0;" :: "n"(32 * kOutWarps) : "memory"); }
 // mbar_wait_bounded_warp without a call: the numbers that are alive across one would go to memory.
 __device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit_ns) {
   if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
@@ -70,6 +69,8 @@ __device__ __forceinline__ void warp_arrive(unsigned long long* bar, int lane) {
   if (lane == 0) mbar_arrive(smem_u32(bar));
 }
 
+// kOutputs: all rows, the states if plan.store says so; else the states alone, for the rows that enter them.
+template <bool kOutputs>
 __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const ChunkPlan plan) {
   extern __shared__ uint8_t raw[];
   ChunkMemory& m = *reinterpret_cast<ChunkMemory*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -78,12 +79,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   const int head = blockIdx.x;
   const LinearSequence seq = linear_sequence(a.batch, blockIdx.y);
   if (seq.rows <= plan.min_rows) return;
-  if (a.out != nullptr && !plan.kept_only) {          // rows that are not active
+  if (kOutputs) {                                     // rows that are not active
     for (int i = threadIdx.x; i < seq.first * (kLinearDim / 8); i += kChunkThreads)
       *reinterpret_cast<uint4*>(a.out + (static_cast<long long>(seq.row0 + i / (kLinearDim / 8)) * a.v_heads + head) * kLinearDim + 8 * (i % (kLinearDim / 8))) =
           make_uint4(0, 0, 0, 0);
   }
-  const int limit = plan.kept_only ? seq.kept : seq.rows;                  // rows that are gone through
+  const int limit = kOutputs ? seq.rows : seq.kept;                        // rows that are gone through
   const int chunks = (limit - seq.first + kChunk - 1) / kChunk;
   if (limit <= seq.first) return;
 
@@ -98,22 +99,24 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&m.full[i]), 1);
-      mbar_init(smem_u32(&m.empty[i]), 1 + kChainWarps + kOutWarps);
+      mbar_init(smem_u32(&m.empty[i]), 1 + kChainWarps);
       mbar_init(smem_u32(&m.values_full[i]), 2);
     }
     for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&m.state_ready[i]), kChainWarps);
+    for (int i = 0; i < kTokenSteps; ++i) {
+      mbar_init(smem_u32(&m.enter_ready[i]), kChainWarps);
+      mbar_init(smem_u32(&m.stay_ready[i]), kChainWarps);
+    }
     mbar_init(smem_u32(&m.dots_full), 1);
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&m.enter_ready[i]), kChainWarps);
     mbar_init(smem_u32(&m.fresh_full), 1);
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&m.stay_ready[i]), kChainWarps);
     mbar_init(smem_u32(&m.state_full), 1);
     mbar_init(smem_u32(&m.fresh_ready), kChainWarps);
     mbar_init(smem_u32(&m.out_full), 1);
-    mbar_init(smem_u32(&m.dots_empty), kOutWarps);
+    mbar_init(smem_u32(&m.out_taken), kChainWarps);
     m.abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == kChainWarps + kOutWarps) tmem_alloc(smem_u32(&m.tmem), 512);
+  if (warp == kChainWarps) tmem_alloc(smem_u32(&m.tmem), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -126,14 +129,90 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   auto wait = [&](unsigned long long* bar, int phase) { return wait_inline(smem_u32(bar), phase & 1, abort_flag, plan.wait_limit_ns); };
   const long long row0 = static_cast<long long>(seq.row0) + seq.first;
   const int rows = limit - seq.first;                                          // of all chunks
-  float* const state = a.states + (static_cast<long long>(seq.slot) * a.v_heads + head) * kLinearDim * kLinearDim;
 
   if (warp < kChainWarps) {
     // ------------------------------ the chain ------------------------------
-    more_registers<kChainRegisters>();
     // No wait that runs out leaves this loop: the warps meet at barriers, and every wait after the first that ran out ends at once.
     const int group = warp >> 2, column = (warp & 3) * 32 + lane;              // a value element
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    float* const state = a.states + (static_cast<long long>(seq.slot) * a.v_heads + head) * kLinearDim * kLinearDim + kKeys * group * kLinearDim + column;
+    const bool gated = kOutputs && a.gate.data != nullptr;
+    // rows of the output: 16 lanes a row
+    const int out_row = 2 * warp + (lane >> 4), piece = lane & 15;
+
+    // O and Q of chunk c as rows in shared memory
+    auto take_outputs = [&](int c) {
+      const float back = kv_exp2(-kv_float_exponent(m.scale[c & 1][column])) * 0.08838834764831845f;
+      const int broken = m.broken[c & 1][column];
+      wait(&m.out_full, c);
+      tc_fence_after();
+#pragma unroll
+      for (int b = 0; b < kTokens / 16; ++b) {
+        const int token = kTokens * group + 16 * b;
+        Pair o[8], q[8];
+        tmem_ld16(lanes + kEnterAt + token, reinterpret_cast<uint32_t*>(o));
+        tmem_ld16(lanes + kReadAt + token, reinterpret_cast<uint32_t*>(q));
+        tmem_ld_wait();
+        if (b == kTokens / 16 - 1) warp_arrive(&m.out_taken, lane);
+#pragma unroll
+        for (int t = 0; t < 16; t += 4) {
+          const float4 read = *reinterpret_cast<const float4*>(&m.read[c & 1][token + t]);
+          const float2 x = (fma2(Pair(read.x, read.y), q[t / 2], o[t / 2]) * Pair(back, back)).values();
+          const float2 y = (fma2(Pair(read.z, read.w), q[t / 2 + 1], o[t / 2 + 1]) * Pair(back, back)).values();
+          float* to = &m.out[(token + t) * kOutRow + column];
+          to[0] = x.x;
+          to[kOutRow] = x.y;
+          to[2 * kOutRow] = y.x;
+          to[3 * kOutRow] = y.y;
+        }
+      }
+      for (int t = max(broken, kTokens * group); t < kTokens * (group + 1); ++t) m.out[t * kOutRow + column] = NAN;
+    };
+    // half of the rows that a thread has of chunk c, from shared memory to the output
+    auto gate_at = [&](int c, int i) {                                         // of row i
+      const int t = min(kOutRows * i + out_row, rows - c * kChunk - 1);
+      return *reinterpret_cast<const uint4*>(a.gate.data + (row0 + c * kChunk + t) * a.gate.row_stride + head * a.gate.head_stride + 8 * piece);
+    };
+    auto write_rows = [&](int c, int which, const uint4* gates) {
+      constexpr int kRows = kOutPasses / 2;
+      float o[kRows][8], sum[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const float* from = &m.out[(kOutRows * (kRows * which + i) + out_row) * kOutRow + 8 * piece];
+        *reinterpret_cast<float4*>(o[i]) = *reinterpret_cast<const float4*>(from);
+        *reinterpret_cast<float4*>(o[i] + 4) = *reinterpret_cast<const float4*>(from + 4);
+      }
+      if (gated) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          sum[i] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum[i] = fmaf(o[i][j], o[i][j], sum[i]);
+        }
+#pragma unroll
+        for (int d = 8; d >= 1; d /= 2)
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
+        float weight[8];
+        unpack8(*reinterpret_cast<const uint4*>(a.norm_weight + 8 * piece), weight);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const float factor = rsqrtf(fmaf(sum[i], 1.0f / kLinearDim, a.eps));
+          float z[8];
+          unpack8(gates[kRows * which + i], z);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[i][j] *= factor * weight[j] * linear_silu(z[j]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int t = c * kChunk + kOutRows * (kRows * which + i) + out_row;
+        if (t < rows)
+          *reinterpret_cast<uint4*>(a.out + ((row0 + t) * a.v_heads + head) * kLinearDim + 8 * piece) =
+              make_uint4(pack_bf16(o[i][0], o[i][1]), pack_bf16(o[i][2], o[i][3]), pack_bf16(o[i][4], o[i][5]), pack_bf16(o[i][6], o[i][7]));
+      }
+    };
+
     Pair s[kKeys / 2];                                                         // key elements kKeys group ..
     float scale = 1.0f;
     {
@@ -142,8 +221,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
       for (int i = 0; i < kKeys; i += 2) {
         float x = 0.0f, y = 0.0f;
         if (!seq.fresh && n > 0) {
-          x = state[(kKeys * group + i) * kLinearDim + column];
-          y = state[(kKeys * group + i + 1) * kLinearDim + column];
+          x = state[i * kLinearDim];
+          y = state[(i + 1) * kLinearDim];
         }
         s[i / 2] = Pair(x, y);
         largest = max3_abs(largest, x, y);
@@ -151,6 +230,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
       m.largest[group][column] = largest;
       chain_barrier();
     }
+    auto load_state = [&](int c) {                                             // after chunk c
+      wait(&m.state_full, c);
+      tc_fence_after();
+#pragma unroll
+      for (int b = 0; b < kKeys / 16; ++b) tmem_ld16(lanes + kStateAt + kKeys * group + 16 * b, reinterpret_cast<uint32_t*>(s + 8 * b));
+      tmem_ld_wait();
+      if (m.broken[c & 1][column] < kChunk) {
+#pragma unroll
+        for (int i = 0; i < kKeys / 2; ++i) s[i] = Pair(NAN, NAN);
+      }
+    };
     float value_before = 0.0f;
     for (int c = 0; c < n; ++c) {
       const uint8_t* stage = m.stages[c % kStages];
@@ -165,7 +255,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
         const float value = fmaxf(m.largest_value[c % kStages][0][column], m.largest_value[c % kStages][1][column]);
         float largest = fmaxf(value, value_before);
 #pragma unroll
-        for (int i = 0; i < kChainGroups; ++i) largest = fmaxf(largest, m.largest[i][column]);
+        for (int i = 0; i < kGroups; ++i) largest = fmaxf(largest, m.largest[i][column]);
         const float held = largest * scale;
         value_before = value;
         rescale = !(held <= 256.0f && held >= 0.5f) && largest > 0.0f && largest < INFINITY;
@@ -174,22 +264,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
           up = kv_exp2(max(min(next - now, 126), -126));
           scale = kv_exp2(next);
         }
-        if (group == 0) {
+        if (group == 0) {                     // what two chunks ago was left here has been read
           m.scale[c & 1][column] = scale;
           m.broken[c & 1][column] = kChunk;
         }
       }
-      if (c > 0) {
-        wait(&m.state_full, c - 1);
-        tc_fence_after();
-#pragma unroll
-        for (int b = 0; b < kKeys / 16; ++b) tmem_ld16(lanes + kStateAt + kKeys * group + 16 * b, reinterpret_cast<uint32_t*>(s + 8 * b));
-        tmem_ld_wait();
-        if (m.broken[(c - 1) & 1][column] < kChunk) {
-#pragma unroll
-          for (int i = 0; i < kKeys / 2; ++i) s[i] = Pair(NAN, NAN);
-        }
-      }
+      if (c > 0) load_state(c - 1);
       if (rescale) {
 #pragma unroll
         for (int i = 0; i < kKeys / 2; ++i) s[i] = s[i] * Pair(up, up);
@@ -206,27 +286,35 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
           warp_arrive(&m.state_ready[b / (kKeys / 32)], lane);
         }
       }
-      float largest_here;
+      float largest_here = 0.0f;
       {
-        const float decay = plan.kept_only ? numbers.decay_kept : numbers.decay, back = kv_exp2(-kv_float_exponent(scale));
-        float largest = 0.0f;
+        const float decay = kOutputs ? numbers.decay : numbers.decay_kept;
 #pragma unroll
         for (int b = 0; b < kKeys / 16; ++b) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float2 x = s[8 * b + i].values();
-            largest = max3_abs(largest, x.x, x.y);
+            largest_here = max3_abs(largest_here, x.x, x.y);
             s[8 * b + i] = s[8 * b + i] * Pair(decay, decay);
           }
           tmem_st16(lanes + kStateAt + kKeys * group + 16 * b, reinterpret_cast<uint32_t*>(s + 8 * b));
         }
-        largest_here = largest * back;
+        largest_here *= kv_exp2(-kv_float_exponent(scale));
+      }
+      if (kOutputs && c > 0) {
+        wait(&m.state_ready[1], c);           // all warps are done with the rows that lie in shared memory
+        take_outputs(c - 1);
       }
       uint32_t v[kTokens / 2];                                                 // tokens kTokens group .., two in a word
       {
         const uint16_t* values = reinterpret_cast<const uint16_t*>(stage + kStageValues) + kTokens * group * kLinearDim + column;
 #pragma unroll
         for (int t = 0; t < kTokens; t += 2) v[t / 2] = values[t * kLinearDim] | static_cast<uint32_t>(values[(t + 1) * kLinearDim]) << 16;
+      }
+      uint4 gates[kOutPasses];
+      if (gated && c > 0) {
+#pragma unroll
+        for (int i = 0; i < kOutPasses; ++i) gates[i] = gate_at(c - 1, i);
       }
       wait(&m.dots_full, c);
       tc_fence_after();
@@ -278,12 +366,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
           warp_arrive(&m.enter_ready[b], lane);
         }
       }
+      if (kOutputs && c > 0) {
+        wait(&m.enter_ready[kTokenSteps - 1], c);                              // all warps' part of the rows is there
+        write_rows(c - 1, 0, gates);
+      }
       // the corrections
       {
         Pair d[kTokens / 2];
         wait(&m.fresh_full, c);
         tc_fence_after();
-        const float* stay = (plan.kept_only ? numbers.stay_kept : numbers.stay) + kTokens * group;
+        const float* stay = (kOutputs ? numbers.stay : numbers.stay_kept) + kTokens * group;
         uint32_t terms[16];
 #pragma unroll
         for (int b = 0; b < kTokens / 16; ++b) tmem_ld16(lanes + kDotsAt + kTokens * group + 16 * b, reinterpret_cast<uint32_t*>(d + 8 * b));
@@ -301,253 +393,188 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
           tmem_st_wait();
           warp_arrive(&m.stay_ready[b], lane);
         }
-        if (lane == 0) mbar_arrive(smem_u32(&m.empty[c % kStages]));
+        if (kOutputs) {
+          if (column < kTokens) m.read[c & 1][kTokens * group + column] = numbers.read[kTokens * group + column];
 #pragma unroll
-        for (int b = 0; b < kTokens / 16; ++b) {
+          for (int b = 0; b < kTokens / 16; ++b) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) split_f16(d[8 * b + i], &terms[i], &terms[8 + i]);
-          tmem_st16(lanes + kFreshAt + kTokens * group + 16 * b, terms);
+            for (int i = 0; i < 8; ++i) split_f16(d[8 * b + i], &terms[i], &terms[8 + i]);
+            tmem_st16(lanes + kFreshAt + kTokens * group + 16 * b, terms);
+          }
+          tmem_st_wait();
+          warp_arrive(&m.fresh_ready, lane);
         }
-        tmem_st_wait();
-        warp_arrive(&m.fresh_ready, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&m.empty[c % kStages]));
       }
+      if (kOutputs && c > 0) write_rows(c - 1, 1, gates);
     }
     if (n > 0) {
-      wait(&m.state_full, n - 1);
-      tc_fence_after();
+      load_state(n - 1);
+      if (plan.store && seq.kept > seq.first) {
+        const float back = kv_exp2(-kv_float_exponent(scale));
 #pragma unroll
-      for (int b = 0; b < kKeys / 16; ++b) tmem_ld16(lanes + kStateAt + kKeys * group + 16 * b, reinterpret_cast<uint32_t*>(s + 8 * b));
-      tmem_ld_wait();
-      if (m.broken[(n - 1) & 1][column] < kChunk) {
+        for (int i = 0; i < kKeys / 2; ++i) {
+          const float2 x = s[i].values();
+          state[2 * i * kLinearDim] = x.x * back;
+          state[(2 * i + 1) * kLinearDim] = x.y * back;
+        }
+      }
+      if (kOutputs) {
+        uint4 gates[kOutPasses];
+        if (gated) {
 #pragma unroll
-        for (int i = 0; i < kKeys / 2; ++i) s[i] = Pair(NAN, NAN);
+          for (int i = 0; i < kOutPasses; ++i) gates[i] = gate_at(n - 1, i);
+        }
+        chain_barrier();
+        take_outputs(n - 1);
+        chain_barrier();
+        write_rows(n - 1, 0, gates);
+        write_rows(n - 1, 1, gates);
       }
     }
-    if (n > 0 && plan.store && seq.kept > seq.first) {
-      const float back = kv_exp2(-kv_float_exponent(scale));
-#pragma unroll
-      for (int i = 0; i < kKeys / 2; ++i) {
-        const float2 x = s[i].values();
-        state[(kKeys * group + 2 * i) * kLinearDim + column] = x.x * back;
-        state[(kKeys * group + 2 * i + 1) * kLinearDim + column] = x.y * back;
-      }
-    }
-  } else if (warp < kChainWarps + kOutWarps) {
-    // ------------------------------ outputs ------------------------------
-    fewer_registers<kOutRegisters>();
-    const int w = warp - kChainWarps, group = w >> 2, column = (w & 3) * 32 + lane;
-    const uint32_t lanes = tmem + (static_cast<uint32_t>((w & 3) * 32) << 16);
-    const bool outputs = a.out != nullptr && !plan.kept_only, gated = outputs && a.gate.data != nullptr;
-    const int half = lane >> 4, piece = lane & 15;
-    uint4 weights = make_uint4(0, 0, 0, 0);
-    if (gated) weights = *reinterpret_cast<const uint4*>(a.norm_weight + 8 * piece);
+  } else if (warp == kChainWarps) {
+    // ------------------------------ products ------------------------------
+    // Products of different shapes need not run in the order of issue: one that reads or writes what another wrote waits for its commit.
+    // A step with N = 64 takes 32 cycles, one with 128 takes 64.  What the chain waits for goes first.
+    constexpr uint32_t kNarrow = instr_desc_f8(kF16, kF16, 0, 0, 128, kChunk), kUpdate = instr_desc_f8(kF16, kF16, 0, 1, 128, kLinearDim);
+    // descriptors: those of a stage's begin, to which constants are added (an address takes their low 14 bits)
+    const uint32_t base = smem_u32(m.stages[0]);
     for (int c = 0; c < n; ++c) {
-      const uint8_t* stage = m.stages[c % kStages];
-      const ChunkNumbers& numbers = *reinterpret_cast<const ChunkNumbers*>(stage + kChunkPairBytes + kChunkNumbersAt);
-      // the gate's rows come while the chunk is under way: 16 lanes a row, four rows a thread, which reads no others
-      const int there = min(kChunk, rows - c * kChunk);
-      if (gated) {
+      const uint32_t at = base + (c % kStages) * kStageBytes;
+      const uint64_t rows_desc = smem_desc_rows<128>(at), update_desc = smem_desc_rows<128>(at, kChunkPanelBytes);
+      auto dots = [&](int half, uint32_t to, uint32_t rows_at) {                  // of a half of each group's key elements
 #pragma unroll
-        for (int i = 0; i < kChunk / 2 / kOutWarps; ++i) {
-          const int t = 2 * kOutWarps * i + 2 * w + half;
-          if (t < there)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                         :: "r"(smem_u32(&m.gate[t * kLinearDim + 8 * piece])),
-                            "l"(a.gate.data + (row0 + c * kChunk + t) * a.gate.row_stride + head * a.gate.head_stride + 8 * piece) : "memory");
-        }
-      }
-      wait(&m.out_full, c);
-      tc_fence_after();
-      if (outputs) {
-        const float back = kv_exp2(-kv_float_exponent(m.scale[c & 1][column])) * 0.08838834764831845f;
-        const int broken = m.broken[c & 1][column];
-        out_barrier();                                                         // the rows of the chunk before have been read
+        for (int i = 0; i < kKeys / 32; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {                                          // 16 tokens
-          const int token = 32 * group + 16 * h;
-          Pair o[8], q[8];
-          tmem_ld16(lanes + kDotsAt + token, reinterpret_cast<uint32_t*>(o));
-          tmem_ld16(lanes + kReadAt + token, reinterpret_cast<uint32_t*>(q));
-          tmem_ld_wait();
-          if (h == 1) warp_arrive(&m.dots_empty, lane);
+          for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-          for (int t = 0; t < 16; t += 4) {
-            const float4 read = *reinterpret_cast<const float4*>(&numbers.read[token + t]);
-            const float2 x = (fma2(Pair(read.x, read.y), q[t / 2], o[t / 2]) * Pair(back, back)).values();
-            const float2 y = (fma2(Pair(read.z, read.w), q[t / 2 + 1], o[t / 2 + 1]) * Pair(back, back)).values();
-            float* to = &m.out[(token + t) * kOutRow + column];
-            to[0] = x.x;
-            to[kOutRow] = x.y;
-            to[2 * kOutRow] = y.x;
-            to[3 * kOutRow] = y.y;
-          }
-        }
-        for (int t = max(broken, kChunk / kOutGroups * group); t < kChunk / kOutGroups * (group + 1); ++t) m.out[t * kOutRow + column] = NAN;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&m.empty[c % kStages]));
-        out_barrier();
-        // two rows' loads, then the arithmetic, then the stores: rows need not wait for each other
-#pragma unroll
-        for (int i0 = 0; i0 < kChunk / 2 / kOutWarps; i0 += 2) {
-          float o[2][8], sum[2] = {0.0f, 0.0f};
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float* from = &m.out[(2 * kOutWarps * (i0 + i) + 2 * w + half) * kOutRow + 8 * piece];
-            *reinterpret_cast<float4*>(o[i]) = *reinterpret_cast<const float4*>(from);
-            *reinterpret_cast<float4*>(o[i] + 4) = *reinterpret_cast<const float4*>(from + 4);
-          }
-          if (gated) {
-            if (i0 == 0) asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int j = 0; j < 8; ++j) sum[i] = fmaf(o[i][j], o[i][j], sum[i]);
-#pragma unroll
-            for (int d = 8; d >= 1; d /= 2)
-#pragma unroll
-              for (int i = 0; i < 2; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
-            float weight[8];
-            unpack8(weights, weight);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float factor = rsqrtf(fmaf(sum[i], 1.0f / kLinearDim, a.eps));
-              float z[8];
-              unpack8(*reinterpret_cast<const uint4*>(&m.gate[(2 * kOutWarps * (i0 + i) + 2 * w + half) * kLinearDim + 8 * piece]), z);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) o[i][j] *= factor * weight[j] * linear_silu(z[j]);
+            for (int term = 0; term < 2; ++term) {
+              const int k = g * (kKeys / 16) + half * (kKeys / 32) + i;
+              umma_f16_ts(to, kTermsAt + operand(k, term), rows_desc + ((rows_at + (k / 4) * kChunkPanelBytes + (k % 4) * 32) >> 4), kNarrow,
+                          (half | i | g | term) != 0);
             }
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int t = 2 * kOutWarps * (i0 + i) + 2 * w + half;
-            if (t < there)
-              *reinterpret_cast<uint4*>(a.out + ((row0 + c * kChunk + t) * a.v_heads + head) * kLinearDim + 8 * piece) =
-                  make_uint4(pack_bf16(o[i][0], o[i][1]), pack_bf16(o[i][2], o[i][3]), pack_bf16(o[i][4], o[i][5]), pack_bf16(o[i][6], o[i][7]));
-          }
-        }
-      } else {
-        warp_arrive(&m.dots_empty, lane);
-        if (lane == 0) mbar_arrive(smem_u32(&m.empty[c % kStages]));
+      };
+      if (!wait(&m.full[c % kStages], c / kStages) || !wait(&m.state_ready[0], c)) break;
+      tc_fence_after();
+      if (elect_one()) dots(0, kDotsAt, 0);
+      __syncwarp();
+      if (!wait(&m.state_ready[1], c)) break;
+      tc_fence_after();
+      if (elect_one()) {
+        dots(1, kDotsAt, 0);
+        umma_commit(smem_u32(&m.dots_full));
       }
-    }
-  } else {
-    fewer_registers<kIssueRegisters>();
-    if (warp == kChainWarps + kOutWarps) {
-      // ------------------------------ products ------------------------------
-      // Products of different shapes need not run in the order of issue: one that reads or writes what another wrote waits for its commit.
-      // A step with N = 64 takes 32 cycles, one with 128 takes 64.  What the chain waits for goes first.
-      constexpr uint32_t kNarrow = instr_desc_f8(kF16, kF16, 0, 0, 128, kChunk), kUpdate = instr_desc_f8(kF16, kF16, 0, 1, 128, kLinearDim);
-      // descriptors: those of a stage's begin, to which constants are added (an address takes their low 14 bits)
-      const uint32_t base = smem_u32(m.stages[0]);
-      for (int c = 0; c < n; ++c) {
-        const uint32_t at = base + (c % kStages) * kStageBytes;
-        const uint64_t rows_desc = smem_desc_rows<128>(at), update_desc = smem_desc_rows<128>(at, kChunkPanelBytes);
-        auto dots = [&](int half, uint32_t to, uint32_t rows_at) {                // of a half of each group's key elements
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int term = i & 1, g = (i >> 1) % kChainGroups, k = g * (kKeys / 16) + half * (kKeys / 32) + (i >> 1) / kChainGroups;
-            if ((i >> 1) / kChainGroups < kKeys / 32)
-              umma_f16_ts(to, kTermsAt + operand(k, term), rows_desc + ((rows_at + (k / 4) * kChunkPanelBytes + (k % 4) * 32) >> 4), kNarrow, (half | i) != 0);
-          }
-        };
-        if (!wait(&m.full[c % kStages], c / kStages) || (c > 0 && !wait(&m.dots_empty, c - 1)) || !wait(&m.state_ready[0], c)) break;
-        tc_fence_after();
-        if (elect_one()) dots(0, kDotsAt, 0);
-        __syncwarp();
-        if (!wait(&m.state_ready[1], c)) break;
+      __syncwarp();
+      if (kOutputs) {
+        if (c > 0 && !wait(&m.out_taken, c - 1)) break;
         tc_fence_after();
         if (elect_one()) {
-          dots(1, kDotsAt, 0);
-          umma_commit(smem_u32(&m.dots_full));
           dots(0, kReadAt, kChunk * 128);
           dots(1, kReadAt, kChunk * 128);
         }
         __syncwarp();
-        bool alive = true;
+      }
+      bool alive = true;
 #pragma unroll
-        for (int half = 0; half < 2 && alive; ++half) {                           // of each group's tokens
-          alive = wait(&m.enter_ready[half], c);
-          tc_fence_after();
-          if (alive && elect_one()) {
+      for (int step = 0; step < kTokenSteps && alive; ++step) {                   // of each group's tokens
+        alive = wait(&m.enter_ready[step], c);
+        tc_fence_after();
+        if (alive && elect_one()) {
 #pragma unroll
-            for (int g = 0; g < kChainGroups; ++g)
+          for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-              for (int term = 0; term < 3; ++term) {                              // both terms by T's first, the first by T's second
-                const int k = g * (kTokens / 16) + half;
-                umma_f16_ts(kDotsAt, kEnterAt + operand(k, term == 1), rows_desc + ((kChunkPairBytes + (term == 2 ? kChunkMatrixBytes : 0) + k * 32) >> 4), kNarrow,
-                            (half | g | term) != 0);
-              }
-            if (half == 1) umma_commit(smem_u32(&m.fresh_full));
-          }
-          __syncwarp();
+            for (int term = 0; term < 3; ++term) {                                // both terms by T's first, the first by T's second
+              const int k = g * kTokenSteps + step;
+              umma_f16_ts(kDotsAt, kEnterAt + operand(k, term == 1), rows_desc + ((kChunkPairBytes + (term == 2 ? kChunkMatrixBytes : 0) + k * 32) >> 4), kNarrow,
+                          (step | g | term) != 0);
+            }
+          if (step == kTokenSteps - 1) umma_commit(smem_u32(&m.fresh_full));
         }
+        __syncwarp();
+      }
 #pragma unroll
-        for (int half = 0; half < 2 && alive; ++half) {
-          alive = wait(&m.stay_ready[half], c);
-          tc_fence_after();
-          if (alive && elect_one()) {
+      for (int step = 0; step < kTokenSteps && alive; ++step) {
+        alive = wait(&m.stay_ready[step], c);
+        tc_fence_after();
+        if (alive && elect_one()) {
 #pragma unroll
-            for (int g = 0; g < kChainGroups; ++g)
+          for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-              for (int term = 0; term < 2; ++term) {
-                const int k = g * (kTokens / 16) + half;
-                umma_f16_ts(kStateAt, kEnterAt + operand(k, term), update_desc + ((k * 16 * 128) >> 4), kUpdate, 1);
-              }
-            if (half == 1) umma_commit(smem_u32(&m.state_full));
+            for (int term = 0; term < 2; ++term) {
+              const int k = g * kTokenSteps + step;
+              umma_f16_ts(kStateAt, kEnterAt + operand(k, term), update_desc + ((k * 16 * 128) >> 4), kUpdate, 1);
+            }
+          if (step == kTokenSteps - 1) {
+            umma_commit(smem_u32(&m.state_full));
+            if (!kOutputs) umma_commit(smem_u32(&m.empty[c % kStages]));
           }
-          __syncwarp();
         }
-        if (!alive || !wait(&m.fresh_ready, c)) break;
+        __syncwarp();
+      }
+      if (!alive) break;
+      if (kOutputs) {
+        if (!wait(&m.fresh_ready, c) || !wait(&m.state_full, c)) break;           // O goes where the state's corrections are read
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int term = 0; term < 3; ++term)                                    // both terms by the scores' first, the first by their second
 #pragma unroll
             for (int k = 0; k < kChunk / 16; ++k)
-              umma_f16_ts(kDotsAt, kFreshAt + operand(k, term == 1),
+              umma_f16_ts(kEnterAt, kFreshAt + operand(k, term == 1),
                           rows_desc + ((kChunkPairBytes + (term == 2 ? 3 : 2) * kChunkMatrixBytes + k * 32) >> 4), kNarrow, (term | k) != 0);
           umma_commit(smem_u32(&m.out_full));
           umma_commit(smem_u32(&m.empty[c % kStages]));
         }
         __syncwarp();
       }
-    } else if (warp == kChainWarps + kOutWarps + 1) {
-      // ------------------------------ loads ------------------------------
-      int c = 0;
-      for (; c < n; ++c) {
-        const int slot = c % kStages;
-        if (!wait(&m.empty[slot], c / kStages + 1)) break;
-        const uint32_t to = smem_u32(m.stages[slot]), bar = smem_u32(&m.full[slot]);
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar, kStageValues);
-          const size_t tile = static_cast<size_t>(tile0 + c);
-          bulk_g2s(to, plan.pairs + (tile * a.k_heads + head / a.group) * kChunkPairBytes, kChunkPairBytes, bar);
-          bulk_g2s(to + kChunkPairBytes, plan.heads + (tile * a.v_heads + head) * kChunkHeadBytes, kChunkHeadBytes, bar);
-        }
-        __syncwarp();
+    }
+  } else if (warp == kChainWarps + 1) {
+    // ------------------------------ loads ------------------------------
+    int c = 0;
+    for (; c < n; ++c) {
+      const int slot = c % kStages;
+      if (!wait(&m.empty[slot], c / kStages + 1)) break;
+      const uint32_t to = smem_u32(m.stages[slot]), bar = smem_u32(&m.full[slot]);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, kStageValues);
+        const size_t tile = static_cast<size_t>(tile0 + c);
+        bulk_g2s(to, plan.pairs + (tile * a.k_heads + head / a.group) * kChunkPairBytes, kChunkPairBytes, bar);
+        bulk_g2s(to + kChunkPairBytes, plan.heads + (tile * a.v_heads + head) * kChunkHeadBytes, kChunkHeadBytes, bar);
       }
-      if (*abort_flag != 0) {                // what is in flight lands before the block leaves
-        volatile int ignore = 0;
-        for (int i = max(0, c - kStages); i < c; ++i) wait_inline(smem_u32(&m.full[i % kStages]), (i / kStages) & 1, &ignore, kWaitBudgetNs);
-      }
-    } else {
-      // ------------------------------ values, and the largest of each column ------------------------------
-      // 16 lanes a row, 16 rows a thread.  (A copy of 256 bytes for each row took 70 cycles to issue, 5000 for the chunk.)
-      const int which = warp & 1, piece = lane & 15, first = 2 * which + (lane >> 4);
-      for (int c = 0; c < n; ++c) {
-        const int slot = c % kStages, there = min(kChunk, rows - c * kChunk);
-        uint8_t* to = m.stages[slot] + kStageValues + first * 2 * kLinearDim + piece * 16;
-        const __nv_bfloat16* from = a.v.data + (row0 + c * kChunk + first) * a.v.row_stride + head * a.v.head_stride + 8 * piece;
-        wait(&m.empty[slot], c / kStages + 1);
+      __syncwarp();
+    }
+    if (*abort_flag != 0) {                // what is in flight lands before the block leaves
+      volatile int ignore = 0;
+      for (int i = max(0, c - kStages); i < c; ++i) wait_inline(smem_u32(&m.full[i % kStages]), (i / kStages) & 1, &ignore, kWaitBudgetNs);
+    }
+  } else {
+    // ------------------------------ values, and the largest of each column ------------------------------
+    // 16 lanes a row, 16 rows a thread.  (A copy of 256 bytes for each row took 70 cycles to issue, 5000 for the chunk.)
+    const int which = warp & 1, piece = lane & 15, first = 2 * which + (lane >> 4);
+    const __nv_bfloat16* from = a.v.data + (row0 + first) * a.v.row_stride + head * a.v.head_stride + 8 * piece;
+    for (int c = 0; c < n; ++c) {
+      const int slot = c % kStages, there = min(kChunk, rows - c * kChunk) - first;
+      uint8_t* const to = m.stages[slot] + kStageValues + first * 2 * kLinearDim + piece * 16;
+      wait(&m.empty[slot], c / kStages + 1);
+      const uint32_t at = smem_u32(to);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const bool is = first + 4 * i < there;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                       :: "r"(smem_u32(to + i * 4 * 2 * kLinearDim)), "l"(is ? from + 4 * i * a.v.row_stride : a.v.data), "r"(is ? 16 : 0) : "memory");
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        uint32_t most[4] = {0, 0, 0, 0};
+      for (int i = 0; i < 16; ++i) {
+        const bool is = 4 * i < there;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(at + i * 4 * 2 * kLinearDim), "l"(is ? from : a.v.data), "r"(is ? 16 : 0) : "memory");
+        from += 4 * a.v.row_stride;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      uint32_t most[4] = {0, 0, 0, 0};
 #pragma unroll 4
+      for (int i = 0; i < 16; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(to + i * 4 * 2 * kLinearDim);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most[j] = __vmaxu2(most[j], (&x.x)[j] & 0x7fff7fffu);
+      }
+      if (__vmaxu2(__vmaxu2(most[0], most[1]), __vmaxu2(most[2], most[3])) != __vminu2(__vmaxu2(__vmaxu2(most[0], most[1]), __vmaxu2(most[2], most[3])), 0x7f7f7f7fu)) {
+        most[0] = most[1] = most[2] = most[3] = 0;
+#pragma unroll 1
         for (int i = 0; i < 16; ++i) {
           const uint4 x = *reinterpret_cast<const uint4*>(to + i * 4 * 2 * kLinearDim);
 #pragma unroll
@@ -558,24 +585,24 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
             most[j] = __vmaxu2(most[j], y);
           }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) most[j] = __vmaxu2(most[j], __shfl_xor_sync(0xffffffffu, most[j], 16));
-        if (lane < 16) {
-          float4* largest = reinterpret_cast<float4*>(&m.largest_value[slot][which][8 * piece]);
-          largest[0] = make_float4(bf16_lo(most[0]), bf16_hi(most[0]), bf16_lo(most[1]), bf16_hi(most[1]));
-          largest[1] = make_float4(bf16_lo(most[2]), bf16_hi(most[2]), bf16_lo(most[3]), bf16_hi(most[3]));
-        }
-        wait(&m.full[slot], c / kStages);                                         // for those that wait for this alone
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&m.values_full[slot]));
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) most[j] = __vmaxu2(most[j], __shfl_xor_sync(0xffffffffu, most[j], 16));
+      if (lane < 16) {
+        float4* largest = reinterpret_cast<float4*>(&m.largest_value[slot][which][8 * piece]);
+        largest[0] = make_float4(bf16_lo(most[0]), bf16_hi(most[0]), bf16_lo(most[1]), bf16_hi(most[1]));
+        largest[1] = make_float4(bf16_lo(most[2]), bf16_hi(most[2]), bf16_lo(most[3]), bf16_hi(most[3]));
+      }
+      wait(&m.full[slot], c / kStages);                                           // for those that wait for this alone
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&m.values_full[slot]));
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (threadIdx.x == 0 && *abort_flag != 0) atomicOr(a.status, kLinearTimeout);
-  if (warp == kChainWarps + kOutWarps) tmem_dealloc(tmem, 512);
+  if (warp == kChainWarps) tmem_dealloc(tmem, 512);
 }
 
 size_t tiles_of(int tokens, int sequences, int min_rows) {
@@ -600,16 +627,16 @@ cudaError_t linear_chunks(const LinearDelta& a, int min_rows, void* workspace, c
   cudaError_t error = linear_prepare(plan, stream);
   if (error != cudaSuccess) return error;
   constexpr int kBytes = static_cast<int>(sizeof(ChunkMemory)) + 1024;
-  error = opt_in_dynamic_smem<linear_chunk_kernel>(kBytes);
+  error = opt_in_dynamic_smem<linear_chunk_kernel<true>>(kBytes);
+  if (error == cudaSuccess) error = opt_in_dynamic_smem<linear_chunk_kernel<false>>(kBytes);
   if (error != cudaSuccess) return error;
   const dim3 grid(a.v_heads, a.batch.sequences);
   // with rows that are computed but do not stay, once for the outputs and once for the states
-  plan.kept_only = a.out == nullptr;
-  plan.store = a.out == nullptr || a.batch.keep == nullptr;
-  linear_chunk_kernel<<<grid, kChunkThreads, kBytes, stream>>>(plan);
-  if (a.out != nullptr && a.batch.keep != nullptr) {
-    plan.kept_only = plan.store = 1;
-    linear_chunk_kernel<<<grid, kChunkThreads, kBytes, stream>>>(plan);
+  plan.store = a.batch.keep == nullptr;
+  if (a.out != nullptr) linear_chunk_kernel<true><<<grid, kChunkThreads, kBytes, stream>>>(plan);
+  if (a.out == nullptr || a.batch.keep != nullptr) {
+    plan.store = 1;
+    linear_chunk_kernel<false><<<grid, kChunkThreads, kBytes, stream>>>(plan);
   }
   return cudaGetLastError();
 }

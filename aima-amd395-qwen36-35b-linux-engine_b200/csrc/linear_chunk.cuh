@@ -41,7 +41,6 @@ struct ChunkPlan {
   LinearDelta a;
   int min_rows;                // sequences with more rows than this are taken here
   int tiles;                   // that `pairs` and `heads` have room for
-  int kept_only;               // the states alone: rows behind the last that enters them are left out
   int store;                   // whether the states are written
   uint8_t* pairs;              // [tiles, k_heads, kChunkPairBytes]
   uint8_t* heads;              // [tiles, v_heads, kChunkHeadBytes]
@@ -116,11 +115,6 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
-template <int kCount>
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kCount)); }
-template <int kCount>
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kCount)); }
-
 cudaError_t linear_prepare(const ChunkPlan& plan, cudaStream_t stream);
 
 }  // namespace aima
