@@ -150,7 +150,7 @@ constexpr int kLinearStepRows = 32;   // rows of a sequence up to which it is ta
 cudaError_t linear_step(const LinearDelta& args, int max_rows, cudaStream_t stream);
 size_t linear_chunk_workspace(int k_heads, int v_heads, int max_tokens, int max_sequences);
 // Sequences of more than min_rows rows.
-cudaError_t linear_chunks(const LinearDelta& args, int min_rows, void* workspace, cudaStream_t stream);
+cudaError_t linear_chunks(const LinearDelta& args, int min_rows, void* workspace, int sm_count, cudaStream_t stream);
 
 struct HeadNorm {
   int tokens, heads, dim, activation;

@@ -11,6 +11,11 @@
 // product: the outputs of the chunk before are taken from tensor memory and turned into rows while R runs, and normed and written while D
 // and S run; warps of their own for that slowed the chain by as much as they saved (9000 cycles a chunk; the floor of the products is
 // 2300).  One warp issues products, three load.
+//
+// Few heads leave multiprocessors idle, so a sequence's chunks are cut into segments then.  What a segment does to the state is
+// S <- M S + B: a first pass finds the state behind the first segment, and M (values of zero, the identity as state) and B (a state of
+// zeros) of those between the first and the last; the states at all borders follow from them, and a second pass goes through all segments
+// at once.  The first pass has no outputs and takes 0.6 of the time of the second.
 #include "linear_chunk.cuh"
 
 #include <algorithm>
@@ -69,9 +74,19 @@ __device__ __forceinline__ void warp_arrive(unsigned long long* bar, int lane) {
   if (lane == 0) mbar_arrive(smem_u32(bar));
 }
 
-// kOutputs: all rows, the states if plan.store says so; else the states alone, for the rows that enter them.
-template <bool kOutputs>
+// What is at a head's `borders`: the states before the segments, then B and M of those between the first and the last.
+__device__ __forceinline__ float* border(const ChunkPlan& plan, int sequence, int head, int which) {
+  return plan.borders + ((static_cast<size_t>(sequence) * plan.a.v_heads + head) * kMaxBorders + which) * kLinearDim * kLinearDim;
+}
+__device__ __forceinline__ int border_b(int segment) { return kMaxSegments + 2 * segment; }
+__device__ __forceinline__ int border_m(int segment) { return kMaxSegments + 2 * segment + 1; }
+
+// kOutput: all rows of a segment, the state behind the last if plan.store says so.  kKept: the states alone, for the rows that enter them.
+// kTransfer: the first pass over segments.
+enum ChunkMode { kOutput, kKept, kTransfer };
+template <ChunkMode kMode>
 __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const ChunkPlan plan) {
+  constexpr bool kOutputs = kMode == kOutput;
   extern __shared__ uint8_t raw[];
   ChunkMemory& m = *reinterpret_cast<ChunkMemory*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const LinearDelta& a = plan.a;
@@ -79,14 +94,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   const int head = blockIdx.x;
   const LinearSequence seq = linear_sequence(a.batch, blockIdx.y);
   if (seq.rows <= plan.min_rows) return;
-  if (kOutputs) {                                     // rows that are not active
+  // segment, and for the first pass whether its M is wanted
+  const int segment = kMode == kTransfer ? (static_cast<int>(blockIdx.z) + 1) / 2 : static_cast<int>(blockIdx.z);
+  const bool transfer = kMode == kTransfer && segment > 0 && blockIdx.z % 2 == 0;
+  if (kOutputs && segment == 0) {                     // rows that are not active
     for (int i = threadIdx.x; i < seq.first * (kLinearDim / 8); i += kChunkThreads)
       *reinterpret_cast<uint4*>(a.out + (static_cast<long long>(seq.row0 + i / (kLinearDim / 8)) * a.v_heads + head) * kLinearDim + 8 * (i % (kLinearDim / 8))) =
           make_uint4(0, 0, 0, 0);
   }
-  const int limit = kOutputs ? seq.rows : seq.kept;                        // rows that are gone through
-  const int chunks = (limit - seq.first + kChunk - 1) / kChunk;
-  if (limit <= seq.first) return;
+  const int limit = kMode == kKept ? seq.kept : seq.rows;                  // rows that are gone through
+  const int all_chunks = (limit - seq.first + kChunk - 1) / kChunk;
+  const int per_segment = (all_chunks + plan.segments - 1) / plan.segments, chunk0 = segment * per_segment;
+  const int chunks = min(per_segment, all_chunks - chunk0);
+  if (limit <= seq.first || chunks <= 0) return;
 
   // its first tile
   int tile0 = 0;
@@ -127,15 +147,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   if (!fits && threadIdx.x == 0) atomicOr(a.status, kLinearBadBatch);
   volatile int* abort_flag = &m.abort_flag;
   auto wait = [&](unsigned long long* bar, int phase) { return wait_inline(smem_u32(bar), phase & 1, abort_flag, plan.wait_limit_ns); };
-  const long long row0 = static_cast<long long>(seq.row0) + seq.first;
-  const int rows = limit - seq.first;                                          // of all chunks
+  tile0 += chunk0;
+  const long long row0 = static_cast<long long>(seq.row0) + seq.first + chunk0 * kChunk;
+  const int rows = limit - seq.first - chunk0 * kChunk;                        // of all its chunks, and behind them
 
   if (warp < kChainWarps) {
     // ------------------------------ the chain ------------------------------
     // No wait that runs out leaves this loop: the warps meet at barriers, and every wait after the first that ran out ends at once.
     const int group = warp >> 2, column = (warp & 3) * 32 + lane;              // a value element
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    float* const state = a.states + (static_cast<long long>(seq.slot) * a.v_heads + head) * kLinearDim * kLinearDim + kKeys * group * kLinearDim + column;
+    const long long part = kKeys * group * kLinearDim + column;                // of a state
+    float* const state = a.states + (static_cast<long long>(seq.slot) * a.v_heads + head) * kLinearDim * kLinearDim + part;
     const bool gated = kOutputs && a.gate.data != nullptr;
     // rows of the output: 16 lanes a row
     const int out_row = 2 * warp + (lane >> 4), piece = lane & 15;
@@ -216,18 +238,35 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
     Pair s[kKeys / 2];                                                         // key elements kKeys group ..
     float scale = 1.0f;
     {
+      // where the state comes from; nullptr: zeros, or the identity.  With segments the first pass keeps the first one's: the second
+      // pass's last segment may write the state before its first one has begun.
+      const float* before = n == 0 || seq.fresh ? nullptr : state;
+      if (kOutputs && plan.segments > 1) before = border(plan, blockIdx.y, head, segment) + part;
+      if (kMode == kTransfer && segment > 0) before = nullptr;
       float largest = 0.0f;
 #pragma unroll
       for (int i = 0; i < kKeys; i += 2) {
         float x = 0.0f, y = 0.0f;
-        if (!seq.fresh && n > 0) {
-          x = state[i * kLinearDim];
-          y = state[(i + 1) * kLinearDim];
+        if (before != nullptr) {
+          x = before[i * kLinearDim];
+          y = before[(i + 1) * kLinearDim];
+        } else if (transfer) {
+          x = kKeys * group + i == column ? 1.0f : 0.0f;
+          y = kKeys * group + i + 1 == column ? 1.0f : 0.0f;
         }
         s[i / 2] = Pair(x, y);
         largest = max3_abs(largest, x, y);
       }
       m.largest[group][column] = largest;
+      if (kMode == kTransfer && segment == 0 && n > 0) {
+        float* const first = border(plan, blockIdx.y, head, 0) + part;
+#pragma unroll
+        for (int i = 0; i < kKeys / 2; ++i) {
+          const float2 x = s[i].values();
+          first[2 * i * kLinearDim] = x.x;
+          first[(2 * i + 1) * kLinearDim] = x.y;
+        }
+      }
       chain_barrier();
     }
     auto load_state = [&](int c) {                                             // after chunk c
@@ -288,7 +327,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
       }
       float largest_here = 0.0f;
       {
-        const float decay = kOutputs ? numbers.decay : numbers.decay_kept;
+        const float decay = kMode == kKept ? numbers.decay_kept : numbers.decay;
 #pragma unroll
         for (int b = 0; b < kKeys / 16; ++b) {
 #pragma unroll
@@ -375,7 +414,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
         Pair d[kTokens / 2];
         wait(&m.fresh_full, c);
         tc_fence_after();
-        const float* stay = (kOutputs ? numbers.stay : numbers.stay_kept) + kTokens * group;
+        const float* stay = (kMode == kKept ? numbers.stay_kept : numbers.stay) + kTokens * group;
         uint32_t terms[16];
 #pragma unroll
         for (int b = 0; b < kTokens / 16; ++b) tmem_ld16(lanes + kDotsAt + kTokens * group + 16 * b, reinterpret_cast<uint32_t*>(d + 8 * b));
@@ -411,13 +450,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
     }
     if (n > 0) {
       load_state(n - 1);
-      if (plan.store && seq.kept > seq.first) {
+      float* after = nullptr;
+      if (kMode == kTransfer) after = border(plan, blockIdx.y, head, segment == 0 ? 1 : transfer ? border_m(segment) : border_b(segment)) + part;
+      else if (plan.store && seq.kept > seq.first && chunk0 + chunks == all_chunks) after = state;
+      if (after != nullptr) {
         const float back = kv_exp2(-kv_float_exponent(scale));
 #pragma unroll
         for (int i = 0; i < kKeys / 2; ++i) {
           const float2 x = s[i].values();
-          state[2 * i * kLinearDim] = x.x * back;
-          state[(2 * i + 1) * kLinearDim] = x.y * back;
+          after[2 * i * kLinearDim] = x.x * back;
+          after[(2 * i + 1) * kLinearDim] = x.y * back;
         }
       }
       if (kOutputs) {
@@ -560,7 +602,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
       const uint32_t at = smem_u32(to);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const bool is = 4 * i < there;
+        const bool is = !transfer && 4 * i < there;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(at + i * 4 * 2 * kLinearDim), "l"(is ? from : a.v.data), "r"(is ? 16 : 0) : "memory");
         from += 4 * a.v.row_stride;
       }
@@ -605,38 +647,93 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   if (warp == kChainWarps) tmem_dealloc(tmem, 512);
 }
 
+// The states before the segments from the first pass: S_(j + 1) = M_j S_j + B_j, a block per head and 16 columns.
+constexpr int kJoinThreads = 256, kJoinColumns = 16;
+__global__ void __launch_bounds__(kJoinThreads) linear_join_kernel(const ChunkPlan plan) {
+  __shared__ float before[kLinearDim][kJoinColumns];
+  const int head = blockIdx.x, sequence = blockIdx.y, column = threadIdx.x % kJoinColumns, first = threadIdx.x / kJoinColumns;
+  const LinearSequence seq = linear_sequence(plan.a.batch, sequence);
+  const int chunks = chunks_of(seq, plan.min_rows), per_segment = (chunks + plan.segments - 1) / plan.segments;
+  const int at = static_cast<int>(blockIdx.z) * kJoinColumns + column;
+  for (int j = 1; j + 1 < plan.segments && (j + 1) * per_segment < chunks; ++j) {
+    const float* from = border(plan, sequence, head, j);
+    for (int r = first; r < kLinearDim; r += kJoinThreads / kJoinColumns) before[r][column] = from[r * kLinearDim + at];
+    __syncthreads();
+    const float* transfer = border(plan, sequence, head, border_m(j));
+    float sum[8];                          // rows first + 16 i
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] = border(plan, sequence, head, border_b(j))[(first + 16 * i) * kLinearDim + at];
+    for (int k = 0; k < kLinearDim; k += 4) {
+      float x[4];
+#pragma unroll
+      for (int l = 0; l < 4; ++l) x[l] = before[k + l][column];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(&transfer[(first + 16 * i) * kLinearDim + k]);
+        sum[i] = fmaf(y.x, x[0], sum[i]);
+        sum[i] = fmaf(y.y, x[1], sum[i]);
+        sum[i] = fmaf(y.z, x[2], sum[i]);
+        sum[i] = fmaf(y.w, x[3], sum[i]);
+      }
+    }
+    float* to = border(plan, sequence, head, j + 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) to[(first + 16 * i) * kLinearDim + at] = sum[i];
+    __syncthreads();                       // a block reads the columns that it wrote
+  }
+}
+
 size_t tiles_of(int tokens, int sequences, int min_rows) {
   return static_cast<size_t>(tokens / kChunk) + std::min(sequences, tokens / (min_rows + 1));
 }
+
+// Segments that a sequence's chunks are cut into: as many as find room for all heads in both passes, if they are worth the launches.
+int segments_of(int heads, int chunks, int sm_count) {
+  int segments = 1;
+  for (int g = 2; g <= kMaxSegments; ++g)
+    if (heads * g <= sm_count && heads * (2 * g - 3) <= sm_count && chunks >= 2 * g) segments = g;
+  return segments;
+}
+constexpr int kMultiprocessors = 148;      // that the workspace reckons with
+size_t border_bytes(int heads) { return static_cast<size_t>(heads) * kMaxBorders * kLinearDim * kLinearDim * sizeof(float); }
 
 }  // namespace
 
 size_t linear_chunk_workspace(int k_heads, int v_heads, int max_tokens, int max_sequences) {
   const size_t tiles = std::max<size_t>(tiles_of(max_tokens, max_sequences, kLinearStepRows), tiles_of(max_tokens, 1, 0));
-  return tiles * (static_cast<size_t>(k_heads) * kChunkPairBytes + static_cast<size_t>(v_heads) * kChunkHeadBytes);
+  // a batch is cut into segments if its heads fill at most half of the multiprocessors
+  const size_t borders = border_bytes(v_heads * std::min(max_sequences, std::max(1, kMultiprocessors / 2 / v_heads)));
+  return borders + tiles * (static_cast<size_t>(k_heads) * kChunkPairBytes + static_cast<size_t>(v_heads) * kChunkHeadBytes);
 }
 
-cudaError_t linear_chunks(const LinearDelta& a, int min_rows, void* workspace, cudaStream_t stream) {
+cudaError_t linear_chunks(const LinearDelta& a, int min_rows, void* workspace, int sm_count, cudaStream_t stream) {
   ChunkPlan plan{};
   plan.a = a;
   plan.min_rows = min_rows;
   plan.tiles = static_cast<int>(tiles_of(a.batch.tokens, a.batch.sequences, min_rows));
-  plan.pairs = static_cast<uint8_t*>(workspace);
+  const int heads = a.v_heads * a.batch.sequences, segments = segments_of(heads, a.batch.max_new / kChunk, std::min(sm_count, kMultiprocessors));
+  plan.borders = static_cast<float*>(workspace);
+  plan.pairs = static_cast<uint8_t*>(workspace) + (segments > 1 ? border_bytes(heads) : 0);
   plan.heads = plan.pairs + static_cast<size_t>(plan.tiles) * a.k_heads * kChunkPairBytes;
   plan.wait_limit_ns = kWaitBudgetNs;
   cudaError_t error = linear_prepare(plan, stream);
-  if (error != cudaSuccess) return error;
   constexpr int kBytes = static_cast<int>(sizeof(ChunkMemory)) + 1024;
-  error = opt_in_dynamic_smem<linear_chunk_kernel<true>>(kBytes);
-  if (error == cudaSuccess) error = opt_in_dynamic_smem<linear_chunk_kernel<false>>(kBytes);
+  if (error == cudaSuccess) error = opt_in_dynamic_smem<linear_chunk_kernel<kOutput>>(kBytes);
+  if (error == cudaSuccess) error = opt_in_dynamic_smem<linear_chunk_kernel<kKept>>(kBytes);
+  if (error == cudaSuccess) error = opt_in_dynamic_smem<linear_chunk_kernel<kTransfer>>(kBytes);
   if (error != cudaSuccess) return error;
-  const dim3 grid(a.v_heads, a.batch.sequences);
+  const auto grid = [&](int parts) { return dim3(a.v_heads, a.batch.sequences, parts); };
   // with rows that are computed but do not stay, once for the outputs and once for the states
-  plan.store = a.batch.keep == nullptr;
-  if (a.out != nullptr) linear_chunk_kernel<true><<<grid, kChunkThreads, kBytes, stream>>>(plan);
+  if (a.out != nullptr) {
+    plan.store = a.batch.keep == nullptr;
+    plan.segments = segments;
+    if (segments > 1) linear_chunk_kernel<kTransfer><<<grid(2 * segments - 3), kChunkThreads, kBytes, stream>>>(plan);
+    if (segments > 2) linear_join_kernel<<<grid(kLinearDim / kJoinColumns), kJoinThreads, 0, stream>>>(plan);
+    linear_chunk_kernel<kOutput><<<grid(segments), kChunkThreads, kBytes, stream>>>(plan);
+  }
   if (a.out == nullptr || a.batch.keep != nullptr) {
-    plan.store = 1;
-    linear_chunk_kernel<false><<<grid, kChunkThreads, kBytes, stream>>>(plan);
+    plan.store = plan.segments = 1;
+    linear_chunk_kernel<kKept><<<grid(1), kChunkThreads, kBytes, stream>>>(plan);
   }
   return cudaGetLastError();
 }

@@ -42,10 +42,14 @@ struct ChunkPlan {
   int min_rows;                // sequences with more rows than this are taken here
   int tiles;                   // that `pairs` and `heads` have room for
   int store;                   // whether the states are written
+  int segments;                // that a sequence's chunks are cut into
+  float* borders;              // [sequences, v_heads, kMaxBorders, 128, 128]: see linear_chunk.cu
   uint8_t* pairs;              // [tiles, k_heads, kChunkPairBytes]
   uint8_t* heads;              // [tiles, v_heads, kChunkHeadBytes]
   unsigned long long wait_limit_ns;
 };
+
+constexpr int kMaxSegments = 8, kMaxBorders = 3 * kMaxSegments;
 
 // Chunks of a sequence: of its active rows, if it is taken here.
 __device__ __forceinline__ int chunks_of(const LinearSequence& s, int min_rows) {

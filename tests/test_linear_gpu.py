@@ -20,6 +20,8 @@ BATCHES = {
     "edges": ([15, 16, 17, 31, 32, 33], [1, 0, 2, 3, 0, 9]),
     "chunk_edges": ([63, 64, 65, 1, 129, 2], [7, 0, 1, 0, 3, 9]),
     "prompt": ([300], [0]),
+    "long": ([1000], [7]),
+    "long_and_short": ([650, 33, 700, 1], [0, 64, 3, 5]),
     "mixed": ([1, 130, 1, 1, 67, 3, 1], [9, 0, 0, 5, 11, 2, 800]),
 }
 
@@ -111,7 +113,7 @@ def test_delta_rule(package, name, gated):
 
 
 @pytest.mark.parametrize("heads", [(1, 1), (1, 5), (3, 3), (16, 32)])
-@pytest.mark.parametrize("rows", [[1], [4, 2], [70, 9]])
+@pytest.mark.parametrize("rows", [[1], [4, 2], [70, 9], [900]])
 def test_delta_rule_heads(package, heads, rows):
     p = Problem(package, rows, k_heads=heads[0], v_heads=heads[1], earlier=[3] * len(rows), gated=True, seed=7)
     wanted = p.delta_wanted()
@@ -120,8 +122,8 @@ def test_delta_rule_heads(package, heads, rows):
     check_delta(got, p.states, wanted, most(rows))
 
 
-@pytest.mark.parametrize("rows", [[5, 3, 1, 8], [200, 70, 1, 64]])
-@pytest.mark.parametrize("keep", [[0, 0, 0, 0], [1, 2, 0, 3], [3, 3, 1, 8], [-5, 1000, 1, 4], [5, 64, 1, 63]])
+@pytest.mark.parametrize("rows", [[5, 3, 1, 8], [200, 70, 1, 64], [700, 70, 1, 129]])
+@pytest.mark.parametrize("keep", [[0, 0, 0, 0], [1, 2, 0, 3], [3, 3, 1, 8], [-5, 1000, 1, 4], [5, 64, 1, 63], [641, 70, 0, 128]])
 @pytest.mark.parametrize("outputs", [True, False])
 def test_delta_rule_keeps_what_it_is_told(package, rows, keep, outputs):
     p = Problem(package, rows, earlier=[100, 0, 4, 1], keep=keep, gated=True)
@@ -142,7 +144,7 @@ def test_delta_rule_without_lengths_and_offsets(package):
     check_delta(p.delta(), p.states, wanted, 6)
 
 
-@pytest.mark.parametrize("rows,short", [([4, 20, 4, 3], {2: 2, 3: 0}), ([4, 200, 100, 70], {2: 50, 3: 0}), ([4, 200, 130, 70], {2: 65, 3: 5})])
+@pytest.mark.parametrize("rows,short", [([4, 20, 4, 3], {2: 2, 3: 0}), ([4, 200, 100, 70], {2: 50, 3: 0}), ([4, 200, 130, 70], {2: 65, 3: 5}), ([4, 700, 650, 640], {2: 600, 3: 0})])
 def test_delta_rule_of_a_padded_batch(package, rows, short):
     p = Problem(package, rows, earlier=[9, 3, 0, 0], slots=[-1, 2, 0, 5], behind=3, short=short)
     wanted = p.delta_wanted()
@@ -211,7 +213,7 @@ def test_delta_rule_of_extreme_gates(package, rows):
     check_delta(got, p.states, wanted, most(rows), typical=False)
 
 
-@pytest.mark.parametrize("rows", [[30, 30], [150, 130]])
+@pytest.mark.parametrize("rows", [[30, 30], [150, 130], [600, 520]])
 @pytest.mark.parametrize("what", ["v", "k", "q", "a", "b", "inf", "state"])
 def test_a_nan_reaches_what_depends_on_it_alone(package, rows, what):
     p = Problem(package, rows, earlier=[3, 3], seed=9)
@@ -356,9 +358,9 @@ def test_two_handles_on_two_streams(package, rows):
         check_delta(out, p.states, want, most(rows))
 
 
-@pytest.mark.parametrize("rows", [[3, 5], [200, 333]])
+@pytest.mark.parametrize("rows", [[3, 5], [200, 333], [1500]])
 def test_a_call_gives_the_same_bits_every_time(package, rows):
-    p = Problem(package, rows, earlier=[2, 0], gated=True, k_heads=4, v_heads=8)
+    p = Problem(package, rows, earlier=[2, 0][:len(rows)], gated=True, k_heads=4, v_heads=8)
     before = p.states.clone()
     results = []
     for _ in range(3):
