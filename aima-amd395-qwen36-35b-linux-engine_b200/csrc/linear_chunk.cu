@@ -47,6 +47,7 @@ struct __align__(1024) ChunkMemory {
   float scale[2][kLinearDim];             // the power of two of a column, by parity of the chunk
   int broken[2][kLinearDim];              // the first token of the chunk whose right side is not finite
   float read[2][kChunk];                  // of ChunkNumbers, for when its stage is gone
+  float weight[kLinearDim];               // a quarter of the norm's
   int sums[kChunkThreads / 32];
   unsigned long long full[kStages], empty[kStages], values_full[kStages];
   unsigned long long state_ready[2], dots_full, enter_ready[kTokenSteps], fresh_full, stay_ready[kTokenSteps], state_full, fresh_ready, out_full, out_taken;
@@ -216,14 +217,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
 #pragma unroll
           for (int i = 0; i < kRows; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
         float weight[8];
-        unpack8(*reinterpret_cast<const uint4*>(a.norm_weight + 8 * piece), weight);
+        *reinterpret_cast<float4*>(weight) = *reinterpret_cast<const float4*>(&m.weight[8 * piece]);
+        *reinterpret_cast<float4*>(weight + 4) = *reinterpret_cast<const float4*>(&m.weight[8 * piece + 4]);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
           const float factor = rsqrtf(fmaf(sum[i], 1.0f / kLinearDim, a.eps));
           float z[8];
           unpack8(gates[kRows * which + i], z);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o[i][j] *= factor * weight[j] * linear_silu(z[j]);
+          for (int j = 0; j < 8; ++j) o[i][j] *= (factor * weight[j]) * (z[j] * linear_four_sigmoid(z[j]));
         }
       }
 #pragma unroll
@@ -258,6 +260,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
         largest = max3_abs(largest, x, y);
       }
       m.largest[group][column] = largest;
+      if (gated && group == 0) m.weight[column] = 0.25f * __bfloat162float(a.norm_weight[column]);
       if (kMode == kTransfer && segment == 0 && n > 0) {
         float* const first = border(plan, blockIdx.y, head, 0) + part;
 #pragma unroll
@@ -649,27 +652,38 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
 
 // The states before the segments from the first pass: S_(j + 1) = M_j S_j + B_j, a block per head and 16 columns.
 constexpr int kJoinThreads = 256, kJoinColumns = 16;
+struct JoinMemory {
+  float transfer[kLinearDim][kLinearDim];
+  float before[kLinearDim][kJoinColumns];
+};
 __global__ void __launch_bounds__(kJoinThreads) linear_join_kernel(const ChunkPlan plan) {
-  __shared__ float before[kLinearDim][kJoinColumns];
+  extern __shared__ uint8_t raw[];
+  JoinMemory& m = *reinterpret_cast<JoinMemory*>(raw);
   const int head = blockIdx.x, sequence = blockIdx.y, column = threadIdx.x % kJoinColumns, first = threadIdx.x / kJoinColumns;
   const LinearSequence seq = linear_sequence(plan.a.batch, sequence);
   const int chunks = chunks_of(seq, plan.min_rows), per_segment = (chunks + plan.segments - 1) / plan.segments;
   const int at = static_cast<int>(blockIdx.z) * kJoinColumns + column;
   for (int j = 1; j + 1 < plan.segments && (j + 1) * per_segment < chunks; ++j) {
+    const float4* transfer = reinterpret_cast<const float4*>(border(plan, sequence, head, border_m(j)));
     const float* from = border(plan, sequence, head, j);
-    for (int r = first; r < kLinearDim; r += kJoinThreads / kJoinColumns) before[r][column] = from[r * kLinearDim + at];
-    __syncthreads();
-    const float* transfer = border(plan, sequence, head, border_m(j));
     float sum[8];                          // rows first + 16 i
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] = border(plan, sequence, head, border_b(j))[(first + 16 * i) * kLinearDim + at];
+    for (int i = 0; i < 8; ++i) {
+      sum[i] = border(plan, sequence, head, border_b(j))[(first + 16 * i) * kLinearDim + at];
+      m.before[first + 16 * i][column] = from[(first + 16 * i) * kLinearDim + at];
+    }
+#pragma unroll
+    for (int i = 0; i < kLinearDim * kLinearDim / 4 / kJoinThreads; ++i)
+      reinterpret_cast<float4*>(m.transfer)[i * kJoinThreads + threadIdx.x] = transfer[i * kJoinThreads + threadIdx.x];
+    __syncthreads();
+#pragma unroll 4
     for (int k = 0; k < kLinearDim; k += 4) {
       float x[4];
 #pragma unroll
-      for (int l = 0; l < 4; ++l) x[l] = before[k + l][column];
+      for (int l = 0; l < 4; ++l) x[l] = m.before[k + l][column];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float4 y = *reinterpret_cast<const float4*>(&transfer[(first + 16 * i) * kLinearDim + k]);
+        const float4 y = *reinterpret_cast<const float4*>(&m.transfer[first + 16 * i][k]);
         sum[i] = fmaf(y.x, x[0], sum[i]);
         sum[i] = fmaf(y.y, x[1], sum[i]);
         sum[i] = fmaf(y.z, x[2], sum[i]);
@@ -721,6 +735,7 @@ cudaError_t linear_chunks(const LinearDelta& a, int min_rows, void* workspace, i
   if (error == cudaSuccess) error = opt_in_dynamic_smem<linear_chunk_kernel<kOutput>>(kBytes);
   if (error == cudaSuccess) error = opt_in_dynamic_smem<linear_chunk_kernel<kKept>>(kBytes);
   if (error == cudaSuccess) error = opt_in_dynamic_smem<linear_chunk_kernel<kTransfer>>(kBytes);
+  if (error == cudaSuccess) error = opt_in_dynamic_smem<linear_join_kernel>(sizeof(JoinMemory));
   if (error != cudaSuccess) return error;
   const auto grid = [&](int parts) { return dim3(a.v_heads, a.batch.sequences, parts); };
   // with rows that are computed but do not stay, once for the outputs and once for the states
@@ -728,7 +743,7 @@ cudaError_t linear_chunks(const LinearDelta& a, int min_rows, void* workspace, i
     plan.store = a.batch.keep == nullptr;
     plan.segments = segments;
     if (segments > 1) linear_chunk_kernel<kTransfer><<<grid(2 * segments - 3), kChunkThreads, kBytes, stream>>>(plan);
-    if (segments > 2) linear_join_kernel<<<grid(kLinearDim / kJoinColumns), kJoinThreads, 0, stream>>>(plan);
+    if (segments > 2) linear_join_kernel<<<grid(kLinearDim / kJoinColumns), kJoinThreads, sizeof(JoinMemory), stream>>>(plan);
     linear_chunk_kernel<kOutput><<<grid(segments), kChunkThreads, kBytes, stream>>>(plan);
   }
   if (a.out == nullptr || a.batch.keep != nullptr) {

@@ -14,7 +14,7 @@
 namespace aima {
 namespace {
 
-constexpr int kRowWarps = 8, kGateWarps = 2;
+constexpr int kRowWarps = 6, kGateWarps = 2;
 constexpr int kPrepareThreads = 32 * (kRowWarps + kGateWarps);
 constexpr int kHeadsAtOnce = kGateWarps;        // whose gates are taken together
 constexpr int kHalfRow = kChunk + 8;            // of a 16-bit matrix in shared memory
@@ -36,8 +36,9 @@ struct __align__(1024) PrepareMemory {
   int broken[2 * kChunk];                       // rows that are not finite
   float sum_high[kHeadsAtOnce][kChunk], sum_low[kHeadsAtOnce][kChunk];         // log2(e) G
   float rate[kHeadsAtOnce][kChunk];             // beta, 0 for a token whose gates are not numbers
-  float down[kHeadsAtOnce][kChunk];             // from a block's first token to a token of it
-  float across[kHeadsAtOnce][4][kChunk];        // from a token to the first one of a later block
+  float down[kHeadsAtOnce][kChunk];             // decay from a block's first token to a token of it
+  float across[kHeadsAtOnce][4][kChunk];        // from a token to the first one of its own block or a later one, over |k|; 0 for earlier ones
+  int steep[kHeadsAtOnce][4];                   // a block whose own decays are too small for that
   int found[2];
   int sums[kPrepareThreads / 32];
   unsigned long long done;
@@ -85,23 +86,17 @@ __device__ __forceinline__ void as_operand(const float (*d)[4], float sign, uint
   }
 }
 
-// A lower triangle in two terms to where the second kernel takes it from, by 256 threads; zeros in the blocks above it.
-template <int kTerms>
-__device__ __forceinline__ void write_terms(const Terms& from, uint8_t* to, int thread) {
-  const int piece = thread & 7, row = thread >> 3;
-#pragma unroll
-  for (int term = 0; term < kTerms; ++term) {
-#pragma unroll
-    for (int r = row; r < kChunk; r += 32)
-      *reinterpret_cast<uint4*>(to + term * kChunkMatrixBytes + swizzled(r, piece)) =
-          piece / 2 <= r / 16 ? *reinterpret_cast<const uint4*>(&from.of[term][r * kHalfRow + 8 * piece]) : make_uint4(0, 0, 0, 0);
+// A lower triangle in two terms to where the second kernel takes it from, by some of the threads; zeros in the blocks above it.
+__device__ __forceinline__ void write_terms(const Terms& from, uint8_t* to, int thread, int threads) {
+#pragma unroll 4
+  for (int i = thread; i < 2 * kChunk * 8; i += threads) {
+    const int piece = i & 7, r = (i >> 3) & (kChunk - 1), term = i >> 9;
+    *reinterpret_cast<uint4*>(to + term * kChunkMatrixBytes + swizzled(r, piece)) =
+        piece / 2 <= r / 16 ? *reinterpret_cast<const uint4*>(&from.of[term][r * kHalfRow + 8 * piece]) : make_uint4(0, 0, 0, 0);
   }
 }
-__device__ __forceinline__ void row_barrier() {
-  tc_fence_before();
-  asm volatile("bar.sync 1, %0;" :: "n"(32 * kRowWarps) : "memory");
-  tc_fence_after();
-}
+// where the gates wait for the lengths of k
+__device__ __forceinline__ void lengths_barrier() { asm volatile("bar.sync 1, %0;" :: "n"(kPrepareThreads) : "memory"); }
 
 __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(const ChunkPlan plan) {
   extern __shared__ uint8_t raw[];
@@ -160,7 +155,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
   const int kept = min(max(seq.kept - begin, 0), rows);
   const long long row0 = seq.row0 + begin;
   bool alive = true;
-  const int half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane, token = row & (kChunk - 1), block = token >> 4;
+  const int half = warp >> 2, row = (warp & 3) * 32 + lane, token = row & (kChunk - 1), block = token >> 4;
   for (int base = 0; there_is && base < a.group; base += kHeadsAtOnce) {
     const int heads = min(kHeadsAtOnce, a.group - base);
     double total[2] = {0.0, 0.0}, last = 0.0;
@@ -211,26 +206,41 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
           m.sum_low[h][t] = static_cast<float>(total[i] - high);
           m.rate[h][t] = beta[i];
           m.down[h][t] = fast_exp2(static_cast<float>(total[i] - mine));
-#pragma unroll
-          for (int b = 1; b < 4; ++b) m.across[h][b][t] = t < 16 * b ? fast_exp2(static_cast<float>(first[b] - total[i])) : 0.0f;
         }
+        // with the lengths of k, which the other warps find meanwhile
+        if (base == 0) lengths_barrier();
+        const double end[4] = {first[1], first[2], first[3], last};            // a token too far: no matter
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const bool steep = first[b] - end[b] > 64.0;
+          if (lane == 0) m.steep[h][b] = steep;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int t = 2 * lane + i;
+            m.across[h][b][t] = t < 16 * b + (steep ? 0 : 16) ? fast_exp2(static_cast<float>(first[b] - total[i])) * m.length[t] : 0.0f;
+          }
+        }
+      } else if (base == 0) {
+        lengths_barrier();
       }
     } else if (base == 0) {
-      // k's rows, then q's: four lanes a row, two rows a thread
+      // k's rows, then q's: four lanes a row, eight rows a warp at a time
       uint8_t* const pair = plan.pairs + (static_cast<size_t>(tile) * a.k_heads + k_head) * kChunkPairBytes;
-      uint4 data[2][4];
+      constexpr int kParts = 2 * kChunk / 8, kPasses = (kParts + kRowWarps - 1) / kRowWarps;
+      uint4 data[kPasses][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int t = 8 * warp + (lane >> 2);
-        const KvRows& from = i == 0 ? a.k : a.q;
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = 8 * (warp + i * kRowWarps) + (lane >> 2), t = r & (kChunk - 1);
+        const KvRows& from = r < kChunk ? a.k : a.q;
+        const __nv_bfloat16* at = from.data + (row0 + t) * from.row_stride + k_head * from.head_stride + 8 * (lane & 3);
 #pragma unroll
         for (int p = 0; p < 4; ++p)
-          data[i][p] = t < rows ? *reinterpret_cast<const uint4*>(from.data + (row0 + t) * from.row_stride + k_head * from.head_stride + 8 * (4 * p + (lane & 3)))
-                                : make_uint4(0, 0, 0, 0);
+          data[i][p] = t < rows && r < 2 * kChunk ? *reinterpret_cast<const uint4*>(at + 32 * p) : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = i * kChunk + 8 * warp + (lane >> 2);
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = 8 * (warp + i * kRowWarps) + (lane >> 2);
+        if (8 * (warp + i * kRowWarps) >= 2 * kChunk) break;
         uint32_t most = 0;
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
@@ -272,7 +282,8 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
         }
       }
       fence_async_proxy();
-      row_barrier();
+      asm volatile("bar.arrive 1, %0;" :: "n"(kPrepareThreads) : "memory");       // the lengths are there, for the gates
+      asm volatile("bar.sync 2, %0;" :: "n"(32 * kRowWarps) : "memory");
       if (warp == 0) {
         if (elect_one()) {
           constexpr uint32_t kForm = instr_desc_f8(kF16, kF16, 0, 0, 128, kChunk);
@@ -286,6 +297,8 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
         }
         __syncwarp();
       }
+    }
+    if (base == 0) {
       alive = mbar_wait_bounded_warp(smem_u32(&m.done), 0, &m.abort_flag, plan.wait_limit_ns);
       tc_fence_after();
     }
@@ -315,39 +328,47 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
 #pragma unroll 1
     for (int h = 0; h < heads; ++h) {
       uint8_t* const out = plan.heads + (static_cast<size_t>(tile) * a.v_heads + k_head * a.group + base + h) * kChunkHeadBytes;
-      if (warp < kRowWarps) {
-        // A, and the scores: a row of [k; q] and 32 columns a thread
-        const bool is_k = row < kChunk;
-        Terms& to = is_k ? m.overlap : m.scores;
-        const float own = (is_k ? m.rate[h][token] : 1.0f) * m.length[row], down = own * m.down[h][token];
-        const float high = m.sum_high[h][token], low = m.sum_low[h][token];
+      {
+        // A, and the scores: a row of [k; q] and 32 columns a thread.  Columns behind the diagonal's block are not looked at again.
+        const int beside = (warp & 1) - half;                        // rows of the two blocks that the columns are of: 0, behind them: 1
+        if (beside >= 0) {
+          const bool is_k = row < kChunk;
+          Terms& to = is_k ? m.overlap : m.scores;
+          const float own = (is_k ? m.rate[h][token] : 1.0f) * m.length[row], down = own * m.down[h][token];
+          const int last_column = is_k ? token - 1 : token;
+          const bool steep = m.steep[h][block] != 0;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {                                // 16 columns
-          const int column = 32 * half + 16 * q;
-          float x[16];
-          tmem_ld16(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + column, reinterpret_cast<uint32_t*>(x));
-          tmem_ld_wait();
-          if (column >> 4 < block) {
+          for (int q = 0; q < 2; ++q) {                              // 16 columns
+            const int column = 32 * half + 16 * q;
+            float x[16];
+            tmem_ld16(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + column, reinterpret_cast<uint32_t*>(x));
+            tmem_ld_wait();
+            if (beside == 0 && steep && column >> 4 == block) {
+              const float high = m.sum_high[h][token], low = m.sum_low[h][token];
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const float4 y = *reinterpret_cast<const float4*>(&m.across[h][block][column + j]), z = *reinterpret_cast<const float4*>(&m.length[column + j]);
-              x[j] *= down * (y.x * z.x);
-              x[j + 1] *= down * (y.y * z.y);
-              x[j + 2] *= down * (y.z * z.z);
-              x[j + 3] *= down * (y.w * z.w);
+              for (int j = 0; j < 16; ++j) {
+                const float apart = fminf((high - m.sum_high[h][column + j]) + (low - m.sum_low[h][column + j]), 0.0f);
+                x[j] *= own * m.length[column + j] * fast_exp2(apart);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(&m.across[h][block][column + j]);
+                x[j] *= down * y.x;
+                x[j + 1] *= down * y.y;
+                x[j + 2] *= down * y.z;
+                x[j + 3] *= down * y.w;
+              }
             }
-          } else if (column >> 4 == block) {
+            if (beside == 0) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float apart = (high - m.sum_high[h][column + j]) + (low - m.sum_low[h][column + j]);
-              x[j] = (is_k ? column + j < token : column + j <= token) ? x[j] * (own * m.length[column + j] * fast_exp2(apart)) : 0.0f;
-            }
-            if (is_k) {
+              for (int j = 0; j < 16; ++j) x[j] = column + j <= last_column ? x[j] : 0.0f;
+              if (is_k && column >> 4 == block) {
 #pragma unroll
-              for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(&m.diagonal[block][(token & 15) * kBlockRow + j]) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                for (int j = 0; j < 16; j += 4)
+                  *reinterpret_cast<float4*>(&m.diagonal[block][(token & 15) * kBlockRow + j]) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+              }
             }
-          }
-          if (column >> 4 < block + !is_k) {
 #pragma unroll
             for (int j = 0; j < 16; j += 8) {
               uint32_t hi[4], lo[4];
@@ -386,7 +407,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
           second[kHalfRow] = static_cast<uint16_t>(lo >> 16);
         }
       } else {
-        write_terms<2>(m.scores, out + 2 * kChunkMatrixBytes, threadIdx.x - 64);
+        write_terms(m.scores, out + 2 * kChunkMatrixBytes, threadIdx.x - 64, kPrepareThreads - 64);
       }
       __syncthreads();
       // the blocks below the diagonal's, a column of them a warp
@@ -413,7 +434,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
         }
       }
       __syncthreads();
-      if (warp >= 2) write_terms<2>(m.inverse, out, threadIdx.x - 64);
+      write_terms(m.inverse, out, threadIdx.x, kPrepareThreads);
     }
     __syncthreads();
   }
