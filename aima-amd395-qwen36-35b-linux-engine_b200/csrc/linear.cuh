@@ -147,7 +147,7 @@ struct LinearDelta {
 };
 constexpr int kLinearStepRows = 32;   // rows of a sequence up to which it is taken token by token, if others of the batch are longer
 // Sequences of at most max_rows rows.
-cudaError_t linear_step(const LinearDelta& args, int max_rows, cudaStream_t stream);
+cudaError_t linear_step(const LinearDelta& args, int max_rows, int sm_count, cudaStream_t stream);
 size_t linear_chunk_workspace(int k_heads, int v_heads, int max_tokens, int max_sequences);
 // Sequences of more than min_rows rows.
 cudaError_t linear_chunks(const LinearDelta& args, int min_rows, void* workspace, int sm_count, cudaStream_t stream);

@@ -281,7 +281,7 @@ AIMA_EXPORT int aima_moe_linear_delta_launch(aima_moe_linear* h, uint32_t layer,
   // Sequences of few rows go token by token, longer ones in chunks; a batch that may have both takes both launches.
   cudaError_t error = cudaSuccess;
   const bool chunks = a.batch.max_new > aima::kLinearStepRows, steps = !chunks || (a.batch.sequences > 1 && a.batch.offsets != nullptr);
-  if (steps) error = aima::linear_step(a, chunks ? aima::kLinearStepRows : a.batch.max_new, static_cast<cudaStream_t>(stream));
+  if (steps) error = aima::linear_step(a, chunks ? aima::kLinearStepRows : a.batch.max_new, h->sm_count, static_cast<cudaStream_t>(stream));
   if (error == cudaSuccess && chunks)
     error = aima::linear_chunks(a, steps ? aima::kLinearStepRows : 0, reinterpret_cast<uint8_t*>(h->status) + 256, h->sm_count, static_cast<cudaStream_t>(stream));
   if (error != cudaSuccess) return fail_cuda(error, "linear delta launch");
