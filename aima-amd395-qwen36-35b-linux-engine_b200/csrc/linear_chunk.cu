@@ -55,6 +55,8 @@ struct __align__(1024) ChunkMemory {
   int abort_flag;
 };
 
+// The launches of a call may begin before the one before them has ended: each waits here for its results, on every way out.
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void chain_barrier() { asm volatile("bar.sync 1, %0;" :: "n"(32 * kChainWarps) : "memory"); }
 // mbar_wait_bounded_warp without a call: the numbers that are alive across one would go to memory.
 __device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned long long limit_ns) {
@@ -82,6 +84,19 @@ __device__ __forceinline__ float* border(const ChunkPlan& plan, int sequence, in
 __device__ __forceinline__ int border_b(int segment) { return kMaxSegments + 2 * segment; }
 __device__ __forceinline__ int border_m(int segment) { return kMaxSegments + 2 * segment + 1; }
 
+// Where the segments of `chunks` chunks begin: all are as long, but for the first, which has plan.first eighths of the others' length.
+struct Segments {
+  int first, per;
+  __host__ __device__ Segments(const ChunkPlan& plan, int chunks) : Segments(plan.segments, plan.first, chunks) {}
+  __host__ __device__ Segments(int segments, int eighths, int chunks) {
+    const int parts = 8 * (segments - 1) + eighths;
+    per = (8 * chunks + parts - 1) / parts;
+    const int left = chunks - (segments - 1) * per;
+    first = left > 1 ? left : 1;
+  }
+  __host__ __device__ int begin(int segment) const { return segment == 0 ? 0 : first + (segment - 1) * per; }
+};
+
 // kOutput: all rows of a segment, the state behind the last if plan.store says so.  kKept: the states alone, for the rows that enter them.
 // kTransfer: the first pass over segments.
 enum ChunkMode { kOutput, kKept, kTransfer };
@@ -93,11 +108,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   const LinearDelta& a = plan.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.x;
+  launch_may_follow();
   const LinearSequence seq = linear_sequence(a.batch, blockIdx.y);
-  if (seq.rows <= plan.min_rows) return;
+  if (seq.rows <= plan.min_rows) {
+    wait_for_launch_before();
+    return;
+  }
   // segment, and for the first pass whether its M is wanted
-  const int segment = kMode == kTransfer ? (static_cast<int>(blockIdx.z) + 1) / 2 : static_cast<int>(blockIdx.z);
-  const bool transfer = kMode == kTransfer && segment > 0 && blockIdx.z % 2 == 0;
+  const int job = static_cast<int>(gridDim.z - 1 - blockIdx.z);            // the first segment, which may be shorter, is begun last
+  const int segment = kMode == kTransfer ? (job + 1) / 2 : job;
+  const bool transfer = kMode == kTransfer && segment > 0 && job % 2 == 0;
   if (kOutputs && segment == 0) {                     // rows that are not active
     for (int i = threadIdx.x; i < seq.first * (kLinearDim / 8); i += kChunkThreads)
       *reinterpret_cast<uint4*>(a.out + (static_cast<long long>(seq.row0 + i / (kLinearDim / 8)) * a.v_heads + head) * kLinearDim + 8 * (i % (kLinearDim / 8))) =
@@ -105,9 +125,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   }
   const int limit = kMode == kKept ? seq.kept : seq.rows;                  // rows that are gone through
   const int all_chunks = (limit - seq.first + kChunk - 1) / kChunk;
-  const int per_segment = (all_chunks + plan.segments - 1) / plan.segments, chunk0 = segment * per_segment;
-  const int chunks = min(per_segment, all_chunks - chunk0);
-  if (limit <= seq.first || chunks <= 0) return;
+  const Segments cut(plan, all_chunks);
+  const int chunk0 = cut.begin(segment), chunks = min(cut.begin(segment + 1), all_chunks) - chunk0;
+  if (limit <= seq.first || chunks <= 0) {
+    wait_for_launch_before();
+    return;
+  }
 
   // its first tile
   int tile0 = 0;
@@ -142,6 +165,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   __syncthreads();
   tc_fence_after();
   for (int w = 0; w < kChunkThreads / 32; ++w) tile0 += m.sums[w];
+  wait_for_launch_before();
   constexpr uint32_t tmem = 0;               // all 512 columns begin at 0
   const bool fits = tile0 + chunks_of(seq, plan.min_rows) <= plan.tiles;       // not if sequences overlap, which the first kernel reports
   const int n = fits ? chunks : 0;
@@ -650,50 +674,75 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   if (warp == kChainWarps) tmem_dealloc(tmem, 512);
 }
 
-// The states before the segments from the first pass: S_(j + 1) = M_j S_j + B_j, a block per head and 16 columns.
-constexpr int kJoinThreads = 256, kJoinColumns = 16;
-struct JoinMemory {
-  float transfer[kLinearDim][kLinearDim];
+// The states before the segments from the first pass: S_(j + 1) = M_j S_j + B_j, a block per head and 32 columns, 4 x 4 elements a
+// thread.  The next M is on its way meanwhile.
+constexpr int kJoinThreads = 256, kJoinColumns = 32, kJoinRow = kLinearDim + 4;
+struct __align__(16) JoinMemory {
+  float transfer[2][kLinearDim * kJoinRow];
   float before[kLinearDim][kJoinColumns];
 };
-__global__ void __launch_bounds__(kJoinThreads) linear_join_kernel(const ChunkPlan plan) {
+__global__ void __launch_bounds__(kJoinThreads, 1) linear_join_kernel(const ChunkPlan plan) {
   extern __shared__ uint8_t raw[];
   JoinMemory& m = *reinterpret_cast<JoinMemory*>(raw);
-  const int head = blockIdx.x, sequence = blockIdx.y, column = threadIdx.x % kJoinColumns, first = threadIdx.x / kJoinColumns;
+  const int head = blockIdx.x, sequence = blockIdx.y, begin = static_cast<int>(blockIdx.z) * kJoinColumns;
+  const int column = 4 * (threadIdx.x & 7), first = threadIdx.x >> 3;        // rows first + 32 i
   const LinearSequence seq = linear_sequence(plan.a.batch, sequence);
-  const int chunks = chunks_of(seq, plan.min_rows), per_segment = (chunks + plan.segments - 1) / plan.segments;
-  const int at = static_cast<int>(blockIdx.z) * kJoinColumns + column;
-  for (int j = 1; j + 1 < plan.segments && (j + 1) * per_segment < chunks; ++j) {
-    const float4* transfer = reinterpret_cast<const float4*>(border(plan, sequence, head, border_m(j)));
-    const float* from = border(plan, sequence, head, j);
-    float sum[8];                          // rows first + 16 i
+  const int chunks = chunks_of(seq, plan.min_rows);
+  const Segments cut(plan, chunks);
+  launch_may_follow();
+  wait_for_launch_before();
+  const auto there = [&](int j) { return j + 1 < plan.segments && cut.begin(j + 1) < chunks; };
+  const auto fetch = [&](int j) {
+    const float* from = border(plan, sequence, head, border_m(j));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sum[i] = border(plan, sequence, head, border_b(j))[(first + 16 * i) * kLinearDim + at];
-      m.before[first + 16 * i][column] = from[(first + 16 * i) * kLinearDim + at];
+    for (int i = 0; i < kLinearDim * kLinearDim / 4 / kJoinThreads; ++i) {
+      const int at = i * kJoinThreads + static_cast<int>(threadIdx.x), row = at / (kLinearDim / 4), piece = at % (kLinearDim / 4);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(&m.transfer[j & 1][row * kJoinRow + 4 * piece])), "l"(from + 4 * at) : "memory");
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (!there(1)) return;
+  fetch(1);
+  {
+    const float* from = border(plan, sequence, head, 1) + begin;
 #pragma unroll
-    for (int i = 0; i < kLinearDim * kLinearDim / 4 / kJoinThreads; ++i)
-      reinterpret_cast<float4*>(m.transfer)[i * kJoinThreads + threadIdx.x] = transfer[i * kJoinThreads + threadIdx.x];
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<float4*>(&m.before[first + 32 * i][column]) = *reinterpret_cast<const float4*>(from + (first + 32 * i) * kLinearDim + column);
+  }
+  for (int j = 1; there(j); ++j) {
+    float4 sum[4];
+    const float* add = border(plan, sequence, head, border_b(j)) + begin;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = *reinterpret_cast<const float4*>(add + (first + 32 * i) * kLinearDim + column);
+    if (there(j + 1)) fetch(j + 1);
+    if (there(j + 1)) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
 #pragma unroll 4
     for (int k = 0; k < kLinearDim; k += 4) {
-      float x[4];
+      float4 x[4];
 #pragma unroll
-      for (int l = 0; l < 4; ++l) x[l] = m.before[k + l][column];
+      for (int l = 0; l < 4; ++l) x[l] = *reinterpret_cast<const float4*>(&m.before[k + l][column]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 y = *reinterpret_cast<const float4*>(&m.transfer[first + 16 * i][k]);
-        sum[i] = fmaf(y.x, x[0], sum[i]);
-        sum[i] = fmaf(y.y, x[1], sum[i]);
-        sum[i] = fmaf(y.z, x[2], sum[i]);
-        sum[i] = fmaf(y.w, x[3], sum[i]);
+      for (int i = 0; i < 4; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(&m.transfer[j & 1][(first + 32 * i) * kJoinRow + k]);
+#pragma unroll
+        for (int l = 0; l < 4; ++l) {
+          const float z = (&y.x)[l];
+          sum[i].x = fmaf(z, x[l].x, sum[i].x);
+          sum[i].y = fmaf(z, x[l].y, sum[i].y);
+          sum[i].z = fmaf(z, x[l].z, sum[i].z);
+          sum[i].w = fmaf(z, x[l].w, sum[i].w);
+        }
       }
     }
-    float* to = border(plan, sequence, head, j + 1);
+    __syncthreads();                       // the states are read; what M lay in is free for the one after the next
+    float* to = border(plan, sequence, head, j + 1) + begin;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) to[(first + 16 * i) * kLinearDim + at] = sum[i];
-    __syncthreads();                       // a block reads the columns that it wrote
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<float4*>(to + (first + 32 * i) * kLinearDim + column) = sum[i];
+      *reinterpret_cast<float4*>(&m.before[first + 32 * i][column]) = sum[i];
+    }
   }
 }
 
@@ -701,12 +750,33 @@ size_t tiles_of(int tokens, int sequences, int min_rows) {
   return static_cast<size_t>(tokens / kChunk) + std::min(sequences, tokens / (min_rows + 1));
 }
 
-// Segments that a sequence's chunks are cut into: as many as find room for all heads in both passes, if they are worth the launches.
-int segments_of(int heads, int chunks, int sm_count) {
-  int segments = 1;
-  for (int g = 2; g <= kMaxSegments; ++g)
-    if (heads * g <= sm_count && heads * (2 * g - 3) <= sm_count && chunks >= 2 * g) segments = g;
-  return segments;
+// Into how many segments a sequence's chunks are cut, and the eighths that the first has: what the two passes are estimated to take
+// least with.  A chunk counts 5 in the second pass and 3 in the first; the first pass and what follows it count as 4 chunks more.
+struct Cut {
+  int segments, first;
+};
+// Jobs of two lengths on `places` multiprocessors, the long ones first; 0: the long ones do not all find room.
+int makespan(int long_jobs, int length, int short_jobs, int short_length, int places) {
+  if (long_jobs > places || (long_jobs == places && short_jobs > 0)) return 0;
+  const int rounds = (short_jobs + places - long_jobs - 1) / std::max(places - long_jobs, 1);
+  return std::max(long_jobs > 0 ? length : 0, rounds * short_length);
+}
+Cut cut_of(int heads, int chunks, int places) {
+  Cut best{1, 8};
+  int least = 5 * chunks;
+  if (2 * heads > places) return best;               // the workspace has no room for borders of more
+  for (int g = 2; g <= kMaxSegments && g <= chunks; ++g) {
+    for (const int eighths : {8, 4, 3, 2}) {
+      const Segments cut(g, eighths, chunks);
+      const int one = makespan(2 * (g - 2) * heads, cut.per, heads, cut.first, places);
+      const int two = makespan((g - 1) * heads, cut.per, heads, cut.first, places);
+      if (one > 0 && two > 0 && 3 * one + 5 * two + 20 < least) {
+        least = 3 * one + 5 * two + 20;
+        best = Cut{g, eighths};
+      }
+    }
+  }
+  return best;
 }
 constexpr int kMultiprocessors = 148;      // that the workspace reckons with
 size_t border_bytes(int heads) { return static_cast<size_t>(heads) * kMaxBorders * kLinearDim * kLinearDim * sizeof(float); }
@@ -725,9 +795,10 @@ cudaError_t linear_chunks(const LinearDelta& a, int min_rows, void* workspace, i
   plan.a = a;
   plan.min_rows = min_rows;
   plan.tiles = static_cast<int>(tiles_of(a.batch.tokens, a.batch.sequences, min_rows));
-  const int heads = a.v_heads * a.batch.sequences, segments = segments_of(heads, a.batch.max_new / kChunk, std::min(sm_count, kMultiprocessors));
+  const int heads = a.v_heads * a.batch.sequences;
+  const Cut cut = cut_of(heads, (a.batch.max_new + kChunk - 1) / kChunk, std::min(sm_count, kMultiprocessors));
   plan.borders = static_cast<float*>(workspace);
-  plan.pairs = static_cast<uint8_t*>(workspace) + (segments > 1 ? border_bytes(heads) : 0);
+  plan.pairs = static_cast<uint8_t*>(workspace) + (cut.segments > 1 ? border_bytes(heads) : 0);
   plan.heads = plan.pairs + static_cast<size_t>(plan.tiles) * a.k_heads * kChunkPairBytes;
   plan.wait_limit_ns = kWaitBudgetNs;
   cudaError_t error = linear_prepare(plan, stream);
@@ -741,16 +812,19 @@ cudaError_t linear_chunks(const LinearDelta& a, int min_rows, void* workspace, i
   // with rows that are computed but do not stay, once for the outputs and once for the states
   if (a.out != nullptr) {
     plan.store = a.batch.keep == nullptr;
-    plan.segments = segments;
-    if (segments > 1) linear_chunk_kernel<kTransfer><<<grid(2 * segments - 3), kChunkThreads, kBytes, stream>>>(plan);
-    if (segments > 2) linear_join_kernel<<<grid(kLinearDim / kJoinColumns), kJoinThreads, sizeof(JoinMemory), stream>>>(plan);
-    linear_chunk_kernel<kOutput><<<grid(segments), kChunkThreads, kBytes, stream>>>(plan);
+    plan.segments = cut.segments;
+    plan.first = cut.first;
+    if (cut.segments > 1) error = launch_pdl(linear_chunk_kernel<kTransfer>, grid(2 * cut.segments - 3), kChunkThreads, kBytes, stream, plan);
+    if (error == cudaSuccess && cut.segments > 2)
+      error = launch_pdl(linear_join_kernel, grid(kLinearDim / kJoinColumns), kJoinThreads, sizeof(JoinMemory), stream, plan);
+    if (error == cudaSuccess) error = launch_pdl(linear_chunk_kernel<kOutput>, grid(cut.segments), kChunkThreads, kBytes, stream, plan);
   }
-  if (a.out == nullptr || a.batch.keep != nullptr) {
+  if (error == cudaSuccess && (a.out == nullptr || a.batch.keep != nullptr)) {
     plan.store = plan.segments = 1;
-    linear_chunk_kernel<kKept><<<grid(1), kChunkThreads, kBytes, stream>>>(plan);
+    plan.first = 8;
+    error = launch_pdl(linear_chunk_kernel<kKept>, grid(1), kChunkThreads, kBytes, stream, plan);
   }
-  return cudaGetLastError();
+  return error;
 }
 
 }  // namespace aima

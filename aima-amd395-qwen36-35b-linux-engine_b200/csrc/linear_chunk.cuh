@@ -42,7 +42,7 @@ struct ChunkPlan {
   int min_rows;                // sequences with more rows than this are taken here
   int tiles;                   // that `pairs` and `heads` have room for
   int store;                   // whether the states are written
-  int segments;                // that a sequence's chunks are cut into
+  int segments, first;         // that a sequence's chunks are cut into, and eighths of the others' length that the first has
   float* borders;              // [sequences, v_heads, kMaxBorders, 128, 128]: see linear_chunk.cu
   uint8_t* pairs;              // [tiles, k_heads, kChunkPairBytes]
   uint8_t* heads;              // [tiles, v_heads, kChunkHeadBytes]
@@ -119,6 +119,7 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
+__device__ __forceinline__ void launch_may_follow() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 cudaError_t linear_prepare(const ChunkPlan& plan, cudaStream_t stream);
 
 }  // namespace aima

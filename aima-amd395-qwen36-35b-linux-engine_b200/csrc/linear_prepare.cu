@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
   const LinearDelta& a = plan.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int k_head = blockIdx.x, tile = blockIdx.y;
+  launch_may_follow();
   if (tile == 0 && k_head == 0) linear_report(a.batch, a.status, threadIdx.x, kPrepareThreads);
 
   // the sequence and chunk of this tile
