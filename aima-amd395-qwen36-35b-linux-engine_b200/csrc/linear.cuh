@@ -145,7 +145,7 @@ struct LinearDelta {
   __nv_bfloat16* out;                 // may be nullptr
   int* status;
 };
-constexpr int kLinearStepRows = 32;   // rows of a sequence up to which it is taken token by token, if others of the batch are longer
+constexpr int kLinearStepRows = 24;   // rows of a sequence up to which it is taken token by token, if others of the batch are longer
 // Sequences of at most max_rows rows.
 cudaError_t linear_step(const LinearDelta& args, int max_rows, int sm_count, cudaStream_t stream);
 size_t linear_chunk_workspace(int k_heads, int v_heads, int max_tokens, int max_sequences);

@@ -507,6 +507,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
     // Products of different shapes need not run in the order of issue: one that reads or writes what another wrote waits for its commit.
     // A step with N = 64 takes 32 cycles, one with 128 takes 64.  What the chain waits for goes first.
     constexpr uint32_t kNarrow = instr_desc_f8(kF16, kF16, 0, 0, 128, kChunk), kUpdate = instr_desc_f8(kF16, kF16, 0, 1, 128, kLinearDim);
+    // T and the scores are triangles: tokens 16 k .. add to what they and those behind them have, and to nothing before
+    const auto below = [](int k) { return instr_desc_f8(kF16, kF16, 0, 0, 128, kChunk - 16 * k); };
     // descriptors: those of a stage's begin, to which constants are added (an address takes their low 14 bits)
     const uint32_t base = smem_u32(m.stages[0]);
     for (int c = 0; c < n; ++c) {
@@ -555,8 +557,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
 #pragma unroll
             for (int term = 0; term < 3; ++term) {                                // both terms by T's first, the first by T's second
               const int k = g * kTokenSteps + step;
-              umma_f16_ts(kDotsAt, kEnterAt + operand(k, term == 1), rows_desc + ((kChunkPairBytes + (term == 2 ? kChunkMatrixBytes : 0) + k * 32) >> 4), kNarrow,
-                          (step | g | term) != 0);
+              umma_f16_ts(kDotsAt + 16 * k, kEnterAt + operand(k, term == 1),
+                          rows_desc + ((kChunkPairBytes + (term == 2 ? kChunkMatrixBytes : 0) + k * (16 * 128 + 32)) >> 4), below(k), (k | term) != 0);
             }
           if (step == kTokenSteps - 1) umma_commit(smem_u32(&m.fresh_full));
         }
@@ -590,8 +592,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
           for (int term = 0; term < 3; ++term)                                    // both terms by the scores' first, the first by their second
 #pragma unroll
             for (int k = 0; k < kChunk / 16; ++k)
-              umma_f16_ts(kEnterAt, kFreshAt + operand(k, term == 1),
-                          rows_desc + ((kChunkPairBytes + (term == 2 ? 3 : 2) * kChunkMatrixBytes + k * 32) >> 4), kNarrow, (term | k) != 0);
+              umma_f16_ts(kEnterAt + 16 * k, kFreshAt + operand(k, term == 1),
+                          rows_desc + ((kChunkPairBytes + (term == 2 ? 3 : 2) * kChunkMatrixBytes + k * (16 * 128 + 32)) >> 4), below(k), (term | k) != 0);
           umma_commit(smem_u32(&m.out_full));
           umma_commit(smem_u32(&m.empty[c % kStages]));
         }
@@ -751,7 +753,7 @@ size_t tiles_of(int tokens, int sequences, int min_rows) {
 }
 
 // Into how many segments a sequence's chunks are cut, and the eighths that the first has: what the two passes are estimated to take
-// least with.  A chunk counts 5 in the second pass and 3 in the first; the first pass and what follows it count as 4 chunks more.
+// least with.  A chunk counts 5 in the second pass and 3 in the first; the launches more count as 28, an eighth of a chunk each or so.
 struct Cut {
   int segments, first;
 };
@@ -770,8 +772,8 @@ Cut cut_of(int heads, int chunks, int places) {
       const Segments cut(g, eighths, chunks);
       const int one = makespan(2 * (g - 2) * heads, cut.per, heads, cut.first, places);
       const int two = makespan((g - 1) * heads, cut.per, heads, cut.first, places);
-      if (one > 0 && two > 0 && 3 * one + 5 * two + 20 < least) {
-        least = 3 * one + 5 * two + 20;
+      if (one > 0 && two > 0 && 3 * one + 5 * two + 28 < least) {
+        least = 3 * one + 5 * two + 28;
         best = Cut{g, eighths};
       }
     }

@@ -86,13 +86,13 @@ __device__ __forceinline__ void as_operand(const float (*d)[4], float sign, uint
   }
 }
 
-// A lower triangle in two terms to where the second kernel takes it from, by some of the threads; zeros in the blocks above it.
+// A lower triangle in two terms to where the second kernel takes it from, by some of the threads; the blocks above it are not read there.
 __device__ __forceinline__ void write_terms(const Terms& from, uint8_t* to, int thread, int threads) {
 #pragma unroll 4
   for (int i = thread; i < 2 * kChunk * 8; i += threads) {
     const int piece = i & 7, r = (i >> 3) & (kChunk - 1), term = i >> 9;
-    *reinterpret_cast<uint4*>(to + term * kChunkMatrixBytes + swizzled(r, piece)) =
-        piece / 2 <= r / 16 ? *reinterpret_cast<const uint4*>(&from.of[term][r * kHalfRow + 8 * piece]) : make_uint4(0, 0, 0, 0);
+    if (piece / 2 <= r / 16)
+      *reinterpret_cast<uint4*>(to + term * kChunkMatrixBytes + swizzled(r, piece)) = *reinterpret_cast<const uint4*>(&from.of[term][r * kHalfRow + 8 * piece]);
   }
 }
 // where the gates wait for the lengths of k
