@@ -118,6 +118,32 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+struct Pair {                  // two FP32 numbers that one instruction takes
+  unsigned long long bits;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ float2 values() const {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(bits));
+    return v;
+  }
+};
+__device__ __forceinline__ Pair operator*(const Pair& a, const Pair& b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
+  return d;
+}
+__device__ __forceinline__ Pair operator+(const Pair& a, const Pair& b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
+  return d;
+}
+__device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return d;
+}
+
 struct LinearConv {
   LinearBatch batch;
   int channels, width;

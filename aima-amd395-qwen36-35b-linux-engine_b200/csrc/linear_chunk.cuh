@@ -85,31 +85,6 @@ __device__ __forceinline__ void split_f16(float x0, float x1, uint32_t* high, ui
       : "=f"(l0), "=f"(l1) : "r"(*high), "f"(x0), "f"(x1));
   *low = cvt_f16x2(l0, l1);
 }
-struct Pair {                  // two FP32 numbers that one instruction takes
-  unsigned long long bits;
-  __device__ __forceinline__ Pair() {}
-  __device__ __forceinline__ Pair(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(x), "f"(y)); }
-  __device__ __forceinline__ float2 values() const {
-    float2 v;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(bits));
-    return v;
-  }
-};
-__device__ __forceinline__ Pair operator*(const Pair& a, const Pair& b) {
-  Pair d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
-  return d;
-}
-__device__ __forceinline__ Pair operator+(const Pair& a, const Pair& b) {
-  Pair d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
-  return d;
-}
-__device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c) {
-  Pair d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
-  return d;
-}
 __device__ __forceinline__ void split_f16(const Pair& x, uint32_t* high, uint32_t* low) {
   const float2 v = x.values();
   split_f16(v.x, v.y, high, low);

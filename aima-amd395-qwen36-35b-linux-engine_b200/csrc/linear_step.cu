@@ -114,20 +114,25 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
   const int part = lane >> 2, column = 16 * warp + 4 * (lane & 3);           // rows 32 i + 4 part + j, columns column .. column + 3
   for (int i = 0; i < units; ++i) {
     const StepMemory::Unit& u = m.units[i];
-    float4 s[4][4];
+    Pair s[4][2][4];                     // of two rows, four columns
     {
       const float* state = state_of(u) + column;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          s[r][j] = u.slot < 0 ? make_float4(0, 0, 0, 0) : *reinterpret_cast<const float4*>(state + (32 * r + 4 * part + j) * kLinearDim);
+        for (int j = 0; j < 2; ++j) {
+          const float4* from = reinterpret_cast<const float4*>(state + (32 * r + 4 * part + 2 * j) * kLinearDim);
+          const float4 x = u.slot < 0 ? make_float4(0, 0, 0, 0) : from[0], y = u.slot < 0 ? make_float4(0, 0, 0, 0) : from[kLinearDim / 4];
+          s[r][j][0] = Pair(x.x, y.x);
+          s[r][j][1] = Pair(x.y, y.y);
+          s[r][j][2] = Pair(x.z, y.z);
+          s[r][j][3] = Pair(x.w, y.w);
+        }
     }
     if (threadIdx.x == 0 && i + 1 < units && m.units[i + 1].slot >= 0) prefetch_l2(state_of(m.units[i + 1]), kStateBytes);
     for (int begin = 0; begin < u.rows; begin += kStepRows) {
       const int count = min(kStepRows, u.rows - begin);
       if (warp < count) {
-        if (begin != 0) fetch_token(u, begin + warp, &token);
         const float4 k = widened(token.k), q = widened(token.q);
         const float kk = warp_sum(dot4(k, k)), qq = warp_sum(dot4(q, q));
         const float4 ku = scaled(k, __frsqrt_rn(kk + a.eps));
@@ -146,26 +151,33 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
         }
       }
       __syncthreads();
-      // the first tokens of the next head, while these are gone through
-      if (begin + kStepRows >= u.rows && i + 1 < units && warp < m.units[i + 1].rows) fetch_token(m.units[i + 1], warp, &token);
+      // the next tokens, or the first ones of the next head, while these are gone through
+      if (begin + kStepRows < u.rows) {
+        if (begin + kStepRows + warp < u.rows) fetch_token(u, begin + kStepRows + warp, &token);
+      } else if (i + 1 < units && warp < m.units[i + 1].rows) {
+        fetch_token(m.units[i + 1], warp, &token);
+      }
       for (int t = 0; t < count; ++t) {
-        float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};        // of S^T k, then of S^T q, for four columns
+        Pair dots[8];                      // S^T k, then S^T q, for four columns: over even rows, over odd ones
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float4 k4 = *reinterpret_cast<const float4*>(&m.rows[t].k[32 * r + 4 * part]);
           const float4 q4 = *reinterpret_cast<const float4*>(&m.rows[t].q[32 * r + 4 * part]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float kj = (&k4.x)[j], qj = (&q4.x)[j];
-            sums[0] = fmaf(s[r][j].x, kj, sums[0]);
-            sums[1] = fmaf(s[r][j].y, kj, sums[1]);
-            sums[2] = fmaf(s[r][j].z, kj, sums[2]);
-            sums[3] = fmaf(s[r][j].w, kj, sums[3]);
-            sums[4] = fmaf(s[r][j].x, qj, sums[4]);
-            sums[5] = fmaf(s[r][j].y, qj, sums[5]);
-            sums[6] = fmaf(s[r][j].z, qj, sums[6]);
-            sums[7] = fmaf(s[r][j].w, qj, sums[7]);
+          for (int j = 0; j < 2; ++j) {
+            const Pair k2 = j == 0 ? Pair(k4.x, k4.y) : Pair(k4.z, k4.w), q2 = j == 0 ? Pair(q4.x, q4.y) : Pair(q4.z, q4.w);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              dots[c] = r + j == 0 ? s[r][j][c] * k2 : fma2(s[r][j][c], k2, dots[c]);
+              dots[4 + c] = r + j == 0 ? s[r][j][c] * q2 : fma2(s[r][j][c], q2, dots[4 + c]);
+            }
           }
+        }
+        float sums[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float2 x = dots[c].values();
+          sums[c] = x.x + x.y;
         }
         // part p ends with the total of sums[p]
         float half[4], quarter[2];
@@ -188,16 +200,15 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
         if (part >= 4) m.rows[t].v[mine] = fmaf(m.overlap[t], d, e * total);   // its value element has been read: by lanes that the shuffle waited for
         const float d0 = __shfl_sync(0xffffffffu, d, lane & 3), d1 = __shfl_sync(0xffffffffu, d, (lane & 3) | 4);
         const float d2 = __shfl_sync(0xffffffffu, d, (lane & 3) | 8), d3 = __shfl_sync(0xffffffffu, d, (lane & 3) | 12);
+        const Pair decay(e, e), add[4] = {Pair(d0, d0), Pair(d1, d1), Pair(d2, d2), Pair(d3, d3)};
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float4 k4 = *reinterpret_cast<const float4*>(&m.rows[t].k[32 * r + 4 * part]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float kj = (&k4.x)[j];
-            s[r][j].x = fmaf(kj, d0, e * s[r][j].x);
-            s[r][j].y = fmaf(kj, d1, e * s[r][j].y);
-            s[r][j].z = fmaf(kj, d2, e * s[r][j].z);
-            s[r][j].w = fmaf(kj, d3, e * s[r][j].w);
+          for (int j = 0; j < 2; ++j) {
+            const Pair k2 = j == 0 ? Pair(k4.x, k4.y) : Pair(k4.z, k4.w);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[r][j][c] = fma2(k2, add[c], decay * s[r][j][c]);
           }
         }
         if (begin + t + 1 == u.kept) {
@@ -205,7 +216,12 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
 #pragma unroll
           for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(state + (32 * r + 4 * part + j) * kLinearDim) = s[r][j];
+            for (int j = 0; j < 2; ++j) {
+              float4* to = reinterpret_cast<float4*>(state + (32 * r + 4 * part + 2 * j) * kLinearDim);
+              const float2 x = s[r][j][0].values(), y = s[r][j][1].values(), z = s[r][j][2].values(), w = s[r][j][3].values();
+              to[0] = make_float4(x.x, y.x, z.x, w.x);
+              to[kLinearDim / 4] = make_float4(x.y, y.y, z.y, w.y);
+            }
         }
       }
       __syncthreads();
