@@ -1,13 +1,15 @@
 // Norm of each head with an optional gate: y = x / sqrt(mean(x^2) + eps) * (w + offset) * act(z), or x * act(z) alone.
 //
 // A head of 64, 128 or 256 lies in 8, 16 or 32 neighbouring lanes, eight elements each: one load per lane and tensor, the sum of
-// squares by shuffles inside them.  All of it is bytes, so a thread of a large call has the loads of four heads under way.
+// squares by shuffles inside them.  All of it is bytes: with 8192 tokens of 16 heads of 256 the norm moves 134 MB in 24.7 us and the
+// sigmoid gate 201 MB in 32.8 us (5.4 and 6.1 TB/s); norm and silu gate of 32 heads of 128, 201 MB in 37.6 us (5.4 TB/s), take
+// 55 % of the exponentials and reciprocals that the multiprocessors can do and two thirds of the instructions.
 #include "linear.cuh"
 
 namespace aima {
 namespace {
 
-constexpr int kNormThreads = 256;
+constexpr int kNormThreads = 128;
 
 template <int kDim, bool kNorm, int kActivation, int kUnits>
 __global__ void __launch_bounds__(kNormThreads) head_norm_kernel(const HeadNorm a, const int units) {
@@ -54,12 +56,18 @@ __global__ void __launch_bounds__(kNormThreads) head_norm_kernel(const HeadNorm 
   }
 }
 
+// Heads that a thread has under way.  us with one / two, tokens of 16 heads on a stream of them: norms of 256 at 64 tokens 2.05 / 2.18,
+// at 1024 4.94 / 4.94, at 2048 8.19 / 7.73, at 8192 27.3 / 24.6; norms of 64 at 2048 3.31 / 3.37, at 4096 5.30 / 5.18, at 16384
+// 14.7 / 13.7; sigmoid gate of 256 at 1024 5.90 / 6.02, at 8192 33.5 / 32.8.  So two from twenty blocks of one a multiprocessor on.
+// Norm and silu gate of 128 with one / two / four: at 4096 11.4 / 12.5 / 12.0, at 8192 20.5 / 22.9 / 20.7, at 16384 38.9 / 42.3 / 37.6, at
+// 32768 75.8 / 80.9 / 70.7.  So four of those from 120 blocks of one on.
 template <int kDim, bool kNorm, int kActivation>
 void launch_units(const HeadNorm& a, cudaStream_t stream) {
-  constexpr int kPerBlock = kNormThreads / (kDim / 8);
+  constexpr bool kBoth = kNorm && kActivation != AIMA_MOE_GATE_NONE;
+  constexpr int kPerBlock = kNormThreads / (kDim / 8), kMost = kBoth ? 4 : 2;
   const int units = a.tokens * a.heads;
-  if (units > 4 * 4 * 148 * kPerBlock)      // four rounds of four heads a thread on every multiprocessor
-    head_norm_kernel<kDim, kNorm, kActivation, 4><<<(units + 4 * kPerBlock - 1) / (4 * kPerBlock), kNormThreads, 0, stream>>>(a, units);
+  if (units > (kBoth ? 120 : 20) * 148 * kPerBlock)
+    head_norm_kernel<kDim, kNorm, kActivation, kMost><<<(units + kMost * kPerBlock - 1) / (kMost * kPerBlock), kNormThreads, 0, stream>>>(a, units);
   else
     head_norm_kernel<kDim, kNorm, kActivation, 1><<<(units + kPerBlock - 1) / kPerBlock, kNormThreads, 0, stream>>>(a, units);
 }

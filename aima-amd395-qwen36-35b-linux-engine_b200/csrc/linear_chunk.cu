@@ -753,7 +753,8 @@ size_t tiles_of(int tokens, int sequences, int min_rows) {
 }
 
 // Into how many segments a sequence's chunks are cut, and the eighths that the first has: what the two passes are estimated to take
-// least with.  A chunk counts 5 in the second pass and 3 in the first; the launches more count as 28, an eighth of a chunk each or so.
+// least with.  A chunk counts 5 in the second pass (about 5 us), 3 in the first; the first pass's launch and the join 22, and 3
+// for each product of the join.
 struct Cut {
   int segments, first;
 };
@@ -772,8 +773,9 @@ Cut cut_of(int heads, int chunks, int places) {
       const Segments cut(g, eighths, chunks);
       const int one = makespan(2 * (g - 2) * heads, cut.per, heads, cut.first, places);
       const int two = makespan((g - 1) * heads, cut.per, heads, cut.first, places);
-      if (one > 0 && two > 0 && 3 * one + 5 * two + 28 < least) {
-        least = 3 * one + 5 * two + 28;
+      const int time = 3 * one + 5 * two + 22 + 3 * (g - 2);
+      if (one > 0 && two > 0 && time < least) {
+        least = time;
         best = Cut{g, eighths};
       }
     }

@@ -18,7 +18,7 @@ def check(got, want):
 
 @pytest.mark.parametrize("activation", ["none", "silu", "sigmoid"])
 @pytest.mark.parametrize("dim", [64, 128, 256])
-@pytest.mark.parametrize("tokens,heads", [(1, 1), (1, 16), (3, 5), (257, 2), (64, 31), (1000, 32)])
+@pytest.mark.parametrize("tokens,heads", [(1, 1), (1, 16), (3, 5), (257, 2), (64, 31), (1000, 32), (9001, 32)])
 def test_head_norm(package, tokens, heads, dim, activation):
     g = torch.Generator(device="cuda").manual_seed(tokens + heads + dim)
     row = torch.randn(tokens, heads, 2 * dim, generator=g, device="cuda").bfloat16()
