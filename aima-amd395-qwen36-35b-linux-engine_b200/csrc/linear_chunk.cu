@@ -805,7 +805,7 @@ cudaError_t linear_chunks(const LinearDelta& a, int min_rows, void* workspace, i
   plan.pairs = static_cast<uint8_t*>(workspace) + (cut.segments > 1 ? border_bytes(heads) : 0);
   plan.heads = plan.pairs + static_cast<size_t>(plan.tiles) * a.k_heads * kChunkPairBytes;
   plan.wait_limit_ns = kWaitBudgetNs;
-  cudaError_t error = linear_prepare(plan, stream);
+  cudaError_t error = linear_prepare(plan, sm_count, stream);
   constexpr int kBytes = static_cast<int>(sizeof(ChunkMemory)) + 1024;
   if (error == cudaSuccess) error = opt_in_dynamic_smem<linear_chunk_kernel<kOutput>>(kBytes);
   if (error == cudaSuccess) error = opt_in_dynamic_smem<linear_chunk_kernel<kKept>>(kBytes);

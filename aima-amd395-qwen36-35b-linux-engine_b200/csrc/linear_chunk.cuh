@@ -95,6 +95,6 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   return y;
 }
 __device__ __forceinline__ void launch_may_follow() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-cudaError_t linear_prepare(const ChunkPlan& plan, cudaStream_t stream);
+cudaError_t linear_prepare(const ChunkPlan& plan, int sm_count, cudaStream_t stream);
 
 }  // namespace aima
