@@ -9,13 +9,18 @@
 //   S <- decay S + (stay D) k,  O = D scores^T               ->  o = (read Q + O) / sqrt(128)
 // Four warp groups have 16 tokens or 32 key elements each of that chain.  What does not depend on the chain is put where it waits for a
 // product: the outputs of the chunk before are taken from tensor memory and turned into rows while R runs, and normed and written while D
-// and S run; warps of their own for that slowed the chain by as much as they saved (9000 cycles a chunk; the floor of the products is
-// 2300).  One warp issues products, three load.
+// and S run; warps of their own for that slowed the chain by as much as they saved.  One warp issues products, three load.  T and the
+// scores are triangles, whose products begin with the row that is not zero.
+//
+// The chain bounds it: three products that wait for one another, with loads, splits and stores of all 16 warps in between.  A chunk
+// takes 6000 cycles without outputs, 8000 with them and 9700 with the gate; its products alone take 1300 and 2000.  8192 tokens of 32
+// heads with gate: first kernel 84 us, first pass 120, join 9, second pass 195.
 //
 // Few heads leave multiprocessors idle, so a sequence's chunks are cut into segments then.  What a segment does to the state is
 // S <- M S + B: a first pass finds the state behind the first segment, and M (values of zero, the identity as state) and B (a state of
 // zeros) of those between the first and the last; the states at all borders follow from them, and a second pass goes through all segments
-// at once.  The first pass has no outputs and takes 0.6 of the time of the second.
+// at once.  The first pass has no outputs and takes 0.6 of the time of the second.  The first segment has no part in the products of M
+// and B, so a multiprocessor that goes through two of half the length is done when the others are: it may be shorter.
 #include "linear_chunk.cuh"
 
 #include <algorithm>
@@ -676,18 +681,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   if (warp == kChainWarps) tmem_dealloc(tmem, 512);
 }
 
-// The states before the segments from the first pass: S_(j + 1) = M_j S_j + B_j, a block per head and 32 columns, 4 x 4 elements a
-// thread.  The next M is on its way meanwhile.
-constexpr int kJoinThreads = 256, kJoinColumns = 32, kJoinRow = kLinearDim + 4;
+// The states before the segments from the first pass: S_(j + 1) = M_j S_j + B_j, a block per head and 32 columns.  A thread
+// takes 4 x 4 elements and half of the sum: 8 loads from shared memory for 64 products.  The next M is on its way meanwhile.
+constexpr int kJoinThreads = 512, kJoinColumns = 32, kJoinRow = kLinearDim + 4;
 struct __align__(16) JoinMemory {
   float transfer[2][kLinearDim * kJoinRow];
-  float before[kLinearDim][kJoinColumns];
+  float before[kLinearDim][kJoinColumns], other[kLinearDim][kJoinColumns];
 };
 __global__ void __launch_bounds__(kJoinThreads, 1) linear_join_kernel(const ChunkPlan plan) {
   extern __shared__ uint8_t raw[];
   JoinMemory& m = *reinterpret_cast<JoinMemory*>(raw);
   const int head = blockIdx.x, sequence = blockIdx.y, begin = static_cast<int>(blockIdx.z) * kJoinColumns;
-  const int column = 4 * (threadIdx.x & 7), first = threadIdx.x >> 3;        // rows first + 32 i
+  const int column = 4 * (threadIdx.x & 7), first = (threadIdx.x >> 3) & 31, part = threadIdx.x >> 8;        // rows first + 32 i
   const LinearSequence seq = linear_sequence(plan.a.batch, sequence);
   const int chunks = chunks_of(seq, plan.min_rows);
   const Segments cut(plan, chunks);
@@ -705,7 +710,7 @@ __global__ void __launch_bounds__(kJoinThreads, 1) linear_join_kernel(const Chun
   };
   if (!there(1)) return;
   fetch(1);
-  {
+  if (part == 0) {
     const float* from = border(plan, sequence, head, 1) + begin;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -715,13 +720,13 @@ __global__ void __launch_bounds__(kJoinThreads, 1) linear_join_kernel(const Chun
     float4 sum[4];
     const float* add = border(plan, sequence, head, border_b(j)) + begin;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = *reinterpret_cast<const float4*>(add + (first + 32 * i) * kLinearDim + column);
+    for (int i = 0; i < 4; ++i) sum[i] = part == 0 ? *reinterpret_cast<const float4*>(add + (first + 32 * i) * kLinearDim + column) : make_float4(0, 0, 0, 0);
     if (there(j + 1)) fetch(j + 1);
     if (there(j + 1)) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
 #pragma unroll 4
-    for (int k = 0; k < kLinearDim; k += 4) {
+    for (int k = part * (kLinearDim / 2); k < (part + 1) * (kLinearDim / 2); k += 4) {
       float4 x[4];
 #pragma unroll
       for (int l = 0; l < 4; ++l) x[l] = *reinterpret_cast<const float4*>(&m.before[k + l][column]);
@@ -738,12 +743,20 @@ __global__ void __launch_bounds__(kJoinThreads, 1) linear_join_kernel(const Chun
         }
       }
     }
-    __syncthreads();                       // the states are read; what M lay in is free for the one after the next
-    float* to = border(plan, sequence, head, j + 1) + begin;
+    if (part != 0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<float4*>(to + (first + 32 * i) * kLinearDim + column) = sum[i];
-      *reinterpret_cast<float4*>(&m.before[first + 32 * i][column]) = sum[i];
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(&m.other[first + 32 * i][column]) = sum[i];
+    }
+    __syncthreads();                       // the states are read; what M lay in is free for the one after the next
+    if (part == 0) {
+      float* to = border(plan, sequence, head, j + 1) + begin;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 y = *reinterpret_cast<const float4*>(&m.other[first + 32 * i][column]);
+        const float4 x = make_float4(sum[i].x + y.x, sum[i].y + y.y, sum[i].z + y.z, sum[i].w + y.w);
+        *reinterpret_cast<float4*>(to + (first + 32 * i) * kLinearDim + column) = x;
+        *reinterpret_cast<float4*>(&m.before[first + 32 * i][column]) = x;
+      }
     }
   }
 }
@@ -753,7 +766,9 @@ size_t tiles_of(int tokens, int sequences, int min_rows) {
 }
 
 // Into how many segments a sequence's chunks are cut, and the eighths that the first has: what the two passes are estimated to take
-// least with.  A chunk counts 5 in the second pass (about 5 us), 3 in the first; the first pass's launch and the join 22, and 3
+// least with.  us as estimated, with segments of one length, without segments: 32 heads, 1024 tokens 90 / 100 / 103, 2048 134 / 141 /
+// 192, 8192 404 / 439 / 716; 8 heads, 1024 78 / 79 / 97, 8192 198 / 198 / 640; 64 heads, 8192 684 / 677 / 799.  512 tokens are not cut (8
+// heads: 57, in eight segments 70).  A chunk counts 5 in the second pass (about 5 us), 3 in the first; the first pass's launch and the join 22, and 3
 // for each product of the join.
 struct Cut {
   int segments, first;

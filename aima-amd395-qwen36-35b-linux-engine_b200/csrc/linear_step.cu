@@ -8,6 +8,9 @@
 // has 16 columns (value elements) of it and all 128 rows: four columns and 16 rows a lane, so the sums over the rows stay in the warp
 // and warps need not wait for each other between tokens.  The next head's state is asked into L2 and its first tokens into registers
 // while this one is gone through.
+//
+// One token is bytes: 64 sequences of 32 heads read and write 268 MB in 49.2 us (5.4 TB/s).  More tokens are the arithmetic and the waits
+// of a token, 1000 cycles for two heads at a time on a multiprocessor: 16 tokens of each of those heads take 143 us.
 #include "linear.cuh"
 
 #include <algorithm>
@@ -247,7 +250,8 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
 }  // namespace
 
 cudaError_t linear_step(const LinearDelta& a, int max_rows, int sm_count, cudaStream_t stream) {
-  // two blocks a multiprocessor, and more only where a block could not list its heads
+  // Two blocks a multiprocessor, and more only where a block could not list its heads.  us so / with a block for each head, 32 heads: 64
+  // sequences 51.2 / 59.4, 256 sequences 173 / 203, 16 sequences of 5 tokens 26.6 / 28.7, 32 sequences 32.8 / 34.8.
   const int units = a.v_heads * a.batch.sequences, blocks = std::max(std::min(units, 2 * sm_count), (units + kStepUnits - 1) / kStepUnits);
   linear_step_kernel<<<blocks, kStepThreads, 0, stream>>>(a, max_rows);
   return cudaGetLastError();
