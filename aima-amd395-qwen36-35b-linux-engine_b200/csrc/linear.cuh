@@ -104,20 +104,6 @@ __device__ __forceinline__ void linear_report(const LinearBatch& b, int* status,
     if (linear_sequence(b, s).bad) atomicOr(status, kLinearBadBatch);
 }
 
-// 4 / (1 + e^-x), to a few units of the last place: of a quarter of the denominator, so that the reciprocal is a normal number
-__device__ __forceinline__ float linear_four_sigmoid(float x) {
-  float quarter, y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(quarter) : "f"(fmaf(x, -1.4426950408889634f, -2.0f)));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(quarter + 0.25f));
-  return y;
-}
-__device__ __forceinline__ float linear_sigmoid(float x) { return 0.25f * linear_four_sigmoid(x); }
-__device__ __forceinline__ float linear_silu(float x) { return (0.25f * x) * linear_four_sigmoid(x); }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
 struct Pair {                  // two FP32 numbers that one instruction takes
   unsigned long long bits;
   __device__ __forceinline__ Pair() {}
@@ -142,6 +128,36 @@ __device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c
   Pair d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
   return d;
+}
+
+// 4 / (1 + e^-x), to a few units of the last place: of a quarter of the denominator, so that the reciprocal is a normal number
+__device__ __forceinline__ float linear_four_sigmoid(float x) {
+  float quarter, y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(quarter) : "f"(fmaf(x, -1.4426950408889634f, -2.0f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(quarter + 0.25f));
+  return y;
+}
+__device__ __forceinline__ float linear_sigmoid(float x) { return 0.25f * linear_four_sigmoid(x); }
+__device__ __forceinline__ float linear_silu(float x) { return (0.25f * x) * linear_four_sigmoid(x); }
+// for two numbers
+__device__ __forceinline__ Pair linear_four_sigmoid(const Pair& x) {
+  const float2 exponent = fma2(x, Pair(-1.4426950408889634f, -1.4426950408889634f), Pair(-2.0f, -2.0f)).values();
+  float a, b;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(exponent.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(exponent.y));
+  const float2 quarter = (Pair(a, b) + Pair(0.25f, 0.25f)).values();
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(quarter.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(quarter.y));
+  return Pair(a, b);
+}
+__device__ __forceinline__ Pair bf16_pair(uint32_t word) { return Pair(bf16_lo(word), bf16_hi(word)); }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_bf16(const Pair& x) {
+  const float2 v = x.values();
+  return pack_bf16(v.x, v.y);
 }
 
 struct LinearConv {

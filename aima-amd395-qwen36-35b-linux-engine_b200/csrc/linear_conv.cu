@@ -5,8 +5,9 @@
 // at a time, summed and put back in their own place.  Runs begin with a sequence, so only a sequence's first run reads its state; the same threads
 // write it, after that, from the inputs themselves.
 //
-// 8192 tokens of 8192 channels move 268 MB in 59.2 us (4.5 TB/s): two thirds of the issue slots and 56 % of the pipe for exponentials and
-// reciprocals are taken.  Runs of 8 rows with all loads first 65.7 us, four channels a thread 76.9.
+// 8192 tokens of 8192 channels move 268 MB in 57.4 us (4.7 TB/s): two channels an instruction, else two thirds of the issue slots
+// (59.4 us); 58 % of the pipe for exponentials and reciprocals are taken.  Earlier forms: runs of 8 rows with all loads first 65.7 us, four channels a
+// thread 76.9.
 #include "linear.cuh"
 
 namespace aima {
@@ -68,27 +69,21 @@ __global__ void __launch_bounds__(kConvThreads, 5) linear_conv_kernel(const Line
     uint4 y[kConvStep];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {             // channels 2 j, 2 j + 1
-      float w[2][kWidth], lo[kBefore + kConvStep], hi[kBefore + kConvStep];
-#pragma unroll
-      for (int i = 0; i < 2 * kWidth; ++i) {
-        const int at = 2 * j * kWidth + i;    // of the thread's weights, eight to a vector
+      const auto weight = [&](int at) {       // of the thread's, eight to a vector
         const uint32_t word = (&weights[at / 8].x)[(at % 8) / 2];
-        w[i / kWidth][i % kWidth] = at % 2 == 0 ? bf16_lo(word) : bf16_hi(word);
-      }
+        return at % 2 == 0 ? bf16_lo(word) : bf16_hi(word);
+      };
+      Pair w[kWidth], in[kBefore + kConvStep];
 #pragma unroll
-      for (int i = 0; i < kBefore + kConvStep; ++i) {
-        lo[i] = bf16_lo((&rows[i].x)[j]);
-        hi[i] = bf16_hi((&rows[i].x)[j]);
-      }
+      for (int i = 0; i < kWidth; ++i) w[i] = Pair(weight(2 * j * kWidth + i), weight((2 * j + 1) * kWidth + i));
+#pragma unroll
+      for (int i = 0; i < kBefore + kConvStep; ++i) in[i] = bf16_pair((&rows[i].x)[j]);
 #pragma unroll
       for (int r = 0; r < kConvStep; ++r) {
-        float y0 = lo[r] * w[0][0], y1 = hi[r] * w[1][0];
+        Pair sum = in[r] * w[0];
 #pragma unroll
-        for (int i = 1; i < kWidth; ++i) {
-          y0 = fmaf(lo[r + i], w[0][i], y0);
-          y1 = fmaf(hi[r + i], w[1][i], y1);
-        }
-        (&y[r].x)[j] = pack_bf16(linear_silu(y0), linear_silu(y1));
+        for (int i = 1; i < kWidth; ++i) sum = fma2(in[r + i], w[i], sum);
+        (&y[r].x)[j] = pack_bf16((sum * Pair(0.25f, 0.25f)) * linear_four_sigmoid(sum));
       }
     }
 #pragma unroll
