@@ -376,11 +376,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
         wait(&m.state_ready[1], c);           // all warps are done with the rows that lie in shared memory
         take_outputs(c - 1);
       }
-      uint32_t v[kTokens / 2];                                                 // tokens kTokens group .., two in a word
+      Pair given[kTokens / 2];                                                 // beta v of tokens kTokens group .., what of the right side can wait here
       {
         const uint16_t* values = reinterpret_cast<const uint16_t*>(stage + kStageValues) + kTokens * group * kLinearDim + column;
 #pragma unroll
-        for (int t = 0; t < kTokens; t += 2) v[t / 2] = values[t * kLinearDim] | static_cast<uint32_t>(values[(t + 1) * kLinearDim]) << 16;
+        for (int t = 0; t < kTokens; t += 4) {
+          const float4 rate = *reinterpret_cast<const float4*>(&numbers.rate[kTokens * group + t]);
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(static_cast<uint32_t>(values[(t + i) * kLinearDim]) << 16);
+          given[t / 2] = Pair(rate.x, rate.y) * (Pair(x[0], x[1]) * Pair(scale, scale));
+          given[t / 2 + 1] = Pair(rate.z, rate.w) * (Pair(x[2], x[3]) * Pair(scale, scale));
+        }
       }
       uint4 gates[kOutPasses];
       if (gated && c > 0) {
@@ -392,7 +399,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
       m.largest[group][column] = largest_here;                                 // all warps have read what the chunk before left here
       // the right side
       {
-        const Pair scales(scale, scale);
         Pair all[kTokens / 2];             // read before the first products write there
 #pragma unroll
         for (int b = 0; b < kTokens / 16; ++b) tmem_ld16(lanes + kDotsAt + kTokens * group + 16 * b, reinterpret_cast<uint32_t*>(all + 8 * b));
@@ -405,12 +411,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
           __half2 check = __half2half2(__ushort_as_half(0));
 #pragma unroll
           for (int t = 0; t < 16; t += 4) {
-            const float4 rate = *reinterpret_cast<const float4*>(&numbers.rate[token + t]), enter = *reinterpret_cast<const float4*>(&numbers.enter[token + t]);
+            const float4 enter = *reinterpret_cast<const float4*>(&numbers.enter[token + t]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const int j = t / 2 + i;
-              const Pair value = Pair(bf16_lo(v[8 * b + j]), bf16_hi(v[8 * b + j])) * scales;
-              r[j] = fma2(i == 0 ? Pair(enter.x, enter.y) : Pair(enter.z, enter.w), r[j], (i == 0 ? Pair(rate.x, rate.y) : Pair(rate.z, rate.w)) * value);
+              r[j] = fma2(i == 0 ? Pair(enter.x, enter.y) : Pair(enter.z, enter.w), r[j], given[8 * b + j]);
               split_f16(r[j], &terms[j], &terms[8 + j]);
               check = __hfma2(*reinterpret_cast<const __half2*>(&terms[j]), __half2half2(__ushort_as_half(0)), check);
             }
@@ -444,9 +449,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
       // the corrections
       {
         Pair d[kTokens / 2];
+        float4 stay[kTokens / 4];
+#pragma unroll
+        for (int t = 0; t < kTokens; t += 4)
+          stay[t / 4] = *reinterpret_cast<const float4*>((kMode == kKept ? numbers.stay_kept : numbers.stay) + kTokens * group + t);
         wait(&m.fresh_full, c);
         tc_fence_after();
-        const float* stay = (kMode == kKept ? numbers.stay_kept : numbers.stay) + kTokens * group;
         uint32_t terms[16];
 #pragma unroll
         for (int b = 0; b < kTokens / 16; ++b) tmem_ld16(lanes + kDotsAt + kTokens * group + 16 * b, reinterpret_cast<uint32_t*>(d + 8 * b));
@@ -455,7 +463,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
         for (int b = 0; b < kTokens / 16; ++b) {
 #pragma unroll
           for (int t = 0; t < 16; t += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(&stay[16 * b + t]);
+            const float4 x = stay[4 * b + t / 4];
             const int j = t / 2;
             split_f16(d[8 * b + j] * Pair(x.x, x.y), &terms[j], &terms[8 + j]);
             split_f16(d[8 * b + j + 1] * Pair(x.z, x.w), &terms[j + 1], &terms[8 + j + 1]);
