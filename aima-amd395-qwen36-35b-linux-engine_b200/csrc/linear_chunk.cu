@@ -9,12 +9,12 @@
 //   S <- decay S + (stay D) k,  O = D scores^T               ->  o = (read Q + O) / sqrt(128)
 // Four warp groups have 16 tokens or 32 key elements each of that chain.  What does not depend on the chain is put where it waits for a
 // product: the outputs of the chunk before are taken from tensor memory and turned into rows while R runs, and normed and written while D
-// and S run; warps of their own for that slowed the chain by as much as they saved.  One warp issues products, three load.  T and the
+// and S run; warps of their own for that cannot keep up, there being room for three beside the one that issues products.  One warp issues products, three load.  T and the
 // scores are triangles, whose products begin with the row that is not zero.
 //
 // The chain bounds it: three products that wait for one another, with loads, splits and stores of all 16 warps in between.  A chunk
-// takes 6000 cycles without outputs, 8000 with them and 9700 with the gate; its products alone take 1300 and 2000.  8192 tokens of 32
-// heads with gate: first kernel 84 us, first pass 120, join 9, second pass 195.
+// takes 6000 cycles without outputs, 7900 with them and 9500 with the gate; its products alone take 1300 and 2000.  8192 tokens of 32
+// heads with gate: first kernel 84 us, first pass 117, join 9, second pass 191.
 //
 // Few heads leave multiprocessors idle, so a sequence's chunks are cut into segments then.  What a segment does to the state is
 // S <- M S + B: a first pass finds the state behind the first segment, and M (values of zero, the identity as state) and B (a state of
