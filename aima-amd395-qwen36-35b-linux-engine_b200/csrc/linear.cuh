@@ -188,8 +188,8 @@ struct LinearDelta {
   int* status;
 };
 // Rows of a sequence up to which it is taken token by token.  us token by token / in chunks, 32 heads with gate: one sequence of 16 rows 18.4 /
-// 25.6, of 24 22.5 / 25.6, of 32 26.6 / 25.6; eight 28.7 / 42, 36.9 / 42, 45.1 / 42; 64 143 / 229, 197 / 235, 250 / 237.
-constexpr int kLinearStepRows = 24;
+// 27.6, of 24 22.5 / 29.7, of 32 28.7 / 29.7; eight 27.5 / 42, 34.8 / 44, 43 / 44; 64 135 / 230, 184 / 232, 236 / 235.
+constexpr int kLinearStepRows = 32;
 // Sequences of at most max_rows rows.
 cudaError_t linear_step(const LinearDelta& args, int max_rows, int sm_count, cudaStream_t stream);
 size_t linear_chunk_workspace(int k_heads, int v_heads, int max_tokens, int max_sequences);

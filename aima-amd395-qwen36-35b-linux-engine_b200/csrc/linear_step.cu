@@ -3,6 +3,8 @@
 //   S <- e^g S;  d = beta (v - S^T k);  S <- S + k d^T;  o = S^T q
 // Both products with the state are taken before it changes, from one pass over it: with r = S^T k and p = S^T q of the old state,
 //   d = beta (v - e^g r),   o = e^g p + (k.q) d,   S <- e^g S + k d^T.
+// The state is held divided by what it has decayed by so far, S / E, so that a token costs three products for an element instead of
+// four: E <- e^g E, S / E <- S / E + k (d / E)^T.  Once E falls below 2^-16 the state takes it up.
 //
 // A block takes one head of one sequence after the other: its state goes through registers once however many tokens there are.  A warp
 // has 16 columns (value elements) of it and all 128 rows: four columns and 16 rows a lane, so the sums over the rows stay in the warp
@@ -10,7 +12,8 @@
 // while this one is gone through.
 //
 // One token is bytes: 64 sequences of 32 heads read and write 268 MB in 49.2 us (5.4 TB/s).  More tokens are the arithmetic and the waits
-// of a token, 1000 cycles for two heads at a time on a multiprocessor: 16 tokens of each of those heads take 143 us.
+// of a token, 1600 cycles for two heads at a time on a multiprocessor: 16 tokens of each of those heads take 135 us, with four
+// products for an element 143.
 #include "linear.cuh"
 
 #include <algorithm>
@@ -117,7 +120,8 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
   const int part = lane >> 2, column = 16 * warp + 4 * (lane & 3);           // rows 32 i + 4 part + j, columns column .. column + 3
   for (int i = 0; i < units; ++i) {
     const StepMemory::Unit& u = m.units[i];
-    Pair s[4][2][4];                     // of two rows, four columns
+    Pair s[4][2][4];                     // of two rows, four columns; times `scale`
+    float scale = 1.0f;
     {
       const float* state = state_of(u) + column;
 #pragma unroll
@@ -196,14 +200,21 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
         }
         const float keep = (lane & 4) != 0 ? quarter[1] : quarter[0], send = (lane & 4) != 0 ? quarter[0] : quarter[1];
         const float total = keep + __shfl_xor_sync(0xffffffffu, send, 4);
-        const float e = m.decay[t];
+        const float e = scale * m.decay[t];
         const int mine = column + (part & 3);                              // the column whose total this lane has
         float d = m.rate[t] * (m.rows[t].v[mine] - e * total);             // of use in parts 0 .. 3
         d = __shfl_sync(0xffffffffu, d, lane & 15);
         if (part >= 4) m.rows[t].v[mine] = fmaf(m.overlap[t], d, e * total);   // its value element has been read: by lanes that the shuffle waited for
         const float d0 = __shfl_sync(0xffffffffu, d, lane & 3), d1 = __shfl_sync(0xffffffffu, d, (lane & 3) | 4);
         const float d2 = __shfl_sync(0xffffffffu, d, (lane & 3) | 8), d3 = __shfl_sync(0xffffffffu, d, (lane & 3) | 12);
-        const Pair decay(e, e), add[4] = {Pair(d0, d0), Pair(d1, d1), Pair(d2, d2), Pair(d3, d3)};
+        scale = e;
+        if (e < 0x1p-16f) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) (&s[0][0][0])[i] = (&s[0][0][0])[i] * Pair(e, e);
+          scale = 1.0f;
+        }
+        const float back = 1.0f / scale;
+        const Pair add[4] = {Pair(d0 * back, d0 * back), Pair(d1 * back, d1 * back), Pair(d2 * back, d2 * back), Pair(d3 * back, d3 * back)};
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float4 k4 = *reinterpret_cast<const float4*>(&m.rows[t].k[32 * r + 4 * part]);
@@ -211,7 +222,7 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
           for (int j = 0; j < 2; ++j) {
             const Pair k2 = j == 0 ? Pair(k4.x, k4.y) : Pair(k4.z, k4.w);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) s[r][j][c] = fma2(k2, add[c], decay * s[r][j][c]);
+            for (int c = 0; c < 4; ++c) s[r][j][c] = fma2(k2, add[c], s[r][j][c]);
           }
         }
         if (begin + t + 1 == u.kept) {
@@ -221,7 +232,8 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               float4* to = reinterpret_cast<float4*>(state + (32 * r + 4 * part + 2 * j) * kLinearDim);
-              const float2 x = s[r][j][0].values(), y = s[r][j][1].values(), z = s[r][j][2].values(), w = s[r][j][3].values();
+              const Pair by(scale, scale);
+              const float2 x = (s[r][j][0] * by).values(), y = (s[r][j][1] * by).values(), z = (s[r][j][2] * by).values(), w = (s[r][j][3] * by).values();
               to[0] = make_float4(x.x, y.x, z.x, w.x);
               to[kLinearDim / 4] = make_float4(x.y, y.y, z.y, w.y);
             }
