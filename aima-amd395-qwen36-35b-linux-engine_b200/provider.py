@@ -1085,7 +1085,7 @@ class LinearAttention:
                 and (out is None or (out.dtype is bfloat16 and out.get_device() == device and out.shape == shape and out.is_contiguous()))):
             self._refuse(batch, (("x", x, (tokens, self.channels)),), out, (tokens, self.channels))
         if out is None:
-            out = x.new_empty(shape)
+            out = self._torch.empty_like(x, memory_format=self._torch.contiguous_format)
         self.lib.check(self.lib.aima_moe_linear_conv_launch(self.handle, layer, batch.ref, x.data_ptr(), stride[0], out.data_ptr(), self._stream()))
         return out
 
@@ -1117,7 +1117,7 @@ class LinearAttention:
         if not outputs:
             out = None
         elif out is None:
-            out = v.new_empty(v_shape)
+            out = self._torch.empty_like(v, memory_format=self._torch.contiguous_format)
         call = _LINEAR_DELTA.pack(_LINEAR_DELTA.size, 0, q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
                                   gate.data_ptr() if gated else 0, z_row, z_head, a.data_ptr(), b.data_ptr(), a_row, b_row,
                                   0 if out is None else out.data_ptr())
@@ -1184,7 +1184,7 @@ def head_norm(x: Any, weight: Any = None, *, offset: float = 0.0, gate: Any = No
     if not (x_one == z_one == 1):
         _refuse_head_norm(x, weight, gate, activation, out)
     if out is None:
-        out = x.new_empty(shape)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     tokens, heads, dim = shape
     call = _HEAD_NORM.pack(_HEAD_NORM.size, tokens, heads, dim, code, offset, eps, 0, x.data_ptr(), x_row, x_head,
                            gate.data_ptr() if gated else 0, z_row, z_head, 0 if weight is None else weight.data_ptr(), out.data_ptr())
