@@ -274,22 +274,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
       const float* before = n == 0 || seq.fresh ? nullptr : state;
       if (kOutputs && plan.segments > 1) before = border(plan, blockIdx.y, head, segment) + part;
       if (kMode == kTransfer && segment > 0) before = nullptr;
+      if (before != nullptr) {
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 2) s[i / 2] = Pair(before[i * kLinearDim], before[(i + 1) * kLinearDim]);
+      } else {
+        const int one = transfer ? column - kKeys * group : -1;                // where the identity has its element
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 2) s[i / 2] = Pair(i == one ? 1.0f : 0.0f, i + 1 == one ? 1.0f : 0.0f);
+      }
+      if (gated && group == 0) m.weight[column] = 0.25f * __bfloat162float(a.norm_weight[column]);
       float largest = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kKeys; i += 2) {
-        float x = 0.0f, y = 0.0f;
-        if (before != nullptr) {
-          x = before[i * kLinearDim];
-          y = before[(i + 1) * kLinearDim];
-        } else if (transfer) {
-          x = kKeys * group + i == column ? 1.0f : 0.0f;
-          y = kKeys * group + i + 1 == column ? 1.0f : 0.0f;
-        }
-        s[i / 2] = Pair(x, y);
-        largest = max3_abs(largest, x, y);
-      }
+      for (int i = 0; i < kKeys / 2; ++i) largest = max3_abs(largest, s[i].values().x, s[i].values().y);
       m.largest[group][column] = largest;
-      if (gated && group == 0) m.weight[column] = 0.25f * __bfloat162float(a.norm_weight[column]);
       if (kMode == kTransfer && segment == 0 && n > 0) {
         float* const first = border(plan, blockIdx.y, head, 0) + part;
 #pragma unroll
