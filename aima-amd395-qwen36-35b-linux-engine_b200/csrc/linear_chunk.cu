@@ -114,6 +114,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.x;
   launch_may_follow();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_u32(&m.full[i]), 1);
+      mbar_init(smem_u32(&m.empty[i]), 1 + kChainWarps);
+      mbar_init(smem_u32(&m.values_full[i]), 2);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&m.state_ready[i]), kChainWarps);
+    for (int i = 0; i < kTokenSteps; ++i) {
+      mbar_init(smem_u32(&m.enter_ready[i]), kChainWarps);
+      mbar_init(smem_u32(&m.stay_ready[i]), kChainWarps);
+    }
+    mbar_init(smem_u32(&m.dots_full), 1);
+    mbar_init(smem_u32(&m.fresh_full), 1);
+    mbar_init(smem_u32(&m.state_full), 1);
+    mbar_init(smem_u32(&m.fresh_ready), kChainWarps);
+    mbar_init(smem_u32(&m.out_full), 1);
+    mbar_init(smem_u32(&m.out_taken), kChainWarps);
+    m.abort_flag = 0;
+    mbar_fence_init();
+  }
   const LinearSequence seq = linear_sequence(a.batch, blockIdx.y);
   if (seq.rows <= plan.min_rows) {
     wait_for_launch_before();
@@ -144,26 +164,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
     for (int s = threadIdx.x; s < static_cast<int>(blockIdx.y); s += kChunkThreads) mine += chunks_of(linear_sequence(a.batch, s), plan.min_rows);
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) m.sums[warp] = mine;
-  }
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(smem_u32(&m.full[i]), 1);
-      mbar_init(smem_u32(&m.empty[i]), 1 + kChainWarps);
-      mbar_init(smem_u32(&m.values_full[i]), 2);
-    }
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&m.state_ready[i]), kChainWarps);
-    for (int i = 0; i < kTokenSteps; ++i) {
-      mbar_init(smem_u32(&m.enter_ready[i]), kChainWarps);
-      mbar_init(smem_u32(&m.stay_ready[i]), kChainWarps);
-    }
-    mbar_init(smem_u32(&m.dots_full), 1);
-    mbar_init(smem_u32(&m.fresh_full), 1);
-    mbar_init(smem_u32(&m.state_full), 1);
-    mbar_init(smem_u32(&m.fresh_ready), kChainWarps);
-    mbar_init(smem_u32(&m.out_full), 1);
-    mbar_init(smem_u32(&m.out_taken), kChainWarps);
-    m.abort_flag = 0;
-    mbar_fence_init();
   }
   if (warp == kChainWarps) tmem_alloc(smem_u32(&m.tmem), 512);
   tc_fence_before();
