@@ -187,9 +187,9 @@ struct LinearDelta {
   __nv_bfloat16* out;                 // may be nullptr
   int* status;
 };
-// Rows of a sequence up to which it is taken token by token.  us token by token / in chunks, 32 heads with gate: one sequence of 16 rows 18.4 /
-// 27.6, of 24 22.5 / 29.7, of 32 28.7 / 29.7; eight 27.5 / 42, 34.8 / 44, 43 / 44; 64 135 / 230, 184 / 232, 236 / 235.
-constexpr int kLinearStepRows = 32;
+// Rows of a sequence up to which it is taken token by token.  us token by token / in chunks, captured, 32 heads with gate: one sequence of
+// 16 rows 12.8 / 19.6, of 24 17.4 / 19.7, of 32 22.2 / 19.7; eight 19.8 / 31.5, 27.3 / 31.7, 34.3 / 31.7; 64 129 / 214, 179 / 217, 231 / 219.
+constexpr int kLinearStepRows = 28;
 // Sequences of at most max_rows rows.
 cudaError_t linear_step(const LinearDelta& args, int max_rows, int sm_count, cudaStream_t stream);
 size_t linear_chunk_workspace(int k_heads, int v_heads, int max_tokens, int max_sequences);

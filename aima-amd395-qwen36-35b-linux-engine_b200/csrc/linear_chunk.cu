@@ -14,7 +14,7 @@
 //
 // The chain bounds it: three products that wait for one another, with loads, splits and stores of all 16 warps in between.  A chunk
 // takes 6000 cycles without outputs, 7900 with them and 9500 with the gate; its products alone take 1300 and 2000.  8192 tokens of 32
-// heads with gate: first kernel 84 us, first pass 117, join 9, second pass 191.
+// heads with gate: first kernel 84 us, first pass 113, join 9, second pass 185.
 //
 // Few heads leave multiprocessors idle, so a sequence's chunks are cut into segments then.  What a segment does to the state is
 // S <- M S + B: a first pass finds the state behind the first segment, and M (values of zero, the identity as state) and B (a state of
@@ -771,10 +771,11 @@ size_t tiles_of(int tokens, int sequences, int min_rows) {
 }
 
 // Into how many segments a sequence's chunks are cut, and the eighths that the first has: what the two passes are estimated to take
-// least with.  us as estimated, with segments of one length, without segments: 32 heads, 1024 tokens 90 / 100 / 103, 2048 134 / 141 /
-// 192, 8192 404 / 439 / 716; 8 heads, 1024 78 / 79 / 97, 8192 198 / 198 / 640; 64 heads, 8192 684 / 677 / 799.  512 tokens are not cut (8
-// heads: 57, in eight segments 70).  A chunk counts 5 in the second pass (about 5 us), 3 in the first; the first pass's launch and the join 22, and 3
-// for each product of the join.
+// least with.  us as estimated, with segments of one length, without segments, captured: 32 heads, 512 tokens 49.1 / 50.2 / 50.2, 1024
+// 71.8 / 79.4 / 89.9, 2048 121 / 124 / 182, 8192 377 / 416 / 694; 8 heads, 512 45.3 / 49.3 / 49.2, 1024 64.4 / 64.4 / 83.3, 8192 181 /
+// 182 / 620; 64 heads, 1024 98.2 / 108 / 108, 8192 625 / 645 / 781.
+// A chunk counts 5 in the second pass (about 5 us), 3 in the first; the first pass's launch and the join 12, and 3 for each product of
+// the join.
 struct Cut {
   int segments, first;
 };
@@ -793,7 +794,7 @@ Cut cut_of(int heads, int chunks, int places) {
       const Segments cut(g, eighths, chunks);
       const int one = makespan(2 * (g - 2) * heads, cut.per, heads, cut.first, places);
       const int two = makespan((g - 1) * heads, cut.per, heads, cut.first, places);
-      const int time = 3 * one + 5 * two + 22 + 3 * (g - 2);
+      const int time = 3 * one + 5 * two + 12 + 3 * (g - 2);
       if (one > 0 && two > 0 && time < least) {
         least = time;
         best = Cut{g, eighths};

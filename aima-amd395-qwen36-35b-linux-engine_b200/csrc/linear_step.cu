@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
 }  // namespace
 
 cudaError_t linear_step(const LinearDelta& a, int max_rows, int sm_count, cudaStream_t stream) {
-  // Two blocks a multiprocessor, and more only where a block could not list its heads.  us so / with a block for each head, 32 heads: 64
-  // sequences 51.2 / 59.4, 256 sequences 173 / 203, 16 sequences of 5 tokens 26.6 / 28.7, 32 sequences 32.8 / 34.8.
+  // Two blocks a multiprocessor, and more only where a block could not list its heads.  us so / with a block for each head, captured, 32
+  // heads: 64 sequences 46.3 / 54.1, 256 sequences 168 / 197, 16 sequences of 5 tokens 17.1 / 18.2, 32 sequences 22.1 / 23.3.
   const int units = a.v_heads * a.batch.sequences, blocks = std::max(std::min(units, 2 * sm_count), (units + kStepUnits - 1) / kStepUnits);
   linear_step_kernel<<<blocks, kStepThreads, 0, stream>>>(a, max_rows);
   return cudaGetLastError();

@@ -690,7 +690,7 @@ typedef struct aima_moe_linear_batch {
   const int32_t* keep;         /* [sequences] or NULL                                           */
 } aima_moe_linear_batch;
 
-/* Device bytes of a handle's workspace: 256, and for batches of more than 32 tokens, per 64 tokens and one more for each sequence,
+/* Device bytes of a handle's workspace: 256, and for batches of more than 28 tokens, per 64 tokens and one more for each sequence,
  * 32 KB per key head and 33.5 KB per value head, and 1.5 MB for each head of as many sequences as fill half of the multiprocessors. */
 int aima_moe_linear_query_workspace(const aima_moe_linear_config* config, uint64_t* bytes);
 int aima_moe_linear_prepare(const aima_moe_linear_config* config, aima_moe_linear** handle);
@@ -707,7 +707,7 @@ int aima_moe_linear_conv_launch(aima_moe_linear* handle, uint32_t layer, const a
  *   S <- exp(g) S,  S <- S + k (beta (v - S^T k))^T,  o = S^T q / sqrt(128),
  *   g = -exp(a_log) softplus(a + dt_bias),  beta = sigmoid(b).
  * With a gate z: out = o / sqrt(mean(o^2) + eps) * norm_weight * silu(z), else out = o.
- * FP32 state, sums and norms.  Sequences of at most 32 rows go token by token, each number good to a few units of 2^-24 of the sums
+ * FP32 state, sums and norms.  Sequences of at most 28 rows go token by token, each number good to a few units of 2^-24 of the sums
  * it comes from; longer ones in chunks of 64 tokens on the tensor cores, whose operands have 22 bits.  There a column of a state, its
  * corrections and its values share a power of two, so they are held to 2^-24 of the largest that the column or its values have within
  * a chunk and the one before: what lies further below that is lost.  A call gives the same bits every time.  A NaN or infinity that a token brings reaches what depends on it and nothing else: no token before it,

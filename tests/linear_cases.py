@@ -108,7 +108,7 @@ def constants(rows):
     return (64.0, 0.0) if rows <= STEP_ROWS else (8192.0, 768.0 / 8192.0)
 
 
-STEP_ROWS = 32
+STEP_ROWS = 28
 
 
 def check_delta(got, states, wanted, most, typical=True):

@@ -106,9 +106,9 @@ def test_the_workspace_is_what_its_query_says(package, lib):
     size = ctypes.c_uint64()
     assert lib.aima_moe_linear_query_workspace(ctypes.byref(config(p)), ctypes.byref(size)) == 0
     assert size.value == 256 + 16 * 4096
-    assert lib.aima_moe_linear_query_workspace(ctypes.byref(config(p, max_tokens=32)), ctypes.byref(size)) == 0
+    assert lib.aima_moe_linear_query_workspace(ctypes.byref(config(p, max_tokens=28)), ctypes.byref(size)) == 0
     assert size.value == 256                         # never a chunk
-    assert lib.aima_moe_linear_query_workspace(ctypes.byref(config(p, max_tokens=33)), ctypes.byref(size)) == 0
+    assert lib.aima_moe_linear_query_workspace(ctypes.byref(config(p, max_tokens=29)), ctypes.byref(size)) == 0
     assert size.value > 256
 
 
@@ -150,8 +150,8 @@ def test_batches_that_are_refused(package, lib, changes, status):
 
 
 @pytest.mark.parametrize("tokens,sequences,most,offsets,launches", [
-    (1, 1, 1, True, 10), (32, 1, 32, True, 10), (33, 1, 33, True, 100), (33, 1, 33, False, 100), (64, 2, 33, True, 110), (66, 2, 33, False, 100),
-    (64, 2, 32, False, 10), (64, 2, 32, True, 10), (4096, 4, 1024, False, 100)])
+    (1, 1, 1, True, 10), (28, 1, 28, True, 10), (29, 1, 29, True, 100), (29, 1, 29, False, 100), (56, 2, 29, True, 110), (58, 2, 29, False, 100),
+    (56, 2, 28, False, 10), (56, 2, 28, True, 10), (4096, 4, 1024, False, 100)])
 def test_few_rows_go_token_by_token_and_many_in_chunks(package, lib, tokens, sequences, most, offsets, launches):
     """With offsets a batch may hold both kinds."""
     h = Handle(package, lib)

@@ -63,7 +63,7 @@ def test_rows_behind_four_gigabytes(package, rows):
     p.check_conv(conv, p.conv_states, conv_wanted)
 
 
-@pytest.mark.parametrize("rows", [[32], [33], [32, 33, 1], [64], [65], [33] * 20])
+@pytest.mark.parametrize("rows", [[28], [29], [28, 29, 1], [64], [65], [29] * 20])
 def test_where_the_forms_meet(package, rows):
     compare(Problem(package, rows, earlier=[3 * (i % 2) for i in range(len(rows))], gated=True))
 
