@@ -194,24 +194,30 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
     }
   };
   const int half = warp >> 2, row = (warp & 3) * 32 + lane, token = row & (kChunk - 1), block = token >> 4;
-  const int jobs = all * a.k_heads;                                  // a tile and a key head
-  int job = blockIdx.x;
+  const int step_tile = static_cast<int>(gridDim.x) / a.k_heads, step_head = static_cast<int>(gridDim.x) - step_tile * a.k_heads;
+  int tile_after = static_cast<int>(blockIdx.x) / a.k_heads, k_head_after = static_cast<int>(blockIdx.x) - tile_after * a.k_heads;
   PrepareMemory::Tile next{};
   float next_a[2], next_b[2];                                        // of a gate warp's first head
-  if (job < jobs) {
-    look_up(job / a.k_heads, 0);
+  if (tile_after < all) {
+    look_up(tile_after, 0);
     __syncthreads();
     next = m.tiles[0];
-    if (warp < kRowWarps) fetch_rows(job % a.k_heads, next.row0, next.rows);
-    else if (warp - kRowWarps < a.group) fetch_gates(job % a.k_heads * a.group + warp - kRowWarps, next.row0, next.rows, next_a, next_b);
+    if (warp < kRowWarps) fetch_rows(k_head_after, next.row0, next.rows);
+    else if (warp - kRowWarps < a.group) fetch_gates(k_head_after * a.group + warp - kRowWarps, next.row0, next.rows, next_a, next_b);
   }
   bool alive = true;
-  for (int turn = 0; job < jobs; job += gridDim.x, turn ^= 1) {
-    const int tile = job / a.k_heads, k_head = job - tile * a.k_heads;
+  for (int turn = 0; tile_after < all; turn ^= 1) {
+    const int tile = tile_after, k_head = k_head_after;
     const int rows = next.rows, kept = next.kept;
     const long long row0 = next.row0;
-    const int job_after = job + static_cast<int>(gridDim.x);
-    if (job_after < jobs) look_up(job_after / a.k_heads, turn ^ 1);
+    tile_after += step_tile;
+    k_head_after += step_head;
+    if (k_head_after >= a.k_heads) {
+      k_head_after -= a.k_heads;
+      ++tile_after;
+    }
+    const bool more = tile_after < all;
+    if (more) look_up(tile_after, turn ^ 1);
     for (int base = 0; base < a.group; base += kHeadsAtOnce) {
       const int heads = min(kHeadsAtOnce, a.group - base);
       double total[2] = {0.0, 0.0}, last = 0.0;
@@ -344,10 +350,9 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
         tc_fence_after();
       }
       __syncthreads();                                                 // the gates are there; A and the scores take the rows' place
-      if (base == 0 && job_after < jobs) {
+      if (base == 0 && more) {
         // the next tile's rows and gates, while this one is gone through
         next = m.tiles[turn ^ 1];
-        const int k_head_after = job_after % a.k_heads;
         if (warp < kRowWarps) fetch_rows(k_head_after, next.row0, next.rows);
         else if (warp - kRowWarps < a.group) fetch_gates(k_head_after * a.group + warp - kRowWarps, next.row0, next.rows, next_a, next_b);
       }
