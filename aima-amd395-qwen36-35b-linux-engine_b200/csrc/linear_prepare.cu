@@ -11,7 +11,7 @@
 // have two f16 terms.
 //
 // Two blocks a multiprocessor go through all tiles, the next one's rows on their way.  Barriers and the latency of the substitution bound
-// it (40 % of the issue slots, 3 TB/s): 8192 tokens of 16 key and 32 value heads take 84 us, of them 41 for the bytes.  Three blocks with 80
+// it (40 % of the issue slots, 2.6 TB/s): 8192 tokens of 16 key and 32 value heads take 84 us, of them 34 for the bytes.  Three blocks with 80
 // registers spill and are no faster (86); two heads in every phase with half of the barriers are slower (93).
 #include "linear_chunk.cuh"
 
