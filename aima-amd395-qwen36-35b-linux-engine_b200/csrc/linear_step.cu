@@ -4,7 +4,9 @@
 // Both products with the state are taken before it changes, from one pass over it: with r = S^T k and p = S^T q of the old state,
 //   d = beta (v - e^g r),   o = e^g p + (k.q) d,   S <- e^g S + k d^T.
 // The state is held divided by what it has decayed by so far, S / E, so that a token costs three products for an element instead of
-// four: E <- e^g E, S / E <- S / E + k (d / E)^T.  Once E falls below 2^-16 the state takes it up.
+// four: E <- e^g E, S / E <- S / E + k (d / E)^T.  Once E falls below 2^-16 the state takes it up, and with every token that a
+// warp's columns have a product with the state or a correction above 2^80 for: S / E may then be beyond FP32 where S is not.  What stays divided
+// grows by less than 28 * 2^96 so, which is no step of the largest numbers.
 //
 // A block takes one head of one sequence after the other: its state goes through registers once however many tokens there are.  A warp
 // has 16 columns (value elements) of it and all 128 rows: four columns and 16 rows a lane, so the sums over the rows stay in the warp
@@ -203,12 +205,13 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
         const float e = scale * m.decay[t];
         const int mine = column + (part & 3);                              // the column whose total this lane has
         float d = m.rate[t] * (m.rows[t].v[mine] - e * total);             // of use in parts 0 .. 3
+        const bool large = __any_sync(0xffffffffu, fmaxf(fabsf(d), fabsf(total)) > 0x1p80f);
         d = __shfl_sync(0xffffffffu, d, lane & 15);
         if (part >= 4) m.rows[t].v[mine] = fmaf(m.overlap[t], d, e * total);   // its value element has been read: by lanes that the shuffle waited for
         const float d0 = __shfl_sync(0xffffffffu, d, lane & 3), d1 = __shfl_sync(0xffffffffu, d, (lane & 3) | 4);
         const float d2 = __shfl_sync(0xffffffffu, d, (lane & 3) | 8), d3 = __shfl_sync(0xffffffffu, d, (lane & 3) | 12);
         scale = e;
-        if (e < 0x1p-16f) {
+        if (e < 0x1p-16f || large) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) (&s[0][0][0])[i] = (&s[0][0][0])[i] * Pair(e, e);
           scale = 1.0f;

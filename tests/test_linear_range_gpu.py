@@ -1,0 +1,35 @@
+"""Linear-attention layers with numbers near the ends of what BF16 and FP32 hold, in both forms of the delta rule."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from linear_cases import DIM, Problem, check_delta  # noqa: E402
+
+
+def check(p):
+    wanted = p.delta_wanted()
+    assert bool(torch.isfinite(wanted["out"]).all()) and float(wanted["states"].abs().max()) < 2.0 ** 127
+    got = p.delta()
+    p.layer.sync()
+    check_delta(got, p.states, wanted, max(p.rows))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows", [[28, 20], [29, 20], [150, 90]])
+def test_large_corrections_while_the_state_decays(package, rows, gated):
+    """Values and states of 2^120 in a state that has decayed by 2^-15, 2^-28 and more: all that the formula has stays finite."""
+    p = Problem(package, rows, earlier=[3] * len(rows), seed=11, gated=False)
+    p.a, p.v = p.a.clone(), p.v.clone()
+    p.a_log.zero_()
+    p.dt_bias.zero_()
+    p.a.zero_()                                  # decay 1/2
+    p.a[::7] = -4.0                              # nearly none
+    p.a[5::13] = 30.0                            # nearly all
+    columns = [0, 1, 3, 126] if not gated else [3]
+    p.v[:, 1, columns] *= 2.0 ** 120
+    p.states[:, 2, :, 4] *= 2.0 ** 120
+    p.states[:, 3, :, 5] *= 2.0 ** 124
+    check(p)
