@@ -130,6 +130,10 @@ __device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c
   return d;
 }
 
+// What numbers have to be multiplied by before they are squared, given the sum or mean of their squares with eps: 1, unless it is beyond
+// FP32 (numbers from 2^60 on; then squares of what is left are at most 2^96) or so small that squares were lost.  eps goes with its square.
+__device__ __forceinline__ float linear_norm_shift(float squares) { return !(squares < INFINITY) ? 0x1p-80f : squares < 0x1p-100f ? 0x1p80f : 1.0f; }
+
 // 4 / (1 + e^-x), to a few units of the last place: of a quarter of the denominator, so that the reciprocal is a normal number
 __device__ __forceinline__ float linear_four_sigmoid(float x) {
   float quarter, y;

@@ -57,6 +57,14 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const float4& v) {
 }
 __device__ __forceinline__ float dot4(const float4& a, const float4& b) { return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, a.x * b.x))); }
 __device__ __forceinline__ float4 scaled(const float4& a, float s) { return make_float4(a.x * s, a.y * s, a.z * s, a.w * s); }
+// x and its squares with eps, both times what makes them numbers that the norm can take
+__device__ __forceinline__ void normable(float4* x, float* squares, float eps) {
+  const float by = linear_norm_shift(*squares);
+  if (by != 1.0f) {                        // the same for all lanes
+    *x = scaled(*x, by);
+    *squares = warp_sum(dot4(*x, *x)) + eps * by * by;
+  }
+}
 
 __device__ __forceinline__ uint2 load_raw(const __nv_bfloat16* p) { return *reinterpret_cast<const uint2*>(p); }
 __device__ __forceinline__ float4 widened(const uint2& raw) { return make_float4(bf16_lo(raw.x), bf16_hi(raw.x), bf16_lo(raw.y), bf16_hi(raw.y)); }
@@ -142,10 +150,14 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
     for (int begin = 0; begin < u.rows; begin += kStepRows) {
       const int count = min(kStepRows, u.rows - begin);
       if (warp < count) {
-        const float4 k = widened(token.k), q = widened(token.q);
-        const float kk = warp_sum(dot4(k, k)), qq = warp_sum(dot4(q, q));
-        const float4 ku = scaled(k, __frsqrt_rn(kk + a.eps));
-        const float4 qu = scaled(q, __frsqrt_rn(qq + a.eps) * 0.08838834764831845f);
+        float4 k = widened(token.k), q = widened(token.q);
+        float kk = warp_sum(dot4(k, k)) + a.eps, qq = warp_sum(dot4(q, q)) + a.eps;
+        if (!(fmaxf(kk, qq) < INFINITY && fminf(kk, qq) >= 0x1p-100f)) {
+          normable(&k, &kk, a.eps);
+          normable(&q, &qq, a.eps);
+        }
+        const float4 ku = scaled(k, __frsqrt_rn(kk));
+        const float4 qu = scaled(q, __frsqrt_rn(qq) * 0.08838834764831845f);
         const float kq = warp_sum(dot4(ku, qu));
         StepRow& row = m.rows[warp];
         *reinterpret_cast<float4*>(&row.k[4 * lane]) = ku;

@@ -33,3 +33,18 @@ def test_large_corrections_while_the_state_decays(package, rows, gated):
     p.states[:, 2, :, 4] *= 2.0 ** 120
     p.states[:, 3, :, 5] *= 2.0 ** 124
     check(p)
+
+
+@pytest.mark.parametrize("rows", [[12, 9], [28, 29], [100, 90]])
+def test_large_and_small_keys_and_queries(package, rows):
+    """Keys and queries count by their direction, whatever their length, until it falls below the norm's epsilon."""
+    p = Problem(package, rows, earlier=[3] * len(rows), seed=12, gated=True)
+    p.q, p.k = p.q.clone(), p.k.clone()
+    most = torch.finfo(torch.bfloat16).max
+    for x, at in ((p.k, 2), (p.q, 3)):
+        x[at] *= 2.0 ** 62
+        x[at + 2, 0] *= 2.0 ** 100
+        x[at + 4] = torch.where(x[at + 4] < 0, -most, most)
+        x[at + 6] *= 2.0 ** -80
+        x[at + 8] *= 2.0 ** -9
+    check(p)
