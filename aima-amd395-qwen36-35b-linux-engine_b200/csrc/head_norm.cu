@@ -35,12 +35,22 @@ __global__ void __launch_bounds__(kNormThreads) head_norm_kernel(const HeadNorm 
     float x[8];
     unpack8(raw[u], x);
     if (kNorm) {
-      float sum = 0.0f;
+      const auto mean = [&](float eps) {     // of the squares, with eps
+        float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
+        for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
 #pragma unroll
-      for (int d = 1; d < kLanes; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      const float scale = __frsqrt_rn(fmaf(sum, 1.0f / kDim, a.eps));
+        for (int d = 1; d < kLanes; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        return fmaf(sum, 1.0f / kDim, eps);
+      };
+      float square = mean(a.eps);
+      if (__any_sync(0xffffffffu, !linear_norm_holds(square))) {
+        const float by = linear_norm_shift(square);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= by;
+        square = mean(a.eps * by * by);
+      }
+      const float scale = __frsqrt_rn(square);
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = x[j] * scale * w[j];
     }

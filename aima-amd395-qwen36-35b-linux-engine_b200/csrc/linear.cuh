@@ -130,8 +130,10 @@ __device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c
   return d;
 }
 
-// What numbers have to be multiplied by before they are squared, given the sum or mean of their squares with eps: 1, unless it is beyond
-// FP32 (numbers from 2^60 on; then squares of what is left are at most 2^96) or so small that squares were lost.  eps goes with its square.
+// Whether a sum or mean of squares, with eps, is one that a norm can go by: 2^-100 .. below infinity.
+__device__ __forceinline__ bool linear_norm_holds(float squares) { return __float_as_uint(squares) - 0x0d800000u < 0x7f800000u - 0x0d800000u; }
+// What the numbers have to be multiplied by before they are squared, else 1.  Beyond FP32 there were numbers from 2^60 on, and what is left
+// of them has squares of at most 2^96; so small, squares may have been lost.  eps goes with the factor's square.
 __device__ __forceinline__ float linear_norm_shift(float squares) { return !(squares < INFINITY) ? 0x1p-80f : squares < 0x1p-100f ? 0x1p80f : 1.0f; }
 
 // 4 / (1 + e^-x), to a few units of the last place: of a quarter of the denominator, so that the reciprocal is a normal number
