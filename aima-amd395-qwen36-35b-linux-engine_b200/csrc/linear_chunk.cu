@@ -250,7 +250,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
         *reinterpret_cast<float4*>(weight + 4) = *reinterpret_cast<const float4*>(&m.weight[8 * piece + 4]);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-          const float factor = rsqrtf(fmaf(sum[i], 1.0f / kLinearDim, a.eps));
+          float square = fmaf(sum[i], 1.0f / kLinearDim, a.eps);
+          if (!linear_norm_holds(square)) {                                    // for the 16 lanes of a row
+            const float by = linear_norm_shift(square);
+            square = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              o[i][j] *= by;
+              square = fmaf(o[i][j], o[i][j], square);
+            }
+#pragma unroll
+            for (int d = 8; d >= 1; d /= 2) square += __shfl_xor_sync(0xffffu << (lane & 16), square, d);
+            square = fmaf(square, 1.0f / kLinearDim, a.eps * by * by);
+          }
+          const float factor = rsqrtf(square);
           float z[8];
           unpack8(gates[kRows * which + i], z);
 #pragma unroll

@@ -261,7 +261,13 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
         if (a.gate.data != nullptr) {
           const float4 z = widened(m.rows[warp].gate[lane]);
           const float4 w = load4(a.norm_weight + 4 * lane);
-          const float scale = __frsqrt_rn(fmaf(warp_sum(dot4(o, o)), 1.0f / kLinearDim, a.eps));
+          float square = fmaf(warp_sum(dot4(o, o)), 1.0f / kLinearDim, a.eps);
+          if (!linear_norm_holds(square)) {
+            const float by = linear_norm_shift(square);
+            o = scaled(o, by);
+            square = fmaf(warp_sum(dot4(o, o)), 1.0f / kLinearDim, a.eps * by * by);
+          }
+          const float scale = __frsqrt_rn(square);
           o.x *= scale * w.x * linear_silu(z.x);
           o.y *= scale * w.y * linear_silu(z.y);
           o.z *= scale * w.z * linear_silu(z.z);

@@ -48,3 +48,16 @@ def test_large_and_small_keys_and_queries(package, rows):
         x[at + 6] *= 2.0 ** -80
         x[at + 8] *= 2.0 ** -9
     check(p)
+
+
+@pytest.mark.parametrize("rows", [[12, 9], [28, 29], [100, 90], [600]])
+def test_large_outputs_are_normed(package, rows):
+    """Outputs whose squares are beyond FP32 under the gate's norm."""
+    p = Problem(package, rows, earlier=[3] * len(rows), seed=13, gated=True)
+    p.v = p.v.clone()
+    p.v[:, 1] *= 2.0 ** 66
+    p.states[:, 1] *= 2.0 ** 66
+    p.v[:, 2] *= 2.0 ** 110
+    p.states[:, 2] *= 2.0 ** 110
+    p.v[:, 3, ::2] *= 2.0 ** 90
+    check(p)
