@@ -253,6 +253,8 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
           double first[4];                                             // of each block
 #pragma unroll
           for (int b = 0; b < 4; ++b) first[b] = __shfl_sync(0xffffffffu, total[0], 8 * b);
+          float across[2][4];                                          // from a token to the first one of blocks 1 .. 3, of its own
+          bool own_steep = false;
           const double mine = lane < 8 ? first[0] : lane < 16 ? first[1] : lane < 24 ? first[2] : first[3];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -261,19 +263,35 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) linear_prepare_kernel(cons
             m.sum_high[h][t] = high;
             m.sum_low[h][t] = static_cast<float>(total[i] - high);
             m.rate[h][t] = beta[i];
-            m.down[h][t] = fast_exp2(static_cast<float>(total[i] - mine));
+            // Decay from the block's first token, and its inverse: their products are the decays within the block, so the whole part of
+            // the exponent stays apart, and they keep their bits however far the two are from 1.
+            const double x = total[i] - mine;
+            const int whole = max(__double2int_rn(x), -126);
+            const float part = static_cast<float>(x - whole);
+            m.down[h][t] = fast_exp2(part) * kv_exp2(whole);
+            across[i][3] = fast_exp2(-part) * kv_exp2(-whole);
           }
-          // with the lengths of k, which the other warps find meanwhile
-          if (base == 0) lengths_barrier();
           const double end[4] = {first[1], first[2], first[3], last};            // a token too far: no matter
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
             const bool steep = first[b] - end[b] > 64.0;
             if (lane == 0) m.steep[h][b] = steep;
+            own_steep = lane >> 3 == b ? steep : own_steep;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (own_steep) across[i][3] = 0.0f;
+#pragma unroll
+            for (int b = 1; b < 4; ++b) across[i][b - 1] = fast_exp2(static_cast<float>(first[b] - total[i]));
+          }
+          // with the lengths of k, which the other warps find meanwhile
+          if (base == 0) lengths_barrier();
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const int t = 2 * lane + i;
-              m.across[h][b][t] = t < 16 * b + (steep ? 0 : 16) ? fast_exp2(static_cast<float>(first[b] - total[i])) * m.length[t] : 0.0f;
+              m.across[h][b][t] = lane >> 3 > b ? 0.0f : (lane >> 3 == b ? across[i][3] : across[i][b == 0 ? 0 : b - 1]) * m.length[t];
             }
           }
         } else if (base == 0) {

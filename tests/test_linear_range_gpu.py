@@ -61,3 +61,36 @@ def test_large_outputs_are_normed(package, rows):
     p.states[:, 2] *= 2.0 ** 110
     p.v[:, 3, ::2] *= 2.0 ** 90
     check(p)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_decays_between_tokens_behind_a_strong_one(package, gated):
+    """One token of each 16 lets the state decay by 2^-62, those behind it by 2^-0.02 or so.  With one key for all tokens, a rate of 1 and
+    one value, the state is key x value after every token, and what the last token corrects away shows the decay from the strong one to
+    it as the kernel has it.  Keys of 64 ones have a length that is exact, and products that are.
+
+    Independent roundings, whose squares add up over many heads: two exponentials (2^-22 each), four products in FP32 (2^-24 each), two
+    terms of the entry of T and of the correction (2^-23 each), a substitution of up to 15 products (2^-25 each), the decays of up to 12
+    corrections (2^-24 each): 1.94 * 2^-22 of the state in all."""
+    rows = [66 + i for i in range(12)]
+    heads = 64
+    p = Problem(package, rows, k_heads=1, v_heads=heads, earlier=[3] * len(rows), seed=14, gated=gated)
+    g = torch.Generator(device="cuda").manual_seed(15)
+    sign = torch.where(torch.randn(DIM, generator=g, device="cuda") < 0, -1.0, 1.0)
+    sign[torch.randperm(DIM, generator=g, device="cuda")[:64]] = 0.0
+    p.k = sign.bfloat16().expand(p.tokens, 1, DIM)
+    p.q = p.k
+    p.v = torch.randn(1, heads, DIM, generator=g, device="cuda").bfloat16().expand(p.tokens, -1, -1)
+    p.a_log.zero_()
+    p.dt_bias.zero_()
+    p.a = (torch.randn(p.tokens, heads, generator=g, device="cuda") * 0.5 - 4.0).bfloat16()
+    for s, row0 in enumerate(p.batch["offsets"][:-1]):
+        p.a[row0 + 1:row0 + rows[s]:16] = 43.0                  # softplus(43) = 43 = 62 log 2
+    p.b = torch.full_like(p.a, 100.0)
+    wanted = p.delta_wanted()
+    got = p.delta()
+    p.layer.sync()
+    check_delta(got, p.states, wanted, max(rows))
+    slots = p.batch["slots"]
+    norm = float((p.states[slots].double() - wanted["states"][slots]).norm() / wanted["states"][slots].norm())
+    assert norm <= 2.0 ** -21, norm
