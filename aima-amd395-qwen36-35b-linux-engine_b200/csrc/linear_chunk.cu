@@ -89,19 +89,6 @@ __device__ __forceinline__ float* border(const ChunkPlan& plan, int sequence, in
 __device__ __forceinline__ int border_b(int segment) { return kMaxSegments + 2 * segment; }
 __device__ __forceinline__ int border_m(int segment) { return kMaxSegments + 2 * segment + 1; }
 
-// Where the segments of `chunks` chunks begin: all are as long, but for the first, which has plan.first eighths of the others' length.
-struct Segments {
-  int first, per;
-  __host__ __device__ Segments(const ChunkPlan& plan, int chunks) : Segments(plan.segments, plan.first, chunks) {}
-  __host__ __device__ Segments(int segments, int eighths, int chunks) {
-    const int parts = 8 * (segments - 1) + eighths;
-    per = (8 * chunks + parts - 1) / parts;
-    const int left = chunks - (segments - 1) * per;
-    first = left > 1 ? left : 1;
-  }
-  __host__ __device__ int begin(int segment) const { return segment == 0 ? 0 : first + (segment - 1) * per; }
-};
-
 // kOutput: all rows of a segment, the state behind the last if plan.store says so.  kKept: the states alone, for the rows that enter them.
 // kTransfer: the first pass over segments.
 enum ChunkMode { kOutput, kKept, kTransfer };
@@ -150,7 +137,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) linear_chunk_kernel(const Ch
   }
   const int limit = kMode == kKept ? seq.kept : seq.rows;                  // rows that are gone through
   const int all_chunks = (limit - seq.first + kChunk - 1) / kChunk;
-  const Segments cut(plan, all_chunks);
+  const Segments cut(plan.segments, plan.first, all_chunks);
   const int chunk0 = cut.begin(segment), chunks = min(cut.begin(segment + 1), all_chunks) - chunk0;
   if (limit <= seq.first || chunks <= 0) {
     wait_for_launch_before();
@@ -713,7 +700,7 @@ __global__ void __launch_bounds__(kJoinThreads, 1) linear_join_kernel(const Chun
   const int column = 4 * (threadIdx.x & 7), first = (threadIdx.x >> 3) & 31, part = threadIdx.x >> 8;        // rows first + 32 i
   const LinearSequence seq = linear_sequence(plan.a.batch, sequence);
   const int chunks = chunks_of(seq, plan.min_rows);
-  const Segments cut(plan, chunks);
+  const Segments cut(plan.segments, plan.first, chunks);
   launch_may_follow();
   wait_for_launch_before();
   const auto there = [&](int j) { return j + 1 < plan.segments && cut.begin(j + 1) < chunks; };
@@ -779,65 +766,23 @@ __global__ void __launch_bounds__(kJoinThreads, 1) linear_join_kernel(const Chun
   }
 }
 
-size_t tiles_of(int tokens, int sequences, int min_rows) {
-  return static_cast<size_t>(tokens / kChunk) + std::min(sequences, tokens / (min_rows + 1));
-}
-
-// Into how many segments a sequence's chunks are cut, and the eighths that the first has: what the two passes are estimated to take
-// least with.  us as estimated, with segments of one length, without segments, captured: 32 heads, 512 tokens 49.1 / 50.2 / 50.2, 1024
-// 71.8 / 79.4 / 89.9, 2048 121 / 124 / 182, 8192 377 / 416 / 694; 8 heads, 512 45.3 / 49.3 / 49.2, 1024 64.4 / 64.4 / 83.3, 8192 181 /
-// 182 / 620; 64 heads, 1024 98.2 / 108 / 108, 8192 625 / 645 / 781.
-// A chunk counts 5 in the second pass (about 5 us), 3 in the first; the first pass's launch and the join 12, and 3 for each product of
-// the join.
-struct Cut {
-  int segments, first;
-};
-// Jobs of two lengths on `places` multiprocessors, the long ones first; 0: the long ones do not all find room.
-int makespan(int long_jobs, int length, int short_jobs, int short_length, int places) {
-  if (long_jobs > places || (long_jobs == places && short_jobs > 0)) return 0;
-  const int rounds = (short_jobs + places - long_jobs - 1) / std::max(places - long_jobs, 1);
-  return std::max(long_jobs > 0 ? length : 0, rounds * short_length);
-}
-Cut cut_of(int heads, int chunks, int places) {
-  Cut best{1, 8};
-  int least = 5 * chunks;
-  if (2 * heads > places) return best;               // the workspace has no room for borders of more
-  for (int g = 2; g <= kMaxSegments && g <= chunks; ++g) {
-    for (const int eighths : {8, 4, 3, 2}) {
-      const Segments cut(g, eighths, chunks);
-      const int one = makespan(2 * (g - 2) * heads, cut.per, heads, cut.first, places);
-      const int two = makespan((g - 1) * heads, cut.per, heads, cut.first, places);
-      const int time = 3 * one + 5 * two + 12 + 3 * (g - 2);
-      if (one > 0 && two > 0 && time < least) {
-        least = time;
-        best = Cut{g, eighths};
-      }
-    }
-  }
-  return best;
-}
-constexpr int kMultiprocessors = 148;      // that the workspace reckons with
-size_t border_bytes(int heads) { return static_cast<size_t>(heads) * kMaxBorders * kLinearDim * kLinearDim * sizeof(float); }
-
 }  // namespace
 
 size_t linear_chunk_workspace(int k_heads, int v_heads, int max_tokens, int max_sequences) {
-  const size_t tiles = std::max<size_t>(tiles_of(max_tokens, max_sequences, kLinearStepRows), tiles_of(max_tokens, 1, 0));
-  // a batch is cut into segments if its heads fill at most half of the multiprocessors
-  const size_t borders = border_bytes(v_heads * std::min(max_sequences, std::max(1, kMultiprocessors / 2 / v_heads)));
-  return borders + tiles * (static_cast<size_t>(k_heads) * kChunkPairBytes + static_cast<size_t>(v_heads) * kChunkHeadBytes);
+  return chunk_workspace(k_heads, v_heads, max_tokens, max_sequences, kLinearStepRows, kChunkPairBytes, kChunkHeadBytes);
 }
 
 cudaError_t linear_chunks(const LinearDelta& a, int min_rows, void* workspace, int sm_count, cudaStream_t stream) {
   ChunkPlan plan{};
   plan.a = a;
   plan.min_rows = min_rows;
-  plan.tiles = static_cast<int>(tiles_of(a.batch.tokens, a.batch.sequences, min_rows));
-  const int heads = a.v_heads * a.batch.sequences;
-  const Cut cut = cut_of(heads, (a.batch.max_new + kChunk - 1) / kChunk, std::min(sm_count, kMultiprocessors));
+  const ChunkLayout layout = chunk_layout(a.k_heads, a.v_heads, a.batch.tokens, a.batch.sequences, a.batch.max_new, min_rows, sm_count, kChunkPairBytes,
+                                          kChunkHeadBytes);
+  const Cut cut = layout.cut;
+  plan.tiles = static_cast<int>(layout.tiles);
   plan.borders = static_cast<float*>(workspace);
-  plan.pairs = static_cast<uint8_t*>(workspace) + (cut.segments > 1 ? border_bytes(heads) : 0);
-  plan.heads = plan.pairs + static_cast<size_t>(plan.tiles) * a.k_heads * kChunkPairBytes;
+  plan.pairs = static_cast<uint8_t*>(workspace) + layout.pairs_at;
+  plan.heads = static_cast<uint8_t*>(workspace) + layout.heads_at;
   plan.wait_limit_ns = kWaitBudgetNs;
   cudaError_t error = linear_prepare(plan, sm_count, stream);
   constexpr int kBytes = static_cast<int>(sizeof(ChunkMemory)) + 1024;

@@ -17,13 +17,14 @@
 #pragma once
 
 #include "linear.cuh"
+#include "linear_segments.cuh"
 #include "tcgen05.cuh"
 
 namespace aima {
 
-constexpr int kChunk = 64;
 constexpr int kChunkPairBytes = 2 * kChunk * kLinearDim * 2;     // k and q of a chunk: two panels of 64 elements, k's rows, then q's, 128-byte swizzle
 constexpr int kChunkPanelBytes = kChunkPairBytes / 2;
+static_assert(kBorderBytes == static_cast<size_t>(kMaxBorders) * kLinearDim * kLinearDim * sizeof(float));
 constexpr int kChunkMatrixBytes = kChunk * kChunk * 2;           // T's first terms, its second, the scores' first, their second: rows of 128 bytes, swizzled
 constexpr int kChunkNumbersAt = 4 * kChunkMatrixBytes;
 struct ChunkNumbers {                                            // of a chunk and value head
@@ -48,8 +49,6 @@ struct ChunkPlan {
   uint8_t* heads;              // [tiles, v_heads, kChunkHeadBytes]
   unsigned long long wait_limit_ns;
 };
-
-constexpr int kMaxSegments = 8, kMaxBorders = 3 * kMaxSegments;
 
 // Chunks of a sequence: of its active rows, if it is taken here.
 __device__ __forceinline__ int chunks_of(const LinearSequence& s, int min_rows) {

@@ -691,7 +691,8 @@ typedef struct aima_moe_linear_batch {
 } aima_moe_linear_batch;
 
 /* Device bytes of a handle's workspace: 256, and for batches of more than 28 tokens, per 64 tokens and one more for each sequence,
- * 32 KB per key head and 33.5 KB per value head, and 1.5 MB for each head of as many sequences as fill half of the multiprocessors. */
+ * 32 KB per key head and 33.5 KB per value head; and, where max_tokens is enough for sequences that are cut into segments (more than 400
+ * or so) and one sequence's value heads fill at most half of the multiprocessors, 1.5 MB for each value head of as many as fill that half. */
 int aima_moe_linear_query_workspace(const aima_moe_linear_config* config, uint64_t* bytes);
 int aima_moe_linear_prepare(const aima_moe_linear_config* config, aima_moe_linear** handle);
 /* Records one layer's tensors.  16-byte aligned, of the handle's device. */
