@@ -644,7 +644,8 @@ int aima_moe_verify_drafts_launch(const aima_moe_verify_drafts* call, void* stre
  *            give zeros and enter nothing).  NULL: every sequence goes on from its slot.
  *   keep     rows of the sequence, from its first on, that enter the state (clamped to 0 .. its rows); the others are computed all
  *            the same.  NULL: all.  With drafted tokens: a call with keep 0 gives their outputs, and once it is known how many stand a
- *            second call on the same rows, without outputs, brings the state there.
+ *            second call on the same rows brings the state there: the delta rule without outputs, the convolution, which always
+ *            has some, into a buffer that nobody reads.
  * All of it is read on the device, so a captured graph can be replayed for other contents. */
 #define AIMA_MOE_LINEAR_HEAD_DIM 128
 typedef struct aima_moe_linear aima_moe_linear;
@@ -700,7 +701,8 @@ int aima_moe_linear_bind_layer(aima_moe_linear* handle, uint32_t layer, const ai
 
 /* out[t, c] = silu(sum_j weight[c, j] x[t - (conv_width - 1) + j, c]), one launch; what lies before a sequence's first row comes from
  * its slot, which then holds its last conv_width - 1 inputs that were kept.  x: bf16 [tokens, channels], 16-byte aligned, rows
- * x_row_stride elements apart (a multiple of 8).  out: bf16 [tokens, channels], contiguous; it may not overlap x. */
+ * x_row_stride elements apart (a multiple of 8).  out: bf16 [tokens, channels], contiguous, 16-byte aligned; it may be neither NULL nor
+ * overlap x. */
 int aima_moe_linear_conv_launch(aima_moe_linear* handle, uint32_t layer, const aima_moe_linear_batch* batch, const void* x,
                                 uint64_t x_row_stride, void* out, void* stream);
 
