@@ -1144,7 +1144,8 @@ class LinearAttention:
         return stream
 
     def sync(self) -> None:
-        """Waits for the last launch and raises AimaMoeError if device-side data of a batch was out of range."""
+        """Waits for the last launch and raises AimaMoeError if device-side data of a batch was out of range.  Launches on other
+        streams and replays of graphs have to be waited for, or ordered before the last launch, by the caller."""
         self.lib.check(self.lib.aima_moe_linear_sync(self.handle))
 
     def release(self) -> None:

@@ -646,7 +646,8 @@ int aima_moe_verify_drafts_launch(const aima_moe_verify_drafts* call, void* stre
  *            the same.  NULL: all.  With drafted tokens: a call with keep 0 gives their outputs, and once it is known how many stand a
  *            second call on the same rows brings the state there: the delta rule without outputs, the convolution, which always
  *            has some, into a buffer that nobody reads.
- * All of it is read on the device, so a captured graph can be replayed for other contents. */
+ * All of it is read on the device, so a captured graph can be replayed for other contents.  Two sequences can claim a row only where
+ * an offset falls, which is reported (aima_moe_linear_sync); outputs and states of sequences with such rows are undefined then. */
 #define AIMA_MOE_LINEAR_HEAD_DIM 128
 typedef struct aima_moe_linear aima_moe_linear;
 
@@ -735,7 +736,10 @@ int aima_moe_linear_delta_launch(aima_moe_linear* handle, uint32_t layer, const 
 /* Synchronises the last stream and reports what launches since the last call found wrong in device-side data:
  * AIMA_MOE_ERR_INVALID_ARGUMENT for a slot, row offset or length outside its range (such a sequence was treated as one without tokens),
  * AIMA_MOE_ERR_TIMEOUT for a bounded wait that ran out.  Calls of one handle share its workspace, captured ones too: issue them, and
- * replay their graphs, on one stream or order them with events.  The convolution uses none of it but the word for reports. */
+ * replay their graphs, on one stream or order them with events.  The convolution uses none of it but the word for reports.
+ * The last stream is that of the handle's last launch call, under capture too.  Launches on other streams, the convolution's and replays of
+ * graphs too, are covered if what it had last was ordered behind them; wait for them before this call, else what they report may come
+ * with a later one or be lost. */
 int aima_moe_linear_sync(aima_moe_linear* handle);
 int aima_moe_linear_release(aima_moe_linear* handle);
 
