@@ -66,18 +66,18 @@ __global__ void __launch_bounds__(kNormThreads) head_norm_kernel(const HeadNorm 
   }
 }
 
-// Heads that a thread has under way.  us with one / two, tokens of 16 heads on a stream of them: norms of 256 at 64 tokens 2.05 / 2.18,
-// at 1024 4.94 / 4.94, at 2048 8.19 / 7.73, at 8192 27.3 / 24.6; norms of 64 at 2048 3.31 / 3.37, at 4096 5.30 / 5.18, at 16384
-// 14.7 / 13.7; sigmoid gate of 256 at 1024 5.90 / 6.02, at 8192 33.5 / 32.8.  So two from twenty blocks of one a multiprocessor on.
-// Norm and silu gate of 128 with one / two / four: at 4096 11.4 / 12.5 / 12.0, at 8192 20.5 / 22.9 / 20.7, at 16384 38.9 / 42.3 / 37.6, at
-// 32768 75.8 / 80.9 / 70.7.  So four of those from 120 blocks of one on.
+// Heads that a thread has under way.  us with one / two, tokens of 16 heads on a stream of them: norms of 256 at 64 tokens 2.1 / 2.3,
+// at 1024 5.1 / 5.1, at 2048 8.6 / 8.2, at 8192 28.7 / 25.9; norms of 64 at 2048 3.7 / 3.8, at 4096 5.5 / 5.4, at 16384 15.2 / 14.3; sigmoid
+// gate of 256 at 1024 6.4 / 6.4, at 2048 10.3 / 10.2, at 8192 34.1 / 33.8; norm and silu gate of 128 at 1024 4.0 / 4.3, at 1500 5.3 / 5.2,
+// at 2048 6.8 / 6.8, at 4096 11.6 / 11.3, at 16384 38.9 / 36.2, at 32768 73.7 / 68.1; norm and sigmoid gate of 128 at 1024 4.4 / 4.6, at 4096
+// 11.4 / 10.9, at 32768 72.7 / 66.6.  So two from twenty blocks of one a multiprocessor (148) on.  Four are no faster: norm and silu gate at
+// 4096 12.0, at 32768 69.6.
 template <int kDim, bool kNorm, int kActivation>
 void launch_units(const HeadNorm& a, cudaStream_t stream) {
-  constexpr bool kBoth = kNorm && kActivation != AIMA_MOE_GATE_NONE;
-  constexpr int kPerBlock = kNormThreads / (kDim / 8), kMost = kBoth ? 4 : 2;
+  constexpr int kPerBlock = kNormThreads / (kDim / 8);
   const int units = a.tokens * a.heads;
-  if (units > (kBoth ? 120 : 20) * 148 * kPerBlock)
-    head_norm_kernel<kDim, kNorm, kActivation, kMost><<<(units + kMost * kPerBlock - 1) / (kMost * kPerBlock), kNormThreads, 0, stream>>>(a, units);
+  if (units > 20 * 148 * kPerBlock)
+    head_norm_kernel<kDim, kNorm, kActivation, 2><<<(units + 2 * kPerBlock - 1) / (2 * kPerBlock), kNormThreads, 0, stream>>>(a, units);
   else
     head_norm_kernel<kDim, kNorm, kActivation, 1><<<(units + kPerBlock - 1) / kPerBlock, kNormThreads, 0, stream>>>(a, units);
 }
