@@ -194,7 +194,8 @@ struct LinearDelta {
   int* status;
 };
 // Rows of a sequence up to which it is taken token by token.  us token by token / in chunks, captured, 32 heads with gate: one sequence of
-// 16 rows 12.8 / 19.6, of 24 17.4 / 19.7, of 32 22.2 / 19.7; eight 19.8 / 31.5, 27.3 / 31.7, 34.3 / 31.7; 64 129 / 214, 179 / 217, 231 / 219.
+// 16 rows 12.8 / 20.2, of 24 17.5 / 20.2, of 28 20.4 / 20.2, of 32 22.3 / 20.1; eight 20.1 / 31.8, 27.6 / 32.0, 31.8 / 32.2, 34.9 / 32.0; 64
+// 130 / 219, 184 / 222, 210 / 224, 236 / 223.
 constexpr int kLinearStepRows = 28;
 // Sequences of at most max_rows rows.
 cudaError_t linear_step(const LinearDelta& args, int max_rows, int sm_count, cudaStream_t stream);

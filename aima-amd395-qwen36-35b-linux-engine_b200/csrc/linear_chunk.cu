@@ -13,8 +13,8 @@
 // scores are triangles, whose products begin with the row that is not zero.
 //
 // The chain bounds it: three products that wait for one another, with loads, splits and stores of all 16 warps in between.  A chunk
-// takes 6000 cycles without outputs, 7900 with them and 9500 with the gate; its products alone take 1300 and 2000.  8192 tokens of 32
-// heads with gate: first kernel 84 us, first pass 113, join 9, second pass 185.
+// takes 6000 cycles without outputs, 7900 with them and 9750 with the gate; its products alone take 1300 and 2000.  8192 tokens of 32
+// heads with gate, from the end of one launch to the next: first kernel 84 us, first pass 100, join 12, second pass 198.
 //
 // Few heads leave multiprocessors idle, so a sequence's chunks are cut into segments then.  What a segment does to the state is
 // S <- M S + B: a first pass finds the state behind the first segment, and M (values of zero, the identity as state) and B (a state of

@@ -5,8 +5,9 @@
 // at a time, summed and put back in their own place.  Runs begin with a sequence, so only a sequence's first run reads its state; the same threads
 // write it, after that, from the inputs themselves.
 //
-// 8192 tokens of 8192 channels move 268 MB in 57.4 us (4.7 TB/s): two channels an instruction, else two thirds of the issue slots
-// (59.4 us); 58 % of the pipe for exponentials and reciprocals are taken.  Earlier forms: runs of 8 rows with all loads first 65.7 us, four channels a
+// 8192 tokens of 8192 channels move 268 MB in 57.0 us (4.7 TB/s): two channels an instruction, else two thirds of the issue slots
+// (59.4 us).  No one part is full: 61 % of the pipe for exponentials and reciprocals, 57 % of the issue slots, and 20 of 64 warps, more of which
+// the registers have no room for.  Earlier forms: runs of 8 rows with all loads first 65.7 us, four channels a
 // thread 76.9.
 #include "linear.cuh"
 

@@ -42,8 +42,8 @@ inline int makespan(int long_jobs, int length, int short_jobs, int short_length,
 }
 
 // What the two passes over the segments are estimated to take least with.  us as estimated, with segments of one length, without segments,
-// captured: 32 heads, 512 tokens 49.1 / 50.2 / 50.2, 1024 71.8 / 79.4 / 89.9, 2048 121 / 124 / 182, 8192 377 / 416 / 694; 8 heads, 512
-// 45.3 / 49.3 / 49.2, 1024 64.4 / 64.4 / 83.3, 8192 181 / 182 / 620; 64 heads, 1024 98.2 / 108 / 108, 8192 625 / 645 / 781.
+// captured: 32 heads, 512 tokens 49.5 / 49.5 / 51.5, 1024 72.4 / 80.0 / 91.4, 2048 123 / 126 / 187, 8192 381 / 422 / 713; 8 heads, 512
+// 45.9 / 45.9 / 50.2, 1024 64.5 / 64.5 / 85.4, 8192 184 / 184 / 638; 64 heads, 1024 100 / 100 / 111, 8192 630 / 655 / 799.
 // A chunk counts 5 in the second pass (about 5 us), 3 in the first; the first pass's launch and the join 12, and 3 for each product of
 // the join.
 inline Cut estimated_cut(int heads, int chunks, int places) {

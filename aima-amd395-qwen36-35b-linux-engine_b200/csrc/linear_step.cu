@@ -13,7 +13,7 @@
 // and warps need not wait for each other between tokens.  The next head's state is asked into L2 and its first tokens into registers
 // while this one is gone through.
 //
-// One token is bytes: 64 sequences of 32 heads read and write 268 MB in 49.2 us (5.4 TB/s).  More tokens are the arithmetic and the waits
+// One token is bytes: 64 sequences of 32 heads read and write 268 MB in 48.7 us (5.5 TB/s).  More tokens are the arithmetic and the waits
 // of a token, 1600 cycles for two heads at a time on a multiprocessor: 16 tokens of each of those heads take 135 us, with four
 // products for an element 143.
 #include "linear.cuh"
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kStepThreads, 2) linear_step_kernel(const Line
 
 cudaError_t linear_step(const LinearDelta& a, int max_rows, int sm_count, cudaStream_t stream) {
   // Two blocks a multiprocessor, and more only where a block could not list its heads.  us so / with a block for each head, captured, 32
-  // heads: 64 sequences 46.3 / 54.1, 256 sequences 168 / 197, 16 sequences of 5 tokens 17.1 / 18.2, 32 sequences 22.1 / 23.3.
+  // heads: 64 sequences 46.6 / 54.1, 256 sequences 167 / 200, 16 sequences of 5 tokens 17.3 / 18.4, 32 sequences 23.0 / 23.8.
   const int units = a.v_heads * a.batch.sequences, blocks = std::max(std::min(units, 2 * sm_count), (units + kStepUnits - 1) / kStepUnits);
   linear_step_kernel<<<blocks, kStepThreads, 0, stream>>>(a, max_rows);
   return cudaGetLastError();
