@@ -3,7 +3,7 @@
 // A head of 64, 128 or 256 lies in 8, 16 or 32 neighbouring lanes, eight elements each: one load per lane and tensor, the sum of
 // squares by shuffles inside them.  All of it is bytes: with 8192 tokens of 16 heads of 256 the norm moves 134 MB in 25.9 us and the
 // sigmoid gate 201 MB in 32.8 us (5.2 and 6.1 TB/s); norm and silu gate of 32 heads of 128, 201 MB in 37.9 us (5.3 TB/s), take
-// 59 % of the exponentials and reciprocals that the multiprocessors can do and three quarters of the instructions.
+// 56 % of the exponentials and reciprocals that the multiprocessors can do and 78 % of the instructions.
 #include "linear.cuh"
 
 namespace aima {
